@@ -1177,6 +1177,11 @@ int uocr_ops_check(void* stream) {
   if (e.code == kDevBadIndex && e.where == 2)
     std::snprintf(buf, sizeof(buf), "expert_ffn_one: expert id %d at position %d is outside [0, %d)", e.b, e.a,
                   kMaxExperts);
+  else if (e.code == kDevBadIndex && e.where == kSiteGroupRows)
+    std::snprintf(buf, sizeof(buf), "grouped_linear_w8a8: the rows of group %d (from row %d) are not in order or out of range",
+                  e.a, e.b);
+  else if (e.code == kDevBadIndex && e.where == kSiteRowIndex)
+    std::snprintf(buf, sizeof(buf), "grouped_linear_w8a8: row %d reads row %d, which x does not have", e.a, e.b);
   else
     std::snprintf(buf, sizeof(buf), "device error %d at site %d (%d, %d)", e.code, e.where, e.a, e.b);
   return fail(e.code == kDevWaitTimeout ? UOCR_ERR_TIMEOUT : UOCR_ERR_DEVICE, buf);

@@ -31,6 +31,9 @@ struct ErrorWord {
   int a;
   int b;
 };
+// Sites (ErrorWord::where) that uocr_ops_check words its message by.
+constexpr int kSiteGroupRows = 80;  // a: group, b: its first row
+constexpr int kSiteRowIndex = 81;   // a: output row, b: the row it names
 __device__ inline void raise_error(ErrorWord* e, int code, int where, int a, int b) {
   if (atomicCAS(&e->code, 0, code) == 0) {
     e->where = where;

@@ -1,0 +1,43 @@
+// Host interface of the 8-bit integer operators: the token quantiser
+// (quantize_tokens.cu) and the products (w8a8.cu).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "moe_common.cuh"
+
+namespace uocr_b200 {
+
+// q, scales = int8 rows of x [rows, cols] (fp32 or bf16, pitch ldx) with one
+// scale per row; q rows at pitch ldq, 16-byte aligned.
+cudaError_t launch_quantize_tokens(const void* x, bool bf16, int64_t rows, int64_t cols, int64_t ldx, int8_t* q,
+                                   int64_t ldq, float* scales, cudaStream_t stream);
+
+// y[r, c] = (sum_k x[row(r), k] w[g, c, k]) x_scales[row(r)] w_scales[g, c]
+// (+ bias[c]) (+ residual[r, c]) for the rows r of group g; with w_up
+// silu(that with w) * (that with w_up), without bias and residual.
+struct W8a8 {
+  const int8_t* x;
+  const float* x_scales;
+  const int* row_index;  // null: row(r) = r
+  int64_t x_rows;
+  const int* starts;     // [groups] first row of each group; null: one group of all rows
+  const int* counts;     // [groups] rows of each group; null: starts has groups + 1 entries
+  int64_t rows, groups, n, k;
+  const int8_t* w;
+  const float* w_scales;
+  const int8_t* w_up;
+  const float* w_up_scales;
+  const float* bias;
+  const void* residual;
+  void* y;
+  int64_t ldx, ldw, ldr, ldy;
+  bool y_bf16;
+  ErrorWord* err;
+};
+cudaError_t launch_w8a8(const W8a8& p, cudaStream_t stream);
+
+}  // namespace uocr_b200

@@ -1,5 +1,5 @@
-"""Python binding of the C ABI in include/uocr_moe.h and include/uocr_decoder.h
-(ctypes over libuocr_moe.so).
+"""Python binding of the C ABI in include/uocr_moe.h, include/uocr_decoder.h and
+include/uocr_int8.h (ctypes over libuocr_moe.so).
 
 This is the host-side mirror tests and bench.py call: torch supplies device
 memory and streams; every computation happens in libuocr_moe.so's sm_100a
@@ -38,6 +38,9 @@ DECODER_EXPORTS = [
     "uocr_decoder_set_head", "uocr_decoder_prefill", "uocr_decoder_decode", "uocr_decoder_profile_decode",
     "uocr_decoder_check",
 ]
+
+# Every symbol include/uocr_int8.h declares.
+INT8_EXPORTS = ["uocr_quantize_tokens", "uocr_linear_w8a8", "uocr_grouped_linear_w8a8"]
 
 # Every symbol include/uocr_moe.h declares.
 EXPORTS = [
@@ -112,6 +115,19 @@ class DecoderLayerSrc(ctypes.Structure):
                                        "down", "shared_gate", "shared_up", "shared_down")]
 
 
+class LinearW8A8Args(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "x_scales", "w", "w_scales", "bias", "residual", "y")] + [
+        (n, ctypes.c_int64) for n in ("m", "n", "k", "ldx", "ldw", "ldr", "ldy")] + [
+        ("y_dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class GroupedW8A8Args(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "x_scales", "row_index", "offsets", "w", "w_scales", "w_up",
+                                               "w_up_scales", "y")] + [
+        (n, ctypes.c_int64) for n in ("rows", "x_rows", "groups", "n", "k", "ldx", "ldw", "ldy")] + [
+        ("y_dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
 def lib() -> ctypes.CDLL:
     global _lib
     if _lib is None:
@@ -159,6 +175,9 @@ def lib() -> ctypes.CDLL:
         L.uocr_decoder_decode.argtypes = [vp, i64, vp, vp, vp]
         L.uocr_decoder_check.argtypes = [vp, vp]
         L.uocr_decoder_profile_decode.argtypes = [vp, i64, ctypes.POINTER(f32), vp]
+        L.uocr_quantize_tokens.argtypes = [vp, i32, i64, i64, i64, vp, i64, vp, vp]
+        L.uocr_linear_w8a8.argtypes = [ctypes.POINTER(LinearW8A8Args), vp]
+        L.uocr_grouped_linear_w8a8.argtypes = [ctypes.POINTER(GroupedW8A8Args), vp]
         _lib = L
     return _lib
 
@@ -419,6 +438,98 @@ def linear(x, w_bf16, y, bias=None, stream=None):
     m, k = x.shape
     n = w_bf16.shape[0]
     _check(lib().uocr_linear(_ptr(x), m, k, _ptr(w_bf16), n, _ptr(bias), _ptr(y), _stream(stream)))
+
+
+_FLOAT_DTYPES: dict = {}
+
+
+def _float_dtype(t, what: str) -> int:
+    if not _FLOAT_DTYPES:
+        import torch
+        _FLOAT_DTYPES.update({torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16})
+    dtype = _FLOAT_DTYPES.get(t.dtype)
+    if dtype is None:
+        raise ValueError(f"{what} must be float32 or bfloat16, not {t.dtype}")
+    return dtype
+
+
+def _rows(t, what: str, shape: tuple, pitch_of: int = 1) -> int:
+    """The row pitch of a 2-D device tensor of this shape whose rows are contiguous (a single row's pitch is its
+    width, rounded up to pitch_of)."""
+    if t.shape != shape or not t.is_cuda:
+        raise ValueError(f"{what} must be a {shape} tensor on the GPU, not {tuple(t.shape)} on {t.device}")
+    s0, s1 = t.stride()
+    if s1 != 1 and shape[1] > 1:
+        raise ValueError(f"{what}'s rows must be contiguous")
+    return s0 if shape[0] > 1 else -(-shape[1] // pitch_of) * pitch_of
+
+
+def _vector(t, what: str, n: int, dtype):
+    if t.dtype != dtype or t.numel() != n or not t.is_cuda or not t.is_contiguous():
+        raise ValueError(f"{what} must be {n} contiguous {dtype} values on the GPU")
+    return t.data_ptr()
+
+
+def _int8(t, what: str, shape: tuple):
+    import torch
+    if t.dtype != torch.int8:
+        raise ValueError(f"{what} must be int8, not {t.dtype}")
+    return _rows(t, what, shape, 16)
+
+
+def quantize_tokens(x, q, scales, stream=None):
+    """q (int8) and scales (fp32) = the rows of x [rows, cols] (fp32 or bf16) quantised with one scale per row
+    (uocr_quantize_tokens)."""
+    import torch
+    rows, cols = x.shape
+    dtype = _float_dtype(x, "x")
+    _check(lib().uocr_quantize_tokens(x.data_ptr(), dtype, rows, cols, _rows(x, "x", (rows, cols)), q.data_ptr(),
+                                      _int8(q, "q", (rows, cols)), _vector(scales, "scales", rows, torch.float32),
+                                      _stream(stream)))
+
+
+def linear_w8a8(x, x_scales, w, w_scales, y, bias=None, residual=None, stream=None):
+    """y[m, n] = x[m, k] . w[n, k]^T in int8 with x_scales per row of x and w_scales per row of w (+ bias[n])
+    (+ residual[m, n], of y's dtype; may be y itself) (uocr_linear_w8a8)."""
+    import torch
+    (m, k), n = x.shape, w.shape[0]
+    args = LinearW8A8Args(
+        x.data_ptr(), _vector(x_scales, "x_scales", m, torch.float32), w.data_ptr(),
+        _vector(w_scales, "w_scales", n, torch.float32),
+        None if bias is None else _vector(bias, "bias", n, torch.float32), _ptr(residual), y.data_ptr(), m, n, k,
+        _int8(x, "x", (m, k)), _int8(w, "w", (n, k)), 0 if residual is None else _rows(residual, "residual", (m, n)),
+        _rows(y, "y", (m, n)), _float_dtype(y, "y"), 0)
+    if residual is not None and residual.dtype != y.dtype:
+        raise ValueError("residual must have y's dtype")
+    _check(lib().uocr_linear_w8a8(ctypes.byref(args), _stream(stream)))
+
+
+def grouped_linear_w8a8(x, x_scales, w, w_scales, offsets, y, row_index=None, w_up=None, w_up_scales=None,
+                        stream=None):
+    """Group g's rows offsets[g] .. offsets[g + 1] - 1 of y [rows, n] = x[row_index[r]] . w[g]^T in int8, or with
+    w_up silu(x . w[g]^T) * (x . w_up[g]^T) (uocr_grouped_linear_w8a8). w, w_up: [groups, n, k] or the stack
+    [groups * n, k]; w_scales: groups * n values; offsets, row_index: int32."""
+    import torch
+    (x_rows, k), (rows, n), groups = x.shape, y.shape, offsets.numel() - 1
+
+    def stack(t, what):
+        if t.dim() == 3:
+            if groups > 1 and n > 1 and t.stride(0) != n * t.stride(1):
+                raise ValueError(f"{what}'s groups must follow one another")
+            t = t.as_strided((t.shape[0] * t.shape[1], t.shape[2]), (t.stride(1) if n > 1 else t.stride(0), t.stride(2)))
+        return _int8(t, what, (groups * n, k))
+
+    ldw = stack(w, "w")
+    if w_up is not None and stack(w_up, "w_up") != ldw:
+        raise ValueError("w_up must have w's pitch")
+    args = GroupedW8A8Args(
+        x.data_ptr(), _vector(x_scales, "x_scales", x_rows, torch.float32),
+        None if row_index is None else _vector(row_index, "row_index", rows, torch.int32),
+        _vector(offsets, "offsets", groups + 1, torch.int32), w.data_ptr(),
+        _vector(w_scales, "w_scales", groups * n, torch.float32), _ptr(w_up),
+        None if w_up is None else _vector(w_up_scales, "w_up_scales", groups * n, torch.float32), y.data_ptr(), rows,
+        x_rows, groups, n, k, _int8(x, "x", (x_rows, k)), ldw, _rows(y, "y", (rows, n)), _float_dtype(y, "y"), 0)
+    _check(lib().uocr_grouped_linear_w8a8(ctypes.byref(args), _stream(stream)))
 
 
 class Decoder:
