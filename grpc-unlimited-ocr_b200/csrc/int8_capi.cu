@@ -1,9 +1,8 @@
 // C ABI of the 8-bit integer operators (include/uocr_int8.h): argument checks
 // and launches. Host code only; the kernels are in quantize_tokens.cu and
-// w8a8.cu.
+// w8a8_gemm.cu.
 #include <cuda_runtime.h>
 
-#include <climits>
 #include <string>
 
 #include "../../include/uocr_int8.h"
@@ -13,6 +12,8 @@
 using namespace uocr_b200;
 
 namespace {
+
+constexpr int64_t kMaxRows = 1 << 30;  // row coordinates, tiles' overhang included, are 32-bit
 
 int bad(const char* op, const char* what) {
   return set_last_error(UOCR_ERR_INVALID_ARGUMENT, std::string(op) + ": " + what);
@@ -31,7 +32,7 @@ bool int8_rows_ok(const int8_t* base, int64_t ld) { return reinterpret_cast<uint
 int check_product(const char* op, const int8_t* x, const float* x_scales, const int8_t* w, const float* w_scales,
                   const void* y, int64_t rows, int64_t n, int64_t k, int64_t ldx, int64_t ldw, int64_t ldy,
                   int32_t y_dtype, int32_t reserved) {
-  if (rows < 0 || n < 0 || k <= 0 || rows > INT_MAX || n > INT_MAX) return bad(op, "bad shape");
+  if (rows < 0 || n < 0 || k <= 0 || rows > kMaxRows || n > kMaxRows) return bad(op, "bad shape");
   if (k > UOCR_W8A8_MAX_K) return set_last_error(UOCR_ERR_UNSUPPORTED, std::string(op) + ": k above 131071");
   if (y_dtype != UOCR_DTYPE_F32 && y_dtype != UOCR_DTYPE_BF16) return bad(op, "y must be f32 or bf16");
   if (reserved != 0) return bad(op, "reserved must be 0");
@@ -52,7 +53,7 @@ extern "C" {
 int uocr_quantize_tokens(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t ldx, int8_t* q,
                          int64_t ldq, float* scales, void* stream) {
   const char* op = "quantize_tokens";
-  if (rows < 0 || cols < 0 || rows > INT_MAX) return bad(op, "bad shape");
+  if (rows < 0 || cols < 0 || rows > kMaxRows) return bad(op, "bad shape");
   if (dtype != UOCR_DTYPE_F32 && dtype != UOCR_DTYPE_BF16) return bad(op, "x must be f32 or bf16");
   if (rows == 0) return UOCR_OK;
   if (scales == nullptr || (cols > 0 && (x == nullptr || q == nullptr))) return bad(op, "null pointer");
@@ -108,8 +109,9 @@ int uocr_grouped_linear_w8a8(const uocr_grouped_w8a8_args* a, void* stream) {
                                a->ldy, a->y_dtype, a->reserved);
   if (rc != UOCR_OK || a->rows == 0 || a->n == 0 || a->groups == 0) return rc;
   if (a->offsets == nullptr) return bad(op, "null pointer");
-  if (a->groups * a->n > INT_MAX) return set_last_error(UOCR_ERR_UNSUPPORTED, std::string(op) + ": groups * n above 2^31 - 1");
-  if (a->x_rows <= 0 || a->x_rows > INT_MAX) return bad(op, "bad shape");
+  if (a->groups * a->n > kMaxRows)
+    return set_last_error(UOCR_ERR_UNSUPPORTED, std::string(op) + ": groups * n above 2^30");
+  if (a->x_rows <= 0 || a->x_rows > kMaxRows) return bad(op, "bad shape");
   if (a->row_index == nullptr && a->x_rows != a->rows) return bad(op, "without row_index x has one row per output row");
   if (a->w_up != nullptr && (a->w_up_scales == nullptr || reinterpret_cast<uintptr_t>(a->w_up) % 16 != 0))
     return bad(op, "w_up needs its scales and a 16-byte aligned base");

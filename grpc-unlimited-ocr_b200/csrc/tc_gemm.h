@@ -1,6 +1,7 @@
 // Host interface of the tcgen05 grouped GEMM (tc_gemm.cu).
 #pragma once
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -69,6 +70,10 @@ struct GroupedGemm {
   int blocks;  // persistent grid size (the SM count)
   RowScatter scatter;  // world 0: routed rows to out_routed
 };
+
+// Tensor map of int8 rows [rows, cols] at `pitch` bytes (16-byte aligned rows):
+// boxes of 128 columns x box_rows rows, 128-byte swizzle, zeros past the edges.
+bool make_int8_tmap(CUtensorMap* map, const int8_t* base, int64_t rows, int64_t cols, int64_t pitch, int box_rows);
 
 size_t grouped_gemm_smem_bytes();
 cudaError_t launch_grouped_gemm(const GroupedGemm& g, cudaStream_t stream);

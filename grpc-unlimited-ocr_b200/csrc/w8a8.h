@@ -1,5 +1,5 @@
 // Host interface of the 8-bit integer operators: the token quantiser
-// (quantize_tokens.cu) and the products (w8a8.cu).
+// (quantize_tokens.cu) and the products (w8a8_gemm.cu).
 #pragma once
 
 #include <cuda_bf16.h>
