@@ -70,9 +70,12 @@ __device__ __forceinline__ void tma_gather4_pair(void* dst, const CUtensorMap* m
       : "memory");
 }
 
-// One arrival on the leader's mbarrier `bar` (a pair_leader_addr) from either CTA.
+// One arrival on the leader's mbarrier `bar` (a pair_leader_addr) from either
+// CTA. Release at CTA scope: what it announces is that TMEM has been read
+// (tcgen05.wait::ld, tcgen05.fence); a release at cluster scope would first
+// wait for the thread's global stores to be performed.
 __device__ __forceinline__ void mbar_arrive_pair(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 // ---- UMMA descriptors ----
