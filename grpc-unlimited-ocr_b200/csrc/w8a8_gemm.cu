@@ -2,22 +2,25 @@
 // signed 8-bit operands with int32 accumulators in TMEM, dense or grouped.
 //
 // The weights are the M operand and the tokens the N operand: a pair of SMs
-// (cta_group::2) multiplies 256 output channels (128 in each SM) by up to 256
+// (cta_group::2) multiplies 256 weight rows (128 in each SM) by up to 256
 // tokens, N being the tile's own token count rounded up to 32. A ragged group
 // so wastes at most 31 tokens' work, where a token tile of 256 rows would
-// waste half of it, and a handful of tokens costs a narrow MMA. The gated form
-// multiplies gate and up rows of the same channels by up to 128 tokens into
-// two accumulators, so that a thread has both values of a channel.
+// waste half of it, and a handful of tokens costs a narrow MMA. The 256 rows
+// are output channels, or in the gated form the gate and up rows of 128
+// channels, 64 and 64 in each SM.
 //
 // One persistent pair of blocks per two SMs, warp-specialised:
-//   warp 0     producer: each CTA's 128 weight rows (one box; two when gated)
-//              and its half of the token rows (boxes of 16 rows, a lane each,
-//              or gather4 of four indexed rows a lane) per 128-byte slice of K;
+//   warps 0, 2, 3  producers, one lane each, per 128-byte slice of K: warp 0
+//              the CTA's 128 weight rows, warp 2 its half of the token rows
+//              (boxes of 128, 64 or 16 rows), or warps 2 and 3 four indexed
+//              rows at a time (gather4);
 //   warp 1     allocates TMEM; in the leader one lane issues the MMAs;
-//   warps 4-11 epilogue: lane = channel, register = token, so the channel's
+//   warps 4-11 epilogue: lane = weight row, register = token, so a channel's
 //              scale stays in a register and a token's row is stored 32
-//              channels at a time, without staging.
+//              channels at a time. When gated, the gate's warp and the up's
+//              warp of the same channels exchange half of their tokens first.
 #include <mutex>
+#include <type_traits>
 
 #include "tc.cuh"
 #include "tc_gemm.h"
@@ -27,45 +30,53 @@ namespace uocr_b200 {
 namespace {
 
 constexpr int kMaxGroups = 512;
-constexpr int kBM = 128;               // channels per CTA
+constexpr int kBM = 128;               // weight rows per CTA
 constexpr int kBK = 128;               // bytes of K per stage (one swizzle atom)
-constexpr int kMaxN = 256;             // tokens per tile (128 when gated)
-constexpr int kRowBytes = kBK;
-constexpr int kThreads = 384;
+constexpr int kMaxN = 256;             // tokens per tile
+constexpr int kABytes = kBM * kBK;
+constexpr int kStageBytes = kABytes + kMaxN / 2 * kBK;
+constexpr int kStages = 6;
 constexpr int kEpilogueWarps = 8;
+constexpr int kWays = kEpilogueWarps / 4;  // epilogue warps of a TMEM lane quarter
+constexpr int kThreads = 128 + kEpilogueWarps * 32;
+constexpr int kXchBytes = 2 * 8 * 32 * 4;  // gated, per epilogue warp: two buffers of half a unit for its partner
+template <bool kGated>
+constexpr int kTokensPerUnit = kGated ? 16 : 32;  // tokens an epilogue warp takes at a time
+template <bool kGated>
+constexpr int kSmem = kStages * kStageBytes + (kGated ? kEpilogueWarps * kXchBytes : 0) + 1024;
 constexpr int kTmemCols = 512;
 constexpr int kBoxRows = 16;
 constexpr int kBand = 8;               // token tiles of a band (decode_tile)
 
-template <bool kGated>
-struct Shape {
-  static constexpr int kTokens = kGated ? kMaxN / 2 : kMaxN;
-  static constexpr int kABytes = (kGated ? 2 : 1) * kBM * kRowBytes;
-  static constexpr int kStageBytes = kABytes + kTokens / 2 * kRowBytes;
-  static constexpr int kStages = kGated ? 5 : 6;
-  static constexpr int kSmem = kStages * kStageBytes + 1024;
-};
-
 struct Args {
-  CUtensorMap x, x_wide, x_half, w, up;  // token boxes of 16 rows (gather: 1), 64, and a full tile's half
+  CUtensorMap x, x_wide, x_half, w, up;  // token boxes of 16 rows (gather: 1), 64 and 128; weight boxes of 128 (gated: 64)
   W8a8 p;
-  int tokens_per_tile;  // at most Shape::kTokens, a multiple of 32
+  int tokens_per_tile;  // at most kMaxN, a multiple of 32
+  int channels;         // output channels per tile of a pair
   int c_tiles, k_blocks;
 };
 
 struct Shared {
-  uint64_t full[6], empty[6];
+  uint64_t full[kStages], empty[kStages];
   uint64_t acc_full[2], acc_empty[2];
   uint64_t drain;
   uint32_t tmem;
+  alignas(16) int index[2][kMaxN / 4];  // gathered rows of a token producer's part of a tile
+  int failed[2];  // an epilogue warp's wait for this accumulator ran out
+  alignas(16) float x_scale[2][kMaxN];
   int tile_start[kMaxGroups + 1];
   int first[kMaxGroups], count[kMaxGroups];
-  alignas(16) float x_scale[2][kMaxN];
 };
 
 struct Tile {
   int g, row0, rows, c0;
 };
+
+// After a wait that ran out: the copies in flight land before this CTA's shared memory is given up.
+__device__ __noinline__ void wait_for_copies() {
+  const uint64_t until = global_timer_ns() + 5000000ull;
+  for (int i = 0; i < (1 << 20) && global_timer_ns() < until; ++i) __nanosleep(1000);
+}
 
 __device__ __forceinline__ int round32(int v) { return (v + 31) & ~31; }
 
@@ -86,7 +97,19 @@ __device__ __forceinline__ Tile decode_tile(int t, const Shared& sh, int groups,
   const int high = min(kBand, r_tiles - band * kBand);
   const int c = in_band / high;
   const int r = (band * kBand + in_band - c * high) * per;
-  return Tile{lo, sh.first[lo] + r, min(per, count - r), c * 2 * kBM};
+  return Tile{lo, sh.first[lo] + r, min(per, count - r), c * a.channels};
+}
+
+// float(a) to nearest, on the integer and FMA pipes: the conversion instruction
+// issues at about one lane a clock, which made the epilogue the kernel's bound
+// (108 us at 8192 x 8192 x 1024 with it). The halves of a become the low
+// mantissa bits of 1.5 * 2^23 and 2^23, both exact; the subtraction is exact
+// too (128 * 65536 = 2^23 undoes the lower half's bias), and the FMA rounds the
+// sum hi * 65536 + lo = a once.
+__device__ __forceinline__ float int_to_float(int a) {
+  const float hi = __int_as_float(0x4B400000 + (a >> 16)) - (12582912.0f + 128.0f);
+  const float lo = __int_as_float((a & 0xffff) | 0x4B000000);
+  return static_cast<float>(a);
 }
 
 // silu(g) * u = g / (1 + exp(-g)) * u. The quotient to 2 ulp (__fdividef): an
@@ -95,21 +118,35 @@ __device__ __forceinline__ Tile decode_tile(int t, const Shared& sh, int groups,
 __device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.0f + expf(-g)) * u; }
 
 template <bool kBf16>
-__device__ __forceinline__ float load_as_f32(const void* base, int64_t i) {
-  return kBf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(base)[i]) : static_cast<const float*>(base)[i];
-}
-template <bool kBf16>
-__device__ __forceinline__ void store_f32(void* base, int64_t i, float v) {
-  if (kBf16)
-    static_cast<__nv_bfloat16*>(base)[i] = __float2bfloat16_rn(v);
-  else
-    static_cast<float*>(base)[i] = v;
+using Out = typename std::conditional<kBf16, __nv_bfloat16, float>::type;
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+// Token i of this lane's channel, v[i], to row i < nr of `out` (the first
+// token's address, rows `pitch` bytes apart). A warp stores 32 channels of a
+// token at a time: whole 32-byte sectors, and a 128-byte line in fp32. Passing
+// the values through shared memory for 16-byte stores was slower (87 against
+// 72 us at 8192 x 8192 x 1024): the operands' copies and the MMAs leave little
+// of its bandwidth.
+template <typename T, int kRows>
+__device__ __forceinline__ void store_rows(const float (&v)[kRows], char* out, int64_t pitch, int nr) {
+  // Without a test per row the rows' arithmetic and stores overlap.
+  if (nr >= kRows) {
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) put(reinterpret_cast<T*>(out + i * pitch), v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+      if (i < nr) put(reinterpret_cast<T*>(out + i * pitch), v[i]);
+  }
 }
 
 template <bool kGated, bool kBf16>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     w8a8_gemm_kernel(const __grid_constant__ Args args) {
-  using S = Shape<kGated>;
   extern __shared__ unsigned char dyn_raw[];
   __shared__ Shared sh;
   unsigned char* smem =
@@ -120,7 +157,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int groups = static_cast<int>(p.groups);
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < S::kStages; ++s) {
+    for (int s = 0; s < kStages; ++s) {
       mbar_init(&sh.full[s], 1);
       mbar_init(&sh.empty[s], 1);
     }
@@ -129,6 +166,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       mbar_init(&sh.acc_empty[i], 2 * kEpilogueWarps);
     }
     mbar_init(&sh.drain, 1);
+    sh.failed[0] = sh.failed[1] = 0;
     fence_mbar_init();
   }
   if (warp == 0) {
@@ -172,84 +210,94 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int step = gridDim.x / 2;
 
   if (warp == 0) {
-    // ---- producer ----
-    const bool gather = p.row_index != nullptr;
-    // A tile's four gathered rows of this lane; rows past the tile or outside x read row 0 (never stored, or scaled
-    // by zero).
-    auto indices = [&](const Tile& tl, int (&idx)[4]) {
-      const int half = round32(tl.rows) / 2;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int j = rank * half + 4 * lane + i;
-        const int v = 4 * lane + i < half && j < tl.rows ? __ldg(p.row_index + tl.row0 + j) : 0;
-        idx[i] = v < 0 || v >= p.x_rows ? 0 : v;
-      }
-    };
-    int stage = 0;
-    uint32_t phase = 0;
-    int idx[4] = {0, 0, 0, 0};
-    int t = blockIdx.x / 2;
-    Tile tl{};
-    if (t < total) {
-      tl = decode_tile(t, sh, groups, args);
-      if (gather) indices(tl, idx);
-    }
-    bool ok = true;
-    while (t < total && ok) {
-      // The next tile and its indices are fetched while this one's copies run.
-      const int next_t = t + step;
-      Tile next{};
-      int next_idx[4] = {0, 0, 0, 0};
-      if (next_t < total) {
-        next = decode_tile(next_t, sh, groups, args);
-        if (gather) indices(next, next_idx);
-      }
-      const int n = round32(tl.rows), half = n / 2;
-      const int w_row = tl.g * static_cast<int>(p.n) + tl.c0 + rank * kBM;
-      for (int kb = 0; kb < args.k_blocks; ++kb) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&sh.empty[stage], phase ^ 1));  // the whole warp goes on or stops
-        if (!ok) {
-          raise_error(p.err, kDevWaitTimeout, 82, t, kb);
-          break;
+    // ---- weight producer: one lane; the leader also announces both CTAs' bytes of a stage ----
+    if (elect_one()) {
+      const uint32_t full0 = pair_leader_addr(&sh.full[0]);
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = blockIdx.x / 2; t < total && ok; t += step) {
+        const Tile tl = decode_tile(t, sh, groups, args);
+        const uint32_t bytes = 2 * kABytes + round32(tl.rows) * kBK;
+        const int w_row = tl.g * static_cast<int>(p.n) + tl.c0 + rank * (args.channels / 2);
+        for (int kb = 0; kb < args.k_blocks; ++kb) {
+          if (!mbar_wait(&sh.empty[stage], phase ^ 1)) {
+            raise_error(p.err, kDevWaitTimeout, 82, t, kb);
+            ok = false;
+            break;
+          }
+          unsigned char* sa = smem + stage * kStageBytes;
+          if (rank == 0) mbar_arrive_expect_tx(&sh.full[stage], bytes);
+          tma_load_2d_pair(sa, &args.w, kb * kBK, w_row, full0 + stage * 8);
+          if (kGated) tma_load_2d_pair(sa + kABytes / 2, &args.up, kb * kBK, w_row, full0 + stage * 8);
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1;
+          }
         }
-        const uint32_t bar = pair_leader_addr(&sh.full[stage]);
-        unsigned char* sa = smem + stage * S::kStageBytes;
-        unsigned char* sb = sa + S::kABytes;
-        if (lane == 0) {
-          if (rank == 0) mbar_arrive_expect_tx(&sh.full[stage], 2 * S::kABytes + n * kRowBytes);
-          tma_load_2d_pair(sa, &args.w, kb * kBK, w_row, bar);
-          if (kGated) tma_load_2d_pair(sa + kBM * kRowBytes, &args.up, kb * kBK, w_row, bar);
+      }
+      if (!ok) wait_for_copies();
+    }
+  } else if (warp == 2 || warp == 3) {
+    // ---- token producers: one lane each; warp 3 takes half of the rows when they are gathered ----
+    const bool gather = p.row_index != nullptr;
+    const uint32_t full0 = pair_leader_addr(&sh.full[0]);
+    int* idx = sh.index[warp - 2];
+    int stage = 0;  // of the elected lane (elect.sync names the same one every time)
+    uint32_t phase = 0;
+    bool ok = gather || warp == 2;
+    for (int t = blockIdx.x / 2; t < total && ok; t += step) {
+      const Tile tl = decode_tile(t, sh, groups, args);
+      const int half = round32(tl.rows) / 2;
+      const int row = tl.row0 + rank * half;  // this CTA's first token row
+      const int part = gather ? half / 2 : half;
+      const int skip = gather ? (warp - 2) * part : 0;
+      if (gather) {
+        // This warp's rows; those past the tile or outside x read row 0 (never stored, or scaled by zero).
+        __syncwarp();
+        for (int i = lane; i < part; i += 32) {
+          const int j = rank * half + skip + i;
+          const int v = j < tl.rows ? __ldg(p.row_index + tl.row0 + j) : 0;
+          idx[i] = v < 0 || v >= p.x_rows ? 0 : v;
         }
         __syncwarp();
-        if (gather) {
-          if (4 * lane < half)
-            tma_gather4_pair(sb + lane * 4 * kRowBytes, &args.x, kb * kBK, idx[0], idx[1], idx[2], idx[3], bar);
-        } else if (half == S::kTokens / 2) {
-          if (lane == 0) tma_load_2d_pair(sb, &args.x_half, kb * kBK, tl.row0 + rank * half, bar);
-        } else {
-          const int wide = half & ~63;  // rows in boxes of 64, the rest in boxes of 16
-          if (lane * 64 < wide)
-            tma_load_2d_pair(sb + lane * 64 * kRowBytes, &args.x_wide, kb * kBK, tl.row0 + rank * half + lane * 64, bar);
-          const int r = wide + (lane - 16) * kBoxRows;
-          if (lane >= 16 && r < half)
-            tma_load_2d_pair(sb + r * kRowBytes, &args.x, kb * kBK, tl.row0 + rank * half + r, bar);
-        }
-        if (++stage == S::kStages) {
-          stage = 0;
-          phase ^= 1;
-        }
       }
-      t = next_t;
-      tl = next;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) idx[i] = next_idx[i];
-    }
-    if (!ok) {  // the copies in flight land before this CTA's shared memory is given up
-      const uint64_t until = global_timer_ns() + 5000000ull;
-      for (int i = 0; i < (1 << 20) && global_timer_ns() < until; ++i) __nanosleep(1000);
+      if (elect_one()) {
+        for (int kb = 0; kb < args.k_blocks; ++kb) {
+          if (!mbar_wait(&sh.empty[stage], phase ^ 1)) {
+            raise_error(p.err, kDevWaitTimeout, 87, t, kb);
+            ok = false;
+            break;
+          }
+          unsigned char* sb = smem + stage * kStageBytes + kABytes;
+          const uint32_t bar = full0 + stage * 8;
+          if (gather) {
+#pragma unroll 4
+            for (int i = 0; i < part; i += 4) {
+              const int4 r = *reinterpret_cast<const int4*>(idx + i);
+              tma_gather4_pair(sb + (skip + i) * kBK, &args.x, kb * kBK, r.x, r.y, r.z, r.w, bar);
+            }
+          } else if (half == kMaxN / 2) {
+            tma_load_2d_pair(sb, &args.x_half, kb * kBK, row, bar);
+          } else {
+            int i = 0;
+            if (half >= 64) {
+              tma_load_2d_pair(sb, &args.x_wide, kb * kBK, row, bar);
+              i = 64;
+            }
+            for (; i < half; i += kBoxRows) tma_load_2d_pair(sb + i * kBK, &args.x, kb * kBK, row + i, bar);
+          }
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+        if (!ok) wait_for_copies();
+      }
+      ok = __all_sync(0xffffffffu, ok);
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0 && elect_one()) {
       // ---- MMA issuer (for both CTAs) ----
       int stage = 0, local = 0;
       uint32_t phase = 0;
@@ -271,17 +319,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             break;
           }
           tc_fence_after();
-          const uint32_t sa = smem_addr(smem + stage * S::kStageBytes);
+          const uint32_t sa = smem_addr(smem + stage * kStageBytes);
           const uint64_t ad = sw128_kmajor_desc(sa);
-          const uint64_t ud = sw128_kmajor_desc(sa + kBM * kRowBytes);
-          const uint64_t bd = sw128_kmajor_desc(sa + S::kABytes);
+          const uint64_t bd = sw128_kmajor_desc(sa + kABytes);
 #pragma unroll
-          for (int k = 0; k < kBK / 32; ++k) {  // 32 bytes of K per instruction: +2 in the address field
+          for (int k = 0; k < kBK / 32; ++k)  // 32 bytes of K per instruction: +2 in the address field
             umma_i8_pair(d, ad + 2 * k, bd + 2 * k, idesc, (kb | k) != 0 ? 1u : 0u);
-            if (kGated) umma_i8_pair(d + kMaxN / 2, ud + 2 * k, bd + 2 * k, idesc, (kb | k) != 0 ? 1u : 0u);
-          }
           umma_commit_pair(&sh.empty[stage]);
-          if (++stage == S::kStages) {
+          if (++stage == kStages) {
             stage = 0;
             phase ^= 1;
           }
@@ -292,40 +337,51 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (!mbar_wait(&sh.drain, 0)) raise_error(p.err, kDevWaitTimeout, 85, 0, 0);
     }
   } else if (warp >= 4) {
-    // ---- epilogue: TMEM lane quarter = warp % 4; the two warps of a quarter take every other 32 tokens ----
-    const int quarter = warp & 3, odd = (warp - 4) >> 2;
+    // ---- epilogue: TMEM lane quarter = warp % 4; the warps of a quarter take units in turn ----
+    using T = Out<kBf16>;
+    const int e = warp - 4, quarter = warp & 3, way = e >> 2;
     const int et = threadIdx.x - 128;
-    int local = 0;
+    unsigned char* area = smem + kStages * kStageBytes;
+    float* xch = reinterpret_cast<float*>(area + e * kXchBytes);
+    const float* xch_other = reinterpret_cast<const float*>(area + (e ^ 2) * kXchBytes);
+    const bool gate = quarter < 2;  // gated: lanes 0-63 hold gate rows, 64-127 up rows
+    const int local_c = kGated ? rank * 64 + (quarter & 1) * 32 : rank * kBM + quarter * 32;
+    const float* w_scales = kGated && !gate ? p.w_up_scales : p.w_scales;
+    constexpr int kUnit = kTokensPerUnit<kGated>;
+    int local = 0, buf = 0;
     bool ok = true;
     for (int t = blockIdx.x / 2; t < total; t += step, ++local) {
       const Tile tl = decode_tile(t, sh, groups, args);
       const int acc = local & 1;
-      const int64_t c = tl.c0 + rank * kBM + quarter * 32 + lane;
+      const int64_t c0 = tl.c0 + local_c, c = c0 + lane;
       const bool c_ok = c < p.n;
-      const float ws = c_ok ? __ldg(p.w_scales + tl.g * p.n + c) : 0.0f;
-      const float us = kGated && c_ok ? __ldg(p.w_up_scales + tl.g * p.n + c) : 0.0f;
-      const float bias = p.bias != nullptr && c_ok ? __ldg(p.bias + c) : 0.0f;
-      if (et < tl.rows) {
-        float s = 0.0f;
-        int64_t r = tl.row0 + et;
-        if (p.row_index != nullptr) {
-          const int v = __ldg(p.row_index + r);
-          if (v < 0 || v >= p.x_rows) {
-            raise_error(p.err, kDevBadIndex, kSiteRowIndex, static_cast<int>(r), v);
-            r = -1;
-          } else {
-            r = v;
+      const float ws = c_ok ? __ldg(w_scales + tl.g * p.n + c) : 0.0f;
+      const float bias = !kGated && p.bias != nullptr && c_ok ? __ldg(p.bias + c) : 0.0f;
+      if (et < round32(tl.rows)) {
+        float s = 0.0f;  // rows past the tile, and rows x does not have: zero
+        if (et < tl.rows) {
+          int64_t r = tl.row0 + et;
+          if (p.row_index != nullptr) {
+            const int v = __ldg(p.row_index + r);
+            if (v < 0 || v >= p.x_rows) {
+              raise_error(p.err, kDevBadIndex, kSiteRowIndex, static_cast<int>(r), v);
+              r = -1;
+            } else {
+              r = v;
+            }
           }
+          if (r >= 0) s = __ldg(p.x_scales + r);
         }
-        if (r >= 0) s = __ldg(p.x_scales + r);
         sh.x_scale[acc][et] = s;
       }
-      named_bar_sync(1, kEpilogueWarps * 32);
       if (ok) {
         ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[acc], (local >> 1) & 1));
         if (!ok) raise_error(p.err, kDevWaitTimeout, 86, t, 0);
       }
-      if (!ok) continue;  // the warps that go on still meet this one at the barrier above
+      if (!ok && lane == 0) sh.failed[acc] = 1;
+      named_bar_sync(1, kEpilogueWarps * 32);  // the scales are there; and all warps go on with this tile or none
+      ok = sh.failed[acc] == 0;
+      if (!ok) continue;
       tc_fence_after();
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * kMaxN);
       auto release = [&] {  // this warp has read its last columns: the accumulator may be written again
@@ -333,47 +389,56 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive_pair(pair_leader_addr(&sh.acc_empty[acc]));
       };
-      if (odd * 32 >= tl.rows) release();
-      for (int j0 = odd * 32; j0 < tl.rows; j0 += 64) {
-        int a[32], u[32];
-        tmem_ld32_async(taddr + j0, a);
-        if (kGated) tmem_ld32_async(taddr + kMaxN / 2 + j0, u);
-        tmem_ld_wait(a);
-        if (kGated) tmem_ld_wait(u);
-        if (j0 + 64 >= tl.rows) release();
-        const int nr = c_ok ? min(32, tl.rows - j0) : 0;
-        float v[32];
+      if (way * kUnit >= tl.rows) release();
+      for (int j0 = way * kUnit; j0 < tl.rows; j0 += kWays * kUnit) {
+        int a[kUnit];
+        tmem_ld_i32(taddr + j0, a);
+        if (j0 + kWays * kUnit >= tl.rows) release();
+        float v[kUnit];
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          const float4 s4 = *reinterpret_cast<const float4*>(&sh.x_scale[acc][j0 + i]);
-          const float s[4] = {s4.x, s4.y, s4.z, s4.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            v[i + e] = static_cast<float>(a[i + e]) * s[e] * ws;
-            if (kGated) v[i + e] = silu_mul(v[i + e], static_cast<float>(u[i + e]) * s[e] * us);
-          }
+        for (int i = 0; i < kUnit; i += 4) {
+          const float4 s = *reinterpret_cast<const float4*>(&sh.x_scale[acc][j0 + i]);
+          v[i] = int_to_float(a[i]) * s.x * ws;
+          v[i + 1] = int_to_float(a[i + 1]) * s.y * ws;
+          v[i + 2] = int_to_float(a[i + 2]) * s.z * ws;
+          v[i + 3] = int_to_float(a[i + 3]) * s.w * ws;
         }
         const int64_t row = tl.row0 + j0;
-        if (!kGated) {
+        const int nr = c_ok ? tl.rows - j0 : 0;
+        char* out = static_cast<char*>(p.y) + (row * p.ldy + c) * sizeof(T);
+        const int64_t pitch = p.ldy * sizeof(T);
+        if (kGated) {
+          // The gate's warp finishes the unit's first half, the up's warp the second.
+          constexpr int kHalf = kUnit / 2;
+          float* mine = xch + buf * kHalf * 32;
+          const float* other = xch_other + buf * kHalf * 32;
+          buf ^= 1;
+#pragma unroll
+          for (int i = 0; i < kHalf; ++i) mine[i * 32 + lane] = gate ? v[kHalf + i] : v[i];
+          named_bar_sync(2 + (quarter & 1) + 2 * way, 64);
+          float o[kHalf];
+#pragma unroll
+          for (int i = 0; i < kHalf; ++i) {
+            const float w = other[i * 32 + lane];
+            o[i] = gate ? silu_mul(v[i], w) : silu_mul(w, v[kHalf + i]);
+          }
+          const int skip = gate ? 0 : kHalf;
+          store_rows<T>(o, out + skip * pitch, pitch, nr - skip);
+        } else {
           if (p.bias != nullptr) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] += bias;
+            for (int i = 0; i < kUnit; ++i) v[i] += bias;
           }
           if (p.residual != nullptr) {
-            float r[32];
+            const T* res = static_cast<const T*>(p.residual) + row * p.ldr + c;
+            float r[kUnit];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) r[i] = i < nr ? load_as_f32<kBf16>(p.residual, (row + i) * p.ldr + c) : 0.0f;
+            for (int i = 0; i < kUnit; ++i) r[i] = i < nr ? to_f32(res[i * p.ldr]) : 0.0f;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] += r[i];
+            for (int i = 0; i < kUnit; ++i) v[i] += r[i];
           }
+          store_rows<T>(v, out, pitch, nr);
         }
-        char* out = static_cast<char*>(p.y) + (row * p.ldy + c) * (kBf16 ? 2 : 4);
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (i < nr) {
-            store_f32<kBf16>(out, 0, v[i]);
-            out += p.ldy * (kBf16 ? 2 : 4);
-          }
       }
     }
   }
@@ -401,14 +466,14 @@ cudaError_t resident_pairs(int* pairs) {
   std::lock_guard<std::mutex> lock(mu);
   if (known[dev] == 0) {
     const auto kernel = w8a8_gemm_kernel<kGated, kBf16>;
-    st = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<kGated>::kSmem);
+    st = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem<kGated>);
     if (st != cudaSuccess) return st;
     int sms = 0;
     if ((st = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return st;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(sms / 2 * 2));
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = Shape<kGated>::kSmem;
+    cfg.dynamicSmemBytes = kSmem<kGated>;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2;
@@ -428,7 +493,8 @@ cudaError_t resident_pairs(int* pairs) {
 // Tokens per tile: as many as fit where there are tiles enough for the pairs.
 // A narrower MMA costs less, down to 64 tokens, so where the tiles are few
 // (one wave or a broken one) the width that ends first is taken.
-int choose_tokens(int64_t rows, int64_t groups, int c_tiles, int pairs, int most) {
+int choose_tokens(int64_t rows, int64_t groups, int c_tiles, int pairs) {
+  constexpr int most = kMaxN;
   if (groups > 1) {
     int bn = most;
     while (bn > 64 && (rows / bn + (groups < rows ? groups : rows) / 2) * c_tiles < pairs) bn /= 2;
@@ -456,18 +522,19 @@ cudaError_t launch(const W8a8& p, cudaStream_t stream) {
   Args a{};
   const bool ok = make_int8_tmap(&a.x, p.x, p.x_rows, p.k, p.ldx, p.row_index != nullptr ? 1 : kBoxRows) &&
                   make_int8_tmap(&a.x_wide, p.x, p.x_rows, p.k, p.ldx, 64) &&
-                  make_int8_tmap(&a.x_half, p.x, p.x_rows, p.k, p.ldx, Shape<kGated>::kTokens / 2) &&
-                  make_int8_tmap(&a.w, p.w, p.groups * p.n, p.k, p.ldw, kBM) &&
-                  (!kGated || make_int8_tmap(&a.up, p.w_up, p.groups * p.n, p.k, p.ldw, kBM));
+                  make_int8_tmap(&a.x_half, p.x, p.x_rows, p.k, p.ldx, kMaxN / 2) &&
+                  make_int8_tmap(&a.w, p.w, p.groups * p.n, p.k, p.ldw, kGated ? kBM / 2 : kBM) &&
+                  (!kGated || make_int8_tmap(&a.up, p.w_up, p.groups * p.n, p.k, p.ldw, kBM / 2));
   if (!ok) return cudaErrorInvalidValue;
   a.p = p;
-  a.c_tiles = static_cast<int>((p.n + 2 * kBM - 1) / (2 * kBM));
+  a.channels = kGated ? kBM : 2 * kBM;
+  a.c_tiles = static_cast<int>((p.n + a.channels - 1) / a.channels);
   a.k_blocks = static_cast<int>((p.k + kBK - 1) / kBK);
-  a.tokens_per_tile = choose_tokens(p.rows, p.groups, a.c_tiles, pairs, Shape<kGated>::kTokens);
+  a.tokens_per_tile = choose_tokens(p.rows, p.groups, a.c_tiles, pairs);
   const int64_t most =
       (p.rows / a.tokens_per_tile + (p.groups < p.rows ? p.groups : p.rows)) * static_cast<int64_t>(a.c_tiles);
   const unsigned blocks = 2u * static_cast<unsigned>(most < pairs ? most : pairs);
-  w8a8_gemm_kernel<kGated, kBf16><<<blocks, kThreads, Shape<kGated>::kSmem, stream>>>(a);
+  w8a8_gemm_kernel<kGated, kBf16><<<blocks, kThreads, kSmem<kGated>, stream>>>(a);
   return cudaGetLastError();
 }
 
