@@ -15,10 +15,15 @@
 //              (boxes of 128, 64 or 16 rows), or warps 2 and 3 four indexed
 //              rows at a time (gather4);
 //   warp 1     allocates TMEM; in the leader one lane issues the MMAs;
-//   warps 4-11 epilogue: lane = weight row, register = token, so a channel's
-//              scale stays in a register and a token's row is stored 32
-//              channels at a time. When gated, the gate's warp and the up's
-//              warp of the same channels exchange half of their tokens first.
+//   warps 4-11 epilogue, 16 tokens x 32 weight rows at a time: the scales,
+//              then bf16 tiles are transposed into shared memory (stmatrix) and
+//              leave as bulk tensor stores, fp32 ones as sectors of 8 channels.
+//              When gated, the gate's warp and the up's warp of the same
+//              channels exchange half of their tokens first.
+// The operands' copies into shared memory and the MMAs' reads of it take
+// nearly all of its bandwidth (64 + 64 bytes a clock at the full MMA rate), and
+// every store and shared-memory access of the epilogue takes a clock of the
+// same pipe: the layout is chosen for few and full ones.
 #include <mutex>
 #include <type_traits>
 
@@ -39,21 +44,26 @@ constexpr int kStages = 6;
 constexpr int kEpilogueWarps = 8;
 constexpr int kWays = kEpilogueWarps / 4;  // epilogue warps of a TMEM lane quarter
 constexpr int kThreads = 128 + kEpilogueWarps * 32;
-constexpr int kXchBytes = 2 * 8 * 32 * 4;  // gated, per epilogue warp: two buffers of half a unit for its partner
+constexpr int kUnit = 16;              // tokens an epilogue warp takes at a time
+constexpr int kOutBytes = kUnit * 32 * 2;        // a unit of 32 channels in bf16
+constexpr int kXchBytes = kUnit / 2 * 32 * 4;    // gated: half a unit's values for the partner warp
+// Per epilogue warp, two buffers of each (a gated warp's output is half a unit).
 template <bool kGated>
-constexpr int kTokensPerUnit = kGated ? 16 : 32;  // tokens an epilogue warp takes at a time
+constexpr int kWarpBytes = kGated ? kOutBytes + 2 * kXchBytes : 2 * kOutBytes;
 template <bool kGated>
-constexpr int kSmem = kStages * kStageBytes + (kGated ? kEpilogueWarps * kXchBytes : 0) + 1024;
+constexpr int kSmem = kStages * kStageBytes + kEpilogueWarps * kWarpBytes<kGated> + 1024;
 constexpr int kTmemCols = 512;
 constexpr int kBoxRows = 16;
 constexpr int kBand = 8;               // token tiles of a band (decode_tile)
 
 struct Args {
+  CUtensorMap y;                         // boxes of a unit's tokens (gated: half) x 32 channels; unset unless tma_store
   CUtensorMap x, x_wide, x_half, w, up;  // token boxes of 16 rows (gather: 1), 64 and 128; weight boxes of 128 (gated: 64)
   W8a8 p;
   int tokens_per_tile;  // at most kMaxN, a multiple of 32
   int channels;         // output channels per tile of a pair
   int c_tiles, k_blocks;
+  bool tma_store;       // y is bf16 and its rows start at 16-byte boundaries
 };
 
 struct Shared {
@@ -100,18 +110,6 @@ __device__ __forceinline__ Tile decode_tile(int t, const Shared& sh, int groups,
   return Tile{lo, sh.first[lo] + r, min(per, count - r), c * a.channels};
 }
 
-// float(a) to nearest, on the integer and FMA pipes: the conversion instruction
-// issues at about one lane a clock, which made the epilogue the kernel's bound
-// (108 us at 8192 x 8192 x 1024 with it). The halves of a become the low
-// mantissa bits of 1.5 * 2^23 and 2^23, both exact; the subtraction is exact
-// too (128 * 65536 = 2^23 undoes the lower half's bias), and the FMA rounds the
-// sum hi * 65536 + lo = a once.
-__device__ __forceinline__ float int_to_float(int a) {
-  const float hi = __int_as_float(0x4B400000 + (a >> 16)) - (12582912.0f + 128.0f);
-  const float lo = __int_as_float((a & 0xffff) | 0x4B000000);
-  return static_cast<float>(a);
-}
-
 // silu(g) * u = g / (1 + exp(-g)) * u. The quotient to 2 ulp (__fdividef): an
 // IEEE division branches, and 32 of them in a row keep a thread's 32 tokens
 // from overlapping (the gated kernel's time at eight pages: 928 us with it).
@@ -125,23 +123,48 @@ __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162flo
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-// Token i of this lane's channel, v[i], to row i < nr of `out` (the first
-// token's address, rows `pitch` bytes apart). A warp stores 32 channels of a
-// token at a time: whole 32-byte sectors, and a 128-byte line in fp32. Passing
-// the values through shared memory for 16-byte stores was slower (87 against
-// 72 us at 8192 x 8192 x 1024): the operands' copies and the MMAs leave little
-// of its bandwidth.
-template <typename T, int kRows>
-__device__ __forceinline__ void store_rows(const float (&v)[kRows], char* out, int64_t pitch, int nr) {
-  // Without a test per row the rows' arithmetic and stores overlap.
-  if (nr >= kRows) {
+// (float(a0) * s0 * w, float(a1) * s1 * w): two tokens' sums scaled, with packed products.
+__device__ __forceinline__ void scale_pair(int a0, int a1, uint64_t s2, uint64_t w2, float& v0, float& v1) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(static_cast<float>(a0)), "f"(static_cast<float>(a1)));
+  asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(v) : "l"(s2));
+  asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(v) : "l"(w2));
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(v0), "=f"(v1) : "l"(v));
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Eight tokens x 32 channels of a warp: v[2 q + e] is channel t / 4 + 8 q of
+// token 2 (t % 4) + e in thread t.
+using Block = float[8];
+
+// Block b of a unit in bf16 to the unit's rows of 64 bytes in shared memory, as the 64-byte swizzle has them.
+__device__ __forceinline__ void stage_block(const Block& v, unsigned char* stg, int b, int lane) {
+  const int token = b * 8 + (lane & 7);
+  stmatrix_x4_trans(stg + token * 64 + (((lane >> 3) ^ ((token >> 1) & 3)) << 4), pack_bf16(v[0], v[1]),
+                    pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+}
+
+// A block to (or a residual's block from) rows at `base`, the address of this
+// thread's first token and channel: tokens below nr, channels below nc.
+template <typename T>
+__device__ __forceinline__ void store_block(const Block& v, T* base, int64_t ld, int nr, int nc) {
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) put(reinterpret_cast<T*>(out + i * pitch), v[i]);
-  } else {
+  for (int e = 0; e < 2; ++e) {
+    if (e >= nr) continue;
 #pragma unroll
-    for (int i = 0; i < kRows; ++i)
-      if (i < nr) put(reinterpret_cast<T*>(out + i * pitch), v[i]);
+    for (int q = 0; q < 4; ++q)
+      if (8 * q < nc) put(base + e * ld + 8 * q, v[2 * q + e]);
   }
+}
+template <typename T>
+__device__ __forceinline__ void load_block(Block& v, const T* base, int64_t ld, int nr, int nc) {
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[2 * q + e] = e < nr && 8 * q < nc ? to_f32(base[e * ld + 8 * q]) : 0.0f;
 }
 
 template <bool kGated, bool kBf16>
@@ -341,22 +364,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     using T = Out<kBf16>;
     const int e = warp - 4, quarter = warp & 3, way = e >> 2;
     const int et = threadIdx.x - 128;
+    const int tr = lane >> 2, tc = 2 * (lane & 3);  // this thread's first channel and token in a block
     unsigned char* area = smem + kStages * kStageBytes;
-    float* xch = reinterpret_cast<float*>(area + e * kXchBytes);
-    const float* xch_other = reinterpret_cast<const float*>(area + (e ^ 2) * kXchBytes);
+    unsigned char* stg = area + e * kWarpBytes<kGated>;
+    float4* xch = reinterpret_cast<float4*>(stg + kOutBytes);
+    const float4* xch_other = reinterpret_cast<const float4*>(area + (e ^ 2) * kWarpBytes<kGated> + kOutBytes);
     const bool gate = quarter < 2;  // gated: lanes 0-63 hold gate rows, 64-127 up rows
     const int local_c = kGated ? rank * 64 + (quarter & 1) * 32 : rank * kBM + quarter * 32;
     const float* w_scales = kGated && !gate ? p.w_up_scales : p.w_scales;
-    constexpr int kUnit = kTokensPerUnit<kGated>;
+    T* y = static_cast<T*>(p.y);
     int local = 0, buf = 0;
     bool ok = true;
     for (int t = blockIdx.x / 2; t < total; t += step, ++local) {
       const Tile tl = decode_tile(t, sh, groups, args);
       const int acc = local & 1;
-      const int64_t c0 = tl.c0 + local_c, c = c0 + lane;
-      const bool c_ok = c < p.n;
-      const float ws = c_ok ? __ldg(w_scales + tl.g * p.n + c) : 0.0f;
-      const float bias = !kGated && p.bias != nullptr && c_ok ? __ldg(p.bias + c) : 0.0f;
+      const int64_t c0 = tl.c0 + local_c, c = c0 + tr;
+      const int nc = static_cast<int>(p.n - c < 32 ? p.n - c : 32);  // channels c, c + 8, .. below c + nc exist
+      uint64_t ws[4];
+      float bias[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float w = 8 * q < nc ? __ldg(w_scales + tl.g * p.n + c + 8 * q) : 0.0f;
+        asm("mov.b64 %0, {%1, %1};" : "=l"(ws[q]) : "f"(w));
+        bias[q] = !kGated && p.bias != nullptr && 8 * q < nc ? __ldg(p.bias + c + 8 * q) : 0.0f;
+      }
       if (et < round32(tl.rows)) {
         float s = 0.0f;  // rows past the tile, and rows x does not have: zero
         if (et < tl.rows) {
@@ -391,56 +422,97 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       };
       if (way * kUnit >= tl.rows) release();
       for (int j0 = way * kUnit; j0 < tl.rows; j0 += kWays * kUnit) {
-        int a[kUnit];
-        tmem_ld_i32(taddr + j0, a);
-        if (j0 + kWays * kUnit >= tl.rows) release();
-        float v[kUnit];
-#pragma unroll
-        for (int i = 0; i < kUnit; i += 4) {
-          const float4 s = *reinterpret_cast<const float4*>(&sh.x_scale[acc][j0 + i]);
-          v[i] = int_to_float(a[i]) * s.x * ws;
-          v[i + 1] = int_to_float(a[i + 1]) * s.y * ws;
-          v[i + 2] = int_to_float(a[i + 2]) * s.z * ws;
-          v[i + 3] = int_to_float(a[i + 3]) * s.w * ws;
-        }
+        int a[2][8];  // [16 lanes][the two blocks' four values]
+        tmem_ld_16x16(taddr + j0, a[0]);
+        tmem_ld_16x16(taddr + (16u << 16) + j0, a[1]);
         const int64_t row = tl.row0 + j0;
-        const int nr = c_ok ? tl.rows - j0 : 0;
-        char* out = static_cast<char*>(p.y) + (row * p.ldy + c) * sizeof(T);
-        const int64_t pitch = p.ldy * sizeof(T);
+        const int nr = tl.rows - j0;
+        Block r[2];
+        if (!kGated && p.residual != nullptr) {
+          const T* res = static_cast<const T*>(p.residual) + (row + tc) * p.ldr + c;
+          load_block(r[0], res, p.ldr, nr - tc, nc);
+          load_block(r[1], res + 8 * p.ldr, p.ldr, nr - tc - 8, nc);
+        }
+        tmem_ld_wait(a[0], a[1]);
+        if (j0 + kWays * kUnit >= tl.rows) release();
+        Block v[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const uint64_t s = *reinterpret_cast<const uint64_t*>(&sh.x_scale[acc][j0 + 8 * b + tc]);
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            scale_pair(a[q >> 1][4 * b + 2 * (q & 1)], a[q >> 1][4 * b + 2 * (q & 1) + 1], s, ws[q], v[b][2 * q],
+                       v[b][2 * q + 1]);
+        }
+        buf ^= 1;
         if (kGated) {
-          // The gate's warp finishes the unit's first half, the up's warp the second.
-          constexpr int kHalf = kUnit / 2;
-          float* mine = xch + buf * kHalf * 32;
-          const float* other = xch_other + buf * kHalf * 32;
-          buf ^= 1;
+          // The gate's warp finishes the unit's first block, the up's warp the second.
+          float4* give = xch + buf * (kXchBytes / 16);
+          const float4* take = xch_other + buf * (kXchBytes / 16);
+          Block g, o;
 #pragma unroll
-          for (int i = 0; i < kHalf; ++i) mine[i * 32 + lane] = gate ? v[kHalf + i] : v[i];
+          for (int i = 0; i < 8; ++i) o[i] = gate ? v[1][i] : v[0][i];
+          give[lane] = make_float4(o[0], o[1], o[2], o[3]);
+          give[32 + lane] = make_float4(o[4], o[5], o[6], o[7]);
           named_bar_sync(2 + (quarter & 1) + 2 * way, 64);
-          float o[kHalf];
+          const float4 t0 = take[lane], t1 = take[32 + lane];
+          const float w[8] = {t0.x, t0.y, t0.z, t0.w, t1.x, t1.y, t1.z, t1.w};
 #pragma unroll
-          for (int i = 0; i < kHalf; ++i) {
-            const float w = other[i * 32 + lane];
-            o[i] = gate ? silu_mul(v[i], w) : silu_mul(w, v[kHalf + i]);
+          for (int i = 0; i < 8; ++i) {
+            g[i] = gate ? v[0][i] : w[i];
+            o[i] = silu_mul(g[i], gate ? w[i] : v[1][i]);
           }
-          const int skip = gate ? 0 : kHalf;
-          store_rows<T>(o, out + skip * pitch, pitch, nr - skip);
+          const int skip = gate ? 0 : 8;
+          if (kBf16 && args.tma_store && nr >= skip + 8) {
+            unsigned char* out = stg + buf * (kOutBytes / 2);
+            if (elect_one()) bulk_wait_read<1>();  // the store before the last has read this buffer
+            __syncwarp();
+            stage_block(o, out, 0, lane);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (elect_one()) {
+              if (c0 < p.n) tma_store_2d(&args.y, static_cast<int>(c0), static_cast<int>(row) + skip, out);
+              bulk_commit();
+            }
+          } else {
+            store_block(o, y + (row + skip + tc) * p.ldy + c, p.ldy, nr - skip - tc, nc);
+          }
         } else {
           if (p.bias != nullptr) {
 #pragma unroll
-            for (int i = 0; i < kUnit; ++i) v[i] += bias;
+            for (int i = 0; i < 8; ++i) {
+              v[0][i] += bias[i / 2];
+              v[1][i] += bias[i / 2];
+            }
           }
           if (p.residual != nullptr) {
-            const T* res = static_cast<const T*>(p.residual) + row * p.ldr + c;
-            float r[kUnit];
 #pragma unroll
-            for (int i = 0; i < kUnit; ++i) r[i] = i < nr ? to_f32(res[i * p.ldr]) : 0.0f;
-#pragma unroll
-            for (int i = 0; i < kUnit; ++i) v[i] += r[i];
+            for (int i = 0; i < 8; ++i) {
+              v[0][i] += r[0][i];
+              v[1][i] += r[1][i];
+            }
           }
-          store_rows<T>(v, out, pitch, nr);
+          if (kBf16 && args.tma_store && nr >= kUnit) {
+            unsigned char* out = stg + buf * kOutBytes;
+            if (elect_one()) bulk_wait_read<1>();
+            __syncwarp();
+            stage_block(v[0], out, 0, lane);
+            stage_block(v[1], out, 1, lane);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (elect_one()) {
+              if (c0 < p.n) tma_store_2d(&args.y, static_cast<int>(c0), static_cast<int>(row), out);
+              bulk_commit();
+            }
+          } else {
+            T* dst = y + (row + tc) * p.ldy + c;
+            store_block(v[0], dst, p.ldy, nr - tc, nc);
+            store_block(v[1], dst + 8 * p.ldy, p.ldy, nr - tc - 8, nc);
+          }
         }
       }
     }
+    if (elect_one()) bulk_wait_read<0>();
   }
   __syncwarp();
   tc_fence_before();
@@ -526,6 +598,9 @@ cudaError_t launch(const W8a8& p, cudaStream_t stream) {
                   make_int8_tmap(&a.w, p.w, p.groups * p.n, p.k, p.ldw, kGated ? kBM / 2 : kBM) &&
                   (!kGated || make_int8_tmap(&a.up, p.w_up, p.groups * p.n, p.k, p.ldw, kBM / 2));
   if (!ok) return cudaErrorInvalidValue;
+  a.tma_store = kBf16 && reinterpret_cast<uintptr_t>(p.y) % 16 == 0 && p.ldy % 8 == 0;
+  if (a.tma_store && !make_store_tmap(&a.y, static_cast<__nv_bfloat16*>(p.y), p.rows, p.n, p.ldy, kGated ? kUnit / 2 : kUnit))
+    return cudaErrorInvalidValue;
   a.p = p;
   a.channels = kGated ? kBM : 2 * kBM;
   a.c_tiles = static_cast<int>((p.n + a.channels - 1) / a.channels);
