@@ -15,7 +15,7 @@
 //              (boxes of 128, 64 or 16 rows), or warps 2 and 3 four indexed
 //              rows at a time (gather4);
 //   warp 1     allocates TMEM; in the leader one lane issues the MMAs;
-//   warps 4-11 epilogue, 16 tokens x 32 weight rows at a time: the scales,
+//   warps 4-11 epilogue, 32 tokens x 32 weight rows at a time: the scales,
 //              then bf16 tiles are transposed into shared memory (stmatrix) and
 //              leave as bulk tensor stores, fp32 ones as sectors of 8 channels.
 //              When gated, the gate's warp and the up's warp of the same
@@ -40,11 +40,11 @@ constexpr int kBK = 128;               // bytes of K per stage (one swizzle atom
 constexpr int kMaxN = 256;             // tokens per tile
 constexpr int kABytes = kBM * kBK;
 constexpr int kStageBytes = kABytes + kMaxN / 2 * kBK;
-constexpr int kStages = 6;
+constexpr int kStages = 5;
 constexpr int kEpilogueWarps = 8;
 constexpr int kWays = kEpilogueWarps / 4;  // epilogue warps of a TMEM lane quarter
 constexpr int kThreads = 128 + kEpilogueWarps * 32;
-constexpr int kUnit = 16;              // tokens an epilogue warp takes at a time
+constexpr int kUnit = 32;              // tokens an epilogue warp takes at a time
 constexpr int kOutBytes = kUnit * 32 * 2;        // a unit of 32 channels in bf16
 constexpr int kXchBytes = kUnit / 2 * 32 * 4;    // gated: half a unit's values for the partner warp
 // Per epilogue warp, two buffers of each (a gated warp's output is half a unit).
@@ -148,7 +148,15 @@ __device__ __forceinline__ void stage_block(const Block& v, unsigned char* stg, 
 }
 
 // A block to (or a residual's block from) rows at `base`, the address of this
-// thread's first token and channel: tokens below nr, channels below nc.
+// thread's first token and channel: tokens below nr, channels below nc, or
+// all of them, without a test that would keep the accesses from overlapping.
+template <typename T>
+__device__ __forceinline__ void store_block(const Block& v, T* base, int64_t ld) {
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) put(base + e * ld + 8 * q, v[2 * q + e]);
+}
 template <typename T>
 __device__ __forceinline__ void store_block(const Block& v, T* base, int64_t ld, int nr, int nc) {
 #pragma unroll
@@ -158,6 +166,13 @@ __device__ __forceinline__ void store_block(const Block& v, T* base, int64_t ld,
     for (int q = 0; q < 4; ++q)
       if (8 * q < nc) put(base + e * ld + 8 * q, v[2 * q + e]);
   }
+}
+template <typename T>
+__device__ __forceinline__ void load_block(Block& v, const T* base, int64_t ld) {
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[2 * q + e] = to_f32(base[e * ld + 8 * q]);
 }
 template <typename T>
 __device__ __forceinline__ void load_block(Block& v, const T* base, int64_t ld, int nr, int nc) {
@@ -373,38 +388,53 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int local_c = kGated ? rank * 64 + (quarter & 1) * 32 : rank * kBM + quarter * 32;
     const float* w_scales = kGated && !gate ? p.w_up_scales : p.w_scales;
     T* y = static_cast<T*>(p.y);
+    const bool has_bias = !kGated && p.bias != nullptr, has_residual = !kGated && p.residual != nullptr;
+    // What the epilogue needs of a tile beside its sums; the next tile's is
+    // fetched while this one's units are stored.
+    struct Scales {
+      Tile tl;
+      float w[4], bias[4];  // of channels tr + 8 q
+      float x;              // of token et
+    };
+    auto fetch = [&](int t) {
+      Scales f{};
+      f.tl = decode_tile(t, sh, groups, args);
+      const int64_t c = f.tl.c0 + local_c + tr;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const bool in = c + 8 * q < p.n;
+        f.w[q] = in ? __ldg(w_scales + f.tl.g * p.n + c + 8 * q) : 0.0f;
+        f.bias[q] = has_bias && in ? __ldg(p.bias + c + 8 * q) : 0.0f;
+      }
+      if (et < f.tl.rows) {  // tokens past the tile, and rows x does not have: zero
+        int64_t r = f.tl.row0 + et;
+        if (p.row_index != nullptr) {
+          const int v = __ldg(p.row_index + r);
+          if (v < 0 || v >= p.x_rows) {
+            raise_error(p.err, kDevBadIndex, kSiteRowIndex, static_cast<int>(r), v);
+            r = -1;
+          } else {
+            r = v;
+          }
+        }
+        if (r >= 0) f.x = __ldg(p.x_scales + r);
+      }
+      return f;
+    };
+    Scales next{};
+    if (blockIdx.x / 2 < total) next = fetch(blockIdx.x / 2);
     int local = 0, buf = 0;
     bool ok = true;
     for (int t = blockIdx.x / 2; t < total; t += step, ++local) {
-      const Tile tl = decode_tile(t, sh, groups, args);
+      const Scales cur = next;
+      const Tile& tl = cur.tl;
       const int acc = local & 1;
       const int64_t c0 = tl.c0 + local_c, c = c0 + tr;
       const int nc = static_cast<int>(p.n - c < 32 ? p.n - c : 32);  // channels c, c + 8, .. below c + nc exist
+      sh.x_scale[acc][et] = cur.x;
       uint64_t ws[4];
-      float bias[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float w = 8 * q < nc ? __ldg(w_scales + tl.g * p.n + c + 8 * q) : 0.0f;
-        asm("mov.b64 %0, {%1, %1};" : "=l"(ws[q]) : "f"(w));
-        bias[q] = !kGated && p.bias != nullptr && 8 * q < nc ? __ldg(p.bias + c + 8 * q) : 0.0f;
-      }
-      if (et < round32(tl.rows)) {
-        float s = 0.0f;  // rows past the tile, and rows x does not have: zero
-        if (et < tl.rows) {
-          int64_t r = tl.row0 + et;
-          if (p.row_index != nullptr) {
-            const int v = __ldg(p.row_index + r);
-            if (v < 0 || v >= p.x_rows) {
-              raise_error(p.err, kDevBadIndex, kSiteRowIndex, static_cast<int>(r), v);
-              r = -1;
-            } else {
-              r = v;
-            }
-          }
-          if (r >= 0) s = __ldg(p.x_scales + r);
-        }
-        sh.x_scale[acc][et] = s;
-      }
+      for (int q = 0; q < 4; ++q) asm("mov.b64 %0, {%1, %1};" : "=l"(ws[q]) : "f"(cur.w[q]));
       if (ok) {
         ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[acc], (local >> 1) & 1));
         if (!ok) raise_error(p.err, kDevWaitTimeout, 86, t, 0);
@@ -421,93 +451,98 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive_pair(pair_leader_addr(&sh.acc_empty[acc]));
       };
       if (way * kUnit >= tl.rows) release();
+      if (t + step < total) next = fetch(t + step);
       for (int j0 = way * kUnit; j0 < tl.rows; j0 += kWays * kUnit) {
-        int a[2][8];  // [16 lanes][the two blocks' four values]
-        tmem_ld_16x16(taddr + j0, a[0]);
-        tmem_ld_16x16(taddr + (16u << 16) + j0, a[1]);
+        int a[2][16];  // [16 lanes][the four blocks' four values]
+        tmem_ld_16x32(taddr + j0, a[0]);
+        tmem_ld_16x32(taddr + (16u << 16) + j0, a[1]);
         const int64_t row = tl.row0 + j0;
         const int nr = tl.rows - j0;
-        Block r[2];
-        if (!kGated && p.residual != nullptr) {
-          const T* res = static_cast<const T*>(p.residual) + (row + tc) * p.ldr + c;
-          load_block(r[0], res, p.ldr, nr - tc, nc);
-          load_block(r[1], res + 8 * p.ldr, p.ldr, nr - tc - 8, nc);
-        }
         tmem_ld_wait(a[0], a[1]);
         if (j0 + kWays * kUnit >= tl.rows) release();
-        Block v[2];
+        buf ^= 1;
+        const bool whole = nr >= kUnit && c0 + 32 <= p.n;
+        Block v[4];
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
+        for (int b = 0; b < 4; ++b) {
           const uint64_t s = *reinterpret_cast<const uint64_t*>(&sh.x_scale[acc][j0 + 8 * b + tc]);
 #pragma unroll
           for (int q = 0; q < 4; ++q)
             scale_pair(a[q >> 1][4 * b + 2 * (q & 1)], a[q >> 1][4 * b + 2 * (q & 1) + 1], s, ws[q], v[b][2 * q],
                        v[b][2 * q + 1]);
         }
-        buf ^= 1;
+        // Blocks first .. first + kOut - 1 of the unit are this warp's to store.
+        constexpr int kOut = kGated ? 2 : 4;
+        int first = 0;
         if (kGated) {
-          // The gate's warp finishes the unit's first block, the up's warp the second.
+          // The gate's warp finishes the unit's first two blocks, the up's warp the others.
+          first = gate ? 0 : 2;
           float4* give = xch + buf * (kXchBytes / 16);
           const float4* take = xch_other + buf * (kXchBytes / 16);
-          Block g, o;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) o[i] = gate ? v[1][i] : v[0][i];
-          give[lane] = make_float4(o[0], o[1], o[2], o[3]);
-          give[32 + lane] = make_float4(o[4], o[5], o[6], o[7]);
-          named_bar_sync(2 + (quarter & 1) + 2 * way, 64);
-          const float4 t0 = take[lane], t1 = take[32 + lane];
-          const float w[8] = {t0.x, t0.y, t0.z, t0.w, t1.x, t1.y, t1.z, t1.w};
+          for (int b = 0; b < 2; ++b)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            g[i] = gate ? v[0][i] : w[i];
-            o[i] = silu_mul(g[i], gate ? w[i] : v[1][i]);
-          }
-          const int skip = gate ? 0 : 8;
-          if (kBf16 && args.tma_store && nr >= skip + 8) {
-            unsigned char* out = stg + buf * (kOutBytes / 2);
-            if (elect_one()) bulk_wait_read<1>();  // the store before the last has read this buffer
-            __syncwarp();
-            stage_block(o, out, 0, lane);
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (elect_one()) {
-              if (c0 < p.n) tma_store_2d(&args.y, static_cast<int>(c0), static_cast<int>(row) + skip, out);
-              bulk_commit();
+            for (int h = 0; h < 2; ++h) {
+              const Block& o = gate ? v[2 + b] : v[b];
+              give[(2 * b + h) * 32 + lane] = make_float4(o[4 * h], o[4 * h + 1], o[4 * h + 2], o[4 * h + 3]);
             }
-          } else {
-            store_block(o, y + (row + skip + tc) * p.ldy + c, p.ldy, nr - skip - tc, nc);
+          named_bar_sync(2 + (quarter & 1) + 2 * way, 64);
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float4 w4 = take[(2 * b + h) * 32 + lane];
+              const float w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float own = gate ? v[b][4 * h + i] : v[2 + b][4 * h + i];
+                v[b][4 * h + i] = silu_mul(gate ? own : w[i], gate ? w[i] : own);
+              }
+            }
+        } else {
+          if (has_bias) {
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+#pragma unroll
+              for (int i = 0; i < 8; ++i) v[b][i] += cur.bias[i / 2];
+          }
+          if (has_residual) {
+            const T* res = static_cast<const T*>(p.residual) + (row + tc) * p.ldr + c;
+            Block r[4];
+            if (whole) {
+#pragma unroll
+              for (int b = 0; b < 4; ++b) load_block(r[b], res + 8 * b * p.ldr, p.ldr);
+            } else {
+#pragma unroll
+              for (int b = 0; b < 4; ++b) load_block(r[b], res + 8 * b * p.ldr, p.ldr, nr - tc - 8 * b, nc);
+            }
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+#pragma unroll
+              for (int i = 0; i < 8; ++i) v[b][i] += r[b][i];
+          }
+        }
+        if (kBf16 && args.tma_store && nr >= 8 * (first + kOut)) {
+          unsigned char* out = stg + buf * (kOut * 8 * 64);
+          if (elect_one()) bulk_wait_read<1>();  // the store before the last has read this buffer
+          __syncwarp();
+#pragma unroll
+          for (int b = 0; b < kOut; ++b) stage_block(v[b], out, b, lane);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (elect_one()) {
+            if (c0 < p.n) tma_store_2d(&args.y, static_cast<int>(c0), static_cast<int>(row) + 8 * first, out);
+            bulk_commit();
           }
         } else {
-          if (p.bias != nullptr) {
+          T* dst = y + (row + 8 * first + tc) * p.ldy + c;
+          if (whole) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              v[0][i] += bias[i / 2];
-              v[1][i] += bias[i / 2];
-            }
-          }
-          if (p.residual != nullptr) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              v[0][i] += r[0][i];
-              v[1][i] += r[1][i];
-            }
-          }
-          if (kBf16 && args.tma_store && nr >= kUnit) {
-            unsigned char* out = stg + buf * kOutBytes;
-            if (elect_one()) bulk_wait_read<1>();
-            __syncwarp();
-            stage_block(v[0], out, 0, lane);
-            stage_block(v[1], out, 1, lane);
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (elect_one()) {
-              if (c0 < p.n) tma_store_2d(&args.y, static_cast<int>(c0), static_cast<int>(row), out);
-              bulk_commit();
-            }
+            for (int b = 0; b < kOut; ++b) store_block(v[b], dst + 8 * b * p.ldy, p.ldy);
           } else {
-            T* dst = y + (row + tc) * p.ldy + c;
-            store_block(v[0], dst, p.ldy, nr - tc, nc);
-            store_block(v[1], dst + 8 * p.ldy, p.ldy, nr - tc - 8, nc);
+#pragma unroll
+            for (int b = 0; b < kOut; ++b)
+              store_block(v[b], dst + 8 * b * p.ldy, p.ldy, nr - tc - 8 * (first + b), nc);
           }
         }
       }
