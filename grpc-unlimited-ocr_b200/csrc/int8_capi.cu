@@ -99,6 +99,19 @@ int uocr_linear_w8a8(const uocr_linear_w8a8_args* a, void* stream) {
   return done(op, st != cudaSuccess ? st : launch_w8a8(p, static_cast<cudaStream_t>(stream)));
 }
 
+int uocr_grouped_w8a8_workspace(const uocr_grouped_w8a8_args* a, int64_t* bytes) {
+  const char* op = "grouped_w8a8_workspace";
+  if (a == nullptr || bytes == nullptr) return bad(op, "null arguments");
+  if (a->rows < 0 || a->k <= 0 || a->rows > kMaxRows || a->k > UOCR_W8A8_MAX_K) return bad(op, "bad shape");
+  W8a8 p{};
+  p.row_index = a->row_index;
+  p.rows = a->rows;
+  p.groups = a->groups;
+  p.k = a->k;
+  *bytes = static_cast<int64_t>(w8a8_workspace_bytes(p));
+  return UOCR_OK;
+}
+
 int uocr_grouped_linear_w8a8(const uocr_grouped_w8a8_args* a, void* stream) {
   const char* op = "grouped_linear_w8a8";
   if (a == nullptr) return bad(op, "null arguments");
@@ -134,6 +147,11 @@ int uocr_grouped_linear_w8a8(const uocr_grouped_w8a8_args* a, void* stream) {
   p.ldw = a->ldw;
   p.ldy = a->ldy;
   p.y_bf16 = a->y_dtype == UOCR_DTYPE_BF16;
+  p.workspace = static_cast<int8_t*>(a->workspace);
+  const size_t need = w8a8_workspace_bytes(p);
+  if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < static_cast<int64_t>(need) ||
+                   reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0))
+    return bad(op, "the workspace is missing, too small or not 16-byte aligned (uocr_grouped_w8a8_workspace)");
   const cudaError_t st = ops_error_word(&p.err);
   return done(op, st != cudaSuccess ? st : launch_w8a8(p, static_cast<cudaStream_t>(stream)));
 }

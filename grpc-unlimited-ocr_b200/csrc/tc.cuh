@@ -75,16 +75,6 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* m
       : "memory");
 }
 
-// Four rows r0..r3 at column c0 (a map with a box of one row), one after another at dst.
-__device__ __forceinline__ void tma_gather4_pair(void* dst, const CUtensorMap* map, int c0, int r0, int r1, int r2,
-                                                 int r3, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], "
-      "[%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_addr(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(bar)
-      : "memory");
-}
-
 // One arrival on the leader's mbarrier `bar` (a pair_leader_addr) from either
 // CTA. Release at CTA scope: what it announces is that TMEM has been read
 // (tcgen05.wait::ld, tcgen05.fence); a release at cluster scope would first

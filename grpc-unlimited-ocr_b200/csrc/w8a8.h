@@ -36,8 +36,11 @@ struct W8a8 {
   void* y;
   int64_t ldx, ldw, ldr, ldy;
   bool y_bf16;
+  int8_t* workspace;     // w8a8_workspace_bytes, 16-byte aligned
   ErrorWord* err;
 };
+// Device memory the product needs for its duration (rows that row_index names, copied together).
+size_t w8a8_workspace_bytes(const W8a8& p);
 cudaError_t launch_w8a8(const W8a8& p, cudaStream_t stream);
 
 }  // namespace uocr_b200

@@ -10,16 +10,20 @@
 // channels, 64 and 64 in each SM.
 //
 // One persistent pair of blocks per two SMs, warp-specialised:
-//   warps 0, 2, 3  producers, one lane each, per 128-byte slice of K: warp 0
-//              the CTA's 128 weight rows, warp 2 its half of the token rows
-//              (boxes of 128, 64 or 16 rows), or warps 2 and 3 four indexed
-//              rows at a time (gather4);
+//   warps 0, 2  producers, one lane each, per 128-byte slice of K: warp 0 the
+//              CTA's 128 weight rows, warp 2 its half of the token rows (boxes
+//              of 128, 64 or 16 rows);
 //   warp 1     allocates TMEM; in the leader one lane issues the MMAs;
 //   warps 4-11 epilogue, 32 tokens x 32 weight rows at a time: the scales,
 //              then bf16 tiles are transposed into shared memory (stmatrix) and
 //              leave as bulk tensor stores, fp32 ones as sectors of 8 channels.
 //              When gated, the gate's warp and the up's warp of the same
 //              channels exchange half of their tokens first.
+// Rows named by an index are first copied together (gather_rows_kernel): TMA
+// gathers four rows of 128 bytes at a time, 44 clocks each, against 512 clocks
+// of MMAs for 32 of them (1108 us at eight pages' gate/up, 649 us without the
+// index), and loads by threads have to be announced across the pair by a
+// release at cluster scope, which takes longer still (1277 us).
 // The operands' copies into shared memory and the MMAs' reads of it take
 // nearly all of its bandwidth (64 + 64 bytes a clock at the full MMA rate), and
 // every store and shared-memory access of the epilogue takes a clock of the
@@ -58,7 +62,7 @@ constexpr int kBand = 8;               // token tiles of a band (decode_tile)
 
 struct Args {
   CUtensorMap y;                         // boxes of a unit's tokens (gated: half) x 32 channels; unset unless tma_store
-  CUtensorMap x, x_wide, x_half, w, up;  // token boxes of 16 rows (gather: 1), 64 and 128; weight boxes of 128 (gated: 64)
+  CUtensorMap x, x_wide, x_half, w, up;  // token boxes of 16, 64 and 128 rows; weight boxes of 128 (gated: 64)
   W8a8 p;
   int tokens_per_tile;  // at most kMaxN, a multiple of 32
   int channels;         // output channels per tile of a pair
@@ -71,7 +75,6 @@ struct Shared {
   uint64_t acc_full[2], acc_empty[2];
   uint64_t drain;
   uint32_t tmem;
-  alignas(16) int index[2][kMaxN / 4];  // gathered rows of a token producer's part of a tile
   int failed[2];  // an epilogue warp's wait for this accumulator ran out
   alignas(16) float x_scale[2][kMaxN];
   int tile_start[kMaxGroups + 1];
@@ -276,31 +279,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       if (!ok) wait_for_copies();
     }
-  } else if (warp == 2 || warp == 3) {
-    // ---- token producers: one lane each; warp 3 takes half of the rows when they are gathered ----
-    const bool gather = p.row_index != nullptr;
-    const uint32_t full0 = pair_leader_addr(&sh.full[0]);
-    int* idx = sh.index[warp - 2];
-    int stage = 0;  // of the elected lane (elect.sync names the same one every time)
-    uint32_t phase = 0;
-    bool ok = gather || warp == 2;
-    for (int t = blockIdx.x / 2; t < total && ok; t += step) {
-      const Tile tl = decode_tile(t, sh, groups, args);
-      const int half = round32(tl.rows) / 2;
-      const int row = tl.row0 + rank * half;  // this CTA's first token row
-      const int part = gather ? half / 2 : half;
-      const int skip = gather ? (warp - 2) * part : 0;
-      if (gather) {
-        // This warp's rows; those past the tile or outside x read row 0 (never stored, or scaled by zero).
-        __syncwarp();
-        for (int i = lane; i < part; i += 32) {
-          const int j = rank * half + skip + i;
-          const int v = j < tl.rows ? __ldg(p.row_index + tl.row0 + j) : 0;
-          idx[i] = v < 0 || v >= p.x_rows ? 0 : v;
-        }
-        __syncwarp();
-      }
-      if (elect_one()) {
+  } else if (warp == 2) {
+    // ---- token producer: one lane ----
+    if (elect_one()) {
+      const uint32_t full0 = pair_leader_addr(&sh.full[0]);
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = blockIdx.x / 2; t < total && ok; t += step) {
+        const Tile tl = decode_tile(t, sh, groups, args);
+        const int half = round32(tl.rows) / 2;
+        const int row = tl.row0 + rank * half;  // this CTA's first token row
         for (int kb = 0; kb < args.k_blocks; ++kb) {
           if (!mbar_wait(&sh.empty[stage], phase ^ 1)) {
             raise_error(p.err, kDevWaitTimeout, 87, t, kb);
@@ -309,13 +298,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           }
           unsigned char* sb = smem + stage * kStageBytes + kABytes;
           const uint32_t bar = full0 + stage * 8;
-          if (gather) {
-#pragma unroll 4
-            for (int i = 0; i < part; i += 4) {
-              const int4 r = *reinterpret_cast<const int4*>(idx + i);
-              tma_gather4_pair(sb + (skip + i) * kBK, &args.x, kb * kBK, r.x, r.y, r.z, r.w, bar);
-            }
-          } else if (half == kMaxN / 2) {
+          if (half == kMaxN / 2) {
             tma_load_2d_pair(sb, &args.x_half, kb * kBK, row, bar);
           } else {
             int i = 0;
@@ -330,9 +313,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             phase ^= 1;
           }
         }
-        if (!ok) wait_for_copies();
       }
-      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) wait_for_copies();
     }
   } else if (warp == 1) {
     if (rank == 0 && elect_one()) {
@@ -621,15 +603,50 @@ int choose_tokens(int64_t rows, int64_t groups, int c_tiles, int pairs) {
   return best;
 }
 
+// The rows that row_index names, one after another at a pitch of `chunks` 16-byte
+// pieces; zeros where x has no such row. A warp a row, four pieces of it in
+// flight a lane.
+__global__ void __launch_bounds__(256) gather_rows_kernel(const int8_t* __restrict__ x, int64_t ldx, int64_t x_rows,
+                                                          const int* __restrict__ row_index, int rows, int chunks,
+                                                          uint4* __restrict__ out) {
+  const int lane = threadIdx.x & 31, warps = gridDim.x * (blockDim.x / 32);
+  for (int r = blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5); r < rows; r += warps) {
+    const int64_t src = __ldg(row_index + r);
+    const bool in = src >= 0 && src < x_rows;
+    const uint4* from = reinterpret_cast<const uint4*>(x + (in ? src : 0) * ldx);
+    uint4* to = out + static_cast<int64_t>(r) * chunks;
+    for (int c0 = lane; c0 < chunks; c0 += 128) {
+      uint4 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        v[u] = in && c0 + 32 * u < chunks ? __ldg(from + c0 + 32 * u) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (c0 + 32 * u < chunks) to[c0 + 32 * u] = v[u];
+    }
+  }
+}
+
 template <bool kGated, bool kBf16>
 cudaError_t launch(const W8a8& p, cudaStream_t stream) {
   int pairs = 0;
   cudaError_t st = resident_pairs<kGated, kBf16>(&pairs);
   if (st != cudaSuccess) return st;
+  const int8_t* x = p.x;
+  int64_t ldx = p.ldx;
+  if (p.row_index != nullptr) {
+    ldx = (p.k + 15) / 16 * 16;
+    const int64_t blocks = (p.rows + 7) / 8, most = static_cast<int64_t>(pairs) * 2 * 8;
+    gather_rows_kernel<<<static_cast<unsigned>(blocks < most ? blocks : most), 256, 0, stream>>>(
+        p.x, p.ldx, p.x_rows, p.row_index, static_cast<int>(p.rows), static_cast<int>(ldx / 16),
+        reinterpret_cast<uint4*>(p.workspace));
+    if ((st = cudaGetLastError()) != cudaSuccess) return st;
+    x = p.workspace;
+  }
   Args a{};
-  const bool ok = make_int8_tmap(&a.x, p.x, p.x_rows, p.k, p.ldx, p.row_index != nullptr ? 1 : kBoxRows) &&
-                  make_int8_tmap(&a.x_wide, p.x, p.x_rows, p.k, p.ldx, 64) &&
-                  make_int8_tmap(&a.x_half, p.x, p.x_rows, p.k, p.ldx, kMaxN / 2) &&
+  const bool ok = make_int8_tmap(&a.x, x, p.rows, p.k, ldx, kBoxRows) &&
+                  make_int8_tmap(&a.x_wide, x, p.rows, p.k, ldx, 64) &&
+                  make_int8_tmap(&a.x_half, x, p.rows, p.k, ldx, kMaxN / 2) &&
                   make_int8_tmap(&a.w, p.w, p.groups * p.n, p.k, p.ldw, kGated ? kBM / 2 : kBM) &&
                   (!kGated || make_int8_tmap(&a.up, p.w_up, p.groups * p.n, p.k, p.ldw, kBM / 2));
   if (!ok) return cudaErrorInvalidValue;
@@ -649,6 +666,10 @@ cudaError_t launch(const W8a8& p, cudaStream_t stream) {
 }
 
 }  // namespace
+
+size_t w8a8_workspace_bytes(const W8a8& p) {
+  return p.row_index != nullptr ? static_cast<size_t>(p.rows) * static_cast<size_t>((p.k + 15) / 16 * 16) : 0;
+}
 
 cudaError_t launch_w8a8(const W8a8& p, cudaStream_t stream) {
   if (p.rows == 0 || p.n == 0) return cudaSuccess;

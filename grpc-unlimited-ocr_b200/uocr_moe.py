@@ -40,7 +40,7 @@ DECODER_EXPORTS = [
 ]
 
 # Every symbol include/uocr_int8.h declares.
-INT8_EXPORTS = ["uocr_quantize_tokens", "uocr_linear_w8a8", "uocr_grouped_linear_w8a8"]
+INT8_EXPORTS = ["uocr_quantize_tokens", "uocr_linear_w8a8", "uocr_grouped_w8a8_workspace", "uocr_grouped_linear_w8a8"]
 
 # Every symbol include/uocr_moe.h declares.
 EXPORTS = [
@@ -125,7 +125,8 @@ class GroupedW8A8Args(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in ("x", "x_scales", "row_index", "offsets", "w", "w_scales", "w_up",
                                                "w_up_scales", "y")] + [
         (n, ctypes.c_int64) for n in ("rows", "x_rows", "groups", "n", "k", "ldx", "ldw", "ldy")] + [
-        ("y_dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+        ("y_dtype", ctypes.c_int32), ("reserved", ctypes.c_int32), ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64)]
 
 
 def lib() -> ctypes.CDLL:
@@ -177,6 +178,7 @@ def lib() -> ctypes.CDLL:
         L.uocr_decoder_profile_decode.argtypes = [vp, i64, ctypes.POINTER(f32), vp]
         L.uocr_quantize_tokens.argtypes = [vp, i32, i64, i64, i64, vp, i64, vp, vp]
         L.uocr_linear_w8a8.argtypes = [ctypes.POINTER(LinearW8A8Args), vp]
+        L.uocr_grouped_w8a8_workspace.argtypes = [ctypes.POINTER(GroupedW8A8Args), ctypes.POINTER(i64)]
         L.uocr_grouped_linear_w8a8.argtypes = [ctypes.POINTER(GroupedW8A8Args), vp]
         _lib = L
     return _lib
@@ -508,7 +510,8 @@ def grouped_linear_w8a8(x, x_scales, w, w_scales, offsets, y, row_index=None, w_
                         stream=None):
     """Group g's rows offsets[g] .. offsets[g + 1] - 1 of y [rows, n] = x[row_index[r]] . w[g]^T in int8, or with
     w_up silu(x . w[g]^T) * (x . w_up[g]^T) (uocr_grouped_linear_w8a8). w, w_up: [groups, n, k] or the stack
-    [groups * n, k]; w_scales: groups * n values; offsets, row_index: int32."""
+    [groups * n, k]; w_scales: groups * n values; offsets, row_index: int32. Where the call needs a workspace it
+    comes from torch's allocator."""
     import torch
     (x_rows, k), (rows, n), groups = x.shape, y.shape, offsets.numel() - 1
 
@@ -528,7 +531,15 @@ def grouped_linear_w8a8(x, x_scales, w, w_scales, offsets, y, row_index=None, w_
         _vector(offsets, "offsets", groups + 1, torch.int32), w.data_ptr(),
         _vector(w_scales, "w_scales", groups * n, torch.float32), _ptr(w_up),
         None if w_up is None else _vector(w_up_scales, "w_up_scales", groups * n, torch.float32), y.data_ptr(), rows,
-        x_rows, groups, n, k, _int8(x, "x", (x_rows, k)), ldw, _rows(y, "y", (rows, n)), _float_dtype(y, "y"), 0)
+        x_rows, groups, n, k, _int8(x, "x", (x_rows, k)), ldw, _rows(y, "y", (rows, n)), _float_dtype(y, "y"), 0, None, 0)
+    if row_index is not None:
+        need = ctypes.c_int64()
+        _check(lib().uocr_grouped_w8a8_workspace(ctypes.byref(args), ctypes.byref(need)))
+        if need.value > 0:
+            workspace = torch.empty(need.value, dtype=torch.uint8, device=y.device)
+            if stream is not None:  # the allocator may hand it out again only when that stream is done with it
+                workspace.record_stream(torch.cuda.ExternalStream(stream) if isinstance(stream, int) else stream)
+            args.workspace, args.workspace_bytes = workspace.data_ptr(), need.value
     _check(lib().uocr_grouped_linear_w8a8(ctypes.byref(args), _stream(stream)))
 
 

@@ -74,7 +74,14 @@ typedef struct uocr_grouped_w8a8_args {
   int64_t ldx, ldw, ldy;
   int32_t y_dtype;          /* UOCR_DTYPE_F32 or UOCR_DTYPE_BF16 */
   int32_t reserved;         /* 0 */
+  void* workspace;          /* device memory for the call's duration, 16-byte aligned; NULL when none is needed */
+  int64_t workspace_bytes;  /* at least what uocr_grouped_w8a8_workspace says */
 } uocr_grouped_w8a8_args;
+
+/* Bytes of workspace the call below needs with these sizes (row_index given,
+ * many rows: the rows it names, copied together; else 0). Only the sizes and
+ * whether row_index is NULL are looked at. */
+int uocr_grouped_w8a8_workspace(const uocr_grouped_w8a8_args* args, int64_t* bytes);
 
 /* Each group of rows with its own matrix: y[r] = x[row_index[r]] w[g]^T, scaled
  * as above; with w_up the gated form silu(x w[g]^T) * (x w_up[g]^T)

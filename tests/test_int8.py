@@ -86,7 +86,8 @@ def test_linear_w8a8_of_no_rows_or_columns():
 
 def _grouped(**kw):
     a = dict(x=BASE, x_scales=BASE, row_index=None, offsets=BASE, w=BASE, w_scales=BASE, w_up=None, w_up_scales=None,
-             y=BASE, rows=8, x_rows=8, groups=4, n=32, k=64, ldx=64, ldw=64, ldy=32, y_dtype=1, reserved=0)
+             y=BASE, rows=8, x_rows=8, groups=4, n=32, k=64, ldx=64, ldw=64, ldy=32, y_dtype=1, reserved=0,
+             workspace=None, workspace_bytes=0)
     a.update(kw)
     return M.lib().uocr_grouped_linear_w8a8(ctypes.byref(M.GroupedW8A8Args(**a)), None)
 
@@ -96,6 +97,8 @@ def _grouped(**kw):
     (dict(k=1 << 18), 2), (dict(y_dtype=3), 1), (dict(reserved=1), 1), (dict(offsets=None), 1), (dict(x=None), 1),
     (dict(x_scales=None), 1), (dict(w=None), 1), (dict(w_scales=None), 1), (dict(y=None), 1), (dict(x_rows=7), 1),
     (dict(x_rows=0, row_index=BASE), 1), (dict(w_up=BASE), 1), (dict(w_up=BASE + 8, w_up_scales=BASE), 1),
+    (dict(rows=4096, row_index=BASE), 1), (dict(rows=4096, row_index=BASE, workspace=BASE, workspace_bytes=64), 1),
+    (dict(rows=4096, row_index=BASE, workspace=BASE + 8, workspace_bytes=1 << 30), 1),
     (dict(ldx=63), 1), (dict(ldw=65), 1), (dict(ldy=16), 1), (dict(x=BASE + 1), 1)])
 def test_grouped_linear_w8a8_refuses(wrong, code):
     assert _grouped(**wrong) == code
@@ -107,6 +110,19 @@ def test_grouped_linear_w8a8_of_nothing():
     assert _grouped(n=0, w=None, y=None) == 0
     assert _grouped(groups=0) == 0
     assert M.lib().uocr_grouped_linear_w8a8(None, None) == 1
+
+
+def test_grouped_w8a8_workspace():
+    need = ctypes.c_int64(-1)
+
+    def ask(**kw):
+        a = dict(rows=4096, k=100, row_index=BASE, groups=4)
+        a.update(kw)
+        return M.lib().uocr_grouped_w8a8_workspace(ctypes.byref(M.GroupedW8A8Args(**a)), ctypes.byref(need))
+    assert ask() == 0 and need.value == 4096 * 112
+    assert ask(row_index=None) == 0 and need.value == 0
+    assert ask(k=0) == 1 and ask(rows=-1) == 1 and ask(k=1 << 20) == 1
+    assert M.lib().uocr_grouped_w8a8_workspace(None, None) == 1
 
 
 def test_binding_refuses_wrong_tensors():
