@@ -53,7 +53,7 @@ extern "C" {
 int uocr_quantize_tokens(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t ldx, int8_t* q,
                          int64_t ldq, float* scales, void* stream) {
   const char* op = "quantize_tokens";
-  if (rows < 0 || cols < 0 || rows > kMaxRows) return bad(op, "bad shape");
+  if (rows < 0 || cols < 0 || rows > kMaxRows || cols > kMaxRows) return bad(op, "bad shape");
   if (dtype != UOCR_DTYPE_F32 && dtype != UOCR_DTYPE_BF16) return bad(op, "x must be f32 or bf16");
   if (rows == 0) return UOCR_OK;
   if (scales == nullptr || (cols > 0 && (x == nullptr || q == nullptr))) return bad(op, "null pointer");
@@ -103,12 +103,7 @@ int uocr_grouped_w8a8_workspace(const uocr_grouped_w8a8_args* a, int64_t* bytes)
   const char* op = "grouped_w8a8_workspace";
   if (a == nullptr || bytes == nullptr) return bad(op, "null arguments");
   if (a->rows < 0 || a->k <= 0 || a->rows > kMaxRows || a->k > UOCR_W8A8_MAX_K) return bad(op, "bad shape");
-  W8a8 p{};
-  p.row_index = a->row_index;
-  p.rows = a->rows;
-  p.groups = a->groups;
-  p.k = a->k;
-  *bytes = static_cast<int64_t>(w8a8_workspace_bytes(p));
+  *bytes = a->row_index == nullptr ? 0 : static_cast<int64_t>(w8a8_gather_bytes(a->rows, a->groups, a->k));
   return UOCR_OK;
 }
 
@@ -148,7 +143,7 @@ int uocr_grouped_linear_w8a8(const uocr_grouped_w8a8_args* a, void* stream) {
   p.ldy = a->ldy;
   p.y_bf16 = a->y_dtype == UOCR_DTYPE_BF16;
   p.workspace = static_cast<int8_t*>(a->workspace);
-  const size_t need = w8a8_workspace_bytes(p);
+  const size_t need = a->row_index == nullptr ? 0 : w8a8_gather_bytes(a->rows, a->groups, a->k);
   if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < static_cast<int64_t>(need) ||
                    reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0))
     return bad(op, "the workspace is missing, too small or not 16-byte aligned (uocr_grouped_w8a8_workspace)");

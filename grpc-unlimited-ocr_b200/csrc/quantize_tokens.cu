@@ -1,10 +1,10 @@
 // Activations to int8 with one scale per token (include/uocr_int8.h).
 //
-// s = max|x| * fl(1 / 127), q = clamp(rint(x / s), +-127) with an IEEE division,
-// so the bits do not depend on the variant below. (quantize_rows_kernel in
+// s = max|x| * fl(1 / 127), q = rint(x / s) with the quotient as an IEEE
+// division rounds it, whatever the variant below. (quantize_rows_kernel in
 // weights.cu divides the maximum by 127: its s may differ in the last bit.)
-// One pass: a thread keeps its part of the row in registers between the
-// maximum and the rounding.
+// |x| / s is at most 127 (1 + 2^-22), so nothing is clamped. One pass: a thread
+// keeps its part of the row in registers between the maximum and the rounding.
 #include <cfloat>
 
 #include "w8a8.h"
@@ -14,10 +14,9 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kChunk = 8;   // elements a thread takes at a time
-constexpr int kKeep = 8;    // chunks of a row a thread keeps
 
 // Elements c .. c + 7 of a row; `vec`: the row is 16-byte aligned and holds all eight.
-__device__ __forceinline__ void load8(const float* row, int64_t c, int64_t cols, bool vec, float (&v)[kChunk]) {
+__device__ __forceinline__ void load8(const float* row, int c, int cols, bool vec, float (&v)[kChunk]) {
   if (vec) {
     const float4 a = *reinterpret_cast<const float4*>(row + c), b = *reinterpret_cast<const float4*>(row + c + 4);
     v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
@@ -27,8 +26,7 @@ __device__ __forceinline__ void load8(const float* row, int64_t c, int64_t cols,
 #pragma unroll
   for (int i = 0; i < kChunk; ++i) v[i] = c + i < cols ? row[c + i] : 0.0f;
 }
-__device__ __forceinline__ void load8(const __nv_bfloat16* row, int64_t c, int64_t cols, bool vec,
-                                      float (&v)[kChunk]) {
+__device__ __forceinline__ void load8(const __nv_bfloat16* row, int c, int cols, bool vec, float (&v)[kChunk]) {
   if (vec) {
     const uint4 a = *reinterpret_cast<const uint4*>(row + c);
     const uint32_t w[4] = {a.x, a.y, a.z, a.w};
@@ -51,16 +49,54 @@ __device__ __forceinline__ uint32_t peak8(const float (&v)[kChunk], uint32_t pea
   return peak;
 }
 
-__device__ __forceinline__ void store8(const float (&v)[kChunk], float scale, bool finite, int8_t* row, int64_t c,
-                                       int64_t cols) {
-  uint32_t w[2] = {0u, 0u};
-  if (finite) {
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+
+struct RowScale {
+  float scale;
+  uint64_t inv2, minus2;  // 1 / scale and -scale, twice
+  bool finite, tiny;
+};
+
+// rint(v / scale) of eight elements to bytes. The quotient by Markstein's
+// method: with y = RN(1 / s), q <- RN(q + RN(v - q s) y) from q = RN(v y) is
+// within an ulp of v / s after one step and RN(v / s) after two, in packed
+// products (an IEEE division and a conversion for each element made the kernel
+// three times slower). Adding 1.5 * 2^23 rounds to an integer, the low byte of
+// the sum. Rows below 2^-90, where a remainder could underflow, are divided.
+__device__ __forceinline__ void store8(const float (&v)[kChunk], const RowScale& s, int8_t* row, int c, int cols) {
+  constexpr float kRound = 12582912.0f;
+  const uint64_t zero2 = 0, round2 = pair(kRound, kRound), one2 = pair(1.0f, 1.0f);
+  uint32_t r[kChunk];
+  if (s.tiny) {
 #pragma unroll
-    for (int i = 0; i < kChunk; ++i) {
-      const float r = fminf(fmaxf(rintf(v[i] / scale), -127.0f), 127.0f);
-      w[i / 4] |= (static_cast<uint32_t>(static_cast<int>(r)) & 0xffu) << (8 * (i % 4));
+    for (int i = 0; i < kChunk; ++i) r[i] = __float_as_uint(v[i] / s.scale + kRound);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kChunk; i += 2) {
+      const uint64_t x = pair(v[i], v[i + 1]);
+      uint64_t q = fma2(x, s.inv2, zero2);
+      q = fma2(fma2(q, s.minus2, x), s.inv2, q);
+      q = fma2(fma2(q, s.minus2, x), s.inv2, q);
+      const uint64_t b = fma2(q, one2, round2);
+      r[i] = static_cast<uint32_t>(b);
+      r[i + 1] = static_cast<uint32_t>(b >> 32);
     }
   }
+  uint32_t w[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    w[h] = s.finite ? __byte_perm(__byte_perm(r[4 * h], r[4 * h + 1], 0x0040),
+                                  __byte_perm(r[4 * h + 2], r[4 * h + 3], 0x0040), 0x5410)
+                    : 0u;
   if (c + kChunk <= cols) {
     *reinterpret_cast<uint2*>(row + c) = make_uint2(w[0], w[1]);
   } else {
@@ -70,33 +106,34 @@ __device__ __forceinline__ void store8(const float (&v)[kChunk], float scale, bo
   }
 }
 
-// kPerRow threads (32: a warp, or the whole block) take a row; the part of a
-// row beyond kPerRow * kKeep chunks is read a second time.
-template <typename T, int kPerRow>
-__global__ void __launch_bounds__(kThreads) quantize_tokens_kernel(const T* __restrict__ x, int64_t rows, int64_t cols,
-                                                                   int64_t ldx, bool aligned, int8_t* __restrict__ q,
-                                                                   int64_t ldq, float* __restrict__ scales) {
+// kPerRow threads (a warp, several, or the whole block) take a row and keep
+// kKeep chunks of it each; what is beyond is read a second time. kAligned: x's rows
+// start at 16-byte boundaries.
+template <typename T, int kPerRow, int kKeep, bool kAligned>
+__global__ void __launch_bounds__(kThreads) quantize_tokens_kernel(const T* __restrict__ x, int64_t rows, int cols,
+                                                                   int64_t ldx, int8_t* __restrict__ q, int64_t ldq,
+                                                                   float* __restrict__ scales) {
   __shared__ uint32_t part[kThreads / 32];
   const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / kPerRow) + threadIdx.x / kPerRow;
-  if (row >= rows) return;  // whole warps; with kPerRow == kThreads never
-  const int t = threadIdx.x % kPerRow;
+  if (kPerRow <= 32 && row >= rows) return;
+  if (row >= rows) cols = 0;  // goes along to the barrier
+  const int c0 = static_cast<int>(threadIdx.x % kPerRow) * kChunk;
+  constexpr int kStride = kPerRow * kChunk;
   const T* src = x + row * ldx;
   int8_t* dst = q + row * ldq;
   float keep[kKeep][kChunk];
   uint32_t peak = 0u;
 #pragma unroll
   for (int u = 0; u < kKeep; ++u) {
-    const int64_t c = static_cast<int64_t>(t + u * kPerRow) * kChunk;
-    if (c < cols) load8(src, c, cols, aligned && c + kChunk <= cols, keep[u]);
+    const int c = c0 + u * kStride;
+    if (c < cols) load8(src, c, cols, kAligned && c + kChunk <= cols, keep[u]);
   }
 #pragma unroll
-  for (int u = 0; u < kKeep; ++u) {
-    const int64_t c = static_cast<int64_t>(t + u * kPerRow) * kChunk;
-    if (c < cols) peak = peak8(keep[u], peak);
-  }
-  for (int64_t c = static_cast<int64_t>(t + kKeep * kPerRow) * kChunk; c < cols; c += kPerRow * kChunk) {
+  for (int u = 0; u < kKeep; ++u)
+    if (c0 + u * kStride < cols) peak = peak8(keep[u], peak);
+  for (int c = c0 + kKeep * kStride; c < cols; c += kStride) {
     float v[kChunk];
-    load8(src, c, cols, aligned && c + kChunk <= cols, v);
+    load8(src, c, cols, kAligned && c + kChunk <= cols, v);
     peak = peak8(v, peak);
   }
   peak = __reduce_max_sync(0xffffffffu, peak);
@@ -104,39 +141,61 @@ __global__ void __launch_bounds__(kThreads) quantize_tokens_kernel(const T* __re
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = peak;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kPerRow / 32; ++w) peak = max(peak, part[w]);
+    for (int w = 0; w < kPerRow / 32; ++w) peak = max(peak, part[threadIdx.x / kPerRow * (kPerRow / 32) + w]);
+    if (row >= rows) return;
   }
-  const bool finite = peak < 0x7f800000u;
-  const float scale = !finite       ? __uint_as_float(0x7fc00000u)
-                      : peak == 0u  ? 1.0f
-                                    : fmaxf(__uint_as_float(peak) * (1.0f / 127.0f), FLT_MIN);
-  if (t == 0) scales[row] = scale;
+  RowScale s;
+  s.finite = peak < 0x7f800000u;
+  s.scale = !s.finite    ? __uint_as_float(0x7fc00000u)
+            : peak == 0u ? 1.0f
+                         : fmaxf(__uint_as_float(peak) * (1.0f / 127.0f), FLT_MIN);
+  s.tiny = s.scale < 0x1p-90f;
+  s.inv2 = pair(1.0f / s.scale, 1.0f / s.scale);
+  s.minus2 = pair(-s.scale, -s.scale);
+  if (c0 == 0) scales[row] = s.scale;
 #pragma unroll
   for (int u = 0; u < kKeep; ++u) {
-    const int64_t c = static_cast<int64_t>(t + u * kPerRow) * kChunk;
-    if (c < cols) store8(keep[u], scale, finite, dst, c, cols);
+    const int c = c0 + u * kStride;
+    if (c < cols) store8(keep[u], s, dst, c, cols);
   }
-  for (int64_t c = static_cast<int64_t>(t + kKeep * kPerRow) * kChunk; c < cols; c += kPerRow * kChunk) {
+  for (int c = c0 + kKeep * kStride; c < cols; c += kStride) {
     float v[kChunk];
-    load8(src, c, cols, aligned && c + kChunk <= cols, v);
-    store8(v, scale, finite, dst, c, cols);
+    load8(src, c, cols, kAligned && c + kChunk <= cols, v);
+    store8(v, s, dst, c, cols);
   }
 }
 
-template <typename T>
-cudaError_t launch(const T* x, int64_t rows, int64_t cols, int64_t ldx, int8_t* q, int64_t ldq, float* scales,
+template <int kPerRow, int kKeep, bool kAligned, typename T>
+cudaError_t launch(const T* x, int64_t rows, int cols, int64_t ldx, int8_t* q, int64_t ldq, float* scales,
                    cudaStream_t stream) {
-  const bool aligned = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (ldx * sizeof(T)) % 16 == 0;
-  // A warp per row where a warp can keep the row; wider rows take a block.
-  if (cols <= 32 * kKeep * kChunk) {
-    const int64_t blocks = (rows + kThreads / 32 - 1) / (kThreads / 32);
-    quantize_tokens_kernel<T, 32><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(x, rows, cols, ldx, aligned,
-                                                                                          q, ldq, scales);
-  } else {
-    quantize_tokens_kernel<T, kThreads><<<static_cast<unsigned>(rows), kThreads, 0, stream>>>(x, rows, cols, ldx,
-                                                                                              aligned, q, ldq, scales);
-  }
+  constexpr int kRows = kThreads / kPerRow;
+  quantize_tokens_kernel<T, kPerRow, kKeep, kAligned>
+      <<<static_cast<unsigned>((rows + kRows - 1) / kRows), kThreads, 0, stream>>>(x, rows, cols, ldx, q, ldq, scales);
   return cudaGetLastError();
+}
+
+template <bool kAligned, typename T>
+cudaError_t choose(const T* x, int64_t rows, int cols, int64_t ldx, int8_t* q, int64_t ldq, float* scales,
+                   cudaStream_t stream) {
+  // Two chunks a thread: enough in flight, and few idle threads. Measured in us:
+  // 4096 x 2048 bf16 12.3 by a warp a row, 7.5 by 128 threads, 8.1 by 256 of one
+  // chunk (3.85 at the card's copy rate); 24576 x 1024 bf16 27 by a warp, 23 by
+  // 64 threads; 32768 x 2048 fp32 49.5 by 128 threads (the copy rate: 51). Few
+  // rows are a matter of latency: 1 x 2048 1.6 by 256 threads, 5.5 by a warp.
+  if (cols <= 512) return launch<32, 2, kAligned>(x, rows, cols, ldx, q, ldq, scales, stream);
+  if (cols <= 2048 && rows <= 592) return launch<256, 1, kAligned>(x, rows, cols, ldx, q, ldq, scales, stream);
+  if (cols <= 1024) return launch<64, 2, kAligned>(x, rows, cols, ldx, q, ldq, scales, stream);
+  if (cols <= 2048) return launch<128, 2, kAligned>(x, rows, cols, ldx, q, ldq, scales, stream);
+  return launch<256, 4, kAligned>(x, rows, cols, ldx, q, ldq, scales, stream);
+}
+
+template <typename T>
+cudaError_t choose(const void* xv, int64_t rows, int cols, int64_t ldx, int8_t* q, int64_t ldq, float* scales,
+                   cudaStream_t stream) {
+  const T* x = static_cast<const T*>(xv);
+  return reinterpret_cast<uintptr_t>(x) % 16 == 0 && (ldx * sizeof(T)) % 16 == 0
+             ? choose<true>(x, rows, cols, ldx, q, ldq, scales, stream)
+             : choose<false>(x, rows, cols, ldx, q, ldq, scales, stream);
 }
 
 }  // namespace
@@ -144,8 +203,9 @@ cudaError_t launch(const T* x, int64_t rows, int64_t cols, int64_t ldx, int8_t* 
 cudaError_t launch_quantize_tokens(const void* x, bool bf16, int64_t rows, int64_t cols, int64_t ldx, int8_t* q,
                                    int64_t ldq, float* scales, cudaStream_t stream) {
   if (rows == 0) return cudaSuccess;
-  return bf16 ? launch(static_cast<const __nv_bfloat16*>(x), rows, cols, ldx, q, ldq, scales, stream)
-              : launch(static_cast<const float*>(x), rows, cols, ldx, q, ldq, scales, stream);
+  const int n = static_cast<int>(cols);
+  return bf16 ? choose<__nv_bfloat16>(x, rows, n, ldx, q, ldq, scales, stream)
+              : choose<float>(x, rows, n, ldx, q, ldq, scales, stream);
 }
 
 }  // namespace uocr_b200

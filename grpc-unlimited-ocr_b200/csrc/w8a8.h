@@ -1,5 +1,5 @@
 // Host interface of the 8-bit integer operators: the token quantiser
-// (quantize_tokens.cu) and the products (w8a8_gemm.cu).
+// (quantize_tokens.cu) and the products (w8a8_gemm.cu, w8a8_rows.cu).
 #pragma once
 
 #include <cuda_bf16.h>
@@ -36,11 +36,17 @@ struct W8a8 {
   void* y;
   int64_t ldx, ldw, ldr, ldy;
   bool y_bf16;
-  int8_t* workspace;     // w8a8_workspace_bytes, 16-byte aligned
+  int8_t* workspace;     // with row_index: w8a8_gather_bytes, 16-byte aligned
   ErrorWord* err;
 };
-// Device memory the product needs for its duration (rows that row_index names, copied together).
-size_t w8a8_workspace_bytes(const W8a8& p);
+// Device memory a grouped product with row_index needs for its duration: the rows it names, copied together.
+size_t w8a8_gather_bytes(int64_t rows, int64_t groups, int64_t k);
 cudaError_t launch_w8a8(const W8a8& p, cudaStream_t stream);
+// The kernel for few rows (w8a8_rows.cu); launch_w8a8 chooses.
+cudaError_t launch_w8a8_rows(const W8a8& p, cudaStream_t stream);
+
+// silu(g) * u = g / (1 + exp(-g)) * u. The quotient to 2 ulp (__fdividef): an
+// IEEE division branches, which keeps a thread's outputs from overlapping.
+__device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.0f + expf(-g)) * u; }
 
 }  // namespace uocr_b200

@@ -113,11 +113,6 @@ __device__ __forceinline__ Tile decode_tile(int t, const Shared& sh, int groups,
   return Tile{lo, sh.first[lo] + r, min(per, count - r), c * a.channels};
 }
 
-// silu(g) * u = g / (1 + exp(-g)) * u. The quotient to 2 ulp (__fdividef): an
-// IEEE division branches, and 32 of them in a row keep a thread's 32 tokens
-// from overlapping (the gated kernel's time at eight pages: 928 us with it).
-__device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.0f + expf(-g)) * u; }
-
 template <bool kBf16>
 using Out = typename std::conditional<kBf16, __nv_bfloat16, float>::type;
 
@@ -667,12 +662,29 @@ cudaError_t launch(const W8a8& p, cudaStream_t stream) {
 
 }  // namespace
 
-size_t w8a8_workspace_bytes(const W8a8& p) {
-  return p.row_index != nullptr ? static_cast<size_t>(p.rows) * static_cast<size_t>((p.k + 15) / 16 * 16) : 0;
+namespace {
+// Which kernel: w8a8_rows.cu reads the weights once per 8 rows (dense: 16) of a
+// group, with little to set up; the kernel above takes 7.5 us or more. Measured
+// in us, rows against this one: dense 2048 x 2048 1 row 3.1 / 8.2, 16 rows 4.5
+// / 8.2; 8192 x 2048 16 rows 7.8 / 8.3; 16384 x 2048 8 rows 9.4 / 10.4, 16 rows
+// 13.8 / 10.5; 102400 x 2048 1 row 36 / 39. 64 groups of 2 x 1024 x 2048 gated:
+// 6 rows 8.2 / 11.7, 60 rows 38 / 37, 240 rows 47 / 52; of 2048 x 1024: 6 rows
+// 6.3 / 7.9, 96 rows 23 / 24, 240 rows 30 / 28. 16 groups of 1024 x 2048, 128
+// rows: 14.8 / 11.5.
+bool few_rows_grouped(int64_t rows, int64_t groups) { return rows <= 256 && rows <= 4 * groups; }
+bool few_rows(const W8a8& p) {
+  if (p.starts != nullptr) return few_rows_grouped(p.rows, p.groups);
+  return p.rows <= 8 || (p.rows <= 16 && p.n * p.k <= (int64_t{1} << 24));
+}
+}  // namespace
+
+size_t w8a8_gather_bytes(int64_t rows, int64_t groups, int64_t k) {
+  return few_rows_grouped(rows, groups) ? 0 : static_cast<size_t>(rows) * static_cast<size_t>((k + 15) / 16 * 16);
 }
 
 cudaError_t launch_w8a8(const W8a8& p, cudaStream_t stream) {
   if (p.rows == 0 || p.n == 0) return cudaSuccess;
+  if (few_rows(p)) return launch_w8a8_rows(p, stream);
   if (p.w_up != nullptr) return p.y_bf16 ? launch<true, true>(p, stream) : launch<true, false>(p, stream);
   return p.y_bf16 ? launch<false, true>(p, stream) : launch<false, false>(p, stream);
 }
