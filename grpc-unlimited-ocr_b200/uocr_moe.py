@@ -197,10 +197,18 @@ def _ptr(t) -> int | None:
     return t.data_ptr()
 
 
+_raw_stream = None
+
+
 def _stream(stream) -> int | None:
     if stream is None:
+        global _raw_stream
         import torch
-        return torch.cuda.current_stream().cuda_stream
+        if _raw_stream is None:
+            # The handle alone, 3 us cheaper than a Stream object, where this torch has it.
+            _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+                lambda device: torch.cuda.current_stream(device).cuda_stream)
+        return _raw_stream(torch.cuda.current_device())
     return stream if isinstance(stream, int) else stream.cuda_stream
 
 
@@ -455,28 +463,29 @@ def _float_dtype(t, what: str) -> int:
     return dtype
 
 
-def _rows(t, what: str, shape: tuple, pitch_of: int = 1) -> int:
-    """The row pitch of a 2-D device tensor of this shape whose rows are contiguous (a single row's pitch is its
-    width, rounded up to pitch_of)."""
-    if t.shape != shape or not t.is_cuda:
-        raise ValueError(f"{what} must be a {shape} tensor on the GPU, not {tuple(t.shape)} on {t.device}")
-    s0, s1 = t.stride()
-    if s1 != 1 and shape[1] > 1:
+def _pitch(t, what: str, rows: int, cols: int) -> int:
+    """The row pitch of a [rows, cols] device tensor whose rows are contiguous."""
+    if t.shape != (rows, cols) or not t.is_cuda:
+        raise ValueError(f"{what} must be a {(rows, cols)} tensor on the GPU, not {tuple(t.shape)} on {t.device}")
+    pitch, step = t.stride()
+    if step != 1 and cols > 1:
         raise ValueError(f"{what}'s rows must be contiguous")
-    return s0 if shape[0] > 1 else -(-shape[1] // pitch_of) * pitch_of
+    return pitch if rows > 1 else cols
 
 
-def _vector(t, what: str, n: int, dtype):
-    if t.dtype != dtype or t.numel() != n or not t.is_cuda or not t.is_contiguous():
+def _pitch_i8(t, what: str, rows: int, cols: int) -> int:
+    """The same of int8 rows; a single row's pitch is its width rounded up to 16."""
+    import torch
+    if t.dtype is not torch.int8:
+        raise ValueError(f"{what} must be int8, not {t.dtype}")
+    pitch = _pitch(t, what, rows, cols)
+    return pitch if rows > 1 else (pitch + 15) // 16 * 16
+
+
+def _vector(t, what: str, n: int, dtype) -> int:
+    if t.dtype is not dtype or t.numel() != n or not t.is_cuda or not t.is_contiguous():
         raise ValueError(f"{what} must be {n} contiguous {dtype} values on the GPU")
     return t.data_ptr()
-
-
-def _int8(t, what: str, shape: tuple):
-    import torch
-    if t.dtype != torch.int8:
-        raise ValueError(f"{what} must be int8, not {t.dtype}")
-    return _rows(t, what, shape, 16)
 
 
 def quantize_tokens(x, q, scales, stream=None):
@@ -484,26 +493,45 @@ def quantize_tokens(x, q, scales, stream=None):
     (uocr_quantize_tokens)."""
     import torch
     rows, cols = x.shape
-    dtype = _float_dtype(x, "x")
-    _check(lib().uocr_quantize_tokens(x.data_ptr(), dtype, rows, cols, _rows(x, "x", (rows, cols)), q.data_ptr(),
-                                      _int8(q, "q", (rows, cols)), _vector(scales, "scales", rows, torch.float32),
-                                      _stream(stream)))
+    _check(lib().uocr_quantize_tokens(x.data_ptr(), _float_dtype(x, "x"), rows, cols, _pitch(x, "x", rows, cols),
+                                      q.data_ptr(), _pitch_i8(q, "q", rows, cols),
+                                      _vector(scales, "scales", rows, torch.float32), _stream(stream)))
 
 
 def linear_w8a8(x, x_scales, w, w_scales, y, bias=None, residual=None, stream=None):
     """y[m, n] = x[m, k] . w[n, k]^T in int8 with x_scales per row of x and w_scales per row of w (+ bias[n])
     (+ residual[m, n], of y's dtype; may be y itself) (uocr_linear_w8a8)."""
     import torch
-    (m, k), n = x.shape, w.shape[0]
+    f32 = torch.float32
+    m, k = x.shape
+    n = w.shape[0]
+    ldr = res = None
+    if residual is not None:
+        if residual.dtype is not y.dtype:
+            raise ValueError("residual must have y's dtype")
+        res, ldr = residual.data_ptr(), _pitch(residual, "residual", m, n)
     args = LinearW8A8Args(
-        x.data_ptr(), _vector(x_scales, "x_scales", m, torch.float32), w.data_ptr(),
-        _vector(w_scales, "w_scales", n, torch.float32),
-        None if bias is None else _vector(bias, "bias", n, torch.float32), _ptr(residual), y.data_ptr(), m, n, k,
-        _int8(x, "x", (m, k)), _int8(w, "w", (n, k)), 0 if residual is None else _rows(residual, "residual", (m, n)),
-        _rows(y, "y", (m, n)), _float_dtype(y, "y"), 0)
-    if residual is not None and residual.dtype != y.dtype:
-        raise ValueError("residual must have y's dtype")
+        x.data_ptr(), _vector(x_scales, "x_scales", m, f32), w.data_ptr(), _vector(w_scales, "w_scales", n, f32),
+        None if bias is None else _vector(bias, "bias", n, f32), res, y.data_ptr(), m, n, k,
+        _pitch_i8(x, "x", m, k), _pitch_i8(w, "w", n, k), ldr or 0, _pitch(y, "y", m, n), _float_dtype(y, "y"), 0)
     _check(lib().uocr_linear_w8a8(ctypes.byref(args), _stream(stream)))
+
+
+def _stack_pitch(t, what: str, groups: int, n: int, k: int) -> int:
+    """The row pitch of int8 matrices [groups, n, k] that follow one another, or of their stack [groups * n, k]."""
+    import torch
+    if t.dim() != 3:
+        return _pitch_i8(t, what, groups * n, k)
+    if t.shape != (groups, n, k) or t.dtype is not torch.int8 or not t.is_cuda:
+        raise ValueError(f"{what} must be int8 {(groups, n, k)} on the GPU, not {t.dtype} {tuple(t.shape)}")
+    of_group, pitch, step = t.stride()
+    if step != 1 and k > 1:
+        raise ValueError(f"{what}'s rows must be contiguous")
+    if n == 1:
+        pitch = of_group if groups > 1 else (k + 15) // 16 * 16
+    elif groups > 1 and of_group != n * pitch:
+        raise ValueError(f"{what}'s groups must follow one another")
+    return pitch
 
 
 def grouped_linear_w8a8(x, x_scales, w, w_scales, offsets, y, row_index=None, w_up=None, w_up_scales=None,
@@ -513,26 +541,24 @@ def grouped_linear_w8a8(x, x_scales, w, w_scales, offsets, y, row_index=None, w_
     [groups * n, k]; w_scales: groups * n values; offsets, row_index: int32. Where the call needs a workspace it
     comes from torch's allocator."""
     import torch
-    (x_rows, k), (rows, n), groups = x.shape, y.shape, offsets.numel() - 1
-
-    def stack(t, what):
-        if t.dim() == 3:
-            if groups > 1 and n > 1 and t.stride(0) != n * t.stride(1):
-                raise ValueError(f"{what}'s groups must follow one another")
-            t = t.as_strided((t.shape[0] * t.shape[1], t.shape[2]), (t.stride(1) if n > 1 else t.stride(0), t.stride(2)))
-        return _int8(t, what, (groups * n, k))
-
-    ldw = stack(w, "w")
-    if w_up is not None and stack(w_up, "w_up") != ldw:
-        raise ValueError("w_up must have w's pitch")
-    args = GroupedW8A8Args(
-        x.data_ptr(), _vector(x_scales, "x_scales", x_rows, torch.float32),
-        None if row_index is None else _vector(row_index, "row_index", rows, torch.int32),
-        _vector(offsets, "offsets", groups + 1, torch.int32), w.data_ptr(),
-        _vector(w_scales, "w_scales", groups * n, torch.float32), _ptr(w_up),
-        None if w_up is None else _vector(w_up_scales, "w_up_scales", groups * n, torch.float32), y.data_ptr(), rows,
-        x_rows, groups, n, k, _int8(x, "x", (x_rows, k)), ldw, _rows(y, "y", (rows, n)), _float_dtype(y, "y"), 0, None, 0)
+    f32, i32 = torch.float32, torch.int32
+    x_rows, k = x.shape
+    rows, n = y.shape
+    groups = offsets.numel() - 1
+    ldw = _stack_pitch(w, "w", groups, n, k)
+    up = up_scales = index = None
+    if w_up is not None:
+        if _stack_pitch(w_up, "w_up", groups, n, k) != ldw:
+            raise ValueError("w_up must have w's pitch")
+        up, up_scales = w_up.data_ptr(), _vector(w_up_scales, "w_up_scales", groups * n, f32)
     if row_index is not None:
+        index = _vector(row_index, "row_index", rows, i32)
+    args = GroupedW8A8Args(
+        x.data_ptr(), _vector(x_scales, "x_scales", x_rows, f32), index,
+        _vector(offsets, "offsets", groups + 1, i32), w.data_ptr(), _vector(w_scales, "w_scales", groups * n, f32),
+        up, up_scales, y.data_ptr(), rows, x_rows, groups, n, k, _pitch_i8(x, "x", x_rows, k), ldw,
+        _pitch(y, "y", rows, n), _float_dtype(y, "y"), 0, None, 0)
+    if index is not None:
         need = ctypes.c_int64()
         _check(lib().uocr_grouped_w8a8_workspace(ctypes.byref(args), ctypes.byref(need)))
         if need.value > 0:
