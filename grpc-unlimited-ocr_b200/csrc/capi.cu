@@ -22,6 +22,7 @@
 #include "moe_kernels.h"
 #include "plan_internal.h"
 #include "prefill.h"
+#include "w8a8.h"
 
 using namespace uocr_b200;
 
@@ -196,7 +197,7 @@ struct uocr_moe_plan {
     counter = c.take<unsigned>(1);
     err = c.take<ErrorWord>(1);
     if (pre_norm && (prefill || ep)) xnorm = c.take<float>(rows * static_cast<size_t>(d.hidden));
-    if (prefill && d.weight_format == UOCR_WEIGHT_INT8)
+    if (prefill && d.weight_format == UOCR_WEIGHT_INT8 && !pdims.int8_act)
       wexp = c.take<__nv_bfloat16>(3 * static_cast<size_t>(d.routed_experts) * F * d.hidden +
                                    3 * S * static_cast<size_t>(d.hidden));
     if (prefill) {
@@ -278,6 +279,9 @@ int uocr_moe_plan_create(const uocr_moe_desc* desc, uocr_moe_plan** out) {
   const bool pre_norm = (d.flags & UOCR_PLAN_PRE_NORM) != 0;
   if (pre_norm && !(d.rms_norm_eps >= 0.0f && d.rms_norm_eps < 1.0e30f))
     return fail(UOCR_ERR_INVALID_ARGUMENT, "plan_create: rms_norm_eps must be a finite value >= 0");
+  const bool int8_act = (d.flags & UOCR_PLAN_INT8_ACTIVATIONS) != 0;
+  if (int8_act && d.weight_format != UOCR_WEIGHT_INT8)
+    return fail(UOCR_ERR_INVALID_ARGUMENT, "plan_create: int8 activations need int8 weights");
   const bool ep = d.ep_world > 1;
   if (d.ep_world < 0 || d.ep_world > kMaxEpRanks)
     return fail(UOCR_ERR_INVALID_ARGUMENT, "plan_create: ep_world must be in [0, 8]");
@@ -331,7 +335,14 @@ int uocr_moe_plan_create(const uocr_moe_desc* desc, uocr_moe_plan** out) {
                                                     static_cast<int>(d.shared_ffn));
   p->pdims = PrefillDims{static_cast<int>(d.max_rows), static_cast<int>(d.hidden), static_cast<int>(d.routed_experts),
                          static_cast<int>(d.experts_per_token), static_cast<int>(d.expert_ffn),
-                         static_cast<int>(d.shared_ffn), d.renormalize};
+                         static_cast<int>(d.shared_ffn), d.renormalize, int8_act ? 1 : 0};
+  if (int8_act && p->prefill) {
+    const cudaError_t wst = prepare_w8a8();
+    if (wst != cudaSuccess) {
+      delete p;
+      return cuda_fail(wst, "plan_create: kernel set-up");
+    }
+  }
   if (ep) {
     p->ep = true;
     const int W = d.ep_world;
@@ -752,6 +763,17 @@ int run_layer(uocr_moe_plan* p, const LayerDev& L, const float* x, int64_t rows,
                   "forward: more than 16 rows needs the prefill path: hidden % 256 == 0, "
                   "expert_ffn and shared_ffn % 128 == 0");
     PrefillCall c = prefill_call(p, L, x, rows, resid, y);
+    if (p->pdims.int8_act) {
+      auto rows_of = [](const void* q, const float* s, int64_t cols) {
+        return Q8Rows{static_cast<const int8_t*>(q), s, cols};
+      };
+      const Int8Experts w{rows_of(L.gate, L.gate_s, H),   rows_of(L.up, L.up_s, H),   rows_of(L.down, L.down_s, F),
+                          rows_of(L.sgate, L.sgate_s, H), rows_of(L.sup, L.sup_s, H), rows_of(L.sdown, L.sdown_s, S)};
+      c.events = ev;
+      UOCR_TRY(launch_prefill_int8(c, w, stream), "forward: int8 prefill");
+      if (nev != nullptr) *nev = 6;
+      return UOCR_OK;
+    }
     if (d.weight_format == UOCR_WEIGHT_INT8) {
       // The reference's m > 1 int8 path: expand to bf16, then the bf16 GEMMs.
       const int64_t EF = static_cast<int64_t>(E) * F, EH = static_cast<int64_t>(E) * H;

@@ -13,6 +13,7 @@
 #include "moe_kernels.h"
 #include "plan_internal.h"
 #include "tc_gemm.h"
+#include "w8a8.h"
 
 using namespace uocr_b200;
 
@@ -67,6 +68,7 @@ struct uocr_decoder {
   uocr_decoder_desc d{};
   DecShape shape{};
   bool int8 = false;
+  bool int8_act = false;  // the prefill's projections on int8 activations
   int sm_count = 1;
   int splits = 1;        // attention blocks (one cluster) per key/value head
   int attn_mode = 0;     // DecAttnMode of the decode attention
@@ -99,6 +101,8 @@ struct uocr_decoder {
   __nv_bfloat16* qb = nullptr;    // [max_prefill, heads * 128]
   __nv_bfloat16* attn = nullptr;  // [max_prefill, heads * 128]
   __nv_bfloat16* wexp = nullptr;  // int8 prefill: one projection expanded to bf16
+  int8_t* rows_q = nullptr;       // int8 activations: [max_prefill, H] rows in front of a projection
+  float* rows_qs = nullptr;       // [max_prefill]
   ErrorWord* err = nullptr;
   // host mirrors of the sequence
   int64_t length = 0;     // positions in the KV cache
@@ -198,6 +202,32 @@ const __nv_bfloat16* gemm_operand(const uocr_decoder* p, const void* w, const fl
   return p->wexp;
 }
 
+// y [rows, n] fp32 (+= with accumulate) = a [rows, k] (bf16, quantised here) . w
+// [n, k] in int8.
+cudaError_t int8_projection(const uocr_decoder* p, const __nv_bfloat16* a, int64_t rows, int64_t k, const void* w,
+                            const float* w_s, int64_t n, float* y, bool accumulate, cudaStream_t stream) {
+  cudaError_t st = launch_quantize_tokens(a, true, rows, k, k, p->rows_q, k, p->rows_qs, stream);
+  if (st != cudaSuccess) return st;
+  W8a8 g{};
+  g.x = p->rows_q;
+  g.x_scales = p->rows_qs;
+  g.x_rows = rows;
+  g.rows = rows;
+  g.groups = 1;
+  g.n = n;
+  g.k = k;
+  g.w = static_cast<const int8_t*>(w);
+  g.w_scales = w_s;
+  g.residual = accumulate ? y : nullptr;
+  g.y = y;
+  g.ldx = k;
+  g.ldw = k;
+  g.ldr = n;
+  g.ldy = n;
+  g.err = p->err;
+  return launch_w8a8(g, stream);
+}
+
 // One decode step: every layer (norm + q/k/v + RoPE + cache, attention,
 // output projection, the MoE block) and the head with the greedy choice. For
 // measurement, ev (kProfilePhases + 1 events per layer slot) receives an event
@@ -258,18 +288,23 @@ int uocr_decoder_create(const uocr_decoder_desc* desc, uocr_decoder** out) {
                  "decoder_create: need layers > 0, vocab > 1, 0 < max_prefill < max_positions");
   if (d.weight_format != UOCR_WEIGHT_BF16 && d.weight_format != UOCR_WEIGHT_INT8)
     return dfail(UOCR_ERR_INVALID_ARGUMENT, "decoder_create: weight_format must be bf16 or int8");
+  const bool int8_act = (d.flags & UOCR_DECODER_INT8_ACTIVATIONS) != 0;
+  if (int8_act && d.weight_format != UOCR_WEIGHT_INT8)
+    return dfail(UOCR_ERR_INVALID_ARGUMENT, "decoder_create: int8 activations need int8 weights");
   if (!(d.rope_theta > 0.0f) || !(d.rms_norm_eps >= 0.0f))
     return dfail(UOCR_ERR_INVALID_ARGUMENT, "decoder_create: rope_theta > 0, rms_norm_eps >= 0");
   Guard guard(d.device);
   auto* p = new uocr_decoder;
   p->d = d;
   p->int8 = d.weight_format == UOCR_WEIGHT_INT8;
+  p->int8_act = int8_act;
   p->shape = DecShape{static_cast<int>(d.hidden), static_cast<int>(d.heads), static_cast<int>(d.kv_heads),
                       static_cast<int>(d.vocab), static_cast<int>(d.max_positions), d.rms_norm_eps};
   p->qkv_rows = (d.heads + 2 * d.kv_heads) * kDecHeadDim;
   int sms = 0;
   cudaError_t st = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, d.device);
   if (st == cudaSuccess) st = prepare_decoder_kernels();
+  if (st == cudaSuccess && int8_act) st = prepare_w8a8();
   if (st == cudaSuccess)
     st = plan_dec_attn(p->shape, (d.flags & UOCR_DECODER_CUDA_CORE_ATTENTION) != 0, &p->splits, &p->attn_mode);
   if (st != cudaSuccess) {
@@ -289,7 +324,7 @@ int uocr_decoder_create(const uocr_decoder_desc* desc, uocr_decoder** out) {
   md.weight_format = d.weight_format;
   md.renormalize = d.renormalize;
   md.device = d.device;
-  md.flags = UOCR_PLAN_PRE_NORM | UOCR_PLAN_NO_GRAPHS;
+  md.flags = UOCR_PLAN_PRE_NORM | UOCR_PLAN_NO_GRAPHS | (int8_act ? UOCR_PLAN_INT8_ACTIVATIONS : 0);
   md.rms_norm_eps = d.rms_norm_eps;
   int rc = uocr_moe_plan_create(&md, &p->moe);
   if (rc != UOCR_OK) {
@@ -356,7 +391,9 @@ int uocr_decoder_create(const uocr_decoder_desc* desc, uocr_decoder** out) {
       static_cast<size_t>(R * p->qkv_rows) * 4,                           // qkv
       static_cast<size_t>(R * A) * 2,                                     // qb
       static_cast<size_t>(R * A) * 2,                                     // attn
-      p->int8 ? static_cast<size_t>(std::max(p->qkv_rows * H, H * A)) * 2 : 0,  // wexp
+      p->int8 && !int8_act ? static_cast<size_t>(std::max(p->qkv_rows * H, H * A)) * 2 : 0,  // wexp
+      int8_act ? static_cast<size_t>(R * std::max(H, A)) : 0,                                // rows_q
+      int8_act ? static_cast<size_t>(R) * 4 : 0,                                             // rows_qs
       sizeof(ErrorWord)};
   size_t total = 0;
   for (size_t v : sizes) total += up256(v);
@@ -390,6 +427,8 @@ int uocr_decoder_create(const uocr_decoder_desc* desc, uocr_decoder** out) {
     take(reinterpret_cast<void**>(&p->qb));
     take(reinterpret_cast<void**>(&p->attn));
     take(reinterpret_cast<void**>(&p->wexp));
+    take(reinterpret_cast<void**>(&p->rows_q));
+    take(reinterpret_cast<void**>(&p->rows_qs));
     take(reinterpret_cast<void**>(&p->err));
   }
   // RoPE frequencies: float(1 / theta^(i / 64)) in double, as PageRope
@@ -502,16 +541,26 @@ int uocr_decoder_prefill(uocr_decoder* p, const float* embeds, int64_t rows, flo
     DEC_TRY(launch_norm_rows_bf16(p->x, rows, static_cast<int>(H), L.input_norm, p->d.rms_norm_eps, p->xn, stream),
             "decoder_prefill: norm");
     cudaError_t st = cudaSuccess;
-    const __nv_bfloat16* wqkv = gemm_operand(p, L.wqkv, L.wqkv_s, p->qkv_rows, H, stream, &st);
-    DEC_TRY(st, "decoder_prefill: int8 expansion");
-    DEC_TRY(gemm(p, p->xn, rows, H, wqkv, p->qkv_rows, p->qkv, false, stream), "decoder_prefill: q/k/v GEMM");
+    if (p->int8_act) {
+      DEC_TRY(int8_projection(p, p->xn, rows, H, L.wqkv, L.wqkv_s, p->qkv_rows, p->qkv, false, stream),
+              "decoder_prefill: q/k/v product");
+    } else {
+      const __nv_bfloat16* wqkv = gemm_operand(p, L.wqkv, L.wqkv_s, p->qkv_rows, H, stream, &st);
+      DEC_TRY(st, "decoder_prefill: int8 expansion");
+      DEC_TRY(gemm(p, p->xn, rows, H, wqkv, p->qkv_rows, p->qkv, false, stream), "decoder_prefill: q/k/v GEMM");
+    }
     DEC_TRY(launch_rope_rows(s, p->qkv, rows, p->inv_freq, p->qb, kc_of(p, l), vc_of(p, l), stream),
             "decoder_prefill: rope");
     DEC_TRY(launch_prefill_attn(s, p->qb, rows, kc_of(p, l), vc_of(p, l), p->attn, stream),
             "decoder_prefill: attention");
-    const __nv_bfloat16* wo = gemm_operand(p, L.wo, L.wo_s, H, A, stream, &st);
-    DEC_TRY(st, "decoder_prefill: int8 expansion");
-    DEC_TRY(gemm(p, p->attn, rows, A, wo, H, p->x, true, stream), "decoder_prefill: output GEMM");
+    if (p->int8_act) {
+      DEC_TRY(int8_projection(p, p->attn, rows, A, L.wo, L.wo_s, H, p->x, true, stream),
+              "decoder_prefill: output product");
+    } else {
+      const __nv_bfloat16* wo = gemm_operand(p, L.wo, L.wo_s, H, A, stream, &st);
+      DEC_TRY(st, "decoder_prefill: int8 expansion");
+      DEC_TRY(gemm(p, p->attn, rows, A, wo, H, p->x, true, stream), "decoder_prefill: output GEMM");
+    }
     DEC_RC(moe_layer_inplace(p->moe, l, p->x, rows, stream));
   }
   DEC_TRY(launch_dec_lmhead(s, p->int8, p->x + (rows - 1) * H, p->final_norm, DecMatrix{p->lm_head, p->lm_head_s},

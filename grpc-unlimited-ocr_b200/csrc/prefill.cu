@@ -13,6 +13,7 @@
 #include "prefill.h"
 #include "combine.cuh"
 #include "route.cuh"
+#include "w8a8.h"
 
 namespace uocr_b200 {
 namespace {
@@ -80,12 +81,12 @@ __global__ void scan_kernel(const int* __restrict__ block_counts, int nblk, int 
 }
 
 // Positions of every selection (stable: token order inside each expert's
-// segment). A row's rank among the earlier rows of its warp that chose the
+// segment), and with row_of the row at each position. A row's rank among the earlier rows of its warp that chose the
 // same expert is a population count over a per-warp, per-expert lane mask
 // (a row's k ids are distinct, so each lane sets its bit once per expert).
 __global__ void __launch_bounds__(kPermBlock) positions_kernel(int T, int K, int E, const int* __restrict__ ids,
                                                                const int* __restrict__ block_offset,
-                                                               int* __restrict__ pos_of) {
+                                                               int* __restrict__ pos_of, int* __restrict__ row_of) {
   __shared__ int wcount[8][kMaxExperts];
   __shared__ unsigned lanes[8][kMaxExperts];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -127,6 +128,7 @@ __global__ void __launch_bounds__(kPermBlock) positions_kernel(int T, int K, int
       p = block_offset[static_cast<int64_t>(blockIdx.x) * E + e] + wcount[warp][e] +
           __popc(lanes[warp][e] & ((1u << lane) - 1u));
     pos_of[static_cast<int64_t>(t) * K + j] = p;
+    if (row_of != nullptr && p >= 0) row_of[p] = t;
   }
 }
 
@@ -223,13 +225,27 @@ void carve_prefill_scratch(const PrefillDims& d, void* base, PrefillScratch* s, 
   s->block_counts = reinterpret_cast<int*>(take(nblk * E * 4));
   s->block_offset = reinterpret_cast<int*>(take(nblk * E * 4));
   s->pos_of = reinterpret_cast<int*>(take(T * K * 4));
-  s->xhat = reinterpret_cast<__nv_bfloat16*>(take(T * H * 2));
+  if (d.int8_act) {
+    s->xq = reinterpret_cast<int8_t*>(take(T * H));
+    s->xq_s = reinterpret_cast<float*>(take(T * 4));
+    s->act_sq = reinterpret_cast<int8_t*>(take(T * (S > 0 ? S : 1)));
+    s->act_sqs = reinterpret_cast<float*>(take(T * 4));
+  } else {
+    s->xhat = reinterpret_cast<__nv_bfloat16*>(take(T * H * 2));
+  }
   s->act_s = reinterpret_cast<__nv_bfloat16*>(take(T * (S > 0 ? S : 1) * 2));
   s->shared_out = reinterpret_cast<float*>(take(T * H * 4));
   if (routed_buffers) {
     s->seg_count = reinterpret_cast<int*>(take(E * 4));
     s->seg_start = reinterpret_cast<int*>(take(E * 4));
-    s->xperm = reinterpret_cast<__nv_bfloat16*>(take(T * K * H * 2));
+    if (d.int8_act) {
+      s->row_of = reinterpret_cast<int*>(take(T * K * 4));
+      s->xq_perm = reinterpret_cast<int8_t*>(take(T * K * H));
+      s->act_q = reinterpret_cast<int8_t*>(take(T * K * F));
+      s->act_qs = reinterpret_cast<float*>(take(T * K * 4));
+    } else {
+      s->xperm = reinterpret_cast<__nv_bfloat16*>(take(T * K * H * 2));
+    }
     s->act = reinterpret_cast<__nv_bfloat16*>(take(T * K * F * 2));
     s->yperm = reinterpret_cast<__nv_bfloat16*>(take(T * K * H * 2));
   }
@@ -255,10 +271,15 @@ cudaError_t launch_prefill_route(const PrefillCall& c, cudaStream_t stream) {
   if ((st = cudaGetLastError()) != cudaSuccess) return st;
   scan_kernel<<<1, kMaxExperts, 0, stream>>>(s.block_counts, nblk, E, s.seg_count, s.seg_start, s.block_offset);
   if ((st = cudaGetLastError()) != cudaSuccess) return st;
-  positions_kernel<<<nblk, kPermBlock, 0, stream>>>(T, K, E, c.ids, s.block_offset, s.pos_of);
+  positions_kernel<<<nblk, kPermBlock, 0, stream>>>(T, K, E, c.ids, s.block_offset, s.pos_of, s.row_of);
   if ((st = cudaGetLastError()) != cudaSuccess) return st;
-  permute_copy_kernel<<<c.sm_count * 8, 256, 0, stream>>>(c.x, T, H, K, s.pos_of, s.xhat, s.xperm);
-  if ((st = cudaGetLastError()) != cudaSuccess) return st;
+  if (d.int8_act) {
+    st = launch_quantize_tokens(c.x, false, T, H, H, s.xq, H, s.xq_s, stream);
+  } else {
+    permute_copy_kernel<<<c.sm_count * 8, 256, 0, stream>>>(c.x, T, H, K, s.pos_of, s.xhat, s.xperm);
+    st = cudaGetLastError();
+  }
+  if (st != cudaSuccess) return st;
   return mark(2);
 }
 
@@ -336,6 +357,62 @@ cudaError_t launch_prefill(const PrefillCall& c, cudaStream_t stream) {
   if ((st = launch_grouped_gemm(prefill_down_gemm(c, true, true), stream)) != cudaSuccess ||
       (st = mark(4)) != cudaSuccess)
     return st;
+  if ((st = launch_prefill_combine(c, stream)) != cudaSuccess) return st;
+  return mark(5);
+}
+
+cudaError_t launch_prefill_int8(const PrefillCall& c, const Int8Experts& w, cudaStream_t stream) {
+  const PrefillDims& d = c.dims;
+  const PrefillScratch& s = c.scratch;
+  const int64_t T = c.rows, H = d.hidden, F = d.ffn, S = d.shared_ffn, R = T * d.top_k;
+  if (T <= 0) return cudaSuccess;
+  auto mark = [&](int i) { return c.events != nullptr ? cudaEventRecord(c.events[i], stream) : cudaSuccess; };
+  cudaError_t st = launch_prefill_route(c, stream);
+  if (st != cudaSuccess) return st;
+  // One product: rows of xq [rows, k] (through row_of for the first) by w (and
+  // up, gated) into y [rows, n].
+  auto product = [&](const int8_t* xq, const float* xs, const int* row_of, int64_t rows, int64_t k, bool routed,
+                     const Q8Rows& m, const Q8Rows* up, int64_t n, void* y, bool y_bf16) {
+    W8a8 p{};
+    p.x = xq;
+    p.x_scales = xs;
+    p.row_index = row_of;
+    p.x_rows = row_of != nullptr ? T : rows;
+    p.starts = routed ? s.seg_start : nullptr;
+    p.counts = routed ? s.seg_count : nullptr;
+    p.rows = rows;
+    p.groups = routed ? d.experts : 1;
+    p.n = n;
+    p.k = k;
+    p.w = m.q;
+    p.w_scales = m.scale;
+    p.w_up = up != nullptr ? up->q : nullptr;
+    p.w_up_scales = up != nullptr ? up->scale : nullptr;
+    p.y = y;
+    p.ldx = k;
+    p.ldw = k;
+    p.ldy = n;
+    p.y_bf16 = y_bf16;
+    p.workspace = s.xq_perm;
+    p.err = c.err;
+    return launch_w8a8(p, stream);
+  };
+  // The activations between the products are bf16, whose 2^-9 is well below
+  // the int8 step of a row's largest value that follows.
+  if ((st = product(s.xq, s.xq_s, s.row_of, R, H, true, w.gate, &w.up, F, s.act, true)) != cudaSuccess) return st;
+  if (S > 0 && (st = product(s.xq, s.xq_s, nullptr, T, H, false, w.sgate, &w.sup, S, s.act_s, true)) != cudaSuccess)
+    return st;
+  if ((st = mark(3)) != cudaSuccess) return st;
+  if ((st = launch_quantize_tokens(s.act, true, R, F, F, s.act_q, F, s.act_qs, stream)) != cudaSuccess) return st;
+  if ((st = product(s.act_q, s.act_qs, nullptr, R, F, true, w.down, nullptr, H, s.yperm, true)) != cudaSuccess)
+    return st;
+  if (S > 0) {
+    st = launch_quantize_tokens(s.act_s, true, T, S, S, s.act_sq, S, s.act_sqs, stream);
+    if (st != cudaSuccess) return st;
+    st = product(s.act_sq, s.act_sqs, nullptr, T, S, false, w.sdown, nullptr, H, s.shared_out, false);
+    if (st != cudaSuccess) return st;
+  }
+  if ((st = mark(4)) != cudaSuccess) return st;
   if ((st = launch_prefill_combine(c, stream)) != cudaSuccess) return st;
   return mark(5);
 }

@@ -19,6 +19,7 @@ struct PrefillDims {
   int ffn;
   int shared_ffn;
   int renormalize;
+  int int8_act = 0;  // int8 weights multiplied by int8 activations (launch_prefill_int8)
 };
 
 // Scratch carved from the plan arena, sized for max_rows.
@@ -34,6 +35,16 @@ struct PrefillScratch {
   __nv_bfloat16* act_s;         // [T, S] shared SwiGLU activations
   __nv_bfloat16* yperm;         // [T*k, H] routed expert outputs
   float* shared_out;            // [T, H] shared expert output
+  // With dims.int8_act, in the place of xhat and xperm: the quantised
+  // activations with a scale per row, and the rows grouped by expert.
+  int* row_of;                  // [T*k] input row of each permuted row
+  int8_t* xq;                   // [T, H]
+  float* xq_s;                  // [T]
+  int8_t* xq_perm;              // [T*k, H]
+  int8_t* act_q;                // [T*k, F]
+  float* act_qs;                // [T*k]
+  int8_t* act_sq;               // [T, S]
+  float* act_sqs;               // [T]
   size_t bytes;
 };
 
@@ -73,6 +84,13 @@ cudaError_t launch_prefill_combine(const PrefillCall& c, cudaStream_t stream);
 cudaError_t launch_router_logits_rows(const float* x, int T, int H, const float* router, const float* bias, int E,
                                       float* logits, cudaStream_t stream);
 cudaError_t launch_prefill(const PrefillCall& c, cudaStream_t stream);
+// The same with int8 weights (one scale per row) and int8 activations (one
+// scale per token, quantised in front of each product): the W8A8 products
+// (w8a8.h) instead of the bf16 GEMMs. dims.int8_act scratch.
+struct Int8Experts {
+  Q8Rows gate, up, down, sgate, sup, sdown;
+};
+cudaError_t launch_prefill_int8(const PrefillCall& c, const Int8Experts& w, cudaStream_t stream);
 
 // The stages of launch_prefill, for the expert-parallel path (ep.cu):
 // router + top-k + permutation (an empty batch writes empty segments), and

@@ -42,6 +42,9 @@ struct W8a8 {
 // Device memory a grouped product with row_index needs for its duration: the rows it names, copied together.
 size_t w8a8_gather_bytes(int64_t rows, int64_t groups, int64_t k);
 cudaError_t launch_w8a8(const W8a8& p, cudaStream_t stream);
+// Sets the product kernels up on the current device (otherwise their first
+// launch does); for callers whose first launch may be inside a stream capture.
+cudaError_t prepare_w8a8();
 // The kernel for few rows (w8a8_rows.cu); launch_w8a8 chooses.
 cudaError_t launch_w8a8_rows(const W8a8& p, cudaStream_t stream);
 

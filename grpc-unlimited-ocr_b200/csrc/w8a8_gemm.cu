@@ -682,6 +682,15 @@ size_t w8a8_gather_bytes(int64_t rows, int64_t groups, int64_t k) {
   return few_rows_grouped(rows, groups) ? 0 : static_cast<size_t>(rows) * static_cast<size_t>((k + 15) / 16 * 16);
 }
 
+cudaError_t prepare_w8a8() {
+  int pairs = 0;
+  cudaError_t st = resident_pairs<false, false>(&pairs);
+  if (st == cudaSuccess) st = resident_pairs<false, true>(&pairs);
+  if (st == cudaSuccess) st = resident_pairs<true, false>(&pairs);
+  if (st == cudaSuccess) st = resident_pairs<true, true>(&pairs);
+  return st;
+}
+
 cudaError_t launch_w8a8(const W8a8& p, cudaStream_t stream) {
   if (p.rows == 0 || p.n == 0) return cudaSuccess;
   if (few_rows(p)) return launch_w8a8_rows(p, stream);

@@ -24,7 +24,9 @@ DTYPE_F32, DTYPE_BF16 = 0, 1
 PLAN_NO_GRAPHS = 1
 PLAN_EP_STRIDED = 4
 PLAN_PRE_NORM = 8
+PLAN_INT8_ACTIVATIONS = 16
 DECODER_CUDA_CORE_ATTENTION = 1
+DECODER_INT8_ACTIVATIONS = 2
 EP_HANDLE_BYTES = 256
 
 # Synthetic tensor kinds (one generator stream per tensor per layer).

@@ -133,3 +133,14 @@ def test_binding_refuses_wrong_tensors():
         M.linear_w8a8(x, s, x, s, torch.zeros(2, 2))
     with pytest.raises(ValueError):
         M.quantize_tokens(torch.zeros(2, 16, dtype=torch.float16), x, s)
+
+
+def test_int8_activations_need_int8_weights():
+    plan = M.MoeDesc(256, 8, 2, 128, 128, 1, 32, M.WEIGHT_BF16, 1, 0, 0, M.PLAN_INT8_ACTIVATIONS)
+    h = ctypes.c_void_p()
+    assert M.lib().uocr_moe_plan_create(ctypes.byref(plan), ctypes.byref(h)) == 1 and not h.value
+    assert "int8 weights" in M.lib().uocr_last_error().decode()
+    dec = M.DecoderDesc(512, 1, 4, 1, 128, 256, 64, 32, 8, 2, 128, 256, 1e4, 1e-6, M.WEIGHT_BF16, 1, 0,
+                        M.DECODER_INT8_ACTIVATIONS)
+    assert M.lib().uocr_decoder_create(ctypes.byref(dec), ctypes.byref(h)) == 1 and not h.value
+    assert "int8 weights" in M.lib().uocr_last_error().decode()
