@@ -172,6 +172,18 @@ __device__ __forceinline__ void tmem_dealloc_pair(uint32_t base, uint32_t cols) 
   asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols) : "memory");
 }
 
+// 16 consecutive int32 columns of this warp's 32 TMEM lanes (lane i of the
+// warp: TMEM lane (addr >> 16) + i), with the wait.
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t addr, int (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr)
+      : "memory");
+}
+
 // Int32 columns col .. col + 31 of 16 TMEM lanes, without the wait
 // (tmem_ld_wait): thread t holds, of 8 columns after another, lane t / 4 at
 // columns 2 (t % 4) and + 1, then lane t / 4 + 8 at the same columns.

@@ -75,9 +75,11 @@ struct GroupedGemm {
 // boxes of 128 columns x box_rows rows, 128-byte swizzle, zeros past the edges.
 bool make_int8_tmap(CUtensorMap* map, const int8_t* base, int64_t rows, int64_t cols, int64_t pitch, int box_rows);
 
-// Tensor map of bf16 rows [rows, cols] at `ld` elements (16-byte aligned
-// rows), for storing boxes of 32 columns x box_rows rows, 64-byte swizzle.
-bool make_store_tmap(CUtensorMap* map, __nv_bfloat16* base, int64_t rows, int64_t cols, int64_t ld, int box_rows);
+// Tensor map of fp32 or bf16 rows [rows, cols] at `ld` elements (16-byte
+// aligned rows), in boxes of 32 columns x box_rows rows: fp32 rows of 128 bytes
+// as they are, bf16 rows of 64 bytes with the 64-byte swizzle.
+bool make_tile_tmap(CUtensorMap* map, const void* base, bool bf16, int64_t rows, int64_t cols, int64_t ld,
+                    int box_rows);
 
 size_t grouped_gemm_smem_bytes();
 cudaError_t launch_grouped_gemm(const GroupedGemm& g, cudaStream_t stream);

@@ -51,9 +51,13 @@ constexpr int kThreads = 128 + kEpilogueWarps * 32;
 constexpr int kUnit = 32;              // tokens an epilogue warp takes at a time
 constexpr int kOutBytes = kUnit * 32 * 2;        // a unit of 32 channels in bf16
 constexpr int kXchBytes = kUnit / 2 * 32 * 4;    // gated: half a unit's values for the partner warp
-// Per epilogue warp, two buffers of each (a gated warp's output is half a unit).
+constexpr int kRows32 = 16;            // tokens of an fp32 unit
+constexpr int kSlotBytes = kRows32 * 32 * 4;     // an fp32 unit of 32 channels
+constexpr int kSlots = 3;
+// Per epilogue warp: two buffers of each in bf16 (a gated warp's output is half
+// a unit), or three fp32 units.
 template <bool kGated>
-constexpr int kWarpBytes = kGated ? kOutBytes + 2 * kXchBytes : 2 * kOutBytes;
+constexpr int kWarpBytes = kGated ? kOutBytes + 2 * kXchBytes : kSlots * kSlotBytes;
 template <bool kGated>
 constexpr int kSmem = kStages * kStageBytes + kEpilogueWarps * kWarpBytes<kGated> + 1024;
 constexpr int kTmemCols = 512;
@@ -62,18 +66,21 @@ constexpr int kBand = 8;               // token tiles of a band (decode_tile)
 
 struct Args {
   CUtensorMap y;                         // boxes of a unit's tokens (gated: half) x 32 channels; unset unless tma_store
+  CUtensorMap residual;                  // the same of the residual (fp32); unset unless tma_residual
   CUtensorMap x, x_wide, x_half, w, up;  // token boxes of 16, 64 and 128 rows; weight boxes of 128 (gated: 64)
   W8a8 p;
   int tokens_per_tile;  // at most kMaxN, a multiple of 32
   int channels;         // output channels per tile of a pair
   int c_tiles, k_blocks;
-  bool tma_store;       // y is bf16 and its rows start at 16-byte boundaries
+  bool tma_store;       // y's rows start at 16-byte boundaries (gated: and y is bf16)
+  bool tma_residual;    // so do the residual's, and y is fp32
 };
 
 struct Shared {
   uint64_t full[kStages], empty[kStages];
   uint64_t acc_full[2], acc_empty[2];
   uint64_t drain;
+  uint64_t residual[kEpilogueWarps][kSlots];
   uint32_t tmem;
   int failed[2];  // an epilogue warp's wait for this accumulator ran out
   alignas(16) float x_scale[2][kMaxN];
@@ -202,6 +209,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       mbar_init(&sh.acc_empty[i], 2 * kEpilogueWarps);
     }
     mbar_init(&sh.drain, 1);
+    for (int w = 0; w < kEpilogueWarps; ++w)
+      for (int i = 0; i < kSlots; ++i) mbar_init(&sh.residual[w][i], 1);
     sh.failed[0] = sh.failed[1] = 0;
     fence_mbar_init();
   }
@@ -400,7 +409,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     };
     Scales next{};
     if (blockIdx.x / 2 < total) next = fetch(blockIdx.x / 2);
-    int local = 0, buf = 0;
+    int local = 0, buf = 0, slot = 0;
+    uint32_t slot_phase = 0;
     bool ok = true;
     for (int t = blockIdx.x / 2; t < total; t += step, ++local) {
       const Scales cur = next;
@@ -412,6 +422,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       uint64_t ws[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) asm("mov.b64 %0, {%1, %1};" : "=l"(ws[q]) : "f"(cur.w[q]));
+      // fp32 units: whole ones pass through this warp's slots, the residual's box on the way in.
+      auto whole_f32 = [&](int j0) { return args.tma_store && tl.rows - j0 >= kRows32 && c0 < p.n; };
+      auto fetch_residual = [&](int j0, int s) {
+        if (!args.tma_residual || j0 >= tl.rows || !whole_f32(j0) || !elect_one()) return;
+        bulk_wait_read<1>();  // the slot's last store, two units ago, has read it
+        mbar_arrive_expect_tx(&sh.residual[e][s], kSlotBytes);
+        tma_load_2d(stg + s * kSlotBytes, &args.residual, static_cast<int>(c0), tl.row0 + j0, &sh.residual[e][s]);
+      };
+      if (!kGated && !kBf16) fetch_residual(way * kRows32, slot);
       if (ok) {
         ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[acc], (local >> 1) & 1));
         if (!ok) raise_error(p.err, kDevWaitTimeout, 86, t, 0);
@@ -427,8 +446,71 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive_pair(pair_leader_addr(&sh.acc_empty[acc]));
       };
-      if (way * kUnit >= tl.rows) release();
       if (t + step < total) next = fetch(t + step);
+      if (!kGated && !kBf16) {
+        // Lane = channel here, so that a token's 32 channels are a line of 128 bytes.
+        const int64_t cl = c0 + lane;
+        const bool cl_ok = cl < p.n;
+        const float w_lane = cl_ok ? __ldg(p.w_scales + tl.g * p.n + cl) : 0.0f;
+        const float bias_lane = has_bias && cl_ok ? __ldg(p.bias + cl) : 0.0f;
+        uint64_t w2;
+        asm("mov.b64 %0, {%1, %1};" : "=l"(w2) : "f"(w_lane));
+        if (way * kRows32 >= tl.rows) release();
+        for (int j0 = way * kRows32; j0 < tl.rows; j0 += kWays * kRows32) {
+          const int next_slot = slot + 1 == kSlots ? 0 : slot + 1;
+          fetch_residual(j0 + kWays * kRows32, next_slot);
+          int a[kRows32];
+          tmem_ld_32x16(taddr + j0, a);
+          if (j0 + kWays * kRows32 >= tl.rows) release();
+          float v[kRows32];
+#pragma unroll
+          for (int i = 0; i < kRows32; i += 4) {
+            const ulonglong2 s = *reinterpret_cast<const ulonglong2*>(&sh.x_scale[acc][j0 + i]);
+            scale_pair(a[i], a[i + 1], s.x, w2, v[i], v[i + 1]);
+            scale_pair(a[i + 2], a[i + 3], s.y, w2, v[i + 2], v[i + 3]);
+          }
+          if (has_bias) {
+#pragma unroll
+            for (int i = 0; i < kRows32; ++i) v[i] += bias_lane;
+          }
+          const int64_t row = tl.row0 + j0;
+          float* out = reinterpret_cast<float*>(stg + slot * kSlotBytes) + lane;
+          const bool whole = whole_f32(j0);
+          if (whole && args.tma_residual) {
+            if (!mbar_wait(&sh.residual[e][slot], (slot_phase >> slot) & 1)) raise_error(p.err, kDevWaitTimeout, 89, t, j0);
+            slot_phase ^= 1u << slot;
+#pragma unroll
+            for (int i = 0; i < kRows32; ++i) v[i] += out[i * 32];
+          } else if (has_residual) {
+            const float* res = static_cast<const float*>(p.residual) + row * p.ldr + cl;
+#pragma unroll
+            for (int i = 0; i < kRows32; ++i)
+              if (cl_ok && i < tl.rows - j0) v[i] += res[i * p.ldr];
+          }
+          if (whole) {
+            if (!args.tma_residual) {
+              if (elect_one()) bulk_wait_read<2>();  // the slot's last store, three units ago, has read it
+              __syncwarp();
+            }
+#pragma unroll
+            for (int i = 0; i < kRows32; ++i) out[i * 32] = v[i];
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (elect_one()) {
+              tma_store_2d(&args.y, static_cast<int>(c0), static_cast<int>(row), stg + slot * kSlotBytes);
+              bulk_commit();
+            }
+          } else if (cl_ok) {
+            float* dst = static_cast<float*>(p.y) + row * p.ldy + cl;
+#pragma unroll
+            for (int i = 0; i < kRows32; ++i)
+              if (i < tl.rows - j0) dst[i * p.ldy] = v[i];
+          }
+          slot = next_slot;
+        }
+        continue;
+      }
+      if (way * kUnit >= tl.rows) release();
       for (int j0 = way * kUnit; j0 < tl.rows; j0 += kWays * kUnit) {
         int a[2][16];  // [16 lanes][the four blocks' four values]
         tmem_ld_16x32(taddr + j0, a[0]);
@@ -645,8 +727,14 @@ cudaError_t launch(const W8a8& p, cudaStream_t stream) {
                   make_int8_tmap(&a.w, p.w, p.groups * p.n, p.k, p.ldw, kGated ? kBM / 2 : kBM) &&
                   (!kGated || make_int8_tmap(&a.up, p.w_up, p.groups * p.n, p.k, p.ldw, kBM / 2));
   if (!ok) return cudaErrorInvalidValue;
-  a.tma_store = kBf16 && reinterpret_cast<uintptr_t>(p.y) % 16 == 0 && p.ldy % 8 == 0;
-  if (a.tma_store && !make_store_tmap(&a.y, static_cast<__nv_bfloat16*>(p.y), p.rows, p.n, p.ldy, kGated ? kUnit / 2 : kUnit))
+  auto aligned = [](const void* base, int64_t ld) {
+    return reinterpret_cast<uintptr_t>(base) % 16 == 0 && ld * (kBf16 ? 2 : 4) % 16 == 0;
+  };
+  a.tma_store = (kBf16 || !kGated) && aligned(p.y, p.ldy);
+  a.tma_residual = !kBf16 && !kGated && a.tma_store && p.residual != nullptr && aligned(p.residual, p.ldr);
+  const int box_rows = !kBf16 ? kRows32 : kGated ? kUnit / 2 : kUnit;
+  if (a.tma_store && !make_tile_tmap(&a.y, p.y, kBf16, p.rows, p.n, p.ldy, box_rows)) return cudaErrorInvalidValue;
+  if (a.tma_residual && !make_tile_tmap(&a.residual, p.residual, kBf16, p.rows, p.n, p.ldr, box_rows))
     return cudaErrorInvalidValue;
   a.p = p;
   a.channels = kGated ? kBM : 2 * kBM;
