@@ -16,7 +16,8 @@
 //   warp 1     allocates TMEM; in the leader one lane issues the MMAs;
 //   warps 4-11 epilogue, 32 tokens x 32 weight rows at a time: the scales,
 //              then bf16 tiles are transposed into shared memory (stmatrix) and
-//              leave as bulk tensor stores, fp32 ones as sectors of 8 channels.
+//              leave as bulk tensor stores, fp32 ones as lines of 32 channels
+//              (gated: sectors of 8), a residual arriving by TMA a unit ahead.
 //              When gated, the gate's warp and the up's warp of the same
 //              channels exchange half of their tokens first.
 // Rows named by an index are first copied together (gather_rows_kernel): TMA
@@ -52,12 +53,13 @@ constexpr int kUnit = 32;              // tokens an epilogue warp takes at a tim
 constexpr int kOutBytes = kUnit * 32 * 2;        // a unit of 32 channels in bf16
 constexpr int kXchBytes = kUnit / 2 * 32 * 4;    // gated: half a unit's values for the partner warp
 constexpr int kRows32 = 16;            // tokens of an fp32 unit
-constexpr int kSlotBytes = kRows32 * 32 * 4;     // an fp32 unit of 32 channels
-constexpr int kSlots = 3;
+constexpr int kSlotBytes = kRows32 * 32 * 4;     // an fp32 unit's residual
+constexpr int kSlots = 2;
 // Per epilogue warp: two buffers of each in bf16 (a gated warp's output is half
-// a unit), or three fp32 units.
+// a unit), or of an fp32 unit's residual.
 template <bool kGated>
-constexpr int kWarpBytes = kGated ? kOutBytes + 2 * kXchBytes : kSlots * kSlotBytes;
+constexpr int kWarpBytes = kGated ? kOutBytes + 2 * kXchBytes : 2 * kOutBytes;
+static_assert(kSlots * kSlotBytes <= 2 * kOutBytes, "the residual's slots take the place of the output buffers");
 template <bool kGated>
 constexpr int kSmem = kStages * kStageBytes + kEpilogueWarps * kWarpBytes<kGated> + 1024;
 constexpr int kTmemCols = 512;
@@ -68,14 +70,18 @@ static_assert(kEpilogueWarps * 32 == kMaxN, "an epilogue thread for each token o
 
 struct Args {
   CUtensorMap y;                         // boxes of a unit's tokens (gated: half) x 32 channels; unset unless tma_store
-  CUtensorMap residual;                  // the same of the residual (fp32); unset unless tma_residual
+  CUtensorMap residual;                  // boxes of an fp32 unit's tokens x 32 channels; unset unless tma_residual
   CUtensorMap x, x_wide, x_half, w, up;  // token boxes of 16, 64 and 128 rows; weight boxes of 128 (gated: 64)
   W8a8 p;
   int tokens_per_tile;  // at most kMaxN, a multiple of 32
   int channels;         // output channels per tile of a pair
   int c_tiles, k_blocks;
-  bool tma_store;       // y's rows start at 16-byte boundaries (gated: and y is bf16)
-  bool tma_residual;    // so do the residual's, and y is fp32
+  bool tma_store;       // y is bf16 and its rows start at 16-byte boundaries
+  bool tma_residual;    // y is fp32 and the residual's rows start at 16-byte boundaries
+};
+
+struct Tile {
+  int g, row0, rows, c0;
 };
 
 struct Shared {
@@ -84,14 +90,11 @@ struct Shared {
   uint64_t drain;
   uint64_t residual[kEpilogueWarps][kSlots];
   uint32_t tmem;
+  Tile tiles[3][32];  // of the three warps that work through one lane: what is next
   int failed[2];  // an epilogue warp's wait for this accumulator ran out
   alignas(16) float x_scale[2][kMaxN];
   int tile_start[kMaxGroups + 1];
   int first[kMaxGroups], count[kMaxGroups];
-};
-
-struct Tile {
-  int g, row0, rows, c0;
 };
 
 // After a wait that ran out: the copies in flight land before this CTA's shared memory is given up.
@@ -256,93 +259,98 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int total = sh.tile_start[groups];
   const int step = gridDim.x / 2;
 
+  // One lane's pass over this pair's tiles, body(tile, n) for the n-th; the
+  // warp works 32 of them out at a time, a lane each (one takes some 1000
+  // clocks, which between two tiles would leave the MMAs waiting).
+  auto each_tile = [&](Tile* table, auto&& body) {
+    bool ok = true;
+    for (int n0 = 0; ok && blockIdx.x / 2 + n0 * step < total; n0 += 32) {
+      const int mine = blockIdx.x / 2 + (n0 + lane) * step;
+      if (mine < total) table[lane] = decode_tile(mine, sh, groups, args);
+      __syncwarp();
+      if (elect_one())
+        for (int i = 0; i < 32 && ok && blockIdx.x / 2 + (n0 + i) * step < total; ++i) ok = body(table[i], n0 + i);
+      ok = __all_sync(0xffffffffu, ok);
+    }
+    return ok;
+  };
+
   if (warp == 0) {
     // ---- weight producer: one lane; the leader also announces both CTAs' bytes of a stage ----
-    if (elect_one()) {
-      const uint32_t full0 = pair_leader_addr(&sh.full[0]);
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (int t = blockIdx.x / 2; t < total && ok; t += step) {
-        const Tile tl = decode_tile(t, sh, groups, args);
-        const uint32_t bytes = 2 * kABytes + round32(tl.rows) * kBK;
-        const int w_row = tl.g * static_cast<int>(p.n) + tl.c0 + rank * (args.channels / 2);
-        for (int kb = 0; kb < args.k_blocks; ++kb) {
-          if (!mbar_wait(&sh.empty[stage], phase ^ 1)) {
-            raise_error(p.err, kDevWaitTimeout, 82, t, kb);
-            ok = false;
-            break;
-          }
-          unsigned char* sa = smem + stage * kStageBytes;
-          if (rank == 0) mbar_arrive_expect_tx(&sh.full[stage], bytes);
-          tma_load_2d_pair(sa, &args.w, kb * kBK, w_row, full0 + stage * 8);
-          if (kGated) tma_load_2d_pair(sa + kABytes / 2, &args.up, kb * kBK, w_row, full0 + stage * 8);
-          if (++stage == kStages) {
-            stage = 0;
-            phase ^= 1;
-          }
+    const uint32_t full0 = pair_leader_addr(&sh.full[0]);
+    int stage = 0;
+    uint32_t phase = 0;
+    const bool ok = each_tile(sh.tiles[0], [&](const Tile& tl, int) {
+      const uint32_t bytes = 2 * kABytes + round32(tl.rows) * kBK;
+      const int w_row = tl.g * static_cast<int>(p.n) + tl.c0 + rank * (args.channels / 2);
+      for (int kb = 0; kb < args.k_blocks; ++kb) {
+        if (!mbar_wait(&sh.empty[stage], phase ^ 1)) {
+          raise_error(p.err, kDevWaitTimeout, 82, tl.row0, kb);
+          return false;
+        }
+        unsigned char* sa = smem + stage * kStageBytes;
+        if (rank == 0) mbar_arrive_expect_tx(&sh.full[stage], bytes);
+        tma_load_2d_pair(sa, &args.w, kb * kBK, w_row, full0 + stage * 8);
+        if (kGated) tma_load_2d_pair(sa + kABytes / 2, &args.up, kb * kBK, w_row, full0 + stage * 8);
+        if (++stage == kStages) {
+          stage = 0;
+          phase ^= 1;
         }
       }
-      if (!ok) wait_for_copies();
-    }
+      return true;
+    });
+    if (!ok) wait_for_copies();
   } else if (warp == 2) {
     // ---- token producer: one lane ----
-    if (elect_one()) {
-      const uint32_t full0 = pair_leader_addr(&sh.full[0]);
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (int t = blockIdx.x / 2; t < total && ok; t += step) {
-        const Tile tl = decode_tile(t, sh, groups, args);
-        const int half = round32(tl.rows) / 2;
-        const int row = tl.row0 + rank * half;  // this CTA's first token row
-        for (int kb = 0; kb < args.k_blocks; ++kb) {
-          if (!mbar_wait(&sh.empty[stage], phase ^ 1)) {
-            raise_error(p.err, kDevWaitTimeout, 87, t, kb);
-            ok = false;
-            break;
+    const uint32_t full0 = pair_leader_addr(&sh.full[0]);
+    int stage = 0;
+    uint32_t phase = 0;
+    const bool ok = each_tile(sh.tiles[1], [&](const Tile& tl, int) {
+      const int half = round32(tl.rows) / 2;
+      const int row = tl.row0 + rank * half;  // this CTA's first token row
+      for (int kb = 0; kb < args.k_blocks; ++kb) {
+        if (!mbar_wait(&sh.empty[stage], phase ^ 1)) {
+          raise_error(p.err, kDevWaitTimeout, 87, tl.row0, kb);
+          return false;
+        }
+        unsigned char* sb = smem + stage * kStageBytes + kABytes;
+        const uint32_t bar = full0 + stage * 8;
+        if (half == kMaxN / 2) {
+          tma_load_2d_pair(sb, &args.x_half, kb * kBK, row, bar);
+        } else {
+          int i = 0;
+          if (half >= 64) {
+            tma_load_2d_pair(sb, &args.x_wide, kb * kBK, row, bar);
+            i = 64;
           }
-          unsigned char* sb = smem + stage * kStageBytes + kABytes;
-          const uint32_t bar = full0 + stage * 8;
-          if (half == kMaxN / 2) {
-            tma_load_2d_pair(sb, &args.x_half, kb * kBK, row, bar);
-          } else {
-            int i = 0;
-            if (half >= 64) {
-              tma_load_2d_pair(sb, &args.x_wide, kb * kBK, row, bar);
-              i = 64;
-            }
-            for (; i < half; i += kBoxRows) tma_load_2d_pair(sb + i * kBK, &args.x, kb * kBK, row + i, bar);
-          }
-          if (++stage == kStages) {
-            stage = 0;
-            phase ^= 1;
-          }
+          for (; i < half; i += kBoxRows) tma_load_2d_pair(sb + i * kBK, &args.x, kb * kBK, row + i, bar);
+        }
+        if (++stage == kStages) {
+          stage = 0;
+          phase ^= 1;
         }
       }
-      if (!ok) wait_for_copies();
-    }
+      return true;
+    });
+    if (!ok) wait_for_copies();
   } else if (warp == 1) {
-    if (rank == 0 && elect_one()) {
-      // ---- MMA issuer (for both CTAs) ----
-      int stage = 0, local = 0;
+    if (rank == 0) {
+      // ---- MMA issuer (for both CTAs): one lane ----
+      int stage = 0;
       uint32_t phase = 0;
-      bool ok = true;
-      for (int t = blockIdx.x / 2; t < total && ok; t += step, ++local) {
-        const Tile tl = decode_tile(t, sh, groups, args);
+      each_tile(sh.tiles[2], [&](const Tile& tl, int local) {
         const uint32_t idesc = i8_idesc(2 * kBM, round32(tl.rows));
         const int acc = local & 1;
         if (!mbar_wait(&sh.acc_empty[acc], ((local >> 1) & 1) ^ 1)) {
-          raise_error(p.err, kDevWaitTimeout, 83, t, 0);
-          break;
+          raise_error(p.err, kDevWaitTimeout, 83, tl.row0, 0);
+          return false;
         }
         tc_fence_after();
         const uint32_t d = tmem_base + static_cast<uint32_t>(acc * kMaxN);
         for (int kb = 0; kb < args.k_blocks; ++kb) {
           if (!mbar_wait(&sh.full[stage], phase)) {
-            raise_error(p.err, kDevWaitTimeout, 84, t, kb);
-            ok = false;
-            break;
+            raise_error(p.err, kDevWaitTimeout, 84, tl.row0, kb);
+            return false;
           }
           tc_fence_after();
           const uint32_t sa = smem_addr(smem + stage * kStageBytes);
@@ -357,10 +365,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             phase ^= 1;
           }
         }
-        if (ok) umma_commit_pair(&sh.acc_full[acc]);
+        umma_commit_pair(&sh.acc_full[acc]);
+        return true;
+      });
+      if (elect_one()) {  // the lane that issued: every MMA is complete before shared memory and TMEM are given up
+        umma_commit_pair(&sh.drain);
+        if (!mbar_wait(&sh.drain, 0)) raise_error(p.err, kDevWaitTimeout, 85, 0, 0);
       }
-      umma_commit_pair(&sh.drain);
-      if (!mbar_wait(&sh.drain, 0)) raise_error(p.err, kDevWaitTimeout, 85, 0, 0);
     }
   } else if (warp >= 4) {
     // ---- epilogue: TMEM lane quarter = warp % 4; the warps of a quarter take units in turn ----
@@ -368,6 +379,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int e = warp - 4, quarter = warp & 3, way = e >> 2;
     const int et = threadIdx.x - 128;
     const int tr = lane >> 2, tc = 2 * (lane & 3);  // this thread's first channel and token in a block
+    // fp32 outputs: lane = channel, so that a token's 32 channels are a line of 128 bytes.
+    constexpr bool kLaneIsChannel = !kGated && !kBf16;
+    const int first_c = kLaneIsChannel ? lane : tr;
     unsigned char* area = smem + kStages * kStageBytes;
     unsigned char* stg = area + e * kWarpBytes<kGated>;
     float4* xch = reinterpret_cast<float4*>(stg + kOutBytes);
@@ -377,19 +391,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const float* w_scales = kGated && !gate ? p.w_up_scales : p.w_scales;
     T* y = static_cast<T*>(p.y);
     const bool has_bias = !kGated && p.bias != nullptr, has_residual = !kGated && p.residual != nullptr;
+    const bool tma_residual = kLaneIsChannel && args.tma_residual;
     // What the epilogue needs of a tile beside its sums; the next tile's is
     // fetched while this one's units are stored.
     struct Scales {
       Tile tl;
-      float w[4], bias[4];  // of channels tr + 8 q
-      float x;              // of token et
+      float w[kLaneIsChannel ? 1 : 4], bias[kLaneIsChannel ? 1 : 4];  // of channels first_c + 8 q
+      float x;                                                        // of token et
     };
-    auto fetch = [&](int t) {
+    // Every 32 tiles each lane works one of them out (some 1000 clocks in a
+    // row, which a tile's epilogue has not got).
+    Tile lane_tile{};
+    auto fetch = [&](int nth) {
+      if ((nth & 31) == 0 && blockIdx.x / 2 + (nth + lane) * step < total)
+        lane_tile = decode_tile(blockIdx.x / 2 + (nth + lane) * step, sh, groups, args);
       Scales f{};
-      f.tl = decode_tile(t, sh, groups, args);
-      const int64_t c = f.tl.c0 + local_c + tr;
+      f.tl = Tile{__shfl_sync(0xffffffffu, lane_tile.g, nth & 31), __shfl_sync(0xffffffffu, lane_tile.row0, nth & 31),
+                  __shfl_sync(0xffffffffu, lane_tile.rows, nth & 31), __shfl_sync(0xffffffffu, lane_tile.c0, nth & 31)};
+      const int64_t c = f.tl.c0 + local_c + first_c;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
+      for (int q = 0; q < (kLaneIsChannel ? 1 : 4); ++q) {
         const bool in = c + 8 * q < p.n;
         f.w[q] = in ? __ldg(w_scales + f.tl.g * p.n + c + 8 * q) : 0.0f;
         f.bias[q] = has_bias && in ? __ldg(p.bias + c + 8 * q) : 0.0f;
@@ -410,7 +431,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       return f;
     };
     Scales next{};
-    if (blockIdx.x / 2 < total) next = fetch(blockIdx.x / 2);
+    if (blockIdx.x / 2 < total) next = fetch(0);
     int local = 0, buf = 0, slot = 0;
     uint32_t slot_phase = 0;
     bool ok = true;
@@ -418,21 +439,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const Scales cur = next;
       const Tile& tl = cur.tl;
       const int acc = local & 1;
-      const int64_t c0 = tl.c0 + local_c, c = c0 + tr;
+      const int64_t c0 = tl.c0 + local_c, c = c0 + first_c;
       const int nc = static_cast<int>(p.n - c < 32 ? p.n - c : 32);  // channels c, c + 8, .. below c + nc exist
       sh.x_scale[acc][et] = cur.x;
-      uint64_t ws[4];
+      uint64_t ws[kLaneIsChannel ? 1 : 4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) asm("mov.b64 %0, {%1, %1};" : "=l"(ws[q]) : "f"(cur.w[q]));
-      // fp32 units: whole ones pass through this warp's slots, the residual's box on the way in.
-      auto whole_f32 = [&](int j0) { return args.tma_store && tl.rows - j0 >= kRows32 && c0 < p.n; };
+      for (int q = 0; q < (kLaneIsChannel ? 1 : 4); ++q) asm("mov.b64 %0, {%1, %1};" : "=l"(ws[q]) : "f"(cur.w[q]));
+      // The residual of an fp32 unit whose 16 tokens all exist, into a slot of this warp.
+      auto whole_unit = [&](int j0) { return tl.rows - j0 >= kRows32 && c0 < p.n; };
       auto fetch_residual = [&](int j0, int s) {
-        if (!args.tma_residual || j0 >= tl.rows || !whole_f32(j0) || !elect_one()) return;
-        bulk_wait_read<1>();  // the slot's last store, two units ago, has read it
+        if (!tma_residual || !whole_unit(j0) || !elect_one()) return;
         mbar_arrive_expect_tx(&sh.residual[e][s], kSlotBytes);
         tma_load_2d(stg + s * kSlotBytes, &args.residual, static_cast<int>(c0), tl.row0 + j0, &sh.residual[e][s]);
       };
-      if (!kGated && !kBf16) fetch_residual(way * kRows32, slot);
+      if (kLaneIsChannel && ok) fetch_residual(way * kRows32, slot);
       if (ok) {
         ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[acc], (local >> 1) & 1));
         if (!ok) raise_error(p.err, kDevWaitTimeout, 86, t, 0);
@@ -448,18 +468,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive_pair(pair_leader_addr(&sh.acc_empty[acc]));
       };
-      if (t + step < total) next = fetch(t + step);
-      if (!kGated && !kBf16) {
-        // Lane = channel here, so that a token's 32 channels are a line of 128 bytes.
-        const int64_t cl = c0 + lane;
-        const bool cl_ok = cl < p.n;
-        const float w_lane = cl_ok ? __ldg(p.w_scales + tl.g * p.n + cl) : 0.0f;
-        const float bias_lane = has_bias && cl_ok ? __ldg(p.bias + cl) : 0.0f;
-        uint64_t w2;
-        asm("mov.b64 %0, {%1, %1};" : "=l"(w2) : "f"(w_lane));
+      if (t + step < total) next = fetch(local + 1);
+      if constexpr (kLaneIsChannel) {
+        const int64_t pitch = p.ldy * 4;
         if (way * kRows32 >= tl.rows) release();
         for (int j0 = way * kRows32; j0 < tl.rows; j0 += kWays * kRows32) {
-          const int next_slot = slot + 1 == kSlots ? 0 : slot + 1;
+          const int next_slot = slot ^ 1;
+          // (The slot's values, two units ago, have been read by the whole warp.)
           fetch_residual(j0 + kWays * kRows32, next_slot);
           int a[kRows32];
           tmem_ld_32x16(taddr + j0, a);
@@ -468,50 +483,40 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int i = 0; i < kRows32; i += 4) {
             const ulonglong2 s = *reinterpret_cast<const ulonglong2*>(&sh.x_scale[acc][j0 + i]);
-            scale_pair(a[i], a[i + 1], s.x, w2, v[i], v[i + 1]);
-            scale_pair(a[i + 2], a[i + 3], s.y, w2, v[i + 2], v[i + 3]);
+            scale_pair(a[i], a[i + 1], s.x, ws[0], v[i], v[i + 1]);
+            scale_pair(a[i + 2], a[i + 3], s.y, ws[0], v[i + 2], v[i + 3]);
           }
           if (has_bias) {
 #pragma unroll
-            for (int i = 0; i < kRows32; ++i) v[i] += bias_lane;
+            for (int i = 0; i < kRows32; ++i) v[i] += cur.bias[0];
           }
-          const int64_t row = tl.row0 + j0;
-          float* out = reinterpret_cast<float*>(stg + slot * kSlotBytes) + lane;
-          const bool whole = whole_f32(j0);
-          if (whole && args.tma_residual) {
+          const int nr = c < p.n ? tl.rows - j0 : 0;
+          if (tma_residual && whole_unit(j0)) {
             if (!mbar_wait(&sh.residual[e][slot], (slot_phase >> slot) & 1)) raise_error(p.err, kDevWaitTimeout, 89, t, j0);
             slot_phase ^= 1u << slot;
+            const float* in = reinterpret_cast<const float*>(stg + slot * kSlotBytes) + lane;
 #pragma unroll
-            for (int i = 0; i < kRows32; ++i) v[i] += out[i * 32];
+            for (int i = 0; i < kRows32; ++i) v[i] += in[i * 32];
           } else if (has_residual) {
-            const float* res = static_cast<const float*>(p.residual) + row * p.ldr + cl;
+            const float* res = static_cast<const float*>(p.residual) + (static_cast<int64_t>(tl.row0) + j0) * p.ldr + c;
 #pragma unroll
             for (int i = 0; i < kRows32; ++i)
-              if (cl_ok && i < tl.rows - j0) v[i] += res[i * p.ldr];
+              if (i < nr) v[i] += res[i * p.ldr];
           }
-          if (whole) {
-            if (!args.tma_residual) {
-              if (elect_one()) bulk_wait_read<2>();  // the slot's last store, three units ago, has read it
-              __syncwarp();
-            }
+          char* out = static_cast<char*>(p.y) + ((static_cast<int64_t>(tl.row0) + j0) * p.ldy + c) * 4;
+          if (nr >= kRows32) {
 #pragma unroll
-            for (int i = 0; i < kRows32; ++i) out[i * 32] = v[i];
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (elect_one()) {
-              tma_store_2d(&args.y, static_cast<int>(c0), static_cast<int>(row), stg + slot * kSlotBytes);
-              bulk_commit();
-            }
-          } else if (cl_ok) {
-            float* dst = static_cast<float*>(p.y) + row * p.ldy + cl;
+            for (int i = 0; i < kRows32; ++i, out += pitch) *reinterpret_cast<float*>(out) = v[i];
+          } else {
 #pragma unroll
-            for (int i = 0; i < kRows32; ++i)
-              if (i < tl.rows - j0) dst[i * p.ldy] = v[i];
+            for (int i = 0; i < kRows32; ++i, out += pitch)
+              if (i < nr) *reinterpret_cast<float*>(out) = v[i];
           }
+          __syncwarp();
           slot = next_slot;
         }
         continue;
-      }
+      } else {
       if (way * kUnit >= tl.rows) release();
       for (int j0 = way * kUnit; j0 < tl.rows; j0 += kWays * kUnit) {
         int a[2][16];  // [16 lanes][the four blocks' four values]
@@ -606,6 +611,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
               store_block(v[b], dst + 8 * b * p.ldy, p.ldy, nr - tc - 8 * (first + b), nc);
           }
         }
+      }
       }
     }
     if (elect_one()) bulk_wait_read<0>();
@@ -740,11 +746,11 @@ cudaError_t launch(const W8a8& p, cudaStream_t stream) {
   auto aligned = [](const void* base, int64_t ld) {
     return reinterpret_cast<uintptr_t>(base) % 16 == 0 && ld * (kBf16 ? 2 : 4) % 16 == 0;
   };
-  a.tma_store = (kBf16 || !kGated) && aligned(p.y, p.ldy);
-  a.tma_residual = !kBf16 && !kGated && a.tma_store && p.residual != nullptr && aligned(p.residual, p.ldr);
-  const int box_rows = !kBf16 ? kRows32 : kGated ? kUnit / 2 : kUnit;
-  if (a.tma_store && !make_tile_tmap(&a.y, p.y, kBf16, p.rows, p.n, p.ldy, box_rows)) return cudaErrorInvalidValue;
-  if (a.tma_residual && !make_tile_tmap(&a.residual, p.residual, kBf16, p.rows, p.n, p.ldr, box_rows))
+  a.tma_store = kBf16 && aligned(p.y, p.ldy);
+  a.tma_residual = !kBf16 && !kGated && p.residual != nullptr && aligned(p.residual, p.ldr);
+  if (a.tma_store && !make_tile_tmap(&a.y, p.y, true, p.rows, p.n, p.ldy, kGated ? kUnit / 2 : kUnit))
+    return cudaErrorInvalidValue;
+  if (a.tma_residual && !make_tile_tmap(&a.residual, p.residual, false, p.rows, p.n, p.ldr, kRows32))
     return cudaErrorInvalidValue;
   a.p = p;
   a.channels = kGated ? kBM : 2 * kBM;
