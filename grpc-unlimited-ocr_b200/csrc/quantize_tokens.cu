@@ -7,6 +7,7 @@
 // keeps its part of the row in registers between the maximum and the rounding.
 #include <cfloat>
 
+#include "ptx.cuh"
 #include "w8a8.h"
 
 namespace uocr_b200 {
@@ -114,6 +115,8 @@ __global__ void __launch_bounds__(kThreads) quantize_tokens_kernel(const T* __re
                                                                    int64_t ldx, int8_t* __restrict__ q, int64_t ldq,
                                                                    float* __restrict__ scales) {
   __shared__ uint32_t part[kThreads / 32];
+  pdl_wait();
+  pdl_launch_dependents();
   const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / kPerRow) + threadIdx.x / kPerRow;
   if (kPerRow <= 32 && row >= rows) return;
   if (row >= rows) cols = 0;  // goes along to the barrier
@@ -169,9 +172,9 @@ template <int kPerRow, int kKeep, bool kAligned, typename T>
 cudaError_t launch(const T* x, int64_t rows, int cols, int64_t ldx, int8_t* q, int64_t ldq, float* scales,
                    cudaStream_t stream) {
   constexpr int kRows = kThreads / kPerRow;
-  quantize_tokens_kernel<T, kPerRow, kKeep, kAligned>
-      <<<static_cast<unsigned>((rows + kRows - 1) / kRows), kThreads, 0, stream>>>(x, rows, cols, ldx, q, ldq, scales);
-  return cudaGetLastError();
+  return launch_pdl(quantize_tokens_kernel<T, kPerRow, kKeep, kAligned>,
+                    static_cast<unsigned>((rows + kRows - 1) / kRows), kThreads, 0, stream, x, rows, cols, ldx, q, ldq,
+                    scales);
 }
 
 template <bool kAligned, typename T>

@@ -11,6 +11,25 @@
 
 namespace uocr_b200 {
 
+// Launches a kernel that may start before the previous grid of the stream ends:
+// every thread of it calls pdl_wait before it reads or writes global memory (a
+// block that ended without would let the grid after it overtake the one before).
+template <typename... Params, typename... Args>
+cudaError_t launch_pdl(void (*kernel)(Params...), unsigned grid, unsigned block, size_t smem, cudaStream_t stream,
+                       Args... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, Params(args)...);
+}
+
 // q, scales = int8 rows of x [rows, cols] (fp32 or bf16, pitch ldx) with one
 // scale per row; q rows at pitch ldq, 16-byte aligned.
 cudaError_t launch_quantize_tokens(const void* x, bool bf16, int64_t rows, int64_t cols, int64_t ldx, int8_t* q,

@@ -219,6 +219,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     sh.failed[0] = sh.failed[1] = 0;
     fence_mbar_init();
   }
+  if (warp == 1) tmem_alloc_pair(&sh.tmem, kTmemCols);
+  pdl_wait();  // what precedes it touches nothing that the grid before may be using
+  pdl_launch_dependents();
   if (warp == 0) {
     int carry = 0;
     for (int g0 = 0; g0 < groups; g0 += 32) {
@@ -250,7 +253,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     if (lane == 0) sh.tile_start[groups] = carry;
   }
-  if (warp == 1) tmem_alloc_pair(&sh.tmem, kTmemCols);
   tc_fence_before();
   __syncthreads();
   cluster_barrier();  // both CTAs' barriers exist before either is signalled from the other
@@ -698,6 +700,8 @@ int choose_tokens(int64_t rows, int64_t groups, int c_tiles, int pairs) {
 __global__ void __launch_bounds__(256) gather_rows_kernel(const int8_t* __restrict__ x, int64_t ldx, int64_t x_rows,
                                                           const int* __restrict__ row_index, int rows, int stripes,
                                                           int chunks, uint4* __restrict__ out) {
+  pdl_wait();
+  pdl_launch_dependents();
   const int per = (rows + stripes - 1) / stripes;
   const int lane = threadIdx.x & 31, warps = gridDim.x * (blockDim.x / 32);
   for (int i = blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5); i < per * stripes; i += warps) {
@@ -729,11 +733,10 @@ cudaError_t launch(const W8a8& p, cudaStream_t stream) {
   if (p.row_index != nullptr) {
     ldx = (p.k + 15) / 16 * 16;
     const int64_t blocks = (p.rows + 7) / 8, most = static_cast<int64_t>(pairs) * 2 * 8;
-    gather_rows_kernel<<<static_cast<unsigned>(blocks < most ? blocks : most), 256, 0, stream>>>(
-        p.x, p.ldx, p.x_rows, p.row_index, static_cast<int>(p.rows), static_cast<int>(p.groups),
-        static_cast<int>(ldx / 16),
-        reinterpret_cast<uint4*>(p.workspace));
-    if ((st = cudaGetLastError()) != cudaSuccess) return st;
+    st = launch_pdl(gather_rows_kernel, static_cast<unsigned>(blocks < most ? blocks : most), 256, 0, stream, p.x, p.ldx,
+                    p.x_rows, p.row_index, static_cast<int>(p.rows), static_cast<int>(p.groups),
+                    static_cast<int>(ldx / 16), reinterpret_cast<uint4*>(p.workspace));
+    if (st != cudaSuccess) return st;
     x = p.workspace;
   }
   Args a{};
@@ -760,8 +763,7 @@ cudaError_t launch(const W8a8& p, cudaStream_t stream) {
   const int64_t most =
       (p.rows / a.tokens_per_tile + (p.groups < p.rows ? p.groups : p.rows)) * static_cast<int64_t>(a.c_tiles);
   const unsigned blocks = 2u * static_cast<unsigned>(most < pairs ? most : pairs);
-  w8a8_gemm_kernel<kGated, kBf16><<<blocks, kThreads, kSmem<kGated>, stream>>>(a);
-  return cudaGetLastError();
+  return launch_pdl(w8a8_gemm_kernel<kGated, kBf16>, blocks, kThreads, kSmem<kGated>, stream, a);
 }
 
 }  // namespace

@@ -66,6 +66,8 @@ __global__ void __launch_bounds__(kThreads, kSplit == 8 ? (kGated ? 3 : 2) : 4) 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gr = lane >> 2, tq = lane & 3;
   const int sub = warp / kSplit, split = warp % kSplit;
+  pdl_wait();
+  pdl_launch_dependents();
 
   // A block's group is the one its place among the groups that have rows names.
   const int place = blockIdx.x / n_blocks;
@@ -243,9 +245,8 @@ template <bool kGated, int kTiles, int kSplit, typename T>
 cudaError_t launch(const W8a8& p, int64_t places, cudaStream_t stream) {
   constexpr int kBlockRows = kWarps / kSplit * kRows;
   const int64_t n_blocks = (p.n + kBlockRows - 1) / kBlockRows;
-  w8a8_rows_kernel<kGated, kTiles, kSplit, T>
-      <<<static_cast<unsigned>(places * n_blocks), kThreads, 0, stream>>>(p, static_cast<int>(n_blocks));
-  return cudaGetLastError();
+  return launch_pdl(w8a8_rows_kernel<kGated, kTiles, kSplit, T>, static_cast<unsigned>(places * n_blocks), kThreads, 0,
+                    stream, p, static_cast<int>(n_blocks));
 }
 
 template <bool kGated, typename T>
