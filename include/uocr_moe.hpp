@@ -21,6 +21,7 @@
 #include <string>
 #include <utility>
 
+#include "uocr_int8.h"
 #include "uocr_moe.h"
 
 namespace uocr_b200 {
@@ -86,6 +87,21 @@ inline void linear(void* stream, const float* x, std::int64_t m, std::int64_t k,
 }
 
 // ---- owners ------------------------------------------------------------------
+
+// The 8-bit integer operators (uocr_int8.h) on the stream, with the same exceptions.
+inline void quantize_tokens(void* stream, const void* x, uocr_dtype dtype, std::int64_t rows, std::int64_t cols,
+                            std::int64_t ldx, std::int8_t* q, std::int64_t ldq, float* scales) {
+  check(uocr_quantize_tokens(x, dtype, rows, cols, ldx, q, ldq, scales, stream));
+}
+inline void linear_w8a8(void* stream, const uocr_linear_w8a8_args& args) { check(uocr_linear_w8a8(&args, stream)); }
+inline std::int64_t grouped_w8a8_workspace(const uocr_grouped_w8a8_args& args) {
+  std::int64_t bytes = 0;
+  check(uocr_grouped_w8a8_workspace(&args, &bytes));
+  return bytes;
+}
+inline void grouped_linear_w8a8(void* stream, const uocr_grouped_w8a8_args& args) {
+  check(uocr_grouped_linear_w8a8(&args, stream));
+}
 
 class Checkpoint;
 

@@ -135,6 +135,37 @@ def test_binding_refuses_wrong_tensors():
         M.quantize_tokens(torch.zeros(2, 16, dtype=torch.float16), x, s)
 
 
+def test_cpp_wrapper(tmp_path):
+    """The header-only C++ layer's int8 functions: the library's refusals as std::invalid_argument."""
+    cxx = shutil.which("g++")
+    if cxx is None:
+        pytest.skip("no C++ compiler")
+    src = tmp_path / "int8.cpp"
+    src.write_text(r"""
+#include <cstdio>
+#include "uocr_moe.hpp"
+template <typename F> static int throws(F&& f) {
+  try { f(); } catch (const std::invalid_argument&) { return 1; }
+  return 0;
+}
+int main() {
+  uocr_linear_w8a8_args l{};
+  l.m = l.n = 1;
+  uocr_grouped_w8a8_args g{};
+  g.rows = 4096, g.n = 1, g.k = 100, g.groups = 4, g.row_index = reinterpret_cast<const int32_t*>(16);
+  std::printf("%d %d %d %lld\n", throws([&] { uocr_b200::linear_w8a8(nullptr, l); }),
+              throws([&] { uocr_b200::grouped_linear_w8a8(nullptr, g); }),
+              throws([&] { uocr_b200::quantize_tokens(nullptr, nullptr, UOCR_DTYPE_I32, 1, 1, 1, nullptr, 16, nullptr); }),
+              static_cast<long long>(uocr_b200::grouped_w8a8_workspace(g)));
+}
+""")
+    exe = tmp_path / "int8"
+    lib = os.path.dirname(M.LIB_PATH)
+    subprocess.run([cxx, "-std=c++17", "-I", INCLUDE, str(src), "-o", str(exe), M.LIB_PATH, f"-Wl,-rpath,{lib}"], check=True)
+    out = subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()
+    assert out == ["1", "1", "1", str(4096 * 112)]
+
+
 def test_int8_activations_need_int8_weights():
     plan = M.MoeDesc(256, 8, 2, 128, 128, 1, 32, M.WEIGHT_BF16, 1, 0, 0, M.PLAN_INT8_ACTIVATIONS)
     h = ctypes.c_void_p()
