@@ -504,18 +504,28 @@ def linear_w8a8(x, x_scales, w, w_scales, y, bias=None, residual=None, stream=No
     """y[m, n] = x[m, k] . w[n, k]^T in int8 with x_scales per row of x and w_scales per row of w (+ bias[n])
     (+ residual[m, n], of y's dtype; may be y itself) (uocr_linear_w8a8)."""
     import torch
-    f32 = torch.float32
+    f32, i8 = torch.float32, torch.int8
     m, k = x.shape
     n = w.shape[0]
+    (ldx, sx), (ldw, sw), (ldy, sy) = x.stride(), w.stride(), y.stride()
+    # The common case in one expression (this call is microseconds of device time); else what is wrong, or a lone column.
+    if not (n > 1 and sx == sw == sy == 1 and w.shape[1] == k and y.shape == (m, n) and x.dtype is i8
+            and w.dtype is i8 and x.is_cuda and w.is_cuda and y.is_cuda):
+        ldx, ldw, ldy = _pitch_i8(x, "x", m, k), _pitch_i8(w, "w", n, k), _pitch(y, "y", m, n)
+    elif m == 1:
+        ldx, ldy = (k + 15) // 16 * 16, n
+    if not (x_scales.dtype is f32 and w_scales.dtype is f32 and x_scales.numel() == m and w_scales.numel() == n
+            and x_scales.is_contiguous() and w_scales.is_contiguous() and x_scales.is_cuda and w_scales.is_cuda):
+        _vector(x_scales, "x_scales", m, f32), _vector(w_scales, "w_scales", n, f32)
     ldr = res = None
     if residual is not None:
         if residual.dtype is not y.dtype:
             raise ValueError("residual must have y's dtype")
         res, ldr = residual.data_ptr(), _pitch(residual, "residual", m, n)
     args = LinearW8A8Args(
-        x.data_ptr(), _vector(x_scales, "x_scales", m, f32), w.data_ptr(), _vector(w_scales, "w_scales", n, f32),
-        None if bias is None else _vector(bias, "bias", n, f32), res, y.data_ptr(), m, n, k,
-        _pitch_i8(x, "x", m, k), _pitch_i8(w, "w", n, k), ldr or 0, _pitch(y, "y", m, n), _float_dtype(y, "y"), 0)
+        x.data_ptr(), x_scales.data_ptr(), w.data_ptr(), w_scales.data_ptr(),
+        None if bias is None else _vector(bias, "bias", n, f32), res, y.data_ptr(), m, n, k, ldx, ldw, ldr or 0, ldy,
+        _float_dtype(y, "y"), 0)
     _check(lib().uocr_linear_w8a8(ctypes.byref(args), _stream(stream)))
 
 
@@ -543,11 +553,24 @@ def grouped_linear_w8a8(x, x_scales, w, w_scales, offsets, y, row_index=None, w_
     [groups * n, k]; w_scales: groups * n values; offsets, row_index: int32. Where the call needs a workspace it
     comes from torch's allocator."""
     import torch
-    f32, i32 = torch.float32, torch.int32
+    f32, i32, i8 = torch.float32, torch.int32, torch.int8
     x_rows, k = x.shape
     rows, n = y.shape
     groups = offsets.numel() - 1
+    (ldx, sx), (ldy, sy) = x.stride(), y.stride()
+    if not (n > 1 and sx == sy == 1 and x.dtype is i8 and x.is_cuda and y.is_cuda):
+        ldx, ldy = _pitch_i8(x, "x", x_rows, k), _pitch(y, "y", rows, n)
+    else:
+        if x_rows == 1:
+            ldx = (k + 15) // 16 * 16
+        if rows == 1:
+            ldy = n
     ldw = _stack_pitch(w, "w", groups, n, k)
+    if not (x_scales.dtype is f32 and w_scales.dtype is f32 and offsets.dtype is i32 and x_scales.numel() == x_rows
+            and w_scales.numel() == groups * n and x_scales.is_contiguous() and w_scales.is_contiguous()
+            and offsets.is_contiguous() and x_scales.is_cuda and w_scales.is_cuda and offsets.is_cuda):
+        _vector(x_scales, "x_scales", x_rows, f32), _vector(w_scales, "w_scales", groups * n, f32)
+        _vector(offsets, "offsets", groups + 1, i32)
     up = up_scales = index = None
     if w_up is not None:
         if _stack_pitch(w_up, "w_up", groups, n, k) != ldw:
@@ -556,10 +579,8 @@ def grouped_linear_w8a8(x, x_scales, w, w_scales, offsets, y, row_index=None, w_
     if row_index is not None:
         index = _vector(row_index, "row_index", rows, i32)
     args = GroupedW8A8Args(
-        x.data_ptr(), _vector(x_scales, "x_scales", x_rows, f32), index,
-        _vector(offsets, "offsets", groups + 1, i32), w.data_ptr(), _vector(w_scales, "w_scales", groups * n, f32),
-        up, up_scales, y.data_ptr(), rows, x_rows, groups, n, k, _pitch_i8(x, "x", x_rows, k), ldw,
-        _pitch(y, "y", rows, n), _float_dtype(y, "y"), 0, None, 0)
+        x.data_ptr(), x_scales.data_ptr(), index, offsets.data_ptr(), w.data_ptr(), w_scales.data_ptr(), up, up_scales,
+        y.data_ptr(), rows, x_rows, groups, n, k, ldx, ldw, ldy, _float_dtype(y, "y"), 0, None, 0)
     if index is not None:
         need = ctypes.c_int64()
         _check(lib().uocr_grouped_w8a8_workspace(ctypes.byref(args), ctypes.byref(need)))

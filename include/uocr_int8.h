@@ -12,8 +12,8 @@
  * void*, status codes with uocr_last_error(), nothing synchronises the stream
  * and nothing is allocated. Rows are row-major with a pitch ("ld") counted in
  * elements. An int8 row starts at a 16-byte boundary: base pointers 16-byte
- * aligned and int8 pitches a multiple of 16. Its width is free: the bytes between the width
- * and the pitch are never used (they may be read).
+ * aligned and int8 pitches a multiple of 16. Its width is free: the bytes from
+ * the width up to the next multiple of 16 may be read, and are not used.
  */
 #ifndef UOCR_INT8_H
 #define UOCR_INT8_H

@@ -399,3 +399,26 @@ def test_binding_refuses_wrong_shapes(cuda):
                  lambda: M.quantize_tokens(x.float(), x, ws)):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.parametrize("rows,n,k", [(1, 1, 5), (1, 33, 40), (4, 1, 16), (3, 2, 1), (300, 1, 33)])
+def test_lone_rows_and_columns(cuda, rows, n, k):
+    """Single rows and columns, whose strides say nothing: plain, and grouped in either layout of the weights."""
+    import torch
+    g = gen_of(rows, n, k)
+    x, w, xs, ws = ints(g, rows, k), ints(g, n, k), scales(g, rows), scales(g, n)
+    want = (x.double() @ w.double().T) * xs.double()[:, None] * ws.double()
+    y = torch.empty(rows, n, device="cuda")
+    M.linear_w8a8(x, xs, w, ws, y)
+    check(y, want, want.abs(), False)
+    off = torch.tensor([0, rows], dtype=torch.int32, device="cuda")
+    for stack in (w, torch.as_strided(w, (1, n, k), (n * w.stride(0), w.stride(0), 1))):
+        z = torch.empty(rows, n, device="cuda")
+        M.grouped_linear_w8a8(x, xs, stack, ws, off, z)
+        assert torch.equal(y, z)
+    two = ints(g, 2 * n, k)
+    off = torch.tensor([0, rows, rows], dtype=torch.int32, device="cuda")
+    z = torch.empty(rows, n, device="cuda")
+    M.grouped_linear_w8a8(x, xs, torch.as_strided(two, (2, n, k), (n * two.stride(0), two.stride(0), 1)),
+                          scales(g, 2 * n), off, z)
+    M.ops_check()
