@@ -33,6 +33,7 @@
 // With few slices of K the copies bound it, at 55 bytes a clock into each SM:
 // at 8192 x 8192 x 1024 the MMAs alone take 57 kcycles, the copies alone 67, all
 // but the stores 81, the whole 91.
+#include <algorithm>
 #include <mutex>
 #include <type_traits>
 
@@ -670,23 +671,31 @@ cudaError_t resident_pairs(int* pairs) {
   return cudaSuccess;
 }
 
-// Tokens per tile: as many as fit where there are tiles enough for the pairs.
-// A narrower MMA costs less, down to 64 tokens, so where the tiles are few
-// (one wave or a broken one) the width that ends first is taken.
+// Tokens per tile: the width that ends first; of equals the widest, or in a
+// single wave the narrowest, which spreads the larger groups over idle pairs
+// (154 rows in 16 uneven groups 6.3 us at 64, 7.2 at 256). A pair's
+// time for a slice of K is its copies', 128 weight rows and half of the tokens
+// in each SM, so a tile of n tokens costs n + 256 and the tiles come in waves.
+// Measured in us, the width taken against 256: dense, 64 x 2048 x 2048 7.4 / 8.1
+// (32); 200 rows 8.2 / 10.6 (32); 500 x 4096 x 2048 8.5 / 10.5 (128); 3000 x 2048
+// x 2048 14.8 / 15.8 (192); 4096 x 2048 x 2048 stays at 256: 20.0, at 160 21.3.
+// Groups' sizes are known on the device only: as if even, half a tile of each
+// lost, and halved widths alone, since a narrower guess that breaks a group
+// once more costs a wave. 2 groups of 200 rows, 2048 x 1024: 7.1 / 8.3 (64); 4
+// of 128 gated stay at 256: 12.3, at 64 16.0; 8 of 150 8.4, at 128 10.1.
 int choose_tokens(int64_t rows, int64_t groups, int c_tiles, int pairs) {
-  constexpr int most = kMaxN;
-  if (groups > 1) {
-    int bn = most;
-    while (bn > 64 && (rows / bn + (groups < rows ? groups : rows) / 2) * c_tiles < pairs) bn /= 2;
-    return bn;
-  }
-  int best = most;
+  const int64_t parts = groups < rows ? groups : rows, even = (rows + parts - 1) / parts;
+  const int narrowest = groups > 1 ? 64 : 32;
+  int best = kMaxN;
   int64_t best_cost = INT64_MAX;
-  for (int bn = most; bn >= 32; bn -= 32) {
-    const int64_t r = (rows + bn - 1) / bn;
-    const int64_t per = ((rows + r - 1) / r + 31) / 32 * 32;
-    const int64_t cost = ((r * c_tiles + pairs - 1) / pairs) * ((per > 64 ? per : 64) + 16);
-    if (cost < best_cost) {
+  for (int bn = kMaxN; bn >= narrowest; bn = groups > 1 ? bn / 2 : bn - 32) {
+    int64_t tiles = (rows + bn - 1) / bn, width = (rows + tiles - 1) / tiles;
+    if (groups > 1) {
+      tiles = std::max(parts, rows / bn + parts / 2);
+      width = std::min<int64_t>(bn, even);
+    }
+    const int64_t waves = (tiles * c_tiles + pairs - 1) / pairs, cost = waves * ((width + 31) / 32 * 32 + 256);
+    if (cost < best_cost || (cost == best_cost && waves == 1)) {
       best_cost = cost;
       best = bn;
     }
@@ -773,18 +782,20 @@ cudaError_t launch(const W8a8& p, cudaStream_t stream) {
 }  // namespace
 
 namespace {
-// Which kernel: w8a8_rows.cu reads the weights once per 8 rows (dense: 16) of a
-// group, with little to set up; the kernel above takes 7.5 us or more. Measured
-// in us, rows against this one: dense 2048 x 2048 1 row 3.1 / 8.2, 16 rows 4.5
-// / 8.2; 8192 x 2048 16 rows 7.8 / 8.3; 16384 x 2048 8 rows 9.4 / 10.4, 16 rows
-// 13.8 / 10.5; 102400 x 2048 1 row 36 / 39. 64 groups of 2 x 1024 x 2048 gated:
-// 6 rows 8.2 / 11.7, 60 rows 38 / 37, 240 rows 47 / 52; of 2048 x 1024: 6 rows
-// 6.3 / 7.9, 96 rows 23 / 24, 240 rows 30 / 28. 16 groups of 1024 x 2048, 128
-// rows: 14.8 / 11.5.
+// Which kernel: w8a8_rows.cu reads the weights once per 8 rows (dense: up to 32)
+// of a group, with little to set up; the kernel above takes 5.6 us or more.
+// Measured in us, rows against this one. Dense, n x k: 1 row 2048 x 2048 2.9 / 7.2,
+// 102400 x 2048 36 / 39; 8 rows 8192 x 2048 6.1 / 7.4; 16 rows 2048 x 2048 4.1 /
+// 7.2, 4096 x 1024 4.1 / 5.7, 4096 x 8192 14.7 / 18.2, 8192 x 1024 7.2 / 5.8, 8192
+// x 2048 8.3 / 7.4; 32 rows 1000 x 1000 4.8 / 6.2, 2048 x 2048 6.4 / 7.4, 4096 x
+// 2048 7.2 / 7.4, 2048 x 8192 21 / 17. Groups: 64 of 2 x 1024 x 2048 gated, 6
+// rows 7.6 / 12.1, 60 rows 37 / 38, 240 rows 46 / 52; 64 of 2048 x 1024, 6 rows
+// 6.2 / 9.7, 96 rows 23.5 / 25.7, 240 rows 30.5 / 29.7; 16 of 1024 x 2048, 32
+// rows 9.7 / 11.5, 128 rows 14.8 / 11.5; 8 of those, 30 rows 7.7 / 9.8, 60 9.8 / 9.9.
 bool few_rows_grouped(int64_t rows, int64_t groups) { return rows <= 256 && rows <= 4 * groups; }
 bool few_rows(const W8a8& p) {
   if (p.starts != nullptr) return few_rows_grouped(p.rows, p.groups);
-  return p.rows <= 8 || (p.rows <= 16 && p.n * p.k <= (int64_t{1} << 24));
+  return p.rows <= 8 || (p.n <= 4096 && (p.rows <= 16 || (p.rows <= 32 && p.k <= 2048)));
 }
 }  // namespace
 

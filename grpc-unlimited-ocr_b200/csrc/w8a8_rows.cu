@@ -11,7 +11,7 @@
 //
 // Bound by the weights' bytes where they are many, else by the latency of one
 // pass: start, offsets, row indices, loads, one exchange, store. K is split
-// over as many warps (up to 8) as it takes to give the device about 4000.
+// over as many warps (up to 8) as the device holds beside each other (choose).
 #include "ptx.cuh"
 #include "w8a8.h"
 
@@ -60,7 +60,7 @@ __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bf
 template <bool kGated, int kTiles, int kSplit, typename T>
 __global__ void __launch_bounds__(kThreads, kSplit == 8 ? (kGated ? 3 : 2) : 4) w8a8_rows_kernel(const W8a8 p, int n_blocks) {
   constexpr int kMats = kGated ? 2 : 1;
-  constexpr int kDeep = (kSplit == 8 ? 4 : 2) / kMats;  // steps in flight
+  constexpr int kDeep = (kSplit == 8 && kTiles < 4 ? 4 : 2) / kMats;  // steps in flight (as many as registers hold)
   __shared__ int part[kWarps][kMats * kTiles][32][4];
   __shared__ int s_first, s_count, s_group, s_has[kWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -254,10 +254,21 @@ cudaError_t choose(const W8a8& p, cudaStream_t stream) {
   // Groups that can have rows, and the warps that take all of K.
   const int64_t places = p.starts == nullptr ? 1 : p.groups < p.rows ? p.groups : p.rows;
   const int64_t warps = places * ((p.n + kRows - 1) / kRows);
-  // Groups mostly have a row or two each; a dense product's 16 tokens are taken in one pass.
-  if (p.starts == nullptr && p.rows > 8) return launch<kGated, 2, 8, T>(p, places, stream);
+  // Groups mostly have a row or two each; a dense product's rows are taken in one
+  // pass (16 by 2048 x 2048 4.3 us, in passes of 8 5.0; by 8192 x 2048 8.3 and
+  // 10.9; 24 by 2048 x 1024 3.9, in passes of 16 5.6).
+  if constexpr (!kGated) {
+    if (p.rows > 16 && p.starts == nullptr) return launch<kGated, 4, 8, T>(p, places, stream);
+    if (p.rows > 8 && p.starts == nullptr) return launch<kGated, 2, 8, T>(p, places, stream);
+  }
+  // Measured in us by 8, 4 and 2 warps for 16 rows' K: 1 row by 2048 x 2048 2.9,
+  // 4.9, 7.0; 8192 x 2048 5.7, 5.9, 8.4; 12000 x 2048 8.3, 7.7, 9.7; 16384 x 2048
+  // 10.7, 8.3, 10.5; 20000 x 2048 12.2, 12.5, 11.4; 102400 x 2048 46, 38, 36; 96
+  // rows of 64 groups of 2048 x 1024 58, 28, 23. Gated (twice the loads a warp)
+  // of 64 groups of 2 x 1024 x 2048: 6 rows 7.7, 9.8, 14.0; 18 rows 17.4, 15.1,
+  // 18.5; 24 rows 20.0, 19.5, 21.1; 30 rows 23.4, 22.9, 22.2.
   if (warps <= 512) return launch<kGated, 1, 8, T>(p, places, stream);
-  if (warps <= 1024) return launch<kGated, 1, 4, T>(p, places, stream);
+  if (warps <= (kGated ? 1536 : 1024)) return launch<kGated, 1, 4, T>(p, places, stream);
   return launch<kGated, 1, 2, T>(p, places, stream);
 }
 
