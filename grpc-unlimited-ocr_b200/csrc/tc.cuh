@@ -48,11 +48,17 @@ __device__ __forceinline__ void prefetch_tmap(const CUtensorMap* map) {
 // MMAs for both, each CTA stages its half of the operands in its own shared
 // memory, and the copies of both report to the leader's mbarrier.
 
-// The leader's copy of a shared-memory object, as a cluster address.
-__device__ __forceinline__ uint32_t pair_leader_addr(const void* p) {
+// A CTA's copy of a shared-memory object, as a cluster address.
+__device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
   uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr(p)), "r"(0));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr(p)), "r"(rank));
   return r;
+}
+
+// 16 bytes to the shared memory of a CTA of the cluster (a cluster_addr, 16-byte aligned).
+__device__ __forceinline__ void st_cluster_v4(uint32_t addr, int a, int b, int c, int d) {
+  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
+               : "memory");
 }
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -66,7 +72,7 @@ __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// A box at (c0, c1) into this CTA; completes on the leader's mbarrier `bar` (a pair_leader_addr).
+// A box at (c0, c1) into this CTA; completes on the leader's mbarrier `bar` (its cluster_addr).
 __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
@@ -75,7 +81,7 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* m
       : "memory");
 }
 
-// One arrival on the leader's mbarrier `bar` (a pair_leader_addr) from either
+// One arrival on the leader's mbarrier `bar` (its cluster_addr) from either
 // CTA. Release at CTA scope: what it announces is that TMEM has been read
 // (tcgen05.wait::ld, tcgen05.fence); a release at cluster scope would first
 // wait for the thread's global stores to be performed.
@@ -118,12 +124,12 @@ __device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint64_t a_desc, u
       : "memory");
 }
 
-// Arrives once on `bar` of both CTAs of the pair when every MMA this thread issued so far has completed.
-__device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
+// Arrives once on `bar` of both CTAs of the pair (ranks leader, leader + 1) when every MMA this thread issued so far has completed.
+__device__ __forceinline__ void umma_commit_pair(uint64_t* bar, uint32_t leader) {
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
           smem_addr(bar)),
-      "h"(static_cast<uint16_t>(3))
+      "h"(static_cast<uint16_t>(3u << leader))
       : "memory");
 }
 

@@ -9,7 +9,8 @@
 // are output channels, or in the gated form the gate and up rows of 128
 // channels, 64 and 64 in each SM.
 //
-// One persistent pair of blocks per two SMs, warp-specialised:
+// One persistent pair of blocks per two SMs (K in parts: a cluster of pairs a
+// tile), warp-specialised:
 //   warps 0, 2  producers, one lane each, per 128-byte slice of K: warp 0 the
 //              CTA's 128 weight rows, warp 2 its half of the token rows (boxes
 //              of 128, 64 or 16 rows);
@@ -20,6 +21,10 @@
 //              (gated: sectors of 8), a residual arriving by TMA a unit ahead.
 //              When gated, the gate's warp and the up's warp of the same
 //              channels exchange half of their tokens first.
+// A dense product of few tiles and a long K has K in two or four parts, a pair
+// for each in one cluster: a slice of K takes 0.19 us whether one pair is at work
+// or all, since a pair waits for its own copies. The int32 sums, exact in any
+// order, meet in shared memory (64 x 2048 x 8192: 9.7 us, by one pair a tile 16.7).
 // Rows named by an index are first copied together (gather_rows_kernel): TMA
 // gathers four rows of 128 bytes at a time, 44 clocks each, against 512 clocks
 // of MMAs for 32 of them (1108 us at eight pages' gate/up, 649 us without the
@@ -197,8 +202,9 @@ __device__ __forceinline__ void load_block(Block& v, const T* base, int64_t ld, 
     for (int q = 0; q < 4; ++q) v[2 * q + e] = e < nr && 8 * q < nc ? to_f32(base[e * ld + 8 * q]) : 0.0f;
 }
 
-template <bool kGated, bool kBf16>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+// kS: pairs of a cluster, which share a tile's K; above 1 a cluster has one tile.
+template <bool kGated, bool kBf16, int kS>
+__global__ void __cluster_dims__(2 * kS, 1, 1) __launch_bounds__(kThreads, 1)
     w8a8_gemm_kernel(const __grid_constant__ Args args) {
   extern __shared__ unsigned char dyn_raw[];
   __shared__ Shared sh;
@@ -206,7 +212,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(dyn_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const W8a8& p = args.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = static_cast<int>(cluster_rank());
+  const int rank = static_cast<int>(cluster_rank() & 1u), part = static_cast<int>(cluster_rank() >> 1);
+  const uint32_t leader = kS > 1 ? cluster_rank() & ~1u : 0u;
+  const int pair0 = static_cast<int>(blockIdx.x) / (2 * kS);
   const int groups = static_cast<int>(p.groups);
 
   if (threadIdx.x == 0) {
@@ -264,19 +272,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem_base = sh.tmem;
   const int total = sh.tile_start[groups];
-  const int step = gridDim.x / 2;
+  const int step = static_cast<int>(gridDim.x) / (2 * kS);
+  const int kb0 = kS > 1 ? part * args.k_blocks / kS : 0;
+  const int kb1 = kS > 1 ? (part + 1) * args.k_blocks / kS : args.k_blocks;
 
   // One lane's pass over this pair's tiles, body(tile, n) for the n-th; the
   // warp works 32 of them out at a time, a lane each (one takes some 1000
   // clocks, which between two tiles would leave the MMAs waiting).
   auto each_tile = [&](Tile* table, auto&& body) {
     bool ok = true;
-    for (int n0 = 0; ok && blockIdx.x / 2 + n0 * step < total; n0 += 32) {
-      const int mine = blockIdx.x / 2 + (n0 + lane) * step;
+    for (int n0 = 0; ok && pair0 + n0 * step < total; n0 += 32) {
+      const int mine = pair0 + (n0 + lane) * step;
       if (mine < total) table[lane] = decode_tile(mine, sh, groups, args);
       __syncwarp();
       if (elect_one())
-        for (int i = 0; i < 32 && ok && blockIdx.x / 2 + (n0 + i) * step < total; ++i) ok = body(table[i], n0 + i);
+        for (int i = 0; i < 32 && ok && pair0 + (n0 + i) * step < total; ++i) ok = body(table[i], n0 + i);
       ok = __all_sync(0xffffffffu, ok);
     }
     return ok;
@@ -284,13 +294,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
   if (warp == 0) {
     // ---- weight producer: one lane; the leader also announces both CTAs' bytes of a stage ----
-    const uint32_t full0 = pair_leader_addr(&sh.full[0]);
+    const uint32_t full0 = cluster_addr(&sh.full[0], leader);
     int stage = 0;
     uint32_t phase = 0;
     const bool ok = each_tile(sh.tiles[0], [&](const Tile& tl, int) {
       const uint32_t bytes = 2 * kABytes + round32(tl.rows) * kBK;
       const int w_row = tl.g * static_cast<int>(p.n) + tl.c0 + rank * (args.channels / 2);
-      for (int kb = 0; kb < args.k_blocks; ++kb) {
+      for (int kb = kb0; kb < kb1; ++kb) {
         if (!mbar_wait(&sh.empty[stage], phase ^ 1)) {
           raise_error(p.err, kDevWaitTimeout, 82, tl.row0, kb);
           return false;
@@ -309,13 +319,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     if (!ok) wait_for_copies();
   } else if (warp == 2) {
     // ---- token producer: one lane ----
-    const uint32_t full0 = pair_leader_addr(&sh.full[0]);
+    const uint32_t full0 = cluster_addr(&sh.full[0], leader);
     int stage = 0;
     uint32_t phase = 0;
     const bool ok = each_tile(sh.tiles[1], [&](const Tile& tl, int) {
       const int half = round32(tl.rows) / 2;
       const int row = tl.row0 + rank * half;  // this CTA's first token row
-      for (int kb = 0; kb < args.k_blocks; ++kb) {
+      for (int kb = kb0; kb < kb1; ++kb) {
         if (!mbar_wait(&sh.empty[stage], phase ^ 1)) {
           raise_error(p.err, kDevWaitTimeout, 87, tl.row0, kb);
           return false;
@@ -354,7 +364,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
         tc_fence_after();
         const uint32_t d = tmem_base + static_cast<uint32_t>(acc * kMaxN);
-        for (int kb = 0; kb < args.k_blocks; ++kb) {
+        for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait(&sh.full[stage], phase)) {
             raise_error(p.err, kDevWaitTimeout, 84, tl.row0, kb);
             return false;
@@ -365,18 +375,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           const uint64_t bd = sw128_kmajor_desc(sa + kABytes);
 #pragma unroll
           for (int k = 0; k < kBK / 32; ++k)  // 32 bytes of K per instruction: +2 in the address field
-            umma_i8_pair(d, ad + 2 * k, bd + 2 * k, idesc, (kb | k) != 0 ? 1u : 0u);
-          umma_commit_pair(&sh.empty[stage]);
+            umma_i8_pair(d, ad + 2 * k, bd + 2 * k, idesc, ((kb - kb0) | k) != 0 ? 1u : 0u);
+          umma_commit_pair(&sh.empty[stage], leader);
           if (++stage == kStages) {
             stage = 0;
             phase ^= 1;
           }
         }
-        umma_commit_pair(&sh.acc_full[acc]);
+        umma_commit_pair(&sh.acc_full[acc], leader);
         return true;
       });
       if (elect_one()) {  // the lane that issued: every MMA is complete before shared memory and TMEM are given up
-        umma_commit_pair(&sh.drain);
+        umma_commit_pair(&sh.drain, leader);
         if (!mbar_wait(&sh.drain, 0)) raise_error(p.err, kDevWaitTimeout, 85, 0, 0);
       }
     }
@@ -399,6 +409,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     T* y = static_cast<T*>(p.y);
     const bool has_bias = !kGated && p.bias != nullptr, has_residual = !kGated && p.residual != nullptr;
     const bool tma_residual = kLaneIsChannel && args.tma_residual;
+    // K in parts: which pair finishes a unit, and where in its shared memory
+    // another's (the src-th of the others') sums of it go, this lane's part of
+    // this warp's: 16 bytes at a pitch of 512.
+    constexpr int kPart = kLaneIsChannel ? kRows32 : kUnit;
+    auto owner = [&](int unit) { return kS == 2 ? (unit >> 1) & 1 : unit % kS; };
+    auto part_sums = [&](int unit, int src) {
+      const int place = kS == 2 ? (unit >> 2) * 2 + (unit & 1) : unit / kS;
+      return smem + ((place * (kS - 1) + src) * 4 + quarter) * (kPart * 128) + lane * 16;
+    };
     // What the epilogue needs of a tile beside its sums; the next tile's is
     // fetched while this one's units are stored.
     struct Scales {
@@ -410,8 +429,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // row, which a tile's epilogue has not got).
     Tile lane_tile{};
     auto fetch = [&](int nth) {
-      if ((nth & 31) == 0 && blockIdx.x / 2 + (nth + lane) * step < total)
-        lane_tile = decode_tile(blockIdx.x / 2 + (nth + lane) * step, sh, groups, args);
+      if ((nth & 31) == 0 && pair0 + (nth + lane) * step < total)
+        lane_tile = decode_tile(pair0 + (nth + lane) * step, sh, groups, args);
       Scales f{};
       f.tl = Tile{__shfl_sync(0xffffffffu, lane_tile.g, nth & 31), __shfl_sync(0xffffffffu, lane_tile.row0, nth & 31),
                   __shfl_sync(0xffffffffu, lane_tile.rows, nth & 31), __shfl_sync(0xffffffffu, lane_tile.c0, nth & 31)};
@@ -438,11 +457,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       return f;
     };
     Scales next{};
-    if (blockIdx.x / 2 < total) next = fetch(0);
+    if (pair0 < total) next = fetch(0);
     int local = 0, buf = 0, slot = 0;
     uint32_t slot_phase = 0;
     bool ok = true;
-    for (int t = blockIdx.x / 2; t < total; t += step, ++local) {
+    for (int t = pair0; t < total; t += step, ++local) {
       const Scales cur = next;
       const Tile& tl = cur.tl;
       const int acc = local & 1;
@@ -467,24 +486,65 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (!ok && lane == 0) sh.failed[acc] = 1;
       named_bar_sync(1, kEpilogueWarps * 32);  // the scales are there; and all warps go on with this tile or none
       ok = sh.failed[acc] == 0;
+      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * kMaxN);
+      if constexpr (kS > 1) {
+        // The pairs' sums over their parts of K: each finishes some units, and
+        // has the others' sums of those brought to where its operands were.
+        cluster_barrier();  // every pair's MMAs are complete: no operand is in use any more
+        if (ok) {
+          tc_fence_after();
+          for (int j0 = way * kPart; j0 < tl.rows; j0 += kWays * kPart) {
+            const int to = owner(j0 / kPart);
+            if (to == part) continue;
+            int a[kPart];
+            if constexpr (kLaneIsChannel) {
+              tmem_ld_32x16(taddr + j0, a);
+            } else {
+              int b[2][16];
+              tmem_ld_16x32(taddr + j0, b[0]);
+              tmem_ld_16x32(taddr + (16u << 16) + j0, b[1]);
+              tmem_ld_wait(b[0], b[1]);
+#pragma unroll
+              for (int i = 0; i < kPart; ++i) a[i] = b[i / 16][i % 16];
+            }
+            const uint32_t dst = cluster_addr(part_sums(j0 / kPart, part - (part > to ? 1 : 0)), 2 * to + rank);
+#pragma unroll
+            for (int i = 0; i < kPart; i += 4) st_cluster_v4(dst + i * 128, a[i], a[i + 1], a[i + 2], a[i + 3]);
+          }
+        }
+        cluster_barrier();
+      }
       if (!ok) continue;
       tc_fence_after();
-      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * kMaxN);
+      // The other pairs' sums of a unit of this one, added to its own.
+      auto add_parts = [&](int unit, int* a, int first, int n) {
+        for (int src = 0; src < kS - 1; ++src) {
+          const int4* in = reinterpret_cast<const int4*>(part_sums(unit, src)) + first / 4 * 32;
+#pragma unroll
+          for (int i = 0; i < n / 4; ++i) {
+            const int4 v = in[i * 32];
+            a[4 * i] += v.x, a[4 * i + 1] += v.y, a[4 * i + 2] += v.z, a[4 * i + 3] += v.w;
+          }
+        }
+      };
       auto release = [&] {  // this warp has read its last columns: the accumulator may be written again
+        if (kS > 1) return;  // there is no further tile
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_pair(pair_leader_addr(&sh.acc_empty[acc]));
+        if (lane == 0) mbar_arrive_pair(cluster_addr(&sh.acc_empty[acc], leader));
       };
       if (t + step < total) next = fetch(local + 1);
       if constexpr (kLaneIsChannel) {
         const int64_t pitch = p.ldy * 4;
         if (way * kRows32 >= tl.rows) release();
         for (int j0 = way * kRows32; j0 < tl.rows; j0 += kWays * kRows32) {
+          if (kS > 1 && owner(j0 / kPart) != part) continue;
           const int next_slot = slot ^ 1;
           // (The slot's values, two units ago, have been read by the whole warp.)
           fetch_residual(j0 + kWays * kRows32, next_slot);
           int a[kRows32];
           tmem_ld_32x16(taddr + j0, a);
+          if constexpr (kS > 1) add_parts(j0 / kPart, a, 0, kRows32);
           if (j0 + kWays * kRows32 >= tl.rows) release();
           float v[kRows32];
 #pragma unroll
@@ -526,12 +586,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       } else {
       if (way * kUnit >= tl.rows) release();
       for (int j0 = way * kUnit; j0 < tl.rows; j0 += kWays * kUnit) {
+        if (kS > 1 && owner(j0 / kPart) != part) continue;
         int a[2][16];  // [16 lanes][the four blocks' four values]
         tmem_ld_16x32(taddr + j0, a[0]);
         tmem_ld_16x32(taddr + (16u << 16) + j0, a[1]);
         const int64_t row = tl.row0 + j0;
         const int nr = tl.rows - j0;
         tmem_ld_wait(a[0], a[1]);
+        if constexpr (kS > 1) {
+          add_parts(j0 / kPart, a[0], 0, 16);
+          add_parts(j0 / kPart, a[1], 16, 16);
+        }
         if (j0 + kWays * kUnit >= tl.rows) release();
         buf ^= 1;
         const bool whole = nr >= kUnit && c0 + 32 <= p.n;
@@ -624,6 +689,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     if (elect_one()) bulk_wait_read<0>();
   }
   __syncwarp();
+  if (kS > 1 && warp < 4) {  // the epilogue's two meetings
+    cluster_barrier();
+    cluster_barrier();
+  }
   tc_fence_before();
   __syncthreads();
   cluster_barrier();  // the pair's MMAs are complete: no operand, accumulator or barrier is in use any more
@@ -635,9 +704,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   cluster_barrier();
 }
 
-// Pairs that run at the same time on the current device (0: the kernel cannot run).
-template <bool kGated, bool kBf16>
-cudaError_t resident_pairs(int* pairs) {
+// Clusters that run at the same time on the current device.
+template <bool kGated, bool kBf16, int kS>
+cudaError_t resident_clusters(int* clusters) {
   static std::mutex mu;
   static int known[kMaxDevices] = {};
   int dev = 0;
@@ -646,18 +715,18 @@ cudaError_t resident_pairs(int* pairs) {
   if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
   std::lock_guard<std::mutex> lock(mu);
   if (known[dev] == 0) {
-    const auto kernel = w8a8_gemm_kernel<kGated, kBf16>;
+    const auto kernel = w8a8_gemm_kernel<kGated, kBf16, kS>;
     st = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem<kGated>);
     if (st != cudaSuccess) return st;
     int sms = 0;
     if ((st = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return st;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(sms / 2 * 2));
+    cfg.gridDim = dim3(static_cast<unsigned>(sms / (2 * kS) * 2 * kS));
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = kSmem<kGated>;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.x = 2 * kS;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
@@ -667,7 +736,7 @@ cudaError_t resident_pairs(int* pairs) {
     if (n <= 0) return cudaErrorNotSupported;
     known[dev] = n;
   }
-  *pairs = known[dev];
+  *clusters = known[dev];
   return cudaSuccess;
 }
 
@@ -683,11 +752,11 @@ cudaError_t resident_pairs(int* pairs) {
 // lost, and halved widths alone, since a narrower guess that breaks a group
 // once more costs a wave. 2 groups of 200 rows, 2048 x 1024: 7.1 / 8.3 (64); 4
 // of 128 gated stay at 256: 12.3, at 64 16.0; 8 of 150 8.4, at 128 10.1.
-int choose_tokens(int64_t rows, int64_t groups, int c_tiles, int pairs) {
+int choose_tokens(int64_t rows, int64_t groups, int c_tiles, int pairs, int64_t* best_cost) {
   const int64_t parts = groups < rows ? groups : rows, even = (rows + parts - 1) / parts;
   const int narrowest = groups > 1 ? 64 : 32;
   int best = kMaxN;
-  int64_t best_cost = INT64_MAX;
+  *best_cost = INT64_MAX;
   for (int bn = kMaxN; bn >= narrowest; bn = groups > 1 ? bn / 2 : bn - 32) {
     int64_t tiles = (rows + bn - 1) / bn, width = (rows + tiles - 1) / tiles;
     if (groups > 1) {
@@ -695,12 +764,31 @@ int choose_tokens(int64_t rows, int64_t groups, int c_tiles, int pairs) {
       width = std::min<int64_t>(bn, even);
     }
     const int64_t waves = (tiles * c_tiles + pairs - 1) / pairs, cost = waves * ((width + 31) / 32 * 32 + 256);
-    if (cost < best_cost || (cost == best_cost && waves == 1)) {
-      best_cost = cost;
+    if (cost < *best_cost || (cost == *best_cost && waves == 1)) {
+      *best_cost = cost;
       best = bn;
     }
   }
   return best;
+}
+
+// Tokens per tile with K in `parts` parts, all tiles' clusters at the same time:
+// the narrowest that lets them (cost INT64_MAX: none does; a second wave of
+// clusters starts 6 us late). A slice of K of 32 tokens is 288 in the cost and
+// takes 0.19 us, on one pair as on 74; the exchange takes 1.5 us at 32 tokens
+// and 5 at 256. Measured in us, in two parts or four / whole: 64 x 2048 x 8192
+// 9.7 (4) / 16.7; 64 x 4096 x 8192 14.6 (2) / 19.2; 64 x 2048 x 2048 7.2 (4) /
+// 7.4; 128 x 300 x 2048 6.6 (4) / 7.4; 500 x 300 x 5000 9.9 (4) / 12.7; 256 x
+// 4096 x 4096 11.1 (2) / 12.4; whole stay 128 x 2048 x 2048 7.7 (2) / 7.5, 256 x
+// 2048 x 2048 8.3 (2) / 8.0 and 500 x 4096 x 4096 15.1 (2) / 13.7.
+int split_tokens(int64_t rows, int c_tiles, int k_blocks, int parts, int clusters, int64_t* cost) {
+  *cost = INT64_MAX;
+  for (int bn = 32; bn <= kMaxN && k_blocks >= parts; bn += 32)
+    if ((rows + bn - 1) / bn * c_tiles <= clusters) {
+      *cost = static_cast<int64_t>((k_blocks + parts - 1) / parts) * (bn + 256) + 1800 + 16 * bn;
+      return bn;
+    }
+  return kMaxN;
 }
 
 // The rows that row_index names, one after another at a pitch of `chunks` 16-byte
@@ -739,7 +827,7 @@ __global__ void __launch_bounds__(256) gather_rows_kernel(const int8_t* __restri
 template <bool kGated, bool kBf16>
 cudaError_t launch(const W8a8& p, cudaStream_t stream) {
   int pairs = 0;
-  cudaError_t st = resident_pairs<kGated, kBf16>(&pairs);
+  cudaError_t st = resident_clusters<kGated, kBf16, 1>(&pairs);
   if (st != cudaSuccess) return st;
   const int8_t* x = p.x;
   int64_t ldx = p.ldx;
@@ -772,11 +860,31 @@ cudaError_t launch(const W8a8& p, cudaStream_t stream) {
   a.channels = kGated ? kBM : 2 * kBM;
   a.c_tiles = static_cast<int>((p.n + a.channels - 1) / a.channels);
   a.k_blocks = static_cast<int>((p.k + kBK - 1) / kBK);
-  a.tokens_per_tile = choose_tokens(p.rows, p.groups, a.c_tiles, pairs);
+  int64_t cost = 0;
+  a.tokens_per_tile = choose_tokens(p.rows, p.groups, a.c_tiles, pairs, &cost);
+  if constexpr (!kGated) {
+    if (p.starts == nullptr) {  // dense: the tiles are known here
+      int twos = 0, fours = 0;
+      if ((st = resident_clusters<kGated, kBf16, 2>(&twos)) != cudaSuccess) return st;
+      if ((st = resident_clusters<kGated, kBf16, 4>(&fours)) != cudaSuccess) return st;
+      cost *= a.k_blocks;
+      int64_t cost2 = 0, cost4 = 0;
+      const int tokens2 = split_tokens(p.rows, a.c_tiles, a.k_blocks, 2, twos, &cost2);
+      const int tokens4 = split_tokens(p.rows, a.c_tiles, a.k_blocks, 4, fours, &cost4);
+      if (std::min(cost2, cost4) < cost) {
+        const bool four = cost4 < cost2;
+        a.tokens_per_tile = four ? tokens4 : tokens2;
+        a.tma_residual = false;  // its slots go by the units one after another
+        const unsigned tiles = static_cast<unsigned>((p.rows + a.tokens_per_tile - 1) / a.tokens_per_tile * a.c_tiles);
+        return four ? launch_pdl(w8a8_gemm_kernel<kGated, kBf16, 4>, tiles * 8, kThreads, kSmem<kGated>, stream, a)
+                    : launch_pdl(w8a8_gemm_kernel<kGated, kBf16, 2>, tiles * 4, kThreads, kSmem<kGated>, stream, a);
+      }
+    }
+  }
   const int64_t most =
       (p.rows / a.tokens_per_tile + (p.groups < p.rows ? p.groups : p.rows)) * static_cast<int64_t>(a.c_tiles);
   const unsigned blocks = 2u * static_cast<unsigned>(most < pairs ? most : pairs);
-  return launch_pdl(w8a8_gemm_kernel<kGated, kBf16>, blocks, kThreads, kSmem<kGated>, stream, a);
+  return launch_pdl(w8a8_gemm_kernel<kGated, kBf16, 1>, blocks, kThreads, kSmem<kGated>, stream, a);
 }
 
 }  // namespace
@@ -784,18 +892,18 @@ cudaError_t launch(const W8a8& p, cudaStream_t stream) {
 namespace {
 // Which kernel: w8a8_rows.cu reads the weights once per 8 rows (dense: up to 32)
 // of a group, with little to set up; the kernel above takes 5.6 us or more.
-// Measured in us, rows against this one. Dense, n x k: 1 row 2048 x 2048 2.9 / 7.2,
-// 102400 x 2048 36 / 39; 8 rows 8192 x 2048 6.1 / 7.4; 16 rows 2048 x 2048 4.1 /
-// 7.2, 4096 x 1024 4.1 / 5.7, 4096 x 8192 14.7 / 18.2, 8192 x 1024 7.2 / 5.8, 8192
-// x 2048 8.3 / 7.4; 32 rows 1000 x 1000 4.8 / 6.2, 2048 x 2048 6.4 / 7.4, 4096 x
-// 2048 7.2 / 7.4, 2048 x 8192 21 / 17. Groups: 64 of 2 x 1024 x 2048 gated, 6
+// Measured in us, rows against this one. Dense, n x k: 1 row 2048 x 2048 2.9 / 6.4,
+// 102400 x 2048 36 / 39; 8 rows 8192 x 2048 6.1 / 7.4, 4096 x 8192 11.0 / 13.4; 16
+// rows 2048 x 2048 4.1 / 6.3, 4096 x 4096 7.4 / 8.4, 2048 x 8192 11.8 / 8.7, 8192
+// x 1024 7.2 / 5.8, 8192 x 2048 8.3 / 7.4; 32 rows 1000 x 1000 4.8 / 6.2, 2048 x
+// 2048 6.4 / 6.4, 4096 x 2048 7.2 / 7.4, 2048 x 4096 10.5 / 7.2. Groups: 64 of 2 x 1024 x 2048 gated, 6
 // rows 7.6 / 12.1, 60 rows 37 / 38, 240 rows 46 / 52; 64 of 2048 x 1024, 6 rows
 // 6.2 / 9.7, 96 rows 23.5 / 25.7, 240 rows 30.5 / 29.7; 16 of 1024 x 2048, 32
 // rows 9.7 / 11.5, 128 rows 14.8 / 11.5; 8 of those, 30 rows 7.7 / 9.8, 60 9.8 / 9.9.
 bool few_rows_grouped(int64_t rows, int64_t groups) { return rows <= 256 && rows <= 4 * groups; }
 bool few_rows(const W8a8& p) {
   if (p.starts != nullptr) return few_rows_grouped(p.rows, p.groups);
-  return p.rows <= 8 || (p.n <= 4096 && (p.rows <= 16 || (p.rows <= 32 && p.k <= 2048)));
+  return p.rows <= 8 || (p.n <= 4096 && ((p.rows <= 16 && p.k <= 4096) || (p.rows <= 32 && p.k <= 2048)));
 }
 }  // namespace
 
@@ -804,11 +912,15 @@ size_t w8a8_gather_bytes(int64_t rows, int64_t groups, int64_t k) {
 }
 
 cudaError_t prepare_w8a8() {
-  int pairs = 0;
-  cudaError_t st = resident_pairs<false, false>(&pairs);
-  if (st == cudaSuccess) st = resident_pairs<false, true>(&pairs);
-  if (st == cudaSuccess) st = resident_pairs<true, false>(&pairs);
-  if (st == cudaSuccess) st = resident_pairs<true, true>(&pairs);
+  int n = 0;
+  cudaError_t st = resident_clusters<false, false, 1>(&n);
+  if (st == cudaSuccess) st = resident_clusters<false, true, 1>(&n);
+  if (st == cudaSuccess) st = resident_clusters<true, false, 1>(&n);
+  if (st == cudaSuccess) st = resident_clusters<true, true, 1>(&n);
+  if (st == cudaSuccess) st = resident_clusters<false, false, 2>(&n);
+  if (st == cudaSuccess) st = resident_clusters<false, true, 2>(&n);
+  if (st == cudaSuccess) st = resident_clusters<false, false, 4>(&n);
+  if (st == cudaSuccess) st = resident_clusters<false, true, 4>(&n);
   return st;
 }
 

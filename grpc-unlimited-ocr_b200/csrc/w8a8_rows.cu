@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(kThreads, kSplit == 8 ? (kGated ? 3 : 2) : 4) 
         sum += part[sub * kSplit + w][tl][owner][reg];
         if (kGated) sum_up += part[sub * kSplit + w][kTiles + tl][owner][reg];
       }
-      float v = static_cast<float>(sum) * o.x * o.w;
+      float v = __fmul_rn(static_cast<float>(sum) * o.x, o.w);  // not fused with a sum: the bits of w8a8_gemm.cu
       if (kGated)
         v = silu_mul(v, static_cast<float>(sum_up) * o.x * o.up);
       else

@@ -174,6 +174,31 @@ def test_linear_w8a8_large(cuda, m, n, k):
     linear_case(m, n, k, True, True, False)
 
 
+@pytest.mark.parametrize("m", [33, 64, 100, 129, 300, 500, 1000])
+@pytest.mark.parametrize("n,k", [(70, 8000), (300, 2049), (1030, 4113), (2048, 4096), (4100, 5000)])
+def test_linear_w8a8_long_k_of_few_tiles(cuda, m, n, k):
+    linear_case(m, n, k, False, True, True, 16)
+    linear_case(m, n, k, True, False, m % 2 == 0)
+
+
+@pytest.mark.parametrize("m,bf16", [(40, False), (40, True), (500, False), (700, True)])
+def test_linear_w8a8_long_k_is_repeatable(cuda, m, bf16):
+    import torch
+    g = gen_of(m, bf16)
+    n, k = 600, 6000
+    x, w, xs, ws = ints(g, m, k), ints(g, n, k), scales(g, m), scales(g, n)
+    b = torch.randn(n, generator=g, device="cuda")
+    y = [torch.empty(m, n, dtype=torch.bfloat16 if bf16 else torch.float32, device="cuda") for _ in range(20)]
+    for out in y:
+        M.linear_w8a8(x, xs, w, ws, out, bias=b)
+    # The sums are exact and the rest is rounded alike: rows taken alone are the same bits.
+    few = torch.empty_like(y[0][:5])
+    M.linear_w8a8(x[:5], xs[:5], w, ws, few, bias=b)
+    assert torch.equal(few, y[0][:5])
+    for out in y[1:]:
+        assert torch.equal(out, y[0])
+
+
 @pytest.mark.parametrize("m", [1, 20, 150])
 def test_linear_w8a8_longest_sums(cuda, m):
     """Rows of the largest width and magnitude: the sums come within 2^14 of 2^31."""
