@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from dataclasses import dataclass
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -131,6 +132,18 @@ class GroupedW8A8Args(ctypes.Structure):
         ("workspace_bytes", ctypes.c_int64)]
 
 
+def _packer(args) -> struct.Struct:
+    """The fields of a ctypes structure (pointers, int64, int32) as a struct format; null pointers are 0. A call packs
+    its arguments in a third of the time that the structure's constructor takes."""
+    code = {ctypes.c_void_p: "P", ctypes.c_int64: "q", ctypes.c_int32: "i"}
+    packer = struct.Struct("@" + "".join(code[kind] for _, kind in args._fields_))
+    assert packer.size == ctypes.sizeof(args)
+    return packer
+
+
+_pack_linear, _pack_grouped = _packer(LinearW8A8Args).pack, _packer(GroupedW8A8Args).pack
+
+
 def lib() -> ctypes.CDLL:
     global _lib
     if _lib is None:
@@ -179,9 +192,9 @@ def lib() -> ctypes.CDLL:
         L.uocr_decoder_check.argtypes = [vp, vp]
         L.uocr_decoder_profile_decode.argtypes = [vp, i64, ctypes.POINTER(f32), vp]
         L.uocr_quantize_tokens.argtypes = [vp, i32, i64, i64, i64, vp, i64, vp, vp]
-        L.uocr_linear_w8a8.argtypes = [ctypes.POINTER(LinearW8A8Args), vp]
-        L.uocr_grouped_w8a8_workspace.argtypes = [ctypes.POINTER(GroupedW8A8Args), ctypes.POINTER(i64)]
-        L.uocr_grouped_linear_w8a8.argtypes = [ctypes.POINTER(GroupedW8A8Args), vp]
+        L.uocr_linear_w8a8.argtypes = [vp, vp]  # structures, by reference or packed
+        L.uocr_grouped_w8a8_workspace.argtypes = [vp, ctypes.POINTER(i64)]
+        L.uocr_grouped_linear_w8a8.argtypes = [vp, vp]
         _lib = L
     return _lib
 
@@ -517,16 +530,16 @@ def linear_w8a8(x, x_scales, w, w_scales, y, bias=None, residual=None, stream=No
     if not (x_scales.dtype is f32 and w_scales.dtype is f32 and x_scales.numel() == m and w_scales.numel() == n
             and x_scales.is_contiguous() and w_scales.is_contiguous() and x_scales.is_cuda and w_scales.is_cuda):
         _vector(x_scales, "x_scales", m, f32), _vector(w_scales, "w_scales", n, f32)
-    ldr = res = None
+    ldr = res = 0
     if residual is not None:
         if residual.dtype is not y.dtype:
             raise ValueError("residual must have y's dtype")
         res, ldr = residual.data_ptr(), _pitch(residual, "residual", m, n)
-    args = LinearW8A8Args(
+    args = _pack_linear(
         x.data_ptr(), x_scales.data_ptr(), w.data_ptr(), w_scales.data_ptr(),
-        None if bias is None else _vector(bias, "bias", n, f32), res, y.data_ptr(), m, n, k, ldx, ldw, ldr or 0, ldy,
+        0 if bias is None else _vector(bias, "bias", n, f32), res, y.data_ptr(), m, n, k, ldx, ldw, ldr, ldy,
         _float_dtype(y, "y"), 0)
-    _check(lib().uocr_linear_w8a8(ctypes.byref(args), _stream(stream)))
+    _check(lib().uocr_linear_w8a8(args, _stream(stream)))
 
 
 def _stack_pitch(t, what: str, groups: int, n: int, k: int) -> int:
@@ -571,25 +584,25 @@ def grouped_linear_w8a8(x, x_scales, w, w_scales, offsets, y, row_index=None, w_
             and offsets.is_contiguous() and x_scales.is_cuda and w_scales.is_cuda and offsets.is_cuda):
         _vector(x_scales, "x_scales", x_rows, f32), _vector(w_scales, "w_scales", groups * n, f32)
         _vector(offsets, "offsets", groups + 1, i32)
-    up = up_scales = index = None
+    up = up_scales = index = 0
     if w_up is not None:
         if _stack_pitch(w_up, "w_up", groups, n, k) != ldw:
             raise ValueError("w_up must have w's pitch")
         up, up_scales = w_up.data_ptr(), _vector(w_up_scales, "w_up_scales", groups * n, f32)
     if row_index is not None:
         index = _vector(row_index, "row_index", rows, i32)
-    args = GroupedW8A8Args(
-        x.data_ptr(), x_scales.data_ptr(), index, offsets.data_ptr(), w.data_ptr(), w_scales.data_ptr(), up, up_scales,
-        y.data_ptr(), rows, x_rows, groups, n, k, ldx, ldw, ldy, _float_dtype(y, "y"), 0, None, 0)
-    if index is not None:
+    args = (x.data_ptr(), x_scales.data_ptr(), index, offsets.data_ptr(), w.data_ptr(), w_scales.data_ptr(), up,
+            up_scales, y.data_ptr(), rows, x_rows, groups, n, k, ldx, ldw, ldy, _float_dtype(y, "y"), 0)
+    space, space_bytes = 0, 0
+    if row_index is not None:
         need = ctypes.c_int64()
-        _check(lib().uocr_grouped_w8a8_workspace(ctypes.byref(args), ctypes.byref(need)))
+        _check(lib().uocr_grouped_w8a8_workspace(_pack_grouped(*args, 0, 0), ctypes.byref(need)))
         if need.value > 0:
             workspace = torch.empty(need.value, dtype=torch.uint8, device=y.device)
             if stream is not None:  # the allocator may hand it out again only when that stream is done with it
                 workspace.record_stream(torch.cuda.ExternalStream(stream) if isinstance(stream, int) else stream)
-            args.workspace, args.workspace_bytes = workspace.data_ptr(), need.value
-    _check(lib().uocr_grouped_linear_w8a8(ctypes.byref(args), _stream(stream)))
+            space, space_bytes = workspace.data_ptr(), need.value
+    _check(lib().uocr_grouped_linear_w8a8(_pack_grouped(*args, space, space_bytes), _stream(stream)))
 
 
 class Decoder:
