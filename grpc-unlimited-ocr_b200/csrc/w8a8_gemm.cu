@@ -772,23 +772,27 @@ int choose_tokens(int64_t rows, int64_t groups, int c_tiles, int pairs, int64_t*
   return best;
 }
 
-// Tokens per tile with K in `parts` parts, all tiles' clusters at the same time:
-// the narrowest that lets them (cost INT64_MAX: none does; a second wave of
-// clusters starts 6 us late). A slice of K of 32 tokens is 288 in the cost and
-// takes 0.19 us, on one pair as on 74; the exchange takes 1.5 us at 32 tokens
-// and 5 at 256. Measured in us, in two parts or four / whole: 64 x 2048 x 8192
-// 9.7 (4) / 16.7; 64 x 4096 x 8192 14.6 (2) / 19.2; 64 x 2048 x 2048 7.2 (4) /
-// 7.4; 128 x 300 x 2048 6.6 (4) / 7.4; 500 x 300 x 5000 9.9 (4) / 12.7; 256 x
-// 4096 x 4096 11.1 (2) / 12.4; whole stay 128 x 2048 x 2048 7.7 (2) / 7.5, 256 x
-// 2048 x 2048 8.3 (2) / 8.0 and 500 x 4096 x 4096 15.1 (2) / 13.7.
-int split_tokens(int64_t rows, int c_tiles, int k_blocks, int parts, int clusters, int64_t* cost) {
-  *cost = INT64_MAX;
-  for (int bn = 32; bn <= kMaxN && k_blocks >= parts; bn += 32)
-    if ((rows + bn - 1) / bn * c_tiles <= clusters) {
-      *cost = static_cast<int64_t>((k_blocks + parts - 1) / parts) * (bn + 256) + 1800 + 16 * bn;
-      return bn;
+// K in `parts` parts where that costs less than `cost`, all tiles' clusters at
+// the same time (a second wave of clusters starts 6 us late): tiles as narrow as
+// lets them. A slice of K of 32 tokens is 288 in the cost and takes 0.19 us, on one
+// pair as on 74; the exchange takes 1.5 us at 32 tokens and 5 at 256. Measured
+// in us, in two parts or four / whole: 64 x 2048 x 8192 9.7 (4) / 16.7; 64 x 4096
+// x 8192 14.6 (2) / 19.2; 64 x 2048 x 2048 7.2 (4) / 7.4; 128 x 300 x 2048 6.6
+// (4) / 7.4; 500 x 300 x 5000 9.9 (4) / 12.7; 256 x 4096 x 4096 11.1 (2) / 12.4;
+// whole stay 128 x 2048 x 2048 7.7 (2) / 7.5, 256 x 2048 x 2048 8.3 (2) / 8.0
+// and 500 x 4096 x 4096 15.1 (2) / 13.7.
+void split_tokens(int64_t rows, Args& a, int parts, int clusters, int64_t* cost, int* chosen) {
+  if (a.k_blocks < parts) return;
+  for (int bn = 32; bn <= kMaxN; bn += 32) {
+    if ((rows + bn - 1) / bn * a.c_tiles > clusters) continue;
+    const int64_t split = static_cast<int64_t>((a.k_blocks + parts - 1) / parts) * (bn + 256) + 1800 + 16 * bn;
+    if (split < *cost) {
+      *cost = split;
+      *chosen = parts;
+      a.tokens_per_tile = bn;
     }
-  return kMaxN;
+    return;
+  }
 }
 
 // The rows that row_index names, one after another at a pitch of `chunks` 16-byte
@@ -841,9 +845,27 @@ cudaError_t launch(const W8a8& p, cudaStream_t stream) {
     x = p.workspace;
   }
   Args a{};
+  a.p = p;
+  a.channels = kGated ? kBM : 2 * kBM;
+  a.c_tiles = static_cast<int>((p.n + a.channels - 1) / a.channels);
+  a.k_blocks = static_cast<int>((p.k + kBK - 1) / kBK);
+  int64_t cost = 0;
+  a.tokens_per_tile = choose_tokens(p.rows, p.groups, a.c_tiles, pairs, &cost);
+  int parts = 1;  // of K
+  if constexpr (!kGated) {
+    if (p.starts == nullptr) {  // dense: the tiles are known here
+      cost *= a.k_blocks;
+      int clusters = 0;
+      if ((st = resident_clusters<kGated, kBf16, 2>(&clusters)) != cudaSuccess) return st;
+      split_tokens(p.rows, a, 2, clusters, &cost, &parts);
+      if ((st = resident_clusters<kGated, kBf16, 4>(&clusters)) != cudaSuccess) return st;
+      split_tokens(p.rows, a, 4, clusters, &cost, &parts);
+    }
+  }
+  // Boxes that no tile can need are left unset: a map costs the call 0.15 us.
   const bool ok = make_int8_tmap(&a.x, x, p.rows, p.k, ldx, kBoxRows) &&
-                  make_int8_tmap(&a.x_wide, x, p.rows, p.k, ldx, 64) &&
-                  make_int8_tmap(&a.x_half, x, p.rows, p.k, ldx, kMaxN / 2) &&
+                  (a.tokens_per_tile < 128 || make_int8_tmap(&a.x_wide, x, p.rows, p.k, ldx, 64)) &&
+                  (a.tokens_per_tile < kMaxN || make_int8_tmap(&a.x_half, x, p.rows, p.k, ldx, kMaxN / 2)) &&
                   make_int8_tmap(&a.w, p.w, p.groups * p.n, p.k, p.ldw, kGated ? kBM / 2 : kBM) &&
                   (!kGated || make_int8_tmap(&a.up, p.w_up, p.groups * p.n, p.k, p.ldw, kBM / 2));
   if (!ok) return cudaErrorInvalidValue;
@@ -851,35 +873,18 @@ cudaError_t launch(const W8a8& p, cudaStream_t stream) {
     return reinterpret_cast<uintptr_t>(base) % 16 == 0 && ld * (kBf16 ? 2 : 4) % 16 == 0;
   };
   a.tma_store = kBf16 && aligned(p.y, p.ldy);
-  a.tma_residual = !kBf16 && !kGated && p.residual != nullptr && aligned(p.residual, p.ldr);
+  // (With K in parts a warp's units do not follow one another as the residual's slots do.)
+  a.tma_residual = !kBf16 && !kGated && parts == 1 && p.residual != nullptr && aligned(p.residual, p.ldr);
   if (a.tma_store && !make_tile_tmap(&a.y, p.y, true, p.rows, p.n, p.ldy, kGated ? kUnit / 2 : kUnit))
     return cudaErrorInvalidValue;
   if (a.tma_residual && !make_tile_tmap(&a.residual, p.residual, false, p.rows, p.n, p.ldr, kRows32))
     return cudaErrorInvalidValue;
-  a.p = p;
-  a.channels = kGated ? kBM : 2 * kBM;
-  a.c_tiles = static_cast<int>((p.n + a.channels - 1) / a.channels);
-  a.k_blocks = static_cast<int>((p.k + kBK - 1) / kBK);
-  int64_t cost = 0;
-  a.tokens_per_tile = choose_tokens(p.rows, p.groups, a.c_tiles, pairs, &cost);
   if constexpr (!kGated) {
-    if (p.starts == nullptr) {  // dense: the tiles are known here
-      int twos = 0, fours = 0;
-      if ((st = resident_clusters<kGated, kBf16, 2>(&twos)) != cudaSuccess) return st;
-      if ((st = resident_clusters<kGated, kBf16, 4>(&fours)) != cudaSuccess) return st;
-      cost *= a.k_blocks;
-      int64_t cost2 = 0, cost4 = 0;
-      const int tokens2 = split_tokens(p.rows, a.c_tiles, a.k_blocks, 2, twos, &cost2);
-      const int tokens4 = split_tokens(p.rows, a.c_tiles, a.k_blocks, 4, fours, &cost4);
-      if (std::min(cost2, cost4) < cost) {
-        const bool four = cost4 < cost2;
-        a.tokens_per_tile = four ? tokens4 : tokens2;
-        a.tma_residual = false;  // its slots go by the units one after another
-        const unsigned tiles = static_cast<unsigned>((p.rows + a.tokens_per_tile - 1) / a.tokens_per_tile * a.c_tiles);
-        return four ? launch_pdl(w8a8_gemm_kernel<kGated, kBf16, 4>, tiles * 8, kThreads, kSmem<kGated>, stream, a)
-                    : launch_pdl(w8a8_gemm_kernel<kGated, kBf16, 2>, tiles * 4, kThreads, kSmem<kGated>, stream, a);
-      }
-    }
+    const unsigned tiles = static_cast<unsigned>((p.rows + a.tokens_per_tile - 1) / a.tokens_per_tile * a.c_tiles);
+    if (parts == 2)
+      return launch_pdl(w8a8_gemm_kernel<kGated, kBf16, 2>, tiles * 4, kThreads, kSmem<kGated>, stream, a);
+    if (parts == 4)
+      return launch_pdl(w8a8_gemm_kernel<kGated, kBf16, 4>, tiles * 8, kThreads, kSmem<kGated>, stream, a);
   }
   const int64_t most =
       (p.rows / a.tokens_per_tile + (p.groups < p.rows ? p.groups : p.rows)) * static_cast<int64_t>(a.c_tiles);
