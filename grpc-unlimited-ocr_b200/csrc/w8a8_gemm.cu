@@ -18,7 +18,7 @@
 //   warps 4-11 epilogue, 32 tokens x 32 weight rows at a time: the scales,
 //              then bf16 tiles are transposed into shared memory (stmatrix) and
 //              leave as bulk tensor stores, fp32 ones as lines of 32 channels
-//              (gated: sectors of 8), a residual arriving by TMA a unit ahead.
+//              (gated: sectors of 8), a residual arriving by TMA two units ahead.
 //              When gated, the gate's warp and the up's warp of the same
 //              channels exchange half of their tokens first.
 // A dense product of few tiles and a long K has K in two or four parts, a pair
@@ -64,14 +64,13 @@ constexpr int kOutBytes = kUnit * 32 * 2;        // a unit of 32 channels in bf1
 constexpr int kXchBytes = kUnit / 2 * 32 * 4;    // gated: half a unit's values for the partner warp
 constexpr int kRows32 = 16;            // tokens of an fp32 unit
 constexpr int kSlotBytes = kRows32 * 32 * 4;     // an fp32 unit's residual
-constexpr int kSlots = 2;
+constexpr int kSlots = 3;              // two 4 % slower at a page of 2048, 6 % at 8192 x 8192 x 1024
 // Per epilogue warp: two buffers of each in bf16 (a gated warp's output is half
-// a unit), or of an fp32 unit's residual.
-template <bool kGated>
-constexpr int kWarpBytes = kGated ? kOutBytes + 2 * kXchBytes : 2 * kOutBytes;
-static_assert(kSlots * kSlotBytes <= 2 * kOutBytes, "the residual's slots take the place of the output buffers");
-template <bool kGated>
-constexpr int kSmem = kStages * kStageBytes + kEpilogueWarps * kWarpBytes<kGated> + 1024;
+// a unit), or the fp32 units' residuals.
+template <bool kGated, bool kBf16>
+constexpr int kWarpBytes = kGated ? kOutBytes + 2 * kXchBytes : kBf16 ? 2 * kOutBytes : kSlots * kSlotBytes;
+template <bool kGated, bool kBf16>
+constexpr int kSmem = kStages * kStageBytes + kEpilogueWarps * kWarpBytes<kGated, kBf16> + 1024;
 constexpr int kTmemCols = 512;
 constexpr int kBoxRows = 16;
 constexpr int kBand = 8;               // token tiles of a band (decode_tile)
@@ -400,9 +399,9 @@ __global__ void __cluster_dims__(2 * kS, 1, 1) __launch_bounds__(kThreads, 1)
     constexpr bool kLaneIsChannel = !kGated && !kBf16;
     const int first_c = kLaneIsChannel ? lane : tr;
     unsigned char* area = smem + kStages * kStageBytes;
-    unsigned char* stg = area + e * kWarpBytes<kGated>;
+    unsigned char* stg = area + e * kWarpBytes<kGated, kBf16>;
     float4* xch = reinterpret_cast<float4*>(stg + kOutBytes);
-    const float4* xch_other = reinterpret_cast<const float4*>(area + (e ^ 2) * kWarpBytes<kGated> + kOutBytes);
+    const float4* xch_other = reinterpret_cast<const float4*>(area + (e ^ 2) * kWarpBytes<kGated, kBf16> + kOutBytes);
     const bool gate = quarter < 2;  // gated: lanes 0-63 hold gate rows, 64-127 up rows
     const int local_c = kGated ? rank * 64 + (quarter & 1) * 32 : rank * kBM + quarter * 32;
     const float* w_scales = kGated && !gate ? p.w_up_scales : p.w_scales;
@@ -478,7 +477,9 @@ __global__ void __cluster_dims__(2 * kS, 1, 1) __launch_bounds__(kThreads, 1)
         mbar_arrive_expect_tx(&sh.residual[e][s], kSlotBytes);
         tma_load_2d(stg + s * kSlotBytes, &args.residual, static_cast<int>(c0), tl.row0 + j0, &sh.residual[e][s]);
       };
-      if (kLaneIsChannel && ok) fetch_residual(way * kRows32, slot);
+      auto ahead = [&](int i) { return slot + i < kSlots ? slot + i : slot + i - kSlots; };
+      if (kLaneIsChannel && ok)
+        for (int i = 0; i < kSlots - 1; ++i) fetch_residual((way + i * kWays) * kRows32, ahead(i));
       if (ok) {
         ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[acc], (local >> 1) & 1));
         if (!ok) raise_error(p.err, kDevWaitTimeout, 86, t, 0);
@@ -539,9 +540,8 @@ __global__ void __cluster_dims__(2 * kS, 1, 1) __launch_bounds__(kThreads, 1)
         if (way * kRows32 >= tl.rows) release();
         for (int j0 = way * kRows32; j0 < tl.rows; j0 += kWays * kRows32) {
           if (kS > 1 && owner(j0 / kPart) != part) continue;
-          const int next_slot = slot ^ 1;
-          // (The slot's values, two units ago, have been read by the whole warp.)
-          fetch_residual(j0 + kWays * kRows32, next_slot);
+          // (The slot's values, a unit ago, have been read by the whole warp.)
+          fetch_residual(j0 + (kSlots - 1) * kWays * kRows32, ahead(kSlots - 1));
           int a[kRows32];
           tmem_ld_32x16(taddr + j0, a);
           if constexpr (kS > 1) add_parts(j0 / kPart, a, 0, kRows32);
@@ -580,7 +580,7 @@ __global__ void __cluster_dims__(2 * kS, 1, 1) __launch_bounds__(kThreads, 1)
               if (i < nr) *reinterpret_cast<float*>(out) = v[i];
           }
           __syncwarp();
-          slot = next_slot;
+          slot = ahead(1);
         }
         continue;
       } else {
@@ -716,14 +716,14 @@ cudaError_t resident_clusters(int* clusters) {
   std::lock_guard<std::mutex> lock(mu);
   if (known[dev] == 0) {
     const auto kernel = w8a8_gemm_kernel<kGated, kBf16, kS>;
-    st = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem<kGated>);
+    st = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem<kGated, kBf16>);
     if (st != cudaSuccess) return st;
     int sms = 0;
     if ((st = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return st;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(sms / (2 * kS) * 2 * kS));
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = kSmem<kGated>;
+    cfg.dynamicSmemBytes = kSmem<kGated, kBf16>;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2 * kS;
@@ -882,14 +882,14 @@ cudaError_t launch(const W8a8& p, cudaStream_t stream) {
   if constexpr (!kGated) {
     const unsigned tiles = static_cast<unsigned>((p.rows + a.tokens_per_tile - 1) / a.tokens_per_tile * a.c_tiles);
     if (parts == 2)
-      return launch_pdl(w8a8_gemm_kernel<kGated, kBf16, 2>, tiles * 4, kThreads, kSmem<kGated>, stream, a);
+      return launch_pdl(w8a8_gemm_kernel<kGated, kBf16, 2>, tiles * 4, kThreads, kSmem<kGated, kBf16>, stream, a);
     if (parts == 4)
-      return launch_pdl(w8a8_gemm_kernel<kGated, kBf16, 4>, tiles * 8, kThreads, kSmem<kGated>, stream, a);
+      return launch_pdl(w8a8_gemm_kernel<kGated, kBf16, 4>, tiles * 8, kThreads, kSmem<kGated, kBf16>, stream, a);
   }
   const int64_t most =
       (p.rows / a.tokens_per_tile + (p.groups < p.rows ? p.groups : p.rows)) * static_cast<int64_t>(a.c_tiles);
   const unsigned blocks = 2u * static_cast<unsigned>(most < pairs ? most : pairs);
-  return launch_pdl(w8a8_gemm_kernel<kGated, kBf16, 1>, blocks, kThreads, kSmem<kGated>, stream, a);
+  return launch_pdl(w8a8_gemm_kernel<kGated, kBf16, 1>, blocks, kThreads, kSmem<kGated, kBf16>, stream, a);
 }
 
 }  // namespace
