@@ -34,7 +34,7 @@
 // nearly all of its bandwidth (64 + 64 bytes a clock at the full MMA rate), and
 // every store and shared-memory access of the epilogue takes a clock of the
 // same pipe: the layout is chosen for few and full ones. Measured at 8192 x
-// 8192 x 4096: 171 us, 3200 TOP/s, the tensor pipe active for 87 % of the time.
+// 8192 x 4096: 171 us, 3200 TOP/s, the tensor pipe active for 85 % of the time.
 // With few slices of K the copies bound it, at 55 bytes a clock into each SM:
 // at 8192 x 8192 x 1024 the MMAs alone take 57 kcycles, the copies alone 67, all
 // but the stores 81, the whole 91.
