@@ -1,5 +1,5 @@
 // W8A8 products of a few rows (include/uocr_int8.h): the weights are streamed
-// once, at most kRowTiles * 8 tokens at a time against them.
+// once, at most kTiles * 8 tokens at a time against them.
 //
 // A warp takes 16 weight rows of one group (gate and up rows when gated) and
 // all of K or a part of it, with mma.sync m16n8k32 on signed bytes: A = 16
