@@ -734,8 +734,8 @@ cudaError_t resident_clusters(int* clusters) {
     cfg.numAttrs = 1;
     int n = 0;
     if ((st = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg)) != cudaSuccess) return st;
-    if (n <= 0) return cudaErrorNotSupported;
-    known[dev] = n;
+    if (n <= 0 && kS == 1) return cudaErrorNotSupported;
+    known[dev] = n > 0 ? n : -1;  // a device may hold no larger cluster: K then stays whole
   }
   *clusters = known[dev];
   return cudaSuccess;
