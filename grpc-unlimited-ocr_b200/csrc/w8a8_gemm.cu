@@ -458,7 +458,7 @@ __global__ void __cluster_dims__(2 * kS, 1, 1) __launch_bounds__(kThreads, 1)
     };
     Scales next{};
     if (pair0 < total) next = fetch(0);
-    int local = 0, buf = 0, slot = 0;
+    int local = 0, xbuf = 0, obuf = 0, slot = 0;  // xbuf turns over with each unit, obuf with each bulk store
     uint32_t slot_phase = 0;
     bool ok = true;
     for (int t = pair0; t < total; t += step, ++local) {
@@ -599,7 +599,7 @@ __global__ void __cluster_dims__(2 * kS, 1, 1) __launch_bounds__(kThreads, 1)
           add_parts(j0 / kPart, a[1], 16, 16);
         }
         if (j0 + kWays * kUnit >= tl.rows) release();
-        buf ^= 1;
+        xbuf ^= 1;
         const bool whole = nr >= kUnit && c0 + 32 <= p.n;
         Block v[4];
 #pragma unroll
@@ -616,8 +616,8 @@ __global__ void __cluster_dims__(2 * kS, 1, 1) __launch_bounds__(kThreads, 1)
         if (kGated) {
           // The gate's warp finishes the unit's first two blocks, the up's warp the others.
           first = gate ? 0 : 2;
-          float4* give = xch + buf * (kXchBytes / 16);
-          const float4* take = xch_other + buf * (kXchBytes / 16);
+          float4* give = xch + xbuf * (kXchBytes / 16);
+          const float4* take = xch_other + xbuf * (kXchBytes / 16);
 #pragma unroll
           for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -662,7 +662,11 @@ __global__ void __cluster_dims__(2 * kS, 1, 1) __launch_bounds__(kThreads, 1)
           }
         }
         if (kBf16 && args.tma_store && nr >= 8 * (first + kOut)) {
-          unsigned char* out = stg + buf * (kOut * 8 * 64);
+          // The buffers alternate with the groups that are committed: a unit
+          // stored directly (a tile's partial end) commits none and takes none,
+          // else the wait would let the one store still pending be this buffer's.
+          obuf ^= 1;
+          unsigned char* out = stg + obuf * (kOut * 8 * 64);
           if (elect_one()) bulk_wait_read<1>();  // the store before the last has read this buffer
           __syncwarp();
 #pragma unroll
