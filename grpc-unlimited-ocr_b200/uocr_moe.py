@@ -559,12 +559,22 @@ def _stack_pitch(t, what: str, groups: int, n: int, k: int) -> int:
     return pitch
 
 
+def _workspace(size: int, device, stream):
+    """`size` bytes from torch's allocator for work on `stream` alone. They come from that stream's own blocks: one that
+    the current stream gave back may still be in use by what that stream has queued."""
+    import torch
+    if stream is None:
+        return torch.empty(size, dtype=torch.uint8, device=device)
+    with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device) if isinstance(stream, int) else stream):
+        return torch.empty(size, dtype=torch.uint8, device=device)
+
+
 def grouped_linear_w8a8(x, x_scales, w, w_scales, offsets, y, row_index=None, w_up=None, w_up_scales=None,
                         stream=None):
     """Group g's rows offsets[g] .. offsets[g + 1] - 1 of y [rows, n] = x[row_index[r]] . w[g]^T in int8, or with
     w_up silu(x . w[g]^T) * (x . w_up[g]^T) (uocr_grouped_linear_w8a8). w, w_up: [groups, n, k] or the stack
     [groups * n, k]; w_scales: groups * n values; offsets, row_index: int32. Where the call needs a workspace it
-    comes from torch's allocator."""
+    comes from torch's allocator, from the blocks of the stream that the call runs on."""
     import torch
     f32, i32, i8 = torch.float32, torch.int32, torch.int8
     x_rows, k = x.shape
@@ -598,9 +608,7 @@ def grouped_linear_w8a8(x, x_scales, w, w_scales, offsets, y, row_index=None, w_
         need = ctypes.c_int64()
         _check(lib().uocr_grouped_w8a8_workspace(_pack_grouped(*args, 0, 0), ctypes.byref(need)))
         if need.value > 0:
-            workspace = torch.empty(need.value, dtype=torch.uint8, device=y.device)
-            if stream is not None:  # the allocator may hand it out again only when that stream is done with it
-                workspace.record_stream(torch.cuda.ExternalStream(stream) if isinstance(stream, int) else stream)
+            workspace = _workspace(need.value, y.device, stream)  # held until the launch is made
             space, space_bytes = workspace.data_ptr(), need.value
     _check(lib().uocr_grouped_linear_w8a8(_pack_grouped(*args, space, space_bytes), _stream(stream)))
 
