@@ -111,7 +111,7 @@ __device__ __forceinline__ void store8(const float (&v)[kChunk], const RowScale&
 // kKeep chunks of it each; what is beyond is read a second time. kAligned: x's rows
 // start at 16-byte boundaries.
 template <typename T, int kPerRow, int kKeep, bool kAligned>
-__global__ void __launch_bounds__(kThreads) quantize_tokens_kernel(const T* __restrict__ x, int64_t rows, int cols,
+__global__ void __launch_bounds__(kThreads) quantize_tokens_kernel(const T* x, int64_t rows, int cols,
                                                                    int64_t ldx, int8_t* __restrict__ q, int64_t ldq,
                                                                    float* __restrict__ scales) {
   __shared__ uint32_t part[kThreads / 32];

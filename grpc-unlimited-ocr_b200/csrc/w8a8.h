@@ -14,6 +14,10 @@ namespace uocr_b200 {
 // Launches a kernel that may start before the previous grid of the stream ends:
 // every thread of it calls pdl_wait before it reads or writes global memory (a
 // block that ended without would let the grid after it overtake the one before).
+// Its inputs may still be being written when it starts: it reads them by plain
+// loads, which stay behind that wait, and not as data that is read-only for the
+// kernel's whole life (the non-coherent loads of __ldg and of const __restrict__
+// pointers, which need not).
 template <typename... Params, typename... Args>
 cudaError_t launch_pdl(void (*kernel)(Params...), unsigned grid, unsigned block, size_t smem, cudaStream_t stream,
                        Args... args) {

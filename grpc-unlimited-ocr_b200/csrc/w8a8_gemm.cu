@@ -244,8 +244,8 @@ __global__ void __cluster_dims__(2 * kS, 1, 1) __launch_bounds__(kThreads, 1)
         int first = 0;
         int64_t count = p.rows;
         if (p.starts != nullptr) {
-          first = __ldg(p.starts + g);
-          count = p.counts != nullptr ? __ldg(p.counts + g) : static_cast<int64_t>(__ldg(p.starts + g + 1)) - first;
+          first = p.starts[g];
+          count = p.counts != nullptr ? p.counts[g] : static_cast<int64_t>(p.starts[g + 1]) - first;
           if (first < 0 || count < 0 || first + count > p.rows) {
             raise_error(p.err, kDevBadIndex, kSiteGroupRows, g, first);
             count = 0;
@@ -438,13 +438,13 @@ __global__ void __cluster_dims__(2 * kS, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int q = 0; q < (kLaneIsChannel ? 1 : 4); ++q) {
         const bool in = c + 8 * q < p.n;
-        f.w[q] = in ? __ldg(w_scales + f.tl.g * p.n + c + 8 * q) : 0.0f;
-        f.bias[q] = has_bias && in ? __ldg(p.bias + c + 8 * q) : 0.0f;
+        f.w[q] = in ? w_scales[f.tl.g * p.n + c + 8 * q] : 0.0f;
+        f.bias[q] = has_bias && in ? p.bias[c + 8 * q] : 0.0f;
       }
       if (et < f.tl.rows) {  // tokens past the tile, and rows x does not have: zero
         int64_t r = f.tl.row0 + et;
         if (p.row_index != nullptr) {
-          const int v = __ldg(p.row_index + r);
+          const int v = p.row_index[r];
           if (v < 0 || v >= p.x_rows) {
             raise_error(p.err, kDevBadIndex, kSiteRowIndex, static_cast<int>(r), v);
             r = -1;
@@ -452,7 +452,7 @@ __global__ void __cluster_dims__(2 * kS, 1, 1) __launch_bounds__(kThreads, 1)
             r = v;
           }
         }
-        if (r >= 0) f.x = __ldg(p.x_scales + r);
+        if (r >= 0) f.x = p.x_scales[r];
       }
       return f;
     };
@@ -807,9 +807,9 @@ void split_tokens(int64_t rows, Args& a, int parts, int clusters, int64_t* cost,
 // to the same tokens at about the same time, while L2 holds their rows (196608
 // rows of 2048 bytes, 64 even groups: 92 us with 80 MB of x read from memory,
 // 111 us and 299 MB in the rows' own order; skewed groups 110 us, 237 MB).
-__global__ void __launch_bounds__(256) gather_rows_kernel(const int8_t* __restrict__ x, int64_t ldx, int64_t x_rows,
-                                                          const int* __restrict__ row_index, int rows, int stripes,
-                                                          int chunks, uint4* __restrict__ out) {
+__global__ void __launch_bounds__(256) gather_rows_kernel(const int8_t* x, int64_t ldx, int64_t x_rows,
+                                                          const int* row_index, int rows, int stripes, int chunks,
+                                                          uint4* __restrict__ out) {
   pdl_wait();
   pdl_launch_dependents();
   const int per = (rows + stripes - 1) / stripes;
@@ -817,7 +817,7 @@ __global__ void __launch_bounds__(256) gather_rows_kernel(const int8_t* __restri
   for (int i = blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5); i < per * stripes; i += warps) {
     const int r = i % stripes * per + i / stripes;
     if (r >= rows) continue;
-    const int64_t src = __ldg(row_index + r);
+    const int64_t src = row_index[r];
     const bool in = src >= 0 && src < x_rows;
     const uint4* from = reinterpret_cast<const uint4*>(x + (in ? src : 0) * ldx);
     uint4* to = out + static_cast<int64_t>(r) * chunks;
@@ -825,7 +825,7 @@ __global__ void __launch_bounds__(256) gather_rows_kernel(const int8_t* __restri
       uint4 v[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u)
-        v[u] = in && c0 + 32 * u < chunks ? __ldg(from + c0 + 32 * u) : make_uint4(0, 0, 0, 0);
+        v[u] = in && c0 + 32 * u < chunks ? from[c0 + 32 * u] : make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (int u = 0; u < 4; ++u)
         if (c0 + 32 * u < chunks) to[c0 + 32 * u] = v[u];

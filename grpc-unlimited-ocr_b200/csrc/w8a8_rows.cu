@@ -30,10 +30,10 @@ __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, ui
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Weights are read once: past L1, and first to leave L2.
+// Weights are read once: past L1.
 __device__ __forceinline__ uint4 load_weights(const int8_t* p) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                : "l"(p));
   return v;
@@ -82,8 +82,8 @@ __global__ void __launch_bounds__(kThreads, kSplit == 8 ? (kGated ? 3 : 2) : 4) 
       int f = 0;
       int64_t c = 0;
       if (mine < p.groups) {
-        f = __ldg(p.starts + mine);
-        c = p.counts != nullptr ? __ldg(p.counts + mine) : static_cast<int64_t>(__ldg(p.starts + mine + 1)) - f;
+        f = p.starts[mine];
+        c = p.counts != nullptr ? p.counts[mine] : static_cast<int64_t>(p.starts[mine + 1]) - f;
         if (f < 0 || c < 0 || f + c > p.rows) {
           if (blockIdx.x == 0) raise_error(p.err, kDevBadIndex, kSiteGroupRows, mine, f);
           c = 0;
@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(kThreads, kSplit == 8 ? (kGated ? 3 : 2) : 4) 
       if (r < count) {
         src = first + r;
         if (p.row_index != nullptr) {
-          src = __ldg(p.row_index + src);
+          src = p.row_index[src];
           if (src >= p.x_rows) src = -1;  // reported below
         }
       }
@@ -165,15 +165,15 @@ __global__ void __launch_bounds__(kThreads, kSplit == 8 ? (kGated ? 3 : 2) : 4) 
       o.in = tok < 8 * kTiles && r0 + tok < count && c < p.n;
       if (!o.in) return o;
       const int64_t row = static_cast<int64_t>(first) + r0 + tok;
-      const int64_t src = p.row_index != nullptr ? __ldg(p.row_index + row) : row;
+      const int64_t src = p.row_index != nullptr ? p.row_index[row] : row;
       const bool has = src >= 0 && src < p.x_rows;
       if (!has) raise_error(p.err, kDevBadIndex, kSiteRowIndex, static_cast<int>(row), static_cast<int>(src));
-      o.x = has ? __ldg(p.x_scales + src) : 0.0f;
-      o.w = __ldg(p.w_scales + g * p.n + c);
+      o.x = has ? p.x_scales[src] : 0.0f;
+      o.w = p.w_scales[g * p.n + c];
       if (kGated) {
-        o.up = __ldg(p.w_up_scales + g * p.n + c);
+        o.up = p.w_up_scales[g * p.n + c];
       } else {
-        if (p.bias != nullptr) o.bias = __ldg(p.bias + c);
+        if (p.bias != nullptr) o.bias = p.bias[c];
         if (p.residual != nullptr) o.residual = to_f32(static_cast<const T*>(p.residual)[row * p.ldr + c]);
       }
       return o;
@@ -188,8 +188,7 @@ __global__ void __launch_bounds__(kThreads, kSplit == 8 ? (kGated ? 3 : 2) : 4) 
         const int64_t kb = static_cast<int64_t>(s + u) * kStep, left = p.k - kb - tq * 16;
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) {
-          b[i][u] = s + u < s1 && left > 0 && xr[i] != nullptr ? __ldg(reinterpret_cast<const uint4*>(xr[i] + kb))
-                                                                : zero;
+          b[i][u] = s + u < s1 && left > 0 && xr[i] != nullptr ? *reinterpret_cast<const uint4*>(xr[i] + kb) : zero;
           if (left < 16) b[i][u] = keep_bytes(b[i][u], left);
         }
       }
