@@ -56,8 +56,9 @@ typedef struct uocr_decoder_desc {
 /* The decode attention's products on the CUDA cores instead of the tensor
  * cores (the default wherever a split's K and V rows fit in shared memory). */
 #define UOCR_DECODER_CUDA_CORE_ATTENTION 1
-/* int8 decoders: the prefill's projections and MoE blocks on int8 activations
- * (UOCR_PLAN_INT8_ACTIVATIONS). Decode steps are as without it. */
+/* int8 decoders: the prefill on int8 activations, its q/k/v and output
+ * projections whatever the prompt's rows, its MoE blocks with more rows than a
+ * decode batch (UOCR_PLAN_INT8_ACTIVATIONS). Decode steps are as without it. */
 #define UOCR_DECODER_INT8_ACTIVATIONS 2
 
 /* One layer's weights, fp32 or bf16 (dtype), host or device (memory); the

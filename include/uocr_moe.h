@@ -107,12 +107,13 @@ typedef struct uocr_moe_desc {
  * Decode batches normalise inside the router and gate/up kernels; the
  * tensor-core decode flag is then ignored. */
 #define UOCR_PLAN_PRE_NORM 8
-/* int8 plans (UOCR_WEIGHT_INT8, else UOCR_ERR_INVALID_ARGUMENT): more than 16
- * rows multiply int8 activations (one scale per token, uocr_quantize_tokens'
- * rule) with the int8 weights on the tensor cores (uocr_int8.h) instead of
- * expanding each layer to bf16 first. About 1 % of quantisation noise is added
- * in front of each product; the expanded copy of a layer's weights is not
- * allocated. Up to 16 rows are as without the flag. */
+/* int8 plans (UOCR_WEIGHT_INT8, else UOCR_ERR_INVALID_ARGUMENT): rows of the
+ * prefill path (more than 16; above a hidden size of 3100 fewer, since the
+ * decode kernels then hold fewer) multiply int8 activations (one scale per
+ * token, uocr_quantize_tokens' rule) with the int8 weights on the tensor cores
+ * (uocr_int8.h) instead of expanding each layer to bf16 first. About 1 % of
+ * quantisation noise is added in front of each product; the expanded copy of a
+ * layer's weights is not allocated. Decode batches are as without the flag. */
 #define UOCR_PLAN_INT8_ACTIVATIONS 16
 
 int uocr_moe_plan_create(const uocr_moe_desc* desc, uocr_moe_plan** plan);
