@@ -1200,8 +1200,8 @@ int uocr_ops_check(void* stream) {
     std::snprintf(buf, sizeof(buf), "expert_ffn_one: expert id %d at position %d is outside [0, %d)", e.b, e.a,
                   kMaxExperts);
   else if (e.code == kDevBadIndex && e.where == kSiteGroupRows)
-    std::snprintf(buf, sizeof(buf), "grouped_linear_w8a8: the rows of group %d (from row %d) are not in order or out of range",
-                  e.a, e.b);
+    std::snprintf(buf, sizeof(buf),
+                  "grouped_linear_w8a8: the rows of group %d (from row %d) are not in order or out of range", e.a, e.b);
   else if (e.code == kDevBadIndex && e.where == kSiteRowIndex)
     std::snprintf(buf, sizeof(buf), "grouped_linear_w8a8: row %d reads row %d, which x does not have", e.a, e.b);
   else

@@ -1,6 +1,6 @@
 // C ABI of the 8-bit integer operators (include/uocr_int8.h): argument checks
-// and launches. Host code only; the kernels are in quantize_tokens.cu and
-// w8a8_gemm.cu.
+// and launches. Host code only; the kernels are in quantize_tokens.cu,
+// w8a8_gemm.cu and w8a8_rows.cu.
 #include <cuda_runtime.h>
 
 #include <string>
@@ -25,7 +25,9 @@ int done(const char* op, cudaError_t st) {
                         std::string(op) + ": " + cudaGetErrorString(st));
 }
 
-bool int8_rows_ok(const int8_t* base, int64_t ld) { return reinterpret_cast<uintptr_t>(base) % 16 == 0 && ld % 16 == 0; }
+bool int8_rows_ok(const int8_t* base, int64_t ld) {
+  return reinterpret_cast<uintptr_t>(base) % 16 == 0 && ld % 16 == 0;
+}
 
 // What the two products check alike. rows, groups and the pointers that may
 // be null are the caller's.

@@ -124,7 +124,8 @@ __device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint64_t a_desc, u
       : "memory");
 }
 
-// Arrives once on `bar` of both CTAs of the pair (ranks leader, leader + 1) when every MMA this thread issued so far has completed.
+// Arrives once on `bar` of both CTAs of the pair (ranks leader, leader + 1) when every MMA this thread issued so far
+// has completed.
 __device__ __forceinline__ void umma_commit_pair(uint64_t* bar, uint32_t leader) {
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(

@@ -71,6 +71,12 @@ cudaError_t prepare_w8a8();
 // The kernel for few rows (w8a8_rows.cu); launch_w8a8 chooses.
 cudaError_t launch_w8a8_rows(const W8a8& p, cudaStream_t stream);
 
+// Values of y's type (and the residual's) as the epilogues take them.
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
 // silu(g) * u = g / (1 + exp(-g)) * u. The quotient to 2 ulp (__fdividef): an
 // IEEE division branches, which keeps a thread's outputs from overlapping.
 __device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.0f + expf(-g)) * u; }

@@ -132,16 +132,12 @@ __device__ __forceinline__ Tile decode_tile(int t, const Shared& sh, int groups,
   const unsigned high = min(static_cast<unsigned>(kBand), r_tiles - band * kBand);
   const unsigned c = in_band / high;
   const unsigned r = (band * kBand + in_band - c * high) * per;
-  return Tile{lo, static_cast<int>(sh.first[lo] + r), static_cast<int>(min(per, count - r)), static_cast<int>(c) * a.channels};
+  return Tile{lo, static_cast<int>(sh.first[lo] + r), static_cast<int>(min(per, count - r)),
+              static_cast<int>(c) * a.channels};
 }
 
 template <bool kBf16>
 using Out = typename std::conditional<kBf16, __nv_bfloat16, float>::type;
-
-__device__ __forceinline__ float to_f32(float v) { return v; }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ void put(float* p, float v) { *p = v; }
-__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
 // (float(a0) * s0 * w, float(a1) * s1 * w): two tokens' sums scaled, with packed products.
 __device__ __forceinline__ void scale_pair(int a0, int a1, uint64_t s2, uint64_t w2, float& v0, float& v1) {
@@ -488,7 +484,8 @@ __global__ void __cluster_dims__(2 * kS, 1, 1) __launch_bounds__(kThreads, 1)
       if (!ok && lane == 0) sh.failed[acc] = 1;
       named_bar_sync(1, kEpilogueWarps * 32);  // the scales are there; and all warps go on with this tile or none
       ok = sh.failed[acc] == 0;
-      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * kMaxN);
+      const uint32_t taddr =
+          tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * kMaxN);
       if constexpr (kS > 1) {
         // The pairs' sums over their parts of K: each finishes some units, and
         // has the others' sums of those brought to where its operands were.
@@ -560,7 +557,8 @@ __global__ void __cluster_dims__(2 * kS, 1, 1) __launch_bounds__(kThreads, 1)
           }
           const int nr = c < p.n ? tl.rows - j0 : 0;
           if (tma_residual && whole_unit(j0)) {
-            if (!mbar_wait(&sh.residual[e][slot], (slot_phase >> slot) & 1)) raise_error(p.err, kDevWaitTimeout, 89, t, j0);
+            if (!mbar_wait(&sh.residual[e][slot], (slot_phase >> slot) & 1))
+              raise_error(p.err, kDevWaitTimeout, 89, t, j0);
             slot_phase ^= 1u << slot;
             const float* in = reinterpret_cast<const float*>(stg + slot * kSlotBytes) + lane;
 #pragma unroll
@@ -585,110 +583,110 @@ __global__ void __cluster_dims__(2 * kS, 1, 1) __launch_bounds__(kThreads, 1)
         }
         continue;
       } else {
-      if (way * kUnit >= tl.rows) release();
-      for (int j0 = way * kUnit; j0 < tl.rows; j0 += kWays * kUnit) {
-        if (kS > 1 && owner(j0 / kPart) != part) continue;
-        int a[2][16];  // [16 lanes][the four blocks' four values]
-        tmem_ld_16x32(taddr + j0, a[0]);
-        tmem_ld_16x32(taddr + (16u << 16) + j0, a[1]);
-        const int64_t row = tl.row0 + j0;
-        const int nr = tl.rows - j0;
-        tmem_ld_wait(a[0], a[1]);
-        if constexpr (kS > 1) {
-          add_parts(j0 / kPart, a[0], 0, 16);
-          add_parts(j0 / kPart, a[1], 16, 16);
-        }
-        if (j0 + kWays * kUnit >= tl.rows) release();
-        xbuf ^= 1;
-        const bool whole = nr >= kUnit && c0 + 32 <= p.n;
-        Block v[4];
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const uint64_t s = *reinterpret_cast<const uint64_t*>(&sh.x_scale[acc][j0 + 8 * b + tc]);
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            scale_pair(a[q >> 1][4 * b + 2 * (q & 1)], a[q >> 1][4 * b + 2 * (q & 1) + 1], s, ws[q], v[b][2 * q],
-                       v[b][2 * q + 1]);
-        }
-        // Blocks first .. first + kOut - 1 of the unit are this warp's to store.
-        constexpr int kOut = kGated ? 2 : 4;
-        int first = 0;
-        if (kGated) {
-          // The gate's warp finishes the unit's first two blocks, the up's warp the others.
-          first = gate ? 0 : 2;
-          float4* give = xch + xbuf * (kXchBytes / 16);
-          const float4* take = xch_other + xbuf * (kXchBytes / 16);
-#pragma unroll
-          for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const Block& o = gate ? v[2 + b] : v[b];
-              give[(2 * b + h) * 32 + lane] = make_float4(o[4 * h], o[4 * h + 1], o[4 * h + 2], o[4 * h + 3]);
-            }
-          named_bar_sync(2 + (quarter & 1) + 2 * way, 64);
-#pragma unroll
-          for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float4 w4 = take[(2 * b + h) * 32 + lane];
-              const float w[4] = {w4.x, w4.y, w4.z, w4.w};
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float own = gate ? v[b][4 * h + i] : v[2 + b][4 * h + i];
-                v[b][4 * h + i] = silu_mul(gate ? own : w[i], gate ? w[i] : own);
-              }
-            }
-        } else {
-          if (has_bias) {
-#pragma unroll
-            for (int b = 0; b < 4; ++b)
-#pragma unroll
-              for (int i = 0; i < 8; ++i) v[b][i] += cur.bias[i / 2];
+        if (way * kUnit >= tl.rows) release();
+        for (int j0 = way * kUnit; j0 < tl.rows; j0 += kWays * kUnit) {
+          if (kS > 1 && owner(j0 / kPart) != part) continue;
+          int a[2][16];  // [16 lanes][the four blocks' four values]
+          tmem_ld_16x32(taddr + j0, a[0]);
+          tmem_ld_16x32(taddr + (16u << 16) + j0, a[1]);
+          const int64_t row = tl.row0 + j0;
+          const int nr = tl.rows - j0;
+          tmem_ld_wait(a[0], a[1]);
+          if constexpr (kS > 1) {
+            add_parts(j0 / kPart, a[0], 0, 16);
+            add_parts(j0 / kPart, a[1], 16, 16);
           }
-          if (has_residual) {
-            const T* res = static_cast<const T*>(p.residual) + (row + tc) * p.ldr + c;
-            Block r[4];
+          if (j0 + kWays * kUnit >= tl.rows) release();
+          xbuf ^= 1;
+          const bool whole = nr >= kUnit && c0 + 32 <= p.n;
+          Block v[4];
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            const uint64_t s = *reinterpret_cast<const uint64_t*>(&sh.x_scale[acc][j0 + 8 * b + tc]);
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              scale_pair(a[q >> 1][4 * b + 2 * (q & 1)], a[q >> 1][4 * b + 2 * (q & 1) + 1], s, ws[q], v[b][2 * q],
+                         v[b][2 * q + 1]);
+          }
+          // Blocks first .. first + kOut - 1 of the unit are this warp's to store.
+          constexpr int kOut = kGated ? 2 : 4;
+          int first = 0;
+          if (kGated) {
+            // The gate's warp finishes the unit's first two blocks, the up's warp the others.
+            first = gate ? 0 : 2;
+            float4* give = xch + xbuf * (kXchBytes / 16);
+            const float4* take = xch_other + xbuf * (kXchBytes / 16);
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const Block& o = gate ? v[2 + b] : v[b];
+                give[(2 * b + h) * 32 + lane] = make_float4(o[4 * h], o[4 * h + 1], o[4 * h + 2], o[4 * h + 3]);
+              }
+            named_bar_sync(2 + (quarter & 1) + 2 * way, 64);
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const float4 w4 = take[(2 * b + h) * 32 + lane];
+                const float w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const float own = gate ? v[b][4 * h + i] : v[2 + b][4 * h + i];
+                  v[b][4 * h + i] = silu_mul(gate ? own : w[i], gate ? w[i] : own);
+                }
+              }
+          } else {
+            if (has_bias) {
+#pragma unroll
+              for (int b = 0; b < 4; ++b)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[b][i] += cur.bias[i / 2];
+            }
+            if (has_residual) {
+              const T* res = static_cast<const T*>(p.residual) + (row + tc) * p.ldr + c;
+              Block r[4];
+              if (whole) {
+#pragma unroll
+                for (int b = 0; b < 4; ++b) load_block(r[b], res + 8 * b * p.ldr, p.ldr);
+              } else {
+#pragma unroll
+                for (int b = 0; b < 4; ++b) load_block(r[b], res + 8 * b * p.ldr, p.ldr, nr - tc - 8 * b, nc);
+              }
+#pragma unroll
+              for (int b = 0; b < 4; ++b)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[b][i] += r[b][i];
+            }
+          }
+          if (kBf16 && args.tma_store && nr >= 8 * (first + kOut)) {
+            // The buffers alternate with the groups that are committed: a unit
+            // stored directly (a tile's partial end) commits none and takes none,
+            // else the wait would let the one store still pending be this buffer's.
+            obuf ^= 1;
+            unsigned char* out = stg + obuf * (kOut * 8 * 64);
+            if (elect_one()) bulk_wait_read<1>();  // the store before the last has read this buffer
+            __syncwarp();
+#pragma unroll
+            for (int b = 0; b < kOut; ++b) stage_block(v[b], out, b, lane);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (elect_one()) {
+              if (c0 < p.n) tma_store_2d(&args.y, static_cast<int>(c0), static_cast<int>(row) + 8 * first, out);
+              bulk_commit();
+            }
+          } else {
+            T* dst = y + (row + 8 * first + tc) * p.ldy + c;
             if (whole) {
 #pragma unroll
-              for (int b = 0; b < 4; ++b) load_block(r[b], res + 8 * b * p.ldr, p.ldr);
+              for (int b = 0; b < kOut; ++b) store_block(v[b], dst + 8 * b * p.ldy, p.ldy);
             } else {
 #pragma unroll
-              for (int b = 0; b < 4; ++b) load_block(r[b], res + 8 * b * p.ldr, p.ldr, nr - tc - 8 * b, nc);
+              for (int b = 0; b < kOut; ++b)
+                store_block(v[b], dst + 8 * b * p.ldy, p.ldy, nr - tc - 8 * (first + b), nc);
             }
-#pragma unroll
-            for (int b = 0; b < 4; ++b)
-#pragma unroll
-              for (int i = 0; i < 8; ++i) v[b][i] += r[b][i];
           }
         }
-        if (kBf16 && args.tma_store && nr >= 8 * (first + kOut)) {
-          // The buffers alternate with the groups that are committed: a unit
-          // stored directly (a tile's partial end) commits none and takes none,
-          // else the wait would let the one store still pending be this buffer's.
-          obuf ^= 1;
-          unsigned char* out = stg + obuf * (kOut * 8 * 64);
-          if (elect_one()) bulk_wait_read<1>();  // the store before the last has read this buffer
-          __syncwarp();
-#pragma unroll
-          for (int b = 0; b < kOut; ++b) stage_block(v[b], out, b, lane);
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (elect_one()) {
-            if (c0 < p.n) tma_store_2d(&args.y, static_cast<int>(c0), static_cast<int>(row) + 8 * first, out);
-            bulk_commit();
-          }
-        } else {
-          T* dst = y + (row + 8 * first + tc) * p.ldy + c;
-          if (whole) {
-#pragma unroll
-            for (int b = 0; b < kOut; ++b) store_block(v[b], dst + 8 * b * p.ldy, p.ldy);
-          } else {
-#pragma unroll
-            for (int b = 0; b < kOut; ++b)
-              store_block(v[b], dst + 8 * b * p.ldy, p.ldy, nr - tc - 8 * (first + b), nc);
-          }
-        }
-      }
       }
     }
     if (elect_one()) bulk_wait_read<0>();
@@ -843,8 +841,8 @@ cudaError_t launch(const W8a8& p, cudaStream_t stream) {
   if (p.row_index != nullptr) {
     ldx = (p.k + 15) / 16 * 16;
     const int64_t blocks = (p.rows + 7) / 8, most = static_cast<int64_t>(pairs) * 2 * 8;
-    st = launch_pdl(gather_rows_kernel, static_cast<unsigned>(blocks < most ? blocks : most), 256, 0, stream, p.x, p.ldx,
-                    p.x_rows, p.row_index, static_cast<int>(p.rows), static_cast<int>(p.groups),
+    st = launch_pdl(gather_rows_kernel, static_cast<unsigned>(blocks < most ? blocks : most), 256, 0, stream, p.x,
+                    p.ldx, p.x_rows, p.row_index, static_cast<int>(p.rows), static_cast<int>(p.groups),
                     static_cast<int>(ldx / 16), reinterpret_cast<uint4*>(p.workspace));
     if (st != cudaSuccess) return st;
     x = p.workspace;

@@ -50,15 +50,11 @@ __device__ __forceinline__ uint4 keep_bytes(uint4 v, int64_t bytes) {
   return v;
 }
 
-__device__ __forceinline__ float to_f32(float v) { return v; }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ void put(float* p, float v) { *p = v; }
-__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
-
 // kTiles: tiles of 8 tokens a warp takes at a time. kSplit: warps that share
 // 16 weight rows. T: y's type. blocks: (groups that have rows) x n_blocks.
 template <bool kGated, int kTiles, int kSplit, typename T>
-__global__ void __launch_bounds__(kThreads, kSplit == 8 ? (kGated ? 3 : 2) : 4) w8a8_rows_kernel(const W8a8 p, int n_blocks) {
+__global__ void __launch_bounds__(kThreads, kSplit == 8 ? (kGated ? 3 : 2) : 4)
+    w8a8_rows_kernel(const W8a8 p, int n_blocks) {
   constexpr int kMats = kGated ? 2 : 1;
   constexpr int kDeep = (kSplit == 8 && kTiles < 4 ? 4 : 2) / kMats;  // steps in flight (as many as registers hold)
   __shared__ int part[kWarps][kMats * kTiles][32][4];

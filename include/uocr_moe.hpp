@@ -86,8 +86,6 @@ inline void linear(void* stream, const float* x, std::int64_t m, std::int64_t k,
   check(uocr_linear(x, m, k, w_bf16, n, bias, y, stream));
 }
 
-// ---- owners ------------------------------------------------------------------
-
 // The 8-bit integer operators (uocr_int8.h) on the stream, with the same exceptions.
 inline void quantize_tokens(void* stream, const void* x, uocr_dtype dtype, std::int64_t rows, std::int64_t cols,
                             std::int64_t ldx, std::int8_t* q, std::int64_t ldq, float* scales) {
@@ -102,6 +100,8 @@ inline std::int64_t grouped_w8a8_workspace(const uocr_grouped_w8a8_args& args) {
 inline void grouped_linear_w8a8(void* stream, const uocr_grouped_w8a8_args& args) {
   check(uocr_grouped_linear_w8a8(&args, stream));
 }
+
+// ---- owners ------------------------------------------------------------------
 
 class Checkpoint;
 
