@@ -2,9 +2,17 @@
 //
 // s = max|x| * fl(1 / 127), q = rint(x / s) with the quotient as an IEEE
 // division rounds it, whatever the variant below. (quantize_rows_kernel in
-// weights.cu divides the maximum by 127: its s may differ in the last bit.)
+// weights.cu divides the maximum by 127: its s may differ in the last bit. The
+// product is what elementwise tensor code makes of a division by a constant, so
+// that a caller who quantises that way has the same bits.)
 // |x| / s is at most 127 (1 + 2^-22), so nothing is clamped. One pass: a thread
 // keeps its part of the row in registers between the maximum and the rounding.
+//
+// Bound by bytes in fp32 (32768 x 2048: 49 us, the card's copy rate) and by
+// latency in bf16, whose rows take as long with half the bytes (54 us; 4096 x
+// 2048 6.9, 1.8 times its floor): a block's loads are out at once and nothing of
+// the next row is, so that its warps mostly wait for them (39 % of DRAM, 52 % of
+// the issue slots, the ALUs 45 %).
 #include <cfloat>
 
 #include "ptx.cuh"
@@ -181,8 +189,8 @@ template <bool kAligned, typename T>
 cudaError_t choose(const T* x, int64_t rows, int cols, int64_t ldx, int8_t* q, int64_t ldq, float* scales,
                    cudaStream_t stream) {
   // Two chunks a thread: enough in flight, and few idle threads. Measured in us:
-  // 4096 x 2048 bf16 12.3 by a warp a row, 7.5 by 128 threads, 8.1 by 256 of one
-  // chunk (3.85 at the card's copy rate); 24576 x 1024 bf16 27 by a warp, 23 by
+  // 4096 x 2048 bf16 12.3 by a warp a row, 7.5 by 128 threads (since then 6.9), 8.1 by
+  // 256 of one chunk (3.85 at the card's copy rate); 24576 x 1024 bf16 27 by a warp, 23 by
   // 64 threads; 32768 x 2048 fp32 49.5 by 128 threads (the copy rate: 51). Few
   // rows are a matter of latency: 1 x 2048 1.6 by 256 threads, 5.5 by a warp.
   if (cols <= 512) return launch<32, 2, kAligned>(x, rows, cols, ldx, q, ldq, scales, stream);

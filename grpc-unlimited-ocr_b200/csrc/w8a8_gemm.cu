@@ -34,8 +34,13 @@
 // nearly all of its bandwidth (64 + 64 bytes a clock at the full MMA rate), and
 // every store and shared-memory access of the epilogue takes a clock of the
 // same pipe: the layout is chosen for few and full ones. Measured at 8192 x
-// 8192 x 4096: 171 us, 3200 TOP/s, the tensor pipe active for 85 % of the time.
-// With few slices of K the copies bound it, at 55 bytes a clock into each SM:
+// 8192 x 4096: 171 us, 3200 TOP/s, the tensor pipe active for 87 % of the time.
+// Two forms of the epilogue go by single bf16 values, a warp's access being four
+// tokens x 8 channels, 16 bytes together: outputs whose rows do not start at 16
+// bytes (8192 x 2047 x 64 23.5 us, with 2048 12.5; 24576 rows of 64 groups by 1001 x
+// 1024 41.8, by 1008 30.9, gated 67.5 and 57.4), and bf16 residuals, read when the
+// sums are there (4096 x 2048 x 2048 23.7 us, without 17.3; fp32 22.6 and 20.1).
+// With few slices of K the copies bound the product, at 55 bytes a clock into each SM:
 // at 8192 x 8192 x 1024 the MMAs alone take 57 kcycles, the copies alone 67, all
 // but the stores 81, the whole 91.
 #include <algorithm>
@@ -908,6 +913,15 @@ namespace {
 // rows 7.6 / 12.1, 60 rows 37 / 38, 240 rows 46 / 52; 64 of 2048 x 1024, 6 rows
 // 6.2 / 9.7, 96 rows 23.5 / 25.7, 240 rows 30.5 / 29.7; 16 of 1024 x 2048, 32
 // rows 9.7 / 11.5, 128 rows 14.8 / 11.5; 8 of those, 30 rows 7.7 / 9.8, 60 9.8 / 9.9.
+// These groups were routed at random. The rule has only their mean size, the sizes
+// being on the device, and that kernel reads a group's weights again for every 8
+// of its rows. 64 groups of 2048 x 1024, then gated ones of 1024 x 2048 with a row
+// index: 96 rows, all groups alike, 29.0 / 25.7 and 45.0 / 52.0, in four groups
+// 16.0 / 7.2 and 35.4 / 12.9, in one 43.8 / 7.5 and 111 / 13.9; 256 rows in one
+// group 112 / 8.9 and 274 / 16.4.
+// Dense gated products (a layer's shared expert) have no form for more than 8
+// rows at a time there: a layer with one of 2 x 2048 x 2048 takes 121.7 us at 17 rows and
+// 155.2 at 32, with that product here 116.6 and 146.2.
 bool few_rows_grouped(int64_t rows, int64_t groups) { return rows <= 256 && rows <= 4 * groups; }
 bool few_rows(const W8a8& p) {
   if (p.starts != nullptr) return few_rows_grouped(p.rows, p.groups);

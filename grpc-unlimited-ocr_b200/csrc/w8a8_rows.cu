@@ -1,5 +1,5 @@
-// W8A8 products of a few rows (include/uocr_int8.h): the weights are streamed
-// once, at most kTiles * 8 tokens at a time against them.
+// W8A8 products of a few rows (include/uocr_int8.h): the weights of a group are
+// streamed once for every kTiles * 8 of its rows (grouped and gated products: 8).
 //
 // A warp takes 16 weight rows of one group (gate and up rows when gated) and
 // all of K or a part of it, with mma.sync m16n8k32 on signed bytes: A = 16
@@ -52,6 +52,11 @@ __device__ __forceinline__ uint4 keep_bytes(uint4 v, int64_t bytes) {
 
 // kTiles: tiles of 8 tokens a warp takes at a time. kSplit: warps that share
 // 16 weight rows. T: y's type. blocks: (groups that have rows) x n_blocks.
+// The bounds on registers cost up to 76 bytes of spills (kSplit 4, and 8 when
+// gated) for a block more on each SM. In us as it is / with one block fewer,
+// spilling nothing: 1 row by 16384 x 2048 8.2 / 10.2, by 102400 x 2048 36.8 / 39.8;
+// 6 rows of 64 gated groups of 1024 x 2048 7.9 / 9.8, 18 rows 15.2 / 18.2; but
+// 1 row by 12000 x 2048 7.4 / 5.5, 24 rows of 12 such groups 13.2 / 11.8.
 template <bool kGated, int kTiles, int kSplit, typename T>
 __global__ void __launch_bounds__(kThreads, kSplit == 8 ? (kGated ? 3 : 2) : 4)
     w8a8_rows_kernel(const W8a8 p, int n_blocks) {
