@@ -1204,6 +1204,24 @@ int uocr_ops_check(void* stream) {
                   "grouped_linear_w8a8: the rows of group %d (from row %d) are not in order or out of range", e.a, e.b);
   else if (e.code == kDevBadIndex && e.where == kSiteRowIndex)
     std::snprintf(buf, sizeof(buf), "grouped_linear_w8a8: row %d reads row %d, which x does not have", e.a, e.b);
+  else if (e.code == kDevBadIndex && e.where == kSiteCachePlace)
+    std::snprintf(buf, sizeof(buf), "rotate_heads: row %d goes to cache or slot %d, which does not exist", e.a, e.b);
+  else if (e.code == kDevBadIndex && e.where == kSiteLength && e.a < 0)
+    std::snprintf(buf, sizeof(buf), "prefix_attention: prefix %d has %d keys, more than fit or fewer than none",
+                  -1 - e.a, e.b);
+  else if (e.code == kDevBadIndex && e.where == kSiteLength)
+    std::snprintf(buf, sizeof(buf), "prefix_attention: sequence %d has %d own keys, more than fit or fewer than none",
+                  e.a, e.b);
+  else if (e.code == kDevBadIndex && e.where == kSiteRowOffsets)
+    std::snprintf(buf, sizeof(buf), "prefix_attention: the rows of sequence %d (from row %d) are not in order or out of range",
+                  e.a, e.b);
+  else if (e.code == kDevBadIndex && e.where == kSiteAncestor)
+    std::snprintf(buf, sizeof(buf), "prefix_attention: a key of sequence %d lies in cache %d, which does not exist", e.a,
+                  e.b);
+  else if (e.code == kDevBadIndex && e.where == kSiteParent)
+    std::snprintf(buf, sizeof(buf), "reorder_states: row %d has parent %d, which does not exist", e.a, e.b);
+  else if (e.code == kDevBadIndex && e.where == kSiteCount)
+    std::snprintf(buf, sizeof(buf), "reorder_states: row %d holds %d units, more than fit or fewer than none", e.a, e.b);
   else
     std::snprintf(buf, sizeof(buf), "device error %d at site %d (%d, %d)", e.code, e.where, e.a, e.b);
   return fail(e.code == kDevWaitTimeout ? UOCR_ERR_TIMEOUT : UOCR_ERR_DEVICE, buf);

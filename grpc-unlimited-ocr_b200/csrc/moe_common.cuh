@@ -34,6 +34,12 @@ struct ErrorWord {
 // Sites (ErrorWord::where) that uocr_ops_check words its message by.
 constexpr int kSiteGroupRows = 80;  // a: group, b: its first row
 constexpr int kSiteRowIndex = 81;   // a: output row, b: the row it names
+constexpr int kSiteCachePlace = 82;  // a: row, b: its cache or slot
+constexpr int kSiteLength = 83;      // a: sequence (prefixes as -1 - prefix), b: its length
+constexpr int kSiteRowOffsets = 84;  // a: sequence, b: its first row
+constexpr int kSiteAncestor = 85;    // a: sequence, b: the cache it names
+constexpr int kSiteParent = 86;      // a: state row, b: its parent
+constexpr int kSiteCount = 87;       // a: state row, b: its units
 __device__ inline void raise_error(ErrorWord* e, int code, int where, int a, int b) {
   if (atomicCAS(&e->code, 0, code) == 0) {
     e->where = where;

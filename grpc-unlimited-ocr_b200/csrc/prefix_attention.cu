@@ -1,0 +1,533 @@
+// Attention of sequences that share prefixes (uocr_prefix_attention): the
+// kernel for few rows, the join of partial results, and the choice of parts.
+//
+// With the rows of all sequences behind a prefix in one tile, the prefix's keys
+// and values are read once for all of them. A softmax over a set of keys is the
+// join of softmaxes over parts of it: from (m_i, l_i, o_i), the parts' maxima,
+// sums of exp(s - m_i) and unnormalised outputs,
+//   m = max m_i,  l = sum l_i exp(m_i - m),  o = sum o_i exp(m_i - m) / l.
+// So prefixes and own keys are cut into parts that fill the card, each block
+// takes one part of one tile of rows, and a second kernel joins a row's parts.
+#include <algorithm>
+
+#include "prefix_attention.cuh"
+#include "w8a8.h"
+
+namespace uocr_b200 {
+namespace {
+
+constexpr int kThreads = 128;
+constexpr int kKeys = 64;    // of a stage
+constexpr int kStages = 3;
+
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], const void* p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(smem_addr(p))
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], const void* p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(smem_addr(p))
+               : "memory");
+}
+// 16 bytes, or zeros where `valid` is false (the source is not read then).
+__device__ __forceinline__ void cp_async16_or_zero(void* dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(valid ? 16 : 0)
+               : "memory");
+}
+template <int kPending>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
+}
+
+// What a block works on: rows x heads of one key/value head (vr = row * group +
+// head, `count` of them from `start`), and a range of keys.
+struct Tile {
+  int first_row;  // of the rows below
+  int start, count;
+  int kv_head;
+  int key0, key1;     // the block's part
+  int limit0;         // keys the row at first_row sees; each row after it sees one more (own keys), or the same
+  int all_see;        // keys that every row of the tile sees
+  bool own;
+  int sequence, slot;
+  const __nv_bfloat16* k;  // of key 0 (without ancestry)
+  const __nv_bfloat16* v;
+};
+
+// Blocks [0, prefix_blocks) take prefixes, the others own keys. Tiles are
+// counted through over the prefixes (sequences): ceil(rows * group / kRows) of
+// each, then the key/value heads, then the parts.
+struct Grid {
+  int prefix_tiles, own_tiles;  // bounds: with row offsets the rows are known to the device alone
+  int prefix_blocks;
+  int own_slots;
+};
+
+// Finds the sequence (prefix) that tile `t` is of; -1 behind the last one.
+template <int kRows, typename RowsOf>
+__device__ int find_tile(int t, int count, const Attention& a, RowsOf rows, int* local, int* first, int* n) {
+  const int lane = threadIdx.x & 31;
+  for (int b0 = 0; b0 < count; b0 += 32) {
+    int r0 = 0;
+    const int mine = b0 + lane < count ? rows(b0 + lane, &r0) : 0;
+    const int tiles = (mine * a.group + kRows - 1) / kRows;
+    int end = tiles;
+#pragma unroll
+    for (int off = 1; off < 32; off *= 2) {
+      const int other = __shfl_up_sync(0xffffffffu, end, off);
+      if (lane >= off) end += other;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, t < end);
+    if (hit != 0) {
+      const int src = __ffs(hit) - 1;
+      *local = t - __shfl_sync(0xffffffffu, end - tiles, src);
+      *first = __shfl_sync(0xffffffffu, r0, src);
+      *n = __shfl_sync(0xffffffffu, mine, src);
+      return b0 + src;
+    }
+    t -= __shfl_sync(0xffffffffu, end, 31);
+  }
+  return -1;
+}
+
+template <int kDim, int kRows>
+__device__ bool find_work(const Attention& a, const Grid& g, Tile* w) {
+  const int block = blockIdx.x;
+  w->own = block >= g.prefix_blocks;
+  int b = w->own ? block - g.prefix_blocks : block;
+  const int parts = w->own ? g.own_slots : a.prefix_slots;
+  const int part = b % parts;
+  b /= parts;
+  w->kv_head = b % a.kv_heads;
+  const int tile = b / a.kv_heads;
+  int local, n, of;
+  if (w->own)
+    of = find_tile<kRows>(tile, a.sequences, a, [&](int i, int* r0) { return rows_of(a, i, r0); }, &local,
+                          &w->first_row, &n);
+  else
+    of = find_tile<kRows>(tile, a.prefixes, a, [&](int i, int* r0) { return prefix_rows_of(a, i, r0); }, &local,
+                          &w->first_row, &n);
+  if (of < 0) return false;
+  w->start = local * kRows;
+  w->count = min(kRows, n * a.group - w->start);
+  w->sequence = of;
+  w->slot = w->own ? a.prefix_slots + part : part;
+  int keys;
+  if (w->own) {
+    const int len = len_of(a, of);
+    w->limit0 = len - n + 1;
+    // the tile's last row sees the most
+    keys = max(0, w->limit0 + (w->start + w->count - 1) / a.group);
+    w->all_see = w->limit0 + w->start / a.group;
+    w->k = a.k + of * a.cache_stride + w->kv_head * a.head_stride;
+    w->v = a.v + of * a.cache_stride + w->kv_head * a.head_stride;
+  } else {
+    keys = w->limit0 = w->all_see = prefix_len_of(a, of);
+    w->k = a.prefix_k + of * a.prefix_stride + w->kv_head * a.prefix_head_stride;
+    w->v = a.prefix_v + of * a.prefix_stride + w->kv_head * a.prefix_head_stride;
+  }
+  const int stages = (keys + kKeys - 1) / kKeys, each = (stages + parts - 1) / parts;
+  w->key0 = min(keys, part * each * kKeys);
+  w->key1 = min(keys, w->key0 + each * kKeys);
+  return true;
+}
+
+// 4 warps: kWarpRows of them side by side along the rows (16 each), the others
+// along a stage's keys, each with its own running maximum, sum and output in
+// registers; keys and values in a ring of padded stages filled by cp.async.
+// mma.sync and not tcgen05: a tile has 16 to 64 rows, of which a tcgen05 tile
+// would use an eighth to a half.
+template <int kDim, int kWarpRows>
+__global__ void __launch_bounds__(kThreads) attention_rows_kernel(Attention a, Grid g) {
+  constexpr int kRows = 16 * kWarpRows, kWarpKeys = kKeys / (4 / kWarpRows);
+  constexpr int kPitch = kDim + 8;  // padded: fragment loads without bank conflicts
+  constexpr int kStage = 2 * kKeys * kPitch;
+  extern __shared__ __align__(16) unsigned char raw[];
+  __nv_bfloat16* ring = reinterpret_cast<__nv_bfloat16*>(raw);
+  pdl_wait();
+  pdl_launch_dependents();
+  Tile w;
+  if (!find_work<kDim, kRows>(a, g, &w)) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int gr = lane >> 2, tq = lane & 3;
+  const int row0 = warp % kWarpRows * 16, warp_key = warp / kWarpRows * kWarpKeys;
+
+  auto fill = [&](int stage, int key) {
+    __nv_bfloat16* ks = ring + stage * kStage;
+    __nv_bfloat16* vs = ks + kKeys * kPitch;
+    for (int c = threadIdx.x; c < kKeys * (kDim / 8); c += kThreads) {
+      const int r = c / (kDim / 8), col = c % (kDim / 8) * 8;
+      const int at = key + r;
+      const bool valid = at < w.key1;
+      const __nv_bfloat16 *k = w.k, *v = w.v;
+      if (w.own && valid && a.ancestry != nullptr) {
+        int cache = a.ancestry[w.sequence * a.ld_ancestry + at];
+        if (cache < 0 || cache >= a.caches) {
+          raise_error(a.err, kDevBadIndex, kSiteAncestor, w.sequence, cache);
+          cache = w.sequence < a.caches ? w.sequence : 0;
+        }
+        const int64_t base = cache * a.cache_stride + w.kv_head * a.head_stride;
+        k = a.k + base;
+        v = a.v + base;
+      }
+      const int64_t off = valid ? static_cast<int64_t>(at) * kDim + col : 0;
+      cp_async16_or_zero(ks + r * kPitch + col, (valid ? k : a.q) + off, valid);
+      cp_async16_or_zero(vs + r * kPitch + col, (valid ? v : a.q) + off, valid);
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) {
+    if (w.key0 + s * kKeys < w.key1) fill(s, w.key0 + s * kKeys);
+    cp_async_commit();
+  }
+
+  // This thread's two rows of the warp's tile, and the warp's queries as A fragments.
+  int limit[2];
+  const __nv_bfloat16* src[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int vr = w.start + row0 + gr + 8 * i;
+    const bool valid = row0 + gr + 8 * i < w.count;
+    const int row = vr / a.group, head = w.kv_head * a.group + vr % a.group;
+    limit[i] = !valid ? 0 : w.own ? w.limit0 + row : w.limit0;
+    src[i] = valid ? a.q + (w.first_row + row) * a.ldq + head * kDim : nullptr;
+  }
+  uint32_t qa[kDim / 16][4];
+#pragma unroll
+  for (int kk = 0; kk < kDim / 16; ++kk)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      qa[kk][i] = src[i & 1] != nullptr
+                      ? *reinterpret_cast<const uint32_t*>(src[i & 1] + kk * 16 + (i >> 1) * 8 + 2 * tq)
+                      : 0u;
+  float o[kDim / 8][4];
+#pragma unroll
+  for (int d = 0; d < kDim / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.0f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+  __shared__ uint32_t odd_keys[kKeys / 32];  // keys of the stage with a value that is no finite number
+
+  int stage = 0;
+  for (int key = w.key0; key < w.key1; key += kKeys) {
+    cp_async_wait<kStages - 2>();
+    __syncthreads();  // the stage has landed for all, and the one filled next has been read by all
+    const int ahead = key + (kStages - 1) * kKeys;
+    if (ahead < w.key1) fill((stage + kStages - 1) % kStages, ahead);
+    cp_async_commit();
+    const __nv_bfloat16* ks = ring + stage * kStage + warp_key * kPitch;
+    const __nv_bfloat16* vs = ks + kKeys * kPitch;
+    stage = (stage + 1) % kStages;
+    float s[kWarpKeys / 8][4];
+#pragma unroll
+    for (int nt = 0; nt < kWarpKeys / 8; nt += 2) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[nt][e] = s[nt + 1][e] = 0.0f;
+#pragma unroll
+      for (int kk = 0; kk < kDim / 16; ++kk) {
+        // matrices: keys nt * 8 .. + 7 at dims 0-7 and 8-15, then the next 8 keys
+        uint32_t b[4];
+        ldmatrix_x4(b, ks + (nt * 8 + (lane & 7) + (lane >> 4) * 8) * kPitch + kk * 16 + (lane >> 3 & 1) * 8);
+        mma_bf16(s[nt], qa[kk], b[0], b[1]);
+        mma_bf16(s[nt + 1], qa[kk], b[2], b[3]);
+      }
+    }
+    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int nt = 0; nt < kWarpKeys / 8; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int at = key + warp_key + nt * 8 + 2 * tq + (e & 1);
+        s[nt][e] = at < min(limit[e >> 1], w.key1) ? s[nt][e] * a.scale_log2 : -INFINITY;
+        top[e >> 1] = fmaxf(top[e >> 1], s[nt][e]);
+      }
+    float alpha[2], shift[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+      top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+      top[i] = fmaxf(m[i], top[i]);
+      shift[i] = top[i] == -INFINITY ? 0.0f : top[i];  // no key yet: 2^(-inf - 0) = 0
+      alpha[i] = exp2_fast(m[i] - shift[i]);
+      m[i] = top[i];
+      l[i] *= alpha[i];
+    }
+#pragma unroll
+    for (int nt = 0; nt < kWarpKeys / 8; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[nt][e] = exp2_fast(s[nt][e] - shift[e >> 1]);
+        l[e >> 1] += s[nt][e];
+      }
+#pragma unroll
+    for (int d = 0; d < kDim / 8; ++d) {
+      o[d][0] *= alpha[0];
+      o[d][1] *= alpha[0];
+      o[d][2] *= alpha[1];
+      o[d][3] *= alpha[1];
+    }
+    // A key that only some of the tile's rows see has the weight 0 in the others, which an infinite or NaN value
+    // would turn into a NaN: such values are added apart, where they are seen, and are 0 in the products.
+    if (key + kKeys > w.all_see && w.all_see < w.key1) {
+      __nv_bfloat16* whole = ring + ((stage + kStages - 1) % kStages) * kStage + kKeys * kPitch;
+      if (threadIdx.x < kKeys / 32) odd_keys[threadIdx.x] = 0;
+      __syncthreads();
+      bool odd = false;
+      for (int c = threadIdx.x; c < kKeys * (kDim / 2); c += kThreads) {
+        const int r = c / (kDim / 2);
+        const uint32_t u = *reinterpret_cast<const uint32_t*>(whole + r * kPitch + c % (kDim / 2) * 2);
+        if ((u & 0x7f80u) == 0x7f80u || (u & 0x7f800000u) == 0x7f800000u) {
+          atomicOr(&odd_keys[r / 32], 1u << (r & 31));
+          odd = true;
+        }
+      }
+      if (__syncthreads_or(odd)) {
+#pragma unroll
+        for (int nt = 0; nt < kWarpKeys / 8; ++nt)
+#pragma unroll
+          for (int col = 0; col < 8; ++col) {
+            const int r = warp_key + nt * 8 + col;
+            if ((odd_keys[r / 32] >> (r & 31) & 1) == 0) continue;
+            const float p[2] = {__shfl_sync(0xffffffffu, s[nt][col & 1], gr * 4 + col / 2),
+                                __shfl_sync(0xffffffffu, s[nt][2 + (col & 1)], gr * 4 + col / 2)};
+#pragma unroll
+            for (int d = 0; d < kDim / 8; ++d)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float v = __bfloat162float(whole[r * kPitch + d * 8 + 2 * tq + (e & 1)]);
+                if (!isfinite(v) && key + r < limit[e >> 1]) o[d][e] = fmaf(p[e >> 1], v, o[d][e]);
+              }
+          }
+        __syncthreads();
+        for (int c = threadIdx.x; c < kKeys * kDim; c += kThreads) {
+          __nv_bfloat16* v = whole + c / kDim * kPitch + c % kDim;
+          if (!isfinite(__bfloat162float(*v))) *v = __float2bfloat16_rn(0.0f);
+        }
+        __syncthreads();
+      }
+    }
+#pragma unroll
+    for (int kk = 0; kk < kWarpKeys / 16; ++kk) {
+      // The weights as the tensor cores take them: rounded to bf16, like the values they meet.
+      const uint32_t p[4] = {pack2(s[2 * kk][0], s[2 * kk][1]), pack2(s[2 * kk][2], s[2 * kk][3]),
+                             pack2(s[2 * kk + 1][0], s[2 * kk + 1][1]), pack2(s[2 * kk + 1][2], s[2 * kk + 1][3])};
+#pragma unroll
+      for (int d = 0; d < kDim / 8; d += 2) {
+        uint32_t b[4];
+        ldmatrix_x4_trans(b, vs + (kk * 16 + (lane & 15)) * kPitch + d * 8 + (lane >> 4) * 8);
+        mma_bf16(o[d], p, b[0], b[1]);
+        mma_bf16(o[d + 1], p, b[2], b[3]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+  }
+  auto cell = [&](int r) {  // of the tile's row r
+    const int vr = w.start + r;
+    const int64_t row = w.first_row + vr / a.group;
+    return (row * a.heads + w.kv_head * a.group + vr % a.group) * a.slots + w.slot;
+  };
+  if constexpr (kWarpRows == 4) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = row0 + gr + 8 * i;
+      if (r >= w.count) continue;
+      const int64_t at = cell(r);
+      if (tq == 0) a.part_ml[at] = make_float2(m[i], l[i]);
+#pragma unroll
+      for (int d = 0; d < kDim / 8; ++d)
+        *reinterpret_cast<float2*>(a.part_o + at * kDim + d * 8 + 2 * tq) = make_float2(o[d][2 * i], o[d][2 * i + 1]);
+    }
+  } else {
+    // The warps along the keys are joined in shared memory, in the ring's place.
+    constexpr int kAlong = 4 / kWarpRows;
+    float* os = reinterpret_cast<float*>(raw);                    // [kAlong][kRows][kDim]
+    float2* mls = reinterpret_cast<float2*>(os + kAlong * kRows * kDim);  // [kAlong][kRows]
+    cp_async_wait_all();
+    __syncthreads();
+    const int along = warp / kWarpRows;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = row0 + gr + 8 * i;
+      if (tq == 0) mls[along * kRows + r] = make_float2(m[i], l[i]);
+#pragma unroll
+      for (int d = 0; d < kDim / 8; ++d)
+        *reinterpret_cast<float2*>(os + (along * kRows + r) * kDim + d * 8 + 2 * tq) =
+            make_float2(o[d][2 * i], o[d][2 * i + 1]);
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < w.count * (kDim / 4); c += kThreads) {
+      const int r = c / (kDim / 4), col = c % (kDim / 4) * 4;
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < kAlong; ++i) top = fmaxf(top, mls[i * kRows + r].x);
+      const float shift = top == -INFINITY ? 0.0f : top;
+      float sum = 0.0f;
+      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int i = 0; i < kAlong; ++i) {
+        const float2 ml = mls[i * kRows + r];
+        const float f = exp2_fast(ml.x - shift);
+        const float4 v = *reinterpret_cast<const float4*>(os + (i * kRows + r) * kDim + col);
+        sum = fmaf(ml.y, f, sum);
+        acc.x = fmaf(v.x, f, acc.x), acc.y = fmaf(v.y, f, acc.y);
+        acc.z = fmaf(v.z, f, acc.z), acc.w = fmaf(v.w, f, acc.w);
+      }
+      const int64_t at = cell(r);
+      if (col == 0) a.part_ml[at] = make_float2(top, sum);
+      *reinterpret_cast<float4*>(a.part_o + at * kDim + col) = acc;
+    }
+  }
+}
+
+// A warp joins the parts of a (row, head).
+template <int kDim>
+__global__ void __launch_bounds__(kThreads) attention_join_kernel(Attention a) {
+  constexpr int kEach = kDim / 32;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int64_t cell = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (cell >= static_cast<int64_t>(a.rows) * a.heads) return;
+  const int64_t row = cell / a.heads;
+  const int head = static_cast<int>(cell % a.heads);
+  if (a.row_offsets != nullptr && (row < a.row_offsets[0] || row >= a.row_offsets[a.sequences])) return;
+  const float2* ml = a.part_ml + cell * a.slots;
+  float top = -INFINITY;
+  for (int s = lane; s < a.slots; s += 32) top = fmaxf(top, ml[s].x);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+  const float shift = top == -INFINITY ? 0.0f : top;
+  float sum = 0.0f, acc[kEach] = {};
+  const float* o = a.part_o + cell * a.slots * kDim + lane * kEach;
+#pragma unroll 4
+  for (int s = 0; s < a.slots; ++s) {
+    const float2 p = ml[s];
+    const float f = exp2_fast(p.x - shift);
+    sum = fmaf(p.y, f, sum);
+    if (p.x == -INFINITY) continue;  // a part without keys
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) acc[i] = fmaf(o[s * kDim + i], f, acc[i]);
+  }
+  const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+  __nv_bfloat16* out = a.out + row * a.ldo + head * kDim + lane * kEach;
+#pragma unroll
+  for (int i = 0; i < kEach; i += 2) *reinterpret_cast<uint32_t*>(out + i) = pack2(acc[i] * inv, acc[i + 1] * inv);
+  if (a.lse != nullptr && lane == 0)
+    a.lse[cell] = sum != 0.0f ? (top + log2f(sum)) * 0.69314718055994530942f : -INFINITY;
+}
+
+// The parts that the prefixes and the own keys are cut into. Blocks of about
+// `keys` keys: as many as fill the card's SMs twice where there are few tiles,
+// whole ranges where there are many.
+struct Plan {
+  int prefix_slots, own_slots, warp_rows;
+  int64_t prefix_tiles, own_tiles;
+};
+
+constexpr int kMaxPrefixSlots = 64, kMaxOwnSlots = 16;
+
+Plan plan_of(const uocr_prefix_attention_args& a) {
+  Plan p{};
+  const int64_t group = a.heads / a.kv_heads;
+  // Rows of a tile by the rows of a prefix: those of a sequence alone where there is no prefix.
+  const int64_t rows = a.rows * group / std::max<int64_t>(a.prefix_capacity > 0 ? a.prefixes : a.sequences, 1);
+  p.warp_rows = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  const int64_t tile = 16 * p.warp_rows;
+  auto tiles = [&](int64_t count, int64_t each) {
+    // With row offsets: each sequence's (prefix's) last tile may be part empty.
+    return a.row_offsets == nullptr ? count * ((each * group + tile - 1) / tile)
+                                    : a.rows * group / tile + std::min(count, a.rows);
+  };
+  p.prefix_tiles = a.prefix_capacity > 0 ? tiles(a.prefixes, a.sequences / a.prefixes) : 0;
+  p.own_tiles = a.capacity > 0 ? tiles(a.sequences, 1) : 0;
+  const int64_t bp = p.prefix_tiles * a.kv_heads, bo = p.own_tiles * a.kv_heads;
+  for (int64_t keys = 2 * kKeys;; keys *= 2) {
+    p.prefix_slots = static_cast<int>(std::min<int64_t>((a.prefix_capacity + keys - 1) / keys, kMaxPrefixSlots));
+    p.own_slots = static_cast<int>(std::min<int64_t>((a.capacity + keys - 1) / keys, kMaxOwnSlots));
+    if (bp * p.prefix_slots + bo * p.own_slots <= 2 * 148) break;
+    if (keys >= a.prefix_capacity && keys >= a.capacity) break;
+  }
+  return p;
+}
+
+template <int kDim, int kWarpRows>
+cudaError_t launch_rows(const Attention& a, const Grid& g, unsigned blocks, cudaStream_t stream) {
+  constexpr size_t kRing = static_cast<size_t>(kStages) * 2 * kKeys * (kDim + 8) * 2;
+  constexpr size_t kJoin = static_cast<size_t>(4 / kWarpRows) * 16 * kWarpRows * (kDim * 4 + 8);
+  static_assert(kJoin <= kRing, "the join takes the ring's place");
+  cudaError_t st = allow_max_dynamic_smem(attention_rows_kernel<kDim, kWarpRows>);
+  if (st != cudaSuccess) return st;
+  return launch_pdl(attention_rows_kernel<kDim, kWarpRows>, blocks, kThreads, kRing, stream, a, g);
+}
+
+template <int kDim>
+cudaError_t launch(const uocr_prefix_attention_args& args, const Attention& a, const Plan& p, cudaStream_t stream) {
+  Grid g{};
+  g.prefix_tiles = static_cast<int>(p.prefix_tiles);
+  g.own_tiles = static_cast<int>(p.own_tiles);
+  g.prefix_blocks = static_cast<int>(p.prefix_tiles * a.kv_heads * p.prefix_slots);
+  g.own_slots = p.own_slots;
+  const int64_t blocks = g.prefix_blocks + p.own_tiles * a.kv_heads * p.own_slots;
+  cudaError_t st = cudaSuccess;
+  if (blocks > 0) {
+    const unsigned n = static_cast<unsigned>(blocks);
+    st = p.warp_rows == 1   ? launch_rows<kDim, 1>(a, g, n, stream)
+         : p.warp_rows == 2 ? launch_rows<kDim, 2>(a, g, n, stream)
+                            : launch_rows<kDim, 4>(a, g, n, stream);
+  }
+  if (st != cudaSuccess) return st;
+  const int64_t cells = args.rows * args.heads, each = kThreads / 32;
+  return launch_pdl(attention_join_kernel<kDim>, static_cast<unsigned>((cells + each - 1) / each), kThreads, 0, stream,
+                    a);
+}
+
+}  // namespace
+
+size_t prefix_attention_bytes(const uocr_prefix_attention_args& a) {
+  const Plan p = plan_of(a);
+  return static_cast<size_t>(a.rows * a.heads) * (p.prefix_slots + p.own_slots) * (a.head_dim * 4 + sizeof(float2));
+}
+
+cudaError_t launch_prefix_attention(const uocr_prefix_attention_args& args, ErrorWord* err, cudaStream_t stream) {
+  const Plan p = plan_of(args);
+  Attention a{};
+  a.q = reinterpret_cast<const __nv_bfloat16*>(args.q);
+  a.prefix_k = reinterpret_cast<const __nv_bfloat16*>(args.prefix_k);
+  a.prefix_v = reinterpret_cast<const __nv_bfloat16*>(args.prefix_v);
+  a.prefix_lens = args.prefix_lens;
+  a.k = reinterpret_cast<const __nv_bfloat16*>(args.k);
+  a.v = reinterpret_cast<const __nv_bfloat16*>(args.v);
+  a.lens = args.lens, a.ancestry = args.ancestry, a.row_offsets = args.row_offsets;
+  a.out = reinterpret_cast<__nv_bfloat16*>(args.out);
+  a.lse = args.lse;
+  a.ldq = args.ldq, a.ldo = args.ldo, a.ld_ancestry = args.ld_ancestry;
+  a.prefix_stride = args.prefix_stride, a.prefix_head_stride = args.prefix_head_stride;
+  a.cache_stride = args.cache_stride, a.head_stride = args.head_stride;
+  a.rows = static_cast<int>(args.rows), a.sequences = static_cast<int>(args.sequences);
+  a.prefixes = static_cast<int>(args.prefixes), a.caches = static_cast<int>(args.caches);
+  a.heads = static_cast<int>(args.heads), a.kv_heads = static_cast<int>(args.kv_heads);
+  a.group = a.heads / a.kv_heads;
+  a.per = static_cast<int>(args.sequences / args.prefixes);
+  a.prefix_capacity = static_cast<int>(args.prefix_capacity), a.capacity = static_cast<int>(args.capacity);
+  a.prefix_slots = p.prefix_slots;
+  a.slots = p.prefix_slots + p.own_slots;
+  a.scale_log2 = args.scale * kLog2e;
+  a.part_o = static_cast<float*>(args.workspace);
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + args.rows * args.heads * a.slots * args.head_dim);
+  a.err = err;
+  return args.head_dim == 64 ? launch<64>(args, a, p, stream) : launch<128>(args, a, p, stream);
+}
+
+}  // namespace uocr_b200

@@ -1,5 +1,5 @@
-"""Python binding of the C ABI in include/uocr_moe.h, include/uocr_decoder.h and
-include/uocr_int8.h (ctypes over libuocr_moe.so).
+"""Python binding of the C ABI in include/uocr_moe.h, include/uocr_decoder.h,
+include/uocr_int8.h and include/uocr_beam.h (ctypes over libuocr_moe.so).
 
 This is the host-side mirror tests and bench.py call: torch supplies device
 memory and streams; every computation happens in libuocr_moe.so's sm_100a
@@ -29,6 +29,8 @@ PLAN_INT8_ACTIVATIONS = 16
 DECODER_CUDA_CORE_ATTENTION = 1
 DECODER_INT8_ACTIVATIONS = 2
 EP_HANDLE_BYTES = 256
+ROPE_PLAIN, ROPE_LINEAR, ROPE_NTK, ROPE_YARN = 0, 1, 2, 3
+BEAM_MAX = 32
 
 # Synthetic tensor kinds (one generator stream per tensor per layer).
 KIND_ROUTER, KIND_GATE, KIND_UP, KIND_DOWN, KIND_SGATE, KIND_SUP, KIND_SDOWN, KIND_X = 1, 2, 3, 4, 5, 6, 7, 8
@@ -44,6 +46,12 @@ DECODER_EXPORTS = [
 
 # Every symbol include/uocr_int8.h declares.
 INT8_EXPORTS = ["uocr_quantize_tokens", "uocr_linear_w8a8", "uocr_grouped_w8a8_workspace", "uocr_grouped_linear_w8a8"]
+
+# Every symbol include/uocr_beam.h declares.
+BEAM_EXPORTS = [
+    "uocr_rope_frequencies", "uocr_rotate_heads", "uocr_prefix_attention_workspace", "uocr_prefix_attention",
+    "uocr_beam_select_workspace", "uocr_beam_select", "uocr_reorder_states",
+]
 
 # Every symbol include/uocr_moe.h declares.
 EXPORTS = [
@@ -132,16 +140,51 @@ class GroupedW8A8Args(ctypes.Structure):
         ("workspace_bytes", ctypes.c_int64)]
 
 
+class RotateHeadsArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "v", "q_norm", "k_norm", "inv_freq", "positions",
+                                               "cache_rows", "slots", "q_out", "k_cache", "v_cache")] + [
+        (n, ctypes.c_int64) for n in ("rows", "q_heads", "kv_heads", "head_dim", "rotary_dim", "ldq", "ldk", "ldv",
+                                      "ldqo", "caches", "capacity", "cache_stride", "head_stride")] + [
+        ("eps", ctypes.c_float), ("magnitude", ctypes.c_float), ("dtype", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32)]
+
+
+class PrefixAttentionArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "prefix_k", "prefix_v", "prefix_lens", "k", "v", "lens",
+                                               "ancestry", "row_offsets", "out", "lse")] + [
+        (n, ctypes.c_int64) for n in ("rows", "sequences", "prefixes", "caches", "heads", "kv_heads", "head_dim",
+                                      "prefix_capacity", "capacity", "ldq", "ldo", "ld_ancestry", "prefix_stride",
+                                      "prefix_head_stride", "cache_stride", "head_stride")] + [
+        ("scale", ctypes.c_float), ("reserved", ctypes.c_int32), ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64)]
+
+
+class BeamSelectArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("logits", "scores", "finished", "tokens", "parents", "new_scores",
+                                               "new_finished")] + [
+        (n, ctypes.c_int64) for n in ("batch", "beams", "select", "vocab", "ld_logits")] + [
+        ("dtype", ctypes.c_int32), ("eos", ctypes.c_int32), ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64)]
+
+
+class ReorderStatesArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("state", "parents", "counts")] + [
+        (n, ctypes.c_int64) for n in ("layers", "groups", "beams", "segments", "units", "unit_bytes", "layer_stride",
+                                      "row_stride", "segment_stride")]
+
+
 def _packer(args) -> struct.Struct:
-    """The fields of a ctypes structure (pointers, int64, int32) as a struct format; null pointers are 0. A call packs
-    its arguments in a third of the time that the structure's constructor takes."""
-    code = {ctypes.c_void_p: "P", ctypes.c_int64: "q", ctypes.c_int32: "i"}
+    """The fields of a ctypes structure (pointers, int64, int32, float) as a struct format; null pointers are 0. A call
+    packs its arguments in a third of the time that the structure's constructor takes."""
+    code = {ctypes.c_void_p: "P", ctypes.c_int64: "q", ctypes.c_int32: "i", ctypes.c_float: "f"}
     packer = struct.Struct("@" + "".join(code[kind] for _, kind in args._fields_))
     assert packer.size == ctypes.sizeof(args)
     return packer
 
 
 _pack_linear, _pack_grouped = _packer(LinearW8A8Args).pack, _packer(GroupedW8A8Args).pack
+_pack_rotate, _pack_attention = _packer(RotateHeadsArgs).pack, _packer(PrefixAttentionArgs).pack
+_pack_select, _pack_reorder = _packer(BeamSelectArgs).pack, _packer(ReorderStatesArgs).pack
 
 
 def lib() -> ctypes.CDLL:
@@ -195,6 +238,13 @@ def lib() -> ctypes.CDLL:
         L.uocr_linear_w8a8.argtypes = [vp, vp]  # structures, by reference or packed
         L.uocr_grouped_w8a8_workspace.argtypes = [vp, ctypes.POINTER(i64)]
         L.uocr_grouped_linear_w8a8.argtypes = [vp, vp]
+        L.uocr_rope_frequencies.argtypes = [i64, ctypes.c_double, i32, ctypes.c_double, i64, vp, ctypes.POINTER(f32)]
+        L.uocr_rotate_heads.argtypes = [vp, vp]
+        L.uocr_prefix_attention_workspace.argtypes = [vp, ctypes.POINTER(i64)]
+        L.uocr_prefix_attention.argtypes = [vp, vp]
+        L.uocr_beam_select_workspace.argtypes = [vp, ctypes.POINTER(i64)]
+        L.uocr_beam_select.argtypes = [vp, vp]
+        L.uocr_reorder_states.argtypes = [vp, vp]
         _lib = L
     return _lib
 
@@ -611,6 +661,183 @@ def grouped_linear_w8a8(x, x_scales, w, w_scales, offsets, y, row_index=None, w_
             workspace = _workspace(need.value, y.device, stream)  # held until the launch is made
             space, space_bytes = workspace.data_ptr(), need.value
     _check(lib().uocr_grouped_linear_w8a8(_pack_grouped(*args, space, space_bytes), _stream(stream)))
+
+
+def _on_current_device(*tensors) -> None:
+    """The kernels run on the current device: every tensor has to be there."""
+    import torch
+    current = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != current:
+            raise ValueError(f"a tensor on {t.device} in a call on cuda:{current}")
+
+
+def _heads(t, what: str, rows: int, dim: int):
+    """(heads, row pitch) of [rows, heads, dim], the heads of a row one after another."""
+    if t.dim() != 3 or t.shape[0] != rows or t.shape[2] != dim:
+        raise ValueError(f"{what} must be [{rows}, heads, {dim}], not {tuple(t.shape)}")
+    heads = t.shape[1]
+    pitch, of_head, step = t.stride()
+    if (step != 1 and dim > 1) or (of_head != dim and heads > 1):
+        raise ValueError(f"{what}'s heads must be contiguous and follow one another")
+    return heads, (pitch if rows > 1 else heads * dim)
+
+
+def _cache_strides(t, like, what: str):
+    """The (cache, head) strides of a bf16 cache [caches, heads, capacity, dim] with contiguous keys, `like`'s too."""
+    import torch
+    if t.dim() != 4 or t.dtype is not torch.bfloat16 or like.dtype is not torch.bfloat16 or like.shape != t.shape:
+        raise ValueError(f"{what} must be two bfloat16 [caches, heads, capacity, dim] of the same shape")
+    caches, heads, capacity, dim = t.shape
+    of_cache, of_head, pitch, step = t.stride()
+    if like.stride() != t.stride() and t.numel() > 0:
+        raise ValueError(f"{what}: keys and values must have the same strides")
+    if (step != 1 and dim > 1) or (pitch != dim and capacity > 1):
+        raise ValueError(f"{what}: the keys of a head must be contiguous and follow one another")
+    return (of_cache if caches > 1 else 0), (of_head if heads > 1 else 0)
+
+
+def rope_frequencies(rotary_dim: int, theta: float = 1e4, scaling: int = ROPE_PLAIN, factor: float = 1.0,
+                     original: int = 0):
+    """(inv_freq, magnitude): the fp32 table of rotary_dim / 2 frequencies (a CPU tensor) and what cos and sin are
+    multiplied by (uocr_rope_frequencies); scaling is a ROPE_* value, original the positions that YaRN stretches."""
+    import torch
+    table, magnitude = torch.empty(max(rotary_dim, 0) // 2), ctypes.c_float()
+    _check(lib().uocr_rope_frequencies(rotary_dim, theta, scaling, factor, original, table.data_ptr(),
+                                       ctypes.byref(magnitude)))
+    return table, magnitude.value
+
+
+def rotate_heads(q, k, v, inv_freq, positions, q_out, k_cache, v_cache, q_norm=None, k_norm=None, cache_rows=None,
+                 slots=None, eps: float = 1e-6, magnitude: float = 1.0, interleaved: bool = False, stream=None):
+    """q [rows, heads, dim] normalised (with q_norm) and rotated into q_out (bf16); k and v [rows, kv_heads, dim]
+    likewise (v as it is) into the bf16 caches [caches, kv_heads, capacity, dim] at cache_rows[r] (else r), slots[r]
+    (else positions[r]) (uocr_rotate_heads). q, k, v: fp32 or bf16; inv_freq: fp32, rotary_dim / 2 of them; positions,
+    cache_rows, slots: int32."""
+    import torch
+    f32, i32 = torch.float32, torch.int32
+    rows, _, dim = q.shape
+    _on_current_device(q, k, v, inv_freq, positions, q_out, k_cache, v_cache, q_norm, k_norm, cache_rows, slots)
+    heads, ldq = _heads(q, "q", rows, dim)
+    kv_heads, ldk = _heads(k, "k", rows, dim)
+    v_heads, ldv = _heads(v, "v", rows, dim)
+    out_heads, ldqo = _heads(q_out, "q_out", rows, dim)
+    if out_heads != heads or q_out.dtype is not torch.bfloat16:
+        raise ValueError("q_out must be bfloat16 of q's shape")
+    if v_heads != kv_heads or k.dtype is not q.dtype or v.dtype is not q.dtype:
+        raise ValueError("k and v must have the same shape and q's dtype")
+    cache_stride, head_stride = _cache_strides(k_cache, v_cache, "the caches")
+    if k_cache.shape[1] != kv_heads or k_cache.shape[3] != dim:
+        raise ValueError(f"the caches must be [caches, {kv_heads}, capacity, {dim}]")
+    if cache_rows is None and k_cache.shape[0] != rows:
+        raise ValueError("without cache_rows there is one cache per row")
+    args = _pack_rotate(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), 0 if q_norm is None else _vector(q_norm, "q_norm", dim, f32),
+        0 if k_norm is None else _vector(k_norm, "k_norm", dim, f32),
+        _vector(inv_freq, "inv_freq", inv_freq.numel(), f32), _vector(positions, "positions", rows, i32),
+        0 if cache_rows is None else _vector(cache_rows, "cache_rows", rows, i32),
+        0 if slots is None else _vector(slots, "slots", rows, i32), q_out.data_ptr(), k_cache.data_ptr(),
+        v_cache.data_ptr(), rows, heads, kv_heads, dim, 2 * inv_freq.numel(), ldq, ldk, ldv, ldqo, k_cache.shape[0],
+        k_cache.shape[2], cache_stride, head_stride, eps, magnitude, _float_dtype(q, "q"), int(interleaved))
+    _check(lib().uocr_rotate_heads(args, _stream(stream)))
+
+
+def prefix_attention(q, prefix_k, prefix_v, prefix_lens, k, v, lens, out, ancestry=None, row_offsets=None,
+                     scale=None, lse=None, stream=None):
+    """out = attention of q [rows, heads, dim] over the shared prefixes [prefixes, kv_heads, prefix_capacity, dim]
+    (prefix_lens keys each; sequence b stands behind prefix b // (sequences / prefixes)) and each sequence's own keys
+    [caches, kv_heads, capacity, dim] (lens of them, key t of sequence b in cache ancestry[b, t], else b)
+    (uocr_prefix_attention). q, out and the caches are bf16, lens, ancestry and row_offsets (sequences + 1 values; None:
+    one row each) int32, lse (optional) fp32 [rows, heads]; scale defaults to dim ** -0.5. The workspace comes from
+    torch's allocator, from the blocks of the stream that the call runs on."""
+    import torch
+    f32, i32, bf16 = torch.float32, torch.int32, torch.bfloat16
+    rows, _, dim = q.shape
+    _on_current_device(q, prefix_k, prefix_v, prefix_lens, k, v, lens, out, ancestry, row_offsets, lse)
+    heads, ldq = _heads(q, "q", rows, dim)
+    out_heads, ldo = _heads(out, "out", rows, dim)
+    if out_heads != heads or q.dtype is not bf16 or out.dtype is not bf16:
+        raise ValueError("q and out must be bfloat16 of the same shape")
+    prefix_stride, prefix_head_stride = _cache_strides(prefix_k, prefix_v, "the prefixes")
+    cache_stride, head_stride = _cache_strides(k, v, "the own caches")
+    prefixes, kv_heads, prefix_capacity, _ = prefix_k.shape
+    caches, _, capacity, _ = k.shape
+    if k.shape[1] != kv_heads or k.shape[3] != dim or prefix_k.shape[3] != dim:
+        raise ValueError(f"the caches must be [caches, {kv_heads}, capacity, {dim}]")
+    sequences, ld_ancestry, table, offsets = lens.numel(), 0, 0, 0
+    if ancestry is not None:
+        if ancestry.dtype is not i32:
+            raise ValueError("ancestry must be int32")
+        ld_ancestry, table = _pitch(ancestry, "ancestry", sequences, capacity), ancestry.data_ptr()
+    if row_offsets is not None:
+        offsets = _vector(row_offsets, "row_offsets", sequences + 1, i32)
+    args = (q.data_ptr(), prefix_k.data_ptr(), prefix_v.data_ptr(), _vector(prefix_lens, "prefix_lens", prefixes, i32),
+            k.data_ptr(), v.data_ptr(), _vector(lens, "lens", sequences, i32), table, offsets, out.data_ptr(),
+            0 if lse is None else _vector(lse, "lse", rows * heads, f32), rows, sequences, prefixes, caches, heads,
+            kv_heads, dim, prefix_capacity, capacity, ldq, ldo, ld_ancestry, prefix_stride, prefix_head_stride,
+            cache_stride, head_stride, dim ** -0.5 if scale is None else scale, 0)
+    need = ctypes.c_int64()
+    _check(lib().uocr_prefix_attention_workspace(_pack_attention(*args, 0, 0), ctypes.byref(need)))
+    if need.value > 0:
+        workspace = _workspace(need.value, q.device, stream)  # held until the launch is made
+        args += (workspace.data_ptr(), need.value)
+    else:
+        args += (0, 0)
+    _check(lib().uocr_prefix_attention(_pack_attention(*args), _stream(stream)))
+
+
+def beam_select(logits, scores, tokens, parents, new_scores, finished=None, new_finished=None, eos: int = -1,
+                stream=None):
+    """The best continuations of every group of beams: logits [batch * beams, vocab] (fp32 or bf16), scores (and
+    finished) [batch, beams]; tokens, parents, new_scores (and new_finished) [batch, select] receive them, best first
+    (uocr_beam_select). Flags, tokens and parents are int32, scores fp32. The workspace comes from torch's allocator, from
+    the blocks of the stream that the call runs on."""
+    import torch
+    f32, i32 = torch.float32, torch.int32
+    _on_current_device(logits, scores, tokens, parents, new_scores, finished, new_finished)
+    batch, beams = scores.shape
+    select, vocab = tokens.shape[1], logits.shape[1]
+    ld = _pitch(logits, "logits", batch * beams, vocab)
+    args = (logits.data_ptr(), _vector(scores, "scores", batch * beams, f32),
+            0 if finished is None else _vector(finished, "finished", batch * beams, i32),
+            _vector(tokens, "tokens", batch * select, i32), _vector(parents, "parents", batch * select, i32),
+            _vector(new_scores, "new_scores", batch * select, f32),
+            0 if new_finished is None else _vector(new_finished, "new_finished", batch * select, i32), batch, beams,
+            select, vocab, ld, _float_dtype(logits, "logits"), eos)
+    need = ctypes.c_int64()
+    _check(lib().uocr_beam_select_workspace(_pack_select(*args, 0, 0), ctypes.byref(need)))
+    workspace = _workspace(max(need.value, 16), logits.device, stream)  # held until the launch is made
+    _check(lib().uocr_beam_select(_pack_select(*args, workspace.data_ptr(), need.value), _stream(stream)))
+
+
+def reorder_states(state, parents, beams: int, counts=None, stream=None):
+    """state[:, g * beams + b] = state[:, g * beams + parents[g, b]] in place (uocr_reorder_states). state is [layers,
+    rows, segments, units, ...] with contiguous segments, or [rows, units]; parents: rows int32 values, local to each
+    group of `beams` rows; counts (int32): units in use of each row, the rest of a row stays."""
+    import torch
+    i32 = torch.int32
+    _on_current_device(state, parents, counts)
+    if state.dim() == 2:
+        state = state[None, :, None]
+    if state.dim() < 4:
+        raise ValueError("state must be [layers, rows, segments, units, ...] or [rows, units]")
+    layers, rows, segments, units = state.shape[:4]
+    width = 1
+    for n in state.shape[4:]:
+        width *= n
+    flat, expect = state.stride()[3:], 1
+    for n, step in zip(reversed(state.shape[3:]), reversed(flat)):
+        if step != expect and n > 1:
+            raise ValueError("a segment of the state must be contiguous")
+        expect *= n
+    if beams < 1 or rows % beams != 0:
+        raise ValueError("the state's rows must be whole groups of beams")
+    eb = state.element_size()
+    of_layer, of_row, of_segment = (s * eb for s in state.stride()[:3])
+    _check(lib().uocr_reorder_states(_pack_reorder(
+        state.data_ptr(), _vector(parents, "parents", rows, i32),
+        0 if counts is None else _vector(counts, "counts", rows, i32), layers, rows // beams, beams, segments, units,
+        width * eb, of_layer, of_row, of_segment), _stream(stream)))
 
 
 class Decoder:

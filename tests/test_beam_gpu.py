@@ -1,0 +1,345 @@
+"""The rotation of heads, the selection of beams and the reordering of states on
+the GPU against plain 64-bit forms.
+
+Tolerances. Rotation: the sum of n <= 256 squares is off by at most n * 2^-24 of
+itself, its root by half of that; rsqrt, the mean, the products with gain,
+cosine and sine and the magnitude add 8 roundings of 2^-24 and the 2 ulp of
+rsqrt and of sine and cosine; the angle, reduced to a turn in 64 bits, is off by
+2^-25 turns, 2^-22.3 of a full amplitude. 2^-15 of the pair's amplitude covers
+them; then half a step of bf16, 2^-8 of the value. Selection: a thread sums 32
+exponentials of 2^-22 + |x| 2^-23 relative error (weighted by exp(x), at most
+2^-21 of the sum), 37 + 8 additions to the block's sum: the log of the sum is off
+by 50 * 2^-24, the score besides by 2^-24 of itself. Reordering moves bits.
+"""
+import math
+
+import pytest
+
+import uocr_moe as M
+
+pytestmark = pytest.mark.gpu
+
+
+def gen_of(*key):
+    import torch
+    return torch.Generator(device="cuda").manual_seed(sum((i + 1) * int(k) for i, k in enumerate(key)) + 1)
+
+
+# ---- rotate_heads
+
+def rotated(x, gain, inv_freq, positions, interleaved, eps, magnitude):
+    """(values, amplitudes) in 64 bits."""
+    import torch
+    x = x.double()
+    if gain is not None:
+        x = x / (x.square().mean(-1, keepdim=True) + eps).sqrt() * gain.double()
+    rot = 2 * inv_freq.numel()
+    angle = (positions.double()[:, None] * inv_freq.double())[:, None, :]
+    c, s = magnitude * angle.cos(), magnitude * angle.sin()
+    y, size = x.clone(), x.abs()
+    at = (slice(0, rot, 2), slice(1, rot, 2)) if interleaved else (slice(0, rot // 2), slice(rot // 2, rot))
+    a, b = x[..., at[0]], x[..., at[1]]
+    y[..., at[0]], y[..., at[1]] = a * c - b * s, b * c + a * s
+    size[..., at[0]] = size[..., at[1]] = abs(magnitude) * (a.abs() + b.abs())
+    return y, size
+
+
+def close(got, want, size):
+    over = (got.double() - want).abs() - (2.0 ** -8 * want.abs() + 2.0 ** -15 * size + 1e-38)
+    assert not over.isnan().any() and (over.numel() == 0 or over.max().item() <= 0.0), over.max().item()
+
+
+def run_rotate(rows, heads, kv, dim, rot, dtype="float32", norm="both", interleaved=False, far=0, caches=None,
+               pad=0, magnitude=1.0, shift=0, own_places=True):
+    import torch
+    g = gen_of(rows, heads, kv, dim, rot)
+    dt = getattr(torch, dtype)
+
+    def make(h):  # rows of a wider buffer, `shift` elements from its start
+        wide = torch.randn(rows, shift + h * dim + pad, generator=g, device="cuda").to(dt)
+        return torch.as_strided(wide, (rows, h, dim), (wide.shape[1], dim, 1), shift)
+
+    q, k, v = make(heads), make(kv), make(kv)
+    caches = rows if caches is None else caches
+    cap = -(-rows // caches) + 3
+    order = torch.randperm(caches * cap, generator=g, device="cuda")[:rows]
+    places, slots = (order // cap).to(torch.int32), (order % cap).to(torch.int32)
+    positions = slots + far if own_places else slots
+    inv = (1.0 / 1e4 ** (torch.arange(rot // 2, device="cuda").double() * 2 / max(rot, 1))).float()
+    gains = {n: torch.rand(dim, generator=g, device="cuda") + 0.5 if norm in (n, "both") else None for n in "qk"}
+    kc = torch.full((caches, kv, cap, dim), 7.0, dtype=torch.bfloat16, device="cuda")
+    vc = torch.full_like(kc, 8.0)
+    out = torch.full((rows, heads * dim + pad), 9.0, dtype=torch.bfloat16, device="cuda")
+    view = torch.as_strided(out, (rows, heads, dim), (out.shape[1], dim, 1))
+    M.rotate_heads(q, k, v, inv, positions, view, kc, vc, q_norm=gains["q"], k_norm=gains["k"], cache_rows=places,
+                   slots=slots if own_places else None, eps=1e-5, magnitude=magnitude, interleaved=interleaved)
+    args = (inv, positions, interleaved, 1e-5, magnitude)
+    close(view, *rotated(q, gains["q"], *args))
+    assert (out[:, heads * dim:] == 9.0).all()
+    at = (places.long(), slice(None), slots.long())
+    close(kc[at], *rotated(k, gains["k"], *args))
+    assert torch.equal(vc[at], v.to(torch.bfloat16))
+    written = torch.zeros(caches, cap, dtype=torch.bool, device="cuda")
+    written[places.long(), slots.long()] = True
+    assert (kc.transpose(1, 2)[~written] == 7.0).all() and (vc.transpose(1, 2)[~written] == 8.0).all()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("heads,kv,dim,rot", [(16, 4, 128, 128), (10, 10, 128, 64), (3, 1, 64, 64), (5, 5, 80, 32),
+                                              (7, 7, 96, 96), (2, 2, 256, 256), (9, 3, 8, 8), (33, 11, 192, 72),
+                                              (4, 2, 128, 0)])
+def test_rotate_heads(cuda, dtype, interleaved, heads, kv, dim, rot):
+    run_rotate(5, heads, kv, dim, rot, dtype, interleaved=interleaved)
+
+
+@pytest.mark.parametrize("kw", [dict(rows=1), dict(rows=1000, caches=3), dict(norm="q"), dict(norm="k"), dict(norm=""),
+                                dict(far=3000000), dict(far=-50000), dict(pad=5), dict(pad=8, dtype="bfloat16"),
+                                dict(pad=3, shift=1, dtype="bfloat16"), dict(shift=3, pad=1), dict(magnitude=1.4),
+                                dict(own_places=False, caches=1)])
+def test_rotate_heads_forms(cuda, kw):
+    run_rotate(**{**dict(rows=9, heads=8, kv=2, dim=128, rot=64), **kw})
+
+
+def test_rotate_heads_in_place_and_without_keys(cuda):
+    import torch
+    g = gen_of(3)
+    q = torch.randn(6, 4, 64, generator=g, device="cuda").to(torch.bfloat16)
+    inv, _ = M.rope_frequencies(64)
+    pos = torch.arange(6, dtype=torch.int32, device="cuda")
+    none = torch.empty(6, 0, 64, dtype=torch.bfloat16, device="cuda")
+    cache = torch.empty(6, 0, 8, 64, dtype=torch.bfloat16, device="cuda")
+    want = rotated(q, None, inv.cuda(), pos, False, 0.0, 1.0)
+    M.rotate_heads(q, none, none, inv.cuda(), pos, q, cache, cache)
+    close(q, *want)
+
+
+@pytest.mark.parametrize("place,slot", [(4, 0), (-1, 0), (0, 8), (0, -1)])
+def test_rotate_heads_reports_places_that_do_not_exist(cuda, place, slot):
+    import torch
+    x = torch.ones(2, 1, 64, device="cuda")
+    cache = torch.zeros(4, 1, 8, 64, dtype=torch.bfloat16, device="cuda")
+    vcache, out = torch.zeros_like(cache), torch.empty(2, 1, 64, dtype=torch.bfloat16, device="cuda")
+    i32 = dict(dtype=torch.int32, device="cuda")
+    M.rotate_heads(x, x, x, torch.ones(32, device="cuda"), torch.zeros(2, **i32), out, cache, vcache,
+                   cache_rows=torch.tensor([1, place], **i32), slots=torch.tensor([2, slot], **i32))
+    with pytest.raises(M.UocrError) as e:
+        M.ops_check()
+    assert e.value.code == 5 and "row 1" in str(e.value)
+    assert (out == 1).all() and (vcache[1, 0, 2] == 1).all() and vcache.sum() == 64
+    M.ops_check()
+
+
+# ---- beam_select
+
+def selected(logits, scores, finished, eos, select):
+    """[batch, select] of (value, flat index), best first, in 64 bits; and [batch, beams, vocab] values."""
+    import torch
+    batch, beams = scores.shape
+    z = logits.double().view(batch, beams, -1)
+    z = torch.where(z.isnan(), -math.inf, z)
+    z = torch.log_softmax(z, -1) + scores.double()[..., None]
+    z = torch.where(z.isnan(), -math.inf, z)
+    if finished is not None:
+        done = finished != 0
+        z[done] = -math.inf
+        z[..., max(eos, 0)] = torch.where(done, scores.double(), z[..., max(eos, 0)])
+    value, at = z.reshape(batch, -1).sort(dim=1, descending=True, stable=True)
+    pad = max(0, select - at.shape[1])
+    value = torch.nn.functional.pad(value, (0, pad), value=-math.inf)
+    at = torch.nn.functional.pad(at, (0, pad))
+    return value[:, :select], at[:, :select], z
+
+
+def check_select(logits, scores, select, finished=None, eos=-1):
+    import torch
+    batch, beams = scores.shape
+    vocab = logits.shape[1]
+    tokens = torch.full((batch, select), -7, dtype=torch.int32, device="cuda")
+    parents, flags = torch.full_like(tokens, -7), torch.full_like(tokens, -7)
+    new = torch.full((batch, select), math.nan, device="cuda")
+    M.beam_select(logits, scores, tokens, parents, new, finished=finished, new_finished=flags, eos=eos)
+    value, at, z = selected(logits, scores, finished, eos, select)
+    dead = value == -math.inf
+    assert torch.equal(new == -math.inf, dead)
+    tol = torch.where(dead, 0.0, 50 * 2.0 ** -24 + 2.0 ** -23 * value.abs())
+    assert ((new.double() - value).abs() <= tol)[~dead].all()
+    tok, par = at % vocab, at // vocab
+    tok[dead], par[dead] = max(eos, 0), 0
+    # The same candidates in the same order, but where two beams' scores are closer than the scores' own error.
+    same = (tokens == tok) & (parents == par)
+    if not same.all():
+        own = z[torch.arange(batch, device="cuda")[:, None], parents.long(), tokens.long()]
+        assert ((own - value).abs() <= 2 * tol)[~same].all() and not (~same & dead).any()
+    done = dead | (tokens == eos)
+    if finished is not None:
+        done |= finished.gather(1, parents.long()) != 0
+    assert torch.equal(flags != 0, done)
+    flat = parents.long() * vocab + tokens
+    for b in range(batch):
+        live = flat[b][~dead[b]]
+        assert live.unique().numel() == live.numel()
+    return tokens, parents, new
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("batch,beams,select,vocab", [
+    (1, 1, 1, 1), (1, 1, 32, 40), (1, 4, 4, 102400), (3, 2, 5, 129), (2, 8, 16, 4096), (1, 32, 32, 5001), (5, 3, 7, 8192),
+    (2, 5, 31, 33333), (40, 8, 8, 20001), (1, 2, 3, 1 << 20)])
+def test_beam_select(cuda, dtype, batch, beams, select, vocab):
+    import torch
+    g = gen_of(batch, beams, select, vocab)
+    logits = (torch.randn(batch * beams, vocab, generator=g, device="cuda") * 3).to(getattr(torch, dtype))
+    check_select(logits, -10 * torch.rand(batch, beams, generator=g, device="cuda"), select)
+
+
+def test_beam_select_ties_go_to_the_lower_beam_and_token(cuda):
+    import torch
+    tokens, parents, _ = check_select(torch.zeros(6, 10000, device="cuda"), torch.zeros(2, 3, device="cuda"), 32)
+    assert torch.equal(tokens, torch.arange(32, dtype=torch.int32, device="cuda").expand(2, 32)) and (parents == 0).all()
+    logits = torch.zeros(3, 9000, device="cuda")
+    logits[:, 8000:8003] = 5.0
+    tokens, parents, _ = check_select(logits, torch.zeros(1, 3, device="cuda"), 7)
+    assert tokens[0].tolist() == [8000, 8001, 8002] * 2 + [8000] and parents[0].tolist() == [0] * 3 + [1] * 3 + [2]
+
+
+@pytest.mark.parametrize("order", ["rising", "falling", "steps"])
+@pytest.mark.parametrize("select", [1, 32])
+def test_beam_select_of_sorted_logits(cuda, order, select):
+    """Large values side by side: whole threads' and warps' worth of them above the others."""
+    import torch
+    x = torch.linspace(-20, 20, 70000, device="cuda")
+    x = x.flip(0) if order == "falling" else torch.floor(x) if order == "steps" else x
+    check_select(torch.stack([x, x.roll(777)]).contiguous(), torch.tensor([[-1.0, -1.5]], device="cuda"), select)
+
+
+def test_beam_select_finished_dead_and_bad_rows(cuda):
+    import torch
+    g = gen_of(8)
+    logits = torch.randn(12, 5000, generator=g, device="cuda")
+    scores = -torch.rand(2, 6, generator=g, device="cuda") * 4
+    finished = torch.zeros(2, 6, dtype=torch.int32, device="cuda")
+    finished[0, 1], finished[1, 0], finished[1, 5] = 1, -3, 1
+    scores[0, 2], scores[1, 3] = -math.inf, math.nan
+    scores[1, 5] = -math.inf
+    logits[0, 100:4000] = math.nan
+    logits[3] = -math.inf
+    logits[4, 77] = math.inf
+    logits[6] = math.nan  # of a finished beam
+    logits[11, :] = -math.inf
+    for eos in (-1, 0, 4999):
+        check_select(logits, scores, 8, finished, eos)
+        check_select(logits, scores, 32, finished, eos)
+
+
+def test_beam_select_when_candidates_run_out(cuda):
+    import torch
+    scores = torch.tensor([[-1.0, -math.inf, -2.0], [-math.inf] * 3], device="cuda")
+    finished = torch.tensor([[1, 0, 0], [0, 1, 0]], dtype=torch.int32, device="cuda")
+    logits = torch.full((6, 50), -math.inf, device="cuda")
+    logits[2, 7] = 0.5
+    tokens, parents, new = check_select(logits, scores, 5, finished, 3)
+    assert tokens[0].tolist() == [3, 7, 3, 3, 3] and parents[0].tolist() == [0, 2, 0, 0, 0]
+    assert new[0, :2].tolist() == [-1.0, -2.0] and (new[1] == -math.inf).all()
+
+
+@pytest.mark.parametrize("dtype,pad,shift", [("float32", 3, 0), ("bfloat16", 5, 0), ("float32", 4, 1),
+                                             ("bfloat16", 8, 1)])
+def test_beam_select_of_rows_at_any_address(cuda, dtype, pad, shift):
+    import torch
+    wide = torch.randn(6, shift + 7001 + pad, generator=gen_of(pad, shift), device="cuda").to(getattr(torch, dtype))
+    check_select(wide[:, shift:shift + 7001], torch.zeros(2, 3, device="cuda"), 6)
+
+
+def test_beam_select_on_a_stream_and_from_a_graph(cuda):
+    import torch
+    g = gen_of(77)
+    logits = torch.randn(8, 60000, generator=g, device="cuda")
+    scores = -torch.rand(2, 4, generator=g, device="cuda")
+    tokens = torch.empty(2, 4, dtype=torch.int32, device="cuda")
+    parents, new = torch.empty_like(tokens), torch.empty(2, 4, device="cuda")
+    want = check_select(logits, scores, 4)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    M.beam_select(logits, scores, tokens, parents, new, stream=side)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip((tokens, parents, new), want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        M.beam_select(logits, scores, tokens, parents, new)
+    logits.copy_(torch.randn(8, 60000, generator=g, device="cuda"))
+    want = check_select(logits, scores, 4)
+    for _ in range(3):
+        new.fill_(5.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip((tokens, parents, new), want))
+
+
+# ---- reorder_states
+
+def reordered(state, parents, beams, counts):
+    """state [layers, rows, segments, units, width]."""
+    import torch
+    want, units = state.clone(), state.shape[3]
+    for r in range(state.shape[1]):
+        p = r // beams * beams + int(parents[r])
+        n = units if counts is None else int(counts[p])
+        want[:, r, :, :n] = state[:, p, :, :n]
+    return want
+
+
+@pytest.mark.parametrize("counted", [False, True])
+@pytest.mark.parametrize("layers,groups,beams,segments,units,width,dtype", [
+    (1, 1, 1, 1, 5, 1, "int32"), (1, 1, 4, 1, 1000, 1, "int32"), (2, 3, 5, 2, 33, 128, "bfloat16"),
+    (3, 2, 8, 4, 17, 64, "bfloat16"), (2, 2, 16, 1, 100, 3, "bfloat16"), (1, 3, 32, 2, 65, 16, "float32"),
+    (2, 1, 31, 1, 77, 7, "uint8"), (1, 2, 9, 3, 13, 20, "uint8"), (4, 1, 17, 1, 1, 1, "uint8")])
+def test_reorder_states(cuda, layers, groups, beams, segments, units, width, dtype, counted):
+    import torch
+    g = gen_of(layers, groups, beams, segments, units, width)
+    rows = groups * beams
+    state = torch.randint(0, 100, (layers, rows, segments, units, width), generator=g, device="cuda").to(
+        getattr(torch, dtype))
+    parents = torch.randint(0, beams, (rows,), generator=g, device="cuda", dtype=torch.int32)
+    parents[:beams] = torch.arange(beams, device="cuda").roll(1)  # one group is a single cycle
+    counts = torch.randint(0, units + 1, (rows,), generator=g, device="cuda",
+                           dtype=torch.int32) if counted else None
+    want = reordered(state, parents, beams, counts)
+    M.reorder_states(state, parents, beams, counts=counts)
+    M.ops_check()
+    assert torch.equal(state, want)
+
+
+def test_reorder_states_of_strided_states(cuda):
+    import torch
+    g = gen_of(5)
+    whole = torch.randint(0, 1000, (3, 8, 2, 40, 8), generator=g, device="cuda", dtype=torch.int32)
+    parents = torch.tensor([3, 0, 0, 1], dtype=torch.int32, device="cuda")
+    want = whole.clone()
+    want[:, 1:5, :, 5:25] = reordered(whole[:, 1:5, :, 5:25], parents, 4, None)
+    M.reorder_states(whole[:, 1:5, :, 5:25], parents, 4)
+    assert torch.equal(whole, want)
+    table = torch.randint(0, 1000, (8, 51), generator=g, device="cuda", dtype=torch.int32)
+    parents = torch.tensor([1, 1, 0, 3, 2, 2, 3, 0], dtype=torch.int32, device="cuda")
+    counts = torch.full((8,), 30, dtype=torch.int32, device="cuda")
+    want = reordered(table[None, :, None, :, None], parents, 4, counts)[0, :, 0, :, 0]
+    M.reorder_states(table, parents, 4, counts=counts)
+    assert torch.equal(table, want)
+
+
+def test_reorder_states_reports_bad_parents_and_counts(cuda):
+    import torch
+    i32 = dict(dtype=torch.int32, device="cuda")
+    state = torch.arange(6, **i32)[:, None].expand(6, 10).contiguous()
+    M.reorder_states(state, torch.tensor([1, 3, -1, 2, 0, 1], **i32), 3)
+    with pytest.raises(M.UocrError) as e:
+        M.ops_check()
+    assert e.value.code == 5 and "parent" in str(e.value)
+    assert state[:, 0].tolist() == [1, 1, 2, 5, 3, 4]
+    state = torch.arange(4, **i32)[:, None].expand(4, 10).contiguous()
+    M.reorder_states(state, torch.tensor([1, 0, 3, 2], **i32), 4, counts=torch.tensor([11, -1, 4, 4], **i32))
+    with pytest.raises(M.UocrError) as e:
+        M.ops_check()
+    assert e.value.code == 5 and "units" in str(e.value)
+    assert state[0].tolist() == [0] * 10 and state[1].tolist() == [0] * 10
+    assert state[2].tolist() == [3] * 4 + [2] * 6

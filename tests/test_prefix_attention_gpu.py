@@ -1,0 +1,298 @@
+"""Attention behind shared prefixes on the GPU against a plain 64-bit form.
+
+Tolerance. With exact bf16 inputs a score's products are exact and its sum of
+`dim` terms is off by at most dim * 2^-23 of the terms' magnitudes (the tensor
+cores may cut instead of round): d = scale * sum |q k| * dim * 2^-23, plus 2^-22
+|s| for the change to base 2; a weight is then off by the factor exp(2 d) and
+2^-21 of the exponential, and by half a step of bf16, 2^-8, as the operand of
+the second product, whose sum over n keys (and the sum of the weights, and the
+joins' factors) is off by (n + 64) * 2^-23 of the magnitudes. So with A = sum p |v|
+the output is off by A * (2^-8 + 2 d + (n + 64) * 2^-22), and by its own rounding,
+2^-8 of itself; lse by d + (n + 64) * 2^-22 + 2^-22 |lse|.
+"""
+import math
+
+import pytest
+
+import uocr_moe as M
+
+pytestmark = pytest.mark.gpu
+
+
+def gen_of(*key):
+    import torch
+    return torch.Generator(device="cuda").manual_seed(sum((i + 1) * int(k) for i, k in enumerate(key)) + 1)
+
+
+def plain(c):
+    """(out, lse, tolerance of out, of lse) in 64 bits; rows of no sequence are NaN."""
+    import torch
+    q, k, v = c["q"].double(), c["k"], c["v"]
+    rows, heads, dim = q.shape
+    kv = k.shape[1]
+    n_seq, prefixes = c["lens"].numel(), c["prefix_lens"].numel()
+    offsets = list(range(n_seq + 1)) if c["row_offsets"] is None else c["row_offsets"].tolist()
+    out, lse, tol, tol_lse = (torch.full(s, math.nan, dtype=torch.float64, device="cuda")
+                              for s in ((rows, heads, dim), (rows, heads), (rows, heads, dim), (rows, heads)))
+    scale = c["scale"]
+    for b in range(n_seq):
+        p, r0, r1, n = b // (n_seq // prefixes), offsets[b], offsets[b + 1], int(c["lens"][b])
+        plen = int(c["prefix_lens"][p])
+        of = torch.full((n,), b, device="cuda") if c["ancestry"] is None else c["ancestry"][b, :n].long()
+        at = torch.arange(n, device="cuda")
+        limit = n - (r1 - r0) + 1 + torch.arange(r1 - r0, device="cuda")
+        seen = torch.cat([torch.ones(r1 - r0, plen, dtype=torch.bool, device="cuda"), at < limit[:, None]], 1)
+        for h in range(heads):
+            g = h // (heads // kv)
+            kk = torch.cat([c["prefix_k"][p, g, :plen], k[of, g, at]]).double()
+            vv = torch.cat([c["prefix_v"][p, g, :plen], v[of, g, at]]).double()
+            qq = q[r0:r1, h]
+            s = torch.where(seen, scale * qq @ kk.T, -math.inf)
+            size = torch.where(seen, abs(scale) * qq.abs() @ kk.abs().T, 0.0)
+            d = (size.amax(1) if s.shape[1] else torch.zeros(r1 - r0, device="cuda")).double() * (dim * 2.0 ** -23 + 2.0 ** -22)
+            top = s.amax(1, keepdim=True) if s.shape[1] else torch.full((r1 - r0, 1), -math.inf, device="cuda").double()
+            w = torch.where(seen, torch.exp(s - torch.where(top.isinf(), 0.0, top)), 0.0)
+            total = w.sum(1, keepdim=True)
+            w = torch.where(total > 0, w / total, 0.0)
+            keys = (seen.sum(1) + 64) * 2.0 ** -22
+            out[r0:r1, h] = w @ vv
+            lse[r0:r1, h] = (torch.log(total) + top)[:, 0]
+            tol[r0:r1, h] = (w @ vv.abs()) * (2.0 ** -8 + 2 * d + keys)[:, None] + 2.0 ** -8 * out[r0:r1, h].abs()
+            tol_lse[r0:r1, h] = d + keys + 2.0 ** -22 * lse[r0:r1, h].abs()
+    return out, lse, tol, tol_lse
+
+
+def make(prefix_lens, lens, heads, kv, dim, rows=None, beams=False, prefix_capacity=None, capacity=None, first_row=0,
+         rows_behind=0, spread=1.0, seed=0):
+    """rows: query rows of each sequence (None: one each, without offsets)."""
+    import torch
+    g = gen_of(len(prefix_lens), sum(prefix_lens), sum(lens), heads, kv, dim, seed)
+    bf16, i32 = torch.bfloat16, torch.int32
+    pcap = max(prefix_lens) + 3 if prefix_capacity is None else prefix_capacity
+    cap = max(lens) + 5 if capacity is None else capacity
+    n = len(lens)
+
+    def values(*shape):
+        return (torch.randn(*shape, generator=g, device="cuda") * spread).to(bf16)
+
+    c = dict(prefix_k=values(len(prefix_lens), kv, pcap, dim), prefix_v=values(len(prefix_lens), kv, pcap, dim),
+             k=values(n, kv, cap, dim), v=values(n, kv, cap, dim), ancestry=None, row_offsets=None, scale=dim ** -0.5)
+    # What lies behind the lengths is no number.
+    for p, length in enumerate(prefix_lens):
+        c["prefix_k"][p, :, length:] = math.nan
+        c["prefix_v"][p, :, length:] = math.inf
+    if beams:
+        per = n // len(prefix_lens)
+        base = torch.arange(n, device="cuda")[:, None] // per * per
+        c["ancestry"] = (torch.randint(0, per, (n, cap), generator=g, device="cuda") + base).to(i32)
+        for b in range(n):
+            c["ancestry"][b, lens[b]:] = 1 << 30
+    else:
+        for b, length in enumerate(lens):
+            c["k"][b, :, length:] = math.nan
+            c["v"][b, :, length:] = math.nan
+    c["prefix_lens"] = torch.tensor(prefix_lens, dtype=i32, device="cuda")
+    c["lens"] = torch.tensor(lens, dtype=i32, device="cuda")
+    total = n if rows is None else first_row + sum(rows) + rows_behind
+    if rows is not None:
+        c["row_offsets"] = torch.tensor([first_row + sum(rows[:i]) for i in range(n + 1)], dtype=i32, device="cuda")
+    c["q"] = values(total, heads, dim)
+    c["out"] = torch.full((total, heads, dim), 33.0, dtype=bf16, device="cuda")
+    c["lse"] = torch.full((total, heads), 44.0, device="cuda")
+    return c
+
+
+def check(c, call=True):
+    import torch
+    if call:
+        M.prefix_attention(**c)
+        M.ops_check()
+    out, lse, tol, tol_lse = plain(c)
+    none = out.isnan()
+    assert (c["out"][none] == 33.0).all() and (c["lse"][none[..., 0]] == 44.0).all()
+    live = ~none[..., 0]
+    got, want = c["out"][live].double(), out[live]
+    over = (got - want).abs() - tol[live]
+    assert not over.isnan().any() and (over.numel() == 0 or over.max().item() <= 0), over.max().item()
+    empty = live & (lse == -math.inf)
+    assert torch.equal(c["lse"] == -math.inf, empty) and (c["out"][empty] == 0).all()
+    some = live & ~empty
+    over = (c["lse"][some].double() - lse[some]).abs() - tol_lse[some]
+    assert not over.isnan().any() and (over.numel() == 0 or over.max().item() <= 0), over.max().item()
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(16, 4, 128), (10, 10, 128), (8, 1, 64), (9, 3, 64), (14, 2, 128), (3, 3, 64)])
+@pytest.mark.parametrize("prefix_lens,lens", [
+    ([4096], [300, 17, 1, 255]), ([1], [1]), ([700, 0, 63], [5, 0, 9, 64, 65, 1]), ([0, 0], [0, 3]),
+    ([128, 129], [0, 0, 0, 0]), ([1000], [1] * 33)])
+def test_one_token_each(cuda, prefix_lens, lens, heads, kv, dim):
+    check(make(prefix_lens, lens, heads, kv, dim))
+
+
+@pytest.mark.parametrize("prefix_lens,lens,heads,kv,dim", [
+    ([4096], [300] * 4, 16, 4, 128), ([100, 300, 5], [37] * 12, 8, 2, 64), ([2500, 2500], [64, 1, 65, 200] * 4, 4, 4, 128)])
+def test_beams_that_share_ancestors(cuda, prefix_lens, lens, heads, kv, dim):
+    check(make(prefix_lens, lens, heads, kv, dim, beams=True))
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(16, 4, 128), (9, 3, 64), (2, 2, 128), (12, 2, 64)])
+@pytest.mark.parametrize("prefix_lens,lens,rows", [
+    ([1001], [61, 30, 9, 100], [37, 30, 1, 80]),
+    ([64, 500], [5, 2, 0, 200], [5, 7, 3, 120]),       # rows before their sequence's keys: some see the prefix alone
+    ([0, 0], [4, 3, 0, 9], [6, 3, 2, 1]),              # and some nothing
+    ([333], [50, 20, 70], [0, 20, 0]),                 # sequences without rows
+    ([2000], [160] * 9, [160] * 9), ([0], [700], [700])])
+def test_rows_of_any_number(cuda, prefix_lens, lens, rows, heads, kv, dim):
+    check(make(prefix_lens, lens, heads, kv, dim, rows=rows))
+
+
+@pytest.mark.parametrize("first,behind", [(0, 7), (3, 0), (5, 70)])
+def test_rows_outside_the_sequences_stay(cuda, first, behind):
+    check(make([300], [40, 8, 3], 8, 2, 128, rows=[20, 8, 1], first_row=first, rows_behind=behind))
+
+
+@pytest.mark.parametrize("sequences", [64, 100])
+def test_many_sequences_on_one_prefix(cuda, sequences):
+    check(make([5000], [1 + i % 40 for i in range(sequences)], 16, 4, 128))
+
+
+def test_a_long_prefix(cuda):
+    check(make([33001], [3, 9], 8, 2, 128))
+
+
+def test_more_keys_than_the_lengths_say(cuda):
+    check(make([70, 5], [3, 9, 1, 0], 8, 2, 128, prefix_capacity=9000, capacity=2000))
+
+
+@pytest.mark.parametrize("spread", [6.0, 0.0])
+def test_peaked_and_flat_scores(cuda, spread):
+    check(make([900, 40], [33, 80, 7, 1], 8, 2, 128, spread=spread))
+
+
+def test_scores_that_rise_along_the_keys(cuda):
+    """The running maximum moves at every key."""
+    import torch
+    c = make([3000], [200, 100], 4, 2, 64)
+    ramp = torch.linspace(-4, 4, 3000, device="cuda")
+    c["q"].fill_(1.0)
+    c["prefix_k"][0, :, :3000] = ramp[:, None].to(torch.bfloat16)
+    check(c)
+
+
+def test_infinite_and_nan_inputs_stay_in_their_rows(cuda):
+    import torch
+    c = make([200], [20, 30, 40], 4, 2, 128, rows=[4, 5, 6])
+    c["q"][6] = math.nan                 # a row of the second sequence
+    c["v"][2, 1, 39] = math.inf          # the last own value of the third: its last row's alone
+    M.prefix_attention(**c)
+    got = c["out"].float()
+    assert got[6].isnan().all() and not got[:6].isnan().any() and not got[7:14].isnan().any()
+    assert got[14, :2].isfinite().all() and got[14, 2:].isinf().all()
+    assert got[:6].isfinite().all() and got[7:14].isfinite().all()
+
+
+def test_scale_and_strides(cuda):
+    import torch
+    c = make([513, 77], [90, 3, 0, 45], 6, 2, 64, rows=[9, 3, 2, 45])
+    c["scale"] = 0.37
+
+    def spread(t, axes):  # the same values inside a larger buffer
+        shape = [s + 8 * (a in axes) for a, s in enumerate(t.shape)]
+        wide = torch.full(shape, math.nan, dtype=t.dtype, device="cuda")
+        view = wide[tuple(slice(0, s) for s in t.shape)]
+        view.copy_(t)
+        return view
+    for name in ("prefix_k", "prefix_v", "k", "v"):
+        c[name] = spread(c[name].transpose(0, 1).contiguous(), (1, 2)).transpose(0, 1)
+    c["q"], c["out"] = spread(c["q"], (1,)), spread(c["out"], (1,))
+    check(c)
+
+
+def test_offsets_above_32_bits(cuda):
+    """A cache of more than 2^32 bytes and 2^31 elements."""
+    import torch
+    kv, dim, cap = 2, 128, 1100
+    caches = 8000  # 2.25e9 elements each
+    n = 3
+    g = gen_of(caches)
+    k = torch.empty(caches, kv, cap, dim, dtype=torch.bfloat16, device="cuda")
+    v = torch.empty_like(k)
+    table = torch.tensor([caches - 1, 0, caches - 7], device="cuda")
+    for t in (k, v):
+        for row in table.tolist():
+            t[row].copy_(torch.randn(kv, cap, dim, generator=g, device="cuda"))
+    c = make([100], [1000, 20, 333], 8, kv, dim, capacity=cap)
+    c["k"], c["v"] = k, v
+    c["ancestry"] = table.to(torch.int32)[:, None].expand(n, cap).contiguous()
+    check(c)
+
+
+@pytest.mark.parametrize("what", ["prefix_lens", "lens", "ancestry", "row_offsets"])
+def test_bad_lengths_offsets_and_ancestors_are_reported(cuda, what):
+    import torch
+    for value in (1 << 30, -5):
+        c = make([200, 100], [20, 30, 10, 5], 4, 2, 128, rows=[3, 3, 3, 3], beams=True)
+        if what == "ancestry":
+            c[what][1, 7] = value
+        else:
+            c[what][1] = value
+        M.prefix_attention(**c)
+        with pytest.raises(M.UocrError) as e:
+            M.ops_check()
+        assert e.value.code == 5 and "prefix_attention" in str(e.value)
+        M.ops_check()
+        if what in ("prefix_lens", "lens"):  # taken as the nearest in range
+            c[what][1] = 0 if value < 0 else c["prefix_k" if what == "prefix_lens" else "k"].shape[2]
+            if value < 0:
+                check(c)
+
+
+def test_runs_are_bitwise_repeatable_on_streams_and_from_graphs(cuda):
+    import torch
+    c = make([3000, 100], [120, 7, 60, 200], 16, 4, 128, beams=True)
+    check(c)
+    want, want_lse = c["out"].clone(), c["lse"].clone()
+    d = make([500], [30, 90, 1], 8, 2, 64, rows=[30, 5, 1], seed=3)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(5):  # two calls at once, with workspaces of their own
+        c["out"].fill_(1.0)
+        torch.cuda.synchronize()
+        M.prefix_attention(**c, stream=side)
+        M.prefix_attention(**d)
+        torch.cuda.synchronize()
+        assert torch.equal(c["out"], want) and torch.equal(c["lse"], want_lse)
+    check(d, call=False)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        M.prefix_attention(**c)
+    # A replay takes the lengths as they are then.
+    c["lens"].copy_(torch.tensor([121, 8, 61, 201], device="cuda"))
+    c["prefix_lens"][1] = 102
+    c["prefix_k"][1, :, 100:102] = 0.5
+    c["prefix_v"][1, :, 100:102] = 0.25
+    c["ancestry"].clamp_(max=3)
+    graph.replay()
+    torch.cuda.synchronize()
+    check(c, call=False)
+
+
+def test_the_lse_joins_parts_of_a_prefix(cuda):
+    """Two halves of a prefix, joined by their lse, are the whole."""
+    import torch
+    c = make([1000], [0, 0, 0], 8, 2, 128, prefix_capacity=1000)
+    check(c)
+    parts = []
+    for half in (slice(0, 400), slice(400, 1000)):
+        d = dict(c, prefix_k=c["prefix_k"][:, :, half].contiguous(), prefix_v=c["prefix_v"][:, :, half].contiguous(),
+                 prefix_lens=torch.tensor([half.stop - half.start], dtype=torch.int32, device="cuda"),
+                 out=torch.empty_like(c["out"]), lse=torch.empty_like(c["lse"]))
+        M.prefix_attention(**d)
+        parts.append((d["out"].double(), d["lse"].double()))
+    (a, la), (b, lb) = parts
+    joined = torch.logaddexp(la, lb)
+    assert (joined - c["lse"].double()).abs().max() < 1e-4
+    both = a * (la - joined).exp()[..., None] + b * (lb - joined).exp()[..., None]
+    _, _, tol, _ = plain(c)
+    # each half and the whole within their tolerances: the halves' add up to at most the whole's of |a| and |b|
+    assert ((both - c["out"].double()).abs() <= 3 * tol + 2.0 ** -7 * (a.abs() + b.abs())).all()
