@@ -24,4 +24,28 @@ cudaError_t launch_beam_select(const uocr_beam_select_args& a, cudaStream_t stre
 
 cudaError_t launch_reorder_states(const uocr_reorder_states_args& a, ErrorWord* err, cudaStream_t stream);
 
+// What a beam search keeps on the device between its steps (beam_search.cu).
+struct BeamState {
+  int beams, steps, vocab, hidden;
+  int eos;
+  int* table;        // [2, beams, steps]: the caches that a beam's keys lie in, then its tokens
+  int* step;         // [1] tokens chosen so far
+  int* prefix_len;   // [1]
+  int* positions;    // [beams] of the tokens that a step consumes
+  int* slots;        // [beams] their places in the beams' caches
+  int* lens;         // [beams] keys of a beam, the new one among them
+  int* tokens;       // [beams] the current tokens
+  int* parents;      // [beams]
+  int* finished;     // [beams]
+  int* new_finished;
+  float* scores;     // [beams]
+  float* new_scores;
+};
+cudaError_t launch_beam_init(const BeamState& s, int prefix_len, cudaStream_t stream);
+// x [beams, hidden] = the tokens' embedding rows; positions, slots and lens of the step.
+cudaError_t launch_beam_embed(const BeamState& s, const __nv_bfloat16* embed, float* x, cudaStream_t stream);
+// The selected beams become the current ones; their tokens are recorded.
+cudaError_t launch_beam_record(const BeamState& s, cudaStream_t stream);
+cudaError_t launch_beam_finish(const BeamState& s, int* tokens, float* scores, int* lengths, cudaStream_t stream);
+
 }  // namespace uocr_b200

@@ -1,6 +1,7 @@
 // C ABI of the operators for sequences that share a page (include/uocr_beam.h):
 // argument checks and launches. Host code only; the kernels are in
-// rotate_heads.cu, prefix_attention.cu, beam_select.cu and reorder_states.cu.
+// rotate_heads.cu, prefix_attention.cu, beam_select.cu and reorder_states.cu,
+// the beam search beside the page decoder in decoder_capi.cu.
 #include <cuda_runtime.h>
 
 #include <algorithm>

@@ -9,6 +9,7 @@
 #include <vector>
 
 #include "../../include/uocr_decoder.h"
+#include "beam.h"
 #include "decoder.h"
 #include "moe_kernels.h"
 #include "plan_internal.h"
@@ -262,6 +263,221 @@ int decode_step(uocr_decoder* p, cudaStream_t stream, cudaEvent_t* ev = nullptr)
                             p->lm_part, p->counters, p->tokens, 1, 0, p->sm_count, stream, pdl),
           "decode: lm_head");
   if (ev != nullptr) DEC_TRY(cudaEventRecord(ev[p->d.layers * (kProfilePhases + 1)], stream), "decode: event");
+  return UOCR_OK;
+}
+
+// ---- beam search ----
+
+// A projection of the prefill kind on a batch of beams: y [rows, n] fp32 at
+// pitch ld (+= with accumulate) = a [rows, k] . w [n, k]^T. Matrices of more rows
+// than the expansion buffer holds (int8 lm_head) go through it in pieces.
+cudaError_t beam_projection(const uocr_decoder* p, const __nv_bfloat16* a, int64_t rows, int64_t k, const void* w,
+                            const float* w_s, int64_t n, float* y, int64_t ld, bool accumulate, cudaStream_t stream) {
+  if (p->int8_act) return int8_projection(p, a, rows, k, w, w_s, n, y, accumulate, stream);
+  const int64_t piece = p->int8 ? std::min(n, p->qkv_rows) : n;
+  for (int64_t c = 0; c < n; c += piece) {
+    const int64_t m = std::min(piece, n - c);
+    const auto* rows_w = static_cast<const char*>(w) + static_cast<size_t>(c * k) * (p->int8 ? 1 : 2);
+    cudaError_t st = cudaSuccess;
+    const __nv_bfloat16* b = gemm_operand(p, rows_w, w_s != nullptr ? w_s + c : nullptr, m, k, stream, &st);
+    if (st != cudaSuccess) return st;
+    GroupedGemm g{};
+    g.mode = 1;
+    g.k_routed = 64;
+    g.n_cols_routed = 256;
+    g.shared_rows = static_cast<int>(rows);
+    g.a_shared = a;
+    g.k_shared = static_cast<int>(k);
+    g.b0_shared = b;
+    g.b1_shared = b;
+    g.b_shared_rows = m;
+    g.n_cols_shared = static_cast<int>((m + 255) / 256 * 256);
+    g.out_shared = y + c;
+    g.ld_out_shared = ld;
+    g.shared_out_f32 = true;
+    g.shared_accumulate = accumulate;
+    g.err = p->err;
+    g.blocks = p->sm_count;
+    st = launch_grouped_gemm(g, stream);
+    if (st != cudaSuccess) return st;
+  }
+  return cudaSuccess;
+}
+
+struct BeamBuffers {
+  BeamState state{};
+  __nv_bfloat16* k = nullptr;  // [layers][beams][kv][steps][128]
+  __nv_bfloat16* v = nullptr;
+  float* logits = nullptr;     // [beams, ld_logits]
+  int64_t ld_logits = 0;
+  void* attention = nullptr;
+  void* select = nullptr;
+  size_t attention_bytes = 0, select_bytes = 0;
+  size_t total = 0;
+};
+
+uocr_prefix_attention_args beam_attention_args(const uocr_decoder* p, int64_t beams, int64_t steps) {
+  uocr_prefix_attention_args a{};
+  a.rows = a.sequences = a.caches = beams;
+  a.prefixes = 1;
+  a.heads = p->d.heads;
+  a.kv_heads = p->d.kv_heads;
+  a.head_dim = kDecHeadDim;
+  a.prefix_capacity = p->d.max_positions;
+  a.capacity = steps;
+  a.ldq = a.ldo = p->d.heads * kDecHeadDim;
+  a.ld_ancestry = steps;
+  a.prefix_head_stride = p->d.max_positions * kDecHeadDim;
+  a.prefix_stride = p->d.kv_heads * a.prefix_head_stride;
+  a.head_stride = steps * kDecHeadDim;
+  a.cache_stride = p->d.kv_heads * a.head_stride;
+  a.scale = 1.0f / std::sqrt(static_cast<float>(kDecHeadDim));
+  return a;
+}
+
+uocr_beam_select_args beam_select_args(const uocr_decoder* p, int64_t beams, int64_t select, int64_t ld) {
+  uocr_beam_select_args a{};
+  a.batch = 1;
+  a.beams = beams;
+  a.select = select;
+  a.vocab = p->d.vocab;
+  a.ld_logits = ld;
+  a.dtype = UOCR_DTYPE_F32;
+  return a;
+}
+
+// The workspace's parts from `base` (null: their size alone).
+BeamBuffers beam_buffers(const uocr_decoder* p, int64_t beams, int64_t steps, void* base) {
+  BeamBuffers b;
+  char* c = static_cast<char*>(base);
+  auto take = [&](size_t bytes) {
+    void* at = c != nullptr ? c + b.total : nullptr;
+    b.total += up256(bytes);
+    return at;
+  };
+  const size_t n = static_cast<size_t>(beams);
+  const size_t cache = static_cast<size_t>(p->d.layers * beams * p->d.kv_heads * steps * kDecHeadDim) * 2;
+  b.k = static_cast<__nv_bfloat16*>(take(cache));
+  b.v = static_cast<__nv_bfloat16*>(take(cache));
+  b.ld_logits = p->int8_act ? p->d.vocab : (p->d.vocab + 255) / 256 * 256;  // the GEMM's tiles are whole
+  b.logits = static_cast<float*>(take(n * b.ld_logits * 4));
+  b.attention_bytes = prefix_attention_bytes(beam_attention_args(p, beams, steps));
+  b.attention = take(b.attention_bytes);
+  b.select_bytes = std::max(beam_select_bytes(beam_select_args(p, beams, beams, b.ld_logits)),
+                            beam_select_bytes(beam_select_args(p, 1, beams, b.ld_logits)));
+  b.select = take(b.select_bytes);
+  BeamState& s = b.state;
+  s.beams = static_cast<int>(beams), s.steps = static_cast<int>(steps);
+  s.vocab = static_cast<int>(p->d.vocab), s.hidden = static_cast<int>(p->d.hidden);
+  s.table = static_cast<int*>(take(2 * n * static_cast<size_t>(steps) * 4));
+  s.step = static_cast<int*>(take(4));
+  s.prefix_len = static_cast<int*>(take(4));
+  for (int** field : {&s.positions, &s.slots, &s.lens, &s.tokens, &s.parents, &s.finished, &s.new_finished})
+    *field = static_cast<int*>(take(n * 4));
+  s.scores = static_cast<float*>(take(n * 4));
+  s.new_scores = static_cast<float*>(take(n * 4));
+  return b;
+}
+
+int check_beams(const uocr_decoder* p, const char* op, int64_t beams, int64_t steps) {
+  const std::string name = std::string(op) + ": ";
+  if (p == nullptr) return dfail(UOCR_ERR_INVALID_ARGUMENT, name + "null decoder");
+  if (beams < 1 || beams > kDecodeMaxRows || beams > p->d.max_prefill)
+    return dfail(UOCR_ERR_INVALID_ARGUMENT, name + "beams outside [1, 16] or above max_prefill");
+  if (steps < 1 || steps > p->d.max_positions)
+    return dfail(UOCR_ERR_INVALID_ARGUMENT, name + "steps outside [1, max_positions]");
+  if (p->d.vocab > (1 << 20)) return dfail(UOCR_ERR_UNSUPPORTED, name + "vocab above 2^20");
+  return UOCR_OK;
+}
+
+// The selection from `logits` for `from` beams, into the state's new values.
+cudaError_t beam_choose(const uocr_decoder* p, const BeamBuffers& b, const float* logits, int64_t from,
+                        cudaStream_t stream) {
+  const BeamState& s = b.state;
+  uocr_beam_select_args a = beam_select_args(p, from, s.beams, b.ld_logits);
+  a.logits = logits;
+  a.scores = s.scores;
+  a.finished = s.finished;
+  a.tokens = s.tokens;
+  a.parents = s.parents;
+  a.new_scores = s.new_scores;
+  a.new_finished = s.new_finished;
+  a.eos = s.eos;
+  a.workspace = b.select;
+  a.workspace_bytes = static_cast<int64_t>(b.select_bytes);
+  return launch_beam_select(a, stream);
+}
+
+// One step of all beams: their current tokens through every layer, the head,
+// the next selection, and the beams' tables in their new order.
+int beam_step(uocr_decoder* p, const BeamBuffers& b, ErrorWord* err, cudaStream_t stream) {
+  const BeamState& s = b.state;
+  const int64_t H = p->d.hidden, A = p->d.heads * kDecHeadDim, KV = p->d.kv_heads * kDecHeadDim, n = s.beams;
+  DEC_TRY(launch_beam_embed(s, p->embed, p->x, stream), "beam_search: embedding");
+  uocr_prefix_attention_args att = beam_attention_args(p, s.beams, s.steps);
+  att.q = reinterpret_cast<const uint16_t*>(p->qb);
+  att.out = reinterpret_cast<uint16_t*>(p->attn);
+  att.prefix_lens = s.prefix_len;
+  att.lens = s.lens;
+  att.ancestry = s.table;
+  att.workspace = b.attention;
+  att.workspace_bytes = static_cast<int64_t>(b.attention_bytes);
+  uocr_rotate_heads_args rot{};
+  rot.q = p->qkv;
+  rot.k = p->qkv + A;
+  rot.v = p->qkv + A + KV;
+  rot.inv_freq = p->inv_freq;
+  rot.positions = s.positions;
+  rot.slots = s.slots;
+  rot.q_out = reinterpret_cast<uint16_t*>(p->qb);
+  rot.rows = rot.caches = n;
+  rot.q_heads = p->d.heads;
+  rot.kv_heads = p->d.kv_heads;
+  rot.head_dim = rot.rotary_dim = kDecHeadDim;
+  rot.ldq = rot.ldk = rot.ldv = p->qkv_rows;
+  rot.ldqo = A;
+  rot.capacity = s.steps;
+  rot.head_stride = att.head_stride;
+  rot.cache_stride = att.cache_stride;
+  rot.magnitude = 1.0f;
+  rot.dtype = UOCR_DTYPE_F32;
+  const int64_t layer_cache = n * att.cache_stride;
+  for (int64_t l = 0; l < p->d.layers; ++l) {
+    const DecLayer& L = p->layers[static_cast<size_t>(l)];
+    DEC_TRY(launch_norm_rows_bf16(p->x, n, static_cast<int>(H), L.input_norm, p->d.rms_norm_eps, p->xn, stream),
+            "beam_search: norm");
+    DEC_TRY(beam_projection(p, p->xn, n, H, L.wqkv, L.wqkv_s, p->qkv_rows, p->qkv, p->qkv_rows, false, stream),
+            "beam_search: q/k/v product");
+    rot.k_cache = reinterpret_cast<uint16_t*>(b.k + l * layer_cache);
+    rot.v_cache = reinterpret_cast<uint16_t*>(b.v + l * layer_cache);
+    DEC_TRY(launch_rotate_heads(rot, err, stream), "beam_search: rotation");
+    att.prefix_k = reinterpret_cast<const uint16_t*>(kc_of(p, l));
+    att.prefix_v = reinterpret_cast<const uint16_t*>(vc_of(p, l));
+    att.k = rot.k_cache;
+    att.v = rot.v_cache;
+    DEC_TRY(launch_prefix_attention(att, err, stream), "beam_search: attention");
+    DEC_TRY(beam_projection(p, p->attn, n, A, L.wo, L.wo_s, H, p->x, H, true, stream), "beam_search: output product");
+    DEC_RC(moe_layer_inplace(p->moe, l, p->x, n, stream));
+  }
+  DEC_TRY(launch_norm_rows_bf16(p->x, n, static_cast<int>(H), p->final_norm, p->d.rms_norm_eps, p->xn, stream),
+          "beam_search: final norm");
+  DEC_TRY(beam_projection(p, p->xn, n, H, p->lm_head, p->lm_head_s, p->d.vocab, b.logits, b.ld_logits, false, stream),
+          "beam_search: lm_head");
+  DEC_TRY(beam_choose(p, b, b.logits, n, stream), "beam_search: selection");
+  uocr_reorder_states_args order{};
+  order.state = s.table;
+  order.parents = s.parents;
+  order.counts = s.lens;  // the caches of the keys so far, and as many tokens
+  order.layers = 2;
+  order.groups = 1;
+  order.beams = n;
+  order.segments = 1;
+  order.units = s.steps;
+  order.unit_bytes = 4;
+  order.row_stride = s.steps * int64_t{4};
+  order.layer_stride = n * order.row_stride;
+  DEC_TRY(launch_reorder_states(order, err, stream), "beam_search: reordering");
+  DEC_TRY(launch_beam_record(s, stream), "beam_search: record");
   return UOCR_OK;
 }
 
@@ -664,6 +880,42 @@ int uocr_decoder_profile_decode(uocr_decoder* p, int64_t steps, float* ms, void*
   for (int k = 0; k <= kProfilePhases; ++k) ms[k] = static_cast<float>(acc[k] / static_cast<double>(steps));
   p->length += steps;
   p->generated += steps;
+  return UOCR_OK;
+}
+
+int uocr_decoder_beam_workspace(const uocr_decoder* p, int64_t beams, int64_t steps, int64_t* bytes) {
+  DEC_RC(check_beams(p, "decoder_beam_workspace", beams, steps));
+  if (bytes == nullptr) return dfail(UOCR_ERR_INVALID_ARGUMENT, "decoder_beam_workspace: null argument");
+  *bytes = static_cast<int64_t>(beam_buffers(p, beams, steps, nullptr).total);
+  return UOCR_OK;
+}
+
+int uocr_decoder_beam_search(uocr_decoder* p, const uocr_beam_search_args* a, void* stream_v) {
+  if (a == nullptr) return dfail(UOCR_ERR_INVALID_ARGUMENT, "decoder_beam_search: null arguments");
+  DEC_RC(check_beams(p, "decoder_beam_search", a->beams, a->steps));
+  if (!p->started) return dfail(UOCR_ERR_INVALID_ARGUMENT, "decoder_beam_search: no prefill started a sequence");
+  if (p->length + a->steps > p->d.max_positions)
+    return dfail(UOCR_ERR_INVALID_ARGUMENT, "decoder_beam_search: the beams would pass max_positions");
+  if (a->eos < -1 || a->eos >= p->d.vocab)
+    return dfail(UOCR_ERR_INVALID_ARGUMENT, "decoder_beam_search: eos must be a token or -1");
+  if (a->reserved != 0) return dfail(UOCR_ERR_INVALID_ARGUMENT, "decoder_beam_search: reserved must be 0");
+  if (a->tokens == nullptr || a->scores == nullptr)
+    return dfail(UOCR_ERR_INVALID_ARGUMENT, "decoder_beam_search: null pointer");
+  BeamBuffers b = beam_buffers(p, a->beams, a->steps, a->workspace);
+  if (a->workspace == nullptr || (reinterpret_cast<uintptr_t>(a->workspace) & 255) != 0 ||
+      a->workspace_bytes < static_cast<int64_t>(b.total))
+    return dfail(UOCR_ERR_INVALID_ARGUMENT,
+                 "decoder_beam_search: the workspace is missing, too small or not 256-byte aligned "
+                 "(uocr_decoder_beam_workspace)");
+  b.state.eos = a->eos;
+  Guard guard(p->d.device);
+  auto stream = static_cast<cudaStream_t>(stream_v);
+  DEC_TRY(launch_beam_init(b.state, static_cast<int>(p->length), stream), "decoder_beam_search: set-up");
+  // The first tokens: one beam, the sequence itself, continues as all of them.
+  DEC_TRY(beam_choose(p, b, p->logits, 1, stream), "decoder_beam_search: selection");
+  DEC_TRY(launch_beam_record(b.state, stream), "decoder_beam_search: record");
+  for (int64_t i = 1; i < a->steps; ++i) DEC_RC(beam_step(p, b, p->err, stream));
+  DEC_TRY(launch_beam_finish(b.state, a->tokens, a->scores, a->lengths, stream), "decoder_beam_search: results");
   return UOCR_OK;
 }
 

@@ -50,7 +50,8 @@ INT8_EXPORTS = ["uocr_quantize_tokens", "uocr_linear_w8a8", "uocr_grouped_w8a8_w
 # Every symbol include/uocr_beam.h declares.
 BEAM_EXPORTS = [
     "uocr_rope_frequencies", "uocr_rotate_heads", "uocr_prefix_attention_workspace", "uocr_prefix_attention",
-    "uocr_beam_select_workspace", "uocr_beam_select", "uocr_reorder_states",
+    "uocr_beam_select_workspace", "uocr_beam_select", "uocr_reorder_states", "uocr_decoder_beam_workspace",
+    "uocr_decoder_beam_search",
 ]
 
 # Every symbol include/uocr_moe.h declares.
@@ -173,6 +174,12 @@ class ReorderStatesArgs(ctypes.Structure):
                                       "row_stride", "segment_stride")]
 
 
+class BeamSearchArgs(ctypes.Structure):
+    _fields_ = [("beams", ctypes.c_int64), ("steps", ctypes.c_int64), ("eos", ctypes.c_int32),
+                ("reserved", ctypes.c_int32), ("tokens", ctypes.c_void_p), ("scores", ctypes.c_void_p),
+                ("lengths", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64)]
+
+
 def _packer(args) -> struct.Struct:
     """The fields of a ctypes structure (pointers, int64, int32, float) as a struct format; null pointers are 0. A call
     packs its arguments in a third of the time that the structure's constructor takes."""
@@ -245,6 +252,8 @@ def lib() -> ctypes.CDLL:
         L.uocr_beam_select_workspace.argtypes = [vp, ctypes.POINTER(i64)]
         L.uocr_beam_select.argtypes = [vp, vp]
         L.uocr_reorder_states.argtypes = [vp, vp]
+        L.uocr_decoder_beam_workspace.argtypes = [vp, i64, i64, ctypes.POINTER(i64)]
+        L.uocr_decoder_beam_search.argtypes = [vp, ctypes.POINTER(BeamSearchArgs), vp]
         _lib = L
     return _lib
 
@@ -889,6 +898,25 @@ class Decoder:
 
     def decode(self, steps: int, tokens=None, logits=None, stream=None):
         _check(lib().uocr_decoder_decode(self.h, steps, _ptr(tokens), _ptr(logits), _stream(stream)))
+
+    def beam_search(self, beams: int, steps: int, tokens, scores, lengths=None, eos: int = -1, stream=None):
+        """The best `beams` continuations of `steps` tokens behind the sequence, which stays as it is: tokens (int32
+        [beams, steps]), scores (fp32 [beams]) and lengths (int32 [beams], up to and with eos) receive them, best first
+        (uocr_decoder_beam_search). The workspace comes from torch's allocator, from the blocks of the stream."""
+        import torch
+        i32, f32, device = torch.int32, torch.float32, self.desc.device
+        need = ctypes.c_int64()
+        _check(lib().uocr_decoder_beam_workspace(self.h, beams, steps, ctypes.byref(need)))
+        token_ptr, score_ptr = _vector(tokens, "tokens", beams * steps, i32), _vector(scores, "scores", beams, f32)
+        length_ptr = None if lengths is None else _vector(lengths, "lengths", beams, i32)
+        if any(t is not None and t.get_device() != device for t in (tokens, scores, lengths)):
+            raise ValueError(f"tokens, scores and lengths must be on the decoder's cuda:{device}")
+        if stream is None:
+            stream = torch.cuda.current_stream(device)
+        workspace = _workspace(need.value + 256, torch.device("cuda", device), stream)  # held until the launches are made
+        base = (workspace.data_ptr() + 255) // 256 * 256
+        args = BeamSearchArgs(beams, steps, eos, 0, token_ptr, score_ptr, length_ptr, base, need.value)
+        _check(lib().uocr_decoder_beam_search(self.h, ctypes.byref(args), _stream(stream)))
 
     def check(self, stream=None):
         _check(lib().uocr_decoder_check(self.h, _stream(stream)))

@@ -5,7 +5,8 @@
  * keys normalised, rotated and appended to caches; attention over the shared
  * prefix, read once for all of them, and over each one's own keys; the
  * selection of the next beams over beams and vocabulary; and the beams' states
- * brought into their new order.
+ * brought into their new order. uocr_decoder_beam_search runs them on the page
+ * decoder of uocr_decoder.h.
  *
  * Conventions are uocr_moe.h's: plain device pointers, a cudaStream_t passed as
  * void*, status codes with uocr_last_error(), nothing synchronises the stream
@@ -19,6 +20,7 @@
 
 #include <stdint.h>
 
+#include "uocr_decoder.h"
 #include "uocr_moe.h"
 
 #ifdef __cplusplus
@@ -173,6 +175,32 @@ typedef struct uocr_reorder_states_args {
  * UOCR_BEAM_MAX. A bad parent is recorded and leaves its row as it is; a count
  * out of range is recorded and taken as the nearest that is in range. */
 int uocr_reorder_states(const uocr_reorder_states_args* args, void* stream);
+
+/* ---- beam search on the page decoder ---- */
+
+typedef struct uocr_beam_search_args {
+  int64_t beams;            /* 1 .. 16, at most the decoder's max_prefill */
+  int64_t steps;            /* tokens of each beam */
+  int32_t eos;              /* the token that ends a beam, or -1 */
+  int32_t reserved;         /* 0 */
+  int32_t* tokens;          /* [beams, steps]: the beams' tokens, best beam first; behind a beam's end its eos */
+  float* scores;            /* [beams]: their log-probabilities */
+  int32_t* lengths;         /* [beams]: tokens up to and with the first eos, or NULL */
+  void* workspace;          /* device memory for the call's duration, 256-byte aligned: the beams' caches */
+  int64_t workspace_bytes;  /* at least what uocr_decoder_beam_workspace says */
+} uocr_beam_search_args;
+
+int uocr_decoder_beam_workspace(const uocr_decoder* dec, int64_t beams, int64_t steps, int64_t* bytes);
+
+/* `steps` tokens for `beams` beams behind the decoder's sequence (a prefill, and
+ * the decode steps after it): the first tokens come from the logits that the
+ * sequence ended with, each later step runs all beams as one batch over the
+ * sequence's cache, shared, and their own. The sequence itself stays as it is: a
+ * decode or another search may follow. The sequence and the steps have to fit
+ * max_positions. Decoders with int8 weights expand them to bf16 in every step, as
+ * their prefill does; with UOCR_DECODER_INT8_ACTIVATIONS the projections and the
+ * head run on int8 activations. */
+int uocr_decoder_beam_search(uocr_decoder* dec, const uocr_beam_search_args* args, void* stream);
 
 #ifdef __cplusplus
 }

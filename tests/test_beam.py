@@ -30,7 +30,8 @@ def test_struct_layouts_match_the_header(tmp_path):
     if cc is None:
         pytest.skip("no C compiler")
     structs = {"uocr_rotate_heads_args": M.RotateHeadsArgs, "uocr_prefix_attention_args": M.PrefixAttentionArgs,
-               "uocr_beam_select_args": M.BeamSelectArgs, "uocr_reorder_states_args": M.ReorderStatesArgs}
+               "uocr_beam_select_args": M.BeamSelectArgs, "uocr_reorder_states_args": M.ReorderStatesArgs,
+               "uocr_beam_search_args": M.BeamSearchArgs}
     lines = ["#include <stddef.h>", "#include <stdio.h>", '#include "uocr_beam.h"', "int main(void) {"]
     for cname, cls in structs.items():
         lines.append(f'  printf("%zu\\n", sizeof({cname}));')
@@ -213,3 +214,12 @@ def test_binding_refuses_tensors_off_the_gpu():
         pytest.skip("needs a current device to compare with")
     with pytest.raises(ValueError):
         M.reorder_states(torch.zeros(4, 4), torch.zeros(4, dtype=torch.int32), 4)
+
+
+def test_beam_search_refuses_before_a_decoder_is_touched():
+    out = ctypes.c_int64()
+    assert M.lib().uocr_decoder_beam_workspace(None, 4, 8, ctypes.byref(out)) == 1
+    assert M.lib().uocr_decoder_beam_search(None, None, None) == 1
+    args = M.BeamSearchArgs(4, 8, -1, 0, BASE, BASE, None, BASE, BIG)
+    assert M.lib().uocr_decoder_beam_search(None, ctypes.byref(args), None) == 1
+    assert M.lib().uocr_last_error().decode().startswith("decoder_beam_search: ")
