@@ -71,6 +71,9 @@ struct Grid {
   int prefix_tiles, own_tiles;  // bounds: with row offsets the rows are known to the device alone
   int prefix_blocks;
   int own_slots;
+  // 1: launched behind a kernel of the same call, which this one takes nothing from. That kernel lets this one start
+  // when it has itself waited for all work before the call, so the wait for it can come last.
+  int late_wait;
 };
 
 // Finds the sequence (prefix) that tile `t` is of; -1 behind the last one.
@@ -154,10 +157,15 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(Attention a, G
   constexpr int kStage = 2 * kKeys * kPitch;
   extern __shared__ __align__(16) unsigned char raw[];
   __nv_bfloat16* ring = reinterpret_cast<__nv_bfloat16*>(raw);
-  pdl_wait();
-  pdl_launch_dependents();
+  if (!g.late_wait) {
+    pdl_wait();
+    pdl_launch_dependents();
+  }
   Tile w;
-  if (!find_work<kDim, kRows>(a, g, &w)) return;
+  if (!find_work<kDim, kRows>(a, g, &w)) {
+    if (g.late_wait) pdl_wait();
+    return;
+  }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gr = lane >> 2, tq = lane & 3;
   const int row0 = warp % kWarpRows * 16, warp_key = warp / kWarpRows * kWarpKeys;
@@ -389,6 +397,7 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(Attention a, G
       *reinterpret_cast<float4*>(a.part_o + at * kDim + col) = acc;
     }
   }
+  if (g.late_wait) pdl_wait();
 }
 
 // A warp joins the parts of a (row, head).
@@ -428,21 +437,33 @@ __global__ void __launch_bounds__(kThreads) attention_join_kernel(Attention a) {
     a.lse[cell] = sum != 0.0f ? (top + log2f(sum)) * 0.69314718055994530942f : -INFINITY;
 }
 
-// The parts that the prefixes and the own keys are cut into. Blocks of about
-// `keys` keys: as many as fill the card's SMs twice where there are few tiles,
-// whole ranges where there are many.
+// The parts that the prefixes and the own keys are cut into, and the kernels.
 struct Plan {
+  bool tc;  // the prefixes by the tensor-core kernel
   int prefix_slots, own_slots, warp_rows;
-  int64_t prefix_tiles, own_tiles;
+  int64_t prefix_tiles, own_tiles;  // of the kernel for few rows
 };
 
-constexpr int kMaxPrefixSlots = 64, kMaxOwnSlots = 16;
+constexpr int kMaxPrefixSlots = 64, kMaxOwnSlots = 16, kMaxTcSlots = 128;
+constexpr int kSms = 148;  // blocks of the tensor-core kernel, one an SM; correct on any number of SMs
+
+// A prefix with many rows is arithmetic, for the tensor cores.
+bool many_rows(const uocr_prefix_attention_args& a) {
+  const int64_t group = a.heads / a.kv_heads;
+  if (a.prefix_capacity == 0 || !(a.scale > 0.0f)) return false;
+  // what a tensor map takes
+  auto far = [](int64_t stride) { return stride <= 0 || stride >= (int64_t{1} << 39); };
+  if ((a.kv_heads > 1 && far(a.prefix_head_stride)) || (a.prefixes > 1 && far(a.prefix_stride))) return false;
+  return a.rows * group / a.prefixes > 64;
+}
 
 Plan plan_of(const uocr_prefix_attention_args& a) {
   Plan p{};
+  p.tc = many_rows(a);
   const int64_t group = a.heads / a.kv_heads;
-  // Rows of a tile by the rows of a prefix: those of a sequence alone where there is no prefix.
-  const int64_t rows = a.rows * group / std::max<int64_t>(a.prefix_capacity > 0 ? a.prefixes : a.sequences, 1);
+  // Rows of a tile by the rows of a prefix; of a sequence where the prefixes are apart.
+  const int64_t sets = p.tc || a.prefix_capacity == 0 ? a.sequences : a.prefixes;
+  const int64_t rows = a.rows * group / std::max<int64_t>(sets, 1);
   p.warp_rows = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
   const int64_t tile = 16 * p.warp_rows;
   auto tiles = [&](int64_t count, int64_t each) {
@@ -450,14 +471,21 @@ Plan plan_of(const uocr_prefix_attention_args& a) {
     return a.row_offsets == nullptr ? count * ((each * group + tile - 1) / tile)
                                     : a.rows * group / tile + std::min(count, a.rows);
   };
-  p.prefix_tiles = a.prefix_capacity > 0 ? tiles(a.prefixes, a.sequences / a.prefixes) : 0;
+  p.prefix_tiles = a.prefix_capacity > 0 && !p.tc ? tiles(a.prefixes, a.sequences / a.prefixes) : 0;
   p.own_tiles = a.capacity > 0 ? tiles(a.sequences, 1) : 0;
   const int64_t bp = p.prefix_tiles * a.kv_heads, bo = p.own_tiles * a.kv_heads;
+  // Parts of about `keys` keys: as many as fill the SMs twice where there are few tiles, whole ranges where there are
+  // many.
   for (int64_t keys = 2 * kKeys;; keys *= 2) {
     p.prefix_slots = static_cast<int>(std::min<int64_t>((a.prefix_capacity + keys - 1) / keys, kMaxPrefixSlots));
     p.own_slots = static_cast<int>(std::min<int64_t>((a.capacity + keys - 1) / keys, kMaxOwnSlots));
-    if (bp * p.prefix_slots + bo * p.own_slots <= 2 * 148) break;
+    if (bp * p.prefix_slots + bo * p.own_slots <= 2 * kSms) break;
     if (keys >= a.prefix_capacity && keys >= a.capacity) break;
+  }
+  // A range of keys meets about as many blocks as there are for each range.
+  if (p.tc) {
+    const int64_t ranges = a.kv_heads * ((a.rows * group + kAttentionTcRows - 1) / kAttentionTcRows);
+    p.prefix_slots = static_cast<int>(std::min<int64_t>(kSms / ranges + 3, kMaxTcSlots));
   }
   return p;
 }
@@ -477,10 +505,14 @@ cudaError_t launch(const uocr_prefix_attention_args& args, const Attention& a, c
   Grid g{};
   g.prefix_tiles = static_cast<int>(p.prefix_tiles);
   g.own_tiles = static_cast<int>(p.own_tiles);
-  g.prefix_blocks = static_cast<int>(p.prefix_tiles * a.kv_heads * p.prefix_slots);
+  g.prefix_blocks = p.tc ? 0 : static_cast<int>(p.prefix_tiles * a.kv_heads * p.prefix_slots);
   g.own_slots = p.own_slots;
   const int64_t blocks = g.prefix_blocks + p.own_tiles * a.kv_heads * p.own_slots;
   cudaError_t st = cudaSuccess;
+  if (p.tc) {
+    if ((st = launch_attention_tc(a, kDim, kSms, stream)) != cudaSuccess) return st;
+    g.late_wait = 1;
+  }
   if (blocks > 0) {
     const unsigned n = static_cast<unsigned>(blocks);
     st = p.warp_rows == 1   ? launch_rows<kDim, 1>(a, g, n, stream)

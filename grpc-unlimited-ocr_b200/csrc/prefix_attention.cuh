@@ -91,4 +91,10 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return reinterpret_cast<const uint32_t&>(h);
 }
 
+// Rows (a row and a query head each) that a block of the tensor-core kernel takes.
+constexpr int kAttentionTcRows = 256;
+// The prefixes' parts of many rows by tcgen05 (prefix_attention_tc.cu): `blocks`
+// resident blocks; at least two slots; a positive scale.
+cudaError_t launch_attention_tc(const Attention& a, int dim, unsigned blocks, cudaStream_t stream);
+
 }  // namespace uocr_b200

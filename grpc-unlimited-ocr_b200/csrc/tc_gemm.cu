@@ -447,6 +447,26 @@ bool make_tile_tmap(CUtensorMap* map, const void* base, bool bf16, int64_t rows,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool make_cache_tmap(CUtensorMap* map, const void* base, int64_t dim, int64_t capacity, int64_t heads, int64_t caches,
+                     int64_t head_stride, int64_t cache_stride, int box_keys) {
+  EncodeTiled fn = encoder();
+  if (fn == nullptr || base == nullptr) return false;
+  const int64_t key = dim * 2;
+  // The stride of a dimension of one is not used: any that is valid.
+  const int64_t of_head = heads > 1 ? head_stride * 2 : key, of_cache = caches > 1 ? cache_stride * 2 : key;
+  constexpr int64_t kFar = int64_t{1} << 40;
+  if (of_head <= 0 || of_cache <= 0 || of_head >= kFar || of_cache >= kFar) return false;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(capacity),
+                              static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(caches)};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(key), static_cast<cuuint64_t>(of_head),
+                                 static_cast<cuuint64_t>(of_cache)};
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_keys), 1, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 size_t grouped_gemm_smem_bytes() {
   return static_cast<size_t>(kStages) * kStageBytes + 4 * kStageTileBytes + 1024;
 }

@@ -81,6 +81,13 @@ bool make_int8_tmap(CUtensorMap* map, const int8_t* base, int64_t rows, int64_t 
 bool make_tile_tmap(CUtensorMap* map, const void* base, bool bf16, int64_t rows, int64_t cols, int64_t ld,
                     int box_rows);
 
+// Tensor map of a bf16 cache [caches, heads, capacity, dim] (dim a multiple of
+// 64, keys contiguous, strides in elements): boxes of 64 dims x box_keys keys of
+// one head, 128-byte swizzle, zeros outside the capacity. False where the strides
+// are not a tensor map's (a repeated cache or head, or one too far away).
+bool make_cache_tmap(CUtensorMap* map, const void* base, int64_t dim, int64_t capacity, int64_t heads, int64_t caches,
+                     int64_t head_stride, int64_t cache_stride, int box_keys);
+
 size_t grouped_gemm_smem_bytes();
 cudaError_t launch_grouped_gemm(const GroupedGemm& g, cudaStream_t stream);
 
