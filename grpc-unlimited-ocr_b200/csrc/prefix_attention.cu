@@ -19,6 +19,7 @@ namespace {
 constexpr int kThreads = 128;
 constexpr int kKeys = 64;    // of a stage
 constexpr int kStages = 3;
+constexpr int kMaxSlots = 160;  // of a row: the most that a plan gives its prefix and its own keys
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -60,7 +61,7 @@ struct Tile {
   int all_see;        // keys that every row of the tile sees
   bool own;
   int sequence, slot;
-  const __nv_bfloat16* k;  // of key 0 (without ancestry)
+  const __nv_bfloat16* k;  // of key 0 (with ancestry: in cache 0)
   const __nv_bfloat16* v;
 };
 
@@ -68,7 +69,6 @@ struct Tile {
 // counted through over the prefixes (sequences): ceil(rows * group / kRows) of
 // each, then the key/value heads, then the parts.
 struct Grid {
-  int prefix_tiles, own_tiles;  // bounds: with row offsets the rows are known to the device alone
   int prefix_blocks;
   int own_slots;
   // 1: launched behind a kernel of the same call, which this one takes nothing from. That kernel lets this one start
@@ -132,8 +132,9 @@ __device__ bool find_work(const Attention& a, const Grid& g, Tile* w) {
     // the tile's last row sees the most
     keys = max(0, w->limit0 + (w->start + w->count - 1) / a.group);
     w->all_see = w->limit0 + w->start / a.group;
-    w->k = a.k + of * a.cache_stride + w->kv_head * a.head_stride;
-    w->v = a.v + of * a.cache_stride + w->kv_head * a.head_stride;
+    const int64_t base = (a.ancestry != nullptr ? 0 : of * a.cache_stride) + w->kv_head * a.head_stride;
+    w->k = a.k + base;
+    w->v = a.v + base;
   } else {
     keys = w->limit0 = w->all_see = prefix_len_of(a, of);
     w->k = a.prefix_k + of * a.prefix_stride + w->kv_head * a.prefix_head_stride;
@@ -170,33 +171,46 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(Attention a, G
   const int gr = lane >> 2, tq = lane & 3;
   const int row0 = warp % kWarpRows * 16, warp_key = warp / kWarpRows * kWarpKeys;
 
+  // A thread copies 16 bytes of every kStep-th key of a stage. Where its keys lie (with ancestry: in any of the caches)
+  // is read a fill ahead of the copies, all keys at once.
+  constexpr int kStep = kThreads / (kDim / 8), kCopies = kKeys / kStep;
+  const int copy_key = threadIdx.x / (kDim / 8), copy_col = threadIdx.x % (kDim / 8) * 8;
+  const bool gathers = w.own && a.ancestry != nullptr;
+  int from[kCopies] = {};
+  auto look_up = [&](int key) {
+    if (!gathers) return;
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) {
+      const int at = key + copy_key + i * kStep;
+      from[i] = at < w.key1 ? a.ancestry[w.sequence * a.ld_ancestry + at] : 0;
+    }
+  };
   auto fill = [&](int stage, int key) {
-    __nv_bfloat16* ks = ring + stage * kStage;
+    __nv_bfloat16* ks = ring + stage * kStage + copy_key * kPitch + copy_col;
     __nv_bfloat16* vs = ks + kKeys * kPitch;
-    for (int c = threadIdx.x; c < kKeys * (kDim / 8); c += kThreads) {
-      const int r = c / (kDim / 8), col = c % (kDim / 8) * 8;
-      const int at = key + r;
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) {
+      const int at = key + copy_key + i * kStep;
       const bool valid = at < w.key1;
-      const __nv_bfloat16 *k = w.k, *v = w.v;
-      if (w.own && valid && a.ancestry != nullptr) {
-        int cache = a.ancestry[w.sequence * a.ld_ancestry + at];
-        if (cache < 0 || cache >= a.caches) {
+      int64_t off = valid ? static_cast<int64_t>(at) * kDim + copy_col : 0;
+      if (gathers) {
+        int cache = from[i];
+        if (valid && (cache < 0 || cache >= a.caches)) {
           raise_error(a.err, kDevBadIndex, kSiteAncestor, w.sequence, cache);
           cache = w.sequence < a.caches ? w.sequence : 0;
         }
-        const int64_t base = cache * a.cache_stride + w.kv_head * a.head_stride;
-        k = a.k + base;
-        v = a.v + base;
+        off += cache * a.cache_stride;
       }
-      const int64_t off = valid ? static_cast<int64_t>(at) * kDim + col : 0;
-      cp_async16_or_zero(ks + r * kPitch + col, (valid ? k : a.q) + off, valid);
-      cp_async16_or_zero(vs + r * kPitch + col, (valid ? v : a.q) + off, valid);
+      cp_async16_or_zero(ks + i * kStep * kPitch, w.k + off, valid);
+      cp_async16_or_zero(vs + i * kStep * kPitch, w.v + off, valid);
     }
   };
+  look_up(w.key0);
 #pragma unroll
   for (int s = 0; s < kStages - 1; ++s) {
     if (w.key0 + s * kKeys < w.key1) fill(s, w.key0 + s * kKeys);
     cp_async_commit();
+    look_up(w.key0 + (s + 1) * kKeys);
   }
 
   // This thread's two rows of the warp's tile, and the warp's queries as A fragments.
@@ -231,6 +245,7 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(Attention a, G
     const int ahead = key + (kStages - 1) * kKeys;
     if (ahead < w.key1) fill((stage + kStages - 1) % kStages, ahead);
     cp_async_commit();
+    look_up(ahead + kKeys);
     const __nv_bfloat16* ks = ring + stage * kStage + warp_key * kPitch;
     const __nv_bfloat16* vs = ks + kKeys * kPitch;
     stage = (stage + 1) % kStages;
@@ -400,39 +415,94 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(Attention a, G
   if (g.late_wait) pdl_wait();
 }
 
-// A warp joins the parts of a (row, head).
-template <int kDim>
+// kWarps warps join the parts of a (row, head): first all maxima and sums, a lane a part, then the outputs of the parts
+// that hold keys, warp by warp every kWarps-th one, eight under way at a time.
+template <int kDim, int kWarps>
 __global__ void __launch_bounds__(kThreads) attention_join_kernel(Attention a) {
-  constexpr int kEach = kDim / 32;
+  constexpr int kEach = kDim / 32, kCells = kThreads / 32 / kWarps;
+  __shared__ float factors[kCells][kMaxSlots];
+  __shared__ float sums[kCells][kWarps][kDim];
   pdl_wait();
   pdl_launch_dependents();
-  const int64_t cell = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (cell >= static_cast<int64_t>(a.rows) * a.heads) return;
-  const int64_t row = cell / a.heads;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, local = warp / kWarps, along = warp % kWarps;
+  const int64_t cell = static_cast<int64_t>(blockIdx.x) * kCells + local;
+  bool live = cell < static_cast<int64_t>(a.rows) * a.heads;
+  const int64_t row = live ? cell / a.heads : 0;
   const int head = static_cast<int>(cell % a.heads);
-  if (a.row_offsets != nullptr && (row < a.row_offsets[0] || row >= a.row_offsets[a.sequences])) return;
+  if (live && a.row_offsets != nullptr) live = row >= a.row_offsets[0] && row < a.row_offsets[a.sequences];
   const float2* ml = a.part_ml + cell * a.slots;
+  float2 mine[kMaxSlots / 32];
   float top = -INFINITY;
-  for (int s = lane; s < a.slots; s += 32) top = fmaxf(top, ml[s].x);
+#pragma unroll
+  for (int i = 0; i < kMaxSlots / 32; ++i) {
+    const int s = i * 32 + lane;
+    mine[i] = live && s < a.slots ? ml[s] : make_float2(-INFINITY, 0.0f);
+    top = fmaxf(top, mine[i].x);
+  }
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
   const float shift = top == -INFINITY ? 0.0f : top;
-  float sum = 0.0f, acc[kEach] = {};
-  const float* o = a.part_o + cell * a.slots * kDim + lane * kEach;
-#pragma unroll 4
-  for (int s = 0; s < a.slots; ++s) {
-    const float2 p = ml[s];
-    const float f = exp2_fast(p.x - shift);
-    sum = fmaf(p.y, f, sum);
-    if (p.x == -INFINITY) continue;  // a part without keys
+  float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) acc[i] = fmaf(o[s * kDim + i], f, acc[i]);
+  for (int i = 0; i < kMaxSlots / 32; ++i) {
+    const int s = i * 32 + lane;
+    const float f = exp2_fast(mine[i].x - shift);
+    sum = fmaf(mine[i].y, f, sum);
+    // A part without keys has no output: its factor is told apart from one that has underflowed.
+    if (along == 0 && s < a.slots) factors[local][s] = mine[i].x == -INFINITY ? -1.0f : f;
   }
+  sum = warp_sum(sum);
+  if (kWarps > 1)
+    __syncthreads();
+  else
+    __syncwarp();
+  float acc[kEach] = {};
+  const float* o = a.part_o + cell * a.slots * kDim + lane * kEach;
+  constexpr int kAhead = 8;
+  for (int s0 = along; live && s0 < a.slots; s0 += kAhead * kWarps) {
+    float v[kAhead][kEach];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int s = s0 + k * kWarps;
+      const bool has = s < a.slots && factors[local][s] >= 0.0f;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) v[k][i] = 0.0f;
+      if (has) {
+        if constexpr (kEach == 4) {
+          const float4 x = *reinterpret_cast<const float4*>(o + static_cast<int64_t>(s) * kDim);
+          v[k][0] = x.x, v[k][1] = x.y, v[k][2] = x.z, v[k][3] = x.w;
+        } else {
+          const float2 x = *reinterpret_cast<const float2*>(o + static_cast<int64_t>(s) * kDim);
+          v[k][0] = x.x, v[k][1] = x.y;
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int s = s0 + k * kWarps;
+      const float f = s < a.slots ? fmaxf(factors[local][s], 0.0f) : 0.0f;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) acc[i] = fmaf(v[k][i], f, acc[i]);
+    }
+  }
+  if (kWarps > 1) {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) sums[local][along][lane * kEach + i] = acc[i];
+    __syncthreads();
+    if (along != 0) return;
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w)
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) acc[i] += sums[local][w][lane * kEach + i];
+  }
+  if (!live) return;
+  // A NaN sum (of NaN scores) stays one.
   const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
   __nv_bfloat16* out = a.out + row * a.ldo + head * kDim + lane * kEach;
-#pragma unroll
-  for (int i = 0; i < kEach; i += 2) *reinterpret_cast<uint32_t*>(out + i) = pack2(acc[i] * inv, acc[i + 1] * inv);
+  if constexpr (kEach == 4)
+    *reinterpret_cast<uint2*>(out) = make_uint2(pack2(acc[0] * inv, acc[1] * inv), pack2(acc[2] * inv, acc[3] * inv));
+  else
+    *reinterpret_cast<uint32_t*>(out) = pack2(acc[0] * inv, acc[1] * inv);
   if (a.lse != nullptr && lane == 0)
     a.lse[cell] = sum != 0.0f ? (top + log2f(sum)) * 0.69314718055994530942f : -INFINITY;
 }
@@ -440,11 +510,13 @@ __global__ void __launch_bounds__(kThreads) attention_join_kernel(Attention a) {
 // The parts that the prefixes and the own keys are cut into, and the kernels.
 struct Plan {
   bool tc;  // the prefixes by the tensor-core kernel
-  int prefix_slots, own_slots, warp_rows;
+  int prefix_slots, own_slots;
+  int prefix_warps, own_warps;  // warps side by side along the rows of a tile
   int64_t prefix_tiles, own_tiles;  // of the kernel for few rows
 };
 
-constexpr int kMaxPrefixSlots = 64, kMaxOwnSlots = 16, kMaxTcSlots = 128;
+constexpr int kMaxPrefixSlots = 64, kMaxOwnSlots = 32, kMaxTcSlots = 128;
+static_assert(kMaxPrefixSlots + kMaxOwnSlots <= kMaxSlots && kMaxTcSlots + kMaxOwnSlots <= kMaxSlots, "");
 constexpr int kSms = 148;  // blocks of the tensor-core kernel, one an SM; correct on any number of SMs
 
 // A prefix with many rows is arithmetic, for the tensor cores.
@@ -461,27 +533,25 @@ Plan plan_of(const uocr_prefix_attention_args& a) {
   Plan p{};
   p.tc = many_rows(a);
   const int64_t group = a.heads / a.kv_heads;
-  // Rows of a tile by the rows of a prefix; of a sequence where the prefixes are apart.
-  const int64_t sets = p.tc || a.prefix_capacity == 0 ? a.sequences : a.prefixes;
-  const int64_t rows = a.rows * group / std::max<int64_t>(sets, 1);
-  p.warp_rows = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  const int64_t tile = 16 * p.warp_rows;
-  auto tiles = [&](int64_t count, int64_t each) {
+  // Rows of a tile by those of a prefix, of a sequence.
+  auto warps_for = [](int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; };
+  p.prefix_warps = warps_for(a.rows * group / a.prefixes);
+  p.own_warps = warps_for(a.rows * group / std::max<int64_t>(a.sequences, 1));
+  auto tiles = [&](int64_t count, int64_t each, int warps) {
+    const int64_t tile = 16 * warps;
     // With row offsets: each sequence's (prefix's) last tile may be part empty.
     return a.row_offsets == nullptr ? count * ((each * group + tile - 1) / tile)
                                     : a.rows * group / tile + std::min(count, a.rows);
   };
-  p.prefix_tiles = a.prefix_capacity > 0 && !p.tc ? tiles(a.prefixes, a.sequences / a.prefixes) : 0;
-  p.own_tiles = a.capacity > 0 ? tiles(a.sequences, 1) : 0;
+  p.prefix_tiles = a.prefix_capacity > 0 && !p.tc ? tiles(a.prefixes, a.sequences / a.prefixes, p.prefix_warps) : 0;
+  p.own_tiles = a.capacity > 0 ? tiles(a.sequences, 1, p.own_warps) : 0;
   const int64_t bp = p.prefix_tiles * a.kv_heads, bo = p.own_tiles * a.kv_heads;
-  // Parts of about `keys` keys: as many as fill the SMs twice where there are few tiles, whole ranges where there are
-  // many.
-  for (int64_t keys = 2 * kKeys;; keys *= 2) {
-    p.prefix_slots = static_cast<int>(std::min<int64_t>((a.prefix_capacity + keys - 1) / keys, kMaxPrefixSlots));
-    p.own_slots = static_cast<int>(std::min<int64_t>((a.capacity + keys - 1) / keys, kMaxOwnSlots));
-    if (bp * p.prefix_slots + bo * p.own_slots <= 2 * kSms) break;
-    if (keys >= a.prefix_capacity && keys >= a.capacity) break;
-  }
+  // Parts of `keys` keys: about four for each of the two blocks of an SM, so that the last ones to run are short beside
+  // the whole, but not so few keys that a part's way out costs what its keys do.
+  const int64_t work = bp * a.prefix_capacity + bo * a.capacity;
+  const int64_t keys = std::max<int64_t>((work / (4 * 2 * kSms) + kKeys - 1) / kKeys, 2) * kKeys;
+  p.prefix_slots = static_cast<int>(std::min<int64_t>((a.prefix_capacity + keys - 1) / keys, kMaxPrefixSlots));
+  p.own_slots = static_cast<int>(std::min<int64_t>((a.capacity + keys - 1) / keys, kMaxOwnSlots));
   // A range of keys meets about as many blocks as there are for each range.
   if (p.tc) {
     const int64_t ranges = a.kv_heads * ((a.rows * group + kAttentionTcRows - 1) / kAttentionTcRows);
@@ -501,28 +571,37 @@ cudaError_t launch_rows(const Attention& a, const Grid& g, unsigned blocks, cuda
 }
 
 template <int kDim>
+cudaError_t launch_rows(int warps, const Attention& a, const Grid& g, int64_t blocks, cudaStream_t stream) {
+  const unsigned n = static_cast<unsigned>(blocks);
+  return warps == 1   ? launch_rows<kDim, 1>(a, g, n, stream)
+         : warps == 2 ? launch_rows<kDim, 2>(a, g, n, stream)
+                      : launch_rows<kDim, 4>(a, g, n, stream);
+}
+
+template <int kDim>
 cudaError_t launch(const uocr_prefix_attention_args& args, const Attention& a, const Plan& p, cudaStream_t stream) {
   Grid g{};
-  g.prefix_tiles = static_cast<int>(p.prefix_tiles);
-  g.own_tiles = static_cast<int>(p.own_tiles);
-  g.prefix_blocks = p.tc ? 0 : static_cast<int>(p.prefix_tiles * a.kv_heads * p.prefix_slots);
+  g.prefix_blocks = static_cast<int>(p.prefix_tiles * a.kv_heads * p.prefix_slots);
   g.own_slots = p.own_slots;
-  const int64_t blocks = g.prefix_blocks + p.own_tiles * a.kv_heads * p.own_slots;
+  const int64_t own_blocks = p.own_tiles * a.kv_heads * p.own_slots;
+  const bool together = !p.tc && p.prefix_warps == p.own_warps;
   cudaError_t st = cudaSuccess;
-  if (p.tc) {
-    if ((st = launch_attention_tc(a, kDim, kSms, stream)) != cudaSuccess) return st;
-    g.late_wait = 1;
-  }
-  if (blocks > 0) {
-    const unsigned n = static_cast<unsigned>(blocks);
-    st = p.warp_rows == 1   ? launch_rows<kDim, 1>(a, g, n, stream)
-         : p.warp_rows == 2 ? launch_rows<kDim, 2>(a, g, n, stream)
-                            : launch_rows<kDim, 4>(a, g, n, stream);
+  if (p.tc)
+    st = launch_attention_tc(a, kDim, kSms, stream);
+  else if (g.prefix_blocks > 0 || (together && own_blocks > 0))
+    st = launch_rows<kDim>(p.prefix_warps, a, g, g.prefix_blocks + (together ? own_blocks : 0), stream);
+  if (st == cudaSuccess && !together && own_blocks > 0) {
+    g.late_wait = p.tc || g.prefix_blocks > 0;
+    g.prefix_blocks = 0;
+    st = launch_rows<kDim>(p.own_warps, a, g, own_blocks, stream);
   }
   if (st != cudaSuccess) return st;
+  // Few rows: all warps of a block on one, for the round trips of its parts.
   const int64_t cells = args.rows * args.heads, each = kThreads / 32;
-  return launch_pdl(attention_join_kernel<kDim>, static_cast<unsigned>((cells + each - 1) / each), kThreads, 0, stream,
-                    a);
+  if (cells <= 4 * kSms)
+    return launch_pdl(attention_join_kernel<kDim, 4>, static_cast<unsigned>(cells), kThreads, 0, stream, a);
+  return launch_pdl(attention_join_kernel<kDim, 1>, static_cast<unsigned>((cells + each - 1) / each), kThreads, 0,
+                    stream, a);
 }
 
 }  // namespace
