@@ -16,6 +16,8 @@ namespace uocr_b200 {
 
 cudaError_t launch_rotate_heads(const uocr_rotate_heads_args& a, ErrorWord* err, cudaStream_t stream);
 
+// Whether the call's units of work are few enough to be counted.
+bool prefix_attention_counts(const uocr_prefix_attention_args& a);
 size_t prefix_attention_bytes(const uocr_prefix_attention_args& a);
 cudaError_t launch_prefix_attention(const uocr_prefix_attention_args& a, ErrorWord* err, cudaStream_t stream);
 

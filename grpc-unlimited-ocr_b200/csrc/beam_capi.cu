@@ -55,6 +55,7 @@ int check_attention_sizes(const char* op, const uocr_prefix_attention_args* a) {
     return bad(op, "without row_offsets there is one row per sequence");
   if (a->rows * a->heads > kMaxCount) return unsupported(op, "rows * heads above 2^30");
   if (a->reserved != 0) return bad(op, "reserved must be 0");
+  if (!prefix_attention_counts(*a)) return unsupported(op, "rows * heads * keys too large");
   return UOCR_OK;
 }
 

@@ -6,8 +6,8 @@
 // join of softmaxes over parts of it: from (m_i, l_i, o_i), the parts' maxima,
 // sums of exp(s - m_i) and unnormalised outputs,
 //   m = max m_i,  l = sum l_i exp(m_i - m),  o = sum o_i exp(m_i - m) / l.
-// So prefixes and own keys are cut into parts that fill the card, each block
-// takes one part of one tile of rows, and a second kernel joins a row's parts.
+// So prefixes and own keys are cut into as many shares as the card holds blocks,
+// and a second kernel joins a row's parts.
 #include <algorithm>
 
 #include "prefix_attention.cuh"
@@ -50,123 +50,85 @@ __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
 }
 
-// What a block works on: rows x heads of one key/value head (vr = row * group +
-// head, `count` of them from `start`), and a range of keys.
-struct Tile {
-  int first_row;  // of the rows below
-  int start, count;
+// A run of a block's units within one range of keys: rows x heads of one
+// key/value head (vr = row * group + head, `count` of them from `start`).
+struct Segment {
+  int first_row, start, count;
   int kv_head;
-  int key0, key1;     // the block's part
-  int limit0;         // keys the row at first_row sees; each row after it sees one more (own keys), or the same
-  int all_see;        // keys that every row of the tile sees
+  int of;                // the prefix or sequence
   bool own;
-  int sequence, slot;
-  const __nv_bfloat16* k;  // of key 0 (with ancestry: in cache 0)
-  const __nv_bfloat16* v;
+  int key0, key1;        // the block's part
+  int limit0;            // keys the row at first_row sees; each row after it sees one more (own keys), or the same
+  int all_see;           // keys that every row of the tile sees
+  int slot, used, slots;  // of the join: this one, how many the range's blocks use, how many there are
+  bool first;            // the range's first block
+  int stages;            // of the block's share
 };
 
-// Blocks [0, prefix_blocks) take prefixes, the others own keys. Tiles are
-// counted through over the prefixes (sequences): ceil(rows * group / kRows) of
-// each, then the key/value heads, then the parts.
+// The work is counted through in units of a tile of rows and a stage of keys,
+// over the prefixes (where this kernel has them), then the sequences' own keys,
+// and every block takes the same number of units, whatever the lengths.
 struct Grid {
-  int prefix_blocks;
-  int own_slots;
+  int prefixes, sequences;  // that this launch has to do with
   // 1: launched behind a kernel of the same call, which this one takes nothing from. That kernel lets this one start
   // when it has itself waited for all work before the call, so the wait for it can come last.
   int late_wait;
 };
 
-// Finds the sequence (prefix) that tile `t` is of; -1 behind the last one.
-template <int kRows, typename RowsOf>
-__device__ int find_tile(int t, int count, const Attention& a, RowsOf rows, int* local, int* first, int* n) {
-  const int lane = threadIdx.x & 31;
-  for (int b0 = 0; b0 < count; b0 += 32) {
-    int r0 = 0;
-    const int mine = b0 + lane < count ? rows(b0 + lane, &r0) : 0;
-    const int tiles = (mine * a.group + kRows - 1) / kRows;
-    int end = tiles;
+// A prefix or a sequence (index e, the prefixes first): its rows and keys.
+struct Source {
+  int rows, first_row, keys;
+  int tiles, stages;
+};
+
+template <int kPrefixRows, int kOwnRows>
+__device__ __forceinline__ unsigned source_units(const Attention& a, const Grid& g, int e, Source* s) {
+  if (e >= g.prefixes + g.sequences) return 0;
+  const bool own = e >= g.prefixes;
+  s->rows = own ? rows_of(a, e - g.prefixes, &s->first_row) : prefix_rows_of(a, e, &s->first_row);
+  s->keys = own ? len_of(a, e - g.prefixes) : prefix_len_of(a, e);
+  const int of_tile = own ? kOwnRows : kPrefixRows;
+  s->tiles = (s->rows * a.group + of_tile - 1) / of_tile;
+  s->stages = max(1, (s->keys + kKeys - 1) / kKeys);  // without keys there still is a part: none
+  return static_cast<unsigned>(a.kv_heads) * s->tiles * s->stages;
+}
+
+// Inclusive sums over the block's threads; *total over all. `part`: a sum a warp.
+__device__ __forceinline__ unsigned block_scan(unsigned v, unsigned* part, unsigned* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
-    for (int off = 1; off < 32; off *= 2) {
-      const int other = __shfl_up_sync(0xffffffffu, end, off);
-      if (lane >= off) end += other;
-    }
-    const unsigned hit = __ballot_sync(0xffffffffu, t < end);
-    if (hit != 0) {
-      const int src = __ffs(hit) - 1;
-      *local = t - __shfl_sync(0xffffffffu, end - tiles, src);
-      *first = __shfl_sync(0xffffffffu, r0, src);
-      *n = __shfl_sync(0xffffffffu, mine, src);
-      return b0 + src;
-    }
-    t -= __shfl_sync(0xffffffffu, end, 31);
+  for (int off = 1; off < 32; off *= 2) {
+    const unsigned other = __shfl_up_sync(0xffffffffu, v, off);
+    if (lane >= off) v += other;
   }
-  return -1;
+  if (lane == 31) part[warp] = v;
+  __syncthreads();
+  *total = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) v += part[w];
+    *total += part[w];
+  }
+  return v;
 }
 
-template <int kDim, int kRows>
-__device__ bool find_work(const Attention& a, const Grid& g, Tile* w) {
-  const int block = blockIdx.x;
-  w->own = block >= g.prefix_blocks;
-  int b = w->own ? block - g.prefix_blocks : block;
-  const int parts = w->own ? g.own_slots : a.prefix_slots;
-  const int part = b % parts;
-  b /= parts;
-  w->kv_head = b % a.kv_heads;
-  const int tile = b / a.kv_heads;
-  int local, n, of;
-  if (w->own)
-    of = find_tile<kRows>(tile, a.sequences, a, [&](int i, int* r0) { return rows_of(a, i, r0); }, &local,
-                          &w->first_row, &n);
-  else
-    of = find_tile<kRows>(tile, a.prefixes, a, [&](int i, int* r0) { return prefix_rows_of(a, i, r0); }, &local,
-                          &w->first_row, &n);
-  if (of < 0) return false;
-  w->start = local * kRows;
-  w->count = min(kRows, n * a.group - w->start);
-  w->sequence = of;
-  w->slot = w->own ? a.prefix_slots + part : part;
-  int keys;
-  if (w->own) {
-    const int len = len_of(a, of);
-    w->limit0 = len - n + 1;
-    // the tile's last row sees the most
-    keys = max(0, w->limit0 + (w->start + w->count - 1) / a.group);
-    w->all_see = w->limit0 + w->start / a.group;
-    const int64_t base = (a.ancestry != nullptr ? 0 : of * a.cache_stride) + w->kv_head * a.head_stride;
-    w->k = a.k + base;
-    w->v = a.v + base;
-  } else {
-    keys = w->limit0 = w->all_see = prefix_len_of(a, of);
-    w->k = a.prefix_k + of * a.prefix_stride + w->kv_head * a.prefix_head_stride;
-    w->v = a.prefix_v + of * a.prefix_stride + w->kv_head * a.prefix_head_stride;
-  }
-  const int stages = (keys + kKeys - 1) / kKeys, each = (stages + parts - 1) / parts;
-  w->key0 = min(keys, part * each * kKeys);
-  w->key1 = min(keys, w->key0 + each * kKeys);
-  return true;
-}
-
-// 4 warps: kWarpRows of them side by side along the rows (16 each), the others
-// along a stage's keys, each with its own running maximum, sum and output in
-// registers; keys and values in a ring of padded stages filled by cp.async.
-// mma.sync and not tcgen05: a tile has 16 to 64 rows, of which a tcgen05 tile
-// would use an eighth to a half.
+// A segment. 4 warps: kWarpRows of them side by side along the rows (16 each),
+// the others along a stage's keys, each with its own running maximum, sum and
+// output in registers; keys and values in a ring of padded stages filled by
+// cp.async. mma.sync and not tcgen05: a tile has 16 to 64 rows, of which a tcgen05
+// tile would use an eighth to a half.
 template <int kDim, int kWarpRows>
-__global__ void __launch_bounds__(kThreads) attention_rows_kernel(Attention a, Grid g) {
+__device__ __forceinline__ void attend(const Attention& a, const Segment& seg, unsigned char* raw, uint32_t* odd_keys) {
+  const Segment w = seg;  // in registers
   constexpr int kRows = 16 * kWarpRows, kWarpKeys = kKeys / (4 / kWarpRows);
   constexpr int kPitch = kDim + 8;  // padded: fragment loads without bank conflicts
   constexpr int kStage = 2 * kKeys * kPitch;
-  extern __shared__ __align__(16) unsigned char raw[];
   __nv_bfloat16* ring = reinterpret_cast<__nv_bfloat16*>(raw);
-  if (!g.late_wait) {
-    pdl_wait();
-    pdl_launch_dependents();
-  }
-  Tile w;
-  if (!find_work<kDim, kRows>(a, g, &w)) {
-    if (g.late_wait) pdl_wait();
-    return;
-  }
+  // key 0 (with ancestry: in cache 0)
+  const int64_t base = w.own ? (a.ancestry != nullptr ? 0 : w.of * a.cache_stride) + w.kv_head * a.head_stride
+                             : w.of * a.prefix_stride + w.kv_head * a.prefix_head_stride;
+  const __nv_bfloat16* keys = (w.own ? a.k : a.prefix_k) + base;
+  const __nv_bfloat16* values = (w.own ? a.v : a.prefix_v) + base;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gr = lane >> 2, tq = lane & 3;
   const int row0 = warp % kWarpRows * 16, warp_key = warp / kWarpRows * kWarpKeys;
@@ -182,7 +144,7 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(Attention a, G
 #pragma unroll
     for (int i = 0; i < kCopies; ++i) {
       const int at = key + copy_key + i * kStep;
-      from[i] = at < w.key1 ? a.ancestry[w.sequence * a.ld_ancestry + at] : 0;
+      from[i] = at < w.key1 ? a.ancestry[w.of * a.ld_ancestry + at] : 0;
     }
   };
   auto fill = [&](int stage, int key) {
@@ -196,13 +158,13 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(Attention a, G
       if (gathers) {
         int cache = from[i];
         if (valid && (cache < 0 || cache >= a.caches)) {
-          raise_error(a.err, kDevBadIndex, kSiteAncestor, w.sequence, cache);
-          cache = w.sequence < a.caches ? w.sequence : 0;
+          raise_error(a.err, kDevBadIndex, kSiteAncestor, w.of, cache);
+          cache = w.of < a.caches ? w.of : 0;
         }
         off += cache * a.cache_stride;
       }
-      cp_async16_or_zero(ks + i * kStep * kPitch, w.k + off, valid);
-      cp_async16_or_zero(vs + i * kStep * kPitch, w.v + off, valid);
+      cp_async16_or_zero(ks + i * kStep * kPitch, keys + off, valid);
+      cp_async16_or_zero(vs + i * kStep * kPitch, values + off, valid);
     }
   };
   look_up(w.key0);
@@ -236,7 +198,6 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(Attention a, G
 #pragma unroll
   for (int d = 0; d < kDim / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.0f;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-  __shared__ uint32_t odd_keys[kKeys / 32];  // keys of the stage with a value that is no finite number
 
   int stage = 0;
   for (int key = w.key0; key < w.key1; key += kKeys) {
@@ -290,12 +251,14 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(Attention a, G
         s[nt][e] = exp2_fast(s[nt][e] - shift[e >> 1]);
         l[e >> 1] += s[nt][e];
       }
+    if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {  // the maxima soon stay
 #pragma unroll
-    for (int d = 0; d < kDim / 8; ++d) {
-      o[d][0] *= alpha[0];
-      o[d][1] *= alpha[0];
-      o[d][2] *= alpha[1];
-      o[d][3] *= alpha[1];
+      for (int d = 0; d < kDim / 8; ++d) {
+        o[d][0] *= alpha[0];
+        o[d][1] *= alpha[0];
+        o[d][2] *= alpha[1];
+        o[d][3] *= alpha[1];
+      }
     }
     // A key that only some of the tile's rows see has the weight 0 in the others, which an infinite or NaN value
     // would turn into a NaN: such values are added apart, where they are seen, and are 0 in the products.
@@ -313,22 +276,18 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(Attention a, G
         }
       }
       if (__syncthreads_or(odd)) {
+        // p * v of an infinite or NaN v is v, whatever p > 0.
+#pragma unroll 1
+        for (int r = warp_key; r < warp_key + kWarpKeys; ++r) {
+          if ((odd_keys[r / 32] >> (r & 31) & 1) == 0) continue;
 #pragma unroll
-        for (int nt = 0; nt < kWarpKeys / 8; ++nt)
+          for (int d = 0; d < kDim / 8; ++d)
 #pragma unroll
-          for (int col = 0; col < 8; ++col) {
-            const int r = warp_key + nt * 8 + col;
-            if ((odd_keys[r / 32] >> (r & 31) & 1) == 0) continue;
-            const float p[2] = {__shfl_sync(0xffffffffu, s[nt][col & 1], gr * 4 + col / 2),
-                                __shfl_sync(0xffffffffu, s[nt][2 + (col & 1)], gr * 4 + col / 2)};
-#pragma unroll
-            for (int d = 0; d < kDim / 8; ++d)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float v = __bfloat162float(whole[r * kPitch + d * 8 + 2 * tq + (e & 1)]);
-                if (!isfinite(v) && key + r < limit[e >> 1]) o[d][e] = fmaf(p[e >> 1], v, o[d][e]);
-              }
-          }
+            for (int e = 0; e < 4; ++e) {
+              const float v = __bfloat162float(whole[r * kPitch + d * 8 + 2 * tq + (e & 1)]);
+              if (!isfinite(v) && key + r < limit[e >> 1]) o[d][e] += v;
+            }
+        }
         __syncthreads();
         for (int c = threadIdx.x; c < kKeys * kDim; c += kThreads) {
           __nv_bfloat16* v = whole + c / kDim * kPitch + c % kDim;
@@ -359,14 +318,21 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(Attention a, G
   auto cell = [&](int r) {  // of the tile's row r
     const int vr = w.start + r;
     const int64_t row = w.first_row + vr / a.group;
-    return (row * a.heads + w.kv_head * a.group + vr % a.group) * a.slots + w.slot;
+    return (row * a.heads + w.kv_head * a.group + vr % a.group) * a.slots;
   };
+  if (w.first)  // the slots that no block comes to
+    for (int c = threadIdx.x; c < w.count * (w.slots - w.used); c += kThreads)
+      a.part_ml[cell(c % w.count) + w.used + c / w.count] = make_float2(-INFINITY, 0.0f);
+  if (w.key0 >= w.key1) {
+    for (int r = threadIdx.x; r < w.count; r += kThreads) a.part_ml[cell(r) + w.slot] = make_float2(-INFINITY, 0.0f);
+    return;
+  }
   if constexpr (kWarpRows == 4) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int r = row0 + gr + 8 * i;
       if (r >= w.count) continue;
-      const int64_t at = cell(r);
+      const int64_t at = cell(r) + w.slot;
       if (tq == 0) a.part_ml[at] = make_float2(m[i], l[i]);
 #pragma unroll
       for (int d = 0; d < kDim / 8; ++d)
@@ -407,10 +373,101 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(Attention a, G
         acc.x = fmaf(v.x, f, acc.x), acc.y = fmaf(v.y, f, acc.y);
         acc.z = fmaf(v.z, f, acc.z), acc.w = fmaf(v.w, f, acc.w);
       }
-      const int64_t at = cell(r);
+      const int64_t at = cell(r) + w.slot;
       if (col == 0) a.part_ml[at] = make_float2(top, sum);
       *reinterpret_cast<float4*>(a.part_o + at * kDim + col) = acc;
     }
+  }
+}
+
+template <int kDim, int kPrefixWarps, int kOwnWarps>
+__global__ void __launch_bounds__(kThreads) attention_rows_kernel(Attention a, Grid g) {
+  constexpr int kPrefixRows = 16 * kPrefixWarps, kOwnRows = 16 * kOwnWarps;
+  extern __shared__ __align__(16) unsigned char raw[];
+  __shared__ uint32_t odd_keys[kKeys / 32];  // keys of the stage with a value that is no finite number
+  __shared__ Segment seg;
+  __shared__ unsigned part[2][kThreads / 32];
+  __shared__ int most[2];  // stages of the longest prefix and sequence
+  if (threadIdx.x < 2) most[threadIdx.x] = 1;
+  if (!g.late_wait) {
+    pdl_wait();
+    pdl_launch_dependents();
+  }
+  __syncthreads();
+  const int sources = g.prefixes + g.sequences;
+  Source mine{};  // of this thread in the first round, which for few sources is the only one
+  const unsigned my_units = source_units<kPrefixRows, kOwnRows>(a, g, threadIdx.x, &mine);
+  if (mine.tiles > 0) atomicMax(&most[static_cast<int>(threadIdx.x) >= g.prefixes], mine.stages);
+  unsigned rest = 0;
+  for (int e = kThreads + threadIdx.x; e < sources; e += kThreads) {
+    Source s{};
+    rest += source_units<kPrefixRows, kOwnRows>(a, g, e, &s);
+    if (s.tiles > 0) atomicMax(&most[e >= g.prefixes], s.stages);
+  }
+  unsigned first_round, total;
+  const unsigned my_upto = block_scan(my_units, part[0], &first_round);
+  total = first_round;
+  if (sources > kThreads) {
+    unsigned others;
+    block_scan(rest, part[1], &others);
+    total += others;
+  }
+  // No range of keys meets more blocks than there are slots for it.
+  const int own_slots = a.slots - a.prefix_slots;
+  unsigned share = max((total + gridDim.x - 1) / gridDim.x, 1u);
+  if (g.prefixes > 0) share = max(share, (most[0] + a.prefix_slots - 2u) / (a.prefix_slots - 1u));
+  if (g.sequences > 0) share = max(share, (most[1] + own_slots - 2u) / (own_slots - 1u));
+  unsigned unit = blockIdx.x * share;
+  const unsigned end = min(total, unit + share);
+  while (unit < end) {
+    unsigned before = 0;
+    for (int e0 = 0; e0 < sources; e0 += kThreads) {
+      const int e = e0 + threadIdx.x;
+      Source s = mine;
+      unsigned n = my_units, upto = my_upto, in_round = first_round;
+      if (e0 > 0) {
+        __syncthreads();  // the sums of the round before have been read
+        n = source_units<kPrefixRows, kOwnRows>(a, g, e, &s);
+        upto = before + block_scan(n, part[1], &in_round);
+      }
+      if (unit < upto && unit >= upto - n) {
+        const unsigned local = unit - (upto - n), range = local / s.stages, stage0 = local - range * s.stages;
+        const unsigned first = unit - stage0, head = range / s.tiles;  // first: the range's first unit
+        const int tile = static_cast<int>(range - head * s.tiles);
+        const int of_tile = e >= g.prefixes ? kOwnRows : kPrefixRows;
+        seg.own = e >= g.prefixes;
+        seg.of = seg.own ? e - g.prefixes : e;
+        seg.kv_head = static_cast<int>(head);
+        seg.first_row = s.first_row;
+        seg.start = tile * of_tile;
+        seg.count = min(of_tile, s.rows * a.group - seg.start);
+        seg.stages = static_cast<int>(min(s.stages - stage0, end - unit));
+        int keys = s.keys;
+        seg.limit0 = seg.all_see = s.keys;
+        if (seg.own) {
+          seg.limit0 = s.keys - s.rows + 1;
+          seg.all_see = seg.limit0 + seg.start / a.group;
+          keys = max(0, seg.limit0 + (seg.start + seg.count - 1) / a.group);  // the tile's last row sees the most
+        }
+        seg.key0 = min(keys, static_cast<int>(stage0) * kKeys);
+        seg.key1 = min(keys, (static_cast<int>(stage0) + seg.stages) * kKeys);
+        seg.first = stage0 == 0;
+        const unsigned block0 = first / share;
+        const int slot0 = seg.own ? a.prefix_slots : 0;
+        seg.slot = static_cast<int>(blockIdx.x - block0) + slot0;
+        seg.used = static_cast<int>((first + s.stages - 1) / share - block0) + 1 + slot0;
+        seg.slots = seg.own ? a.slots : a.prefix_slots;
+      }
+      before += in_round;
+      if (unit < before) break;
+    }
+    __syncthreads();  // the segment is known
+    unit += seg.stages;
+    if (kPrefixWarps == kOwnWarps || seg.own)
+      attend<kDim, kOwnWarps>(a, seg, raw, odd_keys);
+    else
+      attend<kDim, kPrefixWarps>(a, seg, raw, odd_keys);
+    __syncthreads();  // the segment and the ring have been read
   }
   if (g.late_wait) pdl_wait();
 }
@@ -511,8 +568,9 @@ __global__ void __launch_bounds__(kThreads) attention_join_kernel(Attention a) {
 struct Plan {
   bool tc;  // the prefixes by the tensor-core kernel
   int prefix_slots, own_slots;
-  int prefix_warps, own_warps;  // warps side by side along the rows of a tile
-  int64_t prefix_tiles, own_tiles;  // of the kernel for few rows
+  int prefix_warps, own_warps;  // of the kernel for few rows: warps side by side along the rows of a tile
+  int64_t units;  // that there can be
+  unsigned blocks;
 };
 
 constexpr int kMaxPrefixSlots = 64, kMaxOwnSlots = 32, kMaxTcSlots = 128;
@@ -537,22 +595,26 @@ Plan plan_of(const uocr_prefix_attention_args& a) {
   auto warps_for = [](int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; };
   p.prefix_warps = warps_for(a.rows * group / a.prefixes);
   p.own_warps = warps_for(a.rows * group / std::max<int64_t>(a.sequences, 1));
+  if (p.tc || a.prefix_capacity == 0) p.prefix_warps = p.own_warps;
+  // The units there can be, by the capacities; with row offsets each sequence's (prefix's) last tile may be part empty.
   auto tiles = [&](int64_t count, int64_t each, int warps) {
     const int64_t tile = 16 * warps;
-    // With row offsets: each sequence's (prefix's) last tile may be part empty.
     return a.row_offsets == nullptr ? count * ((each * group + tile - 1) / tile)
                                     : a.rows * group / tile + std::min(count, a.rows);
   };
-  p.prefix_tiles = a.prefix_capacity > 0 && !p.tc ? tiles(a.prefixes, a.sequences / a.prefixes, p.prefix_warps) : 0;
-  p.own_tiles = a.capacity > 0 ? tiles(a.sequences, 1, p.own_warps) : 0;
-  const int64_t bp = p.prefix_tiles * a.kv_heads, bo = p.own_tiles * a.kv_heads;
-  // Parts of `keys` keys: about four for each of the two blocks of an SM, so that the last ones to run are short beside
-  // the whole, but not so few keys that a part's way out costs what its keys do.
-  const int64_t work = bp * a.prefix_capacity + bo * a.capacity;
-  const int64_t keys = std::max<int64_t>((work / (4 * 2 * kSms) + kKeys - 1) / kKeys, 2) * kKeys;
-  p.prefix_slots = static_cast<int>(std::min<int64_t>((a.prefix_capacity + keys - 1) / keys, kMaxPrefixSlots));
-  p.own_slots = static_cast<int>(std::min<int64_t>((a.capacity + keys - 1) / keys, kMaxOwnSlots));
-  // A range of keys meets about as many blocks as there are for each range.
+  const int64_t prefix_stages = (a.prefix_capacity + kKeys - 1) / kKeys, own_stages = (a.capacity + kKeys - 1) / kKeys;
+  const int64_t units =
+      a.kv_heads * ((p.tc ? 0 : tiles(a.prefixes, a.sequences / a.prefixes, p.prefix_warps) * prefix_stages) +
+                    tiles(a.sequences, 1, p.own_warps) * own_stages);
+  p.units = units;
+  p.blocks = static_cast<unsigned>(std::min<int64_t>(units, 2 * kSms));
+  // A range of keys meets as many blocks as shares fit into it, and one more; half as many again for lengths that differ.
+  const int64_t share = std::max<int64_t>((units + 2 * kSms - 1) / (2 * kSms), 1);
+  auto slots = [&](int64_t stages, int most) {
+    return static_cast<int>(stages == 0 ? 0 : std::min<int64_t>((stages + share - 1) / share * 3 / 2 + 2, most));
+  };
+  p.prefix_slots = slots(prefix_stages, kMaxPrefixSlots);
+  p.own_slots = slots(own_stages, kMaxOwnSlots);
   if (p.tc) {
     const int64_t ranges = a.kv_heads * ((a.rows * group + kAttentionTcRows - 1) / kAttentionTcRows);
     p.prefix_slots = static_cast<int>(std::min<int64_t>(kSms / ranges + 3, kMaxTcSlots));
@@ -560,40 +622,33 @@ Plan plan_of(const uocr_prefix_attention_args& a) {
   return p;
 }
 
-template <int kDim, int kWarpRows>
+template <int kDim, int kPrefixWarps, int kOwnWarps>
 cudaError_t launch_rows(const Attention& a, const Grid& g, unsigned blocks, cudaStream_t stream) {
   constexpr size_t kRing = static_cast<size_t>(kStages) * 2 * kKeys * (kDim + 8) * 2;
-  constexpr size_t kJoin = static_cast<size_t>(4 / kWarpRows) * 16 * kWarpRows * (kDim * 4 + 8);
+  // 4 / w warps along the keys, 16 w rows
+  constexpr size_t kJoin = static_cast<size_t>(64) * (kDim * 4 + 8);
   static_assert(kJoin <= kRing, "the join takes the ring's place");
-  cudaError_t st = allow_max_dynamic_smem(attention_rows_kernel<kDim, kWarpRows>);
+  cudaError_t st = allow_max_dynamic_smem(attention_rows_kernel<kDim, kPrefixWarps, kOwnWarps>);
   if (st != cudaSuccess) return st;
-  return launch_pdl(attention_rows_kernel<kDim, kWarpRows>, blocks, kThreads, kRing, stream, a, g);
-}
-
-template <int kDim>
-cudaError_t launch_rows(int warps, const Attention& a, const Grid& g, int64_t blocks, cudaStream_t stream) {
-  const unsigned n = static_cast<unsigned>(blocks);
-  return warps == 1   ? launch_rows<kDim, 1>(a, g, n, stream)
-         : warps == 2 ? launch_rows<kDim, 2>(a, g, n, stream)
-                      : launch_rows<kDim, 4>(a, g, n, stream);
+  return launch_pdl(attention_rows_kernel<kDim, kPrefixWarps, kOwnWarps>, blocks, kThreads, kRing, stream, a, g);
 }
 
 template <int kDim>
 cudaError_t launch(const uocr_prefix_attention_args& args, const Attention& a, const Plan& p, cudaStream_t stream) {
   Grid g{};
-  g.prefix_blocks = static_cast<int>(p.prefix_tiles * a.kv_heads * p.prefix_slots);
-  g.own_slots = p.own_slots;
-  const int64_t own_blocks = p.own_tiles * a.kv_heads * p.own_slots;
-  const bool together = !p.tc && p.prefix_warps == p.own_warps;
-  cudaError_t st = cudaSuccess;
-  if (p.tc)
-    st = launch_attention_tc(a, kDim, kSms, stream);
-  else if (g.prefix_blocks > 0 || (together && own_blocks > 0))
-    st = launch_rows<kDim>(p.prefix_warps, a, g, g.prefix_blocks + (together ? own_blocks : 0), stream);
-  if (st == cudaSuccess && !together && own_blocks > 0) {
-    g.late_wait = p.tc || g.prefix_blocks > 0;
-    g.prefix_blocks = 0;
-    st = launch_rows<kDim>(p.own_warps, a, g, own_blocks, stream);
+  g.prefixes = p.tc || args.prefix_capacity == 0 ? 0 : a.prefixes;
+  g.sequences = args.capacity == 0 ? 0 : a.sequences;
+  g.late_wait = p.tc;
+  cudaError_t st = p.tc ? launch_attention_tc(a, kDim, kSms, stream) : cudaSuccess;
+  if (st == cudaSuccess && p.blocks > 0) {
+    switch (p.prefix_warps * 8 + p.own_warps) {
+      case 8 + 1: st = launch_rows<kDim, 1, 1>(a, g, p.blocks, stream); break;
+      case 16 + 1: st = launch_rows<kDim, 2, 1>(a, g, p.blocks, stream); break;
+      case 16 + 2: st = launch_rows<kDim, 2, 2>(a, g, p.blocks, stream); break;
+      case 32 + 1: st = launch_rows<kDim, 4, 1>(a, g, p.blocks, stream); break;
+      case 32 + 2: st = launch_rows<kDim, 4, 2>(a, g, p.blocks, stream); break;
+      default: st = launch_rows<kDim, 4, 4>(a, g, p.blocks, stream);
+    }
   }
   if (st != cudaSuccess) return st;
   // Few rows: all warps of a block on one, for the round trips of its parts.
@@ -605,6 +660,10 @@ cudaError_t launch(const uocr_prefix_attention_args& args, const Attention& a, c
 }
 
 }  // namespace
+
+bool prefix_attention_counts(const uocr_prefix_attention_args& a) {
+  return plan_of(a).units < (int64_t{1} << 31) - 2 * kSms;
+}
 
 size_t prefix_attention_bytes(const uocr_prefix_attention_args& a) {
   const Plan p = plan_of(a);
