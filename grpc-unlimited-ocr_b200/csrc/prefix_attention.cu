@@ -569,7 +569,6 @@ struct Plan {
   bool tc;  // the prefixes by the tensor-core kernel
   int prefix_slots, own_slots;
   int prefix_warps, own_warps;  // of the kernel for few rows: warps side by side along the rows of a tile
-  int64_t units;  // that there can be
   unsigned blocks;
 };
 
@@ -606,7 +605,6 @@ Plan plan_of(const uocr_prefix_attention_args& a) {
   const int64_t units =
       a.kv_heads * ((p.tc ? 0 : tiles(a.prefixes, a.sequences / a.prefixes, p.prefix_warps) * prefix_stages) +
                     tiles(a.sequences, 1, p.own_warps) * own_stages);
-  p.units = units;
   p.blocks = static_cast<unsigned>(std::min<int64_t>(units, 2 * kSms));
   // A range of keys meets as many blocks as shares fit into it, and one more; half as many again for lengths that differ.
   const int64_t share = std::max<int64_t>((units + 2 * kSms - 1) / (2 * kSms), 1);
@@ -662,7 +660,9 @@ cudaError_t launch(const uocr_prefix_attention_args& args, const Attention& a, c
 }  // namespace
 
 bool prefix_attention_counts(const uocr_prefix_attention_args& a) {
-  return plan_of(a).units < (int64_t{1} << 31) - 2 * kSms;
+  // Units in 32 bits, and a prefix's rows x heads; the tensor-core kernel's units are a quarter of those counted here.
+  const double stages = static_cast<double>((a.prefix_capacity + kKeys - 1) / kKeys + (a.capacity + kKeys - 1) / kKeys);
+  return (static_cast<double>(a.rows) * a.heads / 16 + a.kv_heads * static_cast<double>(a.sequences)) * stages < 2.0e9;
 }
 
 size_t prefix_attention_bytes(const uocr_prefix_attention_args& a) {

@@ -100,11 +100,32 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Two values in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, w;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+
 struct __align__(8) TcBarriers {
   uint64_t full[kSlots];
   uint64_t empty[kSlots];
   uint64_t s_full[2];  // a tile's scores are there, and all MMAs before them are done
-  uint64_t p_full[2];  // its weights are there
+  uint64_t p_half[2];  // the weights of its first 64 keys are there
+  uint64_t p_full[2];  // the others'
   uint64_t o_done;     // a segment's MMAs are done
   uint64_t drain;
 };
@@ -116,60 +137,101 @@ struct Segment {
   int tile0, tile1, tiles;      // of 128 keys: [tile0, tile1) of `tiles`
   int len;
   int slot, used;               // of the join; how many the range's rows use
-  int next;                     // 1: there is one
-};
+};                              // tile0 == tile1: there is none
 
 struct TcArgs {
   CUtensorMap k, v;
   Attention a;
 };
 
+// A prefix: its rows and keys.
+struct Prefix {
+  int rows, first_row, len;
+  int pairs, tiles;  // of 256 rows, of 128 keys
+};
 // The units of prefix p: (key/value heads) x (row tile pairs) x (key tiles).
-__device__ __forceinline__ int64_t units_of(const Attention& a, int p, int* rows, int* first, int* pairs, int* tiles,
-                                            int* len) {
-  *rows = prefix_rows_of(a, p, first);
-  *len = prefix_len_of(a, p);
-  *pairs = static_cast<int>((static_cast<int64_t>(*rows) * a.group + kTcRows - 1) / kTcRows);
-  *tiles = max(1, (*len + kTcKeys - 1) / kTcKeys);  // an empty prefix still has a part: no keys
-  return static_cast<int64_t>(a.kv_heads) * *pairs * *tiles;
+__device__ __forceinline__ unsigned units_of(const Attention& a, int p, Prefix* x) {
+  if (p >= a.prefixes) return 0;
+  x->rows = prefix_rows_of(a, p, &x->first_row);
+  x->len = prefix_len_of(a, p);
+  x->pairs = (x->rows * a.group + kTcRows - 1) / kTcRows;
+  x->tiles = max(1, (x->len + kTcKeys - 1) / kTcKeys);  // an empty prefix still has a part: no keys
+  return static_cast<unsigned>(a.kv_heads) * x->pairs * x->tiles;
+}
+__device__ __forceinline__ unsigned warp_scan(unsigned v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int off = 1; off < 32; off *= 2) {
+    const unsigned other = __shfl_up_sync(0xffffffffu, v, off);
+    if (lane >= off) v += other;
+  }
+  return v;
 }
 
-// By a whole warp: the segment at unit u (< end) of block `block`.
-__device__ void find_segment(const Attention& a, int64_t unit, int64_t end, int64_t share, int block, Segment* s) {
+// What the scheduling warp keeps: the first 32 prefixes, which mostly are all.
+struct Schedule {
+  Prefix mine;
+  unsigned units, upto;  // of this lane's prefix, inclusive sum
+  unsigned unit, end, share;
+};
+
+__device__ __forceinline__ Schedule make_schedule(const Attention& a) {
   const int lane = threadIdx.x & 31;
-  int64_t u = unit;  // counted from prefix p0 on
-  for (int p0 = 0; p0 < a.prefixes; p0 += 32) {
-    int rows = 0, first = 0, pairs = 0, tiles = 1, len = 0;
-    const int64_t mine = p0 + lane < a.prefixes ? units_of(a, p0 + lane, &rows, &first, &pairs, &tiles, &len) : 0;
-    int64_t upto = mine;
-#pragma unroll
-    for (int off = 1; off < 32; off *= 2) {
-      const int64_t other = __shfl_up_sync(0xffffffffu, upto, off);
-      if (lane >= off) upto += other;
-    }
-    const unsigned hit = __ballot_sync(0xffffffffu, u < upto);
-    if (hit != 0) {
-      if (lane == __ffs(hit) - 1) {
-        const int64_t local = u - (upto - mine), base = unit - local % tiles;  // base: the range's first unit
-        const int pair = static_cast<int>(local / tiles % pairs);
-        s->prefix = p0 + lane;
-        s->kv_head = static_cast<int>(local / tiles / pairs);
-        s->first_row = first;
-        s->start = pair * kTcRows;
-        s->count = static_cast<int>(min(static_cast<int64_t>(kTcRows), static_cast<int64_t>(rows) * a.group - s->start));
-        s->tiles = tiles;
-        s->tile0 = static_cast<int>(local % tiles);
-        s->tile1 = static_cast<int>(min(static_cast<int64_t>(tiles), s->tile0 + (end - unit)));
-        s->len = len;
-        s->slot = static_cast<int>(block - base / share);
-        s->used = static_cast<int>((base + tiles - 1) / share - base / share) + 1;
-        s->next = 1;
-      }
-      __syncwarp();
-      return;
-    }
-    u -= __shfl_sync(0xffffffffu, upto, 31);
+  Schedule c{};
+  c.units = units_of(a, lane, &c.mine);
+  c.upto = warp_scan(c.units);
+  unsigned total = __shfl_sync(0xffffffffu, c.upto, 31);
+  int most = c.mine.pairs > 0 ? c.mine.tiles : 1;
+  for (int p = 32 + lane; p < (a.prefixes + 31) / 32 * 32; p += 32) {
+    Prefix x{};
+    total += __reduce_add_sync(0xffffffffu, units_of(a, p, &x));
+    if (x.pairs > 0) most = max(most, x.tiles);
   }
+  most = __reduce_max_sync(0xffffffffu, most);
+  // No range of keys meets more than prefix_slots blocks.
+  c.share = max(max((total + gridDim.x - 1) / gridDim.x, (most + a.prefix_slots - 2u) / (a.prefix_slots - 1u)), 1u);
+  c.unit = min(total, blockIdx.x * c.share);
+  c.end = min(total, c.unit + c.share);
+  return c;
+}
+
+// By the scheduling warp: the block's next segment.
+__device__ __forceinline__ void next_segment(const Attention& a, Schedule& c, Segment* s) {
+  const int lane = threadIdx.x & 31;
+  if (c.unit >= c.end) {
+    if (lane == 0) s->tile0 = s->tile1 = 0;
+    __syncwarp();
+    return;
+  }
+  unsigned before = 0;
+  for (int p0 = 0; p0 < a.prefixes; p0 += 32) {
+    Prefix x = c.mine;
+    unsigned n = c.units, upto = c.upto;
+    if (p0 > 0) {
+      n = units_of(a, p0 + lane, &x);
+      upto = before + warp_scan(n);
+    }
+    if (c.unit < upto && c.unit >= upto - n) {
+      const unsigned local = c.unit - (upto - n), range = local / x.tiles, tile0 = local - range * x.tiles;
+      const unsigned first = c.unit - tile0, head = range / x.pairs;  // first: the range's first unit
+      s->prefix = p0 + lane;
+      s->kv_head = static_cast<int>(head);
+      s->first_row = x.first_row;
+      s->start = static_cast<int>(range - head * x.pairs) * kTcRows;
+      s->count = min(kTcRows, x.rows * a.group - s->start);
+      s->tiles = x.tiles;
+      s->tile0 = static_cast<int>(tile0);
+      s->tile1 = static_cast<int>(tile0 + min(x.tiles - tile0, c.end - c.unit));
+      s->len = x.len;
+      const unsigned block0 = first / c.share;
+      s->slot = static_cast<int>(blockIdx.x - block0);
+      s->used = static_cast<int>((first + x.tiles - 1) / c.share - block0) + 1;
+    }
+    before = __shfl_sync(0xffffffffu, upto, 31);
+    if (c.unit < before) break;
+  }
+  __syncwarp();
+  c.unit += s->tile1 - s->tile0;
 }
 
 template <int kDim>
@@ -179,8 +241,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
   constexpr uint32_t kSlotBytes = kHalves * kHalfBytes;
   extern __shared__ unsigned char dyn_raw[];
   __shared__ TcBarriers bars;
-  __shared__ Segment seg;
-  __shared__ int64_t range[3];  // the block's next unit, its end, a block's share
+  __shared__ Segment segs[2];  // the one that is worked on, and the one after it
   __shared__ uint32_t tmem_holder;
   __shared__ int abort_flag;
   const Attention& a = args.a;
@@ -196,6 +257,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&bars.s_full[t], 1);
+      mbar_init(&bars.p_half[t], kTileRows);
       mbar_init(&bars.p_full[t], kTileRows);
     }
     mbar_init(&bars.o_done, 1);
@@ -206,27 +268,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
   if (warp == 1) tmem_alloc(&tmem_holder, kTmemAll);
   pdl_wait();
   pdl_launch_dependents();
+  Schedule schedule{};
   if (warp == 2) {
-    int64_t total = 0;
-    int most = 1;
-    for (int p = lane; p < a.prefixes; p += 32) {
-      int rows, first, pairs, tiles, len;
-      total += units_of(a, p, &rows, &first, &pairs, &tiles, &len);
-      if (pairs > 0) most = max(most, tiles);
-    }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-      total += __shfl_xor_sync(0xffffffffu, total, off);
-      most = max(most, __shfl_xor_sync(0xffffffffu, most, off));
-    }
-    if (lane == 0) {
-      // No range of keys meets more than prefix_slots blocks.
-      const int64_t share = max((total + gridDim.x - 1) / gridDim.x,
-                                static_cast<int64_t>((most + a.prefix_slots - 2) / (a.prefix_slots - 1)));
-      range[0] = min(total, blockIdx.x * share);
-      range[1] = min(total, (blockIdx.x + 1) * share);
-      range[2] = max(share, static_cast<int64_t>(1));
-    }
+    schedule = make_schedule(a);
+    next_segment(a, schedule, &segs[0]);
   }
   tc_fence_before();
   __syncthreads();
@@ -238,100 +283,99 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
   uint32_t issued = 0;  // fills that have been asked for
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegs));
-    for (;;) {
-      if (warp == 2) {
-        const int64_t u = range[0], end = range[1];
-        if (lane == 0) seg.next = 0;
-        __syncwarp();
-        if (u < end) find_segment(a, u, end, range[2], blockIdx.x, &seg);
-        if (lane == 0 && seg.next != 0) range[0] = u + (seg.tile1 - seg.tile0);
-      }
-      __syncthreads();  // the segment is known
-      if (seg.next == 0 || abort_flag != 0) break;
-      const Segment s = seg;
+    uint32_t ahead = 0;  // fills of the segment that were asked for before it began
+    for (;; ++segments) {
+      const Segment s = segs[segments & 1];
       const int tiles = s.tile1 - s.tile0, pair = s.count > kTileRows ? 2 : 1;
-      __syncthreads();  // its Q is there
+      if (tiles == 0 || abort_flag != 0) break;
       if (warp == 0) {
-        if (lane == 0) {
-          // ---- keys and values: K, V, K, V, ... ----
-          uint32_t n = fills;
-          bool ok = true;
-          for (int j = s.tile0; j < s.tile1 && ok; ++j) {
-            // The last tile ends with the prefix: it begins among keys that were there before, which are masked, and
-            // nothing behind the prefix is read.
-            const int key = j == s.tiles - 1 ? s.len - kTcKeys : j * kTcKeys;
-            for (int kv = 0; kv < 2; ++kv, ++n) {
-              const uint32_t slot = n % kSlots;
-              if (!mbar_wait(&bars.empty[slot], (n / kSlots & 1) ^ 1)) {
-                raise_error(a.err, kDevWaitTimeout, 90, j, kv);
-                abort_flag = 1;
-                ok = false;
-                break;
-              }
-              mbar_arrive_expect_tx(&bars.full[slot], kSlotBytes);
-              issued = n + 1;
-              for (int h = 0; h < kHalves; ++h)
-                tma_load_4d(slots + slot * kSlotBytes + h * kHalfBytes, kv == 0 ? &args.k : &args.v, h * 64, key,
-                            s.kv_head, s.prefix, &bars.full[slot]);
-            }
+        // ---- keys and values: K, V, K, V, ... The last tile ends with the prefix: it begins among keys that were there
+        // before, which are masked, and nothing behind the prefix is read. ----
+        auto fill = [&](const Segment& of, uint32_t first, uint32_t k) {
+          const uint32_t n = first + k, slot = n % kSlots;
+          if (!mbar_wait(&bars.empty[slot], (n / kSlots & 1) ^ 1)) {
+            raise_error(a.err, kDevWaitTimeout, 90, of.prefix, static_cast<int>(k));
+            abort_flag = 1;
+            return false;
           }
+          const int tile = of.tile0 + static_cast<int>(k / 2);
+          const int key = tile == of.tiles - 1 ? of.len - kTcKeys : tile * kTcKeys;
+          mbar_arrive_expect_tx(&bars.full[slot], kSlotBytes);
+          issued = n + 1;
+          for (int h = 0; h < kHalves; ++h)
+            tma_load_4d(slots + slot * kSlotBytes + h * kHalfBytes, k % 2 == 0 ? &args.k : &args.v, h * 64, key,
+                        of.kv_head, of.prefix, &bars.full[slot]);
+          return true;
+        };
+        bool ok = true;
+        if (lane == 0)
+          for (uint32_t k = ahead; k < 2u * tiles && ok; ++k) ok = fill(s, fills, k);
+        __syncwarp();
+        named_bar_sync(1, 64);  // the segment after this is known
+        const Segment next = segs[(segments + 1) & 1];
+        // Its first fills wait for no more than this one's products.
+        ahead = min(2u * (next.tile1 - next.tile0), static_cast<uint32_t>(kSlots));
+        if (lane == 0)
+          for (uint32_t k = 0; k < ahead && ok; ++k) ok = fill(next, fills + 2 * tiles, k);
+        __syncwarp();
+      } else if (warp == 2) {
+        next_segment(a, schedule, &segs[(segments + 1) & 1]);
+        named_bar_sync(1, 64);
+      }
+      if (warp == 1) named_bar_sync(2, 32 + 256);  // its Q is there
+      if (warp == 1 && lane == 0) {
+        // ---- MMAs. Those of one thread run in the order of their issue: the scores of a tile's next keys, written
+        // where its weights lie, come behind the product that reads these. ----
+        constexpr uint32_t kScores = bf16_idesc(kTileRows, kTcKeys);
+        constexpr uint32_t kOutput = bf16_idesc(kTileRows, kDim) | kBMajorMn;
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, uint32_t parity, int site) {
+          if (ok && !mbar_wait(bar, parity)) {
+            raise_error(a.err, kDevWaitTimeout, site, s.prefix, static_cast<int>(parity));
+            abort_flag = 1;
+            ok = false;
+          }
+          tc_fence_after();
+        };
+        auto landed = [&](uint32_t n) { wait(&bars.full[n % kSlots], n / kSlots & 1, 91); };
+        auto scores = [&](int t, uint32_t n) {
+          const uint32_t ks = smem_addr(slots + n % kSlots * kSlotBytes);
+          const uint32_t qs = smem_addr(q_tiles + t * kSlotBytes);
+#pragma unroll
+          for (int k = 0; k < kDim / 16; ++k) {
+            const uint32_t off = (k / 4) * kHalfBytes + (k % 4) * 32;
+            umma_bf16(tmem + t * kTcKeys, sw128_kmajor_desc(qs + off), sw128_kmajor_desc(ks + off), kScores, k != 0);
+          }
+          umma_commit(&bars.s_full[t]);
+        };
+        landed(fills);
+        if (ok) {
+          for (int t = 0; t < pair; ++t) scores(t, fills);
+          umma_commit(&bars.empty[fills % kSlots]);
         }
-      } else if (warp == 1) {
-        if (lane == 0) {
-          // ---- MMAs. Those of one thread run in the order of their issue: the scores of a tile's next keys, written
-          // where its weights lie, come behind the product that reads these. ----
-          constexpr uint32_t kScores = bf16_idesc(kTileRows, kTcKeys);
-          constexpr uint32_t kOutput = bf16_idesc(kTileRows, kDim) | kBMajorMn;
-          bool ok = true;
-          auto landed = [&](uint32_t n) {
-            if (ok && !mbar_wait(&bars.full[n % kSlots], n / kSlots & 1)) {
-              raise_error(a.err, kDevWaitTimeout, 91, s.prefix, static_cast<int>(n));
-              abort_flag = 1;
-              ok = false;
-            }
-            tc_fence_after();
-          };
-          auto scores = [&](int t, uint32_t n) {
-            const uint32_t ks = smem_addr(slots + n % kSlots * kSlotBytes);
-            const uint32_t qs = smem_addr(q_tiles + t * kSlotBytes);
+        for (int i = 0; i < tiles && ok; ++i) {
+          const uint32_t v = fills + 2 * i + 1, next_k = v + 1;
+          landed(v);
+          if (i + 1 < tiles) landed(next_k);
+          for (int t = 0; t < pair && ok; ++t) {
+            const uint32_t vs = smem_addr(slots + v % kSlots * kSlotBytes);
+            for (int half = 0; half < 2; ++half) {
+              wait(half == 0 ? &bars.p_half[t] : &bars.p_full[t], (rounds[t] + i) & 1, 92);
+              if (!ok) break;
 #pragma unroll
-            for (int k = 0; k < kDim / 16; ++k) {
-              const uint32_t off = (k / 4) * kHalfBytes + (k % 4) * 32;
-              umma_bf16(tmem + t * kTcKeys, sw128_kmajor_desc(qs + off), sw128_kmajor_desc(ks + off), kScores, k != 0);
-            }
-            umma_commit(&bars.s_full[t]);
-          };
-          landed(fills);
-          if (ok) {
-            for (int t = 0; t < pair; ++t) scores(t, fills);
-            umma_commit(&bars.empty[fills % kSlots]);
-          }
-          for (int i = 0; i < tiles && ok; ++i) {
-            const uint32_t v = fills + 2 * i + 1, next_k = v + 1;
-            landed(v);
-            if (i + 1 < tiles) landed(next_k);
-            for (int t = 0; t < pair && ok; ++t) {
-              if (!mbar_wait(&bars.p_full[t], (rounds[t] + i) & 1)) {
-                raise_error(a.err, kDevWaitTimeout, 92, s.prefix, i);
-                abort_flag = 1;
-                ok = false;
-                break;
-              }
-              tc_fence_after();
-              const uint32_t vs = smem_addr(slots + v % kSlots * kSlotBytes);
-#pragma unroll
-              for (int k = 0; k < kTcKeys / 16; ++k)
+              for (int k = half * kTcKeys / 32; k < (half + 1) * kTcKeys / 32; ++k)
                 umma_bf16_ts(tmem + 2 * kTcKeys + t * kDim, tmem + t * kTcKeys + k * 8,
                              sw128_mnmajor_desc(vs + k * 16 * 128), kOutput, (i | k) != 0);
-              if (t == pair - 1) umma_commit(&bars.empty[v % kSlots]);
-              if (i + 1 < tiles) {
-                scores(t, next_k);
-                if (t == pair - 1) umma_commit(&bars.empty[next_k % kSlots]);
-              }
+            }
+            if (!ok) break;
+            if (t == pair - 1) umma_commit(&bars.empty[v % kSlots]);
+            if (i + 1 < tiles) {
+              scores(t, next_k);
+              if (t == pair - 1) umma_commit(&bars.empty[next_k % kSlots]);
             }
           }
-          umma_commit(&bars.o_done);
         }
+        umma_commit(&bars.o_done);
       }
       fills += 2 * tiles;
       rounds[0] += tiles;
@@ -343,34 +387,38 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegs));
     for (;; ++segments) {
-      __syncthreads();  // the segment is known
-      if (seg.next == 0 || abort_flag != 0) break;
-      const Segment& s = seg;
+      const Segment& s = segs[segments & 1];
       const int tiles = s.tile1 - s.tile0, pair = s.count > kTileRows ? 2 : 1;
+      if (tiles == 0 || abort_flag != 0) break;
       {
-        // A thread brings its row of Q, swizzled like the copies of K.
-        const int r = threadIdx.x - 128;
-        unsigned char* q_tile = q_tiles + (r / kTileRows) * kSlotBytes;
-        const int vr = s.start + r, in_tile = r % kTileRows;
-        const __nv_bfloat16* src = a.q + static_cast<int64_t>(s.first_row + vr / a.group) * a.ldq +
-                                   (s.kv_head * a.group + vr % a.group) * kDim;
-        if (r < pair * kTileRows) {
+        // Q, swizzled like the copies of K: neighbouring threads bring a row's 16-byte pieces.
+        constexpr int kPieces = kDim / 8, kStep = 256 / kPieces;
+        const int thread = threadIdx.x - 128, c = thread % kPieces;
+        uint4 v[kTcRows / kStep];
 #pragma unroll
-          for (int c = 0; c < kDim / 8; ++c) {
-            const uint4 v = r < s.count ? reinterpret_cast<const uint4*>(src)[c] : make_uint4(0, 0, 0, 0);
-            *reinterpret_cast<uint4*>(q_tile + (c / 8) * kHalfBytes + in_tile * 128 + ((c ^ in_tile) & 7) * 16) = v;
-          }
+        for (int i = 0; i < kTcRows / kStep; ++i) {
+          const int r = i * kStep + thread / kPieces, vr = s.start + r;
+          const __nv_bfloat16* src = a.q + static_cast<int64_t>(s.first_row + vr / a.group) * a.ldq +
+                                     (s.kv_head * a.group + vr % a.group) * kDim;
+          v[i] = r < s.count ? reinterpret_cast<const uint4*>(src)[c] : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < kTcRows / kStep; ++i) {
+          const int r = i * kStep + thread / kPieces, in_tile = r % kTileRows;
+          if (r < pair * kTileRows)
+            *reinterpret_cast<uint4*>(q_tiles + (r / kTileRows) * kSlotBytes + (c / 8) * kHalfBytes + in_tile * 128 +
+                                      ((c ^ in_tile) & 7) * 16) = v[i];
         }
         fence_proxy_async_smem();
       }
-      __syncthreads();  // its Q is there
+      named_bar_sync(2, 32 + 256);  // its Q is there
       // ---- a row: its scores to weights ----
       const int t = (warp - 4) / 4, r = threadIdx.x - 128;
       if (t < pair) {
         const uint32_t at = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         const uint32_t s_at = at + t * kTcKeys, o_at = at + 2 * kTcKeys + t * kDim;
         float m = -INFINITY, l = 0.0f;  // m: of the raw scores
-        const int skip_last = seg.tile1 == seg.tiles ? seg.tiles * kTcKeys - seg.len : 0;
+        const int skip_last = s.tile1 == s.tiles ? s.tiles * kTcKeys - s.len : 0;
         bool ok = true;
         for (int i = 0; i < tiles; ++i) {
           if (!__all_sync(0xffffffffu, mbar_wait(&bars.s_full[t], (rounds[0] + i) & 1))) {
@@ -418,25 +466,27 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
             }
           }
           const float shift = m == -INFINITY ? 0.0f : m * a.scale_log2;
-          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          uint32_t p[kTcKeys / 2];
+          const float2 scale2 = make_float2(a.scale_log2, a.scale_log2), shift2 = make_float2(-shift, -shift);
+          float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-          for (int c = 0; c < kTcKeys; c += 4) {
-            float e[4];
+          for (int half = 0; half < 2; ++half) {
+            // The products with the first half's values start while the second half is exponentiated.
+            uint32_t p[kTcKeys / 4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              e[k] = exp2_fast(fmaf(__uint_as_float(x[c + k]), a.scale_log2, -shift));
-              sum[k] += e[k];
+            for (int c = 0; c < kTcKeys / 2; c += 2) {
+              const int at = half * (kTcKeys / 2) + c;
+              float2 e = fma2(make_float2(__uint_as_float(x[at]), __uint_as_float(x[at + 1])), scale2, shift2);
+              e.x = exp2_fast(e.x);
+              e.y = exp2_fast(e.y);
+              sum[c / 2 % 2] = add2(sum[c / 2 % 2], e);
+              p[c / 2] = pack2(e.x, e.y);
             }
-            p[c / 2] = pack2(e[0], e[1]);
-            p[c / 2 + 1] = pack2(e[2], e[3]);
+            tmem_st32(s_at + half * (kTcKeys / 4), p);
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(half == 0 ? &bars.p_half[t] : &bars.p_full[t]);
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-          tmem_st32(s_at, p);
-          tmem_st32(s_at + 32, p + 32);
-          tmem_st_wait();
-          tc_fence_before();
-          mbar_arrive(&bars.p_full[t]);
+          l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         }
         if (ok && !__all_sync(0xffffffffu, mbar_wait(&bars.o_done, segments & 1))) {
           raise_error(a.err, kDevWaitTimeout, 94, s.prefix, 0);
@@ -453,17 +503,28 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
           if (s.tile0 == 0)  // the slots that no block comes to
             for (int k = s.used; k < a.prefix_slots; ++k) a.part_ml[cell + k] = make_float2(-INFINITY, 0.0f);
         }
-        float* dst = a.part_o + (cell + s.slot) * kDim;
+        // 32 columns at a time through 4 KB of the tile's Q, which is done with, so that a store instruction covers whole
+        // lines: four rows of 128 bytes.
+        unsigned char* stage = q_tiles + t * kSlotBytes + (warp & 3) * 4096;
+        const int64_t mine_at = mine ? (cell + s.slot) * kDim : -1;
 #pragma unroll 1
         for (int c = 0; c < kDim; c += 32) {
           uint32_t o[32];
           tmem_ld32_async(o_at + c, o);
           tmem_ld_done(o);
-          if (mine) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              *reinterpret_cast<uint4*>(dst + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          for (int e = 0; e < 8; ++e)
+            *reinterpret_cast<uint4*>(stage + lane * 128 + ((e ^ (lane & 7)) << 4)) =
+                make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int row = k * 4 + lane / 8, e = lane & 7;
+            const int64_t to = __shfl_sync(0xffffffffu, mine_at, row);
+            const uint4 v = *reinterpret_cast<const uint4*>(stage + row * 128 + ((e ^ (row & 7)) << 4));
+            if (to >= 0) *reinterpret_cast<uint4*>(a.part_o + to + c + e * 4) = v;
           }
+          __syncwarp();
         }
         tc_fence_before();
       }
