@@ -18,7 +18,8 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr int kKeys = 64;    // of a stage
-constexpr int kStages = 3;
+constexpr int kStages = 2;
+constexpr int kBlocks = 3;   // of an SM
 constexpr int kMaxSlots = 160;  // of a row: the most that a plan gives its prefix and its own keys
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -381,7 +382,7 @@ __device__ __forceinline__ void attend(const Attention& a, const Segment& seg, u
 }
 
 template <int kDim, int kPrefixWarps, int kOwnWarps>
-__global__ void __launch_bounds__(kThreads) attention_rows_kernel(Attention a, Grid g) {
+__global__ void __launch_bounds__(kThreads, kBlocks) attention_rows_kernel(Attention a, Grid g) {
   constexpr int kPrefixRows = 16 * kPrefixWarps, kOwnRows = 16 * kOwnWarps;
   extern __shared__ __align__(16) unsigned char raw[];
   __shared__ uint32_t odd_keys[kKeys / 32];  // keys of the stage with a value that is no finite number
@@ -605,9 +606,9 @@ Plan plan_of(const uocr_prefix_attention_args& a) {
   const int64_t units =
       a.kv_heads * ((p.tc ? 0 : tiles(a.prefixes, a.sequences / a.prefixes, p.prefix_warps) * prefix_stages) +
                     tiles(a.sequences, 1, p.own_warps) * own_stages);
-  p.blocks = static_cast<unsigned>(std::min<int64_t>(units, 2 * kSms));
+  p.blocks = static_cast<unsigned>(std::min<int64_t>(units, kBlocks * kSms));
   // A range of keys meets as many blocks as shares fit into it, and one more; half as many again for lengths that differ.
-  const int64_t share = std::max<int64_t>((units + 2 * kSms - 1) / (2 * kSms), 1);
+  const int64_t share = std::max<int64_t>((units + kBlocks * kSms - 1) / (kBlocks * kSms), 1);
   auto slots = [&](int64_t stages, int most) {
     return static_cast<int>(stages == 0 ? 0 : std::min<int64_t>((stages + share - 1) / share * 3 / 2 + 2, most));
   };
