@@ -567,7 +567,7 @@ __global__ void __launch_bounds__(kThreads) attention_join_kernel(Attention a) {
 
 // The parts that the prefixes and the own keys are cut into, and the kernels.
 struct Plan {
-  bool tc;  // the prefixes by the tensor-core kernel
+  bool tc, split;  // the prefixes by the tensor-core kernel, its tiles the same rows
   int prefix_slots, own_slots;
   int prefix_warps, own_warps;  // of the kernel for few rows: warps side by side along the rows of a tile
   unsigned blocks;
@@ -584,7 +584,7 @@ bool many_rows(const uocr_prefix_attention_args& a) {
   // what a tensor map takes
   auto far = [](int64_t stride) { return stride <= 0 || stride >= (int64_t{1} << 39); };
   if ((a.kv_heads > 1 && far(a.prefix_head_stride)) || (a.prefixes > 1 && far(a.prefix_stride))) return false;
-  return a.rows * group / a.prefixes > 64;
+  return a.rows * group / a.prefixes > 16;
 }
 
 Plan plan_of(const uocr_prefix_attention_args& a) {
@@ -615,8 +615,10 @@ Plan plan_of(const uocr_prefix_attention_args& a) {
   p.prefix_slots = slots(prefix_stages, kMaxPrefixSlots);
   p.own_slots = slots(own_stages, kMaxOwnSlots);
   if (p.tc) {
-    const int64_t ranges = a.kv_heads * ((a.rows * group + kAttentionTcRows - 1) / kAttentionTcRows);
-    p.prefix_slots = static_cast<int>(std::min<int64_t>(kSms / ranges + 3, kMaxTcSlots));
+    p.split = a.rows * group <= kAttentionTcRows * a.prefixes;
+    const int64_t of_range = kAttentionTcRows * (p.split ? 1 : 2);
+    const int64_t ranges = a.kv_heads * std::max((a.rows * group + of_range - 1) / of_range, p.split ? a.prefixes : 1);
+    p.prefix_slots = static_cast<int>(std::min<int64_t>((kSms / ranges + 3) * (p.split ? 2 : 1), kMaxTcSlots));
   }
   return p;
 }
@@ -661,9 +663,9 @@ cudaError_t launch(const uocr_prefix_attention_args& args, const Attention& a, c
 }  // namespace
 
 bool prefix_attention_counts(const uocr_prefix_attention_args& a) {
-  // Units in 32 bits, and a prefix's rows x heads; the tensor-core kernel's units are a quarter of those counted here.
+  // Units are counted in 32 bits; the tensor-core kernel has at most five for each of these.
   const double stages = static_cast<double>((a.prefix_capacity + kKeys - 1) / kKeys + (a.capacity + kKeys - 1) / kKeys);
-  return (static_cast<double>(a.rows) * a.heads / 16 + a.kv_heads * static_cast<double>(a.sequences)) * stages < 2.0e9;
+  return (static_cast<double>(a.rows) * a.heads / 16 + a.kv_heads * static_cast<double>(a.sequences)) * stages < 8.0e8;
 }
 
 size_t prefix_attention_bytes(const uocr_prefix_attention_args& a) {
@@ -693,6 +695,7 @@ cudaError_t launch_prefix_attention(const uocr_prefix_attention_args& args, Erro
   a.per = static_cast<int>(args.sequences / args.prefixes);
   a.prefix_capacity = static_cast<int>(args.prefix_capacity), a.capacity = static_cast<int>(args.capacity);
   a.prefix_slots = p.prefix_slots;
+  a.split = p.split;
   a.slots = p.prefix_slots + p.own_slots;
   a.scale_log2 = args.scale * kLog2e;
   a.part_o = static_cast<float*>(args.workspace);

@@ -33,6 +33,7 @@ struct Attention {
   int per;                                                        // sequences per prefix
   int prefix_capacity, capacity;
   int prefix_slots, slots;
+  bool split;  // tensor-core kernel: a block's two tiles are the same rows, for every other 128 keys
   float scale_log2;
   float* part_o;     // [rows, heads, slots, dim]
   float2* part_ml;   // [rows, heads, slots]
@@ -91,10 +92,10 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return reinterpret_cast<const uint32_t&>(h);
 }
 
-// Rows (a row and a query head each) that a block of the tensor-core kernel takes.
-constexpr int kAttentionTcRows = 256;
+// Rows (a row and a query head each) of a tile of the tensor-core kernel; a block takes two.
+constexpr int kAttentionTcRows = 128;
 // The prefixes' parts of many rows by tcgen05 (prefix_attention_tc.cu): `blocks`
-// resident blocks; at least two slots; a positive scale.
+// resident blocks; at least four slots (an even number of them to split); a positive scale.
 cudaError_t launch_attention_tc(const Attention& a, int dim, unsigned blocks, cudaStream_t stream);
 
 }  // namespace uocr_b200

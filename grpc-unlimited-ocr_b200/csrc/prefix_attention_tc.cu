@@ -1,25 +1,30 @@
 // Attention behind shared prefixes for many rows, on the tensor cores
 // (uocr_prefix_attention; prefix_attention.cu chooses).
 //
-// A block takes 256 rows (a row and a query head of one key/value head each) as
-// two tiles of 128 and runs the prefix's keys past them, 128 at a time:
+// A block takes rows (a row and a query head of one key/value head each) in two
+// tiles of 128 and runs the prefix's keys past them, 128 at a time:
 //   S = Q K^T   tcgen05.mma, Q and K in shared memory, S in TMEM
 //   P = exp2(S - m), in registers; the sum l; P in bf16 over S in TMEM
 //   O += P V    tcgen05.mma, P in TMEM, V in shared memory, O in TMEM
 // One warp brings keys and values by TMA, one lane issues the MMAs, and one
 // warpgroup a tile does the exponentials, a thread a row, so that a row's maximum
 // and sum need no exchange. The two tiles take turns: while one is exponentiated
-// the other is multiplied.
+// the other is multiplied. With many rows the tiles are 256 rows and see the same
+// keys. With up to 128 they are the same rows, and see every other 128 keys each:
+// their two parts of a row meet in the join like those of two blocks.
 //
 // m is the maximum of the tiles seen when it last had to move: O and l are
 // rescaled only where a later score exceeds it by more than 2^8, which fp32 and
 // bf16 hold without loss, and which hardly happens after the first tile.
 //
-// Work is cut by units of one tile pair and 128 keys, counted through over
+// Work is cut by units of the tiles' rows and 128 keys, counted through over
 // prefixes, heads and rows, the same number for every block, whatever the
 // lengths: a block's share may begin and end inside a range of keys, and the
-// parts of a row meet in the join's slots.
+// parts of a row meet in the join's slots. What a range costs a block besides its
+// keys (bringing Q, the first scores, the way out of O) counts as units before its
+// first key, so that a block with two ranges has fewer keys.
 #include <algorithm>
+#include <type_traits>
 
 #include "prefix_attention.cuh"
 #include "tc.cuh"
@@ -29,8 +34,8 @@
 namespace uocr_b200 {
 namespace {
 
-constexpr int kTcRows = kAttentionTcRows;  // of a block: two tiles
-constexpr int kTileRows = kTcRows / 2;
+constexpr int kTileRows = kAttentionTcRows;
+constexpr unsigned kRangeUnits = 4;  // what a range costs besides its keys: 7 us, where 128 keys take 1.8
 constexpr int kTcKeys = 128;
 constexpr int kSlots = 4;        // shared-memory slots of 128 keys or values
 constexpr int kTcThreads = 384;  // a warpgroup for copies and MMAs, two of rows
@@ -39,25 +44,52 @@ constexpr float kSlack = 8.0f;   // log2 of what a score may exceed m by
 constexpr int kLaunchRegs = 168, kFewRegs = 56, kManyRegs = 224;
 constexpr uint32_t kTmemAll = 512;
 
-// O of N = kDim columns (+)= P in TMEM . V in shared memory (K = 16 keys).
-__device__ __forceinline__ void umma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
-                                             uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-
-// Values [128 keys][64 dims] per 16 KB as TMA leaves them, as the B operand with
-// N = dims contiguous (MN-major, 128-byte swizzle): 64-dim chunks 16 KB apart
-// (the leading offset), 8-key groups 1024 bytes apart.
-__device__ __forceinline__ uint64_t sw128_mnmajor_desc(uint32_t saddr) {
-  return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(kTcKeys * 128 >> 4) << 16) |
-         (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
+// Shared-memory matrix descriptors in halves: the low word names the address and
+// the leading offset and is what moves from product to product; one lane issues
+// them all, and every operation on a descriptor is time between two products.
+// Keys and Q: K-major, 128-byte swizzle, 8-row groups 1024 bytes apart. Values
+// [128 keys][64 dims] per 16 KB as TMA leaves them: B with N = dims contiguous
+// (MN-major), 64-dim chunks 16 KB apart (the leading offset), 8-key groups 1024
+// bytes apart.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);  // group stride, version 1, 128-byte swizzle
+__device__ __forceinline__ uint32_t kmajor_low(uint32_t saddr) { return (saddr >> 4 & 0x3FFFu) | (1u << 16); }
+__device__ __forceinline__ uint32_t mnmajor_low(uint32_t saddr) {
+  return (saddr >> 4 & 0x3FFFu) | (static_cast<uint32_t>(kTcKeys * 128 >> 4) << 16);
 }
 constexpr uint32_t kBMajorMn = 1u << 16;  // instruction descriptor: B is MN-major
+
+// The MMA warp runs as a whole and one lane's predicate lets the instruction
+// through, so that its operands stay uniform registers.
+// D in TMEM (+)= A in shared memory . B in shared memory, K = 16.
+__device__ __forceinline__ void umma_ss(uint32_t leader, uint32_t d_tmem, uint32_t a_low, uint32_t b_low,
+                                        uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+      "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_low), "r"(b_low), "r"(idesc), "r"(accumulate), "n"(kDescHigh), "r"(leader)
+      : "memory");
+}
+// D in TMEM (+)= A in TMEM . B in shared memory, K = 16.
+__device__ __forceinline__ void umma_ts(uint32_t leader, uint32_t d_tmem, uint32_t a_tmem, uint32_t b_low,
+                                        uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+      "mov.b64 b, {%2, %5};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_low), "r"(idesc), "r"(accumulate), "n"(kDescHigh), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void umma_commit_by(uint32_t leader, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar)),
+      "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
 __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int c0, int c1, int c2, int c3,
                                             uint64_t* bar) {
@@ -147,16 +179,17 @@ struct TcArgs {
 // A prefix: its rows and keys.
 struct Prefix {
   int rows, first_row, len;
-  int pairs, tiles;  // of 256 rows, of 128 keys
+  int ranges, tiles;  // of rows (a head's), of 128 keys
 };
-// The units of prefix p: (key/value heads) x (row tile pairs) x (key tiles).
+// The units of prefix p: (key/value heads) x (ranges) x (key tiles and what a range costs).
 __device__ __forceinline__ unsigned units_of(const Attention& a, int p, Prefix* x) {
   if (p >= a.prefixes) return 0;
   x->rows = prefix_rows_of(a, p, &x->first_row);
   x->len = prefix_len_of(a, p);
-  x->pairs = (x->rows * a.group + kTcRows - 1) / kTcRows;
+  const int of_range = a.split ? kTileRows : 2 * kTileRows;
+  x->ranges = (x->rows * a.group + of_range - 1) / of_range;
   x->tiles = max(1, (x->len + kTcKeys - 1) / kTcKeys);  // an empty prefix still has a part: no keys
-  return static_cast<unsigned>(a.kv_heads) * x->pairs * x->tiles;
+  return static_cast<unsigned>(a.kv_heads) * x->ranges * (x->tiles + kRangeUnits);
 }
 __device__ __forceinline__ unsigned warp_scan(unsigned v) {
   const int lane = threadIdx.x & 31;
@@ -166,6 +199,13 @@ __device__ __forceinline__ unsigned warp_scan(unsigned v) {
     if (lane >= off) v += other;
   }
   return v;
+}
+
+// Where a segment's key tile i and its values lie among the fills. Same keys for both tiles: K0 V0 K1 V1 ...; every
+// other one: K0 K1 V0 K2 V1 K3 ... V.
+__device__ __forceinline__ uint32_t key_fill(bool split, int i) { return split ? (i < 2 ? i : 2 * i - 1) : 2 * i; }
+__device__ __forceinline__ uint32_t value_fill(bool split, int i, int tiles) {
+  return split ? (i == tiles - 1 ? 2 * i + 1 : 2 * i + 2) : 2 * i + 1;
 }
 
 // What the scheduling warp keeps: the first 32 prefixes, which mostly are all.
@@ -181,15 +221,16 @@ __device__ __forceinline__ Schedule make_schedule(const Attention& a) {
   c.units = units_of(a, lane, &c.mine);
   c.upto = warp_scan(c.units);
   unsigned total = __shfl_sync(0xffffffffu, c.upto, 31);
-  int most = c.mine.pairs > 0 ? c.mine.tiles : 1;
+  int most = c.mine.ranges > 0 ? c.mine.tiles : 1;
   for (int p = 32 + lane; p < (a.prefixes + 31) / 32 * 32; p += 32) {
     Prefix x{};
     total += __reduce_add_sync(0xffffffffu, units_of(a, p, &x));
-    if (x.pairs > 0) most = max(most, x.tiles);
+    if (x.ranges > 0) most = max(most, x.tiles);
   }
   most = __reduce_max_sync(0xffffffffu, most);
-  // No range of keys meets more than prefix_slots blocks.
-  c.share = max(max((total + gridDim.x - 1) / gridDim.x, (most + a.prefix_slots - 2u) / (a.prefix_slots - 1u)), 1u);
+  // No range of keys meets more blocks than there are slots for (two of a block that splits the keys).
+  const unsigned blocks = a.split ? a.prefix_slots / 2 : a.prefix_slots;
+  c.share = max(max((total + gridDim.x - 1) / gridDim.x, (most + blocks - 2) / (blocks - 1)), 1u);
   c.unit = min(total, blockIdx.x * c.share);
   c.end = min(total, c.unit + c.share);
   return c;
@@ -198,40 +239,45 @@ __device__ __forceinline__ Schedule make_schedule(const Attention& a) {
 // By the scheduling warp: the block's next segment.
 __device__ __forceinline__ void next_segment(const Attention& a, Schedule& c, Segment* s) {
   const int lane = threadIdx.x & 31;
-  if (c.unit >= c.end) {
-    if (lane == 0) s->tile0 = s->tile1 = 0;
-    __syncwarp();
-    return;
-  }
+  if (lane == 0) s->tile0 = s->tile1 = 0;
+  __syncwarp();
   unsigned before = 0;
-  for (int p0 = 0; p0 < a.prefixes; p0 += 32) {
+  for (int p0 = 0; p0 < a.prefixes && c.unit < c.end; p0 += 32) {
     Prefix x = c.mine;
     unsigned n = c.units, upto = c.upto;
     if (p0 > 0) {
       n = units_of(a, p0 + lane, &x);
       upto = before + warp_scan(n);
     }
-    if (c.unit < upto && c.unit >= upto - n) {
-      const unsigned local = c.unit - (upto - n), range = local / x.tiles, tile0 = local - range * x.tiles;
-      const unsigned first = c.unit - tile0, head = range / x.pairs;  // first: the range's first unit
+    const bool mine = c.unit < upto && c.unit >= upto - n;
+    unsigned to = 0;
+    if (mine) {
+      const unsigned each = x.tiles + kRangeUnits;
+      const unsigned local = c.unit - (upto - n), range = local / each, at = local - range * each;
+      const unsigned first = c.unit - at + kRangeUnits, head = range / x.ranges;  // first: the unit of the first keys
+      const int of_range = a.split ? kTileRows : 2 * kTileRows;
+      to = min(c.unit - at + each, c.end);
       s->prefix = p0 + lane;
       s->kv_head = static_cast<int>(head);
       s->first_row = x.first_row;
-      s->start = static_cast<int>(range - head * x.pairs) * kTcRows;
-      s->count = min(kTcRows, x.rows * a.group - s->start);
+      s->start = static_cast<int>(range - head * x.ranges) * of_range;
+      s->count = min(of_range, x.rows * a.group - s->start);
       s->tiles = x.tiles;
-      s->tile0 = static_cast<int>(tile0);
-      s->tile1 = static_cast<int>(tile0 + min(x.tiles - tile0, c.end - c.unit));
+      s->tile0 = static_cast<int>(max(c.unit, first) - first);
+      s->tile1 = static_cast<int>(max(to, first) - first);  // none where the share ends before the first keys
       s->len = x.len;
       const unsigned block0 = first / c.share;
       s->slot = static_cast<int>(blockIdx.x - block0);
       s->used = static_cast<int>((first + x.tiles - 1) / c.share - block0) + 1;
     }
+    const unsigned who = __ballot_sync(0xffffffffu, mine);
     before = __shfl_sync(0xffffffffu, upto, 31);
-    if (c.unit < before) break;
+    if (who != 0) {
+      c.unit = __shfl_sync(0xffffffffu, to, __ffs(who) - 1);
+      break;
+    }
   }
   __syncwarp();
-  c.unit += s->tile1 - s->tile0;
 }
 
 template <int kDim>
@@ -249,7 +295,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(dyn_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   unsigned char* q_tiles = smem;                        // [2][kSlotBytes]
   unsigned char* slots = smem + 2 * kSlotBytes;         // [kSlots][kSlotBytes]
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kSlots; ++i) {
       mbar_init(&bars.full[i], 1);
@@ -276,21 +322,23 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_holder;
+  const uint32_t tmem = static_cast<uint32_t>(uniform(static_cast<int>(tmem_holder)));
   // Counters that run on over the segments: a slot's or a tile's use number gives its barrier's phase. The two kinds
   // of warpgroup keep to code of their own from here on, with the same barriers in it: their registers differ.
   uint32_t fills = 0, rounds[2] = {0, 0}, segments = 0;
   uint32_t issued = 0;  // fills that have been asked for
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegs));
+    const uint32_t leader = elect_one() ? 1u : 0u;
     uint32_t ahead = 0;  // fills of the segment that were asked for before it began
     for (;; ++segments) {
       const Segment s = segs[segments & 1];
-      const int tiles = s.tile1 - s.tile0, pair = s.count > kTileRows ? 2 : 1;
+      const int tiles = uniform(s.tile1 - s.tile0), pair = uniform(s.count) > kTileRows ? 2 : 1;
       if (tiles == 0 || abort_flag != 0) break;
       if (warp == 0) {
-        // ---- keys and values: K, V, K, V, ... The last tile ends with the prefix: it begins among keys that were there
-        // before, which are masked, and nothing behind the prefix is read. ----
+        // ---- keys and values, in the order in which the products take them (key_fill, value_fill). The last tile ends
+        // with the prefix: it begins among keys that were there before, which are masked, and nothing behind the
+        // prefix is read. ----
         auto fill = [&](const Segment& of, uint32_t first, uint32_t k) {
           const uint32_t n = first + k, slot = n % kSlots;
           if (!mbar_wait(&bars.empty[slot], (n / kSlots & 1) ^ 1)) {
@@ -298,12 +346,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
             abort_flag = 1;
             return false;
           }
-          const int tile = of.tile0 + static_cast<int>(k / 2);
+          const uint32_t all = of.tile1 - of.tile0;
+          uint32_t j = k / 2;
+          bool keys = k % 2 == 0;
+          if (a.split && all > 1) {
+            keys = k < 2 || (k % 2 == 1 && k < 2 * all - 2);
+            j = k < 2 ? k : keys ? k / 2 + 1 : k == 2 * all - 1 ? all - 1 : k / 2 - 1;
+          }
+          const int tile = of.tile0 + static_cast<int>(j);
           const int key = tile == of.tiles - 1 ? of.len - kTcKeys : tile * kTcKeys;
           mbar_arrive_expect_tx(&bars.full[slot], kSlotBytes);
           issued = n + 1;
           for (int h = 0; h < kHalves; ++h)
-            tma_load_4d(slots + slot * kSlotBytes + h * kHalfBytes, k % 2 == 0 ? &args.k : &args.v, h * 64, key,
+            tma_load_4d(slots + slot * kSlotBytes + h * kHalfBytes, keys ? &args.k : &args.v, h * 64, key,
                         of.kv_head, of.prefix, &bars.full[slot]);
           return true;
         };
@@ -322,64 +377,84 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
         next_segment(a, schedule, &segs[(segments + 1) & 1]);
         named_bar_sync(1, 64);
       }
-      if (warp == 1) named_bar_sync(2, 32 + 256);  // its Q is there
-      if (warp == 1 && lane == 0) {
+      if (warp == 1) {
+        named_bar_sync(2, 32 + 256);  // its Q is there
         // ---- MMAs. Those of one thread run in the order of their issue: the scores of a tile's next keys, written
         // where its weights lie, come behind the product that reads these. ----
         constexpr uint32_t kScores = bf16_idesc(kTileRows, kTcKeys);
         constexpr uint32_t kOutput = bf16_idesc(kTileRows, kDim) | kBMajorMn;
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t parity, int site) {
-          if (ok && !mbar_wait(bar, parity)) {
-            raise_error(a.err, kDevWaitTimeout, site, s.prefix, static_cast<int>(parity));
+          if (ok && !__all_sync(0xffffffffu, mbar_wait(bar, parity))) {
+            if (leader) raise_error(a.err, kDevWaitTimeout, site, s.prefix, static_cast<int>(parity));
             abort_flag = 1;
             ok = false;
           }
           tc_fence_after();
         };
         auto landed = [&](uint32_t n) { wait(&bars.full[n % kSlots], n / kSlots & 1, 91); };
-        auto scores = [&](int t, uint32_t n) {
-          const uint32_t ks = smem_addr(slots + n % kSlots * kSlotBytes);
-          const uint32_t qs = smem_addr(q_tiles + t * kSlotBytes);
+        const uint32_t q_low = kmajor_low(smem_addr(q_tiles)), k_low = kmajor_low(smem_addr(slots)),
+                       v_low = mnmajor_low(smem_addr(slots));
+        auto scores = [&](auto tile, uint32_t n) {
+          constexpr int t = decltype(tile)::value;
+          const uint32_t k0 = k_low + n % kSlots * (kSlotBytes >> 4);
+          const uint32_t q0 = q_low + (t == 0 || a.split ? 0u : kSlotBytes >> 4);
 #pragma unroll
           for (int k = 0; k < kDim / 16; ++k) {
-            const uint32_t off = (k / 4) * kHalfBytes + (k % 4) * 32;
-            umma_bf16(tmem + t * kTcKeys, sw128_kmajor_desc(qs + off), sw128_kmajor_desc(ks + off), kScores, k != 0);
+            const uint32_t off = ((k / 4) * kHalfBytes + (k % 4) * 32) >> 4;
+            umma_ss(leader, tmem + t * kTcKeys, q0 + off, k0 + off, kScores, k != 0);
           }
-          umma_commit(&bars.s_full[t]);
+          umma_commit_by(leader, &bars.s_full[t]);
         };
-        landed(fills);
-        if (ok) {
-          for (int t = 0; t < pair; ++t) scores(t, fills);
-          umma_commit(&bars.empty[fills % kSlots]);
-        }
-        for (int i = 0; i < tiles && ok; ++i) {
-          const uint32_t v = fills + 2 * i + 1, next_k = v + 1;
+        // A tile's turn: the output of its keys `i`, then the scores of its next ones.
+        auto turn = [&](auto tile, int i, uint32_t round) {
+          constexpr int t = decltype(tile)::value;
+          const bool last_use = a.split || t == pair - 1;
+          const uint32_t v = fills + value_fill(a.split, i, tiles);
           landed(v);
-          if (i + 1 < tiles) landed(next_k);
-          for (int t = 0; t < pair && ok; ++t) {
-            const uint32_t vs = smem_addr(slots + v % kSlots * kSlotBytes);
-            for (int half = 0; half < 2; ++half) {
-              wait(half == 0 ? &bars.p_half[t] : &bars.p_full[t], (rounds[t] + i) & 1, 92);
-              if (!ok) break;
+          const uint32_t v0 = v_low + v % kSlots * (kSlotBytes >> 4);
+          for (int half = 0; half < 2; ++half) {
+            wait(half == 0 ? &bars.p_half[t] : &bars.p_full[t], (rounds[t] + round) & 1, 92);
+            if (!ok) return;
 #pragma unroll
-              for (int k = half * kTcKeys / 32; k < (half + 1) * kTcKeys / 32; ++k)
-                umma_bf16_ts(tmem + 2 * kTcKeys + t * kDim, tmem + t * kTcKeys + k * 8,
-                             sw128_mnmajor_desc(vs + k * 16 * 128), kOutput, (i | k) != 0);
-            }
-            if (!ok) break;
-            if (t == pair - 1) umma_commit(&bars.empty[v % kSlots]);
-            if (i + 1 < tiles) {
-              scores(t, next_k);
-              if (t == pair - 1) umma_commit(&bars.empty[next_k % kSlots]);
-            }
+            for (int k = 0; k < kTcKeys / 32; ++k)
+              umma_ts(leader, tmem + 2 * kTcKeys + t * kDim, tmem + t * kTcKeys + half * (kTcKeys / 4) + k * 8,
+                      v0 + half * (kTcKeys / 2 * 128 >> 4) + (k * 16 * 128 >> 4), kOutput, round | half | k);
           }
+          if (last_use) umma_commit_by(leader, &bars.empty[v % kSlots]);
+          const int next = a.split ? i + 2 : i + 1;
+          if (next >= tiles) return;
+          const uint32_t n = fills + key_fill(a.split, next);
+          landed(n);
+          if (!ok) return;
+          scores(tile, n);
+          if (last_use) umma_commit_by(leader, &bars.empty[n % kSlots]);
+        };
+        constexpr std::integral_constant<int, 0> k0{};
+        constexpr std::integral_constant<int, 1> k1{};
+        landed(fills);
+        if (ok) scores(k0, fills);
+        if (a.split) {
+          umma_commit_by(leader, &bars.empty[fills % kSlots]);
+          if (tiles > 1) {
+            landed(fills + 1);
+            if (ok) scores(k1, fills + 1);
+            umma_commit_by(leader, &bars.empty[(fills + 1) % kSlots]);
+          }
+        } else {
+          if (ok && pair == 2) scores(k1, fills);
+          umma_commit_by(leader, &bars.empty[fills % kSlots]);
         }
-        umma_commit(&bars.o_done);
+        const int step = a.split ? 2 : 1;
+        for (int i = 0, round = 0; i < tiles && ok; i += step, ++round) {
+          turn(k0, i, round);
+          if (ok && (a.split ? i + 1 < tiles : pair == 2)) turn(k1, a.split ? i + 1 : i, round);
+        }
+        umma_commit_by(leader, &bars.o_done);
       }
       fills += 2 * tiles;
-      rounds[0] += tiles;
-      if (pair == 2) rounds[1] += tiles;
+      rounds[0] += a.split ? (tiles + 1) / 2 : tiles;
+      rounds[1] += a.split ? tiles / 2 : pair == 2 ? tiles : 0;
       __syncwarp();
       __syncthreads();  // its TMEM and Q have been read
       tc_fence_after();
@@ -394,16 +469,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
         // Q, swizzled like the copies of K: neighbouring threads bring a row's 16-byte pieces.
         constexpr int kPieces = kDim / 8, kStep = 256 / kPieces;
         const int thread = threadIdx.x - 128, c = thread % kPieces;
-        uint4 v[kTcRows / kStep];
+        constexpr int kCopies = 2 * kTileRows / kStep;
+        uint4 v[kCopies];
 #pragma unroll
-        for (int i = 0; i < kTcRows / kStep; ++i) {
+        for (int i = 0; i < kCopies; ++i) {
           const int r = i * kStep + thread / kPieces, vr = s.start + r;
           const __nv_bfloat16* src = a.q + static_cast<int64_t>(s.first_row + vr / a.group) * a.ldq +
                                      (s.kv_head * a.group + vr % a.group) * kDim;
           v[i] = r < s.count ? reinterpret_cast<const uint4*>(src)[c] : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
-        for (int i = 0; i < kTcRows / kStep; ++i) {
+        for (int i = 0; i < kCopies; ++i) {
           const int r = i * kStep + thread / kPieces, in_tile = r % kTileRows;
           if (r < pair * kTileRows)
             *reinterpret_cast<uint4*>(q_tiles + (r / kTileRows) * kSlotBytes + (c / 8) * kHalfBytes + in_tile * 128 +
@@ -413,14 +489,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
       }
       named_bar_sync(2, 32 + 256);  // its Q is there
       // ---- a row: its scores to weights ----
-      const int t = (warp - 4) / 4, r = threadIdx.x - 128;
-      if (t < pair) {
+      const int t = (warp - 4) / 4, in_tile = (threadIdx.x - 128) % kTileRows, r = a.split ? in_tile : threadIdx.x - 128;
+      // The tile's rounds, and the one that ends with the prefix, if it has it.
+      const int my_rounds = a.split ? (tiles + 1 - t) / 2 : t < pair ? tiles : 0;
+      const bool has_end = s.tile1 == s.tiles && (!a.split || (tiles - 1) % 2 == t);
+      if (my_rounds > 0 || a.split) {
         const uint32_t at = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         const uint32_t s_at = at + t * kTcKeys, o_at = at + 2 * kTcKeys + t * kDim;
         float m = -INFINITY, l = 0.0f;  // m: of the raw scores
-        const int skip_last = s.tile1 == s.tiles ? s.tiles * kTcKeys - s.len : 0;
+        const int skip_last = has_end ? s.tiles * kTcKeys - s.len : 0;
+        const bool has_rows = r - lane < s.count;  // of this warp
         bool ok = true;
-        for (int i = 0; i < tiles; ++i) {
+        for (int i = 0; i < my_rounds; ++i) {
           if (!__all_sync(0xffffffffu, mbar_wait(&bars.s_full[t], (rounds[0] + i) & 1))) {
             raise_error(a.err, kDevWaitTimeout, 93, s.prefix, i);
             abort_flag = 1;
@@ -428,11 +508,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
             break;
           }
           tc_fence_after();
+          if (!has_rows) {
+            mbar_arrive(&bars.p_half[t]);
+            mbar_arrive(&bars.p_full[t]);
+            continue;
+          }
           uint32_t x[kTcKeys];
 #pragma unroll
           for (int c = 0; c < kTcKeys; c += 32) tmem_ld32_async(s_at + c, x + c);
           tmem_ld_done(x);
-          const int skip = i == tiles - 1 ? skip_last : 0;
+          const int skip = i == my_rounds - 1 ? skip_last : 0;
           if (skip > 0) {
 #pragma unroll
             for (int c = 0; c < kTcKeys; ++c)
@@ -497,18 +582,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
         const int vr = s.start + r;
         const int64_t cell =
             (static_cast<int64_t>(s.first_row + vr / a.group) * a.heads + s.kv_head * a.group + vr % a.group) * a.slots;
+        const int slot = a.split ? 2 * s.slot + t : s.slot;
         const bool mine = r < s.count && ok;
         if (mine) {
-          a.part_ml[cell + s.slot] = make_float2(m == -INFINITY ? m : m * a.scale_log2, l);
-          if (s.tile0 == 0)  // the slots that no block comes to
-            for (int k = s.used; k < a.prefix_slots; ++k) a.part_ml[cell + k] = make_float2(-INFINITY, 0.0f);
+          a.part_ml[cell + slot] = make_float2(m == -INFINITY ? m : m * a.scale_log2, l);
+          if (s.tile0 == 0 && (t == 0 || !a.split))  // the slots that no block comes to
+            for (int k = a.split ? 2 * s.used : s.used; k < a.prefix_slots; ++k)
+              a.part_ml[cell + k] = make_float2(-INFINITY, 0.0f);
         }
         // 32 columns at a time through 4 KB of the tile's Q, which is done with, so that a store instruction covers whole
         // lines: four rows of 128 bytes.
         unsigned char* stage = q_tiles + t * kSlotBytes + (warp & 3) * 4096;
-        const int64_t mine_at = mine ? (cell + s.slot) * kDim : -1;
+        const int64_t mine_at = mine ? (cell + slot) * kDim : -1;
 #pragma unroll 1
-        for (int c = 0; c < kDim; c += 32) {
+        for (int c = 0; c < (has_rows && my_rounds > 0 ? kDim : 0); c += 32) {
           uint32_t o[32];
           tmem_ld32_async(o_at + c, o);
           tmem_ld_done(o);
@@ -528,17 +615,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
         }
         tc_fence_before();
       }
-      if ((warp - 4) / 4 < pair) rounds[0] += tiles;  // of this warp's tile
+      rounds[0] += my_rounds;  // of this warp's tile
       __syncthreads();  // its TMEM and Q have been read
     }
   }
-  if (abort_flag != 0 && lane == 0) {
+  if (abort_flag != 0) {
     // A wait gave up: nothing may be in flight when the block ends.
-    if (warp == 0)
+    if (warp == 0 && lane == 0)
       for (uint32_t n = issued > kSlots ? issued - kSlots : 0; n < issued; ++n)
         mbar_wait(&bars.full[n % kSlots], n / kSlots & 1);
-    if (warp == 1) {
-      umma_commit(&bars.drain);
+    if (warp == 1) {  // by the lane that issued the MMAs
+      umma_commit_by(elect_one() ? 1u : 0u, &bars.drain);
       mbar_wait(&bars.drain, 0);
     }
   }
