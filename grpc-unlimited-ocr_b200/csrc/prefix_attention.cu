@@ -9,6 +9,7 @@
 // So prefixes and own keys are cut into as many shares as the card holds blocks,
 // and a second kernel joins a row's parts.
 #include <algorithm>
+#include <type_traits>
 
 #include "prefix_attention.cuh"
 #include "w8a8.h"
@@ -21,6 +22,8 @@ constexpr int kKeys = 64;    // of a stage
 constexpr int kStages = 2;
 constexpr int kBlocks = 3;   // of an SM
 constexpr int kMaxSlots = 160;  // of a row: the most that a plan gives its prefix and its own keys
+constexpr int kMaxPrefixSlots = 64, kMaxOwnSlots = 32, kMaxTcSlots = 128;
+static_assert(kMaxPrefixSlots + kMaxOwnSlots <= kMaxSlots && kMaxTcSlots + kMaxOwnSlots <= kMaxSlots, "");
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -118,8 +121,12 @@ __device__ __forceinline__ unsigned block_scan(unsigned v, unsigned* part, unsig
 // output in registers; keys and values in a ring of padded stages filled by
 // cp.async. mma.sync and not tcgen05: a tile has 16 to 64 rows, of which a tcgen05
 // tile would use an eighth to a half.
-template <int kDim, int kWarpRows>
-__device__ __forceinline__ void attend(const Attention& a, const Segment& seg, unsigned char* raw, uint32_t* odd_keys) {
+// With kLast the block has all own keys of its rows: it joins the prefix's parts
+// to them (behind the wait for the kernel that makes them, with late_wait) and
+// writes the rows; else it writes its part.
+template <int kDim, int kWarpRows, bool kLast>
+__device__ __forceinline__ void attend(const Attention& a, const Segment& seg, unsigned char* raw, uint32_t* odd_keys,
+                                       bool late_wait) {
   const Segment w = seg;  // in registers
   constexpr int kRows = 16 * kWarpRows, kWarpKeys = kKeys / (4 / kWarpRows);
   constexpr int kPitch = kDim + 8;  // padded: fragment loads without bank conflicts
@@ -319,31 +326,16 @@ __device__ __forceinline__ void attend(const Attention& a, const Segment& seg, u
   auto cell = [&](int r) {  // of the tile's row r
     const int vr = w.start + r;
     const int64_t row = w.first_row + vr / a.group;
-    return (row * a.heads + w.kv_head * a.group + vr % a.group) * a.slots;
+    return row * a.heads + w.kv_head * a.group + vr % a.group;
   };
-  if (w.first)  // the slots that no block comes to
-    for (int c = threadIdx.x; c < w.count * (w.slots - w.used); c += kThreads)
-      a.part_ml[cell(c % w.count) + w.used + c / w.count] = make_float2(-INFINITY, 0.0f);
-  if (w.key0 >= w.key1) {
-    for (int r = threadIdx.x; r < w.count; r += kThreads) a.part_ml[cell(r) + w.slot] = make_float2(-INFINITY, 0.0f);
-    return;
-  }
-  if constexpr (kWarpRows == 4) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = row0 + gr + 8 * i;
-      if (r >= w.count) continue;
-      const int64_t at = cell(r) + w.slot;
-      if (tq == 0) a.part_ml[at] = make_float2(m[i], l[i]);
-#pragma unroll
-      for (int d = 0; d < kDim / 8; ++d)
-        *reinterpret_cast<float2*>(a.part_o + at * kDim + d * 8 + 2 * tq) = make_float2(o[d][2 * i], o[d][2 * i + 1]);
-    }
-  } else {
-    // The warps along the keys are joined in shared memory, in the ring's place.
+  if constexpr (kLast) {
     constexpr int kAlong = 4 / kWarpRows;
-    float* os = reinterpret_cast<float*>(raw);                    // [kAlong][kRows][kDim]
+    float* os = reinterpret_cast<float*>(raw);                            // [kAlong][kRows][kDim], in the ring's place
     float2* mls = reinterpret_cast<float2*>(os + kAlong * kRows * kDim);  // [kAlong][kRows]
+    float* own = reinterpret_cast<float*>(mls + kAlong * kRows);          // [kAlong][kRows] factors
+    float* scales = own + kAlong * kRows;                                 // [kRows] 1 / sum
+    // [kRows][prefix_slots] the parts' maxima and sums, then their factors in the maxima's place
+    float2* factors = reinterpret_cast<float2*>(scales + kRows);
     cp_async_wait_all();
     __syncthreads();
     const int along = warp / kWarpRows;
@@ -356,27 +348,171 @@ __device__ __forceinline__ void attend(const Attention& a, const Segment& seg, u
         *reinterpret_cast<float2*>(os + (along * kRows + r) * kDim + d * 8 + 2 * tq) =
             make_float2(o[d][2 * i], o[d][2 * i + 1]);
     }
+    if (late_wait) pdl_wait();  // the prefix's parts
     __syncthreads();
-    for (int c = threadIdx.x; c < w.count * (kDim / 4); c += kThreads) {
-      const int r = c / (kDim / 4), col = c % (kDim / 4) * 4;
-      float top = -INFINITY;
+    for (int c0 = threadIdx.x; c0 < w.count * a.prefix_slots; c0 += 8 * kThreads) {
+      float2 ml[8];
 #pragma unroll
-      for (int i = 0; i < kAlong; ++i) top = fmaxf(top, mls[i * kRows + r].x);
+      for (int k = 0; k < 8; ++k) {
+        const int c = c0 + k * kThreads;
+        if (c < w.count * a.prefix_slots) ml[k] = a.part_ml[cell(c / a.prefix_slots) * a.slots + c % a.prefix_slots];
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (c0 + k * kThreads < w.count * a.prefix_slots) factors[c0 + k * kThreads] = ml[k];
+    }
+    if (threadIdx.x == 0) odd_keys[0] = 0;  // from here on: one more than the last slot with keys
+    __syncthreads();
+    {
+      // All rows at once, kLanes neighbouring threads each.
+      constexpr int kLanes = kThreads / kRows;
+      const int r = threadIdx.x / kLanes, at = threadIdx.x % kLanes;
+      float2* ml = factors + r * a.prefix_slots;
+      const int slots = r < w.count ? a.prefix_slots : 0;
+      float top = -INFINITY;
+      for (int i = at; i < kAlong; i += kLanes) top = fmaxf(top, mls[i * kRows + r].x);
+      for (int s = at; s < slots; s += kLanes) top = fmaxf(top, ml[s].x);
+#pragma unroll
+      for (int off = kLanes / 2; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
       const float shift = top == -INFINITY ? 0.0f : top;
       float sum = 0.0f;
-      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-      for (int i = 0; i < kAlong; ++i) {
-        const float2 ml = mls[i * kRows + r];
-        const float f = exp2_fast(ml.x - shift);
-        const float4 v = *reinterpret_cast<const float4*>(os + (i * kRows + r) * kDim + col);
-        sum = fmaf(ml.y, f, sum);
-        acc.x = fmaf(v.x, f, acc.x), acc.y = fmaf(v.y, f, acc.y);
-        acc.z = fmaf(v.z, f, acc.z), acc.w = fmaf(v.w, f, acc.w);
+      int live = 0;
+      for (int i = at; i < kAlong; i += kLanes) {
+        const float2 p = mls[i * kRows + r];
+        const float f = exp2_fast(p.x - shift);
+        sum = fmaf(p.y, f, sum);
+        own[i * kRows + r] = f;
       }
-      const int64_t at = cell(r) + w.slot;
-      if (col == 0) a.part_ml[at] = make_float2(top, sum);
-      *reinterpret_cast<float4*>(a.part_o + at * kDim + col) = acc;
+      for (int s = at; s < slots; s += kLanes) {
+        const float2 p = ml[s];
+        const float f = exp2_fast(p.x - shift);
+        sum = fmaf(p.y, f, sum);
+        // A part without keys has no output: its factor is told apart from one that has underflowed.
+        ml[s].x = p.x == -INFINITY ? -1.0f : f;
+        if (p.x != -INFINITY) live = s + 1;
+      }
+#pragma unroll
+      for (int off = kLanes / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+      if (live > 0) atomicMax(&odd_keys[0], static_cast<uint32_t>(live));
+      if (at == 0 && r < w.count) {
+        scales[r] = sum != 0.0f ? 1.0f / sum : 0.0f;
+        if (a.lse != nullptr)
+          a.lse[cell(r)] = sum != 0.0f ? (top + log2f(sum)) * 0.69314718055994530942f : -INFINITY;
+      }
+    }
+    __syncthreads();
+    const int live_slots = static_cast<int>(odd_keys[0]);
+    // 16 pieces of parts under way at a time: of four rows where there are many, of one where there are few.
+    auto join_rows = [&](auto rows_at_once) {
+      constexpr int kR = decltype(rows_at_once)::value, kAhead = 16 / kR;
+      constexpr int kPieces = kDim / 4, kGroups = kThreads / kPieces;
+      const int col = threadIdx.x % kPieces * 4;
+      for (int r0 = threadIdx.x / kPieces * kR; r0 < w.count; r0 += kGroups * kR) {
+        float4 acc[kR];
+        const float* parts[kR];
+        auto add = [](float4& sum, const float4& v, float f) {
+          sum.x = fmaf(v.x, f, sum.x), sum.y = fmaf(v.y, f, sum.y);
+          sum.z = fmaf(v.z, f, sum.z), sum.w = fmaf(v.w, f, sum.w);
+        };
+#pragma unroll
+        for (int k = 0; k < kR; ++k) {
+          acc[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          parts[k] = a.part_o + cell(r0 + k) * a.slots * kDim + col;
+        }
+        for (int s0 = 0; s0 < live_slots; s0 += kAhead) {
+          float4 v[kR][kAhead];
+          float f[kR][kAhead];
+#pragma unroll
+          for (int k = 0; k < kR; ++k)
+#pragma unroll
+            for (int s = 0; s < kAhead; ++s) {
+              f[k][s] = r0 + k < w.count && s0 + s < live_slots ? factors[(r0 + k) * a.prefix_slots + s0 + s].x : -1.0f;
+              v[k][s] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+              if (!(f[k][s] < 0.0f)) v[k][s] = *reinterpret_cast<const float4*>(parts[k] + (s0 + s) * kDim);
+            }
+#pragma unroll
+          for (int k = 0; k < kR; ++k)
+#pragma unroll
+            for (int s = 0; s < kAhead; ++s) add(acc[k], v[k][s], f[k][s]);
+        }
+#pragma unroll
+        for (int k = 0; k < kR; ++k) {
+          const int r = r0 + k;
+          if (r >= w.count) break;
+#pragma unroll
+          for (int i = 0; i < kAlong; ++i)
+            add(acc[k], *reinterpret_cast<const float4*>(os + (i * kRows + r) * kDim + col), own[i * kRows + r]);
+          const int vr = w.start + r;
+          const float scale = scales[r];
+          __nv_bfloat16* out = a.out + static_cast<int64_t>(w.first_row + vr / a.group) * a.ldo +
+                               (w.kv_head * a.group + vr % a.group) * kDim + col;
+          *reinterpret_cast<uint2*>(out) =
+              make_uint2(pack2(acc[k].x * scale, acc[k].y * scale), pack2(acc[k].z * scale, acc[k].w * scale));
+        }
+      }
+    };
+    if (w.count > 16)
+      join_rows(std::integral_constant<int, 4>{});
+    else
+      join_rows(std::integral_constant<int, 1>{});
+  } else {
+    if (w.first)  // the slots that no block comes to
+      for (int c = threadIdx.x; c < w.count * (w.slots - w.used); c += kThreads)
+        a.part_ml[cell(c % w.count) * a.slots + w.used + c / w.count] = make_float2(-INFINITY, 0.0f);
+    if (w.key0 >= w.key1) {
+      for (int r = threadIdx.x; r < w.count; r += kThreads) a.part_ml[cell(r) * a.slots + w.slot] = make_float2(-INFINITY, 0.0f);
+      return;
+    }
+    if constexpr (kWarpRows == 4) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = row0 + gr + 8 * i;
+        if (r >= w.count) continue;
+        const int64_t at = cell(r) * a.slots + w.slot;
+        if (tq == 0) a.part_ml[at] = make_float2(m[i], l[i]);
+#pragma unroll
+        for (int d = 0; d < kDim / 8; ++d)
+          *reinterpret_cast<float2*>(a.part_o + at * kDim + d * 8 + 2 * tq) = make_float2(o[d][2 * i], o[d][2 * i + 1]);
+      }
+    } else {
+      // The warps along the keys are joined in shared memory, in the ring's place.
+      constexpr int kAlong = 4 / kWarpRows;
+      float* os = reinterpret_cast<float*>(raw);                    // [kAlong][kRows][kDim]
+      float2* mls = reinterpret_cast<float2*>(os + kAlong * kRows * kDim);  // [kAlong][kRows]
+      cp_async_wait_all();
+      __syncthreads();
+      const int along = warp / kWarpRows;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = row0 + gr + 8 * i;
+        if (tq == 0) mls[along * kRows + r] = make_float2(m[i], l[i]);
+#pragma unroll
+        for (int d = 0; d < kDim / 8; ++d)
+          *reinterpret_cast<float2*>(os + (along * kRows + r) * kDim + d * 8 + 2 * tq) =
+              make_float2(o[d][2 * i], o[d][2 * i + 1]);
+      }
+      __syncthreads();
+      for (int c = threadIdx.x; c < w.count * (kDim / 4); c += kThreads) {
+        const int r = c / (kDim / 4), col = c % (kDim / 4) * 4;
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kAlong; ++i) top = fmaxf(top, mls[i * kRows + r].x);
+        const float shift = top == -INFINITY ? 0.0f : top;
+        float sum = 0.0f;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int i = 0; i < kAlong; ++i) {
+          const float2 ml = mls[i * kRows + r];
+          const float f = exp2_fast(ml.x - shift);
+          const float4 v = *reinterpret_cast<const float4*>(os + (i * kRows + r) * kDim + col);
+          sum = fmaf(ml.y, f, sum);
+          acc.x = fmaf(v.x, f, acc.x), acc.y = fmaf(v.y, f, acc.y);
+          acc.z = fmaf(v.z, f, acc.z), acc.w = fmaf(v.w, f, acc.w);
+        }
+        const int64_t at = cell(r) * a.slots + w.slot;
+        if (col == 0) a.part_ml[at] = make_float2(top, sum);
+        *reinterpret_cast<float4*>(a.part_o + at * kDim + col) = acc;
+      }
     }
   }
 }
@@ -465,12 +601,67 @@ __global__ void __launch_bounds__(kThreads, kBlocks) attention_rows_kernel(Atten
     __syncthreads();  // the segment is known
     unit += seg.stages;
     if (kPrefixWarps == kOwnWarps || seg.own)
-      attend<kDim, kOwnWarps>(a, seg, raw, odd_keys);
+      attend<kDim, kOwnWarps, false>(a, seg, raw, odd_keys, false);
     else
-      attend<kDim, kPrefixWarps>(a, seg, raw, odd_keys);
+      attend<kDim, kPrefixWarps, false>(a, seg, raw, odd_keys, false);
     __syncthreads();  // the segment and the ring have been read
   }
   if (g.late_wait) pdl_wait();
+}
+
+// A block for all own keys of a tile of a sequence's rows, which also joins the
+// prefix's parts and writes the rows. Blocks: tiles of all sequences x heads.
+template <int kDim, int kWarps>
+__global__ void __launch_bounds__(kThreads, kBlocks) attention_last_kernel(Attention a, int late_wait) {
+  constexpr int kRows = 16 * kWarps;
+  extern __shared__ __align__(16) unsigned char raw[];
+  __shared__ uint32_t odd_keys[kKeys / 32];
+  __shared__ Segment seg;
+  if (!late_wait) pdl_wait();
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x;
+    int tile = blockIdx.x / a.kv_heads;
+    if (lane == 0) seg.count = 0;
+    __syncwarp();
+    auto take = [&](int b, int rows, int first_row, int local) {
+      const int len = a.capacity > 0 ? len_of(a, b) : 0;
+      seg.own = true;
+      seg.of = b;
+      seg.kv_head = blockIdx.x % a.kv_heads;
+      seg.first_row = first_row;
+      seg.start = local * kRows;
+      seg.count = min(kRows, rows * a.group - seg.start);
+      seg.limit0 = len - rows + 1;
+      seg.all_see = seg.limit0 + seg.start / a.group;
+      seg.key0 = 0;
+      seg.key1 = max(0, seg.limit0 + (seg.start + seg.count - 1) / a.group);  // the tile's last row sees the most
+    };
+    if (a.row_offsets == nullptr) {
+      const int each = (a.group + kRows - 1) / kRows;
+      if (lane == 0) take(tile / each, 1, tile / each, tile % each);
+    } else {
+      for (int b0 = 0; b0 < a.sequences; b0 += 32) {
+        int first = 0;
+        const int rows = b0 + lane < a.sequences ? rows_of(a, b0 + lane, &first) : 0;
+        const int tiles = (rows * a.group + kRows - 1) / kRows;
+        int upto = tiles;
+#pragma unroll
+        for (int off = 1; off < 32; off *= 2) {
+          const int other = __shfl_up_sync(0xffffffffu, upto, off);
+          if (lane >= off) upto += other;
+        }
+        const bool mine = tile < upto && tile >= upto - tiles;
+        if (mine) take(b0 + lane, rows, first, tile - (upto - tiles));
+        if (__any_sync(0xffffffffu, mine)) break;
+        tile -= __shfl_sync(0xffffffffu, upto, 31);
+      }
+    }
+  }
+  __syncthreads();
+  if (seg.count > 0)
+    attend<kDim, kWarps, true>(a, seg, raw, odd_keys, late_wait != 0);
+  else if (late_wait)
+    pdl_wait();
 }
 
 // kWarps warps join the parts of a (row, head): first all maxima and sums, a lane a part, then the outputs of the parts
@@ -571,10 +762,10 @@ struct Plan {
   int prefix_slots, own_slots;
   int prefix_warps, own_warps;  // of the kernel for few rows: warps side by side along the rows of a tile
   unsigned blocks;
+  bool whole_own;     // the own keys of a tile of rows by one block, which joins the prefix's parts to them
+  int64_t own_tiles;  // there can be
 };
 
-constexpr int kMaxPrefixSlots = 64, kMaxOwnSlots = 32, kMaxTcSlots = 128;
-static_assert(kMaxPrefixSlots + kMaxOwnSlots <= kMaxSlots && kMaxTcSlots + kMaxOwnSlots <= kMaxSlots, "");
 constexpr int kSms = 148;  // blocks of the tensor-core kernel, one an SM; correct on any number of SMs
 
 // A prefix with many rows is arithmetic, for the tensor cores.
@@ -595,7 +786,6 @@ Plan plan_of(const uocr_prefix_attention_args& a) {
   auto warps_for = [](int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; };
   p.prefix_warps = warps_for(a.rows * group / a.prefixes);
   p.own_warps = warps_for(a.rows * group / std::max<int64_t>(a.sequences, 1));
-  if (p.tc || a.prefix_capacity == 0) p.prefix_warps = p.own_warps;
   // The units there can be, by the capacities; with row offsets each sequence's (prefix's) last tile may be part empty.
   auto tiles = [&](int64_t count, int64_t each, int warps) {
     const int64_t tile = 16 * warps;
@@ -603,9 +793,12 @@ Plan plan_of(const uocr_prefix_attention_args& a) {
                                     : a.rows * group / tile + std::min(count, a.rows);
   };
   const int64_t prefix_stages = (a.prefix_capacity + kKeys - 1) / kKeys, own_stages = (a.capacity + kKeys - 1) / kKeys;
+  p.own_tiles = tiles(a.sequences, 1, p.own_warps);
+  // Own keys in parts only where few blocks would have many: a join less, and own parts that are not written and read.
+  p.whole_own = p.own_tiles * a.kv_heads >= kSms || own_stages <= 8;
   const int64_t units =
       a.kv_heads * ((p.tc ? 0 : tiles(a.prefixes, a.sequences / a.prefixes, p.prefix_warps) * prefix_stages) +
-                    tiles(a.sequences, 1, p.own_warps) * own_stages);
+                    (p.whole_own ? 0 : p.own_tiles * own_stages));
   p.blocks = static_cast<unsigned>(std::min<int64_t>(units, kBlocks * kSms));
   // A range of keys meets as many blocks as shares fit into it, and one more; half as many again for lengths that differ.
   const int64_t share = std::max<int64_t>((units + kBlocks * kSms - 1) / (kBlocks * kSms), 1);
@@ -613,7 +806,7 @@ Plan plan_of(const uocr_prefix_attention_args& a) {
     return static_cast<int>(stages == 0 ? 0 : std::min<int64_t>((stages + share - 1) / share * 3 / 2 + 2, most));
   };
   p.prefix_slots = slots(prefix_stages, kMaxPrefixSlots);
-  p.own_slots = slots(own_stages, kMaxOwnSlots);
+  p.own_slots = p.whole_own ? 0 : slots(own_stages, kMaxOwnSlots);
   if (p.tc) {
     p.split = a.rows * group <= kAttentionTcRows * a.prefixes;
     const int64_t of_range = kAttentionTcRows * (p.split ? 1 : 2);
@@ -634,15 +827,25 @@ cudaError_t launch_rows(const Attention& a, const Grid& g, unsigned blocks, cuda
   return launch_pdl(attention_rows_kernel<kDim, kPrefixWarps, kOwnWarps>, blocks, kThreads, kRing, stream, a, g);
 }
 
+template <int kDim, int kWarps>
+cudaError_t launch_last(const Attention& a, unsigned blocks, int late_wait, cudaStream_t stream) {
+  constexpr size_t kRing = static_cast<size_t>(kStages) * 2 * kKeys * (kDim + 8) * 2;
+  const size_t join = 64 * (kDim * 4 + 8 + 4) + 16 * kWarps * (4 + a.prefix_slots * 8);
+  cudaError_t st = allow_max_dynamic_smem(attention_last_kernel<kDim, kWarps>);
+  if (st != cudaSuccess) return st;
+  return launch_pdl(attention_last_kernel<kDim, kWarps>, blocks, kThreads, std::max(kRing, join), stream, a, late_wait);
+}
+
 template <int kDim>
 cudaError_t launch(const uocr_prefix_attention_args& args, const Attention& a, const Plan& p, cudaStream_t stream) {
   Grid g{};
   g.prefixes = p.tc || args.prefix_capacity == 0 ? 0 : a.prefixes;
-  g.sequences = args.capacity == 0 ? 0 : a.sequences;
+  g.sequences = args.capacity == 0 || p.whole_own ? 0 : a.sequences;
   g.late_wait = p.tc;
   cudaError_t st = p.tc ? launch_attention_tc(a, kDim, kSms, stream) : cudaSuccess;
   if (st == cudaSuccess && p.blocks > 0) {
-    switch (p.prefix_warps * 8 + p.own_warps) {
+    const int own = g.sequences == 0 ? p.prefix_warps : p.own_warps;
+    switch ((g.prefixes == 0 ? own : p.prefix_warps) * 8 + own) {
       case 8 + 1: st = launch_rows<kDim, 1, 1>(a, g, p.blocks, stream); break;
       case 16 + 1: st = launch_rows<kDim, 2, 1>(a, g, p.blocks, stream); break;
       case 16 + 2: st = launch_rows<kDim, 2, 2>(a, g, p.blocks, stream); break;
@@ -652,6 +855,13 @@ cudaError_t launch(const uocr_prefix_attention_args& args, const Attention& a, c
     }
   }
   if (st != cudaSuccess) return st;
+  if (p.whole_own) {
+    const int late = p.tc || p.blocks > 0;
+    const unsigned n = static_cast<unsigned>(p.own_tiles * a.kv_heads);
+    return p.own_warps == 1   ? launch_last<kDim, 1>(a, n, late, stream)
+           : p.own_warps == 2 ? launch_last<kDim, 2>(a, n, late, stream)
+                              : launch_last<kDim, 4>(a, n, late, stream);
+  }
   // Few rows: all warps of a block on one, for the round trips of its parts.
   const int64_t cells = args.rows * args.heads, each = kThreads / 32;
   if (cells <= 4 * kSms)

@@ -152,6 +152,13 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return r;
 }
 
+// The greatest of three; NaN where one is.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 struct __align__(8) TcBarriers {
   uint64_t full[kSlots];
   uint64_t empty[kSlots];
@@ -230,7 +237,7 @@ __device__ __forceinline__ Schedule make_schedule(const Attention& a) {
   most = __reduce_max_sync(0xffffffffu, most);
   // No range of keys meets more blocks than there are slots for (two of a block that splits the keys).
   const unsigned blocks = a.split ? a.prefix_slots / 2 : a.prefix_slots;
-  c.share = max(max((total + gridDim.x - 1) / gridDim.x, (most + blocks - 2) / (blocks - 1)), 1u);
+  c.share = max(max((total + gridDim.x - 1) / gridDim.x, (most + blocks - 2) / (blocks - 1)), 2u);
   c.unit = min(total, blockIdx.x * c.share);
   c.end = min(total, c.unit + c.share);
   return c;
@@ -523,19 +530,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
             for (int c = 0; c < kTcKeys; ++c)
               if (c < skip) x[c] = __float_as_uint(-INFINITY);
           }
-          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          float top[4];
 #pragma unroll
-          for (int c = 0; c < kTcKeys; c += 8)
+          for (int e = 0; e < 4; ++e) top[e] = __uint_as_float(x[e]);
+#pragma unroll
+          for (int c = 4; c < kTcKeys; c += 8)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              top[e] = fmaxf(top[e], fmaxf(__uint_as_float(x[c + e]), __uint_as_float(x[c + 4 + e])));
-          const float peak = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+              top[e] = max3_nan(top[e], __uint_as_float(x[c + e]),
+                                __uint_as_float(x[c + 4 + e < kTcKeys ? c + 4 + e : c + e]));
+          const float peak = max3_nan(max3_nan(top[0], top[1], top[2]), top[3], top[3]);
           if (i == 0) {
             m = peak;
           } else {
-            const bool moves = (peak - m) * a.scale_log2 > kSlack;  // also where m is -inf
+            const bool moves = !((peak - m) * a.scale_log2 <= kSlack) && peak != m;  // also where m is -inf or one is NaN
             if (__any_sync(0xffffffffu, moves)) {
-              const float to = fmaxf(m, peak);
+              const float to = max3_nan(m, peak, peak);  // NaN: every weight of the row becomes one
               const float f = to == m ? 1.0f : exp2_fast((m - to) * a.scale_log2);
               m = to;
               l *= f;
