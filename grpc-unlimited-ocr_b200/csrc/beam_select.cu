@@ -1,16 +1,19 @@
 // The best continuations of a group of beams (uocr_beam_select).
 //
 // score(b, t) = scores[b] + logit - (m + log sum exp(logit - m)): within a beam
-// the order is the logits' own, so one pass over a row is enough: a block keeps
-// a chunk of a row in registers, takes its maximum, its sum of exponentials and
-// its `select` best logits; a second kernel joins a group's chunks. Bound: the
-// one read of the logits; for few rows two launches and their rounds.
+// the order is the logits' own, so one pass over a row is enough: a block goes
+// through a part of a row, keeps the maximum, the sum of exponentials and the
+// `select` best logits; a second kernel joins a group's parts. Bound: the one
+// read of the logits; for few rows two launches and their rounds.
 //
-// The best of a chunk without sorting it: the select-th best of the threads'
-// own maxima, taken warp by warp, bounds the select-th best of all from below,
-// which leaves a few dozen elements to rank against one another. Keys are
-// unique (value, then the lower index), so the result is the exact one, ties
-// included, in every case.
+// The best of a part without sorting it: the select-th best of the threads' own
+// maxima, taken warp by warp, bounds the select-th best of all from below. What
+// reaches the bound goes on a list; where that grows the bound is drawn anew from
+// it, higher, so that soon hardly an element passes; what is left at the end, a
+// few dozen, is ranked. Keys are unique (value, then the lower index), so the
+// result is the exact one, ties included, in every case.
+#include <algorithm>
+
 #include "beam.h"
 #include "ptx.cuh"
 #include "w8a8.h"
@@ -18,9 +21,22 @@
 namespace uocr_b200 {
 namespace {
 
+constexpr float kLog2e = 1.4426950408889634f;
+
+// 2^x to 2 ulp; 2^-inf = 0.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kRefine = 256;  // survivors above this are thinned out once more before they are ranked
+constexpr int kEach = 16;     // elements of a thread and round
+constexpr int kRound = kThreads * kEach;
+constexpr int kRanked = 512;  // as many keys are ranked against one another; more are thinned out first
+constexpr int kList = kRound + 2 * UOCR_BEAM_MAX + 64;  // what a round may leave (list_limit), and one round
+__device__ __forceinline__ int list_limit(int select) { return 2 * select + 64; }
 
 // Floats in their order as unsigned integers; 0 stands for no candidate.
 __device__ __forceinline__ uint32_t ordered(float f) {
@@ -72,110 +88,170 @@ struct Select {
   const float* scores;
   const int* finished;
   int64_t ld;
-  int vocab, beams, select, chunks;
+  int vocab, beams, select;
+  int parts, part;  // of a row; elements of a part, a multiple of kRound
   bool vec;         // rows allow 16 bytes at a time
-  float2* sums;     // [rows, chunks]: maximum and sum of exponentials
-  uint64_t* best;   // [rows, chunks, select] keys, descending
+  float2* sums;     // [rows, parts]: maximum m, and sum of 2^(f log2 e - fl(m log2 e))
+  uint64_t* best;   // [rows, parts, select] keys, descending
 };
 
-template <typename T, int kEach>
-__global__ void __launch_bounds__(kThreads) beam_chunks_kernel(Select a) {
-  constexpr int kVec = 16 / sizeof(T);
-  extern __shared__ uint64_t list[];  // [kWarps * select * kEach]: no warp has more than `select` threads at the bound
-  __shared__ uint64_t bounds[2 * kWarps];
-  __shared__ float part[kWarps];
-  __shared__ int count, next;
-  pdl_wait();
-  pdl_launch_dependents();
-  const int64_t row = blockIdx.x / a.chunks;
-  const int chunk = blockIdx.x % a.chunks;
-  // The second kernel asks for nothing of a beam that has ended or does not exist.
-  if ((a.finished != nullptr && a.finished[row] != 0) || !(a.scores[row] > -INFINITY)) return;
-  if (threadIdx.x == 0) count = 0;
-  const T* src = static_cast<const T*>(a.logits) + row * a.ld;
-  const int base = chunk * (kThreads * kEach);
-  float f[kEach];
-  float peak = -INFINITY;
-  int peak_at = 0;
-#pragma unroll
-  for (int j = 0; j < kEach / kVec; ++j) {
-    const int at = base + (j * kThreads + static_cast<int>(threadIdx.x)) * kVec;
-    float* g = f + j * kVec;
-    if (a.vec && at + kVec <= a.vocab) {
-      const uint4 u = *reinterpret_cast<const uint4*>(src + at);
-      const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) g[i] = to_f32(e[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) g[i] = at + i < a.vocab ? to_f32(src[at + i]) : -INFINITY;
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    if (!(f[i] > -INFINITY)) f[i] = -INFINITY;  // NaN
-    if (f[i] > peak) {
-      peak = f[i];
-      peak_at = i;
-    }
-  }
-  auto index = [&](int i) {
-    return static_cast<uint32_t>(base + (i / kVec * kThreads + static_cast<int>(threadIdx.x)) * kVec + i % kVec);
-  };
-  uint64_t top;
-  uint64_t bound = bound_of(key_of(peak, index(peak_at)), a.select, bounds, &top);
-  const float m = top != 0 ? unordered(static_cast<uint32_t>(top >> 32)) : 0.0f;
-  const float at_least = unordered(max(static_cast<uint32_t>(bound >> 32), ordered(-INFINITY)));
-  float sum = 0.0f;
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    sum += __expf(f[i] - m);
-    if (f[i] >= at_least) {
-      const uint64_t key = key_of(f[i], index(i));
-      if (key >= bound) list[atomicAdd(&count, 1)] = key;
-    }
-  }
-  sum = warp_sum(sum);
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = sum;
-  __syncthreads();
-  int n = count;
-  const int64_t cell = row * a.chunks + chunk;
-  if (threadIdx.x == 0) {
-    float s = 0.0f;
-    for (int w = 0; w < kWarps; ++w) s += part[w];
-    a.sums[cell] = make_float2(top != 0 ? m : -INFINITY, top != 0 ? s : 0.0f);
-  }
-  // Many survivors (large values side by side in few threads): dealt out anew, bounded again. In place: what a
-  // thread keeps it has in registers. Ends when a round removes less than a fifth.
-  for (int before = n + n; n > kRefine && n * 5 < before * 4; ) {
-    constexpr int kMost = kEach;  // list entries a thread: kWarps * 32 * kEach / kThreads
+// Cuts the list to its `select` best, in order, and returns the last of them (1:
+// there are fewer), which all that still can be among the best reach. All threads
+// call it, behind a barrier. `best`: UOCR_BEAM_MAX keys.
+__device__ uint64_t cut(uint64_t* list, int* count, int* next, int select, uint64_t* bounds, uint64_t* best) {
+  int n = *count;
+  // Many: those that reach a bound, drawn like the first one, unless that removes next to nothing. In place: what a
+  // thread keeps it has in registers.
+  for (int before = 2 * n; n > kRanked && n * 5 < before * 4;) {
+    constexpr int kMost = (kList + kThreads - 1) / kThreads;
     uint64_t mine[kMost];
-    uint64_t high = 0;
+    uint64_t high = 0, top;
 #pragma unroll
     for (int i = 0; i < kMost; ++i) {
       const int at = i * kThreads + static_cast<int>(threadIdx.x);
       mine[i] = at < n ? list[at] : 0;
       high = max(high, mine[i]);
     }
-    if (threadIdx.x == 0) next = 0;
-    __syncthreads();
-    bound = bound_of(high, a.select, bounds, &top);
+    if (threadIdx.x == 0) *next = 0;
+    const uint64_t bound = bound_of(high, select, bounds, &top);
 #pragma unroll
     for (int i = 0; i < kMost; ++i)
-      if (mine[i] >= bound) list[atomicAdd(&next, 1)] = mine[i];
+      if (mine[i] >= bound) list[atomicAdd(next, 1)] = mine[i];
     __syncthreads();
     before = n;
-    n = next;
+    n = *next;
     __syncthreads();
   }
-  uint64_t* out = a.best + cell * a.select;
+#pragma unroll 1
   for (int i = threadIdx.x; i < n; i += kThreads) {
     const uint64_t key = list[i];
     int rank = 0;
-    for (int j = 0; j < n && rank < a.select; ++j) rank += list[j] > key;
-    if (rank < a.select) out[rank] = key;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) rank += list[j] > key;
+    if (rank < select) best[rank] = key;
   }
-  for (int i = n + threadIdx.x; i < a.select; i += kThreads) out[i] = 0;
+  __syncthreads();
+  n = min(n, select);
+  if (static_cast<int>(threadIdx.x) < n) list[threadIdx.x] = best[threadIdx.x];
+  if (threadIdx.x == 0) *count = n;
+  const uint64_t last = n == select ? best[select - 1] : 1;
+  __syncthreads();
+  return last;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 3) beam_parts_kernel(Select a) {
+  constexpr int kVec = 16 / sizeof(T);
+  extern __shared__ uint64_t list[];  // [kList]
+  __shared__ uint64_t bounds[2 * kWarps];
+  __shared__ float2 warp_sums[kWarps];
+  __shared__ uint64_t best[UOCR_BEAM_MAX];
+  __shared__ int count, next;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int64_t row = blockIdx.x / a.parts;
+  const int part = blockIdx.x % a.parts;
+  // The second kernel asks for nothing of a beam that has ended or does not exist.
+  if ((a.finished != nullptr && a.finished[row] != 0) || !(a.scores[row] > -INFINITY)) return;
+  if (threadIdx.x == 0) count = 0;
+  const T* src = static_cast<const T*>(a.logits) + row * a.ld;
+  const int begin = part * a.part, end = min(a.vocab, begin + a.part);
+  float m = -INFINITY, sum = 0.0f;  // of this thread
+  uint64_t bound = 0;
+  float at_least = -INFINITY;
+  auto load = [&](int base, float* f) {
+#pragma unroll
+    for (int j = 0; j < kEach / kVec; ++j) {
+      const int at = base + (j * kThreads + static_cast<int>(threadIdx.x)) * kVec;
+      float* g = f + j * kVec;
+      if (a.vec && at + kVec <= end) {
+        const uint4 u = *reinterpret_cast<const uint4*>(src + at);
+        const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) g[i] = to_f32(e[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) g[i] = at + i < end ? to_f32(src[at + i]) : -INFINITY;
+      }
+    }
+  };
+  float ahead[kEach];
+  load(begin, ahead);
+  for (int base = begin; base < end; base += kRound) {
+    float f[kEach];
+    float peak = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      f[i] = fmaxf(ahead[i], -INFINITY);  // NaN counts as -inf
+      peak = fmaxf(peak, f[i]);
+    }
+    if (base + kRound < end) load(base + kRound, ahead);
+    if (peak > m) {
+      sum *= exp2_fast(m * kLog2e - peak * kLog2e);  // of no element yet: 0 * 0
+      m = peak;
+    }
+    // 2^(f log2 e - m log2 e), the second product rounded for all elements alike: the join takes it as it is.
+    const float shift = m > -INFINITY ? m * kLog2e : 0.0f;
+    float of_round = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) of_round += exp2_fast(fmaf(f[i], kLog2e, -shift));
+    sum += of_round;
+    auto index = [&](int i) {
+      return static_cast<uint32_t>(base + (i / kVec * kThreads + static_cast<int>(threadIdx.x)) * kVec + i % kVec);
+    };
+    if (bound == 0) {
+      uint64_t first = 0, top;
+#pragma unroll
+      for (int i = kEach - 1; i >= 0; --i)
+        if (f[i] == peak) first = key_of(f[i], index(i));
+      bound = bound_of(first, a.select, bounds, &top);
+      at_least = unordered(max(static_cast<uint32_t>(bound >> 32), ordered(-INFINITY)));
+    }
+    unsigned reach = 0;
+    if (peak >= at_least) {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) reach |= f[i] >= at_least ? 1u << i : 0u;
+    }
+    while (reach != 0) {  // one branch for the few threads that have any
+      const int i = __ffs(reach) - 1;
+      reach &= reach - 1;
+      float v = f[0];
+#pragma unroll
+      for (int k = 1; k < kEach; ++k) v = i == k ? f[k] : v;
+      const uint64_t key = key_of(v, index(i));
+      if (key >= bound) list[atomicAdd(&count, 1)] = key;
+    }
+    __syncthreads();
+    // The bound is drawn anew when the list grows, at once after the first round: from then on few elements pass.
+    if (count > list_limit(a.select)) {
+      bound = max(bound, cut(list, &count, &next, a.select, bounds, best));
+      at_least = unordered(max(static_cast<uint32_t>(bound >> 32), ordered(-INFINITY)));
+    } else {
+      __syncthreads();  // the count has been read by all
+    }
+  }
+  // The block's maximum and sum.
+  float top = m;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+  sum = warp_sum(m > -INFINITY ? sum * exp2_fast(m * kLog2e - top * kLog2e) : 0.0f);
+  if ((threadIdx.x & 31) == 0) warp_sums[threadIdx.x >> 5] = make_float2(top, sum);
+  __syncthreads();
+  const int64_t cell = row * a.parts + part;
+  if (threadIdx.x == 0) {
+    float2 all = warp_sums[0];
+    for (int w = 1; w < kWarps; ++w) {
+      const float2 p = warp_sums[w];
+      const float high = fmaxf(all.x, p.x);
+      if (high == -INFINITY) continue;
+      all = make_float2(high, all.y * exp2_fast(all.x * kLog2e - high * kLog2e) +
+                                  p.y * exp2_fast(p.x * kLog2e - high * kLog2e));
+    }
+    a.sums[cell] = all;
+  }
+  cut(list, &count, &next, a.select, bounds, best);
+  if (static_cast<int>(threadIdx.x) < a.select)
+    a.best[cell * a.select + threadIdx.x] = static_cast<int>(threadIdx.x) < count ? list[threadIdx.x] : 0;
 }
 
 struct Join {
@@ -187,88 +263,129 @@ struct Join {
   int eos;
 };
 
-// A candidate in the order of the selection: the score, then the lower beam and token.
+// A candidate in the order of the selection: the score, then the lower beam and
+// token. The 64-bit score as an integer in the same order, which compares in two
+// instructions where doubles took ten times as long; 0: no candidate.
 struct Cand {
-  double score;
+  uint64_t score;
   uint64_t flat;  // beam << 32 | token
 };
+__device__ __forceinline__ uint64_t ordered64(double v) {
+  const uint64_t u = static_cast<uint64_t>(__double_as_longlong(v));
+  return u >> 63 ? ~u : u | 0x8000000000000000ull;
+}
+__device__ __forceinline__ float score_of(const Cand& c) {
+  const uint64_t u = c.score >> 63 ? c.score & 0x7fffffffffffffffull : ~c.score;
+  return static_cast<float>(__longlong_as_double(static_cast<long long>(u)));
+}
 __device__ __forceinline__ bool better(const Cand& a, const Cand& b) {
-  return a.score > b.score || (a.score == b.score && a.flat < b.flat);
+  return (a.score > b.score) | ((a.score == b.score) & (a.flat < b.flat));  // no branch
 }
 
-// A block joins a group. Only the chunks with the `select` best first entries
-// can hold any of the `select` best candidates, and of those only the entries
-// that are not below the select-th best first entry.
-__global__ void __launch_bounds__(kThreads) beam_join_kernel(Join a) {
-  extern __shared__ Cand heads[];  // [beams * chunks], then [select * select]
+// What a part's exponents are less (its maximum in the log2 domain, as rounded there).
+__device__ __forceinline__ double shift_of(float m) { return static_cast<double>(m * kLog2e); }
+
+constexpr int kJoinThreads = 512;
+constexpr int kLanes = 4;  // neighbouring threads that rank a candidate
+
+// How many of the n candidates are better than `mine`.
+__device__ __forceinline__ int rank_of(const Cand& mine, const Cand* of, int n) {
+  int rank = 0;
+#pragma unroll 4
+  for (int j = threadIdx.x % kLanes; j < n; j += kLanes) rank += better(of[j], mine) ? 1 : 0;
+  rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+  return rank + __shfl_xor_sync(0xffffffffu, rank, 2);
+}
+
+// A block joins a group. Only the parts with the `select` best first entries can
+// hold any of the `select` best candidates, and of those only the entries that are
+// not below the select-th best first entry. Everything of the group is read in one
+// round, the keys too where they fit (kStage).
+template <bool kStaged>
+__global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(Join a) {
+  extern __shared__ Cand heads[];  // [beams * parts], then [select * select], then the keys
   __shared__ double lse[UOCR_BEAM_MAX];
+  __shared__ float scores[UOCR_BEAM_MAX];
+  __shared__ int ended[UOCR_BEAM_MAX];
   __shared__ Cand worst;
   __shared__ int lists[UOCR_BEAM_MAX];
   __shared__ int chosen, count;
   const Select& s = a.s;
-  const int n = s.beams * s.chunks;
+  const int n = s.beams * s.parts;
   Cand* left = heads + n;
+  uint64_t* staged = reinterpret_cast<uint64_t*>(left + s.select * s.select);
   pdl_wait();
   pdl_launch_dependents();
   const int64_t group = blockIdx.x, first = group * s.beams;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint64_t* keys = s.best + first * s.parts * s.select;
+  if (kStaged)
+    for (int i = threadIdx.x; i < n * s.select; i += kJoinThreads) staged[i] = keys[i];
   if (threadIdx.x == 0) chosen = count = 0;
-  for (int b = warp; b < s.beams; b += kWarps) {
+  for (int b = warp; b < s.beams; b += kJoinThreads / 32) {
     const float score = s.scores[first + b];
-    const bool ended = s.finished != nullptr && s.finished[first + b] != 0;
+    const bool done = s.finished != nullptr && s.finished[first + b] != 0;
     double value = INFINITY;  // no candidates
-    if (!ended && score > -INFINITY) {
+    if (!done && score > -INFINITY) {
       float m = -INFINITY;
-      for (int c = lane; c < s.chunks; c += 32) m = fmaxf(m, s.sums[(first + b) * s.chunks + c].x);
-#pragma unroll
-      for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
       double sum = 0.0;
-      for (int c = lane; c < s.chunks; c += 32) {
-        const float2 p = s.sums[(first + b) * s.chunks + c];
-        if (p.x > -INFINITY) sum += static_cast<double>(p.y) * exp(static_cast<double>(p.x) - m);
-      }
+      for (int c0 = 0; c0 < s.parts; c0 += 32) {
+        const float2 p = c0 + lane < s.parts ? s.sums[(first + b) * s.parts + c0 + lane] : make_float2(-INFINITY, 0.0f);
+        float high = fmaxf(m, p.x);
 #pragma unroll
-      for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-      value = m > -INFINITY && m < INFINITY ? m + log(sum) : INFINITY;
+        for (int off = 16; off > 0; off >>= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, off));
+        if (high == -INFINITY) continue;
+        double all = p.x > -INFINITY ? static_cast<double>(p.y) * exp2(shift_of(p.x) - shift_of(high)) : 0.0;
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) all += __shfl_xor_sync(0xffffffffu, all, off);
+        sum = all + (m > -INFINITY ? sum * exp2(shift_of(m) - shift_of(high)) : 0.0);
+        m = high;
+      }
+      if (m > -INFINITY && m < INFINITY) value = (shift_of(m) + log2(sum)) * 0.69314718055994530942;
     }
-    if (lane == 0) lse[b] = value;
+    if (lane == 0) {
+      lse[b] = value;
+      scores[b] = score;
+      ended[b] = done;
+    }
   }
   __syncthreads();
-  // Entry `at` of list `i` (a beam's chunk, or the one candidate of a beam that has ended).
+  // Entry `at` of list `i` (a beam's part, or the one candidate of a beam that has ended).
   auto entry = [&](int i, int at) {
-    const int b = i / s.chunks, c = i % s.chunks;
-    const float score = s.scores[first + b];
-    Cand e{-INFINITY, ~0ull};
-    if (s.finished != nullptr && s.finished[first + b] != 0) {
-      if (c == 0 && at == 0 && score > -INFINITY) {
-        e.score = score;
+    const int b = i / s.parts;
+    const float score = scores[b];
+    Cand e{0, ~0ull};
+    if (ended[b]) {
+      if (i == b * s.parts && at == 0 && score > -INFINITY) {
+        e.score = ordered64(score);
         e.flat = static_cast<uint64_t>(b) << 32 | static_cast<uint32_t>(max(a.eos, 0));
       }
     } else if (lse[b] < INFINITY) {
-      const uint64_t key = s.best[((first + b) * s.chunks + c) * s.select + at];
-      const double v = static_cast<double>(score) + (static_cast<double>(unordered(static_cast<uint32_t>(key >> 32))) - lse[b]);
+      const uint64_t key = kStaged ? staged[i * s.select + at] : keys[static_cast<int64_t>(i) * s.select + at];
+      const double v =
+          static_cast<double>(score) + (static_cast<double>(unordered(static_cast<uint32_t>(key >> 32))) - lse[b]);
       if (key != 0 && v > -INFINITY) {
-        e.score = v;
+        e.score = ordered64(v);
         e.flat = static_cast<uint64_t>(b) << 32 | (0xffffffffu - static_cast<uint32_t>(key));
       }
     }
     return e;
   };
-  for (int i = threadIdx.x; i < n; i += kThreads) heads[i] = entry(i, 0);
+  for (int i = threadIdx.x; i < n; i += kJoinThreads) heads[i] = entry(i, 0);
   __syncthreads();
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const Cand mine = heads[i];
-    if (mine.flat == ~0ull) continue;
-    int rank = 0;
-    for (int j = 0; j < n && rank < s.select; ++j) rank += better(heads[j], mine);
+  for (int i0 = 0; i0 < n; i0 += kJoinThreads / kLanes) {
+    const int i = i0 + threadIdx.x / kLanes;
+    const Cand mine = i < n ? heads[i] : Cand{0, ~0ull};
+    const int rank = rank_of(mine, heads, n);
+    if (mine.score == 0 || threadIdx.x % kLanes != 0) continue;
     if (rank < s.select) lists[atomicAdd(&chosen, 1)] = i;
     if (rank == s.select - 1) worst = mine;
   }
   __syncthreads();
   const bool full = chosen == s.select;
-  for (int i = threadIdx.x; i < chosen * s.select; i += kThreads) {
+  for (int i = threadIdx.x; i < chosen * s.select; i += kJoinThreads) {
     const Cand e = entry(lists[i / s.select], i % s.select);
-    if (e.flat != ~0ull && !(full && better(worst, e))) left[atomicAdd(&count, 1)] = e;
+    if (e.score != 0 && !(full && better(worst, e))) left[atomicAdd(&count, 1)] = e;
   }
   __syncthreads();
   const int m = count;
@@ -279,48 +396,51 @@ __global__ void __launch_bounds__(kThreads) beam_join_kernel(Join a) {
     a.new_scores[at] = score;
     if (a.new_finished != nullptr) a.new_finished[at] = done ? 1 : 0;
   };
-  for (int i = threadIdx.x; i < m; i += kThreads) {
-    const Cand mine = left[i];
-    int rank = 0;
-    for (int j = 0; j < m && rank < s.select; ++j) rank += better(left[j], mine);
-    if (rank >= s.select) continue;
+  for (int i0 = 0; i0 < m; i0 += kJoinThreads / kLanes) {
+    const int i = i0 + threadIdx.x / kLanes;
+    const Cand mine = i < m ? left[i] : Cand{0, ~0ull};
+    const int rank = rank_of(mine, left, m);
+    if (mine.score == 0 || threadIdx.x % kLanes != 0 || rank >= s.select) continue;
     const int b = static_cast<int>(mine.flat >> 32), token = static_cast<int>(mine.flat & 0xffffffffu);
-    const bool ended = s.finished != nullptr && s.finished[first + b] != 0;
-    put(rank, token, b, static_cast<float>(mine.score), ended || token == a.eos);
+    put(rank, token, b, score_of(mine), ended[b] || token == a.eos);
   }
-  for (int i = m + threadIdx.x; i < s.select; i += kThreads) put(i, max(a.eos, 0), 0, -INFINITY, true);
+  for (int i = m + threadIdx.x; i < s.select; i += kJoinThreads) put(i, max(a.eos, 0), 0, -INFINITY, true);
 }
 
-constexpr int kEachMost = 32;
-
-int chunk_each(const uocr_beam_select_args& a) {
-  // Few rows: smaller chunks, so that more SMs read.
-  return a.batch * a.beams * ((a.vocab + kThreads * 16 - 1) / (kThreads * 16)) <= 592 ? 16 : kEachMost;
+// Elements of a part, whole rounds: as many parts as there are blocks on the SMs at a time (three each), so that none
+// waits for another.
+int part_of(const uocr_beam_select_args& a) {
+  const int64_t rows = std::max<int64_t>(a.batch * a.beams, 1);
+  const int64_t parts = std::max<int64_t>(3 * 148 / rows, 1);
+  const int64_t rounds = (a.vocab + kRound - 1) / kRound;
+  return static_cast<int>((rounds + parts - 1) / parts) * kRound;
+}
+int parts_of(const uocr_beam_select_args& a) {
+  const int64_t part = part_of(a);
+  return static_cast<int>((a.vocab + part - 1) / part);
 }
 
-int chunks_of(const uocr_beam_select_args& a) {
-  const int64_t each = static_cast<int64_t>(chunk_each(a)) * kThreads;
-  return static_cast<int>((a.vocab + each - 1) / each);
-}
-
-template <typename T, int kEach>
+template <typename T>
 cudaError_t launch(const uocr_beam_select_args& a, const Join& j, cudaStream_t stream) {
-  const size_t smem = static_cast<size_t>(kWarps) * j.s.select * kEach * sizeof(uint64_t);
-  const size_t join_smem = (static_cast<size_t>(j.s.beams) * j.s.chunks + j.s.select * j.s.select) * sizeof(Cand);
-  cudaError_t st = allow_max_dynamic_smem(beam_chunks_kernel<T, kEach>);
-  if (st == cudaSuccess) st = allow_max_dynamic_smem(beam_join_kernel);
+  const size_t keys = static_cast<size_t>(j.s.beams) * j.s.parts * j.s.select * sizeof(uint64_t);
+  const size_t join_smem = (static_cast<size_t>(j.s.beams) * j.s.parts + j.s.select * j.s.select) * sizeof(Cand);
+  const bool staged = keys <= 64 * 1024;
+  cudaError_t st = allow_max_dynamic_smem(beam_parts_kernel<T>);
+  if (st == cudaSuccess) st = allow_max_dynamic_smem(beam_join_kernel<true>);
+  if (st == cudaSuccess) st = allow_max_dynamic_smem(beam_join_kernel<false>);
   if (st == cudaSuccess)
-    st = launch_pdl(beam_chunks_kernel<T, kEach>, static_cast<unsigned>(a.batch * a.beams * j.s.chunks), kThreads, smem,
-                    stream, j.s);
+    st = launch_pdl(beam_parts_kernel<T>, static_cast<unsigned>(a.batch * a.beams * j.s.parts), kThreads,
+                    kList * sizeof(uint64_t), stream, j.s);
   if (st == cudaSuccess)
-    st = launch_pdl(beam_join_kernel, static_cast<unsigned>(a.batch), kThreads, join_smem, stream, j);
+    st = launch_pdl(staged ? beam_join_kernel<true> : beam_join_kernel<false>, static_cast<unsigned>(a.batch), kJoinThreads,
+                    join_smem + (staged ? keys : 0), stream, j);
   return st;
 }
 
 }  // namespace
 
 size_t beam_select_bytes(const uocr_beam_select_args& a) {
-  return static_cast<size_t>(a.batch * a.beams) * chunks_of(a) * (sizeof(float2) + a.select * sizeof(uint64_t));
+  return static_cast<size_t>(a.batch * a.beams) * parts_of(a) * (sizeof(float2) + a.select * sizeof(uint64_t));
 }
 
 cudaError_t launch_beam_select(const uocr_beam_select_args& a, cudaStream_t stream) {
@@ -329,18 +449,16 @@ cudaError_t launch_beam_select(const uocr_beam_select_args& a, cudaStream_t stre
   s.logits = a.logits, s.scores = a.scores, s.finished = a.finished;
   s.ld = a.ld_logits;
   s.vocab = static_cast<int>(a.vocab), s.beams = static_cast<int>(a.beams), s.select = static_cast<int>(a.select);
-  s.chunks = chunks_of(a);
+  s.parts = parts_of(a);
+  s.part = part_of(a);
   const size_t eb = a.dtype == UOCR_DTYPE_BF16 ? 2 : 4;
   s.vec = reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 && a.ld_logits * eb % 16 == 0;
-  const size_t cells = static_cast<size_t>(a.batch * a.beams) * s.chunks;
+  const size_t cells = static_cast<size_t>(a.batch * a.beams) * s.parts;
   s.best = static_cast<uint64_t*>(a.workspace);
   s.sums = reinterpret_cast<float2*>(s.best + cells * a.select);
   j.tokens = a.tokens, j.parents = a.parents, j.new_scores = a.new_scores, j.new_finished = a.new_finished;
   j.eos = a.eos;
-  const bool small = chunk_each(a) == 16;
-  if (a.dtype == UOCR_DTYPE_BF16)
-    return small ? launch<__nv_bfloat16, 16>(a, j, stream) : launch<__nv_bfloat16, kEachMost>(a, j, stream);
-  return small ? launch<float, 16>(a, j, stream) : launch<float, kEachMost>(a, j, stream);
+  return a.dtype == UOCR_DTYPE_BF16 ? launch<__nv_bfloat16>(a, j, stream) : launch<float>(a, j, stream);
 }
 
 }  // namespace uocr_b200

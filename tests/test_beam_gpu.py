@@ -6,10 +6,11 @@ itself, its root by half of that; rsqrt, the mean, the products with gain,
 cosine and sine and the magnitude add 8 roundings of 2^-24 and the 2 ulp of
 rsqrt and of sine and cosine; the angle, reduced to a turn in 64 bits, is off by
 2^-25 turns, 2^-22.3 of a full amplitude. 2^-15 of the pair's amplitude covers
-them; then half a step of bf16, 2^-8 of the value. Selection: a thread sums 32
+them; then half a step of bf16, 2^-8 of the value. Selection: a thread sums 16
 exponentials of 2^-22 + |x| 2^-23 relative error (weighted by exp(x), at most
-2^-21 of the sum), 37 + 8 additions to the block's sum: the log of the sum is off
-by 50 * 2^-24, the score besides by 2^-24 of itself. Reordering moves bits.
+2^-21 of the sum) a round, adds at most 8 rounds here with a factor each, and 13
+more additions and 2 factors make the block's sum: the log of the sum is off by
+50 * 2^-24, the score besides by 2^-24 of itself. Reordering moves bits.
 """
 import math
 
