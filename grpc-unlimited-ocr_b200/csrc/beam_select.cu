@@ -425,9 +425,9 @@ cudaError_t launch(const uocr_beam_select_args& a, const Join& j, cudaStream_t s
   const size_t keys = static_cast<size_t>(j.s.beams) * j.s.parts * j.s.select * sizeof(uint64_t);
   const size_t join_smem = (static_cast<size_t>(j.s.beams) * j.s.parts + j.s.select * j.s.select) * sizeof(Cand);
   const bool staged = keys <= 64 * 1024;
-  cudaError_t st = allow_max_dynamic_smem(beam_parts_kernel<T>);
-  if (st == cudaSuccess) st = allow_max_dynamic_smem(beam_join_kernel<true>);
-  if (st == cudaSuccess) st = allow_max_dynamic_smem(beam_join_kernel<false>);
+  cudaError_t st = allow_max_dynamic_smem_once<beam_parts_kernel<T>>();
+  if (st == cudaSuccess) st = allow_max_dynamic_smem_once<beam_join_kernel<true>>();
+  if (st == cudaSuccess) st = allow_max_dynamic_smem_once<beam_join_kernel<false>>();
   if (st == cudaSuccess)
     st = launch_pdl(beam_parts_kernel<T>, static_cast<unsigned>(a.batch * a.beams * j.s.parts), kThreads,
                     kList * sizeof(uint64_t), stream, j.s);

@@ -5,6 +5,7 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 namespace uocr_b200 {
@@ -100,6 +101,22 @@ inline cudaError_t allow_max_dynamic_smem(Kernel kernel) {
   if (st == cudaSuccess)
     st = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                               optin - static_cast<int>(attr.sharedSizeBytes));
+  return st;
+}
+
+// The same once for each device (a call in every launch costs a microsecond of the
+// host's); kMaxDevices bits.
+template <auto kKernel>
+inline cudaError_t allow_max_dynamic_smem_once() {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaError_t st = cudaGetDevice(&dev);
+  if (st != cudaSuccess) return st;
+  if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
+  const uint64_t bit = uint64_t{1} << dev;
+  if ((done.load(std::memory_order_acquire) & bit) != 0) return cudaSuccess;
+  st = allow_max_dynamic_smem(kKernel);
+  if (st == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
   return st;
 }
 

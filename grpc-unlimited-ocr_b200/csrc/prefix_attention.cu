@@ -822,7 +822,7 @@ cudaError_t launch_rows(const Attention& a, const Grid& g, unsigned blocks, cuda
   // 4 / w warps along the keys, 16 w rows
   constexpr size_t kJoin = static_cast<size_t>(64) * (kDim * 4 + 8);
   static_assert(kJoin <= kRing, "the join takes the ring's place");
-  cudaError_t st = allow_max_dynamic_smem(attention_rows_kernel<kDim, kPrefixWarps, kOwnWarps>);
+  cudaError_t st = allow_max_dynamic_smem_once<attention_rows_kernel<kDim, kPrefixWarps, kOwnWarps>>();
   if (st != cudaSuccess) return st;
   return launch_pdl(attention_rows_kernel<kDim, kPrefixWarps, kOwnWarps>, blocks, kThreads, kRing, stream, a, g);
 }
@@ -831,7 +831,7 @@ template <int kDim, int kWarps>
 cudaError_t launch_last(const Attention& a, unsigned blocks, int late_wait, cudaStream_t stream) {
   constexpr size_t kRing = static_cast<size_t>(kStages) * 2 * kKeys * (kDim + 8) * 2;
   const size_t join = 64 * (kDim * 4 + 8 + 4) + 16 * kWarps * (4 + a.prefix_slots * 8);
-  cudaError_t st = allow_max_dynamic_smem(attention_last_kernel<kDim, kWarps>);
+  cudaError_t st = allow_max_dynamic_smem_once<attention_last_kernel<kDim, kWarps>>();
   if (st != cudaSuccess) return st;
   return launch_pdl(attention_last_kernel<kDim, kWarps>, blocks, kThreads, std::max(kRing, join), stream, a, late_wait);
 }

@@ -650,19 +650,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
 template <int kDim>
 cudaError_t launch(const TcArgs& t, unsigned blocks, cudaStream_t stream) {
   constexpr size_t kSmem = static_cast<size_t>(2 + kSlots) * kTcKeys * kDim * 2 + 1024;
-  static bool done[kMaxDevices] = {};
-  int dev = 0;
-  cudaError_t st = cudaGetDevice(&dev);
-  if (st != cudaSuccess) return st;
-  if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
-  if (!done[dev]) {
-    // The shares of the register file have to add up to the launch's.
+  // The shares of the register file have to add up to the launch's.
+  static const int registers = [] {
     cudaFuncAttributes attr{};
-    if ((st = cudaFuncGetAttributes(&attr, attention_tc_kernel<kDim>)) != cudaSuccess) return st;
-    if (attr.numRegs != kLaunchRegs) return cudaErrorInvalidKernelImage;
-    if ((st = allow_max_dynamic_smem(attention_tc_kernel<kDim>)) != cudaSuccess) return st;
-    done[dev] = true;
-  }
+    return cudaFuncGetAttributes(&attr, attention_tc_kernel<kDim>) == cudaSuccess ? attr.numRegs : 0;
+  }();
+  if (registers != kLaunchRegs) return cudaErrorInvalidKernelImage;
+  const cudaError_t st = allow_max_dynamic_smem_once<attention_tc_kernel<kDim>>();
+  if (st != cudaSuccess) return st;
   return launch_pdl(attention_tc_kernel<kDim>, blocks, kTcThreads, kSmem, stream, t);
 }
 

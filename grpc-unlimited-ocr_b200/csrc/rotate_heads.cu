@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(kStreamThreads) rotate_stream_kernel(Rotate a,
 
 template <typename T, int kLanes, bool kInterleaved, bool kNorm>
 cudaError_t launch_stream(const Rotate& r, int blocks, int workers, size_t smem, cudaStream_t stream) {
-  cudaError_t st = allow_max_dynamic_smem(rotate_stream_kernel<T, kLanes, kInterleaved, kNorm>);
+  cudaError_t st = allow_max_dynamic_smem_once<rotate_stream_kernel<T, kLanes, kInterleaved, kNorm>>();
   if (st != cudaSuccess) return st;
   return launch_pdl(rotate_stream_kernel<T, kLanes, kInterleaved, kNorm>, static_cast<unsigned>(148 * blocks),
                     workers + kHelpers, smem, stream, r, workers);

@@ -192,6 +192,8 @@ def _packer(args) -> struct.Struct:
 _pack_linear, _pack_grouped = _packer(LinearW8A8Args).pack, _packer(GroupedW8A8Args).pack
 _pack_rotate, _pack_attention = _packer(RotateHeadsArgs).pack, _packer(PrefixAttentionArgs).pack
 _pack_select, _pack_reorder = _packer(BeamSelectArgs).pack, _packer(ReorderStatesArgs).pack
+# The workspace and its size end the packed arguments of the calls that need one.
+_pack_space, _PACKED_SPACE = struct.Struct("@Pq").pack, struct.calcsize("@Pq")
 
 
 def lib() -> ctypes.CDLL:
@@ -247,9 +249,9 @@ def lib() -> ctypes.CDLL:
         L.uocr_grouped_linear_w8a8.argtypes = [vp, vp]
         L.uocr_rope_frequencies.argtypes = [i64, ctypes.c_double, i32, ctypes.c_double, i64, vp, ctypes.POINTER(f32)]
         L.uocr_rotate_heads.argtypes = [vp, vp]
-        L.uocr_prefix_attention_workspace.argtypes = [vp, ctypes.POINTER(i64)]
+        L.uocr_prefix_attention_workspace.argtypes = [vp, vp]  # the size: a c_int64 by reference
         L.uocr_prefix_attention.argtypes = [vp, vp]
-        L.uocr_beam_select_workspace.argtypes = [vp, ctypes.POINTER(i64)]
+        L.uocr_beam_select_workspace.argtypes = [vp, vp]
         L.uocr_beam_select.argtypes = [vp, vp]
         L.uocr_reorder_states.argtypes = [vp, vp]
         L.uocr_decoder_beam_workspace.argtypes = [vp, i64, i64, ctypes.POINTER(i64)]
@@ -724,31 +726,40 @@ def rotate_heads(q, k, v, inv_freq, positions, q_out, k_cache, v_cache, q_norm=N
     (else positions[r]) (uocr_rotate_heads). q, k, v: fp32 or bf16; inv_freq: fp32, rotary_dim / 2 of them; positions,
     cache_rows, slots: int32."""
     import torch
-    f32, i32 = torch.float32, torch.int32
-    rows, _, dim = q.shape
-    _on_current_device(q, k, v, inv_freq, positions, q_out, k_cache, v_cache, q_norm, k_norm, cache_rows, slots)
-    heads, ldq = _heads(q, "q", rows, dim)
-    kv_heads, ldk = _heads(k, "k", rows, dim)
-    v_heads, ldv = _heads(v, "v", rows, dim)
-    out_heads, ldqo = _heads(q_out, "q_out", rows, dim)
-    if out_heads != heads or q_out.dtype is not torch.bfloat16:
-        raise ValueError("q_out must be bfloat16 of q's shape")
-    if v_heads != kv_heads or k.dtype is not q.dtype or v.dtype is not q.dtype:
-        raise ValueError("k and v must have the same shape and q's dtype")
-    cache_stride, head_stride = _cache_strides(k_cache, v_cache, "the caches")
-    if k_cache.shape[1] != kv_heads or k_cache.shape[3] != dim:
-        raise ValueError(f"the caches must be [caches, {kv_heads}, capacity, {dim}]")
-    if cache_rows is None and k_cache.shape[0] != rows:
+    f32, i32, bf16 = torch.float32, torch.int32, torch.bfloat16
+    rows, heads, dim = shape = q.shape
+    kv_heads, rotary = k.shape[1], 2 * inv_freq.numel()
+    (ldq, *lq), (ldk, *lk), (ldv, *lv), (ldqo, *lo) = q.stride(), k.stride(), v.stride(), q_out.stride()
+    of_cache, of_head, *lc = strides = k_cache.stride()
+    caches, cache_heads, capacity, cache_dim = k_cache.shape
+    rotated, dtype = [dim, 1], q.dtype
+    # The common case in one expression (this call is microseconds of device time); else what is wrong, or a form of one.
+    if not (rows > 1 and kv_heads > 1 and caches > 1 and lq == lk == lv == lo == lc == rotated and q_out.shape == shape
+            and k.shape == v.shape == (rows, kv_heads, dim) and v_cache.shape == (caches, kv_heads, capacity, dim)
+            and (cache_heads, cache_dim) == (kv_heads, dim) and v_cache.stride() == strides
+            and q_out.dtype is k_cache.dtype is v_cache.dtype is bf16 and k.dtype is v.dtype is dtype):
+        heads, ldq = _heads(q, "q", rows, dim)
+        kv_heads, ldk = _heads(k, "k", rows, dim)
+        v_heads, ldv = _heads(v, "v", rows, dim)
+        out_heads, ldqo = _heads(q_out, "q_out", rows, dim)
+        if out_heads != heads or q_out.dtype is not bf16:
+            raise ValueError("q_out must be bfloat16 of q's shape")
+        if v_heads != kv_heads or k.dtype is not dtype or v.dtype is not dtype:
+            raise ValueError("k and v must have the same shape and q's dtype")
+        of_cache, of_head = _cache_strides(k_cache, v_cache, "the caches")
+        if cache_heads != kv_heads or cache_dim != dim:
+            raise ValueError(f"the caches must be [caches, {kv_heads}, capacity, {dim}]")
+    if cache_rows is None and caches != rows:
         raise ValueError("without cache_rows there is one cache per row")
-    args = _pack_rotate(
+    _on_current_device(q, k, v, inv_freq, positions, q_out, k_cache, v_cache, q_norm, k_norm, cache_rows, slots)
+    _check(lib().uocr_rotate_heads(_pack_rotate(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), 0 if q_norm is None else _vector(q_norm, "q_norm", dim, f32),
-        0 if k_norm is None else _vector(k_norm, "k_norm", dim, f32),
-        _vector(inv_freq, "inv_freq", inv_freq.numel(), f32), _vector(positions, "positions", rows, i32),
+        0 if k_norm is None else _vector(k_norm, "k_norm", dim, f32), _vector(inv_freq, "inv_freq", rotary // 2, f32),
+        _vector(positions, "positions", rows, i32),
         0 if cache_rows is None else _vector(cache_rows, "cache_rows", rows, i32),
         0 if slots is None else _vector(slots, "slots", rows, i32), q_out.data_ptr(), k_cache.data_ptr(),
-        v_cache.data_ptr(), rows, heads, kv_heads, dim, 2 * inv_freq.numel(), ldq, ldk, ldv, ldqo, k_cache.shape[0],
-        k_cache.shape[2], cache_stride, head_stride, eps, magnitude, _float_dtype(q, "q"), int(interleaved))
-    _check(lib().uocr_rotate_heads(args, _stream(stream)))
+        v_cache.data_ptr(), rows, heads, kv_heads, dim, rotary, ldq, ldk, ldv, ldqo, caches, capacity, of_cache, of_head,
+        eps, magnitude, _float_dtype(q, "q"), interleaved), _stream(stream)))
 
 
 def prefix_attention(q, prefix_k, prefix_v, prefix_lens, k, v, lens, out, ancestry=None, row_offsets=None,
@@ -761,18 +772,26 @@ def prefix_attention(q, prefix_k, prefix_v, prefix_lens, k, v, lens, out, ancest
     torch's allocator, from the blocks of the stream that the call runs on."""
     import torch
     f32, i32, bf16 = torch.float32, torch.int32, torch.bfloat16
-    rows, _, dim = q.shape
+    rows, heads, dim = shape = q.shape
+    prefixes, kv_heads, prefix_capacity, _ = prefix_shape = prefix_k.shape
+    caches, _, capacity, _ = own_shape = k.shape
+    (ldq, *lq), (ldo, *lo) = q.stride(), out.stride()
+    prefix_strides, own_strides = prefix_k.stride(), k.stride()
+    # The common case in one expression; else what is wrong, or a form of one.
+    if not (rows > 1 and prefixes > 0 and kv_heads > 1 and caches > 1 and lq == lo == [dim, 1] and out.shape == shape
+            and prefix_strides[2:] == own_strides[2:] == (dim, 1) and prefix_v.stride() == prefix_strides
+            and v.stride() == own_strides and prefix_v.shape == prefix_shape and v.shape == own_shape
+            and prefix_shape[3] == own_shape[3] == dim and own_shape[1] == kv_heads
+            and q.dtype is out.dtype is prefix_k.dtype is prefix_v.dtype is k.dtype is v.dtype is bf16):
+        heads, ldq = _heads(q, "q", rows, dim)
+        out_heads, ldo = _heads(out, "out", rows, dim)
+        if out_heads != heads or q.dtype is not bf16 or out.dtype is not bf16:
+            raise ValueError("q and out must be bfloat16 of the same shape")
+        prefix_strides = _cache_strides(prefix_k, prefix_v, "the prefixes")
+        own_strides = _cache_strides(k, v, "the own caches")
+        if own_shape[1] != kv_heads or own_shape[3] != dim or prefix_shape[3] != dim:
+            raise ValueError(f"the caches must be [caches, {kv_heads}, capacity, {dim}]")
     _on_current_device(q, prefix_k, prefix_v, prefix_lens, k, v, lens, out, ancestry, row_offsets, lse)
-    heads, ldq = _heads(q, "q", rows, dim)
-    out_heads, ldo = _heads(out, "out", rows, dim)
-    if out_heads != heads or q.dtype is not bf16 or out.dtype is not bf16:
-        raise ValueError("q and out must be bfloat16 of the same shape")
-    prefix_stride, prefix_head_stride = _cache_strides(prefix_k, prefix_v, "the prefixes")
-    cache_stride, head_stride = _cache_strides(k, v, "the own caches")
-    prefixes, kv_heads, prefix_capacity, _ = prefix_k.shape
-    caches, _, capacity, _ = k.shape
-    if k.shape[1] != kv_heads or k.shape[3] != dim or prefix_k.shape[3] != dim:
-        raise ValueError(f"the caches must be [caches, {kv_heads}, capacity, {dim}]")
     sequences, ld_ancestry, table, offsets = lens.numel(), 0, 0, 0
     if ancestry is not None:
         if ancestry.dtype is not i32:
@@ -780,19 +799,19 @@ def prefix_attention(q, prefix_k, prefix_v, prefix_lens, k, v, lens, out, ancest
         ld_ancestry, table = _pitch(ancestry, "ancestry", sequences, capacity), ancestry.data_ptr()
     if row_offsets is not None:
         offsets = _vector(row_offsets, "row_offsets", sequences + 1, i32)
-    args = (q.data_ptr(), prefix_k.data_ptr(), prefix_v.data_ptr(), _vector(prefix_lens, "prefix_lens", prefixes, i32),
-            k.data_ptr(), v.data_ptr(), _vector(lens, "lens", sequences, i32), table, offsets, out.data_ptr(),
-            0 if lse is None else _vector(lse, "lse", rows * heads, f32), rows, sequences, prefixes, caches, heads,
-            kv_heads, dim, prefix_capacity, capacity, ldq, ldo, ld_ancestry, prefix_stride, prefix_head_stride,
-            cache_stride, head_stride, dim ** -0.5 if scale is None else scale, 0)
-    need = ctypes.c_int64()
-    _check(lib().uocr_prefix_attention_workspace(_pack_attention(*args, 0, 0), ctypes.byref(need)))
-    if need.value > 0:
-        workspace = _workspace(need.value, q.device, stream)  # held until the launch is made
-        args += (workspace.data_ptr(), need.value)
-    else:
-        args += (0, 0)
-    _check(lib().uocr_prefix_attention(_pack_attention(*args), _stream(stream)))
+    args = _pack_attention(
+        q.data_ptr(), prefix_k.data_ptr(), prefix_v.data_ptr(), _vector(prefix_lens, "prefix_lens", prefixes, i32),
+        k.data_ptr(), v.data_ptr(), _vector(lens, "lens", sequences, i32), table, offsets, out.data_ptr(),
+        0 if lse is None else _vector(lse, "lse", rows * heads, f32), rows, sequences, prefixes, caches, heads,
+        kv_heads, dim, prefix_capacity, capacity, ldq, ldo, ld_ancestry, prefix_strides[0], prefix_strides[1],
+        own_strides[0], own_strides[1], dim ** -0.5 if scale is None else scale, 0, 0, 0)
+    size = ctypes.c_int64()
+    _check(lib().uocr_prefix_attention_workspace(args, ctypes.byref(size)))
+    need = size.value
+    if need > 0:
+        workspace = _workspace(need, q.device, stream)  # held until the launch is made
+        args = args[:-_PACKED_SPACE] + _pack_space(workspace.data_ptr(), need)
+    _check(lib().uocr_prefix_attention(args, _stream(stream)))
 
 
 def beam_select(logits, scores, tokens, parents, new_scores, finished=None, new_finished=None, eos: int = -1,
@@ -806,17 +825,18 @@ def beam_select(logits, scores, tokens, parents, new_scores, finished=None, new_
     _on_current_device(logits, scores, tokens, parents, new_scores, finished, new_finished)
     batch, beams = scores.shape
     select, vocab = tokens.shape[1], logits.shape[1]
-    ld = _pitch(logits, "logits", batch * beams, vocab)
-    args = (logits.data_ptr(), _vector(scores, "scores", batch * beams, f32),
-            0 if finished is None else _vector(finished, "finished", batch * beams, i32),
-            _vector(tokens, "tokens", batch * select, i32), _vector(parents, "parents", batch * select, i32),
-            _vector(new_scores, "new_scores", batch * select, f32),
-            0 if new_finished is None else _vector(new_finished, "new_finished", batch * select, i32), batch, beams,
-            select, vocab, ld, _float_dtype(logits, "logits"), eos)
-    need = ctypes.c_int64()
-    _check(lib().uocr_beam_select_workspace(_pack_select(*args, 0, 0), ctypes.byref(need)))
-    workspace = _workspace(max(need.value, 16), logits.device, stream)  # held until the launch is made
-    _check(lib().uocr_beam_select(_pack_select(*args, workspace.data_ptr(), need.value), _stream(stream)))
+    rows, out = batch * beams, batch * select
+    args = _pack_select(
+        logits.data_ptr(), _vector(scores, "scores", rows, f32),
+        0 if finished is None else _vector(finished, "finished", rows, i32), _vector(tokens, "tokens", out, i32),
+        _vector(parents, "parents", out, i32), _vector(new_scores, "new_scores", out, f32),
+        0 if new_finished is None else _vector(new_finished, "new_finished", out, i32), batch, beams, select, vocab,
+        _pitch(logits, "logits", rows, vocab), _float_dtype(logits, "logits"), eos, 0, 0)
+    size = ctypes.c_int64()
+    _check(lib().uocr_beam_select_workspace(args, ctypes.byref(size)))
+    need = size.value
+    workspace = _workspace(need or 16, logits.device, stream)  # held until the launch is made
+    _check(lib().uocr_beam_select(args[:-_PACKED_SPACE] + _pack_space(workspace.data_ptr(), need), _stream(stream)))
 
 
 def reorder_states(state, parents, beams: int, counts=None, stream=None):
@@ -830,23 +850,22 @@ def reorder_states(state, parents, beams: int, counts=None, stream=None):
         state = state[None, :, None]
     if state.dim() < 4:
         raise ValueError("state must be [layers, rows, segments, units, ...] or [rows, units]")
-    layers, rows, segments, units = state.shape[:4]
+    layers, rows, segments, units, *inner = state.shape
+    of_layer, of_row, of_segment, *steps = state.stride()
     width = 1
-    for n in state.shape[4:]:
-        width *= n
-    flat, expect = state.stride()[3:], 1
-    for n, step in zip(reversed(state.shape[3:]), reversed(flat)):
-        if step != expect and n > 1:
+    for n, step in zip(reversed(inner), reversed(steps)):
+        if step != width and n > 1:
             raise ValueError("a segment of the state must be contiguous")
-        expect *= n
+        width *= n
+    if steps[0] != width and units > 1:
+        raise ValueError("a segment of the state must be contiguous")
     if beams < 1 or rows % beams != 0:
         raise ValueError("the state's rows must be whole groups of beams")
     eb = state.element_size()
-    of_layer, of_row, of_segment = (s * eb for s in state.stride()[:3])
     _check(lib().uocr_reorder_states(_pack_reorder(
         state.data_ptr(), _vector(parents, "parents", rows, i32),
         0 if counts is None else _vector(counts, "counts", rows, i32), layers, rows // beams, beams, segments, units,
-        width * eb, of_layer, of_row, of_segment), _stream(stream)))
+        width * eb, of_layer * eb, of_row * eb, of_segment * eb), _stream(stream)))
 
 
 class Decoder:
