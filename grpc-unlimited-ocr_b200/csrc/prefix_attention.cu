@@ -44,6 +44,12 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], const void* 
                : "r"(smem_addr(p))
                : "memory");
 }
+// An 8 x 8 matrix of 16-bit elements in a warp's registers, transposed.
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t a) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+  return r;
+}
 // 16 bytes, or zeros where `valid` is false (the source is not read then).
 __device__ __forceinline__ void cp_async16_or_zero(void* dst, const void* src, bool valid) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(valid ? 16 : 0)
@@ -116,6 +122,215 @@ __device__ __forceinline__ unsigned block_scan(unsigned v, unsigned* part, unsig
   return v;
 }
 
+// A segment's keys and values into the ring of padded stages, by cp.async. A thread
+// copies 16 bytes of every kStep-th key of a stage. Where its keys lie (with
+// ancestry: in any of the caches) is read a fill ahead of the copies, all keys at
+// once.
+template <int kDim>
+struct Feed {
+  static constexpr int kPitch = kDim + 8;  // padded: fragment loads without bank conflicts
+  static constexpr int kStage = 2 * kKeys * kPitch;
+  static constexpr int kStep = kThreads / (kDim / 8), kCopies = kKeys / kStep;
+  const Attention& a;
+  const Segment& w;
+  __nv_bfloat16* ring;
+  const __nv_bfloat16* keys;  // of key 0 (with ancestry: in cache 0)
+  const __nv_bfloat16* values;
+  bool gathers;
+  int from[kCopies];
+
+  __device__ __forceinline__ Feed(const Attention& attention, const Segment& segment, unsigned char* raw)
+      : a(attention), w(segment), ring(reinterpret_cast<__nv_bfloat16*>(raw)) {
+    const int64_t base = w.own ? (a.ancestry != nullptr ? 0 : w.of * a.cache_stride) + w.kv_head * a.head_stride
+                               : w.of * a.prefix_stride + w.kv_head * a.prefix_head_stride;
+    keys = (w.own ? a.k : a.prefix_k) + base;
+    values = (w.own ? a.v : a.prefix_v) + base;
+    gathers = w.own && a.ancestry != nullptr;
+  }
+  __device__ __forceinline__ void look_up(int key) {
+    if (!gathers) return;
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) {
+      const int at = key + static_cast<int>(threadIdx.x) / (kDim / 8) + i * kStep;
+      from[i] = at < w.key1 ? a.ancestry[w.of * a.ld_ancestry + at] : 0;
+    }
+  }
+  __device__ __forceinline__ void fill(int stage, int key) {
+    const int copy_key = threadIdx.x / (kDim / 8), col = threadIdx.x % (kDim / 8) * 8;
+    __nv_bfloat16* ks = ring + stage * kStage + copy_key * kPitch + col;
+    __nv_bfloat16* vs = ks + kKeys * kPitch;
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) {
+      const int at = key + copy_key + i * kStep;
+      const bool valid = at < w.key1;
+      int64_t off = valid ? static_cast<int64_t>(at) * kDim + col : 0;
+      if (gathers) {
+        int cache = from[i];
+        if (valid && (cache < 0 || cache >= a.caches)) {
+          raise_error(a.err, kDevBadIndex, kSiteAncestor, w.of, cache);
+          cache = w.of < a.caches ? w.of : 0;
+        }
+        off += cache * a.cache_stride;
+      }
+      cp_async16_or_zero(ks + i * kStep * kPitch, keys + off, valid);
+      cp_async16_or_zero(vs + i * kStep * kPitch, values + off, valid);
+    }
+  }
+  __device__ __forceinline__ void start() {
+    look_up(w.key0);
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) {
+      if (w.key0 + s * kKeys < w.key1) fill(s, w.key0 + s * kKeys);
+      cp_async_commit();
+      look_up(w.key0 + (s + 1) * kKeys);
+    }
+  }
+  // While the stage with `key` is worked on.
+  __device__ __forceinline__ void next(int key, int stage) {
+    const int ahead = key + (kStages - 1) * kKeys;
+    if (ahead < w.key1) fill((stage + kStages - 1) % kStages, ahead);
+    cp_async_commit();
+    look_up(ahead + kKeys);
+  }
+};
+
+// The end of a block that has all own keys of its rows: their kAlong parts, which
+// the warps leave in the ring's place, and the prefix's are joined and the rows
+// written.
+template <int kDim, int kRows, int kAlong>
+struct LastJoin {
+  float* os;        // [kAlong][kRows][kDim]
+  float2* mls;      // [kAlong][kRows]
+  float* own;       // [kAlong][kRows] factors
+  float* scales;    // [kRows] 1 / sum
+  float2* factors;  // [kRows][prefix_slots] the parts' maxima and sums, then their factors in the maxima's place
+  __device__ __forceinline__ explicit LastJoin(unsigned char* raw) {
+    os = reinterpret_cast<float*>(raw);
+    mls = reinterpret_cast<float2*>(os + kAlong * kRows * kDim);
+    own = reinterpret_cast<float*>(mls + kAlong * kRows);
+    scales = own + kAlong * kRows;
+    factors = reinterpret_cast<float2*>(scales + kRows);
+  }
+  static constexpr size_t bytes(int prefix_slots) {
+    return kAlong * kRows * (kDim * 4 + 8 + 4) + kRows * (4 + prefix_slots * 8);
+  }
+  // live: a word of shared memory that nobody else uses by now
+  __device__ __forceinline__ void run(const Attention& a, const Segment& w, uint32_t* live, bool late_wait) const {
+    auto cell = [&](int r) {  // of the tile's row r
+      const int vr = w.start + r;
+      const int64_t row = w.first_row + vr / a.group;
+      return row * a.heads + w.kv_head * a.group + vr % a.group;
+    };
+    if (late_wait) pdl_wait();  // the prefix's parts
+    __syncthreads();
+    for (int c0 = threadIdx.x; c0 < w.count * a.prefix_slots; c0 += 8 * kThreads) {
+      float2 ml[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int c = c0 + k * kThreads;
+        if (c < w.count * a.prefix_slots) ml[k] = a.part_ml[cell(c / a.prefix_slots) * a.slots + c % a.prefix_slots];
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (c0 + k * kThreads < w.count * a.prefix_slots) factors[c0 + k * kThreads] = ml[k];
+    }
+    if (threadIdx.x == 0) *live = 0;  // from here on: one more than the last slot with keys
+    __syncthreads();
+    {
+      // All rows at once, kLanes neighbouring threads each.
+      constexpr int kLanes = kThreads / kRows;
+      const int r = threadIdx.x / kLanes, at = threadIdx.x % kLanes;
+      float2* ml = factors + r * a.prefix_slots;
+      const int slots = r < w.count ? a.prefix_slots : 0;
+      float top = -INFINITY;
+      for (int i = at; i < kAlong; i += kLanes) top = fmaxf(top, mls[i * kRows + r].x);
+      for (int s = at; s < slots; s += kLanes) top = fmaxf(top, ml[s].x);
+#pragma unroll
+      for (int off = kLanes / 2; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+      const float shift = top == -INFINITY ? 0.0f : top;
+      float sum = 0.0f;
+      int used = 0;
+      for (int i = at; i < kAlong; i += kLanes) {
+        const float2 p = mls[i * kRows + r];
+        const float f = exp2_fast(p.x - shift);
+        sum = fmaf(p.y, f, sum);
+        own[i * kRows + r] = f;
+      }
+      for (int s = at; s < slots; s += kLanes) {
+        const float2 p = ml[s];
+        const float f = exp2_fast(p.x - shift);
+        sum = fmaf(p.y, f, sum);
+        // A part without keys has no output: its factor is told apart from one that has underflowed.
+        ml[s].x = p.x == -INFINITY ? -1.0f : f;
+        if (p.x != -INFINITY) used = s + 1;
+      }
+#pragma unroll
+      for (int off = kLanes / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+      if (used > 0) atomicMax(live, static_cast<uint32_t>(used));
+      if (at == 0 && r < w.count) {
+        scales[r] = sum != 0.0f ? 1.0f / sum : 0.0f;
+        if (a.lse != nullptr)
+          a.lse[cell(r)] = sum != 0.0f ? (top + log2f(sum)) * 0.69314718055994530942f : -INFINITY;
+      }
+    }
+    __syncthreads();
+    const int live_slots = static_cast<int>(*live);
+    // 16 pieces of parts under way at a time: of four rows where there are many, of one where there are few.
+    auto join_rows = [&](auto rows_at_once) {
+      constexpr int kR = decltype(rows_at_once)::value, kAhead = 16 / kR;
+      constexpr int kPieces = kDim / 4, kGroups = kThreads / kPieces;
+      const int col = threadIdx.x % kPieces * 4;
+      for (int r0 = threadIdx.x / kPieces * kR; r0 < w.count; r0 += kGroups * kR) {
+        float4 acc[kR];
+        const float* parts[kR];
+        auto add = [](float4& sum, const float4& v, float f) {
+          sum.x = fmaf(v.x, f, sum.x), sum.y = fmaf(v.y, f, sum.y);
+          sum.z = fmaf(v.z, f, sum.z), sum.w = fmaf(v.w, f, sum.w);
+        };
+#pragma unroll
+        for (int k = 0; k < kR; ++k) {
+          acc[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          parts[k] = a.part_o + cell(r0 + k) * a.slots * kDim + col;
+        }
+        for (int s0 = 0; s0 < live_slots; s0 += kAhead) {
+          float4 v[kR][kAhead];
+          float f[kR][kAhead];
+#pragma unroll
+          for (int k = 0; k < kR; ++k)
+#pragma unroll
+            for (int s = 0; s < kAhead; ++s) {
+              f[k][s] = r0 + k < w.count && s0 + s < live_slots ? factors[(r0 + k) * a.prefix_slots + s0 + s].x : -1.0f;
+              v[k][s] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+              if (!(f[k][s] < 0.0f)) v[k][s] = *reinterpret_cast<const float4*>(parts[k] + (s0 + s) * kDim);
+            }
+#pragma unroll
+          for (int k = 0; k < kR; ++k)
+#pragma unroll
+            for (int s = 0; s < kAhead; ++s) add(acc[k], v[k][s], f[k][s]);
+        }
+#pragma unroll
+        for (int k = 0; k < kR; ++k) {
+          const int r = r0 + k;
+          if (r >= w.count) break;
+#pragma unroll
+          for (int i = 0; i < kAlong; ++i)
+            add(acc[k], *reinterpret_cast<const float4*>(os + (i * kRows + r) * kDim + col), own[i * kRows + r]);
+          const int vr = w.start + r;
+          const float scale = scales[r];
+          __nv_bfloat16* out = a.out + static_cast<int64_t>(w.first_row + vr / a.group) * a.ldo +
+                               (w.kv_head * a.group + vr % a.group) * kDim + col;
+          *reinterpret_cast<uint2*>(out) =
+              make_uint2(pack2(acc[k].x * scale, acc[k].y * scale), pack2(acc[k].z * scale, acc[k].w * scale));
+        }
+      }
+    };
+    if (w.count > 16)
+      join_rows(std::integral_constant<int, 4>{});
+    else
+      join_rows(std::integral_constant<int, 1>{});
+  }
+};
+
 // A segment. 4 warps: kWarpRows of them side by side along the rows (16 each),
 // the others along a stage's keys, each with its own running maximum, sum and
 // output in registers; keys and values in a ring of padded stages filled by
@@ -132,56 +347,12 @@ __device__ __forceinline__ void attend(const Attention& a, const Segment& seg, u
   constexpr int kPitch = kDim + 8;  // padded: fragment loads without bank conflicts
   constexpr int kStage = 2 * kKeys * kPitch;
   __nv_bfloat16* ring = reinterpret_cast<__nv_bfloat16*>(raw);
-  // key 0 (with ancestry: in cache 0)
-  const int64_t base = w.own ? (a.ancestry != nullptr ? 0 : w.of * a.cache_stride) + w.kv_head * a.head_stride
-                             : w.of * a.prefix_stride + w.kv_head * a.prefix_head_stride;
-  const __nv_bfloat16* keys = (w.own ? a.k : a.prefix_k) + base;
-  const __nv_bfloat16* values = (w.own ? a.v : a.prefix_v) + base;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gr = lane >> 2, tq = lane & 3;
   const int row0 = warp % kWarpRows * 16, warp_key = warp / kWarpRows * kWarpKeys;
 
-  // A thread copies 16 bytes of every kStep-th key of a stage. Where its keys lie (with ancestry: in any of the caches)
-  // is read a fill ahead of the copies, all keys at once.
-  constexpr int kStep = kThreads / (kDim / 8), kCopies = kKeys / kStep;
-  const int copy_key = threadIdx.x / (kDim / 8), copy_col = threadIdx.x % (kDim / 8) * 8;
-  const bool gathers = w.own && a.ancestry != nullptr;
-  int from[kCopies] = {};
-  auto look_up = [&](int key) {
-    if (!gathers) return;
-#pragma unroll
-    for (int i = 0; i < kCopies; ++i) {
-      const int at = key + copy_key + i * kStep;
-      from[i] = at < w.key1 ? a.ancestry[w.of * a.ld_ancestry + at] : 0;
-    }
-  };
-  auto fill = [&](int stage, int key) {
-    __nv_bfloat16* ks = ring + stage * kStage + copy_key * kPitch + copy_col;
-    __nv_bfloat16* vs = ks + kKeys * kPitch;
-#pragma unroll
-    for (int i = 0; i < kCopies; ++i) {
-      const int at = key + copy_key + i * kStep;
-      const bool valid = at < w.key1;
-      int64_t off = valid ? static_cast<int64_t>(at) * kDim + copy_col : 0;
-      if (gathers) {
-        int cache = from[i];
-        if (valid && (cache < 0 || cache >= a.caches)) {
-          raise_error(a.err, kDevBadIndex, kSiteAncestor, w.of, cache);
-          cache = w.of < a.caches ? w.of : 0;
-        }
-        off += cache * a.cache_stride;
-      }
-      cp_async16_or_zero(ks + i * kStep * kPitch, keys + off, valid);
-      cp_async16_or_zero(vs + i * kStep * kPitch, values + off, valid);
-    }
-  };
-  look_up(w.key0);
-#pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) {
-    if (w.key0 + s * kKeys < w.key1) fill(s, w.key0 + s * kKeys);
-    cp_async_commit();
-    look_up(w.key0 + (s + 1) * kKeys);
-  }
+  Feed<kDim> feed(a, w, raw);
+  feed.start();
 
   // This thread's two rows of the warp's tile, and the warp's queries as A fragments.
   int limit[2];
@@ -211,10 +382,7 @@ __device__ __forceinline__ void attend(const Attention& a, const Segment& seg, u
   for (int key = w.key0; key < w.key1; key += kKeys) {
     cp_async_wait<kStages - 2>();
     __syncthreads();  // the stage has landed for all, and the one filled next has been read by all
-    const int ahead = key + (kStages - 1) * kKeys;
-    if (ahead < w.key1) fill((stage + kStages - 1) % kStages, ahead);
-    cp_async_commit();
-    look_up(ahead + kKeys);
+    feed.next(key, stage);
     const __nv_bfloat16* ks = ring + stage * kStage + warp_key * kPitch;
     const __nv_bfloat16* vs = ks + kKeys * kPitch;
     stage = (stage + 1) % kStages;
@@ -329,132 +497,19 @@ __device__ __forceinline__ void attend(const Attention& a, const Segment& seg, u
     return row * a.heads + w.kv_head * a.group + vr % a.group;
   };
   if constexpr (kLast) {
-    constexpr int kAlong = 4 / kWarpRows;
-    float* os = reinterpret_cast<float*>(raw);                            // [kAlong][kRows][kDim], in the ring's place
-    float2* mls = reinterpret_cast<float2*>(os + kAlong * kRows * kDim);  // [kAlong][kRows]
-    float* own = reinterpret_cast<float*>(mls + kAlong * kRows);          // [kAlong][kRows] factors
-    float* scales = own + kAlong * kRows;                                 // [kRows] 1 / sum
-    // [kRows][prefix_slots] the parts' maxima and sums, then their factors in the maxima's place
-    float2* factors = reinterpret_cast<float2*>(scales + kRows);
+    using Join = LastJoin<kDim, kRows, 4 / kWarpRows>;
+    const Join join(raw);
     cp_async_wait_all();
     __syncthreads();
-    const int along = warp / kWarpRows;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int r = row0 + gr + 8 * i;
-      if (tq == 0) mls[along * kRows + r] = make_float2(m[i], l[i]);
+      const int r = warp / kWarpRows * kRows + row0 + gr + 8 * i;
+      if (tq == 0) join.mls[r] = make_float2(m[i], l[i]);
 #pragma unroll
       for (int d = 0; d < kDim / 8; ++d)
-        *reinterpret_cast<float2*>(os + (along * kRows + r) * kDim + d * 8 + 2 * tq) =
-            make_float2(o[d][2 * i], o[d][2 * i + 1]);
+        *reinterpret_cast<float2*>(join.os + r * kDim + d * 8 + 2 * tq) = make_float2(o[d][2 * i], o[d][2 * i + 1]);
     }
-    if (late_wait) pdl_wait();  // the prefix's parts
-    __syncthreads();
-    for (int c0 = threadIdx.x; c0 < w.count * a.prefix_slots; c0 += 8 * kThreads) {
-      float2 ml[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int c = c0 + k * kThreads;
-        if (c < w.count * a.prefix_slots) ml[k] = a.part_ml[cell(c / a.prefix_slots) * a.slots + c % a.prefix_slots];
-      }
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (c0 + k * kThreads < w.count * a.prefix_slots) factors[c0 + k * kThreads] = ml[k];
-    }
-    if (threadIdx.x == 0) odd_keys[0] = 0;  // from here on: one more than the last slot with keys
-    __syncthreads();
-    {
-      // All rows at once, kLanes neighbouring threads each.
-      constexpr int kLanes = kThreads / kRows;
-      const int r = threadIdx.x / kLanes, at = threadIdx.x % kLanes;
-      float2* ml = factors + r * a.prefix_slots;
-      const int slots = r < w.count ? a.prefix_slots : 0;
-      float top = -INFINITY;
-      for (int i = at; i < kAlong; i += kLanes) top = fmaxf(top, mls[i * kRows + r].x);
-      for (int s = at; s < slots; s += kLanes) top = fmaxf(top, ml[s].x);
-#pragma unroll
-      for (int off = kLanes / 2; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-      const float shift = top == -INFINITY ? 0.0f : top;
-      float sum = 0.0f;
-      int live = 0;
-      for (int i = at; i < kAlong; i += kLanes) {
-        const float2 p = mls[i * kRows + r];
-        const float f = exp2_fast(p.x - shift);
-        sum = fmaf(p.y, f, sum);
-        own[i * kRows + r] = f;
-      }
-      for (int s = at; s < slots; s += kLanes) {
-        const float2 p = ml[s];
-        const float f = exp2_fast(p.x - shift);
-        sum = fmaf(p.y, f, sum);
-        // A part without keys has no output: its factor is told apart from one that has underflowed.
-        ml[s].x = p.x == -INFINITY ? -1.0f : f;
-        if (p.x != -INFINITY) live = s + 1;
-      }
-#pragma unroll
-      for (int off = kLanes / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-      if (live > 0) atomicMax(&odd_keys[0], static_cast<uint32_t>(live));
-      if (at == 0 && r < w.count) {
-        scales[r] = sum != 0.0f ? 1.0f / sum : 0.0f;
-        if (a.lse != nullptr)
-          a.lse[cell(r)] = sum != 0.0f ? (top + log2f(sum)) * 0.69314718055994530942f : -INFINITY;
-      }
-    }
-    __syncthreads();
-    const int live_slots = static_cast<int>(odd_keys[0]);
-    // 16 pieces of parts under way at a time: of four rows where there are many, of one where there are few.
-    auto join_rows = [&](auto rows_at_once) {
-      constexpr int kR = decltype(rows_at_once)::value, kAhead = 16 / kR;
-      constexpr int kPieces = kDim / 4, kGroups = kThreads / kPieces;
-      const int col = threadIdx.x % kPieces * 4;
-      for (int r0 = threadIdx.x / kPieces * kR; r0 < w.count; r0 += kGroups * kR) {
-        float4 acc[kR];
-        const float* parts[kR];
-        auto add = [](float4& sum, const float4& v, float f) {
-          sum.x = fmaf(v.x, f, sum.x), sum.y = fmaf(v.y, f, sum.y);
-          sum.z = fmaf(v.z, f, sum.z), sum.w = fmaf(v.w, f, sum.w);
-        };
-#pragma unroll
-        for (int k = 0; k < kR; ++k) {
-          acc[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          parts[k] = a.part_o + cell(r0 + k) * a.slots * kDim + col;
-        }
-        for (int s0 = 0; s0 < live_slots; s0 += kAhead) {
-          float4 v[kR][kAhead];
-          float f[kR][kAhead];
-#pragma unroll
-          for (int k = 0; k < kR; ++k)
-#pragma unroll
-            for (int s = 0; s < kAhead; ++s) {
-              f[k][s] = r0 + k < w.count && s0 + s < live_slots ? factors[(r0 + k) * a.prefix_slots + s0 + s].x : -1.0f;
-              v[k][s] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-              if (!(f[k][s] < 0.0f)) v[k][s] = *reinterpret_cast<const float4*>(parts[k] + (s0 + s) * kDim);
-            }
-#pragma unroll
-          for (int k = 0; k < kR; ++k)
-#pragma unroll
-            for (int s = 0; s < kAhead; ++s) add(acc[k], v[k][s], f[k][s]);
-        }
-#pragma unroll
-        for (int k = 0; k < kR; ++k) {
-          const int r = r0 + k;
-          if (r >= w.count) break;
-#pragma unroll
-          for (int i = 0; i < kAlong; ++i)
-            add(acc[k], *reinterpret_cast<const float4*>(os + (i * kRows + r) * kDim + col), own[i * kRows + r]);
-          const int vr = w.start + r;
-          const float scale = scales[r];
-          __nv_bfloat16* out = a.out + static_cast<int64_t>(w.first_row + vr / a.group) * a.ldo +
-                               (w.kv_head * a.group + vr % a.group) * kDim + col;
-          *reinterpret_cast<uint2*>(out) =
-              make_uint2(pack2(acc[k].x * scale, acc[k].y * scale), pack2(acc[k].z * scale, acc[k].w * scale));
-        }
-      }
-    };
-    if (w.count > 16)
-      join_rows(std::integral_constant<int, 4>{});
-    else
-      join_rows(std::integral_constant<int, 1>{});
+    join.run(a, w, odd_keys, late_wait);
   } else {
     if (w.first)  // the slots that no block comes to
       for (int c = threadIdx.x; c < w.count * (w.slots - w.used); c += kThreads)
@@ -515,6 +570,101 @@ __device__ __forceinline__ void attend(const Attention& a, const Segment& seg, u
       }
     }
   }
+}
+
+// At most 8 rows that all see the same own keys (a token's heads): the keys are the
+// rows of the tensor-core tiles and the 8 rows their columns, S^T = K Q^T and
+// O^T = V^T P^T, half the products and registers of 16 padded rows. Each warp takes
+// 16 of a stage's keys.
+template <int kDim>
+__device__ __forceinline__ void attend_few(const Attention& a, const Segment& seg, unsigned char* raw,
+                                           uint32_t* free_word, bool late_wait) {
+  constexpr int kPitch = Feed<kDim>::kPitch, kStage = Feed<kDim>::kStage, kRows = 8;
+  const Segment w = seg;  // in registers
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int gr = lane >> 2, tq = lane & 3;
+  Feed<kDim> feed(a, w, raw);
+  feed.start();
+  uint32_t q[kDim / 16][2];  // row gr
+  const __nv_bfloat16* src =
+      a.q + static_cast<int64_t>(w.first_row) * a.ldq + (w.kv_head * a.group + w.start + gr) * kDim;
+#pragma unroll
+  for (int kk = 0; kk < kDim / 16; ++kk)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      q[kk][i] = gr < w.count ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + i * 8 + 2 * tq) : 0u;
+  float o[kDim / 16][4];
+#pragma unroll
+  for (int d = 0; d < kDim / 16; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.0f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};  // rows 2 tq and 2 tq + 1
+  const __nv_bfloat16* ring = reinterpret_cast<const __nv_bfloat16*>(raw);
+  int stage = 0;
+  for (int key = w.key0; key < w.key1; key += kKeys) {
+    cp_async_wait<kStages - 2>();
+    __syncthreads();  // the stage has landed for all, and the one filled next has been read by all
+    feed.next(key, stage);
+    const __nv_bfloat16* ks = ring + stage * kStage + warp * 16 * kPitch;
+    const __nv_bfloat16* vs = ks + kKeys * kPitch;
+    stage = (stage + 1) % kStages;
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // keys gr, gr + 8 x rows 2 tq, + 1
+#pragma unroll
+    for (int kk = 0; kk < kDim / 16; ++kk) {
+      uint32_t k[4];
+      ldmatrix_x4(k, ks + (lane & 15) * kPitch + kk * 16 + (lane >> 4) * 8);
+      mma_bf16(s, k, q[kk][0], q[kk][1]);
+    }
+    const int at = key + warp * 16 + gr;
+    float alpha[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      s[i] = at < w.key1 ? s[i] * a.scale_log2 : -INFINITY;
+      s[2 + i] = at + 8 < w.key1 ? s[2 + i] * a.scale_log2 : -INFINITY;
+      float top = fmaxf(s[i], s[2 + i]);
+#pragma unroll
+      for (int off = 4; off < 32; off *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+      top = fmaxf(top, m[i]);
+      const float shift = top == -INFINITY ? 0.0f : top;
+      alpha[i] = exp2_fast(m[i] - shift);
+      m[i] = top;
+      s[i] = exp2_fast(s[i] - shift);
+      s[2 + i] = exp2_fast(s[2 + i] - shift);
+      l[i] = fmaf(l[i], alpha[i], s[i] + s[2 + i]);
+    }
+    if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
+#pragma unroll
+      for (int d = 0; d < kDim / 16; ++d) {
+        o[d][0] *= alpha[0];
+        o[d][1] *= alpha[1];
+        o[d][2] *= alpha[0];
+        o[d][3] *= alpha[1];
+      }
+    }
+    const uint32_t p0 = transpose_8x8(pack2(s[0], s[1])), p1 = transpose_8x8(pack2(s[2], s[3]));
+#pragma unroll
+    for (int d = 0; d < kDim / 16; ++d) {
+      uint32_t v[4];
+      ldmatrix_x4_trans(v, vs + ((lane & 7) + (lane >> 4) * 8) * kPitch + d * 16 + (lane >> 3 & 1) * 8);
+      mma_bf16(o[d], v, p0, p1);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int off = 4; off < 32; off *= 2) l[i] += __shfl_xor_sync(0xffffffffu, l[i], off);
+  const LastJoin<kDim, kRows, 4> join(raw);
+  cp_async_wait_all();
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = warp * kRows + 2 * tq + i;
+    if (gr == 0) join.mls[r] = make_float2(m[i], l[i]);
+#pragma unroll
+    for (int d = 0; d < kDim / 16; ++d) {
+      join.os[r * kDim + d * 16 + gr] = o[d][i];
+      join.os[r * kDim + d * 16 + gr + 8] = o[d][2 + i];
+    }
+  }
+  join.run(a, w, free_word, late_wait);
 }
 
 template <int kDim, int kPrefixWarps, int kOwnWarps>
@@ -611,9 +761,10 @@ __global__ void __launch_bounds__(kThreads, kBlocks) attention_rows_kernel(Atten
 
 // A block for all own keys of a tile of a sequence's rows, which also joins the
 // prefix's parts and writes the rows. Blocks: tiles of all sequences x heads.
+// kWarps 0: at most 8 rows, without row offsets.
 template <int kDim, int kWarps>
 __global__ void __launch_bounds__(kThreads, kBlocks) attention_last_kernel(Attention a, int late_wait) {
-  constexpr int kRows = 16 * kWarps;
+  constexpr int kRows = kWarps == 0 ? 8 : 16 * kWarps;
   extern __shared__ __align__(16) unsigned char raw[];
   __shared__ uint32_t odd_keys[kKeys / 32];
   __shared__ Segment seg;
@@ -658,10 +809,13 @@ __global__ void __launch_bounds__(kThreads, kBlocks) attention_last_kernel(Atten
     }
   }
   __syncthreads();
-  if (seg.count > 0)
+  if (seg.count == 0) {
+    if (late_wait) pdl_wait();
+  } else if constexpr (kWarps == 0) {
+    attend_few<kDim>(a, seg, raw, odd_keys, late_wait != 0);
+  } else {
     attend<kDim, kWarps, true>(a, seg, raw, odd_keys, late_wait != 0);
-  else if (late_wait)
-    pdl_wait();
+  }
 }
 
 // kWarps warps join the parts of a (row, head): first all maxima and sums, a lane a part, then the outputs of the parts
@@ -829,9 +983,10 @@ cudaError_t launch_rows(const Attention& a, const Grid& g, unsigned blocks, cuda
 
 template <int kDim, int kWarps>
 cudaError_t launch_last(const Attention& a, unsigned blocks, int late_wait, cudaStream_t stream) {
-  constexpr size_t kRing = static_cast<size_t>(kStages) * 2 * kKeys * (kDim + 8) * 2;
-  const size_t join = 64 * (kDim * 4 + 8 + 4) + 16 * kWarps * (4 + a.prefix_slots * 8);
-  cudaError_t st = allow_max_dynamic_smem_once<attention_last_kernel<kDim, kWarps>>();
+  constexpr size_t kRing = static_cast<size_t>(kStages) * Feed<kDim>::kStage * 2;
+  const size_t join = kWarps == 0 ? LastJoin<kDim, 8, 4>::bytes(a.prefix_slots)
+                                  : LastJoin<kDim, 16 * kWarps, 4 / std::max(kWarps, 1)>::bytes(a.prefix_slots);
+  const cudaError_t st = allow_max_dynamic_smem_once<attention_last_kernel<kDim, kWarps>>();
   if (st != cudaSuccess) return st;
   return launch_pdl(attention_last_kernel<kDim, kWarps>, blocks, kThreads, std::max(kRing, join), stream, a, late_wait);
 }
@@ -858,6 +1013,8 @@ cudaError_t launch(const uocr_prefix_attention_args& args, const Attention& a, c
   if (p.whole_own) {
     const int late = p.tc || p.blocks > 0;
     const unsigned n = static_cast<unsigned>(p.own_tiles * a.kv_heads);
+    // One row a sequence and at most 8 heads to a key: the 8-row form (it counts as many tiles).
+    if (a.row_offsets == nullptr && a.group <= 8) return launch_last<kDim, 0>(a, n, late, stream);
     return p.own_warps == 1   ? launch_last<kDim, 1>(a, n, late, stream)
            : p.own_warps == 2 ? launch_last<kDim, 2>(a, n, late, stream)
                               : launch_last<kDim, 4>(a, n, late, stream);

@@ -35,7 +35,9 @@ namespace uocr_b200 {
 namespace {
 
 constexpr int kTileRows = kAttentionTcRows;
-constexpr unsigned kRangeUnits = 4;  // what a range costs besides its keys: 7 us, where 128 keys take 1.8
+// What a range costs besides its keys, 7 us, in units: 128 keys take 1.8 us for two tiles of rows, 0.6 (the memory's
+// rate) where the tiles split them.
+__device__ __forceinline__ unsigned range_units(const Attention& a) { return a.split ? 12 : 4; }
 constexpr int kTcKeys = 128;
 constexpr int kSlots = 4;        // shared-memory slots of 128 keys or values
 constexpr int kTcThreads = 384;  // a warpgroup for copies and MMAs, two of rows
@@ -196,7 +198,7 @@ __device__ __forceinline__ unsigned units_of(const Attention& a, int p, Prefix* 
   const int of_range = a.split ? kTileRows : 2 * kTileRows;
   x->ranges = (x->rows * a.group + of_range - 1) / of_range;
   x->tiles = max(1, (x->len + kTcKeys - 1) / kTcKeys);  // an empty prefix still has a part: no keys
-  return static_cast<unsigned>(a.kv_heads) * x->ranges * (x->tiles + kRangeUnits);
+  return static_cast<unsigned>(a.kv_heads) * x->ranges * (x->tiles + range_units(a));
 }
 __device__ __forceinline__ unsigned warp_scan(unsigned v) {
   const int lane = threadIdx.x & 31;
@@ -259,9 +261,9 @@ __device__ __forceinline__ void next_segment(const Attention& a, Schedule& c, Se
     const bool mine = c.unit < upto && c.unit >= upto - n;
     unsigned to = 0;
     if (mine) {
-      const unsigned each = x.tiles + kRangeUnits;
+      const unsigned each = x.tiles + range_units(a);
       const unsigned local = c.unit - (upto - n), range = local / each, at = local - range * each;
-      const unsigned first = c.unit - at + kRangeUnits, head = range / x.ranges;  // first: the unit of the first keys
+      const unsigned first = c.unit - at + range_units(a), head = range / x.ranges;  // first: the unit of the first keys
       const int of_range = a.split ? kTileRows : 2 * kTileRows;
       to = min(c.unit - at + each, c.end);
       s->prefix = p0 + lane;
