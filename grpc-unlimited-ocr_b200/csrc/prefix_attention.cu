@@ -21,6 +21,9 @@ constexpr int kThreads = 128;
 constexpr int kKeys = 64;    // of a stage
 constexpr int kStages = 2;
 constexpr int kBlocks = 3;   // of an SM
+// Stages of a block at least: with 1, 2 and 4 the four rows of a page of 273 keys take 13.9, 14.2 and 12.9 us, the
+// parts that fewer make costing the join more than the blocks save.
+constexpr int kMinShare = 4;
 constexpr int kMaxSlots = 160;  // of a row: the most that a plan gives its prefix and its own keys
 constexpr int kMaxPrefixSlots = 64, kMaxOwnSlots = 32, kMaxTcSlots = 128;
 static_assert(kMaxPrefixSlots + kMaxOwnSlots <= kMaxSlots && kMaxTcSlots + kMaxOwnSlots <= kMaxSlots, "");
@@ -701,7 +704,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) attention_rows_kernel(Atten
   }
   // No range of keys meets more blocks than there are slots for it.
   const int own_slots = a.slots - a.prefix_slots;
-  unsigned share = max((total + gridDim.x - 1) / gridDim.x, 1u);
+  unsigned share = max((total + gridDim.x - 1) / gridDim.x, static_cast<unsigned>(kMinShare));
   if (g.prefixes > 0) share = max(share, (most[0] + a.prefix_slots - 2u) / (a.prefix_slots - 1u));
   if (g.sequences > 0) share = max(share, (most[1] + own_slots - 2u) / (own_slots - 1u));
   unsigned unit = blockIdx.x * share;
@@ -955,7 +958,7 @@ Plan plan_of(const uocr_prefix_attention_args& a) {
                     (p.whole_own ? 0 : p.own_tiles * own_stages));
   p.blocks = static_cast<unsigned>(std::min<int64_t>(units, kBlocks * kSms));
   // A range of keys meets as many blocks as shares fit into it, and one more; half as many again for lengths that differ.
-  const int64_t share = std::max<int64_t>((units + kBlocks * kSms - 1) / (kBlocks * kSms), 1);
+  const int64_t share = std::max<int64_t>((units + kBlocks * kSms - 1) / (kBlocks * kSms), kMinShare);
   auto slots = [&](int64_t stages, int most) {
     return static_cast<int>(stages == 0 ? 0 : std::min<int64_t>((stages + share - 1) / share * 3 / 2 + 2, most));
   };
@@ -965,7 +968,10 @@ Plan plan_of(const uocr_prefix_attention_args& a) {
     p.split = a.rows * group <= kAttentionTcRows * a.prefixes;
     const int64_t of_range = kAttentionTcRows * (p.split ? 1 : 2);
     const int64_t ranges = a.kv_heads * std::max((a.rows * group + of_range - 1) / of_range, p.split ? a.prefixes : 1);
-    p.prefix_slots = static_cast<int>(std::min<int64_t>((kSms / ranges + 3) * (p.split ? 2 : 1), kMaxTcSlots));
+    // Blocks a range can meet: as many as there are for each, and no more than its keys make (two tiles a block at least).
+    const int64_t tiles = (a.prefix_capacity + 127) / 128;
+    const int64_t blocks = std::max<int64_t>(std::min(kSms / ranges + 3, tiles / 2 + 2), 3);
+    p.prefix_slots = static_cast<int>(std::min<int64_t>(blocks * (p.split ? 2 : 1), kMaxTcSlots));
   }
   return p;
 }
