@@ -83,6 +83,9 @@ __device__ uint64_t bound_of(uint64_t best, int select, uint64_t* shared, uint64
   return bound;
 }
 
+// A maximum in the log2 domain, rounded here and everywhere to the same float: fused into a difference it would not be.
+__device__ __forceinline__ float log2_of(float m) { return __fmul_rn(m, kLog2e); }
+
 struct Select {
   const void* logits;
   const float* scores;
@@ -187,11 +190,11 @@ __global__ void __launch_bounds__(kThreads, 3) beam_parts_kernel(Select a) {
     }
     if (base + kRound < end) load(base + kRound, ahead);
     if (peak > m) {
-      sum *= exp2_fast(m * kLog2e - peak * kLog2e);  // of no element yet: 0 * 0
+      sum *= exp2_fast(log2_of(m) - log2_of(peak));  // of no element yet: 0 * 0
       m = peak;
     }
     // 2^(f log2 e - m log2 e), the second product rounded for all elements alike: the join takes it as it is.
-    const float shift = m > -INFINITY ? m * kLog2e : 0.0f;
+    const float shift = m > -INFINITY ? log2_of(m) : 0.0f;
     float of_round = 0.0f;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) of_round += exp2_fast(fmaf(f[i], kLog2e, -shift));
@@ -234,7 +237,7 @@ __global__ void __launch_bounds__(kThreads, 3) beam_parts_kernel(Select a) {
   float top = m;
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-  sum = warp_sum(m > -INFINITY ? sum * exp2_fast(m * kLog2e - top * kLog2e) : 0.0f);
+  sum = warp_sum(m > -INFINITY ? sum * exp2_fast(log2_of(m) - log2_of(top)) : 0.0f);
   if ((threadIdx.x & 31) == 0) warp_sums[threadIdx.x >> 5] = make_float2(top, sum);
   __syncthreads();
   const int64_t cell = row * a.parts + part;
@@ -244,8 +247,8 @@ __global__ void __launch_bounds__(kThreads, 3) beam_parts_kernel(Select a) {
       const float2 p = warp_sums[w];
       const float high = fmaxf(all.x, p.x);
       if (high == -INFINITY) continue;
-      all = make_float2(high, all.y * exp2_fast(all.x * kLog2e - high * kLog2e) +
-                                  p.y * exp2_fast(p.x * kLog2e - high * kLog2e));
+      all = make_float2(high, all.y * exp2_fast(log2_of(all.x) - log2_of(high)) +
+                                  p.y * exp2_fast(log2_of(p.x) - log2_of(high)));
     }
     a.sums[cell] = all;
   }
@@ -283,7 +286,7 @@ __device__ __forceinline__ bool better(const Cand& a, const Cand& b) {
 }
 
 // What a part's exponents are less (its maximum in the log2 domain, as rounded there).
-__device__ __forceinline__ double shift_of(float m) { return static_cast<double>(m * kLog2e); }
+__device__ __forceinline__ double shift_of(float m) { return static_cast<double>(log2_of(m)); }
 
 constexpr int kJoinThreads = 512;
 constexpr int kLanes = 4;  // neighbouring threads that rank a candidate

@@ -344,3 +344,134 @@ def test_reorder_states_reports_bad_parents_and_counts(cuda):
     assert e.value.code == 5 and "units" in str(e.value)
     assert state[0].tolist() == [0] * 10 and state[1].tolist() == [0] * 10
     assert state[2].tolist() == [3] * 4 + [2] * 6
+
+
+# ---- many rows
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("heads,kv,dim,rot", [(16, 4, 128, 128), (10, 10, 128, 64), (3, 1, 64, 64), (5, 5, 80, 32),
+                                              (2, 2, 256, 256), (9, 3, 8, 8), (4, 2, 128, 0), (30, 30, 64, 64),
+                                              (28, 1, 128, 96)])
+def test_rotate_heads_of_many_rows(cuda, dtype, interleaved, heads, kv, dim, rot):
+    run_rotate(4001, heads, kv, dim, rot, dtype, interleaved=interleaved, caches=13)
+
+
+@pytest.mark.parametrize("kw", [dict(norm="q"), dict(norm="k"), dict(norm=""), dict(far=3000000), dict(pad=8, dtype="bfloat16"),
+                                dict(pad=4), dict(pad=5), dict(pad=7, shift=1, dtype="bfloat16"), dict(shift=4, pad=4),
+                                dict(own_places=False, caches=1), dict(rows=2368), dict(rows=2367), dict(rows=20000, caches=5),
+                                dict(norm="", magnitude=1.4, dtype="bfloat16")])
+def test_rotate_heads_of_many_rows_forms(cuda, kw):
+    run_rotate(**{**dict(rows=5003, heads=8, kv=2, dim=128, rot=64, caches=7), **kw})
+
+
+def test_rotate_heads_of_many_rows_in_place_and_without_keys(cuda):
+    import torch
+    rows = 9001
+    q = torch.randn(rows, 4, 64, generator=gen_of(3), device="cuda").to(torch.bfloat16)
+    inv, _ = M.rope_frequencies(64)
+    pos = torch.arange(rows, dtype=torch.int32, device="cuda")
+    none = torch.empty(rows, 0, 64, dtype=torch.bfloat16, device="cuda")
+    cache = torch.empty(rows, 0, 8, 64, dtype=torch.bfloat16, device="cuda")
+    want = rotated(q, None, inv.cuda(), pos, False, 0.0, 1.0)
+    M.rotate_heads(q, none, none, inv.cuda(), pos, q, cache, cache)
+    close(q, *want)
+
+
+def test_rotate_heads_of_many_rows_reports_places_that_do_not_exist(cuda):
+    import torch
+    rows = 6000
+    x = torch.ones(rows, 1, 64, device="cuda")
+    cache = torch.zeros(4, 1, 2000, 64, dtype=torch.bfloat16, device="cuda")
+    vcache, out = torch.zeros_like(cache), torch.empty(rows, 1, 64, dtype=torch.bfloat16, device="cuda")
+    at = torch.arange(rows, dtype=torch.int32, device="cuda")
+    places, slots = at // 2000, at % 2000
+    good = torch.ones(rows, dtype=torch.bool, device="cuda")
+    for row, place, slot in ((7, 4, 0), (2500, -1, 5), (4444, 1, 2000), (5999, 3, -1)):
+        places[row], slots[row], good[row] = place, slot, False
+    M.rotate_heads(x, x, x, torch.ones(32, device="cuda"), torch.zeros_like(at), out, cache, vcache,
+                   cache_rows=places, slots=slots)
+    with pytest.raises(M.UocrError) as e:
+        M.ops_check()
+    assert e.value.code == 5
+    want = torch.zeros(4, 2000, device="cuda")
+    want[places[good].long(), slots[good].long()] = 1
+    assert (out == 1).all() and torch.equal(vcache[:, 0].float(), want[..., None].expand(4, 2000, 64))
+    assert torch.equal(cache, vcache)
+    M.ops_check()
+
+
+@pytest.mark.parametrize("rows", [5, 7000])
+def test_rotate_heads_on_a_stream_and_from_a_graph(cuda, rows):
+    import torch
+    g = gen_of(rows, 21)
+    q, k, v = (torch.randn(rows, h, 128, generator=g, device="cuda") for h in (8, 2, 2))
+    inv, _ = M.rope_frequencies(128)
+    inv = inv.cuda()
+    pos = torch.arange(rows, dtype=torch.int32, device="cuda")
+    kc = torch.zeros(1, 2, 2 * rows, 128, dtype=torch.bfloat16, device="cuda")
+    vc, out = torch.zeros_like(kc), torch.empty(rows, 8, 128, dtype=torch.bfloat16, device="cuda")
+    places = torch.zeros_like(pos)
+
+    def verify():
+        close(out, *rotated(q, None, inv, pos, False, 1e-6, 1.0))
+        close(kc[0, :, pos.long()].transpose(0, 1), *rotated(k, None, inv, pos, False, 1e-6, 1.0))
+        assert torch.equal(vc[0, :, pos.long()].transpose(0, 1), v.to(torch.bfloat16))
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    M.rotate_heads(q, k, v, inv, pos, out, kc, vc, cache_rows=places, stream=side)
+    torch.cuda.synchronize()
+    verify()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        M.rotate_heads(q, k, v, inv, pos, out, kc, vc, cache_rows=places)
+    pos += rows // 2
+    q.mul_(1.5)
+    v.neg_()
+    graph.replay()
+    torch.cuda.synchronize()
+    verify()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("batch,beams,select,vocab", [(4, 32, 32, 102400), (150, 3, 8, 8193), (1, 32, 32, 1 << 20),
+                                                      (500, 1, 1, 4097), (64, 16, 32, 20000)])
+def test_beam_select_of_large_groups(cuda, dtype, batch, beams, select, vocab):
+    import torch
+    g = gen_of(batch, beams, select, vocab, 3)
+    logits = (torch.randn(batch * beams, vocab, generator=g, device="cuda") * 3).to(getattr(torch, dtype))
+    scores = -10 * torch.rand(batch, beams, generator=g, device="cuda")
+    for b in range(0, batch, 20):  # in pieces: the plain form holds several copies in 64 bits
+        of = slice(b, min(b + 20, batch))
+        check_select(logits[of.start * beams:of.stop * beams], scores[of].contiguous(), select)
+    tokens = torch.empty(batch, select, dtype=torch.int32, device="cuda")
+    parents, new = torch.empty_like(tokens), torch.empty(batch, select, device="cuda")
+    M.beam_select(logits, scores, tokens, parents, new)
+    for b in (0, batch // 2, batch - 1):
+        one = check_select(logits[b * beams:(b + 1) * beams], scores[b:b + 1].contiguous(), select)
+        # A group's parts depend on how many rows the call has, and with them a sum's last bits.
+        assert (new[b] - one[2][0]).abs().max() <= 50 * 2.0 ** -23 + 2.0 ** -22 * new[b].abs().max()
+
+
+def test_reorder_states_on_a_stream_and_from_a_graph(cuda):
+    import torch
+    g = gen_of(31)
+    state = torch.randint(0, 1000, (2, 8, 2, 50, 64), generator=g, device="cuda", dtype=torch.int32)
+    parents = torch.tensor([3, 0, 0, 1, 1, 2, 3, 0], dtype=torch.int32, device="cuda")
+    counts = torch.tensor([50, 3, 0, 49, 20, 21, 1, 50], dtype=torch.int32, device="cuda")
+    want = reordered(state, parents, 4, counts)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    M.reorder_states(state, parents, 4, counts=counts, stream=side)
+    torch.cuda.synchronize()
+    assert torch.equal(state, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        M.reorder_states(state, parents, 4, counts=counts)
+    for turn in range(3):
+        parents.copy_(torch.randint(0, 4, (8,), generator=g, device="cuda"))
+        counts.copy_(torch.randint(0, 51, (8,), generator=g, device="cuda"))
+        want = reordered(state, parents, 4, counts)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(state, want)

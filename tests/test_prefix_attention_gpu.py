@@ -296,3 +296,124 @@ def test_the_lse_joins_parts_of_a_prefix(cuda):
     _, _, tol, _ = plain(c)
     # each half and the whole within their tolerances: the halves' add up to at most the whole's of |a| and |b|
     assert ((both - c["out"].double()).abs() <= 3 * tol + 2.0 ** -7 * (a.abs() + b.abs())).all()
+
+
+# ---- many rows of many prefixes, and keys in parts
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_many_prefixes_with_many_rows(cuda, dim):
+    lengths = [(37 * i) % 700 if i % 5 else 0 for i in range(40)]
+    check(make(lengths, [(11 * i) % 90 for i in range(200)], 8, 2, dim))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_many_prefixes_with_more_rows_than_a_tile(cuda, dim):
+    rows = [50 + i % 3 if i % 7 else 0 for i in range(70)]
+    lens = [n + (5 * i) % 60 for i, n in enumerate(rows)]
+    check(make([(53 * i) % 400 for i in range(35)], lens, 8, 2, dim, rows=rows))
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(16, 4, 128), (8, 2, 64), (12, 1, 128)])
+@pytest.mark.parametrize("rows", [[90, 2, 2], [2, 1, 0], [0, 0, 96], [600, 0, 1], [1, 129, 300]])
+def test_prefixes_with_unlike_rows(cuda, rows, heads, kv, dim):
+    check(make([1000, 50, 2700], [max(n, 40) for n in rows], heads, kv, dim, rows=rows, first_row=2, rows_behind=3))
+
+
+@pytest.mark.parametrize("what", ["prefix_lens", "lens", "ancestry", "row_offsets"])
+def test_bad_values_with_many_rows_are_reported(cuda, what):
+    import torch
+    for value in (1 << 30, -5):
+        c = make([200, 100], [20, 30, 10, 5], 8, 2, 128, rows=[30, 40, 10, 30], beams=True)
+        if what == "ancestry":
+            c[what][1, 7] = value
+        else:
+            c[what][1] = value
+        M.prefix_attention(**c)
+        with pytest.raises(M.UocrError) as e:
+            M.ops_check()
+        assert e.value.code == 5 and "prefix_attention" in str(e.value)
+        M.ops_check()
+        if what in ("prefix_lens", "lens") and value < 0:
+            c[what][1] = 0
+            check(c)
+
+
+@pytest.mark.parametrize("scale", [-0.2, 0.0])
+def test_scales_that_are_not_positive(cuda, scale):
+    c = make([600, 90], [40, 70, 20, 33], 8, 2, 128, rows=[40, 30, 20, 1])
+    c["scale"] = scale
+    check(c)
+
+
+@pytest.mark.parametrize("rows", [None, [40, 50, 30, 64]])
+def test_heads_and_sequences_that_share_memory(cuda, rows):
+    c = make([300, 200], [60, 70, 30, 90], 8, 2, 64, rows=rows)
+    for name in ("prefix_k", "prefix_v"):
+        c[name] = c[name][:, :1].expand(-1, 2, -1, -1)
+    for name in ("k", "v"):
+        c[name] = c[name][:, 1:].expand(-1, 2, -1, -1)
+    check(c)
+
+
+def test_nan_rows_of_many_stay_alone(cuda):
+    import torch
+    c = make([900, 300], [60, 70], 8, 2, 128, rows=[60, 70])
+    c["q"][17] = math.nan
+    c["prefix_v"][1, :, 11] = math.inf  # the second prefix's rows alone
+    M.prefix_attention(**c)
+    got = c["out"].float()
+    others = [r for r in range(60) if r != 17]
+    assert got[17].isnan().all() and got[others].isfinite().all() and got[60:].isinf().all()
+
+
+@pytest.mark.parametrize("beams", [False, True])
+@pytest.mark.parametrize("heads,kv,dim", [(8, 2, 128), (12, 12, 64), (24, 2, 64)])
+@pytest.mark.parametrize("prefix_lens,lens", [([100], [3000, 10, 0, 600]), ([0, 70], [1, 2000]), ([300], [5000])])
+def test_long_own_keys(cuda, prefix_lens, lens, heads, kv, dim, beams):
+    check(make(prefix_lens, lens, heads, kv, dim, beams=beams))
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 128), (9, 1, 64)])
+def test_long_own_keys_of_several_rows(cuda, heads, kv, dim):
+    check(make([400, 1], [2000, 3, 900, 700], heads, kv, dim, rows=[5, 6, 0, 33]))
+    check(make([400], [2500], heads, kv, dim, rows=[150], beams=True))
+
+
+def test_a_prefix_for_each_of_many_sequences(cuda):
+    check(make([(17 * i) % 300 for i in range(140)], [(29 * i) % 900 for i in range(140)], 4, 1, 64, capacity=905))
+    check(make([(17 * i) % 300 for i in range(300)], [(29 * i) % 90 for i in range(300)], 4, 2, 128))
+
+
+@pytest.mark.parametrize("heads,kv", [(24, 2), (16, 4), (8, 1)])
+def test_many_beams_with_and_without_own_keys(cuda, heads, kv):
+    check(make([500, 0], [0, 3, 90, 64, 65, 0, 1, 200] * 10, heads, kv, 128, beams=True))
+
+
+def test_many_rows_on_a_stream_and_from_a_graph(cuda):
+    import torch
+    c = make([900, 0, 300], [60, 70, 40], 8, 2, 128, rows=[60, 70, 33])
+    d = make([500], [1000, 7], 8, 2, 64, seed=5)
+    check(c)
+    want, side = c["out"].clone(), torch.cuda.Stream()
+    for _ in range(4):
+        c["out"].fill_(33.0)
+        torch.cuda.synchronize()
+        M.prefix_attention(**c, stream=side)
+        M.prefix_attention(**d)
+        torch.cuda.synchronize()
+        assert torch.equal(c["out"], want)
+    check(d, call=False)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        M.prefix_attention(**c)
+    c["prefix_lens"].copy_(torch.tensor([0, 500, 301], device="cuda"))
+    for name in ("prefix_k", "prefix_v"):
+        c[name][1, :, :500] = 0.5
+        c[name][2, :, 300] = 0.25
+    c["row_offsets"].copy_(torch.tensor([0, 20, 90, 163], device="cuda"))
+    c["lens"].copy_(torch.tensor([20, 70, 45], device="cuda"))
+    for name in ("k", "v"):
+        c[name].nan_to_num_(0.125)
+    graph.replay()
+    torch.cuda.synchronize()
+    check(c, call=False)
