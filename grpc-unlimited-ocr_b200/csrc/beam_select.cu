@@ -51,13 +51,14 @@ __device__ __forceinline__ uint64_t key_of(float f, uint32_t index) {
 }
 
 // The warp's keys in descending order over its lanes.
-__device__ __forceinline__ uint64_t sort_lanes(uint64_t key) {
+template <typename Key>
+__device__ __forceinline__ Key sort_lanes(Key key) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int size = 2; size <= 32; size *= 2)
 #pragma unroll
     for (int step = size / 2; step > 0; step /= 2) {
-      const uint64_t other = __shfl_xor_sync(0xffffffffu, key, step);
+      const Key other = __shfl_xor_sync(0xffffffffu, key, step);
       const bool keep_high = ((lane & size) == 0) == ((lane & step) == 0);
       key = (other > key) == keep_high ? other : key;
     }
@@ -65,21 +66,15 @@ __device__ __forceinline__ uint64_t sort_lanes(uint64_t key) {
 }
 
 // A lower bound on the select-th best of the block's elements, from each
-// thread's best: the best of the warps' select-th ones. All threads call it;
-// *top receives the best of all. `shared`: 2 * kWarps keys.
-__device__ uint64_t bound_of(uint64_t best, int select, uint64_t* shared, uint64_t* top) {
-  const uint64_t sorted = sort_lanes(best);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (lane == select - 1) shared[warp] = sorted;
-  if (lane == 0) shared[kWarps + warp] = sorted;
+// thread's best: the best of the warps' select-th ones. All threads call it.
+template <typename Key>
+__device__ __forceinline__ Key bound_of(Key best, int select, uint64_t* shared) {
+  const Key sorted = sort_lanes(best);
+  if (static_cast<int>(threadIdx.x & 31) == select - 1) shared[threadIdx.x >> 5] = sorted;
   __syncthreads();
-  uint64_t bound = 1, first = 0;
+  Key bound = 1;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    bound = max(bound, shared[w]);
-    first = max(first, shared[kWarps + w]);
-  }
-  *top = first;
+  for (int w = 0; w < kWarps; ++w) bound = max(bound, static_cast<Key>(shared[w]));
   return bound;
 }
 
@@ -108,7 +103,7 @@ __device__ uint64_t cut(uint64_t* list, int* count, int* next, int select, uint6
   for (int before = 2 * n; n > kRanked && n * 5 < before * 4;) {
     constexpr int kMost = (kList + kThreads - 1) / kThreads;
     uint64_t mine[kMost];
-    uint64_t high = 0, top;
+    uint64_t high = 0;
 #pragma unroll
     for (int i = 0; i < kMost; ++i) {
       const int at = i * kThreads + static_cast<int>(threadIdx.x);
@@ -116,7 +111,7 @@ __device__ uint64_t cut(uint64_t* list, int* count, int* next, int select, uint6
       high = max(high, mine[i]);
     }
     if (threadIdx.x == 0) *next = 0;
-    const uint64_t bound = bound_of(high, select, bounds, &top);
+    const uint64_t bound = bound_of(high, select, bounds);
 #pragma unroll
     for (int i = 0; i < kMost; ++i)
       if (mine[i] >= bound) list[atomicAdd(next, 1)] = mine[i];
@@ -126,12 +121,13 @@ __device__ uint64_t cut(uint64_t* list, int* count, int* next, int select, uint6
     __syncthreads();
   }
 #pragma unroll 1
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const uint64_t key = list[i];
+  for (int i = threadIdx.x / 2; i < (n + 15) / 16 * 16; i += kThreads / 2) {  // two neighbouring threads a key; whole warps
+    const uint64_t key = i < n ? list[i] : ~0ull;
     int rank = 0;
-#pragma unroll 4
-    for (int j = 0; j < n; ++j) rank += list[j] > key;
-    if (rank < select) best[rank] = key;
+#pragma unroll 8
+    for (int j = threadIdx.x & 1; j < n; j += 2) rank += list[j] > key;
+    rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+    if (i < n && rank < select) best[rank] = key;
   }
   __syncthreads();
   n = min(n, select);
@@ -146,7 +142,7 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads, 3) beam_parts_kernel(Select a) {
   constexpr int kVec = 16 / sizeof(T);
   extern __shared__ uint64_t list[];  // [kList]
-  __shared__ uint64_t bounds[2 * kWarps];
+  __shared__ uint64_t bounds[kWarps];
   __shared__ float2 warp_sums[kWarps];
   __shared__ uint64_t best[UOCR_BEAM_MAX];
   __shared__ int count, next;
@@ -154,9 +150,8 @@ __global__ void __launch_bounds__(kThreads, 3) beam_parts_kernel(Select a) {
   pdl_launch_dependents();
   const int64_t row = blockIdx.x / a.parts;
   const int part = blockIdx.x % a.parts;
-  // The second kernel asks for nothing of a beam that has ended or does not exist.
-  if ((a.finished != nullptr && a.finished[row] != 0) || !(a.scores[row] > -INFINITY)) return;
-  if (threadIdx.x == 0) count = 0;
+  const bool ended = a.finished != nullptr && a.finished[row] != 0;
+  const float score = a.scores[row];
   const T* src = static_cast<const T*>(a.logits) + row * a.ld;
   const int begin = part * a.part, end = min(a.vocab, begin + a.part);
   float m = -INFINITY, sum = 0.0f;  // of this thread
@@ -178,8 +173,13 @@ __global__ void __launch_bounds__(kThreads, 3) beam_parts_kernel(Select a) {
       }
     }
   };
-  float ahead[kEach];
+  float ahead[kEach], further[kEach];  // the next two rounds'
   load(begin, ahead);
+  if (begin + kRound < end) load(begin + kRound, further);
+  // The second kernel asks for nothing of a beam that has ended or does not exist. Found out with the first loads under
+  // way, not before them: one round trip less where the beam goes on.
+  if (ended || !(score > -INFINITY)) return;
+  if (threadIdx.x == 0) count = 0;
   for (int base = begin; base < end; base += kRound) {
     float f[kEach];
     float peak = -INFINITY;
@@ -188,7 +188,9 @@ __global__ void __launch_bounds__(kThreads, 3) beam_parts_kernel(Select a) {
       f[i] = fmaxf(ahead[i], -INFINITY);  // NaN counts as -inf
       peak = fmaxf(peak, f[i]);
     }
-    if (base + kRound < end) load(base + kRound, ahead);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) ahead[i] = further[i];
+    if (base + 2 * kRound < end) load(base + 2 * kRound, further);
     if (peak > m) {
       sum *= exp2_fast(log2_of(m) - log2_of(peak));  // of no element yet: 0 * 0
       m = peak;
@@ -203,12 +205,10 @@ __global__ void __launch_bounds__(kThreads, 3) beam_parts_kernel(Select a) {
       return static_cast<uint32_t>(base + (i / kVec * kThreads + static_cast<int>(threadIdx.x)) * kVec + i % kVec);
     };
     if (bound == 0) {
-      uint64_t first = 0, top;
-#pragma unroll
-      for (int i = kEach - 1; i >= 0; --i)
-        if (f[i] == peak) first = key_of(f[i], index(i));
-      bound = bound_of(first, a.select, bounds, &top);
-      at_least = unordered(max(static_cast<uint32_t>(bound >> 32), ordered(-INFINITY)));
+      // By the values alone, in half the steps: of equal ones the first cut tells the best.
+      const uint32_t value = max(bound_of(ordered(peak), a.select, bounds), ordered(-INFINITY));
+      bound = static_cast<uint64_t>(value) << 32;
+      at_least = unordered(value);
     }
     unsigned reach = 0;
     if (peak >= at_least) {
@@ -264,6 +264,7 @@ struct Join {
   float* new_scores;
   int* new_finished;
   int eos;
+  int depth;  // 1 .. select
 };
 
 // A candidate in the order of the selection: the score, then the lower beam and
@@ -300,13 +301,15 @@ __device__ __forceinline__ int rank_of(const Cand& mine, const Cand* of, int n) 
   return rank + __shfl_xor_sync(0xffffffffu, rank, 2);
 }
 
-// A block joins a group. Only the parts with the `select` best first entries can
-// hold any of the `select` best candidates, and of those only the entries that are
-// not below the select-th best first entry. Everything of the group is read in one
-// round, the keys too where they fit (kStage).
+// A block joins a group, whose lists (parts) are in descending order. The `depth`
+// first entries of each are ranked against one another: further entries of a list
+// are candidates only where the last of those is among the `select` best, and then
+// only the ones that are not below the select-th best. (With the first entries alone
+// 200 candidates were left of sixteen pages' 24 lists, and 3.7 us for their ranks.)
+// Everything of the group is read in one round, the keys too where they fit (kStage).
 template <bool kStaged>
 __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(Join a) {
-  extern __shared__ Cand heads[];  // [beams * parts], then [select * select], then the keys
+  extern __shared__ Cand heads[];  // [beams * parts * depth], then [select * select], then the keys
   __shared__ double lse[UOCR_BEAM_MAX];
   __shared__ float scores[UOCR_BEAM_MAX];
   __shared__ int ended[UOCR_BEAM_MAX];
@@ -314,8 +317,8 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(Join a) {
   __shared__ int lists[UOCR_BEAM_MAX];
   __shared__ int chosen, count;
   const Select& s = a.s;
-  const int n = s.beams * s.parts;
-  Cand* left = heads + n;
+  const int n = s.beams * s.parts, depth = a.depth;
+  Cand* left = heads + n * depth;
   uint64_t* staged = reinterpret_cast<uint64_t*>(left + s.select * s.select);
   pdl_wait();
   pdl_launch_dependents();
@@ -374,20 +377,24 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(Join a) {
     }
     return e;
   };
-  for (int i = threadIdx.x; i < n; i += kJoinThreads) heads[i] = entry(i, 0);
+  // Entry `at` of all lists, then the next one's: neighbouring threads have different lists.
+  for (int i = threadIdx.x; i < n * depth; i += kJoinThreads) heads[i] = entry(i % n, i / n);
   __syncthreads();
-  for (int i0 = 0; i0 < n; i0 += kJoinThreads / kLanes) {
+  for (int i0 = 0; i0 < n * depth; i0 += kJoinThreads / kLanes) {
     const int i = i0 + threadIdx.x / kLanes;
-    const Cand mine = i < n ? heads[i] : Cand{0, ~0ull};
-    const int rank = rank_of(mine, heads, n);
-    if (mine.score == 0 || threadIdx.x % kLanes != 0) continue;
-    if (rank < s.select) lists[atomicAdd(&chosen, 1)] = i;
+    const Cand mine = i < n * depth ? heads[i] : Cand{0, ~0ull};
+    const int rank = rank_of(mine, heads, n * depth);
+    if (mine.score == 0 || threadIdx.x % kLanes != 0 || rank >= s.select) continue;
+    left[atomicAdd(&count, 1)] = mine;
     if (rank == s.select - 1) worst = mine;
+    if (i >= n * (depth - 1)) lists[atomicAdd(&chosen, 1)] = i % n;
   }
   __syncthreads();
-  const bool full = chosen == s.select;
-  for (int i = threadIdx.x; i < chosen * s.select; i += kJoinThreads) {
-    const Cand e = entry(lists[i / s.select], i % s.select);
+  const bool full = count == s.select;
+  const int further = s.select - depth, deep = chosen;  // at most select / depth lists: `left` has room for them
+  __syncthreads();
+  for (int i = threadIdx.x; i < deep * further; i += kJoinThreads) {
+    const Cand e = entry(lists[i / further], depth + i % further);
     if (e.score != 0 && !(full && better(worst, e))) left[atomicAdd(&count, 1)] = e;
   }
   __syncthreads();
@@ -426,7 +433,7 @@ int parts_of(const uocr_beam_select_args& a) {
 template <typename T>
 cudaError_t launch(const uocr_beam_select_args& a, const Join& j, cudaStream_t stream) {
   const size_t keys = static_cast<size_t>(j.s.beams) * j.s.parts * j.s.select * sizeof(uint64_t);
-  const size_t join_smem = (static_cast<size_t>(j.s.beams) * j.s.parts + j.s.select * j.s.select) * sizeof(Cand);
+  const size_t join_smem = (static_cast<size_t>(j.s.beams) * j.s.parts * j.depth + j.s.select * j.s.select) * sizeof(Cand);
   const bool staged = keys <= 64 * 1024;
   cudaError_t st = allow_max_dynamic_smem_once<beam_parts_kernel<T>>();
   if (st == cudaSuccess) st = allow_max_dynamic_smem_once<beam_join_kernel<true>>();
@@ -461,6 +468,8 @@ cudaError_t launch_beam_select(const uocr_beam_select_args& a, cudaStream_t stre
   s.sums = reinterpret_cast<float2*>(s.best + cells * a.select);
   j.tokens = a.tokens, j.parents = a.parents, j.new_scores = a.new_scores, j.new_finished = a.new_finished;
   j.eos = a.eos;
+  // As many entries as the block ranks in one go.
+  j.depth = std::clamp(kJoinThreads / kLanes / (s.beams * s.parts), 1, s.select);
   return a.dtype == UOCR_DTYPE_BF16 ? launch<__nv_bfloat16>(a, j, stream) : launch<float>(a, j, stream);
 }
 
