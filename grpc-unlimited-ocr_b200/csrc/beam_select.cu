@@ -154,83 +154,113 @@ __global__ void __launch_bounds__(kThreads, 3) beam_parts_kernel(Select a) {
   const float score = a.scores[row];
   const T* src = static_cast<const T*>(a.logits) + row * a.ld;
   const int begin = part * a.part, end = min(a.vocab, begin + a.part);
-  float m = -INFINITY, sum = 0.0f;  // of this thread
-  uint64_t bound = 0;
-  float at_least = -INFINITY;
-  auto load = [&](int base, float* f) {
+  // A round's elements of this thread, as they lie in memory: kVec side by side, then those kThreads * kVec further on.
+  struct Raw {
+    uint4 v[kEach / kVec];
+  };
+  auto index = [&](int base, int i) {
+    return base + (i / kVec * kThreads + static_cast<int>(threadIdx.x)) * kVec + i % kVec;
+  };
+  auto load = [&](int base) {
+    Raw r;
+    if (a.vec && base + kRound <= end) {
+      const uint4* p = reinterpret_cast<const uint4*>(src + base) + threadIdx.x;
+#pragma unroll
+      for (int j = 0; j < kEach / kVec; ++j) r.v[j] = p[j * kThreads];
+      return r;
+    }
 #pragma unroll
     for (int j = 0; j < kEach / kVec; ++j) {
-      const int at = base + (j * kThreads + static_cast<int>(threadIdx.x)) * kVec;
-      float* g = f + j * kVec;
-      if (a.vec && at + kVec <= end) {
-        const uint4 u = *reinterpret_cast<const uint4*>(src + at);
-        const T* e = reinterpret_cast<const T*>(&u);
+      uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) g[i] = to_f32(e[i]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) g[i] = at + i < end ? to_f32(src[at + i]) : -INFINITY;
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) {
+          const int at = index(base, j * kVec + i);
+          w[i] = at < end ? __float_as_uint(src[at]) : 0xff800000u;
+        } else {
+          const int at = index(base, j * kVec + 2 * i);
+          const unsigned short* of = reinterpret_cast<const unsigned short*>(src);
+          w[i] = (at < end ? of[at] : 0xff80u) | (at + 1 < end ? of[at + 1] : 0xff80u) << 16;
+        }
       }
+      r.v[j] = make_uint4(w[0], w[1], w[2], w[3]);
     }
+    return r;
   };
-  float ahead[kEach], further[kEach];  // the next two rounds'
-  load(begin, ahead);
-  if (begin + kRound < end) load(begin + kRound, further);
+  auto value_of = [](const Raw& r, int i) {
+    const uint4& u = r.v[i / kVec];
+    const int at = i % kVec;
+    const int word = sizeof(T) == 4 ? at : at / 2;
+    const uint32_t w = word == 0 ? u.x : word == 1 ? u.y : word == 2 ? u.z : u.w;
+    return __uint_as_float(sizeof(T) == 4 ? w : at % 2 == 0 ? w << 16 : w & 0xffff0000u);
+  };
+  Raw ahead = load(begin);
   // The second kernel asks for nothing of a beam that has ended or does not exist. Found out with the first loads under
   // way, not before them: one round trip less where the beam goes on.
   if (ended || !(score > -INFINITY)) return;
   if (threadIdx.x == 0) count = 0;
+  float m = -INFINITY, sum = 0.0f;  // of this thread
+  uint64_t bound = 0;
+  float at_least = -INFINITY;
   for (int base = begin; base < end; base += kRound) {
     float f[kEach];
     float peak = -INFINITY;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      f[i] = fmaxf(ahead[i], -INFINITY);  // NaN counts as -inf
-      peak = fmaxf(peak, f[i]);
+      f[i] = value_of(ahead, i);
+      peak = fmaxf(peak, f[i]);  // of no NaN
     }
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) ahead[i] = further[i];
-    if (base + 2 * kRound < end) load(base + 2 * kRound, further);
+    if (base + kRound < end) ahead = load(base + kRound);
     if (peak > m) {
       sum *= exp2_fast(log2_of(m) - log2_of(peak));  // of no element yet: 0 * 0
       m = peak;
     }
     // 2^(f log2 e - m log2 e), the second product rounded for all elements alike: the join takes it as it is.
     const float shift = m > -INFINITY ? log2_of(m) : 0.0f;
-    float of_round = 0.0f;
+    float2 of_round = make_float2(0.0f, 0.0f);
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) of_round += exp2_fast(fmaf(f[i], kLog2e, -shift));
-    sum += of_round;
-    auto index = [&](int i) {
-      return static_cast<uint32_t>(base + (i / kVec * kThreads + static_cast<int>(threadIdx.x)) * kVec + i % kVec);
-    };
+    for (int i = 0; i < kEach; i += 2) {
+      const float2 x = fma2(make_float2(f[i], f[i + 1]), make_float2(kLog2e, kLog2e), make_float2(-shift, -shift));
+      of_round = add2(of_round, make_float2(exp2_fast(x.x), exp2_fast(x.y)));
+    }
+    float added = of_round.x + of_round.y;
+    if (added != added) {  // NaN counts as -inf; beside +inf the sum is not asked for
+      added = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) added += exp2_fast(fmaf(fmaxf(f[i], -INFINITY), kLog2e, -shift));
+    }
+    sum += added;
     if (bound == 0) {
       // By the values alone, in half the steps: of equal ones the first cut tells the best.
       const uint32_t value = max(bound_of(ordered(peak), a.select, bounds), ordered(-INFINITY));
       bound = static_cast<uint64_t>(value) << 32;
       at_least = unordered(value);
     }
-    unsigned reach = 0;
+    bool many = false;
     if (peak >= at_least) {
+      unsigned reach = 0;
 #pragma unroll
       for (int i = 0; i < kEach; ++i) reach |= f[i] >= at_least ? 1u << i : 0u;
-    }
-    while (reach != 0) {  // one branch for the few threads that have any
-      const int i = __ffs(reach) - 1;
-      reach &= reach - 1;
-      float v = f[0];
+      while (reach != 0) {  // few threads have any, and those mostly one
+        const int i = __ffs(reach) - 1;
+        reach &= reach - 1;
+        float v[kEach / 2];
 #pragma unroll
-      for (int k = 1; k < kEach; ++k) v = i == k ? f[k] : v;
-      const uint64_t key = key_of(v, index(i));
-      if (key >= bound) list[atomicAdd(&count, 1)] = key;
+        for (int k = 0; k < 8; ++k) v[k] = (i & 8) != 0 ? f[k + 8] : f[k];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = (i & 4) != 0 ? v[k + 4] : v[k];
+        const float lo = (i & 2) != 0 ? v[2] : v[0], hi = (i & 2) != 0 ? v[3] : v[1];
+        const uint64_t key = key_of((i & 1) != 0 ? hi : lo, static_cast<uint32_t>(index(base, i)));
+        if (key < bound) continue;
+        const int at = atomicAdd(&count, 1);
+        list[at] = key;
+        many |= at >= list_limit(a.select);
+      }
     }
-    __syncthreads();
     // The bound is drawn anew when the list grows, at once after the first round: from then on few elements pass.
-    if (count > list_limit(a.select)) {
+    if (__syncthreads_or(many)) {
       bound = max(bound, cut(list, &count, &next, a.select, bounds, best));
       at_least = unordered(max(static_cast<uint32_t>(bound >> 32), ordered(-INFINITY)));
-    } else {
-      __syncthreads();  // the count has been read by all
     }
   }
   // The block's maximum and sum.
