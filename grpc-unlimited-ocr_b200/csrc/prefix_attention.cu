@@ -578,16 +578,59 @@ __device__ __forceinline__ void attend(const Attention& a, const Segment& seg, u
 // At most 8 rows that all see the same own keys (a token's heads): the keys are the
 // rows of the tensor-core tiles and the 8 rows their columns, S^T = K Q^T and
 // O^T = V^T P^T, half the products and registers of 16 padded rows. Each warp takes
-// 16 of a stage's keys.
+// 16 of 64 keys and brings them itself, into three slots of its own for 16 keys or
+// values (K V K, then V K V): no barrier before the join, and with 52 KB a block
+// four blocks an SM, so that 512 ranges of own keys are under way at once (with
+// three some had to wait for the end of others: 59 us for sixteen pages, now 57).
+template <int kDim>
+struct FewRing {
+  static constexpr int kSlot = 16 * (kDim + 8), kSlots = 3;
+  static constexpr size_t kBytes = static_cast<size_t>(kThreads / 32) * kSlots * kSlot * 2;
+};
 template <int kDim>
 __device__ __forceinline__ void attend_few(const Attention& a, const Segment& seg, unsigned char* raw,
                                            uint32_t* free_word, bool late_wait) {
-  constexpr int kPitch = Feed<kDim>::kPitch, kStage = Feed<kDim>::kStage, kRows = 8;
+  constexpr int kPitch = kDim + 8, kRows = 8;
+  constexpr int kStep = 32 / (kDim / 8), kCopies = 16 / kStep;  // a lane copies 16 bytes of every kStep-th key
   const Segment w = seg;  // in registers
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gr = lane >> 2, tq = lane & 3;
-  Feed<kDim> feed(a, w, raw);
-  feed.start();
+  const bool gathers = a.ancestry != nullptr;
+  const int64_t base = (gathers ? 0 : w.of * a.cache_stride) + w.kv_head * a.head_stride;
+  const int copy_key = warp * 16 + lane / (kDim / 8), col = lane % (kDim / 8) * 8;
+  __nv_bfloat16* const ring = reinterpret_cast<__nv_bfloat16*>(raw) + warp * FewRing<kDim>::kSlots * FewRing<kDim>::kSlot;
+  int from[kCopies];  // the caches of the next 64 keys, read ahead of the copies
+  auto look_up = [&](int key) {
+    if (!gathers) return;
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) {
+      const int at = key + copy_key + i * kStep;
+      from[i] = at < w.key1 ? a.ancestry[w.of * a.ld_ancestry + at] : 0;
+    }
+  };
+  auto copy = [&](const __nv_bfloat16* of, int slot, int key, bool check) {
+    __nv_bfloat16* to = ring + slot * FewRing<kDim>::kSlot + lane / (kDim / 8) * kPitch + col;
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) {
+      const int at = key + copy_key + i * kStep;
+      const bool valid = at < w.key1;
+      int64_t off = valid ? static_cast<int64_t>(at) * kDim + col : 0;
+      if (gathers) {
+        if (check && valid && (from[i] < 0 || from[i] >= a.caches)) {
+          raise_error(a.err, kDevBadIndex, kSiteAncestor, w.of, from[i]);
+          from[i] = w.of < a.caches ? w.of : 0;
+        }
+        off += from[i] * a.cache_stride;
+      }
+      cp_async16_or_zero(to + i * kStep * kPitch, of + base + off, valid);
+    }
+  };
+  look_up(w.key0);
+  if (w.key0 < w.key1) copy(a.k, 0, w.key0, true);
+  cp_async_commit();
+  if (w.key0 < w.key1) copy(a.v, 1, w.key0, false);
+  cp_async_commit();
+  look_up(w.key0 + kKeys);
   uint32_t q[kDim / 16][2];  // row gr
   const __nv_bfloat16* src =
       a.q + static_cast<int64_t>(w.first_row) * a.ldq + (w.kv_head * a.group + w.start + gr) * kDim;
@@ -600,15 +643,15 @@ __device__ __forceinline__ void attend_few(const Attention& a, const Segment& se
 #pragma unroll
   for (int d = 0; d < kDim / 16; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.0f;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};  // rows 2 tq and 2 tq + 1
-  const __nv_bfloat16* ring = reinterpret_cast<const __nv_bfloat16*>(raw);
-  int stage = 0;
+  int slot = 0;  // of the keys; the values' is the one after it, the next keys' the third
   for (int key = w.key0; key < w.key1; key += kKeys) {
-    cp_async_wait<kStages - 2>();
-    __syncthreads();  // the stage has landed for all, and the one filled next has been read by all
-    feed.next(key, stage);
-    const __nv_bfloat16* ks = ring + stage * kStage + warp * 16 * kPitch;
-    const __nv_bfloat16* vs = ks + kKeys * kPitch;
-    stage = (stage + 1) % kStages;
+    const int next = key + kKeys, slot1 = (slot + 1) % 3, slot2 = (slot + 2) % 3;
+    cp_async_wait<1>();
+    __syncwarp();  // the keys have landed, the values before them have been read
+    if (next < w.key1) copy(a.k, slot2, next, true);
+    cp_async_commit();
+    const __nv_bfloat16* ks = ring + slot * FewRing<kDim>::kSlot;
+    const __nv_bfloat16* vs = ring + slot1 * FewRing<kDim>::kSlot;
     float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // keys gr, gr + 8 x rows 2 tq, + 1
 #pragma unroll
     for (int kk = 0; kk < kDim / 16; ++kk) {
@@ -643,6 +686,12 @@ __device__ __forceinline__ void attend_few(const Attention& a, const Segment& se
       }
     }
     const uint32_t p0 = transpose_8x8(pack2(s[0], s[1])), p1 = transpose_8x8(pack2(s[2], s[3]));
+    cp_async_wait<1>();
+    __syncwarp();  // the values have landed, the keys have been read
+    if (next < w.key1) copy(a.v, slot, next, false);
+    cp_async_commit();
+    look_up(next + kKeys);
+    slot = slot2;
 #pragma unroll
     for (int d = 0; d < kDim / 16; ++d) {
       uint32_t v[4];
@@ -766,7 +815,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) attention_rows_kernel(Atten
 // prefix's parts and writes the rows. Blocks: tiles of all sequences x heads.
 // kWarps 0: at most 8 rows, without row offsets.
 template <int kDim, int kWarps>
-__global__ void __launch_bounds__(kThreads, kBlocks) attention_last_kernel(Attention a, int late_wait) {
+__global__ void __launch_bounds__(kThreads, kWarps == 0 ? 4 : kBlocks) attention_last_kernel(Attention a, int late_wait) {
   constexpr int kRows = kWarps == 0 ? 8 : 16 * kWarps;
   extern __shared__ __align__(16) unsigned char raw[];
   __shared__ uint32_t odd_keys[kKeys / 32];
@@ -989,7 +1038,7 @@ cudaError_t launch_rows(const Attention& a, const Grid& g, unsigned blocks, cuda
 
 template <int kDim, int kWarps>
 cudaError_t launch_last(const Attention& a, unsigned blocks, int late_wait, cudaStream_t stream) {
-  constexpr size_t kRing = static_cast<size_t>(kStages) * Feed<kDim>::kStage * 2;
+  constexpr size_t kRing = kWarps == 0 ? FewRing<kDim>::kBytes : static_cast<size_t>(kStages) * Feed<kDim>::kStage * 2;
   const size_t join = kWarps == 0 ? LastJoin<kDim, 8, 4>::bytes(a.prefix_slots)
                                   : LastJoin<kDim, 16 * kWarps, 4 / std::max(kWarps, 1)>::bytes(a.prefix_slots);
   const cudaError_t st = allow_max_dynamic_smem_once<attention_last_kernel<kDim, kWarps>>();
