@@ -21,6 +21,7 @@
 #include <string>
 #include <utility>
 
+#include "uocr_beam.h"
 #include "uocr_int8.h"
 #include "uocr_moe.h"
 
@@ -99,6 +100,33 @@ inline std::int64_t grouped_w8a8_workspace(const uocr_grouped_w8a8_args& args) {
 }
 inline void grouped_linear_w8a8(void* stream, const uocr_grouped_w8a8_args& args) {
   check(uocr_grouped_linear_w8a8(&args, stream));
+}
+
+// The operators for sequences that share a page (uocr_beam.h), with the same exceptions.
+// table: inv_freq [rotary_dim / 2]; returns the factor of cos and sin.
+inline float rope_frequencies(std::int64_t rotary_dim, double theta, uocr_rope_scaling scaling, double factor,
+                              std::int64_t original, float* table) {
+  float magnitude = 1.0f;
+  check(uocr_rope_frequencies(rotary_dim, theta, scaling, factor, original, table, &magnitude));
+  return magnitude;
+}
+inline void rotate_heads(void* stream, const uocr_rotate_heads_args& args) { check(uocr_rotate_heads(&args, stream)); }
+inline std::int64_t prefix_attention_workspace(const uocr_prefix_attention_args& args) {
+  std::int64_t bytes = 0;
+  check(uocr_prefix_attention_workspace(&args, &bytes));
+  return bytes;
+}
+inline void prefix_attention(void* stream, const uocr_prefix_attention_args& args) {
+  check(uocr_prefix_attention(&args, stream));
+}
+inline std::int64_t beam_select_workspace(const uocr_beam_select_args& args) {
+  std::int64_t bytes = 0;
+  check(uocr_beam_select_workspace(&args, &bytes));
+  return bytes;
+}
+inline void beam_select(void* stream, const uocr_beam_select_args& args) { check(uocr_beam_select(&args, stream)); }
+inline void reorder_states(void* stream, const uocr_reorder_states_args& args) {
+  check(uocr_reorder_states(&args, stream));
 }
 
 // ---- owners ------------------------------------------------------------------

@@ -223,3 +223,42 @@ def test_beam_search_refuses_before_a_decoder_is_touched():
     args = M.BeamSearchArgs(4, 8, -1, 0, BASE, BASE, None, BASE, BIG)
     assert M.lib().uocr_decoder_beam_search(None, ctypes.byref(args), None) == 1
     assert M.lib().uocr_last_error().decode().startswith("decoder_beam_search: ")
+
+
+def test_cpp_wrapper(tmp_path):
+    """The header-only C++ layer's functions: values through it, the library's refusals as std::invalid_argument."""
+    cxx = shutil.which("g++")
+    if cxx is None:
+        pytest.skip("no C++ compiler")
+    src = tmp_path / "beam.cpp"
+    src.write_text(r"""
+#include <cstdio>
+#include "uocr_moe.hpp"
+template <typename F> static int throws(F&& f) {
+  try { f(); } catch (const std::invalid_argument&) { return 1; }
+  return 0;
+}
+int main() {
+  float table[32];
+  const float magnitude = uocr_b200::rope_frequencies(64, 1e4, UOCR_ROPE_YARN, 4.0, 4096, table);
+  uocr_rotate_heads_args r{};
+  r.rows = 1, r.q_heads = 1, r.head_dim = 7;
+  uocr_prefix_attention_args a{};
+  a.rows = -1;
+  uocr_beam_select_args s{};
+  s.batch = 1, s.beams = 33;
+  uocr_reorder_states_args o{};
+  o.layers = 1, o.groups = 1, o.beams = 33;
+  std::printf("%d %d %d %d %d %d %.6f\n", throws([&] { uocr_b200::rotate_heads(nullptr, r); }),
+              throws([&] { uocr_b200::prefix_attention(nullptr, a); }),
+              throws([&] { uocr_b200::prefix_attention_workspace(a); }),
+              throws([&] { uocr_b200::beam_select(nullptr, s); }),
+              throws([&] { uocr_b200::beam_select_workspace(s); }),
+              throws([&] { uocr_b200::reorder_states(nullptr, o); }), magnitude);
+}
+""")
+    exe = tmp_path / "beam"
+    lib = os.path.dirname(M.LIB_PATH)
+    subprocess.run([cxx, "-std=c++17", "-I", INCLUDE, str(src), "-o", str(exe), M.LIB_PATH, f"-Wl,-rpath,{lib}"], check=True)
+    out = subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()
+    assert out[:6] == ["1"] * 6 and abs(float(out[6]) - (0.1 * math.log(4.0) + 1)) < 1e-6
