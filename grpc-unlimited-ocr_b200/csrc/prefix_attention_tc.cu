@@ -326,8 +326,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
       if (tiles == 0 || abort_flag != 0) break;
       if (warp == 0) {
         // ---- keys and values, in the order in which the products take them (key_fill, value_fill). The last tile ends
-        // with the prefix: it begins among keys that were there before, which are masked, and nothing behind the
-        // prefix is read. ----
+        // with the prefix: it begins among keys that the tile before it has too, and nothing behind the prefix is read. ----
         auto fill = [&](const Segment& of, uint32_t first, uint32_t k) {
           const uint32_t n = first + k, slot = n % kSlots;
           if (!mbar_wait(&bars.empty[slot], (n / kSlots & 1) ^ 1)) {
@@ -479,15 +478,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
       named_bar_sync(2, 32 + 256);  // its Q is there
       // ---- a row: its scores to weights ----
       const int t = (warp - 4) / 4, in_tile = (threadIdx.x - 128) % kTileRows, r = a.split ? in_tile : threadIdx.x - 128;
-      // The tile's rounds, and the one that ends with the prefix, if it has it.
       const int my_rounds = a.split ? (tiles + 1 - t) / 2 : t < pair ? tiles : 0;
-      const bool has_end = s.tile1 == s.tiles && (!a.split || (tiles - 1) % 2 == t);
       if (my_rounds > 0 || a.split) {
         const uint32_t at = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         const uint32_t s_at = at + t * kTcKeys, o_at = at + 2 * kTcKeys + t * kDim;
         float m = -INFINITY, l = 0.0f;  // m: of the raw scores
-        const int skip_last = has_end ? s.tiles * kTcKeys - s.len : 0;
         const bool has_rows = r - lane < s.count;  // of this warp
+        // Rounds times two, where the tiles split the keys: of the prefix's last tile but one, if it shares keys with the
+        // last. (An empty prefix is told apart below.)
+        const int doubled = a.split ? 1 : 0;
+        const int shared_from = s.len % kTcKeys != 0 ? s.tiles - 2 - s.tile0 - (a.split ? t : 0) : 1 << 30;
         bool ok = true;
         for (int i = 0; i < my_rounds; ++i) {
           if (!__all_sync(0xffffffffu, mbar_wait(&bars.s_full[t], (rounds[0] + i) & 1))) {
@@ -506,11 +506,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
 #pragma unroll
           for (int c = 0; c < kTcKeys; c += 32) tmem_ld32_async(s_at + c, x + c);
           tmem_ld_done(x);
-          const int skip = i == my_rounds - 1 ? skip_last : 0;
-          if (skip > 0) {
+          // A key that the prefix's last two tiles both have counts half in each. (Not 0 in one of them: an infinite value
+          // times 0 is NaN.) In a single tile they lie before the first key, where the copy brings zeros, and are none.
+          if ((i << doubled) >= shared_from) {
+            const int twice = -s.len & (kTcKeys - 1);
+            const float less = s.tiles == 1 ? INFINITY : 1.0f / a.scale_log2;
+            if ((i << doubled) > shared_from) {  // the last
 #pragma unroll
-            for (int c = 0; c < kTcKeys; ++c)
-              if (c < skip) x[c] = __float_as_uint(-INFINITY);
+              for (int c = 0; c < kTcKeys; ++c)
+                if (c < twice) x[c] = __float_as_uint(__uint_as_float(x[c]) - less);
+            } else {
+#pragma unroll
+              for (int c = 0; c < kTcKeys; ++c)
+                if (c >= kTcKeys - twice) x[c] = __float_as_uint(__uint_as_float(x[c]) - less);
+            }
           }
           float top[4];
 #pragma unroll
@@ -577,7 +586,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
         const int slot = a.split ? 2 * s.slot + t : s.slot;
         const bool mine = r < s.count && ok;
         if (mine) {
-          a.part_ml[cell + slot] = make_float2(m == -INFINITY ? m : m * a.scale_log2, l);
+          a.part_ml[cell + slot] = m == -INFINITY || s.len == 0 ? make_float2(-INFINITY, 0.0f) : make_float2(m * a.scale_log2, l);
           if (s.tile0 == 0 && (t == 0 || !a.split))  // the slots that no block comes to
             for (int k = a.split ? 2 * s.used : s.used; k < a.prefix_slots; ++k)
               a.part_ml[cell + k] = make_float2(-INFINITY, 0.0f);

@@ -355,6 +355,17 @@ def test_heads_and_sequences_that_share_memory(cuda, rows):
     check(c)
 
 
+@pytest.mark.parametrize("length", [64, 128, 129, 200, 257, 300, 511])
+def test_infinite_values_stay_infinite(cuda, length):
+    """One visible value after another is infinite: so are its rows, and no other."""
+    for key in sorted({0, length // 3, length // 2, length - 2, length - 1}):
+        c = make([length, 90], [60, 70], 8, 2, 128, rows=[60, 70])
+        c["prefix_v"][0, 1, key] = -math.inf
+        M.prefix_attention(**c)
+        got = c["out"].float()
+        assert (got[:60, 4:] == -math.inf).all() and got[:60, :4].isfinite().all() and got[60:].isfinite().all()
+
+
 def test_nan_rows_of_many_stay_alone(cuda):
     import torch
     c = make([900, 300], [60, 70], 8, 2, 128, rows=[60, 70])
