@@ -21,8 +21,8 @@ constexpr int kThreads = 128;
 constexpr int kKeys = 64;    // of a stage
 constexpr int kStages = 2;
 constexpr int kBlocks = 3;   // of an SM
-// Stages of a block at least: with 1, 2 and 4 the four rows of a page of 273 keys take 13.9, 14.2 and 12.9 us, the
-// parts that fewer make costing the join more than the blocks save.
+// Stages of a block at least: with 2, 3, 4 and 6 the four rows of a page take 12.8, 14.4, 11.7 and 15.2 us, the parts
+// that fewer make costing the join more than the blocks save.
 constexpr int kMinShare = 4;
 constexpr int kMaxSlots = 160;  // of a row: the most that a plan gives its prefix and its own keys
 constexpr int kMaxPrefixSlots = 64, kMaxOwnSlots = 32, kMaxTcSlots = 128;
@@ -200,7 +200,7 @@ struct Feed {
 // The end of a block that has all own keys of its rows: their kAlong parts, which
 // the warps leave in the ring's place, and the prefix's are joined and the rows
 // written.
-template <int kDim, int kRows, int kAlong>
+template <int kDim, int kRows, int kAlong, int kBlock = kThreads>  // kBlock: threads
 struct LastJoin {
   float* os;        // [kAlong][kRows][kDim]
   float2* mls;      // [kAlong][kRows]
@@ -226,22 +226,22 @@ struct LastJoin {
     };
     if (late_wait) pdl_wait();  // the prefix's parts
     __syncthreads();
-    for (int c0 = threadIdx.x; c0 < w.count * a.prefix_slots; c0 += 8 * kThreads) {
+    for (int c0 = threadIdx.x; c0 < w.count * a.prefix_slots; c0 += 8 * kBlock) {
       float2 ml[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const int c = c0 + k * kThreads;
+        const int c = c0 + k * kBlock;
         if (c < w.count * a.prefix_slots) ml[k] = a.part_ml[cell(c / a.prefix_slots) * a.slots + c % a.prefix_slots];
       }
 #pragma unroll
       for (int k = 0; k < 8; ++k)
-        if (c0 + k * kThreads < w.count * a.prefix_slots) factors[c0 + k * kThreads] = ml[k];
+        if (c0 + k * kBlock < w.count * a.prefix_slots) factors[c0 + k * kBlock] = ml[k];
     }
     if (threadIdx.x == 0) *live = 0;  // from here on: one more than the last slot with keys
     __syncthreads();
     {
       // All rows at once, kLanes neighbouring threads each.
-      constexpr int kLanes = kThreads / kRows;
+      constexpr int kLanes = kBlock / kRows;
       const int r = threadIdx.x / kLanes, at = threadIdx.x % kLanes;
       float2* ml = factors + r * a.prefix_slots;
       const int slots = r < w.count ? a.prefix_slots : 0;
@@ -281,7 +281,7 @@ struct LastJoin {
     // 16 pieces of parts under way at a time: of four rows where there are many, of one where there are few.
     auto join_rows = [&](auto rows_at_once) {
       constexpr int kR = decltype(rows_at_once)::value, kAhead = 16 / kR;
-      constexpr int kPieces = kDim / 4, kGroups = kThreads / kPieces;
+      constexpr int kPieces = kDim / 4, kGroups = kBlock / kPieces;
       const int col = threadIdx.x % kPieces * 4;
       for (int r0 = threadIdx.x / kPieces * kR; r0 < w.count; r0 += kGroups * kR) {
         float4 acc[kR];
@@ -578,38 +578,49 @@ __device__ __forceinline__ void attend(const Attention& a, const Segment& seg, u
 // At most 8 rows that all see the same own keys (a token's heads): the keys are the
 // rows of the tensor-core tiles and the 8 rows their columns, S^T = K Q^T and
 // O^T = V^T P^T, half the products and registers of 16 padded rows. Each warp takes
-// 16 of 64 keys and brings them itself, into three slots of its own for 16 keys or
-// values (K V K, then V K V): no barrier before the join, and with 52 KB a block
-// four blocks an SM, so that 512 ranges of own keys are under way at once (with
-// three some had to wait for the end of others: 59 us for sixteen pages, now 57).
-template <int kDim>
+// 16 of a round's keys and brings them itself, into three slots of its own for 16
+// keys or values (K V K, then V K V): no barrier before the join, and with 52 KB a
+// block of four warps four blocks an SM, so that 512 ranges of own keys are under
+// way at once (with three some had to wait for the end of others: sixteen pages 59
+// against 57 us). Blocks that have an SM to themselves take eight warps and half the
+// rounds: four beams 13.5 against 11.7 us.
+template <int kDim, int kWarps>
 struct FewRing {
   static constexpr int kSlot = 16 * (kDim + 8), kSlots = 3;
-  static constexpr size_t kBytes = static_cast<size_t>(kThreads / 32) * kSlots * kSlot * 2;
+  static constexpr size_t kBytes = static_cast<size_t>(kWarps) * kSlots * kSlot * 2;
 };
-template <int kDim>
-__device__ __forceinline__ void attend_few(const Attention& a, const Segment& seg, unsigned char* raw,
-                                           uint32_t* free_word, bool late_wait) {
-  constexpr int kPitch = kDim + 8, kRows = 8;
+template <int kDim, int kWarps>
+__device__ __forceinline__ void attend_few(const Attention& a, unsigned char* raw, uint32_t* free_word, bool late_wait) {
+  constexpr int kPitch = kDim + 8, kRows = 8, kRound = 16 * kWarps;
   constexpr int kStep = 32 / (kDim / 8), kCopies = 16 / kStep;  // a lane copies 16 bytes of every kStep-th key
-  const Segment w = seg;  // in registers
+  using Ring = FewRing<kDim, kWarps>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gr = lane >> 2, tq = lane & 3;
   const bool gathers = a.ancestry != nullptr;
-  const int64_t base = (gathers ? 0 : w.of * a.cache_stride) + w.kv_head * a.head_stride;
   const int copy_key = warp * 16 + lane / (kDim / 8), col = lane % (kDim / 8) * 8;
-  __nv_bfloat16* const ring = reinterpret_cast<__nv_bfloat16*>(raw) + warp * FewRing<kDim>::kSlots * FewRing<kDim>::kSlot;
-  int from[kCopies];  // the caches of the next 64 keys, read ahead of the copies
-  auto look_up = [&](int key) {
+  Segment w{};  // a sequence's row and a key/value head
+  w.of = w.first_row = blockIdx.x / a.kv_heads;
+  w.kv_head = blockIdx.x % a.kv_heads;
+  w.count = a.group;
+  const int64_t base = (gathers ? 0 : w.of * a.cache_stride) + w.kv_head * a.head_stride;
+  __nv_bfloat16* const ring = reinterpret_cast<__nv_bfloat16*>(raw) + warp * Ring::kSlots * Ring::kSlot;
+  int from[kCopies];  // the caches of the next round's keys, read ahead of the copies
+  auto look_up = [&](int key, int end) {
     if (!gathers) return;
 #pragma unroll
     for (int i = 0; i < kCopies; ++i) {
       const int at = key + copy_key + i * kStep;
-      from[i] = at < w.key1 ? a.ancestry[w.of * a.ld_ancestry + at] : 0;
+      from[i] = at < end ? a.ancestry[w.of * a.ld_ancestry + at] : 0;
     }
   };
+  look_up(0, a.capacity);  // beside the length, not behind it: what is no key's is not used
+  if (a.capacity > 0) {
+    const int n = a.lens[w.of];
+    if ((n < 0 || n > a.capacity) && threadIdx.x == 0) raise_error(a.err, kDevBadIndex, kSiteLength, w.of, n);
+    w.key1 = min(max(n, 0), a.capacity);
+  }
   auto copy = [&](const __nv_bfloat16* of, int slot, int key, bool check) {
-    __nv_bfloat16* to = ring + slot * FewRing<kDim>::kSlot + lane / (kDim / 8) * kPitch + col;
+    __nv_bfloat16* to = ring + slot * Ring::kSlot + lane / (kDim / 8) * kPitch + col;
 #pragma unroll
     for (int i = 0; i < kCopies; ++i) {
       const int at = key + copy_key + i * kStep;
@@ -620,17 +631,16 @@ __device__ __forceinline__ void attend_few(const Attention& a, const Segment& se
           raise_error(a.err, kDevBadIndex, kSiteAncestor, w.of, from[i]);
           from[i] = w.of < a.caches ? w.of : 0;
         }
-        off += from[i] * a.cache_stride;
+        off += valid ? from[i] * a.cache_stride : 0;
       }
       cp_async16_or_zero(to + i * kStep * kPitch, of + base + off, valid);
     }
   };
-  look_up(w.key0);
-  if (w.key0 < w.key1) copy(a.k, 0, w.key0, true);
+  if (w.key1 > 0) copy(a.k, 0, 0, true);
   cp_async_commit();
-  if (w.key0 < w.key1) copy(a.v, 1, w.key0, false);
+  if (w.key1 > 0) copy(a.v, 1, 0, false);
   cp_async_commit();
-  look_up(w.key0 + kKeys);
+  look_up(kRound, w.key1);
   uint32_t q[kDim / 16][2];  // row gr
   const __nv_bfloat16* src =
       a.q + static_cast<int64_t>(w.first_row) * a.ldq + (w.kv_head * a.group + w.start + gr) * kDim;
@@ -644,14 +654,14 @@ __device__ __forceinline__ void attend_few(const Attention& a, const Segment& se
   for (int d = 0; d < kDim / 16; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.0f;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};  // rows 2 tq and 2 tq + 1
   int slot = 0;  // of the keys; the values' is the one after it, the next keys' the third
-  for (int key = w.key0; key < w.key1; key += kKeys) {
-    const int next = key + kKeys, slot1 = (slot + 1) % 3, slot2 = (slot + 2) % 3;
+  for (int key = 0; key < w.key1; key += kRound) {
+    const int next = key + kRound, slot1 = (slot + 1) % 3, slot2 = (slot + 2) % 3;
     cp_async_wait<1>();
     __syncwarp();  // the keys have landed, the values before them have been read
     if (next < w.key1) copy(a.k, slot2, next, true);
     cp_async_commit();
-    const __nv_bfloat16* ks = ring + slot * FewRing<kDim>::kSlot;
-    const __nv_bfloat16* vs = ring + slot1 * FewRing<kDim>::kSlot;
+    const __nv_bfloat16* ks = ring + slot * Ring::kSlot;
+    const __nv_bfloat16* vs = ring + slot1 * Ring::kSlot;
     float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // keys gr, gr + 8 x rows 2 tq, + 1
 #pragma unroll
     for (int kk = 0; kk < kDim / 16; ++kk) {
@@ -690,7 +700,7 @@ __device__ __forceinline__ void attend_few(const Attention& a, const Segment& se
     __syncwarp();  // the values have landed, the keys have been read
     if (next < w.key1) copy(a.v, slot, next, false);
     cp_async_commit();
-    look_up(next + kKeys);
+    look_up(next + kRound, w.key1);
     slot = slot2;
 #pragma unroll
     for (int d = 0; d < kDim / 16; ++d) {
@@ -703,7 +713,7 @@ __device__ __forceinline__ void attend_few(const Attention& a, const Segment& se
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int off = 4; off < 32; off *= 2) l[i] += __shfl_xor_sync(0xffffffffu, l[i], off);
-  const LastJoin<kDim, kRows, 4> join(raw);
+  const LastJoin<kDim, kRows, kWarps, 32 * kWarps> join(raw);
   cp_async_wait_all();
   __syncthreads();
 #pragma unroll
@@ -813,10 +823,9 @@ __global__ void __launch_bounds__(kThreads, kBlocks) attention_rows_kernel(Atten
 
 // A block for all own keys of a tile of a sequence's rows, which also joins the
 // prefix's parts and writes the rows. Blocks: tiles of all sequences x heads.
-// kWarps 0: at most 8 rows, without row offsets.
 template <int kDim, int kWarps>
-__global__ void __launch_bounds__(kThreads, kWarps == 0 ? 4 : kBlocks) attention_last_kernel(Attention a, int late_wait) {
-  constexpr int kRows = kWarps == 0 ? 8 : 16 * kWarps;
+__global__ void __launch_bounds__(kThreads, kBlocks) attention_last_kernel(Attention a, int late_wait) {
+  constexpr int kRows = 16 * kWarps;
   extern __shared__ __align__(16) unsigned char raw[];
   __shared__ uint32_t odd_keys[kKeys / 32];
   __shared__ Segment seg;
@@ -863,11 +872,21 @@ __global__ void __launch_bounds__(kThreads, kWarps == 0 ? 4 : kBlocks) attention
   __syncthreads();
   if (seg.count == 0) {
     if (late_wait) pdl_wait();
-  } else if constexpr (kWarps == 0) {
-    attend_few<kDim>(a, seg, raw, odd_keys, late_wait != 0);
   } else {
     attend<kDim, kWarps, true>(a, seg, raw, odd_keys, late_wait != 0);
   }
+}
+
+// The same for one row a sequence and at most 8 heads to a key/value head. Blocks: sequences x key/value heads.
+template <int kDim, int kWarps>
+__global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) attention_few_kernel(Attention a, int late_wait) {
+  extern __shared__ __align__(16) unsigned char raw[];
+  __shared__ uint32_t free_word;
+  if (!late_wait) pdl_wait();
+  // The next grid waits for this one, which waits for the one before it. Among small calls its early start is worth
+  // 1.5 us; behind many blocks it costs one (sixteen pages 58.5 against 59.4).
+  if (kWarps == 8) pdl_launch_dependents();
+  attend_few<kDim, kWarps>(a, raw, &free_word, late_wait != 0);
 }
 
 // kWarps warps join the parts of a (row, head): first all maxima and sums, a lane a part, then the outputs of the parts
@@ -1038,12 +1057,19 @@ cudaError_t launch_rows(const Attention& a, const Grid& g, unsigned blocks, cuda
 
 template <int kDim, int kWarps>
 cudaError_t launch_last(const Attention& a, unsigned blocks, int late_wait, cudaStream_t stream) {
-  constexpr size_t kRing = kWarps == 0 ? FewRing<kDim>::kBytes : static_cast<size_t>(kStages) * Feed<kDim>::kStage * 2;
-  const size_t join = kWarps == 0 ? LastJoin<kDim, 8, 4>::bytes(a.prefix_slots)
-                                  : LastJoin<kDim, 16 * kWarps, 4 / std::max(kWarps, 1)>::bytes(a.prefix_slots);
+  constexpr size_t kRing = static_cast<size_t>(kStages) * Feed<kDim>::kStage * 2;
+  const size_t join = LastJoin<kDim, 16 * kWarps, 4 / kWarps>::bytes(a.prefix_slots);
   const cudaError_t st = allow_max_dynamic_smem_once<attention_last_kernel<kDim, kWarps>>();
   if (st != cudaSuccess) return st;
   return launch_pdl(attention_last_kernel<kDim, kWarps>, blocks, kThreads, std::max(kRing, join), stream, a, late_wait);
+}
+template <int kDim, int kWarps>
+cudaError_t launch_few(const Attention& a, unsigned blocks, int late_wait, cudaStream_t stream) {
+  const size_t join = LastJoin<kDim, 8, kWarps, 32 * kWarps>::bytes(a.prefix_slots);
+  const cudaError_t st = allow_max_dynamic_smem_once<attention_few_kernel<kDim, kWarps>>();
+  if (st != cudaSuccess) return st;
+  return launch_pdl(attention_few_kernel<kDim, kWarps>, blocks, 32 * kWarps, std::max(FewRing<kDim, kWarps>::kBytes, join),
+                    stream, a, late_wait);
 }
 
 template <int kDim>
@@ -1068,8 +1094,8 @@ cudaError_t launch(const uocr_prefix_attention_args& args, const Attention& a, c
   if (p.whole_own) {
     const int late = p.tc || p.blocks > 0;
     const unsigned n = static_cast<unsigned>(p.own_tiles * a.kv_heads);
-    // One row a sequence and at most 8 heads to a key: the 8-row form (it counts as many tiles).
-    if (a.row_offsets == nullptr && a.group <= 8) return launch_last<kDim, 0>(a, n, late, stream);
+    if (a.row_offsets == nullptr && a.group <= 8)  // as many tiles: one a sequence
+      return n <= kSms ? launch_few<kDim, 8>(a, n, late, stream) : launch_few<kDim, 4>(a, n, late, stream);
     return p.own_warps == 1   ? launch_last<kDim, 1>(a, n, late, stream)
            : p.own_warps == 2 ? launch_last<kDim, 2>(a, n, late, stream)
                               : launch_last<kDim, 4>(a, n, late, stream);
