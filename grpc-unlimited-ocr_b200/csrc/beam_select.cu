@@ -66,16 +66,29 @@ __device__ __forceinline__ Key sort_lanes(Key key) {
 }
 
 // A lower bound on the select-th best of the block's elements, from each
-// thread's best: the best of the warps' select-th ones. All threads call it.
+// thread's best: for j = 1, 2, 4 and 8 groups of warps, every group has a warp with
+// ceil(select / j) elements that reach the group's best such warp's last one, and so
+// j ceil(select / j) >= select elements reach the least of the groups'. (The 16th
+// of 4096 is reached by 16, this by some 35, the best of the warps' 16th, j = 1, by
+// 116.) All threads call it; `shared`: 4 * kWarps keys.
 template <typename Key>
 __device__ __forceinline__ Key bound_of(Key best, int select, uint64_t* shared) {
+  static_assert(kWarps == 8, "four kinds of groups, a lane each of their warps");
   const Key sorted = sort_lanes(best);
-  if (static_cast<int>(threadIdx.x & 31) == select - 1) shared[threadIdx.x >> 5] = sorted;
-  __syncthreads();
-  Key bound = 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kind = lane / kWarps;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) bound = max(bound, static_cast<Key>(shared[w]));
-  return bound;
+  for (int k = 0; k < 4; ++k)
+    if (lane == ((select - 1) >> k)) shared[k * kWarps + warp] = sorted;  // ceil(select / 2^k) - 1
+  __syncthreads();
+  Key bound = static_cast<Key>(shared[lane]);
+#pragma unroll
+  for (int step = 0; step < 3; ++step) {
+    const Key other = __shfl_xor_sync(0xffffffffu, bound, 1 << step);
+    bound = step < 3 - kind ? max(bound, other) : min(bound, other);
+  }
+  bound = max(bound, __shfl_xor_sync(0xffffffffu, bound, 8));
+  bound = max(bound, __shfl_xor_sync(0xffffffffu, bound, 16));
+  return max(bound, static_cast<Key>(1));
 }
 
 // A maximum in the log2 domain, rounded here and everywhere to the same float: fused into a difference it would not be.
@@ -142,7 +155,7 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads, 3) beam_parts_kernel(Select a) {
   constexpr int kVec = 16 / sizeof(T);
   extern __shared__ uint64_t list[];  // [kList]
-  __shared__ uint64_t bounds[kWarps];
+  __shared__ uint64_t bounds[4 * kWarps];
   __shared__ float2 warp_sums[kWarps];
   __shared__ uint64_t best[UOCR_BEAM_MAX];
   __shared__ int count, next;
@@ -236,7 +249,7 @@ __global__ void __launch_bounds__(kThreads, 3) beam_parts_kernel(Select a) {
       bound = static_cast<uint64_t>(value) << 32;
       at_least = unordered(value);
     }
-    bool many = false;
+    bool many = base == begin && base + kRound < end;
     if (peak >= at_least) {
       unsigned reach = 0;
 #pragma unroll
@@ -257,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, 3) beam_parts_kernel(Select a) {
         many |= at >= list_limit(a.select);
       }
     }
-    // The bound is drawn anew when the list grows, at once after the first round: from then on few elements pass.
+    // The bound is drawn anew after the first round, from when on few elements pass, and when the list grows.
     if (__syncthreads_or(many)) {
       bound = max(bound, cut(list, &count, &next, a.select, bounds, best));
       at_least = unordered(max(static_cast<uint32_t>(bound >> 32), ordered(-INFINITY)));
