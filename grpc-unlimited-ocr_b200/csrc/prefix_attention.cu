@@ -446,10 +446,13 @@ __device__ __forceinline__ void attend(const Attention& a, const Segment& seg, u
       if (threadIdx.x < kKeys / 32) odd_keys[threadIdx.x] = 0;
       __syncthreads();
       bool odd = false;
-      for (int c = threadIdx.x; c < kKeys * (kDim / 2); c += kThreads) {
-        const int r = c / (kDim / 2);
-        const uint32_t u = *reinterpret_cast<const uint32_t*>(whole + r * kPitch + c % (kDim / 2) * 2);
-        if ((u & 0x7f80u) == 0x7f80u || (u & 0x7f800000u) == 0x7f800000u) {
+#pragma unroll 4
+      for (int c = threadIdx.x; c < kKeys * (kDim / 8); c += kThreads) {
+        const int r = c / (kDim / 8);
+        const uint4 u = *reinterpret_cast<const uint4*>(whole + r * kPitch + c % (kDim / 8) * 8);
+        // An exponent of ones, plus one in its last place, carries into the sign's.
+        auto ones = [](uint32_t x) { return (x & 0x7f807f80u) + 0x00800080u; };
+        if (((ones(u.x) | ones(u.y) | ones(u.z) | ones(u.w)) & 0x80008000u) != 0) {
           atomicOr(&odd_keys[r / 32], 1u << (r & 31));
           odd = true;
         }
