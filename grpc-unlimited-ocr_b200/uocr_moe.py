@@ -674,13 +674,40 @@ def grouped_linear_w8a8(x, x_scales, w, w_scales, offsets, y, row_index=None, w_
     _check(lib().uocr_grouped_linear_w8a8(_pack_grouped(*args, space, space_bytes), _stream(stream)))
 
 
-def _on_current_device(*tensors) -> None:
-    """The kernels run on the current device: every tensor has to be there."""
-    import torch
-    current = torch.cuda.current_device()
+_torch = None  # once a call has needed it: an import statement in every call costs 0.2 us
+
+
+def _torch_types():
+    """(torch, float32, int32, bfloat16)"""
+    global _torch
+    if _torch is None:
+        import torch
+        torch.cuda.current_device()
+        _torch = torch, torch.float32, torch.int32, torch.bfloat16, getattr(torch._C, "_cuda_getDevice",
+                                                                          torch.cuda.current_device)
+    return _torch[:4]
+
+
+def _on_current_device(*tensors) -> int:
+    """The kernels run on the current device, which is returned: every tensor has to be there."""
+    _torch_types()
+    current = _torch[4]()
     for t in tensors:
         if t is not None and t.get_device() != current:
             raise ValueError(f"a tensor on {t.device} in a call on cuda:{current}")
+    return current
+
+
+def _stream_on(stream, device: int):
+    """`stream`, or the current one of the current device."""
+    return _stream(stream) if stream is not None or _raw_stream is None else _raw_stream(device)
+
+
+def _values(t, what: str, n: int, dtype) -> int:
+    """_vector's pointer, of a tensor whose device has been looked at."""
+    if t.dtype is not dtype or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{what} must be {n} contiguous {dtype} values on the GPU")
+    return t.data_ptr()
 
 
 def _heads(t, what: str, rows: int, dim: int):
@@ -725,8 +752,7 @@ def rotate_heads(q, k, v, inv_freq, positions, q_out, k_cache, v_cache, q_norm=N
     likewise (v as it is) into the bf16 caches [caches, kv_heads, capacity, dim] at cache_rows[r] (else r), slots[r]
     (else positions[r]) (uocr_rotate_heads). q, k, v: fp32 or bf16; inv_freq: fp32, rotary_dim / 2 of them; positions,
     cache_rows, slots: int32."""
-    import torch
-    f32, i32, bf16 = torch.float32, torch.int32, torch.bfloat16
+    _, f32, i32, bf16 = _torch_types()
     rows, heads, dim = shape = q.shape
     kv_heads, rotary = k.shape[1], 2 * inv_freq.numel()
     (ldq, *lq), (ldk, *lk), (ldv, *lv), (ldqo, *lo) = q.stride(), k.stride(), v.stride(), q_out.stride()
@@ -751,15 +777,15 @@ def rotate_heads(q, k, v, inv_freq, positions, q_out, k_cache, v_cache, q_norm=N
             raise ValueError(f"the caches must be [caches, {kv_heads}, capacity, {dim}]")
     if cache_rows is None and caches != rows:
         raise ValueError("without cache_rows there is one cache per row")
-    _on_current_device(q, k, v, inv_freq, positions, q_out, k_cache, v_cache, q_norm, k_norm, cache_rows, slots)
+    device = _on_current_device(q, k, v, inv_freq, positions, q_out, k_cache, v_cache, q_norm, k_norm, cache_rows, slots)
     _check(lib().uocr_rotate_heads(_pack_rotate(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), 0 if q_norm is None else _vector(q_norm, "q_norm", dim, f32),
-        0 if k_norm is None else _vector(k_norm, "k_norm", dim, f32), _vector(inv_freq, "inv_freq", rotary // 2, f32),
-        _vector(positions, "positions", rows, i32),
-        0 if cache_rows is None else _vector(cache_rows, "cache_rows", rows, i32),
-        0 if slots is None else _vector(slots, "slots", rows, i32), q_out.data_ptr(), k_cache.data_ptr(),
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), 0 if q_norm is None else _values(q_norm, "q_norm", dim, f32),
+        0 if k_norm is None else _values(k_norm, "k_norm", dim, f32), _values(inv_freq, "inv_freq", rotary // 2, f32),
+        _values(positions, "positions", rows, i32),
+        0 if cache_rows is None else _values(cache_rows, "cache_rows", rows, i32),
+        0 if slots is None else _values(slots, "slots", rows, i32), q_out.data_ptr(), k_cache.data_ptr(),
         v_cache.data_ptr(), rows, heads, kv_heads, dim, rotary, ldq, ldk, ldv, ldqo, caches, capacity, of_cache, of_head,
-        eps, magnitude, _float_dtype(q, "q"), interleaved), _stream(stream)))
+        eps, magnitude, _float_dtype(q, "q"), interleaved), _stream_on(stream, device)))
 
 
 def prefix_attention(q, prefix_k, prefix_v, prefix_lens, k, v, lens, out, ancestry=None, row_offsets=None,
@@ -770,8 +796,7 @@ def prefix_attention(q, prefix_k, prefix_v, prefix_lens, k, v, lens, out, ancest
     (uocr_prefix_attention). q, out and the caches are bf16, lens, ancestry and row_offsets (sequences + 1 values; None:
     one row each) int32, lse (optional) fp32 [rows, heads]; scale defaults to dim ** -0.5. The workspace comes from
     torch's allocator, from the blocks of the stream that the call runs on."""
-    import torch
-    f32, i32, bf16 = torch.float32, torch.int32, torch.bfloat16
+    _, f32, i32, bf16 = _torch_types()
     rows, heads, dim = shape = q.shape
     prefixes, kv_heads, prefix_capacity, _ = prefix_shape = prefix_k.shape
     caches, _, capacity, _ = own_shape = k.shape
@@ -791,27 +816,28 @@ def prefix_attention(q, prefix_k, prefix_v, prefix_lens, k, v, lens, out, ancest
         own_strides = _cache_strides(k, v, "the own caches")
         if own_shape[1] != kv_heads or own_shape[3] != dim or prefix_shape[3] != dim:
             raise ValueError(f"the caches must be [caches, {kv_heads}, capacity, {dim}]")
-    _on_current_device(q, prefix_k, prefix_v, prefix_lens, k, v, lens, out, ancestry, row_offsets, lse)
+    device = _on_current_device(q, prefix_k, prefix_v, prefix_lens, k, v, lens, out, ancestry, row_offsets, lse)
     sequences, ld_ancestry, table, offsets = lens.numel(), 0, 0, 0
     if ancestry is not None:
         if ancestry.dtype is not i32:
             raise ValueError("ancestry must be int32")
         ld_ancestry, table = _pitch(ancestry, "ancestry", sequences, capacity), ancestry.data_ptr()
     if row_offsets is not None:
-        offsets = _vector(row_offsets, "row_offsets", sequences + 1, i32)
+        offsets = _values(row_offsets, "row_offsets", sequences + 1, i32)
     args = _pack_attention(
-        q.data_ptr(), prefix_k.data_ptr(), prefix_v.data_ptr(), _vector(prefix_lens, "prefix_lens", prefixes, i32),
-        k.data_ptr(), v.data_ptr(), _vector(lens, "lens", sequences, i32), table, offsets, out.data_ptr(),
-        0 if lse is None else _vector(lse, "lse", rows * heads, f32), rows, sequences, prefixes, caches, heads,
+        q.data_ptr(), prefix_k.data_ptr(), prefix_v.data_ptr(), _values(prefix_lens, "prefix_lens", prefixes, i32),
+        k.data_ptr(), v.data_ptr(), _values(lens, "lens", sequences, i32), table, offsets, out.data_ptr(),
+        0 if lse is None else _values(lse, "lse", rows * heads, f32), rows, sequences, prefixes, caches, heads,
         kv_heads, dim, prefix_capacity, capacity, ldq, ldo, ld_ancestry, prefix_strides[0], prefix_strides[1],
         own_strides[0], own_strides[1], dim ** -0.5 if scale is None else scale, 0, 0, 0)
     size = ctypes.c_int64()
     _check(lib().uocr_prefix_attention_workspace(args, ctypes.byref(size)))
     need = size.value
     if need > 0:
-        workspace = _workspace(need, q.device, stream)  # held until the launch is made
+        # Held until the launch is made.
+        workspace = q.new_empty((need + 1) // 2) if stream is None else _workspace(need, q.device, stream)
         args = args[:-_PACKED_SPACE] + _pack_space(workspace.data_ptr(), need)
-    _check(lib().uocr_prefix_attention(args, _stream(stream)))
+    _check(lib().uocr_prefix_attention(args, _stream_on(stream, device)))
 
 
 def beam_select(logits, scores, tokens, parents, new_scores, finished=None, new_finished=None, eos: int = -1,
@@ -820,32 +846,32 @@ def beam_select(logits, scores, tokens, parents, new_scores, finished=None, new_
     finished) [batch, beams]; tokens, parents, new_scores (and new_finished) [batch, select] receive them, best first
     (uocr_beam_select). Flags, tokens and parents are int32, scores fp32. The workspace comes from torch's allocator, from
     the blocks of the stream that the call runs on."""
-    import torch
-    f32, i32 = torch.float32, torch.int32
-    _on_current_device(logits, scores, tokens, parents, new_scores, finished, new_finished)
+    _, f32, i32, _ = _torch_types()
+    device = _on_current_device(logits, scores, tokens, parents, new_scores, finished, new_finished)
     batch, beams = scores.shape
     select, vocab = tokens.shape[1], logits.shape[1]
     rows, out = batch * beams, batch * select
     args = _pack_select(
-        logits.data_ptr(), _vector(scores, "scores", rows, f32),
-        0 if finished is None else _vector(finished, "finished", rows, i32), _vector(tokens, "tokens", out, i32),
-        _vector(parents, "parents", out, i32), _vector(new_scores, "new_scores", out, f32),
-        0 if new_finished is None else _vector(new_finished, "new_finished", out, i32), batch, beams, select, vocab,
+        logits.data_ptr(), _values(scores, "scores", rows, f32),
+        0 if finished is None else _values(finished, "finished", rows, i32), _values(tokens, "tokens", out, i32),
+        _values(parents, "parents", out, i32), _values(new_scores, "new_scores", out, f32),
+        0 if new_finished is None else _values(new_finished, "new_finished", out, i32), batch, beams, select, vocab,
         _pitch(logits, "logits", rows, vocab), _float_dtype(logits, "logits"), eos, 0, 0)
     size = ctypes.c_int64()
     _check(lib().uocr_beam_select_workspace(args, ctypes.byref(size)))
     need = size.value
-    workspace = _workspace(need or 16, logits.device, stream)  # held until the launch is made
-    _check(lib().uocr_beam_select(args[:-_PACKED_SPACE] + _pack_space(workspace.data_ptr(), need), _stream(stream)))
+    # Held until the launch is made.
+    workspace = scores.new_empty(need // 4 + 4) if stream is None else _workspace(need + 16, scores.device, stream)
+    args = args[:-_PACKED_SPACE] + _pack_space(workspace.data_ptr(), need)
+    _check(lib().uocr_beam_select(args, _stream_on(stream, device)))
 
 
 def reorder_states(state, parents, beams: int, counts=None, stream=None):
     """state[:, g * beams + b] = state[:, g * beams + parents[g, b]] in place (uocr_reorder_states). state is [layers,
     rows, segments, units, ...] with contiguous segments, or [rows, units]; parents: rows int32 values, local to each
     group of `beams` rows; counts (int32): units in use of each row, the rest of a row stays."""
-    import torch
-    i32 = torch.int32
-    _on_current_device(state, parents, counts)
+    i32 = _torch_types()[2]
+    device = _on_current_device(state, parents, counts)
     if state.dim() == 2:
         state = state[None, :, None]
     if state.dim() < 4:
@@ -863,9 +889,9 @@ def reorder_states(state, parents, beams: int, counts=None, stream=None):
         raise ValueError("the state's rows must be whole groups of beams")
     eb = state.element_size()
     _check(lib().uocr_reorder_states(_pack_reorder(
-        state.data_ptr(), _vector(parents, "parents", rows, i32),
-        0 if counts is None else _vector(counts, "counts", rows, i32), layers, rows // beams, beams, segments, units,
-        width * eb, of_layer * eb, of_row * eb, of_segment * eb), _stream(stream)))
+        state.data_ptr(), _values(parents, "parents", rows, i32),
+        0 if counts is None else _values(counts, "counts", rows, i32), layers, rows // beams, beams, segments, units,
+        width * eb, of_layer * eb, of_row * eb, of_segment * eb), _stream_on(stream, device)))
 
 
 class Decoder:
