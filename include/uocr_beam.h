@@ -196,8 +196,9 @@ int uocr_decoder_beam_workspace(const uocr_decoder* dec, int64_t beams, int64_t 
  * the decode steps after it): the first tokens come from the logits that the
  * sequence ended with, each later step runs all beams as one batch over the
  * sequence's cache, shared, and their own. The sequence itself stays as it is: a
- * decode or another search may follow. The sequence and the steps have to fit
- * max_positions. Decoders with int8 weights expand them to bf16 in every step, as
+ * decode or another search may follow. A captured search may be replayed as long
+ * as the sequence is the one it was captured with. The sequence and the steps have
+ * to fit max_positions. Decoders with int8 weights expand them to bf16 in every step, as
  * their prefill does; with UOCR_DECODER_INT8_ACTIVATIONS the projections and the
  * head run on int8 activations. */
 int uocr_decoder_beam_search(uocr_decoder* dec, const uocr_beam_search_args* args, void* stream);

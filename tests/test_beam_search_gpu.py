@@ -169,3 +169,25 @@ def test_beam_search_refusals(cuda):
     with pytest.raises(ValueError):
         dec.beam_search(2, 2, torch.empty(2, 2, dtype=torch.int64, device=cuda), torch.empty(2, device=cuda))
     dec.close()
+
+
+@pytest.mark.parametrize("beams", [3, 8])
+def test_a_captured_search_repeats_itself(cuda, beams):
+    """Its replays continue the sequence that it was captured with, whatever else was searched between them."""
+    import torch
+    dims, dec, _ = _build(torch, cuda, SHAPES[0], M.WEIGHT_BF16)
+    dec.prefill(torch.from_numpy(D.synth_prompt(dims, 5, 12)).to(cuda))
+    want = _search(torch, dec, beams, 5)
+    tokens = torch.zeros(beams, 5, dtype=torch.int32, device="cuda")
+    scores = torch.zeros(beams, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        dec.beam_search(beams, 5, tokens, scores)
+    for _ in range(2):
+        tokens.zero_()
+        graph.replay()
+        dec.check()
+        assert np.array_equal(tokens.cpu().numpy(), want[0]) and np.array_equal(scores.cpu().numpy(), want[1])
+        _search(torch, dec, 2, 3)
+    del graph
+    dec.close()
