@@ -38,9 +38,9 @@ constexpr int kRanked = 512;  // as many keys are ranked against one another; mo
 constexpr int kList = kRound + 2 * UOCR_BEAM_MAX + 64;  // what a round may leave (list_limit), and one round
 __device__ __forceinline__ int list_limit(int select) { return 2 * select + 64; }
 
-// Floats in their order as unsigned integers; 0 stands for no candidate.
+// Floats in their order as unsigned integers, -0 as 0; 0 stands for no candidate.
 __device__ __forceinline__ uint32_t ordered(float f) {
-  const uint32_t u = __float_as_uint(f);
+  const uint32_t u = __float_as_uint(f + 0.0f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float unordered(uint32_t o) {
@@ -318,7 +318,7 @@ struct Cand {
   uint64_t flat;  // beam << 32 | token
 };
 __device__ __forceinline__ uint64_t ordered64(double v) {
-  const uint64_t u = static_cast<uint64_t>(__double_as_longlong(v));
+  const uint64_t u = static_cast<uint64_t>(__double_as_longlong(v + 0.0));  // -0 as 0
   return u >> 63 ? ~u : u | 0x8000000000000000ull;
 }
 __device__ __forceinline__ float score_of(const Cand& c) {

@@ -204,6 +204,19 @@ def test_beam_select_ties_go_to_the_lower_beam_and_token(cuda):
     assert tokens[0].tolist() == [8000, 8001, 8002] * 2 + [8000] and parents[0].tolist() == [0] * 3 + [1] * 3 + [2]
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_beam_select_takes_both_zeros_for_equal(cuda, dtype):
+    import torch
+    logits = torch.full((2, 9000), -5.0, device="cuda", dtype=getattr(torch, dtype))
+    logits[:, 100:130], logits[:, 110:8000:7] = -0.0, 0.0
+    tokens, parents, _ = check_select(logits, torch.zeros(1, 2, device="cuda"), 20)
+    assert tokens[0].tolist() == list(range(100, 120)) and (parents == 0).all()
+    scores = torch.tensor([[-0.0, 0.0, -0.0]], device="cuda")
+    finished = torch.ones(1, 3, dtype=torch.int32, device="cuda")
+    _, parents, _ = check_select(torch.zeros(3, 50, device="cuda"), scores, 3, finished, 7)
+    assert parents[0].tolist() == [0, 1, 2]
+
+
 @pytest.mark.parametrize("order", ["rising", "falling", "steps"])
 @pytest.mark.parametrize("select", [1, 32])
 def test_beam_select_of_sorted_logits(cuda, order, select):
