@@ -310,13 +310,16 @@ struct Join {
   int depth;  // 1 .. select
 };
 
-// A candidate in the order of the selection: the score, then the lower beam and
-// token. The 64-bit score as an integer in the same order, which compares in two
-// instructions where doubles took ten times as long; 0: no candidate.
+// A candidate in the order of the selection: the score, then the lower beam, within
+// a beam the higher logit (scores far from 0 can no longer tell those apart), then
+// the lower token. The 64-bit score as an integer in the same order, which compares
+// in two instructions where doubles took ten times as long; 0: no candidate.
 struct Cand {
   uint64_t score;
-  uint64_t flat;  // beam << 32 | token
+  uint64_t flat;  // beam << 52 | inverted ordered logit << 20 | token
 };
+constexpr int kTokenBits = 20, kBeamAt = 52;
+static_assert(UOCR_BEAM_MAX <= 1 << (64 - kBeamAt), "");
 __device__ __forceinline__ uint64_t ordered64(double v) {
   const uint64_t u = static_cast<uint64_t>(__double_as_longlong(v + 0.0));  // -0 as 0
   return u >> 63 ? ~u : u | 0x8000000000000000ull;
@@ -407,7 +410,7 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(Join a) {
     if (ended[b]) {
       if (i == b * s.parts && at == 0 && score > -INFINITY) {
         e.score = ordered64(score);
-        e.flat = static_cast<uint64_t>(b) << 32 | static_cast<uint32_t>(max(a.eos, 0));
+        e.flat = static_cast<uint64_t>(b) << kBeamAt | static_cast<uint32_t>(max(a.eos, 0));
       }
     } else if (lse[b] < INFINITY) {
       const uint64_t key = kStaged ? staged[i * s.select + at] : keys[static_cast<int64_t>(i) * s.select + at];
@@ -415,7 +418,8 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(Join a) {
           static_cast<double>(score) + (static_cast<double>(unordered(static_cast<uint32_t>(key >> 32))) - lse[b]);
       if (key != 0 && v > -INFINITY) {
         e.score = ordered64(v);
-        e.flat = static_cast<uint64_t>(b) << 32 | (0xffffffffu - static_cast<uint32_t>(key));
+        e.flat = static_cast<uint64_t>(b) << kBeamAt | static_cast<uint64_t>(~static_cast<uint32_t>(key >> 32)) << kTokenBits |
+                 (0xffffffffu - static_cast<uint32_t>(key));
       }
     }
     return e;
@@ -454,7 +458,7 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(Join a) {
     const Cand mine = i < m ? left[i] : Cand{0, ~0ull};
     const int rank = rank_of(mine, left, m);
     if (mine.score == 0 || threadIdx.x % kLanes != 0 || rank >= s.select) continue;
-    const int b = static_cast<int>(mine.flat >> 32), token = static_cast<int>(mine.flat & 0xffffffffu);
+    const int b = static_cast<int>(mine.flat >> kBeamAt), token = static_cast<int>(mine.flat & ((1u << kTokenBits) - 1));
     put(rank, token, b, score_of(mine), ended[b] || token == a.eos);
   }
   for (int i = m + threadIdx.x; i < s.select; i += kJoinThreads) put(i, max(a.eos, 0), 0, -INFINITY, true);

@@ -150,7 +150,8 @@ int uocr_beam_select_workspace(const uocr_beam_select_args* args, int64_t* bytes
 
 /* Of each batch entry's candidates (b, t) with the score scores[b] +
  * log_softmax(logits[b])[t] the `select` best, best first, equal ones by the
- * lower beam, then the lower token. A finished beam has one candidate: its eos
+ * lower beam, within a beam by the higher logit (a score far from 0 cannot tell
+ * close ones apart), then the lower token. A finished beam has one candidate: its eos
  * again (token 0 with eos -1), its score unchanged. A candidate whose score is
  * NaN or -inf is none (a NaN logit, as -inf; a row that holds +inf has none).
  * Where candidates run out: token max(eos, 0), parent 0, score -inf, finished.

@@ -217,6 +217,25 @@ def test_beam_select_takes_both_zeros_for_equal(cuda, dtype):
     assert parents[0].tolist() == [0, 1, 2]
 
 
+@pytest.mark.parametrize("score", [-1e9, -1e30])
+def test_beam_select_of_scores_that_hide_the_logits(cuda, score):
+    """Within a beam the logits' order stays; equal scores of two beams go to the lower one."""
+    import torch
+    logits = torch.randn(3, 30000, generator=gen_of(9), device="cuda")
+    logits[2] = logits[1]
+    scores = torch.tensor([[score * 2, score, score]], device="cuda")
+    tokens, parents, new = (torch.empty(1, 32, dtype=d, device="cuda") for d in (torch.int32, torch.int32, torch.float32))
+    M.beam_select(logits, scores, tokens, parents, new)
+    assert (new == score).all()
+    if score == -1e30:  # all of a beam's scores are one 64-bit value
+        want = logits[1].sort(descending=True, stable=True)[1][:32]
+        assert (parents == 1).all() and torch.equal(tokens[0].long(), want)
+    else:
+        want = logits[1].sort(descending=True, stable=True)[1][:16]
+        assert torch.equal(parents[0].long(), torch.tensor([1, 2] * 16, device="cuda"))
+        assert torch.equal(tokens[0].long(), want.repeat_interleave(2))
+
+
 @pytest.mark.parametrize("order", ["rising", "falling", "steps"])
 @pytest.mark.parametrize("select", [1, 32])
 def test_beam_select_of_sorted_logits(cuda, order, select):
