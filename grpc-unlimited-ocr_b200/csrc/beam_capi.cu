@@ -183,8 +183,8 @@ int uocr_prefix_attention(const uocr_prefix_attention_args* a, void* stream) {
       return bad(op, "without ancestry there is one cache per sequence");
     if (a->ancestry != nullptr && a->ld_ancestry < a->capacity) return bad(op, "a pitch is smaller than its row");
   }
-  if (a->workspace == nullptr || !aligned(a->workspace, 16) ||
-      a->workspace_bytes < static_cast<int64_t>(prefix_attention_bytes(*a)))
+  const int64_t need = static_cast<int64_t>(prefix_attention_bytes(*a));  // 0 without prefixes' keys
+  if (need > 0 && (a->workspace == nullptr || !aligned(a->workspace, 16) || a->workspace_bytes < need))
     return bad(op, "the workspace is missing, too small or not 16-byte aligned (uocr_prefix_attention_workspace)");
   ErrorWord* err = nullptr;
   const cudaError_t st = ops_error_word(&err);

@@ -156,6 +156,14 @@ def test_many_sequences_on_one_prefix(cuda, sequences):
     check(make([5000], [1 + i % 40 for i in range(sequences)], 16, 4, 128))
 
 
+@pytest.mark.parametrize("heads,kv,rows", [(8, 2, None), (24, 2, None), (8, 2, [3, 20, 1])])
+def test_without_room_for_keys(cuda, heads, kv, rows):
+    """Capacities of zero: of the prefixes, of the own keys, of both."""
+    check(make([0], [5, 70, 9], heads, kv, 128, rows=rows, prefix_capacity=0))
+    check(make([40], [0, 0, 0], heads, kv, 128, rows=rows, capacity=0))
+    check(make([0], [0, 0, 0], heads, kv, 128, rows=rows, prefix_capacity=0, capacity=0))
+
+
 def test_a_long_prefix(cuda):
     check(make([33001], [3, 9], 8, 2, 128))
 
