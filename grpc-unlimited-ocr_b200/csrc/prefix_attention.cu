@@ -580,7 +580,8 @@ __device__ __forceinline__ void attend(const Attention& a, const Segment& seg, u
 // keys or values (K V K, then V K V): no barrier before the join, and with 52 KB a
 // block of four warps four blocks an SM, so that 512 ranges of own keys are under
 // way at once (with three some had to wait for the end of others: sixteen pages 59
-// against 57 us). Blocks that have an SM to themselves take eight warps and half the
+// against 57 us). A lane reads one key's ancestor, and the copies are a loop: the
+// first instructions of a kernel come from memory like its data. Blocks that have an SM to themselves take eight warps and half the
 // rounds: four beams 13.5 against 11.7 us.
 template <int kDim, int kWarps>
 struct FewRing {
@@ -602,14 +603,10 @@ __device__ __forceinline__ void attend_few(const Attention& a, unsigned char* ra
   w.count = a.group;
   const int64_t base = (gathers ? 0 : w.of * a.cache_stride) + w.kv_head * a.head_stride;
   __nv_bfloat16* const ring = reinterpret_cast<__nv_bfloat16*>(raw) + warp * Ring::kSlots * Ring::kSlot;
-  int from[kCopies];  // the caches of the next round's keys, read ahead of the copies
+  int from = 0;  // the cache of this lane's key of the next round, read ahead of the copies
   auto look_up = [&](int key, int end) {
-    if (!gathers) return;
-#pragma unroll
-    for (int i = 0; i < kCopies; ++i) {
-      const int at = key + copy_key + i * kStep;
-      from[i] = at < end ? a.ancestry[w.of * a.ld_ancestry + at] : 0;
-    }
+    const int at = key + warp * 16 + lane;
+    if (gathers) from = lane < 16 && at < end ? a.ancestry[w.of * a.ld_ancestry + at] : 0;
   };
   look_up(0, a.capacity);  // beside the length, not behind it: what is no key's is not used
   if (a.capacity > 0) {
@@ -617,26 +614,29 @@ __device__ __forceinline__ void attend_few(const Attention& a, unsigned char* ra
     if ((n < 0 || n > a.capacity) && threadIdx.x == 0) raise_error(a.err, kDevBadIndex, kSiteLength, w.of, n);
     w.key1 = min(max(n, 0), a.capacity);
   }
-  auto copy = [&](const __nv_bfloat16* of, int slot, int key, bool check) {
+  auto check = [&](int key) {
+    if (!gathers || (from >= 0 && from < a.caches)) return;
+    if (key + warp * 16 + lane < w.key1) raise_error(a.err, kDevBadIndex, kSiteAncestor, w.of, from);
+    from = w.of < a.caches ? w.of : 0;
+  };
+  auto copy = [&](const __nv_bfloat16* of, int slot, int key) {  // by the whole warp
     __nv_bfloat16* to = ring + slot * Ring::kSlot + lane / (kDim / 8) * kPitch + col;
-#pragma unroll
+#pragma unroll 2
     for (int i = 0; i < kCopies; ++i) {
       const int at = key + copy_key + i * kStep;
       const bool valid = at < w.key1;
       int64_t off = valid ? static_cast<int64_t>(at) * kDim + col : 0;
       if (gathers) {
-        if (check && valid && (from[i] < 0 || from[i] >= a.caches)) {
-          raise_error(a.err, kDevBadIndex, kSiteAncestor, w.of, from[i]);
-          from[i] = w.of < a.caches ? w.of : 0;
-        }
-        off += valid ? from[i] * a.cache_stride : 0;
+        const int64_t cache = __shfl_sync(0xffffffffu, from, lane / (kDim / 8) + i * kStep);
+        off += valid ? cache * a.cache_stride : 0;
       }
       cp_async16_or_zero(to + i * kStep * kPitch, of + base + off, valid);
     }
   };
-  if (w.key1 > 0) copy(a.k, 0, 0, true);
+  check(0);
+  if (w.key1 > 0) copy(a.k, 0, 0);
   cp_async_commit();
-  if (w.key1 > 0) copy(a.v, 1, 0, false);
+  if (w.key1 > 0) copy(a.v, 1, 0);
   cp_async_commit();
   look_up(kRound, w.key1);
   uint32_t q[kDim / 16][2];  // row gr
@@ -656,7 +656,8 @@ __device__ __forceinline__ void attend_few(const Attention& a, unsigned char* ra
     const int next = key + kRound, slot1 = (slot + 1) % 3, slot2 = (slot + 2) % 3;
     cp_async_wait<1>();
     __syncwarp();  // the keys have landed, the values before them have been read
-    if (next < w.key1) copy(a.k, slot2, next, true);
+    check(next);
+    if (next < w.key1) copy(a.k, slot2, next);
     cp_async_commit();
     const __nv_bfloat16* ks = ring + slot * Ring::kSlot;
     const __nv_bfloat16* vs = ring + slot1 * Ring::kSlot;
@@ -696,7 +697,7 @@ __device__ __forceinline__ void attend_few(const Attention& a, unsigned char* ra
     const uint32_t p0 = transpose_8x8(pack2(s[0], s[1])), p1 = transpose_8x8(pack2(s[2], s[3]));
     cp_async_wait<1>();
     __syncwarp();  // the values have landed, the keys have been read
-    if (next < w.key1) copy(a.v, slot, next, false);
+    if (next < w.key1) copy(a.v, slot, next);
     cp_async_commit();
     look_up(next + kRound, w.key1);
     slot = slot2;
