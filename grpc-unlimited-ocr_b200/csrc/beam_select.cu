@@ -4,10 +4,12 @@
 // the order is the logits' own, so one pass over a row is enough: a block goes
 // through a part of a row, keeps the maximum, the sum of exponentials and the
 // `select` best logits; a second kernel joins a group's parts. Bound: the one
-// read of the logits; for few rows two launches and their rounds.
+// read of the logits; for few rows two launches and their rounds. 128 rows of 102400
+// logits take 23.1 us (2.3 TB/s: instructions and barriers, 8.0 at the copy rate),
+// four rows 7.9.
 //
-// The best of a part without sorting it: the select-th best of the threads' own
-// maxima, taken warp by warp, bounds the select-th best of all from below. What
+// The best of a part without sorting it: the threads' own maxima, sorted within
+// warps, bound the select-th best of all from below. What
 // reaches the bound goes on a list; where that grows the bound is drawn anew from
 // it, higher, so that soon hardly an element passes; what is left at the end, a
 // few dozen, is ranked. Keys are unique (value, then the lower index), so the
