@@ -35,9 +35,10 @@ namespace uocr_b200 {
 namespace {
 
 constexpr int kTileRows = kAttentionTcRows;
-// What a range costs besides its keys, 7 us, in units: 128 keys take 1.8 us for two tiles of rows, 0.6 (the memory's
-// rate) where the tiles split them.
-__device__ __forceinline__ unsigned range_units(const Attention& a) { return a.split ? 12 : 4; }
+// What a range costs besides its keys, in units: 128 keys take 1.8 us for two tiles of rows, 0.6 (the memory's rate) where
+// the tiles split them. With 4, 6, 8 and 12 for the latter sixteen pages take 53.3, 53.5, 54.2 and 55.1 us, with 2, 3 and
+// 4 for the former prompts on a page 107.9, 107.6 and 107.7, a document 51.2, 51.2 and 52.0.
+__device__ __forceinline__ unsigned range_units(const Attention& a) { return a.split ? 4 : 3; }
 constexpr int kTcKeys = 128;
 constexpr int kSlots = 4;        // shared-memory slots of 128 keys or values
 constexpr int kTcThreads = 384;  // a warpgroup for copies and MMAs, two of rows
