@@ -118,7 +118,8 @@ int uocr_prefix_attention_workspace(const uocr_prefix_attention_args* args, int6
  * once for all its sequences. A row that sees no key is 0, its lse -inf. What
  * lies in a cache behind a length is not read into a result, NaN included.
  * Scores, sums and the products' accumulators are fp32; the weights of the
- * values are rounded to bf16 (the tensor cores' operand). head_dim is 64 or 128.
+ * values are rounded to bf16 (the tensor cores' operand), one below 2^-126 of a
+ * row's greatest so far counts as 0. head_dim is 64 or 128.
  * Rows outside row_offsets[0] .. row_offsets[sequences] are left as they are.
  * A length out of range is recorded and taken as the nearest that is in range;
  * a sequence whose row offsets are not in order is recorded, its rows
