@@ -1,6 +1,6 @@
 // The best continuations of a group of beams (uocr_beam_select).
 //
-// score(b, t) = scores[b] + logit - (m + log sum exp(logit - m)): within a beam
+// score(b, t) = scores[b] + (logit - m) - log sum exp(logit - m): within a beam
 // the order is the logits' own, so one pass over a row is enough: a block goes
 // through a part of a row, keeps the maximum, the sum of exponentials and the
 // `select` best logits; a second kernel joins a group's parts. Bound: the one
@@ -93,8 +93,9 @@ __device__ __forceinline__ Key bound_of(Key best, int select, uint64_t* shared) 
   return max(bound, static_cast<Key>(1));
 }
 
-// A maximum in the log2 domain, rounded here and everywhere to the same float: fused into a difference it would not be.
-__device__ __forceinline__ float log2_of(float m) { return __fmul_rn(m, kLog2e); }
+// e^(f - m) for f <= m, m above -inf. The difference comes first: from 2^24 on the rounding of a product m log2 e is
+// more than 1, and of the lowest floats, which mask tokens, the product is -inf.
+__device__ __forceinline__ float exp_of(float f, float m) { return exp2_fast((f - m) * kLog2e); }
 
 struct Select {
   const void* logits;
@@ -104,7 +105,7 @@ struct Select {
   int vocab, beams, select;
   int parts, part;  // of a row; elements of a part, a multiple of kRound
   bool vec;         // rows allow 16 bytes at a time
-  float2* sums;     // [rows, parts]: maximum m, and sum of 2^(f log2 e - fl(m log2 e))
+  float2* sums;     // [rows, parts]: maximum m, and sum of exp(f - m)
   uint64_t* best;   // [rows, parts, select] keys, descending
 };
 
@@ -227,22 +228,22 @@ __global__ void __launch_bounds__(kThreads, 3) beam_parts_kernel(Select a) {
     }
     if (base + kRound < end) ahead = load(base + kRound);
     if (peak > m) {
-      sum *= exp2_fast(log2_of(m) - log2_of(peak));  // of no element yet: 0 * 0
+      sum *= exp_of(m, peak);  // of no element yet: 0 * 0
       m = peak;
     }
-    // 2^(f log2 e - m log2 e), the second product rounded for all elements alike: the join takes it as it is.
-    const float shift = m > -INFINITY ? log2_of(m) : 0.0f;
+    const float shift = m > -INFINITY ? m : 0.0f;
     float2 of_round = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int i = 0; i < kEach; i += 2) {
-      const float2 x = fma2(make_float2(f[i], f[i + 1]), make_float2(kLog2e, kLog2e), make_float2(-shift, -shift));
+      const float2 x = fma2(add2(make_float2(f[i], f[i + 1]), make_float2(-shift, -shift)),
+                            make_float2(kLog2e, kLog2e), make_float2(0.0f, 0.0f));
       of_round = add2(of_round, make_float2(exp2_fast(x.x), exp2_fast(x.y)));
     }
     float added = of_round.x + of_round.y;
     if (added != added) {  // NaN counts as -inf; beside +inf the sum is not asked for
       added = 0.0f;
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) added += exp2_fast(fmaf(fmaxf(f[i], -INFINITY), kLog2e, -shift));
+      for (int i = 0; i < kEach; ++i) added += exp_of(fmaxf(f[i], -INFINITY), shift);
     }
     sum += added;
     if (bound == 0) {
@@ -282,7 +283,7 @@ __global__ void __launch_bounds__(kThreads, 3) beam_parts_kernel(Select a) {
   float top = m;
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-  sum = warp_sum(m > -INFINITY ? sum * exp2_fast(log2_of(m) - log2_of(top)) : 0.0f);
+  sum = warp_sum(m > -INFINITY ? sum * exp_of(m, top) : 0.0f);
   if ((threadIdx.x & 31) == 0) warp_sums[threadIdx.x >> 5] = make_float2(top, sum);
   __syncthreads();
   const int64_t cell = row * a.parts + part;
@@ -292,8 +293,7 @@ __global__ void __launch_bounds__(kThreads, 3) beam_parts_kernel(Select a) {
       const float2 p = warp_sums[w];
       const float high = fmaxf(all.x, p.x);
       if (high == -INFINITY) continue;
-      all = make_float2(high, all.y * exp2_fast(log2_of(all.x) - log2_of(high)) +
-                                  p.y * exp2_fast(log2_of(p.x) - log2_of(high)));
+      all = make_float2(high, all.y * exp_of(all.x, high) + p.y * exp_of(p.x, high));
     }
     a.sums[cell] = all;
   }
@@ -334,9 +334,6 @@ __device__ __forceinline__ bool better(const Cand& a, const Cand& b) {
   return (a.score > b.score) | ((a.score == b.score) & (a.flat < b.flat));  // no branch
 }
 
-// What a part's exponents are less (its maximum in the log2 domain, as rounded there).
-__device__ __forceinline__ double shift_of(float m) { return static_cast<double>(log2_of(m)); }
-
 constexpr int kJoinThreads = 512;
 constexpr int kLanes = 4;  // neighbouring threads that rank a candidate
 
@@ -358,7 +355,8 @@ __device__ __forceinline__ int rank_of(const Cand& mine, const Cand* of, int n) 
 template <bool kStaged>
 __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(Join a) {
   extern __shared__ Cand heads[];  // [beams * parts * depth], then [select * select], then the keys
-  __shared__ double lse[UOCR_BEAM_MAX];
+  __shared__ double log_sums[UOCR_BEAM_MAX];  // log sum exp(f - top); INFINITY: no candidates
+  __shared__ float tops[UOCR_BEAM_MAX];
   __shared__ float scores[UOCR_BEAM_MAX];
   __shared__ int ended[UOCR_BEAM_MAX];
   __shared__ Cand worst;
@@ -379,9 +377,9 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(Join a) {
   for (int b = warp; b < s.beams; b += kJoinThreads / 32) {
     const float score = s.scores[first + b];
     const bool done = s.finished != nullptr && s.finished[first + b] != 0;
-    double value = INFINITY;  // no candidates
+    double value = INFINITY;
+    float m = -INFINITY;
     if (!done && score > -INFINITY) {
-      float m = -INFINITY;
       double sum = 0.0;
       for (int c0 = 0; c0 < s.parts; c0 += 32) {
         const float2 p = c0 + lane < s.parts ? s.sums[(first + b) * s.parts + c0 + lane] : make_float2(-INFINITY, 0.0f);
@@ -389,16 +387,18 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(Join a) {
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, off));
         if (high == -INFINITY) continue;
-        double all = p.x > -INFINITY ? static_cast<double>(p.y) * exp2(shift_of(p.x) - shift_of(high)) : 0.0;
+        const double top = static_cast<double>(high);
+        double all = p.x > -INFINITY ? static_cast<double>(p.y) * exp(static_cast<double>(p.x) - top) : 0.0;
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) all += __shfl_xor_sync(0xffffffffu, all, off);
-        sum = all + (m > -INFINITY ? sum * exp2(shift_of(m) - shift_of(high)) : 0.0);
+        sum = all + (m > -INFINITY ? sum * exp(static_cast<double>(m) - top) : 0.0);
         m = high;
       }
-      if (m > -INFINITY && m < INFINITY) value = (shift_of(m) + log2(sum)) * 0.69314718055994530942;
+      if (m > -INFINITY && m < INFINITY) value = log(sum);
     }
     if (lane == 0) {
-      lse[b] = value;
+      log_sums[b] = value;
+      tops[b] = m;
       scores[b] = score;
       ended[b] = done;
     }
@@ -414,11 +414,12 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(Join a) {
         e.score = ordered64(score);
         e.flat = static_cast<uint64_t>(b) << kBeamAt | static_cast<uint32_t>(max(a.eos, 0));
       }
-    } else if (lse[b] < INFINITY) {
+    } else if (log_sums[b] < INFINITY) {
       const uint64_t key = kStaged ? staged[i * s.select + at] : keys[static_cast<int64_t>(i) * s.select + at];
-      const double v =
-          static_cast<double>(score) + (static_cast<double>(unordered(static_cast<uint32_t>(key >> 32))) - lse[b]);
-      if (key != 0 && v > -INFINITY) {
+      // The maximum first: far from 0 it and the sum's log have no number in common.
+      const double logit = static_cast<double>(unordered(static_cast<uint32_t>(key >> 32)));
+      const double v = static_cast<double>(score) + ((logit - static_cast<double>(tops[b])) - log_sums[b]);
+      if (key != 0 && static_cast<float>(v) > -INFINITY) {  // as it is handed out
         e.score = ordered64(v);
         e.flat = static_cast<uint64_t>(b) << kBeamAt | static_cast<uint64_t>(~static_cast<uint32_t>(key >> 32)) << kTokenBits |
                  (0xffffffffu - static_cast<uint32_t>(key));

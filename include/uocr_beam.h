@@ -154,7 +154,9 @@ int uocr_beam_select_workspace(const uocr_beam_select_args* args, int64_t* bytes
  * lower beam, within a beam by the higher logit (a score far from 0 cannot tell
  * close ones apart), then the lower token. A finished beam has one candidate: its eos
  * again (token 0 with eos -1), its score unchanged. A candidate whose score is
- * NaN or -inf is none (a NaN logit, as -inf; a row that holds +inf has none).
+ * NaN or -inf, or rounds to -inf, is none (a NaN logit, as -inf; a row that holds
+ * +inf has none). Finite logits of any size, masks of the type's lowest value
+ * among them, are logits like others.
  * Where candidates run out: token max(eos, 0), parent 0, score -inf, finished.
  * new_finished: the parent was finished, or the token is eos. The scores'
  * comparison is made in 64 bits on sums of fp32 exponentials. */

@@ -507,3 +507,95 @@ def test_reorder_states_on_a_stream_and_from_a_graph(cuda):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(state, want)
+
+
+# ---- logits of any magnitude
+
+def check_any_logits(logits, scores, select):
+    """check_select for logits so large that log_softmax may not form the maximum plus the sum's log in one number; a
+    score that float32 holds as -inf is no candidate."""
+    import torch
+    batch, beams = scores.shape
+    vocab = logits.shape[1]
+    tokens = torch.full((batch, select), -7, dtype=torch.int32, device="cuda")
+    parents, flags = torch.full_like(tokens, -7), torch.full_like(tokens, -7)
+    new = torch.full((batch, select), math.nan, device="cuda")
+    M.beam_select(logits, scores, tokens, parents, new, new_finished=flags)
+    z = logits.double().view(batch, beams, vocab)
+    z = z - z.amax(-1, keepdim=True)
+    z = z - z.exp().sum(-1, keepdim=True).log() + scores.double()[..., None]
+    z = torch.where(z.float() == -math.inf, -math.inf, z)
+    # Within a beam the logits' order stays where scores cannot tell them apart: equal logits alone do here.
+    value, at = z.reshape(batch, -1).sort(dim=1, descending=True, stable=True)
+    value, at = value[:, :select], at[:, :select]
+    dead = value == -math.inf
+    assert torch.equal(new == -math.inf, dead) and torch.equal(flags != 0, dead)
+    tol = torch.where(dead, 0.0, 50 * 2.0 ** -24 + 2.0 ** -23 * value.abs())
+    assert ((new.double() - value).abs() <= tol)[~dead].all()
+    tok, par = at % vocab, at // vocab
+    tok[dead], par[dead] = 0, 0
+    same = (tokens == tok) & (parents == par)
+    own = z[torch.arange(batch, device="cuda")[:, None], parents.long(), tokens.long()]
+    assert ((own - value).abs() <= 2 * tol)[~same].all() and not (~same & dead).any()
+    flat = parents.long() * vocab + tokens
+    for b in range(batch):
+        live = flat[b][~dead[b]]
+        assert live.unique().numel() == live.numel()
+
+
+MASKS = [-1e10, -1e20, -1e30, "lowest"]
+
+
+def mask_of(mask, dtype):
+    import torch
+    return torch.finfo(dtype).min if mask == "lowest" else mask
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("mask", MASKS)
+@pytest.mark.parametrize("where", ["threads", "warps", "rounds", "tail", "head", "all but a few", "all but one", "all"])
+@pytest.mark.parametrize("vocab", [20001, 102400])
+def test_beam_select_of_masked_logits(cuda, dtype, mask, where, vocab):
+    """Tokens masked by a large finite value: over whole threads, warps, rounds and parts of a row."""
+    import torch
+    dt = getattr(torch, dtype)
+    logits = (torch.randn(6, vocab, generator=gen_of(vocab, len(where)), device="cuda") * 3).to(dt)
+    at = torch.arange(vocab, device="cuda")
+    side = 16 // logits.element_size()  # elements of a thread side by side
+    thread = at // side % 256
+    masked = {"threads": thread % 3 == 1, "warps": thread // 32 % 2 == 0, "rounds": at // 4096 % 2 == 0,
+              "tail": at >= vocab - 9001, "head": at < vocab - 100, "all but a few": at % (vocab // 90) != 5,
+              "all but one": at != 777, "all": at >= 0}[where]
+    logits[:, masked] = mask_of(mask, dt)
+    logits[4] = (torch.randn(vocab, generator=gen_of(vocab), device="cuda") * 3).to(dt)  # a row without a mask
+    scores = -torch.rand(2, 3, generator=gen_of(5), device="cuda")
+    check_any_logits(logits, scores, 8)
+    check_any_logits(logits, scores, 32)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("level", [3e38, 1e30, 1e10, 2.0 ** 33, -2.0 ** 33, -1e20, -3e38])
+def test_beam_select_of_large_logits(cuda, dtype, level):
+    """Rows about one large value, and rows with one such value above or below ordinary ones."""
+    import torch
+    dt = getattr(torch, dtype)
+    g = gen_of(11)
+    logits = torch.randn(6, 9001, generator=g, device="cuda") * 3
+    logits[:2] = level * (1 + torch.randint(0, 3, (2, 9001), generator=g, device="cuda") * 2.0 ** -6)
+    logits[2:4, 4321] = level
+    logits[4, 100:8000] = level
+    logits[5, ::2], logits[5, 1::2] = level, torch.finfo(dt).min
+    check_any_logits(logits.to(dt), -torch.rand(2, 3, generator=g, device="cuda"), 8)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_beam_select_takes_a_score_that_rounds_to_minus_infinity_for_none(cuda, dtype):
+    import torch
+    dt = getattr(torch, dtype)
+    logits = torch.full((1, 5000), torch.finfo(dt).min, device="cuda", dtype=dt)
+    logits[0, 70] = 3e38
+    check_any_logits(logits, torch.zeros(1, 1, device="cuda"), 3)
+    tokens, parents, flags = (torch.empty(1, 3, dtype=torch.int32, device="cuda") for _ in range(3))
+    new = torch.empty(1, 3, device="cuda")
+    M.beam_select(logits, torch.zeros(1, 1, device="cuda"), tokens, parents, new, new_finished=flags, eos=9)
+    assert tokens[0].tolist() == [70, 9, 9] and new[0].tolist() == [0.0, -math.inf, -math.inf] and flags[0].tolist() == [0, 1, 1]
