@@ -9,6 +9,7 @@
 // So prefixes and own keys are cut into as many shares as the card holds blocks,
 // and a second kernel joins a row's parts.
 #include <algorithm>
+#include <cfloat>
 #include <type_traits>
 
 #include "prefix_attention.cuh"
@@ -997,7 +998,7 @@ constexpr int kSms = 148;  // blocks of the tensor-core kernel, one an SM; corre
 // 47.8 against 50.3, 55.0 against 56.6).
 bool many_rows(const uocr_prefix_attention_args& a) {
   const int64_t group = a.heads / a.kv_heads;
-  if (a.prefix_capacity == 0 || !(a.scale > 0.0f)) return false;
+  if (a.prefix_capacity == 0 || !(a.scale >= FLT_MIN)) return false;  // it divides by the scale
   // what a tensor map takes
   auto far = [](int64_t stride) { return stride <= 0 || stride >= (int64_t{1} << 39); };
   if ((a.kv_heads > 1 && far(a.prefix_head_stride)) || (a.prefixes > 1 && far(a.prefix_stride))) return false;

@@ -497,6 +497,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
         // last. (An empty prefix is told apart below.)
         const int doubled = a.split ? 1 : 0;
         const int shared_from = s.len % kTcKeys != 0 ? s.tiles - 2 - s.tile0 - (a.split ? t : 0) : 1 << 30;
+        // The exponents are fma(x, scale, -m scale). What the rounding of m scale is off by, all weights of a row have in
+        // common: up to 2^-14 where it is at most 1024, but from 2^31 on more than their range. A row whose m is farther
+        // off takes it from its scores (`base`), and the tile is read anew.
+        float base = 0.0f;
+        bool based = false;  // one of the warp's rows
+        auto is_far = [&](float m) { return fabsf(m * a.scale_log2) > 1024.0f && m != -INFINITY; };
         bool ok = true;
         for (int i = 0; i < my_rounds; ++i) {
           if (!__all_sync(0xffffffffu, mbar_wait(&bars.s_full[t], (rounds[0] + i) & 1))) {
@@ -512,51 +518,67 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
             continue;
           }
           uint32_t x[kTcKeys];
+          for (bool again = true; again;) {
+            again = false;
 #pragma unroll
-          for (int c = 0; c < kTcKeys; c += 32) tmem_ld32_async(s_at + c, x + c);
-          tmem_ld_done(x);
-          // A key that the prefix's last two tiles both have counts half in each. (Not 0 in one of them: an infinite value
-          // times 0 is NaN.) In a single tile they lie before the first key, where the copy brings zeros, and are none.
-          if ((i << doubled) >= shared_from) {
-            const int twice = -s.len & (kTcKeys - 1);
-            const float less = s.tiles == 1 ? INFINITY : 1.0f / a.scale_log2;
-            if ((i << doubled) > shared_from) {  // the last
+            for (int c = 0; c < kTcKeys; c += 32) tmem_ld32_async(s_at + c, x + c);
+            tmem_ld_done(x);
+            // A key that the prefix's last two tiles both have counts half in each. (Not 0 in one of them: an infinite value
+            // times 0 is NaN.) In a single tile they lie before the first key, where the copy brings zeros, and are none.
+            if (based || (i << doubled) >= shared_from) {
+              const int twice = -s.len & (kTcKeys - 1);
+              const float less = s.tiles == 1 ? INFINITY : 1.0f / a.scale_log2;
+              if (based) {
 #pragma unroll
-              for (int c = 0; c < kTcKeys; ++c)
-                if (c < twice) x[c] = __float_as_uint(__uint_as_float(x[c]) - less);
-            } else {
+                for (int c = 0; c < kTcKeys; ++c) x[c] = __float_as_uint(__uint_as_float(x[c]) - base);
+              }
+              if ((i << doubled) > shared_from) {  // the last
 #pragma unroll
-              for (int c = 0; c < kTcKeys; ++c)
-                if (c >= kTcKeys - twice) x[c] = __float_as_uint(__uint_as_float(x[c]) - less);
+                for (int c = 0; c < kTcKeys; ++c)
+                  if (c < twice) x[c] = __float_as_uint(__uint_as_float(x[c]) - less);
+              } else if ((i << doubled) == shared_from) {
+#pragma unroll
+                for (int c = 0; c < kTcKeys; ++c)
+                  if (c >= kTcKeys - twice) x[c] = __float_as_uint(__uint_as_float(x[c]) - less);
+              }
             }
-          }
-          float top[4];
+            float top[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) top[e] = __uint_as_float(x[e]);
+            for (int e = 0; e < 4; ++e) top[e] = __uint_as_float(x[e]);
 #pragma unroll
-          for (int c = 4; c < kTcKeys; c += 8)
+            for (int c = 4; c < kTcKeys; c += 8)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              top[e] = max3_nan(top[e], __uint_as_float(x[c + e]),
-                                __uint_as_float(x[c + 4 + e < kTcKeys ? c + 4 + e : c + e]));
-          const float peak = max3_nan(max3_nan(top[0], top[1], top[2]), top[3], top[3]);
-          if (i == 0) {
-            m = peak;
-          } else {
-            const bool moves = !((peak - m) * a.scale_log2 <= kSlack) && peak != m;  // also where m is -inf or one is NaN
-            if (__any_sync(0xffffffffu, moves)) {
-              const float to = max3_nan(m, peak, peak);  // NaN: every weight of the row becomes one
-              const float f = to == m ? 1.0f : exp2_fast((m - to) * a.scale_log2);
-              m = to;
-              l *= f;
+              for (int e = 0; e < 4; ++e)
+                top[e] = max3_nan(top[e], __uint_as_float(x[c + e]),
+                                  __uint_as_float(x[c + 4 + e < kTcKeys ? c + 4 + e : c + e]));
+            const float peak = max3_nan(max3_nan(top[0], top[1], top[2]), top[3], top[3]);
+            if (i == 0) {
+              m = peak;
+              again = __any_sync(0xffffffffu, is_far(m));
+            } else {
+              const bool moves = !((peak - m) * a.scale_log2 <= kSlack) && peak != m;  // also where m is -inf or one is NaN
+              if (__any_sync(0xffffffffu, moves)) {
+                const float to = max3_nan(m, peak, peak);  // NaN: every weight of the row becomes one
+                const float f = to == m ? 1.0f : exp2_fast((m - to) * a.scale_log2);
+                m = to;
+                l *= f;
+                again = __any_sync(0xffffffffu, is_far(m));
 #pragma unroll
-              for (int c = 0; c < kDim; c += 32) {
-                uint32_t o[32];
-                tmem_ld32_async(o_at + c, o);
-                tmem_ld_done(o);
+                for (int c = 0; c < kDim; c += 32) {
+                  uint32_t o[32];
+                  tmem_ld32_async(o_at + c, o);
+                  tmem_ld_done(o);
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                tmem_st32(o_at + c, o);
+                  for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                  tmem_st32(o_at + c, o);
+                }
+              }
+            }
+            if (again) {
+              based = true;
+              if (is_far(m)) {
+                base += m;
+                m = l == 0.0f ? -INFINITY : 0.0f;
               }
             }
           }
@@ -595,7 +617,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
         const int slot = a.split ? 2 * s.slot + t : s.slot;
         const bool mine = r < s.count && ok;
         if (mine) {
-          a.part_ml[cell + slot] = m == -INFINITY || s.len == 0 ? make_float2(-INFINITY, 0.0f) : make_float2(m * a.scale_log2, l);
+          a.part_ml[cell + slot] = m == -INFINITY || s.len == 0 ? make_float2(-INFINITY, 0.0f) : make_float2(__fmul_rn(base, a.scale_log2) + m * a.scale_log2, l);
           if (s.tile0 == 0 && (t == 0 || !a.split))  // the slots that no block comes to
             for (int k = a.split ? 2 * s.used : s.used; k < a.prefix_slots; ++k)
               a.part_ml[cell + k] = make_float2(-INFINITY, 0.0f);

@@ -436,3 +436,107 @@ def test_many_rows_on_a_stream_and_from_a_graph(cuda):
     graph.replay()
     torch.cuda.synchronize()
     check(c, call=False)
+
+
+# ---- scores of any magnitude
+
+def level_case(level, rows, lengths, dim, scale_log=8):
+    """Rows of sequences behind prefixes; a row's scores are exact in fp32: sums of products of powers of two, most of
+    them `level` * 2^-8, and of some keys, the row's greatest, all the same."""
+    import torch
+    c = make(lengths, [40 + 7 * i for i in range(len(rows))], 8, 2, dim, rows=rows)
+    c["scale"] = 2.0 ** scale_log
+    # score = scale * q . k = scale * dim * q * k
+    unit = level / (c["scale"] * dim)
+    q = 2.0 ** 8
+    c["q"].fill_(q)
+    for name in ("prefix_k", "k"):
+        t = c[name]
+        real = t[..., 0].isfinite()
+        t[real] = 0.0
+        index = torch.arange(t.shape[2], device="cuda")
+        best = (index % 5 == 3).expand(t.shape[:3]) & real
+        # positive levels: the best keys alone have them; negative ones: all keys, the best half as far down
+        t[real] = 0.0 if level > 0 else 2.0 * unit / q
+        t[best] = unit / q
+    return c
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("level", [2.0 ** 12, 2.0 ** 26, 2.0 ** 31, 2.0 ** 34, 2.0 ** 60, -2.0 ** 12, -2.0 ** 26,
+                                   -2.0 ** 33, -2.0 ** 34, -2.0 ** 60])
+@pytest.mark.parametrize("rows,lengths", [([60, 70], [300, 200]), ([9, 11], [300, 90]), ([600, 3], [1000, 128]),
+                                          ([2, 1], [700, 130])])
+def test_scores_of_any_magnitude(cuda, level, rows, lengths, dim):
+    """Many keys with a row's greatest score share its weight, however large the score is and however many rows there are."""
+    import torch
+    c = level_case(level, rows, lengths, dim)
+    M.prefix_attention(**c)
+    M.ops_check()
+    per, r0 = len(rows) // len(lengths), 0
+    for b, n in enumerate(rows):
+        plen, own = lengths[b // per], int(c["lens"][b])
+        for j in range(n):
+            seen = max(0, own - (n - 1 - j))
+            pick = torch.arange(plen, device="cuda") % 5 == 3
+            mine = torch.arange(seen, device="cuda") % 5 == 3
+            if j not in (0, n // 2, n - 1) or not (pick.any() or mine.any()):
+                continue
+            for h in (0, 7):
+                v = torch.cat([c["prefix_v"][b // per, h // 4, :plen][pick], c["v"][b, h // 4, :seen][mine]]).double()
+                want = v.mean(0)
+                # n equal weights, 1 or (a key that two tiles have) 1/2 each: exact in bf16; their fp32 sums, and the result's rounding
+                tol = (v.shape[0] + 64) * 2.0 ** -22 * v.abs().mean(0) + 2.0 ** -8 * want.abs() + 1e-30
+                got = c["out"][r0 + j, h].double()
+                assert ((got - want).abs() <= tol).all(), (b, j, h, (got - want).abs().max().item())
+                lse = level + math.log(v.shape[0])
+                assert abs(c["lse"][r0 + j, h].item() - lse) <= 2.0 ** -21 * abs(lse)
+        r0 += n
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("rows", [[60, 70], [300, 9], [2, 1]])
+@pytest.mark.parametrize("levels", [[-2.0 ** 34, 1.0], [1.0, -2.0 ** 34], [-2.0 ** 40, -2.0 ** 34, -2.0 ** 33, -2.0 ** 12, -2.0 ** 11, 1.0],
+                                    [-2.0 ** 12, -2.0 ** 10, 1.0, -2.0 ** 36], [-2.0 ** 60, -2.0 ** 60, -2.0 ** 11, 1.0]])
+def test_scores_that_come_from_afar(cuda, levels, rows, dim):
+    """Keys with ordinary scores before, behind and between keys far below them, 150 of each in turn: those have no weight."""
+    import torch
+    c = make([1000, 515], [40, 50], 8, 2, dim, rows=rows)
+    c["scale"] = 1.0
+    c["q"].zero_()
+    c["q"][..., 0] = 1.0
+    ordinary = []  # of each prefix, the keys that count, and those that do without them: the highest level's
+    for p, n in enumerate([1000, 515]):
+        level = torch.tensor(levels, device="cuda")[torch.arange(n, device="cuda") // 150 % len(levels)]
+        t = c["prefix_k"][p, :, :n]
+        t.copy_(torch.where((level == 1.0)[None, :, None], t, level[None, :, None].to(t.dtype)))
+        ordinary.append((level == 1.0, level == level.max()))
+    M.prefix_attention(**c)
+    M.ops_check()
+    r0 = 0
+    for b, n in enumerate(rows):
+        own = int(c["lens"][b])
+        for j in (0, n // 2, n - 1):
+            seen = max(0, own - (n - 1 - j))
+            for h in (0, 7):
+                g, (at, highest) = h // 4, ordinary[b]
+                plen = at.numel()
+                at = at if at.any() or seen > 0 else highest
+                s = torch.cat([c["prefix_k"][b, g, :plen, 0][at], c["k"][b, g, :seen, 0]]).double()
+                v = torch.cat([c["prefix_v"][b, g, :plen][at], c["v"][b, g, :seen]]).double()
+                w = torch.softmax(s, 0)
+                # The scores are single products with 1, exact. A weight is rounded to bf16 and off by the rounding of a
+                # shift of up to 1024 (2^-14 of an exponent) and 2^-20 else; then the sums, and the result's rounding.
+                tol = (w @ v.abs()) * (2.0 ** -8 + 2.0 ** -13 + (s.numel() + 64) * 2.0 ** -22) + 2.0 ** -8 * (w @ v).abs()
+                got = c["out"][r0 + j, h].double()
+                assert ((got - w @ v).abs() <= tol).all(), (b, j, h, ((got - w @ v).abs() - tol).max().item())
+                lse = torch.logsumexp(s, 0).item()
+                assert abs(c["lse"][r0 + j, h].item() - lse) <= 2.0 ** -13 + (s.numel() + 64) * 2.0 ** -22 + 2.0 ** -21 * abs(lse)
+        r0 += n
+
+
+def test_a_scale_too_small_for_its_inverse(cuda):
+    c = make([600, 90], [40, 70, 20, 33], 8, 2, 128, rows=[40, 30, 20, 1])
+    for scale in (1e-38, 1e-39, 1e-44):
+        c["scale"] = scale
+        check(c)
