@@ -79,6 +79,7 @@ struct Segment {
 // and every block takes the same number of units, whatever the lengths.
 struct Grid {
   int prefixes, sequences;  // that this launch has to do with
+  unsigned most_units;      // there can be
   // 1: launched behind a kernel of the same call, which this one takes nothing from. That kernel lets this one start
   // when it has itself waited for all work before the call, so the wait for it can come last.
   int late_wait;
@@ -108,15 +109,15 @@ __device__ __forceinline__ unsigned block_scan(unsigned v, unsigned* part, unsig
 #pragma unroll
   for (int off = 1; off < 32; off *= 2) {
     const unsigned other = __shfl_up_sync(0xffffffffu, v, off);
-    if (lane >= off) v += other;
+    if (lane >= off) v = add_saturated(v, other);
   }
   if (lane == 31) part[warp] = v;
   __syncthreads();
   *total = 0;
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) {
-    if (w < warp) v += part[w];
-    *total += part[w];
+    if (w < warp) v = add_saturated(v, part[w]);
+    *total = add_saturated(*total, part[w]);
   }
   return v;
 }
@@ -750,7 +751,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) attention_rows_kernel(Atten
   unsigned rest = 0;
   for (int e = kThreads + threadIdx.x; e < sources; e += kThreads) {
     Source s{};
-    rest += source_units<kPrefixRows, kOwnRows>(a, g, e, &s);
+    rest = add_saturated(rest, source_units<kPrefixRows, kOwnRows>(a, g, e, &s));
     if (s.tiles > 0) atomicMax(&most[e >= g.prefixes], s.stages);
   }
   unsigned first_round, total;
@@ -759,8 +760,9 @@ __global__ void __launch_bounds__(kThreads, kBlocks) attention_rows_kernel(Atten
   if (sources > kThreads) {
     unsigned others;
     block_scan(rest, part[1], &others);
-    total += others;
+    total = add_saturated(total, others);
   }
+  if (total > g.most_units) total = 0;  // row offsets out of order: recorded
   // No range of keys meets more blocks than there are slots for it.
   const int own_slots = a.slots - a.prefix_slots;
   unsigned share = max((total + gridDim.x - 1) / gridDim.x, static_cast<unsigned>(kMinShare));
@@ -987,6 +989,7 @@ struct Plan {
   int prefix_slots, own_slots;
   int prefix_warps, own_warps;  // of the kernel for few rows: warps side by side along the rows of a tile
   unsigned blocks;
+  int64_t units;      // of that kernel's work, there can be
   bool whole_own;     // the own keys of a tile of rows by one block, which joins the prefix's parts to them
   int64_t own_tiles;  // there can be
 };
@@ -1024,7 +1027,7 @@ Plan plan_of(const uocr_prefix_attention_args& a) {
   // Own keys in parts only where few blocks would have many: a join less, and own parts that are not written and read.
   // Four sequences of 300, 512 and 1024 own keys take 12.2, 13.7 and 20.2 us whole, 15.3, 16.6 and 16.4 in parts.
   p.whole_own = p.own_tiles * a.kv_heads >= kSms || own_stages <= 8;
-  const int64_t units =
+  const int64_t units = p.units =
       a.kv_heads * ((p.tc ? 0 : tiles(a.prefixes, a.sequences / a.prefixes, p.prefix_warps) * prefix_stages) +
                     (p.whole_own ? 0 : p.own_tiles * own_stages));
   p.blocks = static_cast<unsigned>(std::min<int64_t>(units, kBlocks * kSms));
@@ -1081,6 +1084,7 @@ cudaError_t launch(const uocr_prefix_attention_args& args, const Attention& a, c
   g.prefixes = p.tc || args.prefix_capacity == 0 ? 0 : a.prefixes;
   g.sequences = args.capacity == 0 || p.whole_own ? 0 : a.sequences;
   g.late_wait = p.tc;
+  g.most_units = static_cast<unsigned>(p.units);
   cudaError_t st = p.tc ? launch_attention_tc(a, kDim, kSms, stream) : cudaSuccess;
   if (st == cudaSuccess && p.blocks > 0) {
     const int own = g.sequences == 0 ? p.prefix_warps : p.own_warps;

@@ -34,6 +34,7 @@ struct Attention {
   int prefix_capacity, capacity;
   int prefix_slots, slots;
   bool split;  // tensor-core kernel: a block's two tiles are the same rows, for every other 128 keys
+  unsigned tc_units;  // and the most units it can have
   float scale_log2;
   float* part_o;     // [rows, heads, slots, dim]
   float2* part_ml;   // [rows, heads, slots]
@@ -67,6 +68,13 @@ __device__ __forceinline__ int prefix_rows_of(const Attention& a, int p, int* fi
     return 0;
   }
   return r1 - r0;
+}
+
+// a + b, or the most that an unsigned holds. Rows that offsets out of order name many times over would otherwise make
+// sums of units that have gone past it; where a sum is above what there can be, no units are worked on.
+__device__ __forceinline__ unsigned add_saturated(unsigned a, unsigned b) {
+  const unsigned s = a + b;
+  return s < a ? ~0u : s;
 }
 
 __device__ __forceinline__ int prefix_len_of(const Attention& a, int p) {

@@ -38,7 +38,7 @@ constexpr int kTileRows = kAttentionTcRows;
 // What a range costs besides its keys, in units: 128 keys take 1.8 us for two tiles of rows, 0.6 (the memory's rate) where
 // the tiles split them. With 4, 6, 8 and 12 for the latter sixteen pages take 53.3, 53.5, 54.2 and 55.1 us, with 2, 3 and
 // 4 for the former prompts on a page 107.9, 107.6 and 107.7, a document 51.2, 51.2 and 52.0.
-__device__ __forceinline__ unsigned range_units(const Attention& a) { return a.split ? 4 : 3; }
+__host__ __device__ __forceinline__ unsigned range_units(const Attention& a) { return a.split ? 4 : 3; }
 constexpr int kTcKeys = 128;
 constexpr int kSlots = 4;        // shared-memory slots of 128 keys or values
 constexpr int kTcThreads = 384;  // a warpgroup for copies and MMAs, two of rows
@@ -186,7 +186,7 @@ __device__ __forceinline__ unsigned warp_scan(unsigned v) {
 #pragma unroll
   for (int off = 1; off < 32; off *= 2) {
     const unsigned other = __shfl_up_sync(0xffffffffu, v, off);
-    if (lane >= off) v += other;
+    if (lane >= off) v = add_saturated(v, other);
   }
   return v;
 }
@@ -214,9 +214,10 @@ __device__ __forceinline__ Schedule make_schedule(const Attention& a) {
   int most = c.mine.ranges > 0 ? c.mine.tiles : 1;
   for (int p = 32 + lane; p < (a.prefixes + 31) / 32 * 32; p += 32) {
     Prefix x{};
-    total += __reduce_add_sync(0xffffffffu, units_of(a, p, &x));
+    total = add_saturated(total, __shfl_sync(0xffffffffu, warp_scan(units_of(a, p, &x)), 31));
     if (x.ranges > 0) most = max(most, x.tiles);
   }
+  if (total > a.tc_units) total = 0;  // row offsets out of order: recorded
   most = __reduce_max_sync(0xffffffffu, most);
   // No range of keys meets more blocks than there are slots for (two of a block that splits the keys).
   const unsigned blocks = a.split ? a.prefix_slots / 2 : a.prefix_slots;
@@ -688,6 +689,9 @@ cudaError_t launch(const TcArgs& t, unsigned blocks, cudaStream_t stream) {
 cudaError_t launch_attention_tc(const Attention& a, int dim, unsigned blocks, cudaStream_t stream) {
   TcArgs t{};
   t.a = a;
+  const int64_t of_range = a.split ? kTileRows : 2 * kTileRows, tiles = (a.prefix_capacity + kTcKeys - 1) / kTcKeys;
+  t.a.tc_units = static_cast<unsigned>(
+      a.kv_heads * (static_cast<int64_t>(a.rows) * a.group / of_range + std::min(a.prefixes, a.rows)) * (tiles + range_units(a)));
   if (!make_cache_tmap(&t.k, a.prefix_k, dim, a.prefix_capacity, a.kv_heads, a.prefixes, a.prefix_head_stride,
                        a.prefix_stride, kTcKeys) ||
       !make_cache_tmap(&t.v, a.prefix_v, dim, a.prefix_capacity, a.kv_heads, a.prefixes, a.prefix_head_stride,

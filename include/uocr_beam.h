@@ -123,8 +123,9 @@ int uocr_prefix_attention_workspace(const uocr_prefix_attention_args* args, int6
  * Rows outside row_offsets[0] .. row_offsets[sequences] are left as they are.
  * A length out of range is recorded and taken as the nearest that is in range;
  * a sequence whose row offsets are not in order is recorded, its rows
- * unspecified; a bad ancestor is recorded, and the sequence's own cache (cache 0
- * where it has none) read in its place. */
+ * unspecified (where such offsets name rows many times over, all rows); a bad
+ * ancestor is recorded, and the sequence's own cache (cache 0 where it has none)
+ * read in its place. */
 int uocr_prefix_attention(const uocr_prefix_attention_args* args, void* stream);
 
 /* ---- selection of beams ---- */

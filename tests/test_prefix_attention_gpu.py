@@ -540,3 +540,35 @@ def test_a_scale_too_small_for_its_inverse(cuda):
     for scale in (1e-38, 1e-39, 1e-44):
         c["scale"] = scale
         check(c)
+
+
+@pytest.mark.parametrize("heads,keys", [(1, 32800), (32, 16000)])
+def test_row_offsets_that_name_rows_many_times_over(cuda, heads, keys):
+    """The sum of what they name is more than 2^32 units of work, for the kernels of few and of many rows: reported, and
+    nothing outside the rows is written."""
+    import torch
+    n, dim, bf16, i32 = 16384, 64, torch.bfloat16, torch.int32
+    memory = torch.randn(keys + n, dim, generator=gen_of(heads, keys), device="cuda").to(bf16)
+    prefix = torch.as_strided(memory, (n, 1, keys, dim), (0 if heads == 1 else dim, keys * dim, dim, 1))
+    none = torch.empty(n, 1, 0, dim, dtype=bf16, device="cuda")
+    whole = torch.full((n + 2, heads, dim), 33.0, dtype=bf16, device="cuda")
+    q = torch.randn(n, heads, dim, generator=gen_of(heads), device="cuda").to(bf16)
+    offsets = torch.zeros(n + 1, dtype=i32, device="cuda")
+    offsets[1::2] = n
+    c = dict(q=q, prefix_k=prefix, prefix_v=prefix, prefix_lens=torch.full((n,), keys, dtype=i32, device="cuda"), k=none,
+             v=none, lens=torch.zeros(n, dtype=i32, device="cuda"), out=whole[1:-1], row_offsets=offsets)
+    M.prefix_attention(**c)
+    with pytest.raises(M.UocrError) as e:
+        M.ops_check()
+    assert e.value.code == 5 and "rows" in str(e.value)
+    assert (whole[0] == 33.0).all() and (whole[-1] == 33.0).all()
+    # The same call in order, a row each behind a few keys.
+    offsets.copy_(torch.arange(n + 1, device="cuda"))
+    c["prefix_lens"].fill_(70)
+    M.prefix_attention(**c)
+    M.ops_check()
+    for row in (0, 1, 8191, n - 1):
+        k = prefix[row, 0, :70].double()
+        w = torch.softmax(q[row].double() @ k.T * dim ** -0.5, -1)
+        tol = (w @ k.abs()) * (2.0 ** -8 + 2.0 ** -12) + 2.0 ** -8 * (w @ k).abs()  # see above; 134 keys, |s| below 40
+        assert ((whole[1 + row].double() - w @ k).abs() <= tol).all()
