@@ -36,6 +36,24 @@ bool aligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) %
 bool cache_ok(const void* p, int64_t stride, int64_t head_stride) {
   return aligned(p, 16) && stride % 8 == 0 && head_stride % 8 == 0 && stride >= 0 && head_stride >= 0;
 }
+// Whether the pieces of `extent` at a dimension's multiples of a stride, of every dimension, lie apart as views of memory
+// do: each stride is at least what the dimensions of smaller strides span.
+struct Dim {
+  int64_t count, stride;
+};
+bool apart(int64_t extent, std::initializer_list<Dim> list) {
+  Dim dims[4];
+  size_t n = 0;
+  for (const Dim& d : list)
+    if (d.count > 1) dims[n++] = d;
+  std::sort(dims, dims + n, [](const Dim& a, const Dim& b) { return a.stride < b.stride; });
+  double span = static_cast<double>(extent);  // counts and strides of any size
+  for (size_t i = 0; i < n; ++i) {
+    if (static_cast<double>(dims[i].stride) < span) return false;
+    span += static_cast<double>(dims[i].stride) * static_cast<double>(dims[i].count - 1);
+  }
+  return true;
+}
 // a * b * ... stays a sum of bytes that int64_t holds.
 bool product_fits(std::initializer_list<int64_t> v) {
   double p = 1.0;
@@ -140,8 +158,8 @@ int uocr_rotate_heads(const uocr_rotate_heads_args* a, void* stream) {
     if (!in(a->caches, 1, kMaxCount) || !in(a->capacity, 1, kMaxCount)) return bad(op, "bad shape");
     if (!cache_ok(a->k_cache, a->cache_stride, a->head_stride) || !cache_ok(a->v_cache, a->cache_stride, a->head_stride))
       return bad(op, "the caches' bases and strides must be multiples of 16 bytes");
-    if (a->kv_heads > 1 && a->head_stride < a->capacity * a->head_dim && a->cache_stride < a->capacity * a->head_dim)
-      return bad(op, "a cache's heads overlap");
+    if (!apart(a->capacity * a->head_dim, {{a->kv_heads, a->head_stride}, {a->caches, a->cache_stride}}))
+      return bad(op, "the caches or their heads overlap");
   }
   ErrorWord* err = nullptr;
   const cudaError_t st = ops_error_word(&err);

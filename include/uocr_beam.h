@@ -73,7 +73,8 @@ typedef struct uocr_rotate_heads_args {
  * in 64 bits, so that far positions keep their angle — rounded to bf16: q into
  * q_out, k and v (v only rounded) into the caches at [cache_rows[r], :, slots[r]].
  * head_dim is a multiple of 8 up to 256, rotary_dim one of 8 up to head_dim (0:
- * no rotation). The caches' bases and strides are multiples of 16 bytes. A row
+ * no rotation). The caches' bases and strides are multiples of 16 bytes, and caches
+ * and heads lie apart. A row
  * whose cache or slot does not exist is not appended (recorded); of two rows
  * with the same place, either may stay. */
 int uocr_rotate_heads(const uocr_rotate_heads_args* args, void* stream);

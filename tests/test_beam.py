@@ -262,3 +262,26 @@ int main() {
     subprocess.run([cxx, "-std=c++17", "-I", INCLUDE, str(src), "-o", str(exe), M.LIB_PATH, f"-Wl,-rpath,{lib}"], check=True)
     out = subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()
     assert out[:6] == ["1"] * 6 and abs(float(out[6]) - (0.1 * math.log(4.0) + 1)) < 1e-6
+
+
+@pytest.mark.parametrize("wrong", [
+    dict(head_stride=0), dict(head_stride=512), dict(head_stride=1016), dict(cache_stride=0), dict(cache_stride=1024),
+    dict(cache_stride=2040), dict(kv_heads=1, cache_stride=1016), dict(caches=1, cache_stride=0, head_stride=1016),
+    dict(head_stride=4096, cache_stride=1016), dict(head_stride=4088, cache_stride=1024)])
+def test_rotate_heads_refuses_caches_that_overlap(wrong):
+    """Each stride alone, in both orders of caches and heads: the caches are written."""
+    base = dict(ROTATE, q_out=BASE + 4096)
+    assert _call("uocr_rotate_heads", M.RotateHeadsArgs, base, wrong) == 1
+    assert "overlap" in M.lib().uocr_last_error().decode()
+
+
+@pytest.mark.parametrize("right", [dict(), dict(caches=1, cache_stride=0), dict(kv_heads=1, head_stride=0),
+                                   dict(head_stride=4096, cache_stride=1024), dict(head_stride=1 << 40, cache_stride=1 << 30)])
+def test_rotate_heads_takes_caches_that_lie_apart(right):
+    """The first check behind the overlap's is the device's, which this machine may not have."""
+    base = dict(ROTATE, q_out=BASE + 4096)
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("the addresses are none of a device's")
+    _call("uocr_rotate_heads", M.RotateHeadsArgs, base, right)
+    assert "overlap" not in M.lib().uocr_last_error().decode()
