@@ -257,6 +257,8 @@ int uocr_reorder_states(const uocr_reorder_states_args* a, void* stream) {
   if (!product_fits({a->layers, a->groups, a->segments, segment}) ||
       a->layers * a->groups * a->segments > kMaxCount / ((segment + 127) / 128))
     return unsupported(op, "too large");
+  if (!apart(segment, {{a->layers, a->layer_stride}, {a->groups * a->beams, a->row_stride}, {a->segments, a->segment_stride}}))
+    return bad(op, "layers, rows or segments overlap");
   ErrorWord* err = nullptr;
   const cudaError_t st = ops_error_word(&err);
   return done(op, st != cudaSuccess ? st : launch_reorder_states(*a, err, static_cast<cudaStream_t>(stream)));

@@ -179,7 +179,8 @@ typedef struct uocr_reorder_states_args {
  * all beams at once: counts[parent] units of every segment; what follows them in
  * the row stays. A beam that is its own parent is not touched. beams is at most
  * UOCR_BEAM_MAX. A bad parent is recorded and leaves its row as it is; a count
- * out of range is recorded and taken as the nearest that is in range. */
+ * out of range is recorded and taken as the nearest that is in range. Layers, rows
+ * and segments lie apart, in any order. */
 int uocr_reorder_states(const uocr_reorder_states_args* args, void* stream);
 
 /* ---- beam search on the page decoder ---- */

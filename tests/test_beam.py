@@ -285,3 +285,24 @@ def test_rotate_heads_takes_caches_that_lie_apart(right):
         pytest.skip("the addresses are none of a device's")
     _call("uocr_rotate_heads", M.RotateHeadsArgs, base, right)
     assert "overlap" not in M.lib().uocr_last_error().decode()
+
+
+@pytest.mark.parametrize("wrong", [
+    dict(row_stride=128), dict(row_stride=255), dict(segment_stride=256), dict(layer_stride=3071), dict(layer_stride=128),
+    dict(segment_stride=256, row_stride=256), dict(layers=1, groups=1, beams=2, segments=3, row_stride=300),
+    dict(segments=1, layer_stride=1024), dict(layer_stride=256, row_stride=511)])
+def test_reorder_states_refuses_rows_that_overlap(wrong):
+    assert _call("uocr_reorder_states", M.ReorderStatesArgs, REORDER, wrong) == 1
+    assert "overlap" in M.lib().uocr_last_error().decode()
+
+
+@pytest.mark.parametrize("right", [
+    dict(), dict(layer_stride=3072), dict(layer_stride=256, row_stride=512), dict(segment_stride=1536, row_stride=128),
+    dict(layers=1, layer_stride=0), dict(segments=1, segment_stride=0, row_stride=128), dict(beams=1, groups=1, row_stride=0)])
+def test_reorder_states_takes_any_order_of_layers_rows_and_segments(right):
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("the addresses are none of a device's")
+    _call("uocr_reorder_states", M.ReorderStatesArgs, REORDER, right)
+    error = M.lib().uocr_last_error().decode()
+    assert "overlap" not in error and "segment" not in error
