@@ -1000,17 +1000,17 @@ constexpr int kSms = 148;  // blocks of the tensor-core kernel, one an SM; corre
 // about 32 rows on (16 rows 14.9 us against 12.2, 20 rows 15.0 against 14.7, 32 rows 15.1 against 15.0; of sixteen pages
 // 47.8 against 50.3, 55.0 against 56.6).
 bool many_rows(const uocr_prefix_attention_args& a) {
-  const int64_t group = a.heads / a.kv_heads;
-  if (a.prefix_capacity == 0 || !(a.scale >= FLT_MIN)) return false;  // it divides by the scale
-  // what a tensor map takes
+  return a.prefix_capacity > 0 && a.rows * (a.heads / a.kv_heads) / a.prefixes > 16;
+}
+// Whether that kernel takes the call's scale, which it divides by, and strides, for its tensor maps.
+bool tc_takes(const uocr_prefix_attention_args& a) {
   auto far = [](int64_t stride) { return stride <= 0 || stride >= (int64_t{1} << 39); };
-  if ((a.kv_heads > 1 && far(a.prefix_head_stride)) || (a.prefixes > 1 && far(a.prefix_stride))) return false;
-  return a.rows * group / a.prefixes > 16;
+  return a.scale >= FLT_MIN && !(a.kv_heads > 1 && far(a.prefix_head_stride)) && !(a.prefixes > 1 && far(a.prefix_stride));
 }
 
-Plan plan_of(const uocr_prefix_attention_args& a) {
+Plan plan_of(const uocr_prefix_attention_args& a, bool tc) {
   Plan p{};
-  p.tc = many_rows(a);
+  p.tc = tc;
   const int64_t group = a.heads / a.kv_heads;
   // Rows of a tile by those of a prefix, of a sequence.
   auto warps_for = [](int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; };
@@ -1124,12 +1124,18 @@ bool prefix_attention_counts(const uocr_prefix_attention_args& a) {
 }
 
 size_t prefix_attention_bytes(const uocr_prefix_attention_args& a) {
-  const Plan p = plan_of(a);
-  return static_cast<size_t>(a.rows * a.heads) * (p.prefix_slots + p.own_slots) * (a.head_dim * 4 + sizeof(float2));
+  // By the sizes alone: room for either kernel where the scale or the strides may decide.
+  const Plan few = plan_of(a, false);
+  int slots = few.prefix_slots + few.own_slots;
+  if (many_rows(a)) {
+    const Plan many = plan_of(a, true);
+    slots = std::max(slots, many.prefix_slots + many.own_slots);
+  }
+  return static_cast<size_t>(a.rows * a.heads) * slots * (a.head_dim * 4 + sizeof(float2));
 }
 
 cudaError_t launch_prefix_attention(const uocr_prefix_attention_args& args, ErrorWord* err, cudaStream_t stream) {
-  const Plan p = plan_of(args);
+  const Plan p = plan_of(args, many_rows(args) && tc_takes(args));
   Attention a{};
   a.q = reinterpret_cast<const __nv_bfloat16*>(args.q);
   a.prefix_k = reinterpret_cast<const __nv_bfloat16*>(args.prefix_k);

@@ -108,7 +108,7 @@ typedef struct uocr_prefix_attention_args {
 } uocr_prefix_attention_args;
 
 /* Bytes of workspace the call below needs with these sizes (pointers are not
- * looked at, but for row_offsets being NULL or not). */
+ * looked at, but for row_offsets being NULL or not; nor are scale, pitches and strides). */
 int uocr_prefix_attention_workspace(const uocr_prefix_attention_args* args, int64_t* bytes);
 
 /* out = softmax(scale * q k^T) v. Sequence b stands behind prefix

@@ -306,3 +306,22 @@ def test_reorder_states_takes_any_order_of_layers_rows_and_segments(right):
     _call("uocr_reorder_states", M.ReorderStatesArgs, REORDER, right)
     error = M.lib().uocr_last_error().decode()
     assert "overlap" not in error and "segment" not in error
+
+
+def test_prefix_attention_workspace_depends_on_sizes_alone():
+    """A query before scale, pitches and strides are set says what the call will need."""
+    def need(**kw):
+        out = ctypes.c_int64(-1)
+        a = dict(ATTENTION)
+        a.update(kw)
+        assert M.lib().uocr_prefix_attention_workspace(ctypes.byref(M.PrefixAttentionArgs(**a)), ctypes.byref(out)) == 0
+        return out.value
+    unset = dict(scale=0.0, ldq=0, ldo=0, ld_ancestry=0, prefix_stride=0, prefix_head_stride=0, cache_stride=0, head_stride=0)
+    for rows, sequences, prefixes, heads, kv in ((6, 6, 2, 4, 2), (40, 40, 1, 16, 4), (200, 4, 1, 8, 2), (700, 140, 70, 4, 4),
+                                                 (6000, 24, 1, 16, 4), (128, 128, 16, 16, 4)):
+        for keys, own in ((100, 20), (4096, 300), (33000, 2000), (70, 0), (0, 20)):
+            sizes = dict(rows=rows, sequences=sequences, prefixes=prefixes, caches=sequences, heads=heads, kv_heads=kv,
+                         prefix_capacity=keys, capacity=own, row_offsets=None if rows == sequences else BASE)
+            assert need(**sizes) == need(**sizes, **unset), sizes
+            assert need(**sizes) == need(**sizes, **dict(unset, scale=0.125))
+            assert need(**sizes) == need(**sizes, **dict(unset, prefix_stride=keys * 1024, prefix_head_stride=keys * 128))
