@@ -191,3 +191,85 @@ def test_a_captured_search_repeats_itself(cuda, beams):
         _search(torch, dec, 2, 3)
     del graph
     dec.close()
+
+
+@pytest.mark.parametrize("fmt", [M.WEIGHT_BF16, M.WEIGHT_INT8])
+def test_a_search_behind_decoded_tokens_continues_them(cuda, fmt):
+    """Its scores are those of its tokens behind the prompt and the decoded tokens, and no worse than the oracle's best."""
+    import torch
+    shape = SHAPES[0]
+    dims, dec, weights = _build(torch, cuda, shape, fmt)
+    prompt = D.synth_prompt(dims, 5, 12)
+    first, toks = (torch.empty(n, dtype=torch.int32, device=cuda) for n in (1, 3))
+    dec.prefill(torch.from_numpy(prompt).to(cuda), token=first)
+    dec.decode(3, toks)
+    torch.cuda.synchronize()
+    consumed = (first.item(), *toks[:2].tolist())  # the third is chosen, not yet part of the sequence
+    tokens, scores, _ = _search(torch, dec, 4, 5)
+    ora = _Scored(dims, weights, prompt)
+
+    def score(t):
+        return sum(_log_softmax(ora.logits(consumed + tuple(t[:i])))[v] for i, v in enumerate(t))
+    want = [score(t) for t in tokens.tolist()]
+    tol = 2 * 5 * TOL[fmt] * ora.largest
+    # A search elsewhere (one decoded token less, or none) would have other scores: the test can tell.
+    elsewhere = [abs(sum(_log_softmax(ora.logits(consumed[:n] + tuple(t[:i])))[v] for i, v in enumerate(t)) - w)
+                 for t, w in zip(tokens.tolist(), want) for n in (0, 2)]
+    print(f"search behind decoded tokens, fmt {fmt}: {np.abs(scores - want).max():.4f} off, tolerance {tol:.3f}, "
+          f"elsewhere {min(elsewhere):.3f} to {max(elsewhere):.3f} off")
+    assert np.abs(scores - want).max() <= tol and max(elsewhere) > 2 * tol
+    alive = [(0.0, ())]
+    for _ in range(5):
+        cand = [(s + lp[t], h + (int(t),)) for s, h in alive
+                for lp in [_log_softmax(ora.logits(consumed + h))] for t in np.argsort(-lp)[:4]]
+        alive = sorted(cand, key=lambda c: -c[0])[:4]
+    assert scores[0] >= alive[0][0] - 2 * tol
+    dec.close()
+
+
+@pytest.mark.parametrize("decoded", [0, 3])
+def test_one_beam_is_the_greedy_sequence(cuda, decoded):
+    """Token by token, up to one that the oracle's logits cannot tell from the other's within both errors."""
+    import torch
+    shape = SHAPES[0]
+    dims, dec, weights = _build(torch, cuda, shape, M.WEIGHT_BF16)
+    prompt = D.synth_prompt(dims, 5, 12)
+    x = torch.from_numpy(prompt).to(cuda)
+    first, before, greedy = (torch.empty(n, dtype=torch.int32, device=cuda) for n in (1, 3, 8))
+    dec.prefill(x, token=first)
+    if decoded:
+        dec.decode(decoded, before)
+    one, _, _ = _search(torch, dec, 1, 7)
+    dec.decode(7, greedy)
+    torch.cuda.synchronize()
+    start = (first.item(), *before.tolist())[:decoded]
+    # The greedy sequence's next token is the one chosen last; decode() says those after it.
+    chosen = before[-1].item() if decoded else first.item()
+    sequence = [chosen, *greedy.tolist()]
+    ora = _Scored(dims, weights, prompt)
+    for i, (a, b) in enumerate(zip(one[0].tolist(), sequence)):
+        if a != b:
+            z = ora.logits(start + tuple(sequence[:i]))
+            assert abs(z[a] - z[b]) <= 2 * TOL[M.WEIGHT_BF16] * np.abs(z).max(), (i, a, b)
+            break
+    assert one[0, 0] == chosen
+    dec.close()
+
+
+@pytest.mark.parametrize("beams", [3, 8])
+@pytest.mark.parametrize("rows", [1100, 2500])
+def test_a_search_behind_a_long_page(cuda, rows, beams):
+    """A prefix that many blocks share, by the attention kernels for few and for many rows."""
+    import torch
+    shape = (512, 2, 4, 1, 1024, 8, 2, 128, 256, rows, 5)
+    dims, dec, weights = _build(torch, cuda, shape, M.WEIGHT_BF16)
+    prompt = D.synth_prompt(dims, 5, rows)
+    dec.prefill(torch.from_numpy(prompt).to(cuda))
+    tokens, scores, lengths = _search(torch, dec, beams, 5)
+    ora = _Scored(dims, weights, prompt)
+    want = [ora.score(t) for t in tokens.tolist()]
+    tol = 2 * 5 * TOL[M.WEIGHT_BF16] * ora.largest
+    print(f"search behind {rows} rows, {beams} beams: {np.abs(scores - want).max():.4f} off, tolerance {tol:.3f}")
+    assert np.abs(scores - want).max() <= tol and (lengths == 5).all() and (np.diff(scores) <= 0).all()
+    assert scores[0] >= ora.search(beams, 5)[0][0] - 2 * tol
+    dec.close()
