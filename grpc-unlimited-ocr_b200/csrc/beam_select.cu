@@ -6,7 +6,8 @@
 // `select` best logits; a second kernel joins a group's parts. Bound: the one
 // read of the logits; for few rows two launches and their rounds. 128 rows of 102400
 // logits take 23.1 us (2.3 TB/s: instructions and barriers, 8.0 at the copy rate),
-// four rows 7.9.
+// four rows 7.9; with all but 100 tokens masked 54.8 (-inf: 44.2) and 12.6, since
+// what equals the bound then reaches it.
 //
 // The best of a part without sorting it: the threads' own maxima, sorted within
 // warps, bound the select-th best of all from below. What

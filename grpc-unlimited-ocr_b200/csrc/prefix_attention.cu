@@ -22,7 +22,7 @@ constexpr int kThreads = 128;
 constexpr int kKeys = 64;    // of a stage
 constexpr int kStages = 2;
 constexpr int kBlocks = 3;   // of an SM
-// Stages of a block at least: with 2, 3, 4 and 6 the four rows of a page take 12.8, 14.4, 11.7 and 15.2 us, the parts
+// Stages of a block at least: with 2, 3, 4 and 6 the four rows of a page take 13.1, 14.0, 12.8 and 15.3 us, the parts
 // that fewer make costing the join more than the blocks save.
 constexpr int kMinShare = 4;
 constexpr int kMaxSlots = 160;  // of a row: the most that a plan gives its prefix and its own keys
@@ -581,10 +581,10 @@ __device__ __forceinline__ void attend(const Attention& a, const Segment& seg, u
 // 16 of a round's keys and brings them itself, into three slots of its own for 16
 // keys or values (K V K, then V K V): no barrier before the join, and with 52 KB a
 // block of four warps four blocks an SM, so that 512 ranges of own keys are under
-// way at once (with three some had to wait for the end of others: sixteen pages 59
-// against 57 us). A lane reads one key's ancestor, and the copies are a loop: the
+// way at once (with three some have to wait for the end of others: sixteen pages
+// 58.7 against 53.3 us). A lane reads one key's ancestor, and the copies are a loop: the
 // first instructions of a kernel come from memory like its data. Blocks that have an SM to themselves take eight warps and half the
-// rounds: four beams 13.5 against 11.7 us.
+// rounds: four beams 13.9 against 12.8 us.
 template <int kDim, int kWarps>
 struct FewRing {
   static constexpr int kSlot = 16 * (kDim + 8), kSlots = 3;
@@ -885,8 +885,8 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) attention_few_kernel
   extern __shared__ __align__(16) unsigned char raw[];
   __shared__ uint32_t free_word;
   if (!late_wait) pdl_wait();
-  // The next grid waits for this one, which waits for the one before it. Among small calls its early start is worth
-  // 1.5 us; behind many blocks it costs one (sixteen pages 58.5 against 59.4).
+  // The next grid waits for this one, which waits for the one before it. Among attention calls its early start makes
+  // little difference (four beams 12.8 us with and 13.0 without it, sixteen pages, which go without, 53.1 and 53.3).
   if (kWarps == 8) pdl_launch_dependents();
   attend_few<kDim, kWarps>(a, raw, &free_word, late_wait != 0);
 }
@@ -996,9 +996,15 @@ struct Plan {
 
 constexpr int kSms = 148;  // blocks of the tensor-core kernel, one an SM; correct on any number of SMs
 
-// A prefix with many rows is arithmetic, for the tensor-core kernel. At 4096 keys its start and way out are worth it from
-// about 32 rows on (16 rows 14.9 us against 12.2, 20 rows 15.0 against 14.7, 32 rows 15.1 against 15.0; of sixteen pages
-// 47.8 against 50.3, 55.0 against 56.6).
+// A prefix with many rows is arithmetic, for the tensor-core kernel: from more than 16 on, where the other kernel's tiles
+// grow (us, this one's and the other's, 60 own keys; a page of 100, 256, 1024 and 4096 keys, then sixteen such pages):
+//   16 rows  11.1 13.3  11.8 10.9  12.0 11.0  13.7 12.7    13.0 15.6  13.7 12.8  18.8 18.3  34.2 36.1
+//   20 rows  11.3 15.1  11.8 12.5  12.0 12.7  13.8 14.7    13.2 17.3  14.1 14.4  19.1 20.7  34.8 38.9
+//   24 rows  11.3 15.3  12.0 12.7  12.2 12.8  13.8 14.8    16.4 17.6  17.4 14.6  21.4 21.3  35.1 39.7
+//   32 rows  11.5 15.7  12.1 12.9  12.3 13.0  14.2 15.3    17.1 18.3  18.0 17.3  22.4 21.8  36.4 41.5
+//   64 rows  11.7 20.0  12.2 16.1  12.5 16.6  14.4 20.9    22.2 29.6  23.4 25.7  28.7 35.4  44.0 63.8
+// So it loses a little between 16 pages of 256 and 1024 keys at 24 and 32 rows, and at 7 sequences of 37 rows of heads of
+// 64 behind 1001 keys (16.5 against 13.5).
 bool many_rows(const uocr_prefix_attention_args& a) {
   return a.prefix_capacity > 0 && a.rows * (a.heads / a.kv_heads) / a.prefixes > 16;
 }
@@ -1025,7 +1031,7 @@ Plan plan_of(const uocr_prefix_attention_args& a, bool tc) {
   const int64_t prefix_stages = (a.prefix_capacity + kKeys - 1) / kKeys, own_stages = (a.capacity + kKeys - 1) / kKeys;
   p.own_tiles = tiles(a.sequences, 1, p.own_warps);
   // Own keys in parts only where few blocks would have many: a join less, and own parts that are not written and read.
-  // Four sequences of 300, 512 and 1024 own keys take 12.2, 13.7 and 20.2 us whole, 15.3, 16.6 and 16.4 in parts.
+  // Four sequences of 300, 512 and 1024 own keys take 12.6, 14.0 and 21.9 us whole, 15.4, 16.4 and 16.5 in parts.
   p.whole_own = p.own_tiles * a.kv_heads >= kSms || own_stages <= 8;
   const int64_t units = p.units =
       a.kv_heads * ((p.tc ? 0 : tiles(a.prefixes, a.sequences / a.prefixes, p.prefix_warps) * prefix_stages) +

@@ -103,7 +103,7 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 // Rows (a row and a query head each) of a tile of the tensor-core kernel; a block takes two.
 constexpr int kAttentionTcRows = 128;
 // The prefixes' parts of many rows by tcgen05 (prefix_attention_tc.cu): `blocks`
-// resident blocks; at least four slots (an even number of them to split); a positive scale.
+// resident blocks; at least three slots, six and an even number to split; a scale that is a normal number above 0.
 cudaError_t launch_attention_tc(const Attention& a, int dim, unsigned blocks, cudaStream_t stream);
 
 }  // namespace uocr_b200

@@ -15,7 +15,8 @@
 //
 // m is the maximum of the tiles seen when it last had to move: O and l are
 // rescaled only where a later score exceeds it by more than 2^8, which fp32 and
-// bf16 hold without loss, and which hardly happens after the first tile.
+// bf16 hold without loss, and which hardly happens after the first tile. Scores far
+// from 0 are taken from a base of their row (`base` below).
 //
 // Work is cut by units of the tiles' rows and 128 keys, counted through over
 // prefixes, heads and rows, the same number for every block, whatever the
@@ -36,8 +37,8 @@ namespace {
 
 constexpr int kTileRows = kAttentionTcRows;
 // What a range costs besides its keys, in units: 128 keys take 1.8 us for two tiles of rows, 0.6 (the memory's rate) where
-// the tiles split them. With 4, 6, 8 and 12 for the latter sixteen pages take 53.3, 53.5, 54.2 and 55.1 us, with 2, 3 and
-// 4 for the former prompts on a page 107.9, 107.6 and 107.7, a document 51.2, 51.2 and 52.0.
+// the tiles split them. With 4, 6, 8 and 12 for the latter sixteen pages take 53.3, 53.6, 54.3 and 55.3 us, with 2, 3 and
+// 4 for the former prompts on a page 108.6, 108.4 and 108.4, a document 51.3, 51.2 and 52.1.
 __host__ __device__ __forceinline__ unsigned range_units(const Attention& a) { return a.split ? 4 : 3; }
 constexpr int kTcKeys = 128;
 constexpr int kSlots = 4;        // shared-memory slots of 128 keys or values
