@@ -577,6 +577,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
               }
             }
             if (again) {
+              tmem_st_wait();  // O may be rescaled once more
               based = true;
               if (is_far(m)) {
                 base += m;
@@ -619,7 +620,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const __gri
         const int slot = a.split ? 2 * s.slot + t : s.slot;
         const bool mine = r < s.count && ok;
         if (mine) {
-          a.part_ml[cell + slot] = m == -INFINITY || s.len == 0 ? make_float2(-INFINITY, 0.0f) : make_float2(__fmul_rn(base, a.scale_log2) + m * a.scale_log2, l);
+          a.part_ml[cell + slot] = m == -INFINITY || s.len == 0
+                                       ? make_float2(-INFINITY, 0.0f)
+                                       : make_float2(__fmul_rn(base, a.scale_log2) + m * a.scale_log2, l);
           if (s.tile0 == 0 && (t == 0 || !a.split))  // the slots that no block comes to
             for (int k = a.split ? 2 * s.used : s.used; k < a.prefix_slots; ++k)
               a.part_ml[cell + k] = make_float2(-INFINITY, 0.0f);
@@ -691,8 +694,8 @@ cudaError_t launch_attention_tc(const Attention& a, int dim, unsigned blocks, cu
   TcArgs t{};
   t.a = a;
   const int64_t of_range = a.split ? kTileRows : 2 * kTileRows, tiles = (a.prefix_capacity + kTcKeys - 1) / kTcKeys;
-  t.a.tc_units = static_cast<unsigned>(
-      a.kv_heads * (static_cast<int64_t>(a.rows) * a.group / of_range + std::min(a.prefixes, a.rows)) * (tiles + range_units(a)));
+  const int64_t ranges = static_cast<int64_t>(a.rows) * a.group / of_range + std::min(a.prefixes, a.rows);
+  t.a.tc_units = static_cast<unsigned>(a.kv_heads * ranges * (tiles + range_units(a)));
   if (!make_cache_tmap(&t.k, a.prefix_k, dim, a.prefix_capacity, a.kv_heads, a.prefixes, a.prefix_head_stride,
                        a.prefix_stride, kTcKeys) ||
       !make_cache_tmap(&t.v, a.prefix_v, dim, a.prefix_capacity, a.kv_heads, a.prefixes, a.prefix_head_stride,
